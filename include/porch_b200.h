@@ -243,6 +243,44 @@ int pb_allgather_rows_async(pb_comm* comm, const pb_tensor* shard, int64_t total
  * gather issued so far has completed. */
 int pb_comm_wait(pb_comm* comm);
 
+/* ---- operators of a transformer's decode step --------------------------- */
+/* No counterpart in the reference, whose operators end at matmul and
+ * softmax. Each takes tensors of one device (a lazy one is realised first),
+ * enqueues its kernels on this thread's stream and returns realised tensors;
+ * nothing waits. Strided views are read in place where their innermost axis
+ * is contiguous. */
+
+/* A tensor with a copy of `count` floats at device address `pointer` (memory
+ * of another library on the same GPU). Waits for what `stream` (a CUstream,
+ * NULL for the legacy default stream) holds, and for the copy, so the source
+ * may be reused on return. */
+int pb_tensor_from_device(const int64_t* shape, size_t rank, uint64_t pointer, size_t count,
+                          void* stream, int device, pb_tensor** out);
+
+/* RMS norm of each query and key head with a weight per channel, and the
+ * rotation of its first 2 * R2 channels by the token's position:
+ *   y = R(position) (weight * x / sqrt(mean(x^2) + eps))
+ * q [T, Hq, D], k [T, Hk, D]; weights [D]; cos, sin [positions, R2] with
+ * 2 * R2 <= D <= 1024; positions [T], whole numbers below the table's length
+ * (any other value makes that token's heads NaN). Pairs are channels
+ * (i, i + R2), or (2i, 2i + 1) when `interleaved`. */
+int pb_qk_norm_rope(const pb_tensor* q, const pb_tensor* k, const pb_tensor* q_weight,
+                    const pb_tensor* k_weight, const pb_tensor* cos, const pb_tensor* sin,
+                    const pb_tensor* positions, float eps, int interleaved,
+                    pb_tensor** q_out, pb_tensor** k_out);
+/* Its gradient: from dq_out, dk_out (shapes of q and k) and the forward's
+ * inputs, out[0..3] = dq, dk, dq_weight, dk_weight. The weights' sums are
+ * taken in an order fixed by the sizes and the GPU's number of SMs. */
+int pb_qk_norm_rope_backward(const pb_tensor* dq_out, const pb_tensor* dk_out,
+                             const pb_tensor* q, const pb_tensor* k, const pb_tensor* q_weight,
+                             const pb_tensor* k_weight, const pb_tensor* cos, const pb_tensor* sin,
+                             const pb_tensor* positions, float eps, int interleaved,
+                             pb_tensor* out[4]);
+
+/* Sources of representative instantiations of the operators' kernels, in
+ * pb_expr_describe's format; needs no GPU. */
+int pb_operator_sources(char* text, size_t capacity, size_t* needed);
+
 /* ---- failure-detection test hook ---------------------------------------- */
 /* No counterpart in the reference, which has no device-side waits. While
  * enabled (it is off by default), tensor-core GEMM plans built from then on

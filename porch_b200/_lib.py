@@ -92,6 +92,10 @@ def _declare(L: ctypes.CDLL) -> None:
         "pb_fill_synthetic": (c_int, [c_void_p, c_size_t, c_uint64, c_int, c_double, c_double]),
         "pb_matmul_3xtf32_noalloc": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
                                              c_void_p]),
+        "pb_tensor_from_device": (c_int, [P(c_int64), c_size_t, c_uint64, c_size_t, c_void_p, c_int, P(T)]),
+        "pb_qk_norm_rope": (c_int, [T, T, T, T, T, T, T, c_float, c_int, P(T), P(T)]),
+        "pb_qk_norm_rope_backward": (c_int, [T, T, T, T, T, T, T, T, T, c_float, c_int, P(T)]),
+        "pb_operator_sources": (c_int, [c_char_p, c_size_t, P(c_size_t)]),
         "pb_comm_unique_id": (c_int, [c_char_p]),
         "pb_comm_init": (c_int, [c_int, c_char_p, c_int, c_int, c_double, P(c_void_p)]),
         "pb_comm_info": (c_int, [c_void_p, P(c_int), P(c_int), P(c_int)]),

@@ -273,6 +273,17 @@ class Tensor:
         _check(lib().pb_tensor_device_pointer(self._h, byref(p), byref(b)))
         return p.value, b.value
 
+    @property
+    def __cuda_array_interface__(self) -> dict:
+        """The values in place, for another library on the same GPU (as
+        device_data(): a raw handle, so a consumer that does not order its
+        work behind `stream` calls synchronize() first)."""
+        pointer, _ = self.device_data()
+        stream = c_void_p()
+        _check_rt(lib().pbrt_stream_current(_builtins.max(0, self.placement()), byref(stream)))
+        return {"shape": tuple(self.shape()), "typestr": "<f4", "data": (pointer, False), "version": 3,
+                "stream": stream.value}
+
     def __getitem__(self, key) -> Expr:
         if not isinstance(key, tuple):
             key = (key,)
@@ -339,6 +350,30 @@ def tensor_from_pointer(shape: Sequence[int], pointer: int, count: int, device: 
     out = c_void_p()
     fn = lib().pb_tensor_create_async if asynchronous else lib().pb_tensor_create
     _check(fn(s, r, ctypes.cast(pointer, ctypes.POINTER(c_float)), count, int(device), byref(out)))
+    return Tensor(out.value)
+
+
+def tensor_from_device(array, device: int = 0) -> Tensor:
+    """A tensor with a copy of a contiguous float32 array of another library
+    on the same GPU (anything with __cuda_array_interface__)."""
+    face = array.__cuda_array_interface__
+    shape = face["shape"]
+    if face["typestr"] != "<f4":
+        raise InvalidArgument("tensor_from_device needs a float32 array")
+    strides, step = face.get("strides"), 4
+    if strides is not None:
+        for extent, stride in zip(reversed(shape), reversed(strides)):
+            if extent > 1 and stride != step:
+                raise InvalidArgument("tensor_from_device needs a contiguous array")
+            step *= extent
+    # The interface numbers the legacy and the per-thread default streams 1 and 2, as the driver does.
+    s, r = _shape_arg(shape)
+    count = 1
+    for extent in shape:
+        count *= extent
+    out = c_void_p()
+    _check(lib().pb_tensor_from_device(s, r, face["data"][0] or 0, count, face.get("stream") or None, int(device),
+                                       byref(out)))
     return Tensor(out.value)
 
 
@@ -488,6 +523,43 @@ def softmax(a, axis: int) -> Expr:
     out = c_void_p()
     _check(lib().pb_expr_softmax(ea._h, int(axis), byref(out)))
     return Expr(out.value)
+
+
+# ---------------------------------------------------------- decode step --
+def _realised(x) -> Tensor:
+    return x if isinstance(x, Tensor) else materialize(x)
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps: float = 1e-6,
+                 interleaved: bool = False) -> tuple[Tensor, Tensor]:
+    """RMS norm of every head of q [T, Hq, D] and k [T, Hk, D] with a weight
+    per channel, and the rotation of its first 2 * R2 channels by the token's
+    position; cos, sin [positions, R2], positions [T] whole numbers. Pairs are
+    channels (i, i + R2), or (2i, 2i + 1) when interleaved. An extension."""
+    t = [_realised(x) for x in (q, k, q_weight, k_weight, cos, sin, positions)]
+    oq, ok = c_void_p(), c_void_p()
+    _check(lib().pb_qk_norm_rope(*[x._h for x in t], eps, interleaved, byref(oq), byref(ok)))
+    return Tensor(oq.value), Tensor(ok.value)
+
+
+def qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, cos, sin, positions, eps: float = 1e-6,
+                          interleaved: bool = False) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """Gradients (q, k, q_weight, k_weight) of qk_norm_rope, from those of its
+    results and its inputs. An extension."""
+    t = [_realised(x) for x in (dq, dk, q, k, q_weight, k_weight, cos, sin, positions)]
+    out = (c_void_p * 4)()
+    _check(lib().pb_qk_norm_rope_backward(*[x._h for x in t], eps, interleaved, out))
+    return tuple(Tensor(h) for h in out)
+
+
+def operator_sources() -> str:
+    """Sources of representative instantiations of the decode-step kernels,
+    in describe()'s format."""
+    need = c_size_t(0)
+    _check(lib().pb_operator_sources(None, 0, byref(need)))
+    buf = ctypes.create_string_buffer(need.value)
+    _check(lib().pb_operator_sources(buf, need.value, byref(need)))
+    return buf.value.decode()
 
 
 def describe(e, with_source: bool = False) -> str:

@@ -104,7 +104,8 @@ def build(force: bool = False) -> Path:
 def check_kernels(out_dir: Path | None = None) -> list[str]:
     """Lower the benchmark graph shapes on placeholders (NVRTC -> sm_100a
     cubin inside the library), dump the generated sources and compile each
-    with nvcc for sm_100a. Returns the kernel names checked."""
+    with nvcc for sm_100a, and so the decode-step operators' kernels. Returns
+    the kernel names checked."""
     from . import api  # noqa: WPS433 (import after the library is built)
 
     out_dir = out_dir or (ROOT / "_build" / "kernels")
@@ -121,6 +122,11 @@ def check_kernels(out_dir: Path | None = None) -> list[str]:
             sources_out.append(path)
             names.append(kname)
         del chunks
+    for kname, src in _split_kernels(api.operator_sources()):
+        path = out_dir / f"operator_{kname}.cu"
+        path.write_text(src)
+        sources_out.append(path)
+        names.append(kname)
     nvcc = shutil.which("nvcc") or str(CUDA_HOME / "bin" / "nvcc")
     if Path(nvcc).exists():
         def one(path: Path) -> None:

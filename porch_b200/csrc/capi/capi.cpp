@@ -3,9 +3,11 @@
 #include "lower.hpp"
 
 #include "../front/detail.hpp"
+#include "../front/operators.hpp"
 #include "porch/backend.hpp"
 #include "porch/ops.hpp"
 
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 #include <memory>
@@ -644,6 +646,90 @@ int pb_comm_wait(pb_comm* comm) {
     return guarded([&] {
         require(comm, "communicator");
         porch::detail::wait_communicator(*comm->value);
+    });
+}
+
+// ---- operators of a decode step ------------------------------------------
+int pb_tensor_from_device(const int64_t* shape, size_t rank, uint64_t pointer, size_t count, void* stream,
+                          int device, pb_tensor** out) {
+    return guarded([&] {
+        require(out, "out");
+        *out = nullptr;
+        auto s = shape_of(shape, rank);
+        if (count != porch::detail::checked_numel(s))
+            throw std::invalid_argument("tensor data size does not match shape");
+        if (count != 0 && pointer == 0) throw std::invalid_argument("pointer is null");
+        int ndev = 0;
+        porch::detail::check(pbrt_device_count(&ndev));
+        const int at = porch::detail::checked_ordinal(device, ndev);
+        auto mine = porch::detail::current_stream(at);
+        auto r = porch::detail::new_result(std::move(s), at, mine);
+        if (count != 0) {
+            porch::detail::check(pbrt_stream_synchronize(at, static_cast<pbrt_stream>(stream)));
+            porch::detail::check(pbrt_memcpy_d2d_async(at, r.ptr, pointer, count * sizeof(float), mine->stream));
+            porch::detail::check(pbrt_stream_synchronize(at, mine->stream));
+        }
+        *out = wrap(porch::tensor_access::from_storage(std::move(r.shape), std::move(r.storage),
+                                                       porch::device{device}));
+    });
+}
+
+namespace {
+    porch::detail::norm_rope_args norm_rope_of(const pb_tensor* q, const pb_tensor* k, const pb_tensor* q_weight,
+                                               const pb_tensor* k_weight, const pb_tensor* cos,
+                                               const pb_tensor* sin, const pb_tensor* positions, float eps,
+                                               int interleaved) {
+        require(q, "q");
+        require(k, "k");
+        require(q_weight, "q_weight");
+        require(k_weight, "k_weight");
+        require(cos, "cos");
+        require(sin, "sin");
+        require(positions, "positions");
+        return {&q->value,   &k->value,   &q_weight->value,  &k_weight->value, &cos->value,
+                &sin->value, &positions->value, eps, interleaved != 0};
+    }
+} // namespace
+
+int pb_qk_norm_rope(const pb_tensor* q, const pb_tensor* k, const pb_tensor* q_weight, const pb_tensor* k_weight,
+                    const pb_tensor* cos, const pb_tensor* sin, const pb_tensor* positions, float eps,
+                    int interleaved, pb_tensor** q_out, pb_tensor** k_out) {
+    return guarded([&] {
+        require(q_out, "q_out");
+        require(k_out, "k_out");
+        *q_out = *k_out = nullptr;
+        auto r = porch::detail::qk_norm_rope(
+            norm_rope_of(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved));
+        *q_out = wrap(std::move(r[0]));
+        *k_out = wrap(std::move(r[1]));
+    });
+}
+
+int pb_qk_norm_rope_backward(const pb_tensor* dq_out, const pb_tensor* dk_out, const pb_tensor* q,
+                             const pb_tensor* k, const pb_tensor* q_weight, const pb_tensor* k_weight,
+                             const pb_tensor* cos, const pb_tensor* sin, const pb_tensor* positions, float eps,
+                             int interleaved, pb_tensor* out[4]) {
+    return guarded([&] {
+        require(out, "out");
+        require(dq_out, "dq_out");
+        require(dk_out, "dk_out");
+        out[0] = out[1] = out[2] = out[3] = nullptr;
+        auto r = porch::detail::qk_norm_rope_backward(
+            dq_out->value, dk_out->value,
+            norm_rope_of(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved));
+        for (size_t i = 0; i < 4; ++i) out[i] = wrap(std::move(r[i]));
+    });
+}
+
+int pb_operator_sources(char* text, size_t capacity, size_t* needed) {
+    return guarded([&] {
+        const std::string s = porch::detail::operator_sources();
+        if (needed) *needed = s.size() + 1;
+        if (text != nullptr && capacity != 0) {
+            const size_t n = std::min(s.size(), capacity - 1);
+            std::memcpy(text, s.data(), n);
+            text[n] = '\0';
+        }
     });
 }
 
