@@ -277,6 +277,61 @@ int pb_qk_norm_rope_backward(const pb_tensor* dq_out, const pb_tensor* dk_out,
                              const pb_tensor* positions, float eps, int interleaved,
                              pb_tensor* out[4]);
 
+/* ---- a paged key/value cache --------------------------------------------- */
+/* Pools of `pages` pages of `page_size` (a power of two, 8 to 256) slots for
+ * keys and for values, [pages, kv_heads, page_size, head_dim], in float32 or
+ * bfloat16; head_dim a multiple of 8 up to 256. The values start undefined;
+ * nothing reads a slot past a sequence's length. Calls that write a cache
+ * (append, evict) and calls that read it are ordered on the device in the
+ * order in which they are made. */
+typedef struct pb_kv_cache_s pb_kv_cache;
+typedef struct pb_kv_batch_s pb_kv_batch;
+enum pb_cache_type { PB_CACHE_F32 = 0, PB_CACHE_BF16 = 1 };
+int pb_kv_cache_create(int64_t pages, int64_t page_size, int64_t kv_heads, int64_t head_dim,
+                       int type, int device, pb_kv_cache** out);
+void pb_kv_cache_release(pb_kv_cache* cache);
+/* Device addresses of the pools and the bytes of each. A raw handle: order
+ * other work on it yourself (pb_synchronize). */
+int pb_kv_cache_data(const pb_kv_cache* cache, uint64_t* keys, uint64_t* values, size_t* bytes);
+/* The sequences of one step: `tables` [sequences, width] names the pages of
+ * each, `lengths` its slots in use (new tokens included). `appended` (NULL: 1
+ * each, 0 for an empty one) says how many of them are new, the last ones;
+ * `newest` (NULL: length - 1) the position of the newest slot, which is more
+ * than that once slots were evicted. Checked and uploaded once for the step;
+ * pb_kv_batch_on gives the same sequences over another layer's cache of the
+ * same shape without a second upload. */
+int pb_kv_batch_create(pb_kv_cache* cache, const int32_t* tables, size_t sequences, size_t width,
+                       const int64_t* lengths, const int64_t* appended, const int64_t* newest,
+                       pb_kv_batch** out);
+int pb_kv_batch_on(const pb_kv_batch* batch, pb_kv_cache* cache, pb_kv_batch** out);
+void pb_kv_batch_release(pb_kv_batch* batch);
+/* Writes k and v, [new tokens of all sequences, kv_heads, head_dim], into
+ * the new slots (rounded to nearest in a bfloat16 cache). */
+int pb_kv_append(pb_kv_batch* batch, const pb_tensor* k, const pb_tensor* v);
+/* softmax(scale q K^T) V for one query per sequence: q and the result
+ * [sequences, q_heads, head_dim], q_heads a multiple of kv_heads (query head
+ * i reads key head i / (q_heads / kv_heads)). An empty sequence gives zeros.
+ * Sums, maxima and the result are float32 for either cache type. */
+int pb_paged_attention(const pb_tensor* q, pb_kv_batch* batch, float scale, pb_tensor** out);
+/* The same, and new scores [sequences, kv_heads, longest length]: `scores`
+ * (NULL or slots past its end: 0) plus each slot's attention weight summed
+ * over the query heads of its key head; 0 past a sequence's length. */
+int pb_paged_attention_scored(const pb_tensor* q, pb_kv_batch* batch, const pb_tensor* scores,
+                              float scale, pb_tensor** out, pb_tensor** new_scores);
+/* Keeps, per sequence and key head, `budget` slots: the newest `recent`
+ * positions, the first `sinks` positions, and of the rest those with the
+ * highest scores (NaN lowest; equal ones: the lower slot). Kept slots past
+ * the budget move into the places below it that became free, the j-th to the
+ * j-th, keys and values alike; the sequence then has min(length, budget)
+ * slots. scores [sequences, kv_heads, n] (0 past its end); positions, of the
+ * same form, holds what an earlier call returned (NULL, negative or past its
+ * end: consecutive up to `newest`). Returns both for the kept slots,
+ * [sequences, kv_heads, budget] (0 and -1 past the new length); the inputs
+ * stay as they are. A page that serves two places is refused. */
+int pb_kv_evict(pb_kv_batch* batch, const pb_tensor* scores, const pb_tensor* positions,
+                int64_t budget, int64_t recent, int64_t sinks, pb_tensor** new_scores,
+                pb_tensor** new_positions);
+
 /* Sources of representative instantiations of the operators' kernels, in
  * pb_expr_describe's format; needs no GPU. */
 int pb_operator_sources(char* text, size_t capacity, size_t* needed);

@@ -3,7 +3,7 @@
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_uint64, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p
 from pathlib import Path
 
 LIBRARY = Path(__file__).resolve().parent / "lib" / "libporch_b200.so"
@@ -95,6 +95,16 @@ def _declare(L: ctypes.CDLL) -> None:
         "pb_tensor_from_device": (c_int, [P(c_int64), c_size_t, c_uint64, c_size_t, c_void_p, c_int, P(T)]),
         "pb_qk_norm_rope": (c_int, [T, T, T, T, T, T, T, c_float, c_int, P(T), P(T)]),
         "pb_qk_norm_rope_backward": (c_int, [T, T, T, T, T, T, T, T, T, c_float, c_int, P(T)]),
+        "pb_kv_cache_create": (c_int, [c_int64, c_int64, c_int64, c_int64, c_int, c_int, P(T)]),
+        "pb_kv_cache_release": (None, [T]),
+        "pb_kv_cache_data": (c_int, [T, P(c_uint64), P(c_uint64), P(c_size_t)]),
+        "pb_kv_batch_create": (c_int, [T, P(c_int32), c_size_t, c_size_t, P(c_int64), P(c_int64), P(c_int64), P(T)]),
+        "pb_kv_batch_on": (c_int, [T, T, P(T)]),
+        "pb_kv_batch_release": (None, [T]),
+        "pb_kv_append": (c_int, [T, T, T]),
+        "pb_paged_attention": (c_int, [T, T, c_float, P(T)]),
+        "pb_paged_attention_scored": (c_int, [T, T, T, c_float, P(T), P(T)]),
+        "pb_kv_evict": (c_int, [T, T, T, c_int64, c_int64, c_int64, P(T), P(T)]),
         "pb_operator_sources": (c_int, [c_char_p, c_size_t, P(c_size_t)]),
         "pb_comm_unique_id": (c_int, [c_char_p]),
         "pb_comm_init": (c_int, [c_int, c_char_p, c_int, c_int, c_double, P(c_void_p)]),

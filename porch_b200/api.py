@@ -552,6 +552,153 @@ def qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, cos, sin, positions,
     return tuple(Tensor(h) for h in out)
 
 
+class _Pool:
+    """A cache pool in place, for another library on the same GPU; a bfloat16
+    pool as its 16 raw bits. Keeps the cache alive."""
+
+    def __init__(self, cache: "KVCache", pointer: int):
+        stream = c_void_p()
+        _check_rt(lib().pbrt_stream_current(cache.device, byref(stream)))
+        self.cache = cache
+        self.__cuda_array_interface__ = {
+            "shape": (cache.pages, cache.kv_heads, cache.page_size, cache.head_dim),
+            "typestr": "<u2" if cache.dtype == "bf16" else "<f4", "data": (pointer, False), "version": 3,
+            "stream": stream.value}
+
+
+class KVCache:
+    """Pools of pages of keys and values, [pages, kv_heads, page_size,
+    head_dim], in "f32" or "bf16". An extension."""
+
+    def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: str = "f32", device: int = 0):
+        self._h = c_void_p()
+        if dtype not in ("f32", "bf16"):
+            raise InvalidArgument('cache: dtype must be "f32" or "bf16"')
+        _check(lib().pb_kv_cache_create(int(pages), int(page_size), int(kv_heads), int(head_dim),
+                                        int(dtype == "bf16"), int(device), byref(self._h)))
+        self.pages, self.page_size, self.kv_heads, self.head_dim = int(pages), int(page_size), int(kv_heads), int(head_dim)
+        self.dtype, self.device = dtype, int(device)
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h is not None and h.value:
+            try:
+                lib().pb_kv_cache_release(h)
+            except Exception:
+                pass
+            self._h = c_void_p(None)
+
+    def device_data(self) -> tuple[int, int, int]:
+        """(address of the keys, of the values, bytes of each)."""
+        k, v, n = c_uint64(), c_uint64(), c_size_t()
+        _check(lib().pb_kv_cache_data(self._h, byref(k), byref(v), byref(n)))
+        return k.value, v.value, n.value
+
+    def pools(self) -> tuple[_Pool, _Pool]:
+        """Keys and values in place (__cuda_array_interface__)."""
+        k, v, _ = self.device_data()
+        return _Pool(self, k), _Pool(self, v)
+
+    def batch(self, tables, lengths, appended=None, newest=None) -> "Batch":
+        """The sequences of one step: tables [sequences, width] of page
+        numbers, lengths in slots (new tokens included), how many of them are
+        new (default 1), and the newest slot's position (default length - 1)."""
+        return Batch(self, tables, lengths, appended, newest)
+
+
+class Batch:
+    """Page tables and lengths of one step's sequences (KVCache.batch)."""
+
+    def __init__(self, cache: KVCache, tables, lengths, appended=None, newest=None):
+        self._h = c_void_p()
+        self.cache = cache
+        table = np.asarray(tables)
+        if table.ndim != 2:
+            raise InvalidArgument("cache batch: tables must be [sequences, width]")
+        if table.size and (table.min() < -(1 << 31) or table.max() >= 1 << 31):
+            raise OutOfRange("cache batch: a page is not one of the cache's")
+        table = np.ascontiguousarray(table, dtype=np.int32)
+        n, width = table.shape
+
+        def whole(values):
+            if values is None:
+                return None
+            a = np.ascontiguousarray(values, dtype=np.int64)
+            if a.shape != (n,):
+                raise InvalidArgument("cache batch: one length, new tokens and newest position per sequence")
+            return a
+
+        self.lengths, fresh, last = whole(lengths), whole(appended), whole(newest)
+
+        def at(a, kind):
+            return None if a is None else a.ctypes.data_as(ctypes.POINTER(kind))
+
+        _check(lib().pb_kv_batch_create(cache._h, at(table, ctypes.c_int32), n, width, at(self.lengths, c_int64),
+                                        at(fresh, c_int64), at(last, c_int64), byref(self._h)))
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h is not None and h.value:
+            try:
+                lib().pb_kv_batch_release(h)
+            except Exception:
+                pass
+            self._h = c_void_p(None)
+
+    def on(self, cache: KVCache) -> "Batch":
+        """The same sequences over another layer's cache of the same shape,
+        without a second upload."""
+        other = Batch.__new__(Batch)
+        other._h, other.cache, other.lengths = c_void_p(), cache, self.lengths
+        _check(lib().pb_kv_batch_on(self._h, cache._h, byref(other._h)))
+        return other
+
+    def append(self, k, v) -> None:
+        """Writes the new tokens' keys and values, [new tokens, kv_heads,
+        head_dim] in the order of the sequences."""
+        k, v = _realised(k), _realised(v)
+        _check(lib().pb_kv_append(self._h, k._h, v._h))
+
+
+def paged_attention(q, batch: Batch, scale: float | None = None) -> Tensor:
+    """softmax(scale q K^T) V of one query per sequence, [sequences, q_heads,
+    head_dim], over the batch's slots; scale defaults to head_dim ** -0.5. An
+    extension."""
+    t = _realised(q)
+    out = c_void_p()
+    _check(lib().pb_paged_attention(t._h, batch._h, batch.cache.head_dim ** -0.5 if scale is None else scale,
+                                    byref(out)))
+    return Tensor(out.value)
+
+
+def paged_attention_scored(q, batch: Batch, scores=None, scale: float | None = None) -> tuple[Tensor, Tensor]:
+    """paged_attention, and `scores` (None: zeros) plus each slot's attention
+    weight summed over the query heads of its key head, [sequences, kv_heads,
+    longest]. An extension."""
+    t = _realised(q)
+    s = None if scores is None else _realised(scores)
+    out, new = c_void_p(), c_void_p()
+    _check(lib().pb_paged_attention_scored(t._h, batch._h, None if s is None else s._h,
+                                           batch.cache.head_dim ** -0.5 if scale is None else scale,
+                                           byref(out), byref(new)))
+    return Tensor(out.value), Tensor(new.value)
+
+
+def cache_evict(batch: Batch, scores, positions=None, *, budget: int, recent: int = 0,
+                sinks: int = 0) -> tuple[Tensor, Tensor]:
+    """Keeps `budget` slots per sequence and key head: the newest `recent`
+    positions, the first `sinks`, and the highest scored of the rest; rows
+    move in place. Returns the kept slots' scores and positions, [sequences,
+    kv_heads, budget]; the next batch has lengths min(length, budget) plus its
+    new tokens. An extension."""
+    s = _realised(scores)
+    p = None if positions is None else _realised(positions)
+    new_scores, new_positions = c_void_p(), c_void_p()
+    _check(lib().pb_kv_evict(batch._h, s._h, None if p is None else p._h, int(budget), int(recent), int(sinks),
+                             byref(new_scores), byref(new_positions)))
+    return Tensor(new_scores.value), Tensor(new_positions.value)
+
+
 def operator_sources() -> str:
     """Sources of representative instantiations of the decode-step kernels,
     in describe()'s format."""

@@ -27,6 +27,14 @@ struct pb_comm_s {
     std::unique_ptr<porch::detail::communicator> value;
 };
 
+struct pb_kv_cache_s {
+    std::shared_ptr<porch::detail::kv_cache> value;
+};
+
+struct pb_kv_batch_s {
+    std::shared_ptr<porch::detail::kv_batch> value;
+};
+
 namespace {
 
     thread_local std::string tl_error;
@@ -718,6 +726,101 @@ int pb_qk_norm_rope_backward(const pb_tensor* dq_out, const pb_tensor* dk_out, c
             dq_out->value, dk_out->value,
             norm_rope_of(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved));
         for (size_t i = 0; i < 4; ++i) out[i] = wrap(std::move(r[i]));
+    });
+}
+
+int pb_kv_cache_create(int64_t pages, int64_t page_size, int64_t kv_heads, int64_t head_dim, int type, int device,
+                       pb_kv_cache** out) {
+    return guarded([&] {
+        require(out, "out");
+        *out = nullptr;
+        *out = new pb_kv_cache_s{porch::detail::make_cache(pages, page_size, kv_heads, head_dim,
+                                                           static_cast<porch::detail::cache_type>(type), device)};
+    });
+}
+
+void pb_kv_cache_release(pb_kv_cache* cache) { delete cache; }
+
+int pb_kv_cache_data(const pb_kv_cache* cache, uint64_t* keys, uint64_t* values, size_t* bytes) {
+    return guarded([&] {
+        require(cache, "cache");
+        if (keys) *keys = porch::detail::address(cache->value->k);
+        if (values) *values = porch::detail::address(cache->value->v);
+        if (bytes) *bytes = cache->value->k.size_bytes();
+    });
+}
+
+int pb_kv_batch_create(pb_kv_cache* cache, const int32_t* tables, size_t sequences, size_t width,
+                       const int64_t* lengths, const int64_t* appended, const int64_t* newest, pb_kv_batch** out) {
+    return guarded([&] {
+        require(out, "out");
+        *out = nullptr;
+        require(cache, "cache");
+        require(lengths, "lengths");
+        if (width != 0) require(tables, "tables");
+        *out = new pb_kv_batch_s{
+            porch::detail::make_batch(cache->value, tables, sequences, width, lengths, appended, newest)};
+    });
+}
+
+int pb_kv_batch_on(const pb_kv_batch* batch, pb_kv_cache* cache, pb_kv_batch** out) {
+    return guarded([&] {
+        require(out, "out");
+        *out = nullptr;
+        require(batch, "batch");
+        require(cache, "cache");
+        *out = new pb_kv_batch_s{porch::detail::batch_on(*batch->value, cache->value)};
+    });
+}
+
+void pb_kv_batch_release(pb_kv_batch* batch) { delete batch; }
+
+int pb_kv_append(pb_kv_batch* batch, const pb_tensor* k, const pb_tensor* v) {
+    return guarded([&] {
+        require(batch, "batch");
+        require(k, "k");
+        require(v, "v");
+        porch::detail::cache_append(*batch->value, k->value, v->value);
+    });
+}
+
+int pb_paged_attention(const pb_tensor* q, pb_kv_batch* batch, float scale, pb_tensor** out) {
+    return guarded([&] {
+        require(out, "out");
+        *out = nullptr;
+        require(q, "q");
+        require(batch, "batch");
+        *out = wrap(std::move(porch::detail::paged_attention(q->value, *batch->value, scale, false, nullptr)[0]));
+    });
+}
+
+int pb_paged_attention_scored(const pb_tensor* q, pb_kv_batch* batch, const pb_tensor* scores, float scale,
+                              pb_tensor** out, pb_tensor** new_scores) {
+    return guarded([&] {
+        require(out, "out");
+        require(new_scores, "new_scores");
+        *out = *new_scores = nullptr;
+        require(q, "q");
+        require(batch, "batch");
+        auto r = porch::detail::paged_attention(q->value, *batch->value, scale, true,
+                                                scores != nullptr ? &scores->value : nullptr);
+        *out = wrap(std::move(r[0]));
+        *new_scores = wrap(std::move(r[1]));
+    });
+}
+
+int pb_kv_evict(pb_kv_batch* batch, const pb_tensor* scores, const pb_tensor* positions, int64_t budget,
+                int64_t recent, int64_t sinks, pb_tensor** new_scores, pb_tensor** new_positions) {
+    return guarded([&] {
+        require(new_scores, "new_scores");
+        require(new_positions, "new_positions");
+        *new_scores = *new_positions = nullptr;
+        require(batch, "batch");
+        require(scores, "scores");
+        auto r = porch::detail::cache_evict(*batch->value, scores->value,
+                                            positions != nullptr ? &positions->value : nullptr, budget, recent, sinks);
+        *new_scores = wrap(std::move(r[0]));
+        *new_positions = wrap(std::move(r[1]));
     });
 }
 

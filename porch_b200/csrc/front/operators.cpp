@@ -8,6 +8,16 @@
 
 namespace porch::detail {
 
+    namespace {
+        uint64_t compile(const std::string& source) {
+            std::vector<const char*> options;
+            for (const auto& o : kernel_options()) options.push_back(o.c_str());
+            uint64_t key = 0;
+            check(pbrt_compile(source.c_str(), options.data(), static_cast<int>(options.size()), 1, &key));
+            return key;
+        }
+    } // namespace
+
     pbrt_function op_kernel::on(int device) {
         if (device < 0 || device >= static_cast<int>(function.size()))
             throw std::invalid_argument("device ordinal out of range");
@@ -29,10 +39,7 @@ namespace porch::detail {
         if (entry == nullptr) {
             auto k = std::make_unique<op_kernel>();
             make(*k);
-            std::vector<const char*> options;
-            for (const auto& o : kernel_options()) options.push_back(o.c_str());
-            check(pbrt_compile(k->source.c_str(), options.data(), static_cast<int>(options.size()), 1,
-                               &k->image_key));
+            k->image_key = compile(k->source);
             entry = std::move(k);
         }
         return *entry;
@@ -145,7 +152,10 @@ namespace porch::detail {
     std::string operator_sources() {
         std::vector<std::pair<std::string, std::string>> all;
         norm_rope_sources(all);
+        paged_cache_sources(all);
+        paged_attention_sources(all);
         std::ostringstream os;
+        for (const auto& [name, source] : all) (void)compile(source); // NVRTC takes it, too
         for (const auto& [name, source] : all) os << "kernel " << name << " : operator\n" << source << "\n";
         return os.str();
     }

@@ -97,9 +97,56 @@ namespace porch::detail {
     std::array<tensor, 2> qk_norm_rope(const norm_rope_args& a);
     std::array<tensor, 4> qk_norm_rope_backward(const tensor& dq, const tensor& dk, const norm_rope_args& a);
 
+    // --------------------------------------------------------------- cache --
+    enum class cache_type : int { f32 = 0, bf16 = 1 };
+
+    // Pools of pages of keys and values: [pages, heads, page_size, dim], so
+    // the rows of one page and head are one contiguous block.
+    struct kv_cache {
+        int64_t pages = 0, page_size = 0, heads = 0, dim = 0;
+        cache_type type = cache_type::f32;
+        int device = 0;
+        cuda_jit::device_buffer k, v;
+        int width() const { return type == cache_type::bf16 ? 2 : 4; } // bytes of a value
+    };
+    std::shared_ptr<kv_cache> make_cache(int64_t pages, int64_t page_size, int64_t heads, int64_t dim,
+                                         cache_type type, int device);
+
+    // The sequences of one step: page tables, slots in use and the rows that
+    // the step's new tokens go to, checked on the host and uploaded once for
+    // every layer and call of the step.
+    struct kv_batch {
+        std::shared_ptr<kv_cache> cache;
+        std::vector<int64_t> lengths;
+        std::vector<int64_t> newest;   // position of each sequence's newest slot
+        int64_t longest = 0, tokens = 0; // tokens: new ones, over all sequences
+        int64_t table_width = 0;
+        bool shared_pages = false;       // a page serves two sequences, or one twice
+        cuda_jit::device_buffer data;    // int32: lengths, newest, tables, then 8-byte rows
+        uint64_t lengths_at = 0, newest_at = 0, tables_at = 0, rows_at = 0; // device addresses
+        int64_t sequences() const { return static_cast<int64_t>(lengths.size()); }
+    };
+    std::shared_ptr<kv_batch> make_batch(std::shared_ptr<kv_cache> cache, const int32_t* tables, size_t sequences,
+                                         size_t width, const int64_t* lengths, const int64_t* appended,
+                                         const int64_t* newest);
+
+    // The same sequences over another cache of the same shape; shares the upload.
+    std::shared_ptr<kv_batch> batch_on(const kv_batch& batch, std::shared_ptr<kv_cache> cache);
+
+    // Writes the step's new keys and values, [tokens, heads, dim], into their rows.
+    void cache_append(kv_batch& batch, const tensor& k, const tensor& v);
+    // {attention, new scores} (the second only when `scored`).
+    std::vector<tensor> paged_attention(const tensor& q, kv_batch& batch, float scale, bool scored,
+                                        const tensor* scores);
+    std::array<tensor, 2> cache_evict(kv_batch& batch, const tensor& scores, const tensor* positions,
+                                      int64_t budget, int64_t recent, int64_t sinks);
+
     // Sources of representative instantiations of every operator kernel, in
     // the "kernel <name> ..." format of describe_plan, for build checks.
     std::string operator_sources();
-    void norm_rope_sources(std::vector<std::pair<std::string, std::string>>& out);
+    using kernel_list = std::vector<std::pair<std::string, std::string>>;
+    void norm_rope_sources(kernel_list& out);
+    void paged_cache_sources(kernel_list& out);
+    void paged_attention_sources(kernel_list& out);
 
 } // namespace porch::detail

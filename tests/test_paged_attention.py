@@ -1,0 +1,214 @@
+"""Attention over a paged cache against its definition in 64 bits (the
+tolerances are derived in paged.Host.attend). Every slot that no sequence uses
+holds NaN throughout."""
+
+import numpy as np
+import pytest
+
+import paged
+
+CASES = [
+    # lengths, kv heads, query heads per kv head, head size, page, type
+    ([1], 1, 1, 8, 8, "f32"),
+    ([1], 1, 1, 8, 8, "bf16"),
+    ([17], 2, 4, 64, 16, "bf16"),
+    ([64, 63, 65, 1], 2, 3, 128, 64, "bf16"),
+    ([64, 63, 65, 1], 2, 3, 128, 64, "f32"),
+    ([0, 130, 0], 1, 8, 96, 8, "bf16"),
+    ([0, 0], 2, 2, 64, 8, "bf16"),
+    ([300, 5, 129], 3, 5, 80, 128, "bf16"),
+    ([300, 5, 129], 3, 5, 80, 128, "f32"),
+    ([257], 1, 12, 40, 256, "bf16"),
+    ([257, 100], 1, 16, 72, 32, "f32"),
+    ([200, 90], 2, 17, 64, 16, "bf16"),
+    ([200, 90], 1, 40, 32, 16, "f32"),
+    ([513, 70], 2, 2, 256, 64, "bf16"),
+    ([513, 70], 2, 2, 256, 64, "f32"),
+    ([4099], 1, 1, 64, 16, "f32"),
+    ([9001, 3], 2, 6, 128, 128, "bf16"),
+    ([20000], 1, 9, 112, 64, "bf16"),
+    ([7] * 300, 1, 2, 24, 8, "bf16"),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lengths,heads,group,dim,page,dtype", CASES)
+def test_against_the_definition(gpu, lengths, heads, group, dim, page, dtype):
+    rng = np.random.default_rng(sum(lengths) + dim)
+    host = paged.Host(rng, lengths, heads, dim, page, dtype)
+    _, batch = host.build(gpu)
+    q = rng.normal(0, 2, (len(lengths), heads * group, dim)).astype(np.float32)
+    t = gpu.tensor(list(q.shape), q)
+    out, tol, new, new_tol = host.attend(q, dim**-0.5)
+    got = gpu.paged_attention(t, batch).cpu().reshape(q.shape)
+    assert (np.abs(got - out) <= tol).all()
+    again, weights = gpu.paged_attention_scored(t, batch)
+    assert np.array_equal(again.cpu().reshape(q.shape), got)
+    assert (np.abs(weights.cpu().reshape(new.shape) - new) <= new_tol).all()
+    # Running scores, of fewer slots than there are now, and of more.
+    for slots in (max(lengths) // 2, max(lengths) + 9):
+        scores = rng.uniform(0, 3, (len(lengths), heads, slots)).astype(np.float32)
+        _, _, new, new_tol = host.attend(q, 0.3, scores)
+        _, weights = gpu.paged_attention_scored(t, batch, gpu.tensor(list(scores.shape), scores), scale=0.3)
+        assert weights.shape() == list(new.shape)
+        assert (np.abs(weights.cpu().reshape(new.shape) - new) <= new_tol).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_logits_far_apart(gpu, dtype):
+    # One slot with nearly all the weight, wherever it stands; logits of
+    # thousands; and equal logits, whose weights are 1 / n.
+    rng = np.random.default_rng(2)
+    host = paged.Host(rng, [700, 129, 64], 1, 64, 32, dtype)
+    for s, at in enumerate([0, 128, 40]):
+        host.k[s][at] *= 60
+    _, batch = host.build(gpu)
+    q = np.concatenate([5 * paged.bf16(host.k[s][at])[None] for s, at in enumerate([0, 128, 40])])
+    q = np.concatenate([q, -q, 0 * q], 1)
+    out, tol, new, new_tol = host.attend(q, 1.0)
+    got, weights = gpu.paged_attention_scored(gpu.tensor(list(q.shape), q), batch, scale=1.0)
+    assert (np.abs(got.cpu().reshape(q.shape) - out) <= tol).all()
+    assert (np.abs(weights.cpu().reshape(new.shape) - new) <= new_tol).all()
+
+
+@pytest.mark.gpu
+def test_values_that_are_not_finite_stay_in_their_row(gpu):
+    rng = np.random.default_rng(2)
+    host = paged.Host(rng, [100, 90, 65], 2, 64, 16, "bf16")
+    q = rng.normal(0, 1, (3, 4, 64)).astype(np.float32)
+    _, batch = host.build(gpu)
+    want = gpu.paged_attention(gpu.tensor([3, 4, 64], q), batch).cpu().reshape(q.shape)
+    host.v[1][89, 0, 5] = np.nan
+    host.k[2][64, 1, 0] = np.nan
+    _, batch = host.build(gpu)
+    got = gpu.paged_attention(gpu.tensor([3, 4, 64], q), batch).cpu().reshape(q.shape)
+    bad = np.zeros(q.shape, bool)
+    bad[1, :2, 5] = True
+    bad[2, 2:] = True
+    assert np.isnan(got[bad]).all() and np.array_equal(got[~bad], want[~bad])
+
+
+@pytest.mark.gpu
+def test_pools_past_two_to_the_31_values(gpu):
+    # 2^24 + 2^20 rows of 128 values: the last pages lie past 2^31 values and
+    # past 2^32 bytes.
+    pages, page, dim = ((1 << 24) + (1 << 20)) // 64, 64, 128
+    cache = gpu.KVCache(pages, page, 1, dim, dtype="bf16")
+    rng = np.random.default_rng(2)
+    host = paged.Host(rng, [150], 1, dim, page, "bf16")
+    host.tables = np.array([[pages - 1, 3, pages - 2]], dtype=np.int32)
+    batch = cache.batch(host.tables, [150], appended=[150])
+    batch.append(gpu.tensor([150, 1, dim], host.k[0]), gpu.tensor([150, 1, dim], host.v[0]))
+    q = rng.normal(0, 1, (1, 3, dim)).astype(np.float32)
+    out, tol, _, _ = host.attend(q, 1.0)
+    got = gpu.paged_attention(gpu.tensor([1, 3, dim], q), batch, scale=1.0).cpu().reshape(q.shape)
+    assert (np.abs(got - out) <= tol).all()
+    scores = gpu.tensor([1, 1, 150], rng.uniform(0, 1, 150).astype(np.float32))
+    kept, _ = gpu.cache_evict(batch, scores, budget=70, recent=9)
+    source, _, _ = paged.evict([150], [149], scores.cpu().reshape(1, 1, 150), None, 70, 9, 0)
+    host.k[0], host.v[0], host.lengths = host.k[0][source[0, 0]], host.v[0][source[0, 0]], [70]
+    out, tol, _, _ = host.attend(q, 1.0)
+    got = gpu.paged_attention(gpu.tensor([1, 3, dim], q), cache.batch(host.tables, [70]), scale=1.0)
+    assert (np.abs(got.cpu().reshape(q.shape) - out) <= tol).all()
+
+
+@pytest.mark.gpu
+def test_queries_read_in_place_and_pages_shared_by_sequences(gpu):
+    rng = np.random.default_rng(6)
+    host = paged.Host(rng, [40, 40], 2, 64, 8, "f32")
+    host.tables[1] = host.tables[0]
+    host.k[1], host.v[1] = host.k[0], host.v[0]
+    cache = gpu.KVCache(host.pages, 8, 2, 64)
+    one = cache.batch(host.tables[:1], [40], appended=[40])
+    one.append(gpu.tensor([40, 2, 64], host.k[0]), gpu.tensor([40, 2, 64], host.v[0]))
+    both = cache.batch(host.tables, [40, 40], appended=[0, 0])
+    fused = rng.normal(0, 1, (2, 10, 65)).astype(np.float32)
+    q = gpu.materialize(gpu.tensor([2, 10, 65], fused)[gpu.all, 3:7, 1:65])
+    out, tol, _, _ = host.attend(fused[:, 3:7, 1:], 0.125)
+    assert (np.abs(gpu.paged_attention(q, both).cpu().reshape(out.shape) - out) <= tol).all()
+    # Another layer's cache, the same tables: other values.
+    other = gpu.KVCache(host.pages, 8, 2, 64)
+    one.on(other).append(gpu.tensor([40, 2, 64], host.v[0]), gpu.tensor([40, 2, 64], host.k[0]))
+    assert (np.abs(gpu.paged_attention(q, both).cpu().reshape(out.shape) - out) <= tol).all()
+    host.k, host.v = host.v, host.k
+    out, tol, _, _ = host.attend(fused[:, 3:7, 1:], 0.125)
+    assert (np.abs(gpu.paged_attention(q, both.on(other)).cpu().reshape(out.shape) - out) <= tol).all()
+
+
+@pytest.mark.gpu
+def test_the_same_every_time_and_from_another_thread(gpu):
+    import threading
+
+    rng = np.random.default_rng(6)
+    host = paged.Host(rng, [3000, 40, 777], 2, 64, 32, "bf16")
+    q = rng.normal(0, 1, (3, 8, 64)).astype(np.float32)
+    cache, batch = host.build(gpu)
+    t = gpu.tensor([3, 8, 64], q)
+    first = [x.cpu() for x in gpu.paged_attention_scored(t, batch)]
+    got = []
+
+    def work():
+        for _ in range(3):
+            got.append([x.cpu() for x in gpu.paged_attention_scored(t, batch)])
+
+    th = threading.Thread(target=work)
+    th.start()
+    work()
+    th.join()
+    assert len(got) == 6 and all(np.array_equal(a, b) for g in got for a, b in zip(first, g))
+
+
+def test_refusals_that_need_no_device(api):
+    for bad in ((0, 16, 1, 64), (4, 12, 1, 64), (4, 4, 1, 64), (4, 512, 1, 64), (4, 16, 0, 64), (4, 16, 1, 60),
+                (4, 16, 1, 264), (4, 16, 1, 0), (1 << 25, 256, 1, 64)):
+        with pytest.raises(api.InvalidArgument, match="cache"):
+            api.KVCache(*bad)
+    with pytest.raises(api.InvalidArgument, match="dtype"):
+        api.KVCache(4, 16, 1, 64, dtype="f16")
+
+
+@pytest.mark.gpu
+def test_refusals(gpu):
+    cache = gpu.KVCache(6, 16, 2, 64)
+    tables = np.array([[0, 1], [2, 3]], np.int32)
+    batch = cache.batch(tables, [20, 32])
+
+    def refused(error, match, call, *args, **more):
+        with pytest.raises(error, match=match):
+            call(*args, **more)
+
+    bad = gpu.InvalidArgument
+    refused(bad, "too short", cache.batch, tables, [20, 33])
+    refused(bad, "length", cache.batch, tables, [20, -1])
+    refused(gpu.OutOfRange, "page 6", cache.batch, [[0, 6]], [32])
+    refused(gpu.OutOfRange, "page -1", cache.batch, [[0, -1]], [32])
+    refused(gpu.OutOfRange, "page", cache.batch, [[0, 1 << 40]], [32])
+    refused(bad, "new tokens", cache.batch, tables, [20, 32], appended=[21, 0])
+    refused(bad, "newest", cache.batch, tables, [20, 32], newest=[19, 30])
+    refused(bad, "newest", cache.batch, tables, [20, 32], newest=[19, 1 << 24])
+    refused(bad, "same row", cache.batch, [[0, 1], [0, 1]], [20, 20])
+    refused(bad, "one length", cache.batch, tables, [20])
+    refused(bad, "width", cache.batch, [0, 1], [20])
+    refused(bad, "sequences", cache.batch, np.zeros((0, 2), np.int32), [])
+    refused(bad, "shape, type or device", batch.on, gpu.KVCache(6, 16, 2, 64, dtype="bf16"))
+    zeros = gpu.zeros
+    refused(bad, "new tokens", batch.append, zeros([3, 2, 64]), zeros([2, 2, 64]))
+    refused(bad, "new tokens", batch.append, zeros([2, 2, 64]), zeros([2, 2, 32]))
+    refused(bad, "q must be", gpu.paged_attention, zeros([2, 4, 32]), batch)
+    refused(bad, "q must be", gpu.paged_attention, zeros([1, 4, 64]), batch)
+    refused(bad, "multiple", gpu.paged_attention, zeros([2, 3, 64]), batch)
+    refused(bad, "multiple", gpu.paged_attention, zeros([2, 1, 64]), batch)
+    refused(bad, "finite", gpu.paged_attention, zeros([2, 4, 64]), batch, scale=float("nan"))
+    refused(bad, "scores must be", gpu.paged_attention_scored, zeros([2, 4, 64]), batch, zeros([2, 4, 32]))
+    scores = zeros([2, 2, 32])
+    refused(bad, "scores must be", gpu.cache_evict, batch, zeros([2, 32]), budget=8)
+    refused(bad, "positions must be", gpu.cache_evict, batch, scores, zeros([1, 2, 8]), budget=8)
+    refused(bad, "budget", gpu.cache_evict, batch, scores, budget=0)
+    refused(bad, "recent and sinks", gpu.cache_evict, batch, scores, budget=8, recent=9)
+    refused(bad, "recent and sinks", gpu.cache_evict, batch, scores, budget=8, recent=5, sinks=4)
+    refused(bad, "recent and sinks", gpu.cache_evict, batch, scores, budget=8, sinks=-1)
+    shared = cache.batch([[0, 1], [0, 2]], [20, 20], appended=[0, 0])
+    refused(bad, "more than one place", gpu.cache_evict, shared, scores, budget=8)
+    with pytest.raises(RuntimeError, match="placeholder"):
+        gpu.paged_attention(gpu.placeholder([2, 4, 64]), batch)
