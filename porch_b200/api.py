@@ -660,6 +660,18 @@ class Batch:
         _check(lib().pb_kv_append(self._h, k._h, v._h))
 
 
+def attention_plan(lengths, kv_heads: int, ctas: int, chunks: int = 1) -> str:
+    """How the attention of a batch with these lengths is shared out over
+    `ctas` CTAs (pb_kv_plan_describe); needs no GPU."""
+    a = np.ascontiguousarray(lengths, dtype=np.int64)
+    args = (a.ctypes.data_as(ctypes.POINTER(c_int64)), a.size, int(kv_heads), int(chunks), int(ctas))
+    need = c_size_t(0)
+    _check(lib().pb_kv_plan_describe(*args, None, 0, byref(need)))
+    buf = ctypes.create_string_buffer(need.value)
+    _check(lib().pb_kv_plan_describe(*args, buf, need.value, byref(need)))
+    return buf.value.decode()
+
+
 def paged_attention(q, batch: Batch, scale: float | None = None) -> Tensor:
     """softmax(scale q K^T) V of one query per sequence, [sequences, q_heads,
     head_dim], over the batch's slots; scale defaults to head_dim ** -0.5. An

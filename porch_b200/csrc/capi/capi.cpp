@@ -824,16 +824,30 @@ int pb_kv_evict(pb_kv_batch* batch, const pb_tensor* scores, const pb_tensor* po
     });
 }
 
-int pb_operator_sources(char* text, size_t capacity, size_t* needed) {
-    return guarded([&] {
-        const std::string s = porch::detail::operator_sources();
+namespace {
+    void copy_text(const std::string& s, char* text, size_t capacity, size_t* needed) {
         if (needed) *needed = s.size() + 1;
         if (text != nullptr && capacity != 0) {
             const size_t n = std::min(s.size(), capacity - 1);
             std::memcpy(text, s.data(), n);
             text[n] = '\0';
         }
+    }
+} // namespace
+
+int pb_kv_plan_describe(const int64_t* lengths, size_t sequences, int64_t kv_heads, int64_t chunks, int64_t ctas,
+                        char* text, size_t capacity, size_t* needed) {
+    return guarded([&] {
+        if (sequences != 0) require(lengths, "lengths");
+        std::vector<int64_t> n(lengths, lengths + sequences);
+        if (kv_heads < 1 || chunks < 1 || ctas < 1 || std::any_of(n.begin(), n.end(), [](int64_t v) { return v < 0; }))
+            throw std::invalid_argument("plan: lengths must not be negative, heads, chunks and CTAs positive");
+        copy_text(porch::detail::attention_schedule(n, kv_heads, chunks, ctas), text, capacity, needed);
     });
+}
+
+int pb_operator_sources(char* text, size_t capacity, size_t* needed) {
+    return guarded([&] { copy_text(porch::detail::operator_sources(), text, capacity, needed); });
 }
 
 int pb_profile_enable(int enable) {

@@ -112,6 +112,18 @@ namespace porch::detail {
     std::shared_ptr<kv_cache> make_cache(int64_t pages, int64_t page_size, int64_t heads, int64_t dim,
                                          cache_type type, int device);
 
+    // How attention's CTAs share a batch's slots, uploaded.
+    struct batch_plan {
+        int64_t chunks = 1; // query heads of a key head come in this many rows
+        int64_t limit = 0;  // CTAs asked for
+        int64_t ctas = 0, joins = 0;
+        cuda_jit::device_buffer data; // 16 bytes per CTA, then 16 per row to join
+    };
+    struct batch_plans {
+        std::mutex mutex;
+        std::vector<std::unique_ptr<batch_plan>> made;
+    };
+
     // The sequences of one step: page tables, slots in use and the rows that
     // the step's new tokens go to, checked on the host and uploaded once for
     // every layer and call of the step.
@@ -123,12 +135,21 @@ namespace porch::detail {
         int64_t table_width = 0;
         bool shared_pages = false;       // a page serves two sequences, or one twice
         cuda_jit::device_buffer data;    // int32: lengths, newest, tables, then 8-byte rows
+        // Made once with the batch for the usual number of query heads, and
+        // by the first call that needs another.
+        std::shared_ptr<batch_plans> plans = std::make_shared<batch_plans>();
         uint64_t lengths_at = 0, newest_at = 0, tables_at = 0, rows_at = 0; // device addresses
         int64_t sequences() const { return static_cast<int64_t>(lengths.size()); }
     };
     std::shared_ptr<kv_batch> make_batch(std::shared_ptr<kv_cache> cache, const int32_t* tables, size_t sequences,
                                          size_t width, const int64_t* lengths, const int64_t* appended,
                                          const int64_t* newest);
+
+    const batch_plan& plan_of(kv_batch& batch, int64_t chunks, int64_t ctas);
+    int attention_ctas_per_sm(const kv_cache& c);
+    // The plan as text ("work <row> <tile> <tiles>" per CTA, "join <row>
+    // <first CTA> <parts> <place>" per row), without a device.
+    std::string attention_schedule(const std::vector<int64_t>& lengths, int64_t heads, int64_t chunks, int64_t ctas);
 
     // The same sequences over another cache of the same shape; shares the upload.
     std::shared_ptr<kv_batch> batch_on(const kv_batch& batch, std::shared_ptr<kv_cache> cache);

@@ -19,101 +19,665 @@ namespace porch::detail {
             if (!ok) throw std::invalid_argument(message);
         }
 
+        // The whole layout of a kernel follows from these.
+        struct form {
+            int heads = 1, dim = 0, page = 0;
+            bool bf16 = false, scored = false;
+            int tiles8 = 1; // groups of 8 query heads that a row holds (1 or 2)
+            int width() const { return bf16 ? 2 : 4; }
+            int planes() const { return (dim * width() + 127) / 128; }
+            int unit() const { return planes() * 8192; }                       // 64 slots of K or of V
+            int steps() const { return ((dim * width() + 31) / 32 + 1) & ~1; } // 32-byte k-steps, an even number
+            int terms() const { return bf16 ? 3 : 2; }
+            int q_row() const { return steps() * 32 + 16; }
+            int p_row() const { return 64 * width() + 16; }
+            int small() const { // everything but the ring
+                return terms() * tiles8 * 8 * (q_row() + p_row()) + 2 * 4 * tiles8 * 8 * 4 + 256;
+            }
+            int per_sm() const { return choose().first; }
+            int ring() const { return choose().second; }
+            int smem() const { return 1024 + ring() * unit() + small(); }
+
+          private:
+            // CTAs of an SM and units of a CTA's ring. Two CTAs hide each
+            // other's barriers; a third and fourth only pay where a tile is
+            // so small (8 KB units) that its chain of barriers takes longer
+            // than its bytes. At least three units, so that one is in flight
+            // while two are read.
+            std::pair<int, int> choose() const {
+                for (int n = unit() <= 8192 ? 4 : 2; n > 1; n /= 2) {
+                    const int r = ((228 * 1024) / n - 2048 - small()) / unit();
+                    if (r >= 3) return {n, std::min(r, 6)};
+                }
+                return {1, std::min((227 * 1024 - 1024 - small()) / unit(), 6)};
+            }
+        };
+
         const char* device_source() {
             return R"PB(
 typedef long long pb_i64;
-#if PB_BF16
-typedef unsigned short pb_cell;
-static __device__ __forceinline__ float pb_value(pb_cell c) { return __uint_as_float((pb_u32)c << 16); }
+#define PB_WAIT_CYCLES 4000000000ll
+#define PB_HT (8 * PB_NT)                // query heads of a row, padded
+#define PB_PLANES ((PB_D * PB_ESZ + 127) / 128)
+#define PB_UNIT (PB_PLANES * 8192)       // 64 slots, one 128-byte plane after the other
+#define PB_CE (128 / PB_ESZ)             // values of a plane's row
+#define PB_BOX (PB_PS < 64 ? PB_PS : 64) // slots of one tile load
+#define PB_STEPS ((((PB_D * PB_ESZ + 31) / 32) + 1) & ~1)
+#define PB_QROW (PB_STEPS * 32 + 16)
+#define PB_PROW (64 * PB_ESZ + 16)
+#define PB_MT ((PB_D + 15) / 16)         // 16-channel tiles of the result
+#define PB_MTW ((PB_MT + 3) / 4)         // of one warp
+#if PB_ESZ == 2
+#define PB_TERMS 3
 #else
-typedef float pb_cell;
-static __device__ __forceinline__ float pb_value(pb_cell c) { return c; }
+#define PB_TERMS 2
 #endif
 
-static __device__ __forceinline__ float pb_block_reduce(float v, bool maximum, float* sh) {
-#pragma unroll
-    for (int m = 16; m > 0; m /= 2) {
-        const float o = __shfl_xor_sync(0xffffffffu, v, m);
-        v = maximum ? fmaxf(v, o) : v + o;
+struct __align__(64) pb_tmap { unsigned long long opaque[16]; };
+
+static __device__ __forceinline__ pb_u32 pb_smem(const void* p) { return (pb_u32)__cvta_generic_to_shared(p); }
+static __device__ __forceinline__ void pb_mbar_init(pb_u32 bar, pb_u32 count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" :: "r"(bar), "r"(count) : "memory");
+}
+static __device__ __forceinline__ void pb_mbar_arrive(pb_u32 bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory");
+}
+static __device__ __forceinline__ void pb_mbar_expect_tx(pb_u32 bar, pb_u32 bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" :: "r"(bar), "r"(bytes) : "memory");
+}
+static __device__ __forceinline__ pb_u32 pb_mbar_try(pb_u32 bar, pb_u32 parity) {
+    pb_u32 ok;
+    asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok;
+}
+// Bounded wait: false when the budget ran out or another role gave up.
+static __device__ __forceinline__ bool pb_wait(pb_u32 bar, pb_u32 parity, volatile int* abort_flag, int* err, int site) {
+    if (pb_mbar_try(bar, parity)) return true;
+    const long long start = clock64();
+    for (;;) {
+        if (pb_mbar_try(bar, parity)) return true;
+        if (*abort_flag) return false;
+        if (clock64() - start > PB_WAIT_CYCLES) {
+            *abort_flag = 1;
+            if (atomicCAS(err, 0, 0x7d00 + site) == 0) {
+                err[1] = site;
+                err[2] = (int)blockIdx.x;
+            }
+            return false;
+        }
     }
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = sh[0];
-    for (int i = 1; i < 8; ++i) v = maximum ? fmaxf(v, sh[i]) : v + sh[i];
-    return v;
+}
+static __device__ __forceinline__ void pb_tma_load(pb_u32 dst, const pb_tmap* map, pb_u32 bar, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+                 :: "r"(dst), "l"((unsigned long long)map), "r"(bar), "r"(x), "r"(y) : "memory");
+}
+// Named barrier 1 over the 128 computing threads, with an OR of a predicate:
+// a wait that ran out anywhere makes all of them leave at the same place.
+static __device__ __forceinline__ bool pb_bar_any(bool v) {
+    pb_u32 r;
+    asm volatile("{\n .reg .pred p, q;\n setp.ne.u32 q, %1, 0;\n bar.red.or.pred p, 1, 128, q;\n selp.u32 %0, 1, 0, p;\n}\n"
+                 : "=r"(r) : "r"((pb_u32)v) : "memory");
+    return r != 0;
+}
+static __device__ __forceinline__ float pb_exp2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
 }
 
-// One block per sequence and query head: logits to `weights`, then their
-// softmax in place, then the weighted sum of V.
-extern "C" __global__ void __launch_bounds__(256) pb_attend(
-    const float* q, const pb_cell* pk, const pb_cell* pv, const int* lengths, const int* tables, float* weights,
-    float* out, pb_i64 longest, int width, int heads, int group, float scale) {
+static __device__ __forceinline__ void pb_ldm4(pb_u32* r, pb_u32 addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+static __device__ __forceinline__ void pb_ldm4t(pb_u32* r, pb_u32 addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+#if PB_ESZ == 2
+static __device__ __forceinline__ void pb_mma(float* c, const pb_u32* a, const pb_u32* b) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+// The upper 16 bits of x rounded to nearest even bfloat16.
+static __device__ __forceinline__ unsigned short pb_bf16(float x) {
+    unsigned short r;
+    asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(r) : "f"(x));
+    return r;
+}
+static __device__ __forceinline__ float pb_value(unsigned short x) { return __uint_as_float((pb_u32)x << 16); }
+// x = t0 + t1 + t2, bfloat16 each: 24 bits, so exactly (until t2 underflows).
+static __device__ __forceinline__ void pb_split_store(pb_u32 at, pb_u32 step, float x) {
+#pragma unroll
+    for (int t = 0; t < 3; ++t) {
+        const unsigned short h = pb_bf16(x);
+        x -= pb_value(h);
+        asm volatile("st.shared.u16 [%0], %1;" :: "r"(at + t * step), "h"(h) : "memory");
+    }
+}
+#else
+static __device__ __forceinline__ void pb_mma(float* c, const pb_u32* a, const pb_u32* b) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+static __device__ __forceinline__ float pb_tf32(float x) {
+    pb_u32 r;
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
+    return __uint_as_float(r);
+}
+// x = t0 + t1 + e, tf32 each, |e| <= 2^-22 |x|.
+static __device__ __forceinline__ void pb_split_store(pb_u32 at, pb_u32 step, float x) {
+    const float hi = pb_tf32(x);
+    asm volatile("st.shared.f32 [%0], %1;" :: "r"(at), "f"(hi) : "memory");
+    asm volatile("st.shared.f32 [%0], %1;" :: "r"(at + step), "f"(pb_tf32(x - hi)) : "memory");
+}
+// hi and lo of four fragment values.
+static __device__ __forceinline__ void pb_split_frag(const pb_u32* a, pb_u32* hi, pb_u32* lo) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float x = __uint_as_float(a[i]), h = pb_tf32(x);
+        hi[i] = __float_as_uint(h);
+        lo[i] = __float_as_uint(pb_tf32(x - h));
+    }
+}
+#endif
+
+// Where a row's tiles come from. Rows are (sequence, key head, chunk of query
+// heads), tiles 64 slots of a row; a CTA works through a run of tiles.
+struct pb_at { int row, tile; int s, h, chunk, length, tiles; };
+static __device__ __forceinline__ void pb_enter(pb_at& a, const int* lengths, int chunks) {
+    a.chunk = a.row % chunks;
+    a.h = (a.row / chunks) % PB_H;
+    a.s = a.row / chunks / PB_H;
+    a.length = lengths[a.s];
+    a.tiles = (a.length + 63) >> 6;
+}
+// The next tile; skips sequences without slots. True when it is another row's.
+static __device__ __forceinline__ bool pb_next(pb_at& a, const int* lengths, int chunks) {
+    if (++a.tile < a.tiles) return false;
+    a.tile = 0;
+    do {
+        ++a.row;
+        pb_enter(a, lengths, chunks);
+    } while (a.tiles == 0);
+    return true;
+}
+
+extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
+    const __grid_constant__ pb_tmap map_k, const __grid_constant__ pb_tmap map_v, const float* q, const int* lengths,
+    const int* tables, const int4* work, float* out, float* partial, float2* partial_ml, float* logits, float* lse,
+    int width, int group, int chunks, pb_i64 q_seq, pb_i64 q_head, int longest, float scale2, int* err) {
+    extern __shared__ char raw[];
+    __shared__ pb_u64 bars[2 * PB_RING];
+    __shared__ int abort_flag;
+    const pb_u32 ring = (pb_smem(raw) + 1023u) & ~1023u;
+    const pb_u32 qs = ring + PB_RING * PB_UNIT;
+    const pb_u32 ps = qs + PB_TERMS * PB_HT * PB_QROW;
+    float* wmax = reinterpret_cast<float*>(raw + (ps + PB_TERMS * PB_HT * PB_PROW - pb_smem(raw)));
+    float* wsum = wmax + 4 * PB_HT;
+    const pb_u32 full = pb_smem(bars), empty = full + 8 * PB_RING;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < PB_RING; ++i) {
+            pb_mbar_init(full + 8 * i, 1);
+            pb_mbar_init(empty + 8 * i, 4);
+        }
+        abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    __shared__ float sh[8];
-    const pb_i64 row = blockIdx.x;
-    const int s = (int)(row / heads), kvh = (int)(row % heads) / group, n = lengths[s];
-    const int* table = tables + (pb_i64)s * width;
-    float* w = weights + row * longest;
-    const float* x = q + row * PB_D;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    float top = __int_as_float(0xff800000);
-    for (int i = warp; i < n; i += 8) {
-        const pb_cell* k = pk + (((pb_i64)table[i / PB_PS] * PB_H + kvh) * PB_PS + i % PB_PS) * PB_D;
-        float a = 0.0f;
-        for (int d = lane; d < PB_D; d += 32) a = fmaf(x[d], pb_value(k[d]), a);
+    const int4 mine = work[blockIdx.x];
+    pb_at at;
+    at.row = mine.x;
+    at.tile = mine.y;
+    pb_enter(at, lengths, chunks);
+
+    if (warp == 4) {
+        // ---- producer: K then V of each tile into the ring
+        int slot = 0, unit = 0;
+        pb_u32 parity = 1; // the first round finds every unit free
+        bool bad = false;
+        for (int i = 0; i < mine.z && !bad; ++i) {
+            if (i) pb_next(at, lengths, chunks);
+            const int base = at.tile * 64, boxes = (min(64, at.length - base) + PB_BOX - 1) / PB_BOX;
+            int y = 0;
+            if (lane < boxes) {
+                const int first = base + lane * PB_BOX;
+                y = (tables[(pb_i64)at.s * width + first / PB_PS] * PB_H + at.h) * PB_PS + first % PB_PS;
+            }
+#pragma unroll 1
+            for (int which = 0; which < 2 && !bad; ++which) {
+                bad = !pb_wait(empty + 8 * slot, parity, &abort_flag, err, 1 + which);
+                bad = __any_sync(0xffffffffu, bad);
+                if (bad) break;
+                if (lane == 0) pb_mbar_expect_tx(full + 8 * slot, boxes * PB_BOX * 128 * PB_PLANES);
+                __syncwarp();
+                if (lane < boxes) {
+                    const pb_u32 dst = ring + slot * PB_UNIT + lane * PB_BOX * 128;
 #pragma unroll
-        for (int m = 16; m > 0; m /= 2) a += __shfl_xor_sync(0xffffffffu, a, m);
-        a *= scale;
-        if (lane == 0) w[i] = a;
-        top = fmaxf(top, a);
+                    for (int c = 0; c < PB_PLANES; ++c)
+                        pb_tma_load(dst + c * 8192, which ? &map_v : &map_k, full + 8 * slot, c * PB_CE, y);
+                }
+                ++unit;
+                if (++slot == PB_RING) { slot = 0; parity ^= 1u; }
+            }
+        }
+        // Nothing may land after this CTA is gone: wait (bounded) for what
+        // is still in flight, which is only ever the case after an abort.
+        if (bad && lane == 0) {
+            for (int u = unit > PB_RING ? unit - PB_RING : 0; u < unit; ++u) {
+                const long long start = clock64();
+                while (!pb_mbar_try(full + 8 * (u % PB_RING), (u / PB_RING) & 1) && clock64() - start <= PB_WAIT_CYCLES) {
+                }
+            }
+        }
+        return;
     }
-    top = pb_block_reduce(top, true, sh);
-    float sum = 0.0f;
-    for (int i = threadIdx.x; i < n; i += 256) {
-        const float p = expf(w[i] - top);
-        w[i] = p;
-        sum += p;
+
+    // ---- four computing warps
+    const int g = lane >> 2, t = lane & 3;
+    int slot = 0;
+    pb_u32 parity = 0;
+    bool bad = false, fresh = true;
+    int segment = 0; // how many rows this CTA has begun
+    float m[PB_NT][2], l[PB_NT][2], o[PB_MTW][PB_NT][4];
+    bool begun_at_zero = true;
+    for (int i = 0; i < mine.z; ++i) {
+        if (i) fresh = pb_next(at, lengths, chunks);
+        const int hg = min(PB_HT, group - at.chunk * PB_HT);             // query heads of this row
+        const int head0 = at.h * group + at.chunk * PB_HT;                // the first
+        if (fresh) {
+            begun_at_zero = at.tile == 0;
+            // The row's queries, split into terms; zero past the head size.
+            for (int e = threadIdx.x; e < PB_HT * (PB_STEPS * 32 / PB_ESZ); e += 128) {
+                const int head = e / (PB_STEPS * 32 / PB_ESZ), d = e % (PB_STEPS * 32 / PB_ESZ);
+                const float x = head < hg && d < PB_D ? __ldg(q + at.s * q_seq + (head0 + head) * q_head + d) : 0.0f;
+                pb_split_store(qs + head * PB_QROW + d * PB_ESZ, PB_HT * PB_QROW, x);
+            }
+#pragma unroll
+            for (int n = 0; n < PB_NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) { m[n][e] = __int_as_float(0xff800000); l[n][e] = 0.0f; }
+#pragma unroll
+            for (int a = 0; a < PB_MTW; ++a)
+#pragma unroll
+                for (int n = 0; n < PB_NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[a][n][e] = 0.0f;
+            if (pb_bar_any(bad)) { bad = true; break; }
+        }
+        const int base = at.tile * 64, valid = min(64, at.length - base);
+
+        // ---- S^T = K Q^T: this warp's 16 slots x all heads
+        bad |= !pb_wait(full + 8 * slot, parity, &abort_flag, err, 3);
+        float c[PB_TERMS][PB_NT][4];
+#pragma unroll
+        for (int x = 0; x < PB_TERMS; ++x)
+#pragma unroll
+            for (int n = 0; n < PB_NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) c[x][n][e] = 0.0f;
+        {
+            const int r = 16 * warp + (lane & 15);
+            const pb_u32 krow = ring + slot * PB_UNIT + r * 128;
+            const pb_u32 qrow = qs + (lane & 7) * PB_QROW + (lane >> 3) * 16;
+#pragma unroll
+            for (int k2 = 0; k2 < PB_STEPS / 2; ++k2) {
+                pb_u32 a[2][4];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int chunk = (2 * k2 + k) * 2; // 16-byte chunk of the row; its plane and place
+                    pb_ldm4(a[k], krow + (chunk >> 3) * 8192 + ((((chunk & 7) + (lane >> 4)) ^ (r & 7)) << 4));
+                }
+#if PB_ESZ == 2
+#pragma unroll
+                for (int x = 0; x < PB_TERMS; ++x)
+#pragma unroll
+                    for (int n = 0; n < PB_NT; ++n) {
+                        pb_u32 b[4];
+                        pb_ldm4(b, qrow + (x * PB_HT + n * 8) * PB_QROW + k2 * 64);
+                        pb_mma(c[x][n], a[0], b);
+                        pb_mma(c[x][n], a[1], b + 2);
+                    }
+#else
+                pb_u32 hi[2][4], lo[2][4];
+                pb_split_frag(a[0], hi[0], lo[0]);
+                pb_split_frag(a[1], hi[1], lo[1]);
+#pragma unroll
+                for (int n = 0; n < PB_NT; ++n) {
+                    pb_u32 b[4], b2[4];
+                    pb_ldm4(b, qrow + (n * 8) * PB_QROW + k2 * 64);
+                    pb_ldm4(b2, qrow + (PB_HT + n * 8) * PB_QROW + k2 * 64);
+                    pb_mma(c[0][n], hi[0], b);
+                    pb_mma(c[1][n], hi[0], b2);
+                    pb_mma(c[0][n], hi[1], b + 2);
+                    pb_mma(c[1][n], lo[0], b);
+                    pb_mma(c[1][n], hi[1], b2 + 2);
+                    pb_mma(c[1][n], lo[1], b + 2);
+                }
+#endif
+            }
+        }
+        __syncwarp();
+        if (lane == 0) pb_mbar_arrive(empty + 8 * slot);
+        if (++slot == PB_RING) { slot = 0; parity ^= 1u; }
+
+        // Logits in units of log2, -inf past the sequence's end. Thread: slots
+        // 16 warp + g and + 8, heads 8 n + 2 t and + 1.
+        float s[PB_NT][4], top[PB_NT][2];
+#pragma unroll
+        for (int n = 0; n < PB_NT; ++n) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int at_slot = 16 * warp + g + (e >> 1) * 8;
+#if PB_TERMS == 3
+                const float x = (c[2][n][e] + c[1][n][e] + c[0][n][e]) * scale2;
+#else
+                const float x = (c[1][n][e] + c[0][n][e]) * scale2;
+#endif
+                s[n][e] = at_slot < valid ? x : __int_as_float(0xff800000);
+#if PB_SCORED
+                const int head = 8 * n + 2 * t + (e & 1);
+                if (at_slot < valid && head < hg)
+                    logits[((pb_i64)at.s * PB_H * group + head0 + head) * longest + base + at_slot] = x;
+#endif
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float x = fmaxf(s[n][e], s[n][e + 2]);
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                top[n][e] = x;
+            }
+            if (g == 0) *reinterpret_cast<float2*>(wmax + warp * PB_HT + 8 * n + 2 * t) = make_float2(top[n][0], top[n][1]);
+        }
+        if (pb_bar_any(bad)) { bad = true; break; }
+
+        // ---- weights relative to the running maximum, split into terms
+        float corr[PB_NT][2];
+#pragma unroll
+        for (int n = 0; n < PB_NT; ++n) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float2 x = *reinterpret_cast<const float2*>(wmax + w * PB_HT + 8 * n + 2 * t);
+                top[n][0] = fmaxf(top[n][0], x.x);
+                top[n][1] = fmaxf(top[n][1], x.y);
+            }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float now = fmaxf(m[n][e], top[n][e]);
+                corr[n][e] = pb_exp2(m[n][e] - now);
+                m[n][e] = now;
+                l[n][e] *= corr[n][e];
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float p = pb_exp2(s[n][e] - m[n][e & 1]);
+                l[n][e & 1] += p;
+                const int at_slot = 16 * warp + g + (e >> 1) * 8, head = 8 * n + 2 * t + (e & 1);
+#if PB_ESZ == 2
+                const int place = at_slot;
+#else
+                const int place = (at_slot & ~7) + ((at_slot & 7) >> 1) + (at_slot & 1) * 4; // as V's fragments count slots
+#endif
+                pb_split_store(ps + head * PB_PROW + place * PB_ESZ, PB_HT * PB_PROW, p);
+            }
+        }
+        bad |= !pb_wait(full + 8 * slot, parity, &abort_flag, err, 4);
+        if (pb_bar_any(bad)) { bad = true; break; }
+
+        // ---- O^T += V^T P^T: this warp's channels x all heads. The tile's sum
+        // starts from zero in the tensor core, whose additions cut low bits,
+        // and is added to the running one in fp32, rounded to nearest.
+        {
+            const pb_u32 vunit = ring + slot * PB_UNIT;
+            const pb_u32 prow = ps + (lane & 7) * PB_PROW + (lane >> 3) * 16;
+            float d[PB_MTW][PB_NT][2][4];
+#pragma unroll
+            for (int a = 0; a < PB_MTW; ++a)
+#pragma unroll
+                for (int n = 0; n < PB_NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) d[a][n][0][e] = d[a][n][1][e] = 0.0f;
+#pragma unroll
+            for (int k2 = 0; k2 < 2 * PB_ESZ / 2; ++k2) { // two k-steps at a time
+                pb_u32 b[PB_TERMS][PB_NT][4];
+#pragma unroll
+                for (int x = 0; x < PB_TERMS; ++x)
+#pragma unroll
+                    for (int n = 0; n < PB_NT; ++n) pb_ldm4(b[x][n], prow + (x * PB_HT + n * 8) * PB_PROW + k2 * 64);
+#pragma unroll
+                for (int a = 0; a < PB_MTW; ++a) {
+                    const int mt = warp + 4 * a;
+                    if (mt < PB_MT) {
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            pb_u32 v[4];
+#if PB_ESZ == 2
+                            const int first = (2 * k2 + k) * 16;
+                            const int r = first + (lane >> 4) * 8 + (lane & 7);
+                            const int chunk = mt * 2 + ((lane >> 3) & 1);
+                            pb_ldm4t(v, vunit + (chunk >> 3) * 8192 + r * 128 + (((chunk & 7) ^ (r & 7)) << 4));
+                            if (valid < 64) { // what lies past the end may be anything
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    const int left = valid - (first + 2 * t + (e >> 1) * 8);
+                                    v[e] = left >= 2 ? v[e] : (left == 1 ? v[e] & 0xffffu : 0u);
+                                }
+                            }
+#pragma unroll
+                            for (int n = 0; n < PB_NT; ++n) {
+                                pb_mma(d[a][n][0], v, b[0][n] + 2 * k);
+                                pb_mma(d[a][n][1], v, b[2][n] + 2 * k);
+                                pb_mma(d[a][n][1], v, b[1][n] + 2 * k);
+                            }
+#else
+                            // Slots 2 t and 2 t + 1 stand for columns t and t + 4:
+                            // their rows' swizzles put the loads on distinct banks.
+                            const int first = (2 * k2 + k) * 8 + 2 * t;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const int r = first + (e >> 1), ch = mt * 16 + g + (e & 1) * 8;
+                                const pb_u32 where = vunit + (ch >> 5) * 8192 + r * 128 + ((((ch & 31) >> 2) ^ (r & 7)) << 4) + (ch & 3) * 4;
+                                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[e]) : "r"(where) : "memory");
+                                if (r >= valid) v[e] = 0u;
+                            }
+                            pb_u32 hi[4], lo[4];
+                            pb_split_frag(v, hi, lo);
+#pragma unroll
+                            for (int n = 0; n < PB_NT; ++n) {
+                                pb_mma(d[a][n][0], hi, b[0][n] + 2 * k);
+                                pb_mma(d[a][n][1], hi, b[1][n] + 2 * k);
+                                pb_mma(d[a][n][1], lo, b[0][n] + 2 * k);
+                            }
+#endif
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int a = 0; a < PB_MTW; ++a)
+#pragma unroll
+                for (int n = 0; n < PB_NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        o[a][n][e] = fmaf(o[a][n][e], corr[n][e & 1], d[a][n][1][e] + d[a][n][0][e]);
+        }
+        __syncwarp();
+        if (lane == 0) pb_mbar_arrive(empty + 8 * slot);
+        if (++slot == PB_RING) { slot = 0; parity ^= 1u; }
+
+        // ---- the row ends, or this CTA's part of it
+        const bool row_ends = at.tile + 1 == at.tiles;
+        if (row_ends || i + 1 == mine.z) {
+#pragma unroll
+            for (int n = 0; n < PB_NT; ++n) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float x = l[n][e];
+                    x += __shfl_xor_sync(0xffffffffu, x, 4);
+                    x += __shfl_xor_sync(0xffffffffu, x, 8);
+                    x += __shfl_xor_sync(0xffffffffu, x, 16);
+                    l[n][e] = x;
+                }
+                if (g == 0) *reinterpret_cast<float2*>(wsum + warp * PB_HT + 8 * n + 2 * t) = make_float2(l[n][0], l[n][1]);
+            }
+            if (pb_bar_any(bad)) { bad = true; break; }
+            const bool whole = begun_at_zero && row_ends;
+            const pb_i64 part = (pb_i64)blockIdx.x * 2 + (segment ? 1 : 0);
+#pragma unroll
+            for (int n = 0; n < PB_NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int head = 8 * n + 2 * t + e;
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) sum += wsum[w * PB_HT + head];
+                    if (head >= hg) continue;
+                    const pb_i64 global = (pb_i64)at.s * PB_H * group + head0 + head;
+                    float* to = whole ? out + global * PB_D : partial + (part * PB_HT + head) * PB_D;
+                    const float inv = whole ? 1.0f / sum : 1.0f;
+#pragma unroll
+                    for (int a = 0; a < PB_MTW; ++a) {
+                        const int ch = (warp + 4 * a) * 16 + g;
+                        if (ch < PB_D) to[ch] = o[a][n][e] * inv;
+                        if (ch + 8 < PB_D) to[ch + 8] = o[a][n][e + 2] * inv;
+                    }
+                    if (warp == 0 && g == 0) {
+                        if (!whole) partial_ml[part * PB_HT + head] = make_float2(m[n][e], sum);
+#if PB_SCORED
+                        else lse[global] = m[n][e] + log2f(sum);
+#endif
+                    }
+                }
+            ++segment;
+        }
     }
-    sum = pb_block_reduce(sum, false, sh);
-    for (int i = threadIdx.x; i < n; i += 256) w[i] /= sum;
-    __syncthreads();
-    for (int d = threadIdx.x; d < PB_D; d += 256) {
-        float a = 0.0f;
-        for (int i = 0; i < n; ++i)
-            a = fmaf(w[i], pb_value(pv[(((pb_i64)table[i / PB_PS] * PB_H + kvh) * PB_PS + i % PB_PS) * PB_D + d]), a);
-        out[row * PB_D + d] = a;
-    }
+    if (bad) abort_flag = 1;
 }
 
-extern "C" __global__ void __launch_bounds__(256) pb_attend_scores(
-    const float* weights, const int* lengths, const float* scores, float* out, pb_i64 longest, pb_i64 ns, int group) {
+// Joins the parts of a row that several CTAs worked on, and writes zeros for a
+// row without slots. Block: one query head of one such row.
+extern "C" __global__ void __launch_bounds__(128) pb_paged_join(
+    const int4* rows, const float* partial, const float2* partial_ml, float* out, float* lse, int group, int chunks) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    __shared__ float weight[128];
+    const int4 r = rows[blockIdx.x / PB_HT]; // row, first CTA, number of parts, the first part's place
+    const int head = blockIdx.x % PB_HT, chunk = r.x % chunks, kvh = (r.x / chunks) % PB_H, s = r.x / chunks / PB_H;
+    if (head >= group - chunk * PB_HT) return;
+    const pb_i64 global = (pb_i64)s * PB_H * group + kvh * group + chunk * PB_HT + head;
+    float top = __int_as_float(0xff800000);
+    for (int i = 0; i < r.z; ++i) top = fmaxf(top, partial_ml[(pb_i64)(2 * (r.y + i) + (i ? 0 : r.w)) * PB_HT + head].x);
+    float sum = 0.0f, acc[(PB_D + 127) / 128] = {};
+    for (int from = 0; from < r.z; from += 128) {
+        const int n = min(128, r.z - from);
+        __syncthreads();
+        if (threadIdx.x < n) {
+            const int i = from + threadIdx.x;
+            weight[threadIdx.x] = pb_exp2(partial_ml[(pb_i64)(2 * (r.y + i) + (i ? 0 : r.w)) * PB_HT + head].x - top);
+        }
+        __syncthreads();
+        for (int j = 0; j < n; ++j) {
+            const int i = from + j;
+            const pb_i64 part = (pb_i64)(2 * (r.y + i) + (i ? 0 : r.w)) * PB_HT + head;
+            sum = fmaf(weight[j], partial_ml[part].y, sum);
+#pragma unroll
+            for (int a = 0; a < (PB_D + 127) / 128; ++a)
+                if (threadIdx.x + 128 * a < PB_D) acc[a] = fmaf(weight[j], partial[part * PB_D + threadIdx.x + 128 * a], acc[a]);
+        }
+    }
+#pragma unroll
+    for (int a = 0; a < (PB_D + 127) / 128; ++a)
+        if (threadIdx.x + 128 * a < PB_D) out[global * PB_D + threadIdx.x + 128 * a] = r.z ? acc[a] / sum : 0.0f;
+#if PB_SCORED
+    if (threadIdx.x == 0) lse[global] = r.z ? top + log2f(sum) : 0.0f;
+#endif
+}
+
+#if PB_SCORED
+// new[s, h, i] = scores[s, h, i] + sum over the group of 2^(logit - lse).
+extern "C" __global__ void __launch_bounds__(256) pb_paged_scores(
+    const float* logits, const float* lse, const int* lengths, const float* scores, float* out, pb_i64 longest,
+    pb_i64 ns, int group) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const pb_u32 blocks = (pb_u32)((longest + 255) / 256);
     const pb_i64 i = (pb_i64)(blockIdx.x % blocks) * 256 + threadIdx.x, row = blockIdx.x / blocks;
     if (i >= longest) return;
     float a = 0.0f;
     if (i < lengths[row / PB_H]) {
-        a = i < ns ? scores[row * ns + i] : 0.0f;
-        for (int g = 0; g < group; ++g) a += weights[(row * group + g) * longest + i];
+        for (int g = 0; g < group; ++g) a += pb_exp2(logits[(row * group + g) * longest + i] - lse[row * group + g]);
+        if (i < ns) a += scores[row * ns + i];
     }
     out[row * longest + i] = a;
 }
+#endif
 )PB";
         }
 
-        std::string defines(int64_t heads, int64_t dim, int64_t page, bool bf16) {
+        std::string defines(const form& f) {
             std::ostringstream os;
-            os << "#define PB_H " << heads << "\n#define PB_D " << dim << "\n#define PB_PS " << page
-               << "\n#define PB_BF16 " << (bf16 ? 1 : 0) << "\n";
+            os << "#define PB_H " << f.heads << "\n#define PB_D " << f.dim << "\n#define PB_PS " << f.page
+               << "\n#define PB_ESZ " << f.width() << "\n#define PB_NT " << f.tiles8 << "\n#define PB_RING " << f.ring()
+               << "\n#define PB_PER_SM " << f.per_sm() << "\n#define PB_SCORED " << (f.scored ? 1 : 0) << "\n";
             return os.str();
         }
 
-        op_kernel& kernel_of(const char* name, const std::string& defs) {
+        op_kernel& kernel_of(const char* name, const form& f, uint32_t smem) {
+            const std::string defs = defines(f);
             return op_kernel_for(std::string{name} + "\n" + defs, [&](op_kernel& k) {
                 k.name = name;
                 k.source = std::string{kernel_prelude()} + defs + device_source();
+                k.smem = smem;
             });
+        }
+
+        // Even runs of 64-slot tiles, over all rows one after the other: the
+        // CTAs' shares differ by one tile at most, whatever the lengths. A run
+        // begins and ends inside a row at most once each, so a CTA leaves at
+        // most two parts behind.
+        struct schedule {
+            std::vector<int32_t> work; // per CTA: row, tile, tiles, 0
+            std::vector<int32_t> join; // per row to join or clear: row, first CTA, parts, its place
+        };
+
+        schedule make_schedule(const std::vector<int64_t>& lengths, int64_t heads, int64_t chunks, int64_t ctas) {
+            schedule r;
+            const int64_t per = heads * chunks;
+            int64_t total = 0;
+            for (int64_t n : lengths) total += (n + 63) / 64 * per;
+            const int64_t n = std::min(total, ctas);
+            int64_t cta = 0, from = 0; // `from`: the row's first tile in the whole order
+            auto start = [&](int64_t c) { return n == 0 ? 0 : static_cast<int64_t>(static_cast<__int128>(total) * c / n); };
+            for (size_t s = 0; s < lengths.size(); ++s) {
+                const int64_t tiles = (lengths[s] + 63) / 64;
+                for (int64_t j = 0; j < per; ++j) {
+                    const int64_t row = static_cast<int64_t>(s) * per + j;
+                    auto add = [&](int64_t first, int64_t parts, int64_t place) {
+                        for (int64_t v : {row, first, parts, place}) r.join.push_back(static_cast<int32_t>(v));
+                    };
+                    if (tiles == 0) {
+                        add(0, 0, 0);
+                        continue;
+                    }
+                    // CTAs that begin in this row.
+                    while (cta < n && start(cta) < from + tiles) {
+                        for (int64_t v : {row, start(cta) - from, start(cta + 1) - start(cta), int64_t{0}})
+                            r.work.push_back(static_cast<int32_t>(v));
+                        ++cta;
+                    }
+                    // Its first part belongs to the last CTA that begins at or before it.
+                    int64_t first = cta - 1;
+                    while (start(first) > from) --first;
+                    const int64_t parts = cta - first;
+                    if (parts > 1) add(first, parts, start(first) < from ? 1 : 0);
+                    from += tiles;
+                }
+            }
+            return r;
         }
 
     } // namespace
@@ -139,41 +703,133 @@ extern "C" __global__ void __launch_bounds__(256) pb_attend_scores(
         expect(device == c.device && (scores == nullptr || device_of(*scores, "paged_attention_scored") == device),
                "paged_attention: operands must live on the cache's device");
         auto stream = current_stream(device);
-        op_operand x = operand(q, stream, false), xs;
+        op_operand x = operand(q, stream, true), xs;
         if (scores != nullptr) xs = operand(*scores, stream, false);
+        form f;
+        f.heads = static_cast<int>(c.heads);
+        f.dim = static_cast<int>(c.dim);
+        f.page = static_cast<int>(c.page_size);
+        f.bf16 = c.type == cache_type::bf16;
+        f.scored = scored;
+        int heads = static_cast<int>(shape[1]), group = static_cast<int>(shape[1] / c.heads);
+        // 16 query heads share a tile's loads, 8 where 16 would leave the ring
+        // less than three units.
+        f.tiles8 = group > 8 ? 2 : 1;
+        if (f.ring() < 3) f.tiles8 = 1;
+        int chunks = (group + 8 * f.tiles8 - 1) / (8 * f.tiles8);
+        const int64_t rows = n * c.heads * chunks;
+        expect(rows < (int64_t{1} << 27), "paged_attention: too many sequences and heads");
+        const batch_plan& plan = plan_of(batch, chunks, int64_t{f.per_sm()} * sm_count(device));
+
         op_result out = new_result(shape, device, stream);
         order_read(*cuda_jit::buffer_access::state(batch.data), stream);
         order_read(*cuda_jit::buffer_access::state(c.k), stream);
         order_read(*cuda_jit::buffer_access::state(c.v), stream);
-        const std::string defs = defines(c.heads, c.dim, c.page_size, c.type == cache_type::bf16);
+        if (plan.data.size_bytes() != 0) order_read(*cuda_jit::buffer_access::state(plan.data), stream);
+
         int64_t longest = batch.longest;
-        int heads = static_cast<int>(shape[1]), group = static_cast<int>(shape[1] / c.heads);
-        int width = static_cast<int>(batch.table_width);
-        auto scratch = allocate(device, static_cast<size_t>(std::max<int64_t>(1, n * heads * longest)) * sizeof(float), stream);
-        uint64_t weights = address(scratch), pk = address(c.k), pv = address(c.v);
-        void* params[] = {&x.ptr, &pk,      &pv,    &batch.lengths_at, &batch.tables_at, &weights,
-                          &out.ptr, &longest, &width, &heads,          &group,           &scale};
-        op_launch(kernel_of("pb_attend", defs), device, stream, {static_cast<uint32_t>(n * heads), 1, 1}, 256, params);
+        int width = static_cast<int>(batch.table_width), longest32 = static_cast<int>(longest);
+        // Workspace: the parts of split rows, and for scores the logits and
+        // each head's log-sum.
+        const size_t part_heads = static_cast<size_t>(plan.ctas) * 2 * static_cast<size_t>(8 * f.tiles8);
+        const size_t parts = part_heads * static_cast<size_t>(c.dim), sums = scored ? static_cast<size_t>(n * heads) : 0;
+        const size_t all = parts + 2 * part_heads + sums + (scored ? static_cast<size_t>(n * heads * longest) : 0);
+        auto scratch = allocate(device, std::max<size_t>(1, all) * sizeof(float), stream);
+        uint64_t ml = address(scratch), partial = ml + 2 * part_heads * 4, lse = partial + parts * 4, logits = lse + sums * 4;
+        uint64_t work = address(plan.data), join = work + static_cast<uint64_t>(plan.ctas) * 16, err = 0;
+        if (plan.ctas > 0) {
+            check(pbrt_error_word(device, &err));
+            struct alignas(64) map {
+                unsigned char bytes[128];
+            } mk, mv;
+            const uint64_t dims[2] = {static_cast<uint64_t>(c.dim), static_cast<uint64_t>(c.pages * c.heads * c.page_size)};
+            const uint64_t strides[1] = {static_cast<uint64_t>(c.dim * c.width())};
+            const uint32_t box[2] = {static_cast<uint32_t>(128 / c.width()), static_cast<uint32_t>(std::min<int64_t>(64, c.page_size))};
+            const uint32_t ones[2] = {1, 1};
+            // bfloat16 or float32, 128-byte swizzle, 256-byte L2 promotion, zeros past the head size.
+            for (auto [m, p] : {std::pair{&mk, &c.k}, std::pair{&mv, &c.v}})
+                check(pbrt_tensor_map_encode_tiled(m->bytes, f.bf16 ? 9 : 7, 2, address(*p), dims, strides, box, ones, 0, 3, 3, 0));
+            float scale2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
+            void* params[] = {&mk,     &mv,    &x.ptr, &batch.lengths_at, &batch.tables_at, &work,
+                              &out.ptr, &partial, &ml, &logits, &lse, &width, &group, &chunks,
+                              &x.strides[0], &x.strides[1], &longest32, &scale2, &err};
+            op_launch(kernel_of("pb_paged_attention", f, static_cast<uint32_t>(f.smem())), device, stream,
+                      {static_cast<uint32_t>(plan.ctas), 1, 1}, 160, params);
+        }
+        if (plan.joins > 0) {
+            void* params[] = {&join, &partial, &ml, &out.ptr, &lse, &group, &chunks};
+            op_launch(kernel_of("pb_paged_join", f, 0), device, stream,
+                      {static_cast<uint32_t>(plan.joins * 8 * f.tiles8), 1, 1}, 128, params);
+        }
         std::vector<tensor> results;
         results.push_back(finish(std::move(out)));
         if (scored) {
             op_result os = new_result({n, c.heads, longest}, device, stream);
             if (longest != 0) {
-                void* sparams[] = {&weights, &batch.lengths_at, &xs.ptr, &os.ptr, &longest, &ns, &group};
                 const int64_t blocks = (longest + 255) / 256 * n * c.heads;
                 expect(blocks <= 0x7fffffff, "paged_attention_scored: too many slots");
-                op_launch(kernel_of("pb_attend_scores", defs), device, stream, {static_cast<uint32_t>(blocks), 1, 1},
-                          256, sparams);
+                void* params[] = {&logits, &lse, &batch.lengths_at, &xs.ptr, &os.ptr, &longest, &ns, &group};
+                op_launch(kernel_of("pb_paged_scores", f, 0), device, stream, {static_cast<uint32_t>(blocks), 1, 1}, 256,
+                          params);
             }
             results.push_back(finish(std::move(os)));
         }
         return results;
     }
 
+    int attention_ctas_per_sm(const kv_cache& c) {
+        form f;
+        f.heads = static_cast<int>(c.heads);
+        f.dim = static_cast<int>(c.dim);
+        f.bf16 = c.type == cache_type::bf16;
+        return f.per_sm();
+    }
+
+    const batch_plan& plan_of(kv_batch& batch, int64_t chunks, int64_t ctas) {
+        std::scoped_lock lock{batch.plans->mutex};
+        for (const auto& p : batch.plans->made)
+            if (p->chunks == chunks && p->limit == ctas) return *p;
+        schedule s = make_schedule(batch.lengths, batch.cache->heads, chunks, ctas);
+        auto p = std::make_unique<batch_plan>();
+        p->chunks = chunks;
+        p->limit = ctas;
+        p->ctas = static_cast<int64_t>(s.work.size() / 4);
+        p->joins = static_cast<int64_t>(s.join.size() / 4);
+        s.work.insert(s.work.end(), s.join.begin(), s.join.end());
+        const int device = batch.cache->device;
+        auto stream = upload_stream(device);
+        p->data = allocate(device, s.work.size() * sizeof(int32_t), stream);
+        check(pbrt_memcpy_h2d_async(device, address(p->data), s.work.data(), s.work.size() * sizeof(int32_t), stream->stream));
+        check(pbrt_stream_synchronize(device, stream->stream));
+        batch.plans->made.push_back(std::move(p));
+        return *batch.plans->made.back();
+    }
+
+    std::string attention_schedule(const std::vector<int64_t>& lengths, int64_t heads, int64_t chunks, int64_t ctas) {
+        const schedule s = make_schedule(lengths, heads, chunks, ctas);
+        std::ostringstream os;
+        for (size_t i = 0; i < s.work.size(); i += 4)
+            os << "work " << s.work[i] << " " << s.work[i + 1] << " " << s.work[i + 2] << "\n";
+        for (size_t i = 0; i < s.join.size(); i += 4)
+            os << "join " << s.join[i] << " " << s.join[i + 1] << " " << s.join[i + 2] << " " << s.join[i + 3] << "\n";
+        return os.str();
+    }
+
     void paged_attention_sources(kernel_list& out) {
-        for (const bool bf16 : {true, false})
-            out.emplace_back(std::string{"pb_attend_"} + (bf16 ? "bf16" : "f32"),
-                             std::string{kernel_prelude()} + defines(8, 128, 64, bf16) + device_source());
+        for (const auto& [dim, width, tiles8, page] :
+             {std::array<int, 4>{128, 2, 1, 64}, std::array<int, 4>{64, 2, 1, 16}, std::array<int, 4>{64, 4, 1, 16},
+              std::array<int, 4>{128, 4, 1, 8}, std::array<int, 4>{256, 4, 1, 256}, std::array<int, 4>{256, 2, 2, 32},
+              std::array<int, 4>{72, 2, 2, 32}, std::array<int, 4>{8, 4, 2, 32}}) {
+            form f;
+            f.heads = 8;
+            f.dim = dim;
+            f.bf16 = width == 2;
+            f.tiles8 = tiles8;
+            f.page = page;
+            f.scored = true;
+            out.emplace_back("pb_paged_attention_" + std::to_string(dim) + (f.bf16 ? "_bf16_" : "_f32_") + std::to_string(8 * tiles8),
+                             std::string{kernel_prelude()} + defines(f) + device_source());
+        }
     }
 
 } // namespace porch::detail

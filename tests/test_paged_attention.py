@@ -168,6 +168,51 @@ def test_refusals_that_need_no_device(api):
         api.KVCache(4, 16, 1, 64, dtype="f16")
 
 
+@pytest.mark.parametrize("seed", range(40))
+def test_every_tile_is_worked_on_once_and_every_split_row_joined(api, seed):
+    # Walks the CTAs as the kernel does.
+    rng = np.random.default_rng(seed)
+    n = int(rng.integers(1, 30))
+    lengths = [int(x) if rng.random() > 0.2 else 0 for x in np.exp(rng.uniform(0, 9, n))]
+    heads, chunks, ctas = int(rng.integers(1, 6)), int(rng.integers(1, 4)), int(rng.integers(1, 600))
+    if seed == 0:
+        lengths = [0] * n
+    tiles = np.repeat([-(-x // 64) for x in lengths], heads * chunks)
+    work, join = [], {}
+    for line in api.attention_plan(lengths, heads, ctas, chunks).splitlines():
+        kind, *v = line.split()
+        if kind == "work":
+            work.append([int(x) for x in v])
+        else:
+            row, *rest = (int(x) for x in v)
+            assert row not in join
+            join[row] = rest
+    assert len(work) == min(ctas, tiles.sum())
+    assert not work or max(w[2] for w in work) - min(w[2] for w in work) <= 1
+    seen, parts = np.zeros(tiles.sum(), int), {}
+    first = np.concatenate([[0], np.cumsum(tiles)])
+    for c, (row, tile, count) in enumerate(work):
+        segment, at_zero = 0, tile == 0
+        for i in range(count):
+            assert tile < tiles[row]
+            seen[first[row] + tile] += 1
+            ends = tile + 1 == tiles[row]
+            if ends or i + 1 == count:
+                if not (at_zero and ends):
+                    parts.setdefault(row, []).append((c, 1 if segment else 0))
+                segment += 1
+            if i + 1 < count:
+                tile += 1
+                if ends:
+                    tile, at_zero = 0, True
+                    row += 1
+                    while tiles[row] == 0:
+                        row += 1
+    assert (seen == 1).all()
+    want = {r: [] for r in np.flatnonzero(tiles == 0)} | parts
+    assert want == {r: [(c + i, 0 if i else place) for i in range(k)] for r, (c, k, place) in join.items()}
+
+
 @pytest.mark.gpu
 def test_refusals(gpu):
     cache = gpu.KVCache(6, 16, 2, 64)
