@@ -257,6 +257,13 @@ int pb_comm_wait(pb_comm* comm);
 int pb_tensor_from_device(const int64_t* shape, size_t rank, uint64_t pointer, size_t count,
                           void* stream, int device, pb_tensor** out);
 
+/* What another library on the same GPU needs to read the values in place:
+ * shape (up to `capacity` extents; *rank receives the rank), device address
+ * (as pb_tensor_device_pointer) and this thread's stream (a CUstream), which
+ * the values are ordered on. */
+int pb_tensor_interface(const pb_tensor* tensor, int64_t* shape, size_t capacity, size_t* rank,
+                        uint64_t* pointer, void** stream);
+
 /* RMS norm of each query and key head with a weight per channel, and the
  * rotation of its first 2 * R2 channels by the token's position:
  *   y = R(position) (weight * x / sqrt(mean(x^2) + eps))

@@ -106,9 +106,9 @@ class Expr:
         if h is not None and h.value:
             try:
                 lib().pb_expr_release(h)
+                self._h = c_void_p(None)
             except Exception:  # interpreter shutdown
                 pass
-            self._h = c_void_p(None)
 
     # -- metadata
     def shape(self) -> list[int]:
@@ -195,19 +195,20 @@ def _unary(op: int, a) -> Expr:
 class Tensor:
     """porch::tensor (a shared handle)."""
 
-    __slots__ = ("_h",)
+    __slots__ = ("_h", "_face")
 
     def __init__(self, handle: int):
         self._h = c_void_p(handle)
+        self._face = None
 
     def __del__(self):
         h = getattr(self, "_h", None)
         if h is not None and h.value:
             try:
                 lib().pb_tensor_release(h)
+                self._h = c_void_p(None)
             except Exception:
                 pass
-            self._h = c_void_p(None)
 
     # -- metadata
     def shape(self) -> list[int]:
@@ -278,11 +279,14 @@ class Tensor:
         """The values in place, for another library on the same GPU (as
         device_data(): a raw handle, so a consumer that does not order its
         work behind `stream` calls synchronize() first)."""
-        pointer, _ = self.device_data()
-        stream = c_void_p()
-        _check_rt(lib().pbrt_stream_current(_builtins.max(0, self.placement()), byref(stream)))
-        return {"shape": tuple(self.shape()), "typestr": "<f4", "data": (pointer, False), "version": 3,
-                "stream": stream.value}
+        if self._face is None:
+            # The address of a realised tensor's values stays what it is once
+            # it was handed out, so consumers that ask twice cost one call.
+            shape, rank, pointer, stream = (c_int64 * 16)(), c_size_t(), c_uint64(), c_void_p()
+            _check(lib().pb_tensor_interface(self._h, shape, 16, byref(rank), byref(pointer), byref(stream)))
+            self._face = {"shape": tuple(shape[:rank.value]), "typestr": "<f4", "data": (pointer.value, False),
+                          "version": 3, "stream": stream.value}
+        return self._face
 
     def __getitem__(self, key) -> Expr:
         if not isinstance(key, tuple):
@@ -584,9 +588,9 @@ class KVCache:
         if h is not None and h.value:
             try:
                 lib().pb_kv_cache_release(h)
+                self._h = c_void_p(None)
             except Exception:
                 pass
-            self._h = c_void_p(None)
 
     def device_data(self) -> tuple[int, int, int]:
         """(address of the keys, of the values, bytes of each)."""
@@ -641,9 +645,9 @@ class Batch:
         if h is not None and h.value:
             try:
                 lib().pb_kv_batch_release(h)
+                self._h = c_void_p(None)
             except Exception:
                 pass
-            self._h = c_void_p(None)
 
     def on(self, cache: KVCache) -> "Batch":
         """The same sequences over another layer's cache of the same shape,

@@ -682,6 +682,26 @@ int pb_tensor_from_device(const int64_t* shape, size_t rank, uint64_t pointer, s
     });
 }
 
+int pb_tensor_interface(const pb_tensor* t, int64_t* shape, size_t capacity, size_t* rank, uint64_t* pointer,
+                        void** stream) {
+    return guarded([&] {
+        require(t, "tensor");
+        require(rank, "rank");
+        require(pointer, "pointer");
+        require(stream, "stream");
+        const auto& buffer = t->value.device_data();
+        const auto& st = porch::cuda_jit::buffer_access::state(buffer);
+        auto extents = t->value.shape();
+        *rank = extents.size();
+        for (size_t i = 0; i < extents.size() && i < capacity; ++i) shape[i] = extents[i];
+        *pointer = st ? st->ptr : 0;
+        // Behind the producer, if that is another thread's stream.
+        auto mine = porch::detail::current_stream(st ? st->device : t->value.placement().ordinal());
+        if (st && st->ptr != 0) porch::detail::order_read(*st, mine);
+        *stream = mine->stream;
+    });
+}
+
 namespace {
     porch::detail::norm_rope_args norm_rope_of(const pb_tensor* q, const pb_tensor* k, const pb_tensor* q_weight,
                                                const pb_tensor* k_weight, const pb_tensor* cos,

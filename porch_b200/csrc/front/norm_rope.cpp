@@ -361,8 +361,14 @@ extern "C" __global__ void __launch_bounds__(256) pb_norm_rope_weights(const flo
             return std::string{kernel_prelude()} + "#define " + part + " 1\n" + defines(s) + device_source();
         }
 
+        const char kNormRope[] = "pb_norm_rope";
+        const char kNormRopeGrad[] = "pb_norm_rope_grad";
+        const char kNormRopeWeights[] = "pb_norm_rope_weights";
+
         op_kernel& kernel_of(const shape_key& s, const char* name, const char* part) {
-            return op_kernel_for(std::string{name} + "\n" + defines(s), [&](op_kernel& k) {
+            const op_key key{reinterpret_cast<int64_t>(name), s.dim, s.half, s.q_heads, s.k_heads, s.vec, s.lanes,
+                             s.per, s.interleaved, s.wide};
+            return op_kernel_for(key, [&](op_kernel& k) {
                 k.name = name;
                 k.source = source_of(s, part);
             });
@@ -438,7 +444,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_norm_rope_weights(const flo
         if (c.tokens != 0) {
             shape_key& s = c.key;
             choose_lanes(s, std::min(vector_width(x.q), vector_width(x.k)));
-            op_kernel& kernel = kernel_of(s, "pb_norm_rope", "PB_FORWARD");
+            op_kernel& kernel = kernel_of(s, kNormRope, "PB_FORWARD");
             const int64_t units = c.tokens * ((s.q_heads + s.per - 1) / s.per + (s.k_heads + s.per - 1) / s.per);
             const int64_t blocks = (units + 256 / s.lanes - 1) / (256 / s.lanes);
             expect(blocks <= 0x7fffffff, "qk_norm_rope: too many tokens");
@@ -468,8 +474,8 @@ extern "C" __global__ void __launch_bounds__(256) pb_norm_rope_weights(const flo
         } else {
             shape_key& s = c.key;
             choose_lanes(s, std::min({vector_width(x.q), vector_width(x.k), vector_width(gq), vector_width(gk)}));
-            op_kernel& kernel = kernel_of(s, "pb_norm_rope_grad", "PB_BACKWARD");
-            op_kernel& weights = kernel_of(s, "pb_norm_rope_weights", "PB_BACKWARD");
+            op_kernel& kernel = kernel_of(s, kNormRopeGrad, "PB_BACKWARD");
+            op_kernel& weights = kernel_of(s, kNormRopeWeights, "PB_BACKWARD");
             const int64_t groups = 256 / s.lanes;
             const int64_t units = c.tokens * ((std::max(s.q_heads, s.k_heads) + s.per - 1) / s.per);
             const int64_t blocks = std::min<int64_t>((units + groups - 1) / groups, int64_t{4} * sm_count(device));

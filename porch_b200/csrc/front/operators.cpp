@@ -31,9 +31,19 @@ namespace porch::detail {
         return f;
     }
 
-    op_kernel& op_kernel_for(const std::string& key, const std::function<void(op_kernel&)>& make) {
+    namespace {
+        struct key_hash {
+            size_t operator()(const op_key& k) const {
+                uint64_t h = 0xcbf29ce484222325ULL;
+                for (const int64_t v : k) h = (h ^ static_cast<uint64_t>(v)) * 0x9e3779b97f4a7c15ULL;
+                return h ^ (h >> 32);
+            }
+        };
+    } // namespace
+
+    op_kernel& op_kernel_for(const op_key& key, const std::function<void(op_kernel&)>& make) {
         static std::mutex mutex;
-        static auto* table = new std::unordered_map<std::string, std::unique_ptr<op_kernel>>(); // lives until exit
+        static auto* table = new std::unordered_map<op_key, std::unique_ptr<op_kernel>, key_hash>(); // lives until exit
         std::scoped_lock lock{mutex};
         auto& entry = (*table)[key];
         if (entry == nullptr) {

@@ -32,9 +32,10 @@ namespace porch::detail {
         pbrt_function on(int device);
     };
 
-    // The kernel for `key` (which spells out every constant of the source),
-    // made by `make` the first time.
-    op_kernel& op_kernel_for(const std::string& key, const std::function<void(op_kernel&)>& make);
+    // The kernel for `key` (its name's address and every constant of its
+    // source), made by `make` the first time.
+    using op_key = std::array<int64_t, 12>;
+    op_kernel& op_kernel_for(const op_key& key, const std::function<void(op_kernel&)>& make);
 
     // Launches `k` on `stream`; every kernel here begins with
     // griddepcontrol.wait, so the launch overlaps the previous kernel's tail.

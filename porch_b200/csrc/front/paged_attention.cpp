@@ -626,11 +626,15 @@ extern "C" __global__ void __launch_bounds__(256) pb_paged_scores(
             return os.str();
         }
 
+        const char kAttention[] = "pb_paged_attention";
+        const char kJoin[] = "pb_paged_join";
+        const char kScores[] = "pb_paged_scores";
+
         op_kernel& kernel_of(const char* name, const form& f, uint32_t smem) {
-            const std::string defs = defines(f);
-            return op_kernel_for(std::string{name} + "\n" + defs, [&](op_kernel& k) {
+            const op_key key{reinterpret_cast<int64_t>(name), f.heads, f.dim, f.page, f.bf16, f.scored, f.tiles8};
+            return op_kernel_for(key, [&](op_kernel& k) {
                 k.name = name;
-                k.source = std::string{kernel_prelude()} + defs + device_source();
+                k.source = std::string{kernel_prelude()} + defines(f) + device_source();
                 k.smem = smem;
             });
         }
@@ -753,12 +757,12 @@ extern "C" __global__ void __launch_bounds__(256) pb_paged_scores(
             void* params[] = {&mk,     &mv,    &x.ptr, &batch.lengths_at, &batch.tables_at, &work,
                               &out.ptr, &partial, &ml, &logits, &lse, &width, &group, &chunks,
                               &x.strides[0], &x.strides[1], &longest32, &scale2, &err};
-            op_launch(kernel_of("pb_paged_attention", f, static_cast<uint32_t>(f.smem())), device, stream,
+            op_launch(kernel_of(kAttention, f, static_cast<uint32_t>(f.smem())), device, stream,
                       {static_cast<uint32_t>(plan.ctas), 1, 1}, 160, params);
         }
         if (plan.joins > 0) {
             void* params[] = {&join, &partial, &ml, &out.ptr, &lse, &group, &chunks};
-            op_launch(kernel_of("pb_paged_join", f, 0), device, stream,
+            op_launch(kernel_of(kJoin, f, 0), device, stream,
                       {static_cast<uint32_t>(plan.joins * 8 * f.tiles8), 1, 1}, 128, params);
         }
         std::vector<tensor> results;
@@ -769,7 +773,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_paged_scores(
                 const int64_t blocks = (longest + 255) / 256 * n * c.heads;
                 expect(blocks <= 0x7fffffff, "paged_attention_scored: too many slots");
                 void* params[] = {&logits, &lse, &batch.lengths_at, &xs.ptr, &os.ptr, &longest, &ns, &group};
-                op_launch(kernel_of("pb_paged_scores", f, 0), device, stream, {static_cast<uint32_t>(blocks), 1, 1}, 256,
+                op_launch(kernel_of(kScores, f, 0), device, stream, {static_cast<uint32_t>(blocks), 1, 1}, 256,
                           params);
             }
             results.push_back(finish(std::move(os)));

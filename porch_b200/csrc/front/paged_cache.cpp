@@ -208,23 +208,23 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
 )PB";
         }
 
-        std::string append_defines(int64_t heads, int64_t dim, int64_t page, bool bf16, bool wide) {
+        std::string defines(const kv_cache& c, bool wide) {
             std::ostringstream os;
-            os << "#define PB_H " << heads << "\n#define PB_D " << dim << "\n#define PB_PS " << page
-               << "\n#define PB_BF16 " << (bf16 ? 1 : 0) << "\n#define PB_WIDE " << (wide ? 1 : 0) << "\n";
+            os << "#define PB_H " << c.heads << "\n#define PB_D " << c.dim << "\n#define PB_PS " << c.page_size
+               << "\n#define PB_ROW " << c.dim * c.width() << "\n#define PB_BF16 " << (c.type == cache_type::bf16 ? 1 : 0)
+               << "\n#define PB_WIDE " << (wide ? 1 : 0) << "\n";
             return os.str();
         }
 
-        std::string evict_defines(int64_t heads, int64_t dim, int64_t page, int width) {
-            std::ostringstream os;
-            os << "#define PB_H " << heads << "\n#define PB_PS " << page << "\n#define PB_ROW " << dim * width << "\n";
-            return os.str();
-        }
+        const char kAppend[] = "pb_cache_append";
+        const char kSelect[] = "pb_evict_select";
+        const char kMove[] = "pb_evict_move";
 
-        op_kernel& kernel_of(const char* name, const std::string& defines, const char* source) {
-            return op_kernel_for(std::string{name} + "\n" + defines, [&](op_kernel& k) {
+        op_kernel& kernel_of(const char* name, const kv_cache& c, bool wide = true) {
+            const op_key key{reinterpret_cast<int64_t>(name), c.heads, c.dim, c.page_size, static_cast<int64_t>(c.type), wide};
+            return op_kernel_for(key, [&](op_kernel& k) {
                 k.name = name;
-                k.source = std::string{kernel_prelude()} + defines + source;
+                k.source = std::string{kernel_prelude()} + defines(c, wide) + (name == kAppend ? append_source() : evict_source());
             });
         }
 
@@ -350,9 +350,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
         auto stream = current_stream(device);
         op_operand xk = operand(k, stream, true), xv = operand(v, stream, true);
         const bool wide = std::min(vector_width(xk), vector_width(xv)) == 4;
-        op_kernel& kernel = kernel_of("pb_cache_append",
-                                      append_defines(c.heads, c.dim, c.page_size, c.type == cache_type::bf16, wide),
-                                      append_source());
+        op_kernel& kernel = kernel_of(kAppend, c, wide);
         order_read(*cuda_jit::buffer_access::state(batch.data), stream);
         order_write(*cuda_jit::buffer_access::state(c.k), stream);
         order_write(*cuda_jit::buffer_access::state(c.v), stream);
@@ -388,9 +386,8 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
         if (positions != nullptr) xp = operand(*positions, stream, false);
         const std::vector<index_t> out{n, c.heads, budget};
         op_result os = new_result(out, device, stream), op = new_result(out, device, stream);
-        const std::string defines = evict_defines(c.heads, c.dim, c.page_size, c.width());
-        op_kernel& select = kernel_of("pb_evict_select", defines, evict_source());
-        op_kernel& move = kernel_of("pb_evict_move", defines, evict_source());
+        op_kernel& select = kernel_of(kSelect, c);
+        op_kernel& move = kernel_of(kMove, c);
         int64_t rows = n * c.heads;
         auto scratch = allocate(device, static_cast<size_t>(rows * budget) * 2 * sizeof(int32_t), stream);
         uint64_t from = address(scratch), holes = from + static_cast<uint64_t>(rows * budget) * sizeof(int32_t);
@@ -414,10 +411,16 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
     }
 
     void paged_cache_sources(kernel_list& out) {
-        const std::string p = kernel_prelude();
-        out.emplace_back("pb_cache_append_bf16", p + append_defines(8, 128, 64, true, true) + append_source());
-        out.emplace_back("pb_cache_append_f32", p + append_defines(5, 80, 8, false, false) + append_source());
-        out.emplace_back("pb_evict", p + evict_defines(8, 128, 64, 2) + evict_source());
+        kv_cache c;
+        c.heads = 5;
+        c.dim = 80;
+        c.page_size = 8;
+        for (const auto type : {cache_type::f32, cache_type::bf16}) {
+            c.type = type;
+            const std::string tag = type == cache_type::bf16 ? "_bf16" : "_f32", p = kernel_prelude();
+            out.emplace_back("pb_cache_append" + tag, p + defines(c, type == cache_type::bf16) + append_source());
+            out.emplace_back("pb_evict" + tag, p + defines(c, true) + evict_source());
+        }
     }
 
 } // namespace porch::detail
