@@ -56,10 +56,10 @@ namespace porch::detail {
     }
 
     void op_launch(op_kernel& k, int device, const std::shared_ptr<stream_ref>& stream,
-                   std::array<uint32_t, 3> grid, uint32_t threads, void** params) {
-        const uint32_t block[3] = {threads, 1, 1};
-        check(pbrt_launch_ex(device, k.on(device), grid.data(), block, k.smem, stream->stream, params, nullptr,
-                             PBRT_LAUNCH_PDL));
+                   std::array<uint32_t, 3> grid, uint32_t threads, void** params, uint32_t cluster, uint32_t smem) {
+        const uint32_t block[3] = {threads, 1, 1}, clusters[3] = {cluster, 1, 1};
+        check(pbrt_launch_ex(device, k.on(device), grid.data(), block, smem != 0 ? smem : k.smem, stream->stream, params,
+                             cluster > 1 ? clusters : nullptr, PBRT_LAUNCH_PDL));
     }
 
     int sm_count(int device) {

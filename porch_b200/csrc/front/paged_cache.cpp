@@ -116,17 +116,9 @@ static __device__ __forceinline__ int pb_block_rank(bool flag, int* warps, int& 
     return before + __popc(votes & ((1u << lane) - 1u));
 }
 
-// One block per sequence and key head: a radix select of the budget-th
-// largest key (4 passes of 8 bits), then one pass in slot order that lists
-// the free places below the budget and the kept slots past it.
-extern "C" __global__ void __launch_bounds__(1024) pb_evict_select(
-    const float* scores, const float* places, const int* lengths, const int* newest, float* out_scores,
-    float* out_places, int* from, int* holes, pb_i64 ns, pb_i64 np, int budget, int recent, int sinks) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    __shared__ int hist[256];
-    __shared__ int warps[32];
-    __shared__ int chosen[2]; // digit, keys of it still wanted
-    const pb_i64 row = blockIdx.x;
+static __device__ __forceinline__ pb_row pb_row_of(const float* scores, const float* places, const int* lengths,
+                                                   const int* newest, pb_i64 ns, pb_i64 np, int recent, int sinks,
+                                                   pb_i64 row) {
     const int s = (int)(row / PB_H);
     pb_row r;
     r.scores = scores + row * ns;
@@ -137,95 +129,370 @@ extern "C" __global__ void __launch_bounds__(1024) pb_evict_select(
     r.newest = (float)newest[s];
     r.recent_from = r.newest - (float)recent;
     r.sinks = (float)sinks;
-    int* map = from + row * budget;
-    int* hole = holes + row * budget;
-    for (int i = threadIdx.x; i < budget; i += 1024) map[i] = i;
+    return r;
+}
+static __device__ __forceinline__ void pb_keep(const pb_row& r, float* out_scores, float* out_places, pb_i64 to, int i) {
+    out_scores[to] = pb_score(r, i);
+    out_places[to] = pb_place(r, i);
+}
+
+// Exclusive sums of two counts over the block's threads, and their totals.
+static __device__ __forceinline__ int2 pb_block_scan(int2 v, int2* warps, int2& total) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, n = blockDim.x >> 5;
+    int2 x = v;
+#pragma unroll
+    for (int m = 1; m < 32; m *= 2) {
+        const int a = __shfl_up_sync(0xffffffffu, x.x, m), b = __shfl_up_sync(0xffffffffu, x.y, m);
+        if (lane >= m) { x.x += a; x.y += b; }
+    }
+    __syncthreads();
+    if (lane == 31) warps[w] = x;
+    __syncthreads();
+    int2 before = make_int2(0, 0);
+    total = before;
+    int2 mine = lane < n ? warps[lane] : make_int2(0, 0);
+    int2 sum = mine;
+#pragma unroll
+    for (int m = 1; m < 32; m *= 2) {
+        const int a = __shfl_up_sync(0xffffffffu, sum.x, m), b = __shfl_up_sync(0xffffffffu, sum.y, m);
+        if (lane >= m) { sum.x += a; sum.y += b; }
+    }
+    total.x = __shfl_sync(0xffffffffu, sum.x, 31);
+    total.y = __shfl_sync(0xffffffffu, sum.y, 31);
+    before.x = __shfl_sync(0xffffffffu, sum.x - mine.x, w);
+    before.y = __shfl_sync(0xffffffffu, sum.y - mine.y, w);
+    return make_int2(before.x + x.x - v.x, before.y + x.y - v.y);
+}
+
+// The digit of the `want`-th largest key among 256 counted bins, how many
+// keys of its bin are wanted, and whether that is all of them. One warp.
+static __device__ __forceinline__ void pb_pick(const int* bins, int want, int* chosen) {
+    const int lane = threadIdx.x & 31;
+    int own[8], sum = 0; // bins 255 - 8 lane, downwards
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum += own[j] = bins[255 - 8 * lane - j];
+    int upto = sum;
+#pragma unroll
+    for (int m = 1; m < 32; m *= 2) {
+        const int a = __shfl_up_sync(0xffffffffu, upto, m);
+        if (lane >= m) upto += a;
+    }
+    int left = want - (upto - sum);
+    if (left > 0 && left <= sum) {
+        int j = 0;
+        while (own[j] < left) left -= own[j++];
+        chosen[0] = 255 - 8 * lane - j;
+        chosen[1] = left;
+        chosen[2] = own[j] == left;
+    }
+}
+
+#ifdef PB_CLUSTER
+static __device__ __forceinline__ pb_u32 pb_rank() {
+    pb_u32 r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+static __device__ __forceinline__ void pb_cluster_sync() {
+#if PB_CLUSTER > 1
+    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+#else
+    __syncthreads();
+#endif
+}
+// An int of CTA `rank` of the cluster.
+static __device__ __forceinline__ int pb_peer(const int* p, pb_u32 rank) {
+    int v;
+    pb_u32 a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((pb_u32)__cvta_generic_to_shared(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+
+// One cluster per sequence and key head. Each CTA holds the keys of a run of
+// slots in shared memory (its threads own consecutive ones, an odd stride
+// apart, so that they read distinct banks), and the row is read once:
+//  1. radix select of the budget-th largest key, 8 bits a pass, the counts
+//     summed over the cluster through distributed shared memory; it ends as
+//     soon as a bin is wanted whole;
+//  2. exclusive sums over the slots' order rank ties, free places and late
+//     slots. The j-th late slot goes to the j-th free place.
+// What bounds it: the latency of the passes (two barriers each), not bytes.
+extern "C" __global__ void __launch_bounds__(1024) pb_evict_select(
+    const float* scores, const float* places, const int* lengths, const int* newest, float* out_scores,
+    float* out_places, int* holes, int* lates, int* counts, pb_i64 ns, pb_i64 np, int budget, int recent, int sinks,
+    int pairs, int per_thread) {
+    extern __shared__ pb_u32 keys[];
+    __shared__ int hist[2][256], bins[256], chosen[3], totals[3];
+    __shared__ int2 warps[32];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const pb_i64 row = blockIdx.x / PB_CLUSTER;
+    const pb_u32 rank = PB_CLUSTER > 1 ? pb_rank() : 0;
+    const pb_row r = pb_row_of(scores, places, lengths, newest, ns, np, recent, sinks, row);
+    const int threads = blockDim.x, run = threads * per_thread, first = rank * run;
+    for (int i = first + threadIdx.x; i < min(first + run, budget); i += threads)
+        if (i >= r.length) { // nothing is kept there
+            out_scores[row * budget + i] = 0.0f;
+            out_places[row * budget + i] = -1.0f;
+        }
+    // The budget may reach past the slots that the cluster covers.
+    for (int i = PB_CLUSTER * run + rank * threads + threadIdx.x; i < budget; i += PB_CLUSTER * threads) {
+        out_scores[row * budget + i] = 0.0f;
+        out_places[row * budget + i] = -1.0f;
+    }
+    if (r.length <= budget) { // the same in every CTA of the cluster
+        for (int i = first + threadIdx.x; i < min(first + run, r.length); i += threads)
+            pb_keep(r, out_scores, out_places, row * budget + i, i);
+        if (rank == 0 && threadIdx.x == 0) counts[row] = 0;
+        return;
+    }
+    const int stride = per_thread | 1, n = min(run, r.length - first); // n may be negative
+    for (int i = threadIdx.x; i < n; i += threads) keys[i / per_thread * stride + i % per_thread] = pb_key(r, first + i);
+    const pb_u32* own = keys + threadIdx.x * stride;
+    const int mine = max(0, min(per_thread, n - (int)threadIdx.x * per_thread));
+
+    pb_u32 limit = 0; // the bits of the threshold so far
+    int want = budget;
+    bool whole = false;
+    for (int i = threadIdx.x; i < 256; i += threads) hist[0][i] = 0;
+    __syncthreads();
+    for (int pass = 0; pass < 4 && !whole; ++pass) {
+        const int shift = 24 - 8 * pass;
+        int* h = hist[pass & 1];
+        for (int j = 0; j < mine; ++j) {
+            const pb_u32 key = own[j];
+            if (pass == 0 || ((key ^ limit) >> (shift + 8)) == 0) atomicAdd(&h[(key >> shift) & 255u], 1);
+        }
+        pb_cluster_sync();
+        for (int i = threadIdx.x; i < 256; i += threads) {
+            int sum = 0;
+#pragma unroll
+            for (int c = 0; c < PB_CLUSTER; ++c) sum += PB_CLUSTER > 1 ? pb_peer(h + i, c) : h[i];
+            bins[i] = sum;
+            hist[(pass & 1) ^ 1][i] = 0; // every CTA has read it: it was before this barrier
+        }
+        __syncthreads();
+        if (threadIdx.x < 32) pb_pick(bins, want, chosen);
+        __syncthreads();
+        limit |= (pb_u32)chosen[0] << shift;
+        want = chosen[1];
+        whole = chosen[2];
+    }
+    // Kept: keys above the limit, and of those equal to it the first `want`
+    // (all of them where a bin was wanted whole: then the limit's low bits are 0).
+    int2 total;
+    int ties = 0;
+    if (!whole) {
+        int count = 0;
+        for (int j = 0; j < mine; ++j) count += own[j] == limit;
+        ties = pb_block_scan(make_int2(count, 0), warps, total).x;
+        if (threadIdx.x == 0) totals[0] = total.x;
+        pb_cluster_sync();
+        if (PB_CLUSTER > 1)
+            for (pb_u32 c = 0; c < rank; ++c) ties += pb_peer(totals, c);
+    }
+    pb_u64 kept = 0; // up to 64 slots a thread
+    int2 count = make_int2(0, 0); // free places, late slots
+    int seen = ties;
+    const int slot0 = first + threadIdx.x * per_thread;
+    for (int j = 0; j < mine; ++j) {
+        const pb_u32 key = own[j];
+        const bool keep = whole ? key >= limit : key > limit || (key == limit && seen++ < want);
+        kept |= (pb_u64)keep << j;
+        const bool low = slot0 + j < budget;
+        count.x += low && !keep;
+        count.y += !low && keep;
+    }
+    int2 at = pb_block_scan(count, warps, total);
+    if (PB_CLUSTER > 1) {
+        if (threadIdx.x == 0) { totals[1] = total.x; totals[2] = total.y; }
+        pb_cluster_sync();
+        for (pb_u32 c = 0; c < rank; ++c) {
+            at.x += pb_peer(totals + 1, c);
+            at.y += pb_peer(totals + 2, c);
+        }
+    }
+    for (int j = 0; j < mine; ++j) {
+        const int i = slot0 + j;
+        const bool keep = kept >> j & 1u;
+        if (i < budget) {
+            if (keep) pb_keep(r, out_scores, out_places, row * budget + i, i);
+            else holes[row * pairs + at.x++] = i;
+        } else if (keep) {
+            lates[row * pairs + at.y++] = i;
+        }
+    }
+    if (PB_CLUSTER > 1) {
+        if (rank == PB_CLUSTER - 1 && threadIdx.x == threads - 1) counts[row] = at.y;
+        pb_cluster_sync(); // nobody leaves while its shared memory is read
+    } else if (threadIdx.x == threads - 1) {
+        counts[row] = at.y;
+    }
+}
+#endif
+
+#ifndef PB_CLUSTER
+// Rank of this thread's flag among the block's 1024, and their number.
+static __device__ __forceinline__ int pb_block_rank(bool flag, int2* warps, int& total) {
+    int2 sum;
+    const int2 r = pb_block_scan(make_int2(flag, 0), warps, sum);
+    total = sum.x;
+    return r.x;
+}
+
+// The same for rows too long for a cluster's shared memory: one block per
+// row, which reads the row again in every pass.
+extern "C" __global__ void __launch_bounds__(1024) pb_evict_select_long(
+    const float* scores, const float* places, const int* lengths, const int* newest, float* out_scores,
+    float* out_places, int* holes, int* lates, int* counts, pb_i64 ns, pb_i64 np, int budget, int recent, int sinks,
+    int pairs, int per_thread) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    __shared__ int hist[256], chosen[3];
+    __shared__ int2 warps[32];
+    const pb_i64 row = blockIdx.x;
+    const pb_row r = pb_row_of(scores, places, lengths, newest, ns, np, recent, sinks, row);
+    pb_u32 limit = 0;
+    int want = budget;
     if (r.length > budget) {
-        pb_u32 prefix = 0;
-        int want = budget;
         for (int shift = 24; shift >= 0; shift -= 8) {
             if (threadIdx.x < 256) hist[threadIdx.x] = 0;
             __syncthreads();
             for (int i = threadIdx.x; i < r.length; i += 1024) {
                 const pb_u32 key = pb_key(r, i);
-                if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255u], 1);
+                if (shift == 24 || ((key ^ limit) >> (shift + 8)) == 0) atomicAdd(&hist[(key >> shift) & 255u], 1);
             }
             __syncthreads();
-            if (threadIdx.x == 0) {
-                int d = 255, left = want;
-                while (hist[d] < left) left -= hist[d--];
-                chosen[0] = d;
-                chosen[1] = left;
-            }
+            if (threadIdx.x < 32) pb_pick(hist, want, chosen);
             __syncthreads();
-            prefix |= (pb_u32)chosen[0] << shift;
+            limit |= (pb_u32)chosen[0] << shift;
             want = chosen[1];
             __syncthreads();
         }
-        int ties = 0, nholes = 0, nlate = 0, total = 0;
-        for (int base = 0; base < r.length; base += 1024) {
-            const int i = base + threadIdx.x;
-            const pb_u32 key = i < r.length ? pb_key(r, i) : 0u;
-            const bool tie = i < r.length && key == prefix;
-            const int rank = ties + pb_block_rank(tie, warps, total);
-            ties += total;
-            const bool kept = i < r.length && (key > prefix || (tie && rank < want));
-            const int h = nholes + pb_block_rank(i < budget && !kept, warps, total);
-            nholes += total;
-            if (i < budget && !kept) hole[h] = i;
-            __syncthreads(); // the list of places is complete below `base + 1024`
-            const int l = nlate + pb_block_rank(i >= budget && kept, warps, total);
-            nlate += total;
-            if (i >= budget && kept) map[hole[l]] = i;
+    }
+    int ties = 0, nholes = 0, nlate = 0, total = 0;
+    for (pb_i64 base = 0; base < max(r.length, budget); base += 1024) {
+        const int i = (int)(base + threadIdx.x); // lengths and budgets are at most 2^30
+        const bool live = i < r.length, all = r.length <= budget;
+        const pb_u32 key = live && !all ? pb_key(r, i) : 0u;
+        const bool tie = live && !all && key == limit;
+        const int place = ties + pb_block_rank(tie, warps, total);
+        ties += total;
+        const bool kept = live && (all || key > limit || (tie && place < want));
+        const bool hole = live && i < budget && !kept;
+        const int h = nholes + pb_block_rank(hole, warps, total);
+        nholes += total;
+        const int l = nlate + pb_block_rank(i >= budget && kept, warps, total);
+        nlate += total;
+        if (hole) holes[row * pairs + h] = i;
+        if (i >= budget && kept) lates[row * pairs + l] = i;
+        if (i < budget && kept) pb_keep(r, out_scores, out_places, row * budget + i, i);
+        if (i < budget && !live) {
+            out_scores[row * budget + i] = 0.0f;
+            out_places[row * budget + i] = -1.0f;
         }
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < budget; i += 1024) {
-        const bool live = i < r.length;
-        out_scores[row * budget + i] = live ? pb_score(r, map[i]) : 0.0f;
-        out_places[row * budget + i] = live ? pb_place(r, map[i]) : -1.0f;
-    }
+    if (threadIdx.x == 0) counts[row] = nlate;
 }
 
-// Warps copy the rows that moved, keys and values.
+// Moves the late rows, keys and values, with their scores and positions. A
+// warp takes PB_MOVES pairs, all loads before the first store, so that it has
+// as many bytes on the way as a row's size allows. Sources lie at or past the
+// budget, destinations below it.
 extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
-    char* pk, char* pv, const int* tables, const int* lengths, const int* from, pb_i64 rows, int width, int budget) {
+    char* pk, char* pv, const int* tables, const float* scores, const float* places, const int* lengths,
+    const int* newest, float* out_scores, float* out_places, const int* holes, const int* lates, const int* counts,
+    pb_i64 ns, pb_i64 np, pb_i64 rows, int width, int budget, int pairs) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const pb_i64 id = ((pb_i64)blockIdx.x * 256 + threadIdx.x) / 32;
-    const int lane = threadIdx.x & 31;
-    if (id >= rows * budget) return;
-    const pb_i64 row = id / budget;
-    const int i = (int)(id - row * budget), src = from[id], s = (int)(row / PB_H), h = (int)(row % PB_H);
-    if (src == i || i >= lengths[s]) return;
-    const pb_i64 table = (pb_i64)s * width;
-    const pb_i64 a = (((pb_i64)tables[table + src / PB_PS] * PB_H + h) * PB_PS + src % PB_PS) * PB_ROW;
-    const pb_i64 b = (((pb_i64)tables[table + i / PB_PS] * PB_H + h) * PB_PS + i % PB_PS) * PB_ROW;
-    for (int c = lane * 16; c < PB_ROW; c += 512) {
-        *reinterpret_cast<uint4*>(pk + b + c) = *reinterpret_cast<const uint4*>(pk + a + c);
-        *reinterpret_cast<uint4*>(pv + b + c) = *reinterpret_cast<const uint4*>(pv + a + c);
+    const int groups = (pairs + PB_MOVES - 1) / PB_MOVES, lane = threadIdx.x & 31;
+    const pb_i64 id = ((pb_i64)blockIdx.x * 256 + threadIdx.x) / 32, row = id / groups;
+    if (row >= rows) return;
+    const int j0 = (int)(id - row * groups) * PB_MOVES, count = counts[row];
+    if (j0 >= count) return;
+    const int s = (int)(row / PB_H), h = (int)(row % PB_H);
+    const int* table = tables + (pb_i64)s * width;
+    int from = 0, to = 0;
+    if (lane < PB_MOVES && j0 + lane < count) {
+        from = lates[row * pairs + j0 + lane];
+        to = holes[row * pairs + j0 + lane];
+        const pb_row r = pb_row_of(scores, places, lengths, newest, ns, np, 0, 0, row);
+        pb_keep(r, out_scores, out_places, row * budget + to, from);
     }
+    // 16 bytes a lane: chunk c of the 2 * PB_ROW bytes of a slot, keys first.
+    uint4 v[PB_MOVES][PB_CHUNKS];
+    pb_i64 to_row[PB_MOVES];
+#pragma unroll
+    for (int m = 0; m < PB_MOVES; ++m) {
+        const int f = __shfl_sync(0xffffffffu, from, m), t = __shfl_sync(0xffffffffu, to, m);
+        const pb_i64 a = (((pb_i64)table[f / PB_PS] * PB_H + h) * PB_PS + f % PB_PS) * PB_ROW;
+        to_row[m] = (((pb_i64)table[t / PB_PS] * PB_H + h) * PB_PS + t % PB_PS) * PB_ROW;
+#pragma unroll
+        for (int c = 0; c < PB_CHUNKS; ++c) {
+            const int at = (c * 32 + lane) * 16;
+            if (j0 + m < count && at < 2 * PB_ROW)
+                v[m][c] = *reinterpret_cast<const uint4*>(at < PB_ROW ? pk + a + at : pv + a + at - PB_ROW);
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < PB_MOVES; ++m)
+#pragma unroll
+        for (int c = 0; c < PB_CHUNKS; ++c) {
+            const int at = (c * 32 + lane) * 16;
+            const pb_i64 b = to_row[m];
+            if (j0 + m < count && at < 2 * PB_ROW)
+                *reinterpret_cast<uint4*>(at < PB_ROW ? pk + b + at : pv + b + at - PB_ROW) = v[m][c];
+        }
 }
+#endif
 )PB";
         }
 
-        std::string defines(const kv_cache& c, bool wide) {
+        int moves_of(const kv_cache& c) { return 2 * c.dim * c.width() <= 512 ? 4 : 2; } // pairs a warp moves
+
+        std::string defines(const kv_cache& c, bool wide, int cluster = 0) {
             std::ostringstream os;
             os << "#define PB_H " << c.heads << "\n#define PB_D " << c.dim << "\n#define PB_PS " << c.page_size
                << "\n#define PB_ROW " << c.dim * c.width() << "\n#define PB_BF16 " << (c.type == cache_type::bf16 ? 1 : 0)
-               << "\n#define PB_WIDE " << (wide ? 1 : 0) << "\n";
+               << "\n#define PB_WIDE " << (wide ? 1 : 0) << "\n#define PB_MOVES " << moves_of(c)
+               << "\n#define PB_CHUNKS " << (2 * c.dim * c.width() + 511) / 512 << "\n";
+            if (cluster != 0) os << "#define PB_CLUSTER " << cluster << "\n";
             return os.str();
         }
 
         const char kAppend[] = "pb_cache_append";
         const char kSelect[] = "pb_evict_select";
+        const char kSelectLong[] = "pb_evict_select_long";
         const char kMove[] = "pb_evict_move";
 
-        op_kernel& kernel_of(const char* name, const kv_cache& c, bool wide = true) {
-            const op_key key{reinterpret_cast<int64_t>(name), c.heads, c.dim, c.page_size, static_cast<int64_t>(c.type), wide};
+        op_kernel& kernel_of(const char* name, const kv_cache& c, bool wide = true, int cluster = 0, uint32_t smem = 0) {
+            const op_key key{reinterpret_cast<int64_t>(name), c.heads, c.dim, c.page_size, static_cast<int64_t>(c.type), wide, cluster};
             return op_kernel_for(key, [&](op_kernel& k) {
                 k.name = name;
-                k.source = std::string{kernel_prelude()} + defines(c, wide) + (name == kAppend ? append_source() : evict_source());
+                k.source = std::string{kernel_prelude()} + defines(c, wide, cluster) +
+                           (name == kAppend ? append_source() : evict_source());
+                k.smem = smem;
             });
+        }
+
+        // How the select shares out a row of `longest` slots.
+        struct select_shape {
+            int cluster = 0, threads = 0, per_thread = 0; // cluster 0: the long form
+        };
+        constexpr int kSelectSmem = 200 * 1024; // keys of a CTA, 4 bytes each
+        select_shape shape_for(int64_t longest, int64_t rows, int sms) {
+            select_shape r;
+            // A cluster for each row as long as all CTAs fit the GPU twice
+            // and each has a few thousand slots; larger where the keys need it.
+            int64_t c = 1;
+            while (c < 8 && rows * c * 2 <= 2 * sms && longest >= 4096 * c) c *= 2;
+            auto fits = [&](int64_t n) {
+                const int64_t run = (longest + n - 1) / n;
+                r.threads = run <= 2048 ? 256 : 1024;
+                r.per_thread = static_cast<int>((run + r.threads - 1) / r.threads);
+                return r.per_thread <= 64 && int64_t{r.threads} * (r.per_thread | 1) * 4 <= kSelectSmem;
+            };
+            while (c <= 8 && !fits(c)) c *= 2;
+            if (c <= 8) r.cluster = static_cast<int>(c);
+            return r;
         }
 
     } // namespace
@@ -386,26 +653,38 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
         if (positions != nullptr) xp = operand(*positions, stream, false);
         const std::vector<index_t> out{n, c.heads, budget};
         op_result os = new_result(out, device, stream), op = new_result(out, device, stream);
-        op_kernel& select = kernel_of(kSelect, c);
-        op_kernel& move = kernel_of(kMove, c);
         int64_t rows = n * c.heads;
-        auto scratch = allocate(device, static_cast<size_t>(rows * budget) * 2 * sizeof(int32_t), stream);
-        uint64_t from = address(scratch), holes = from + static_cast<uint64_t>(rows * budget) * sizeof(int32_t);
+        // No row has more late slots than it has places, or slots past the budget.
+        int pairs = static_cast<int>(std::max<int64_t>(1, std::min(budget, batch.longest - budget)));
+        const size_t list = static_cast<size_t>(rows) * static_cast<size_t>(pairs);
+        auto scratch = allocate(device, (2 * list + static_cast<size_t>(rows)) * sizeof(int32_t), stream);
+        uint64_t holes = address(scratch), lates = holes + list * 4, counts = lates + list * 4;
         order_read(*cuda_jit::buffer_access::state(batch.data), stream);
-        order_write(*cuda_jit::buffer_access::state(c.k), stream);
-        order_write(*cuda_jit::buffer_access::state(c.v), stream);
-        uint64_t pk = address(c.k), pv = address(c.v);
         int b = static_cast<int>(budget), rc = static_cast<int>(recent), sk = static_cast<int>(sinks);
         int width = static_cast<int>(batch.table_width);
         int64_t nsv = ns, npv = np;
-        void* sparams[] = {&xs.ptr, &xp.ptr, &batch.lengths_at, &batch.newest_at, &os.ptr, &op.ptr, &from,
-                           &holes,  &nsv,    &npv,              &b,               &rc,     &sk};
-        op_launch(select, device, stream, {static_cast<uint32_t>(rows), 1, 1}, 1024, sparams);
+        select_shape f = shape_for(batch.longest, rows, sm_count(device));
+        void* sparams[] = {&xs.ptr, &xp.ptr, &batch.lengths_at, &batch.newest_at, &os.ptr, &op.ptr, &holes, &lates,
+                           &counts, &nsv,    &npv,              &b,               &rc,     &sk,     &pairs, &f.per_thread};
+        if (f.cluster != 0) {
+            const uint32_t smem = static_cast<uint32_t>(f.threads * (f.per_thread | 1) * 4);
+            op_launch(kernel_of(kSelect, c, true, f.cluster, kSelectSmem), device, stream,
+                      {static_cast<uint32_t>(rows * f.cluster), 1, 1}, static_cast<uint32_t>(f.threads), sparams,
+                      static_cast<uint32_t>(f.cluster), smem);
+        } else {
+            op_launch(kernel_of(kSelectLong, c), device, stream, {static_cast<uint32_t>(rows), 1, 1}, 1024, sparams);
+        }
         if (batch.longest > budget) {
-            const int64_t blocks = (rows * budget + 7) / 8;
+            order_write(*cuda_jit::buffer_access::state(c.k), stream);
+            order_write(*cuda_jit::buffer_access::state(c.v), stream);
+            uint64_t pk = address(c.k), pv = address(c.v);
+            const int64_t groups = (pairs + moves_of(c) - 1) / moves_of(c);
+            const int64_t blocks = (rows * groups + 7) / 8;
             expect(blocks <= 0x7fffffff, "cache_evict: too many rows");
-            void* mparams[] = {&pk, &pv, &batch.tables_at, &batch.lengths_at, &from, &rows, &width, &b};
-            op_launch(move, device, stream, {static_cast<uint32_t>(blocks), 1, 1}, 256, mparams);
+            void* mparams[] = {&pk,     &pv,    &batch.tables_at, &xs.ptr, &xp.ptr, &batch.lengths_at, &batch.newest_at,
+                               &os.ptr, &op.ptr, &holes,          &lates,  &counts, &nsv,              &npv,
+                               &rows,   &width, &b,               &pairs};
+            op_launch(kernel_of(kMove, c), device, stream, {static_cast<uint32_t>(blocks), 1, 1}, 256, mparams);
         }
         return {finish(std::move(os)), finish(std::move(op))};
     }
@@ -420,6 +699,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
             const std::string tag = type == cache_type::bf16 ? "_bf16" : "_f32", p = kernel_prelude();
             out.emplace_back("pb_cache_append" + tag, p + defines(c, type == cache_type::bf16) + append_source());
             out.emplace_back("pb_evict" + tag, p + defines(c, true) + evict_source());
+            out.emplace_back("pb_evict_select" + tag, p + defines(c, true, type == cache_type::bf16 ? 8 : 1) + evict_source());
         }
     }
 

@@ -36,6 +36,11 @@ CASES = [
     ([70001, 20], 1, 16, 128, "bf16", 4097, 1024, 4),
     ([200000], 1, 8, 256, "bf16", 100000, 1000, 4),
     ([300, 250], 1, 40, 8, "f32", 280, 20, 260),
+    ([9000] * 3 + [8, 8999], 8, 16, 64, "bf16", 700, 64, 4),
+    ([33000, 32999, 5], 2, 16, 64, "bf16", 20000, 64, 4),
+    ([420000, 1500], 1, 8, 256, "bf16", 3000, 500, 4),
+    ([420000, 1500], 1, 8, 256, "f32", 419000, 500, 4),
+    ([30, 20], 2, 8, 8, "f32", 5000, 500, 4),
 ]
 
 
