@@ -56,9 +56,9 @@ namespace porch::detail {
     }
 
     void op_launch(op_kernel& k, int device, const std::shared_ptr<stream_ref>& stream,
-                   std::array<uint32_t, 3> grid, uint32_t threads, void** params, uint32_t cluster, uint32_t smem) {
+                   std::array<uint32_t, 3> grid, uint32_t threads, void** params, uint32_t cluster) {
         const uint32_t block[3] = {threads, 1, 1}, clusters[3] = {cluster, 1, 1};
-        check(pbrt_launch_ex(device, k.on(device), grid.data(), block, smem != 0 ? smem : k.smem, stream->stream, params,
+        check(pbrt_launch_ex(device, k.on(device), grid.data(), block, k.smem, stream->stream, params,
                              cluster > 1 ? clusters : nullptr, PBRT_LAUNCH_PDL));
     }
 

@@ -39,10 +39,8 @@ namespace porch::detail {
 
     // Launches `k` on `stream`; every kernel here begins with
     // griddepcontrol.wait, so the launch overlaps the previous kernel's tail.
-    // `smem`: less dynamic shared memory than the kernel may have (0: all of it).
     void op_launch(op_kernel& k, int device, const std::shared_ptr<stream_ref>& stream,
-                   std::array<uint32_t, 3> grid, uint32_t threads, void** params, uint32_t cluster = 1,
-                   uint32_t smem = 0);
+                   std::array<uint32_t, 3> grid, uint32_t threads, void** params, uint32_t cluster = 1);
 
     int sm_count(int device);
 

@@ -95,25 +95,12 @@ static __device__ __forceinline__ float pb_place(const pb_row& r, int i) {
     return r.newest - (float)(r.length - 1 - i);
 }
 static __device__ __forceinline__ float pb_score(const pb_row& r, int i) { return i < r.ns ? r.scores[i] : 0.0f; }
-static __device__ __forceinline__ pb_u32 pb_key(const pb_row& r, int i) {
-    const float p = pb_place(r, i);
-    return p > r.recent_from || p < r.sinks ? 0xffffffffu : pb_order(pb_score(r, i));
+static __device__ __forceinline__ pb_u32 pb_key_of(const pb_row& r, int i, float score, float place) {
+    const float p = place >= 0.0f ? place : r.newest - (float)(r.length - 1 - i); // NaN is no place
+    return p > r.recent_from || p < r.sinks ? 0xffffffffu : pb_order(score);
 }
-
-// Rank of this thread's flag among the block's 1024, and their number.
-static __device__ __forceinline__ int pb_block_rank(bool flag, int* warps, int& total) {
-    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const pb_u32 votes = __ballot_sync(0xffffffffu, flag);
-    __syncthreads();
-    if (lane == 0) warps[w] = __popc(votes);
-    __syncthreads();
-    int before = 0;
-    total = 0;
-    for (int i = 0; i < 32; ++i) {
-        if (i < w) before += warps[i];
-        total += warps[i];
-    }
-    return before + __popc(votes & ((1u << lane) - 1u));
+static __device__ __forceinline__ pb_u32 pb_key(const pb_row& r, int i) {
+    return pb_key_of(r, i, pb_score(r, i), i < r.np ? r.places[i] : -1.0f);
 }
 
 static __device__ __forceinline__ pb_row pb_row_of(const float* scores, const float* places, const int* lengths,
@@ -187,6 +174,58 @@ static __device__ __forceinline__ void pb_pick(const int* bins, int want, int* c
     }
 }
 
+// Up to PB_MOVES pairs of one row: late slot and free place, one a lane.
+struct pb_pairs { int from, to, count; };
+static __device__ __forceinline__ pb_pairs pb_list(const int* holes, const int* lates, const int* counts, pb_i64 id,
+                                                   pb_i64 last, int groups, int pairs) {
+    pb_pairs p = {0, 0, 0};
+    if (id >= last) return p;
+    const int lane = threadIdx.x & 31;
+    const pb_i64 row = id / groups;
+    const int j = (int)(id - row * groups) * PB_MOVES;
+    if (lane < PB_MOVES && j + lane < pairs) { // read beside the count; what lies past it is not used
+        p.from = lates[row * pairs + j + lane];
+        p.to = holes[row * pairs + j + lane];
+    }
+    p.count = min(PB_MOVES, counts[row] - j);
+    if (lane >= p.count) p.from = p.to = 0;
+    return p;
+}
+
+// Moves the pairs' rows, keys and values, with their scores and positions: one
+// warp, all loads before the first store, so that it has as many bytes on the
+// way as PB_MOVES rows. Sources lie at or past the budget, destinations below.
+static __device__ __forceinline__ void pb_move(const pb_pairs& p, const pb_row& r, char* pk, char* pv, const int* tables,
+                                               float* out_scores, float* out_places, pb_i64 row, int width, int budget) {
+    const int lane = threadIdx.x & 31, h = (int)(row % PB_H);
+    const int* table = tables + row / PB_H * width;
+    // 16 bytes a lane: chunk c of the 2 * PB_ROW bytes of a slot, keys first.
+    uint4 v[PB_MOVES][PB_CHUNKS];
+    pb_i64 to_row[PB_MOVES];
+#pragma unroll
+    for (int m = 0; m < PB_MOVES; ++m) {
+        const int f = __shfl_sync(0xffffffffu, p.from, m), t = __shfl_sync(0xffffffffu, p.to, m);
+        const pb_i64 a = (((pb_i64)__ldg(table + f / PB_PS) * PB_H + h) * PB_PS + f % PB_PS) * PB_ROW;
+        to_row[m] = (((pb_i64)__ldg(table + t / PB_PS) * PB_H + h) * PB_PS + t % PB_PS) * PB_ROW;
+#pragma unroll
+        for (int c = 0; c < PB_CHUNKS; ++c) {
+            const int at = (c * 32 + lane) * 16;
+            if (m < p.count && at < 2 * PB_ROW)
+                v[m][c] = *reinterpret_cast<const uint4*>(at < PB_ROW ? pk + a + at : pv + a + at - PB_ROW);
+        }
+    }
+    if (lane < p.count) pb_keep(r, out_scores, out_places, row * budget + p.to, p.from);
+#pragma unroll
+    for (int m = 0; m < PB_MOVES; ++m)
+#pragma unroll
+        for (int c = 0; c < PB_CHUNKS; ++c) {
+            const int at = (c * 32 + lane) * 16;
+            const pb_i64 b = to_row[m];
+            if (m < p.count && at < 2 * PB_ROW)
+                *reinterpret_cast<uint4*>(at < PB_ROW ? pk + b + at : pv + b + at - PB_ROW) = v[m][c];
+        }
+}
+
 #ifdef PB_CLUSTER
 static __device__ __forceinline__ pb_u32 pb_rank() {
     pb_u32 r;
@@ -209,34 +248,52 @@ static __device__ __forceinline__ int pb_peer(const int* p, pb_u32 rank) {
     return v;
 }
 
+// Sums of two of the counts that CTAs of lower rank left in `totals`.
+static __device__ __forceinline__ int2 pb_before(const int* totals, pb_u32 rank, int2* sums) {
+#if PB_CLUSTER > 1
+    if (threadIdx.x < 32) {
+        int2 v = make_int2(0, 0);
+        if (threadIdx.x < rank) v = make_int2(pb_peer(totals, threadIdx.x), pb_peer(totals + 1, threadIdx.x));
+#pragma unroll
+        for (int m = 4; m > 0; m /= 2) {
+            v.x += __shfl_down_sync(0xffffffffu, v.x, m);
+            v.y += __shfl_down_sync(0xffffffffu, v.y, m);
+        }
+        if (threadIdx.x == 0) *sums = v;
+    }
+    __syncthreads();
+    return *sums;
+#else
+    return make_int2(0, 0);
+#endif
+}
+
 // One cluster per sequence and key head. Each CTA holds the keys of a run of
-// slots in shared memory (its threads own consecutive ones, an odd stride
-// apart, so that they read distinct banks), and the row is read once:
+// slots; a thread owns PB_KPT consecutive ones, handed over through shared
+// memory (an odd stride apart, so that threads use distinct banks), and the
+// row is read once:
 //  1. radix select of the budget-th largest key, 8 bits a pass, the counts
 //     summed over the cluster through distributed shared memory; it ends as
 //     soon as a bin is wanted whole;
 //  2. exclusive sums over the slots' order rank ties, free places and late
-//     slots. The j-th late slot goes to the j-th free place.
+//     slots. The j-th late slot goes to the j-th free place;
+//  3. where they are few (`fused`) its warps move them, which saves a launch.
 // What bounds it: the latency of the passes (two barriers each), not bytes.
-extern "C" __global__ void __launch_bounds__(1024) pb_evict_select(
+extern "C" __global__ void __launch_bounds__(PB_THREADS, PB_THREADS < 1024 ? 2 : 1) pb_evict_select(
     const float* scores, const float* places, const int* lengths, const int* newest, float* out_scores,
     float* out_places, int* holes, int* lates, int* counts, pb_i64 ns, pb_i64 np, int budget, int recent, int sinks,
-    int pairs, int per_thread) {
+    int pairs, char* pk, char* pv, const int* tables, int width, int fused) {
+    constexpr int threads = PB_THREADS, run = PB_THREADS * PB_KPT, stride = PB_KPT | 1;
     extern __shared__ pb_u32 keys[];
-    __shared__ int hist[2][256], bins[256], chosen[3], totals[3];
-    __shared__ int2 warps[32];
+    __shared__ int hist[2][256], bins[256], chosen[3], totals[4];
+    __shared__ int2 warps[32], before;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const pb_i64 row = blockIdx.x / PB_CLUSTER;
     const pb_u32 rank = PB_CLUSTER > 1 ? pb_rank() : 0;
     const pb_row r = pb_row_of(scores, places, lengths, newest, ns, np, recent, sinks, row);
-    const int threads = blockDim.x, run = threads * per_thread, first = rank * run;
-    for (int i = first + threadIdx.x; i < min(first + run, budget); i += threads)
-        if (i >= r.length) { // nothing is kept there
-            out_scores[row * budget + i] = 0.0f;
-            out_places[row * budget + i] = -1.0f;
-        }
-    // The budget may reach past the slots that the cluster covers.
-    for (int i = PB_CLUSTER * run + rank * threads + threadIdx.x; i < budget; i += PB_CLUSTER * threads) {
+    const int first = rank * run;
+    // Nothing is kept past the length; the budget may reach past the cluster's slots.
+    for (int i = max(r.length, first) + threadIdx.x; i < (rank == PB_CLUSTER - 1 ? budget : min(first + run, budget)); i += threads) {
         out_scores[row * budget + i] = 0.0f;
         out_places[row * budget + i] = -1.0f;
     }
@@ -246,10 +303,25 @@ extern "C" __global__ void __launch_bounds__(1024) pb_evict_select(
         if (rank == 0 && threadIdx.x == 0) counts[row] = 0;
         return;
     }
-    const int stride = per_thread | 1, n = min(run, r.length - first); // n may be negative
-    for (int i = threadIdx.x; i < n; i += threads) keys[i / per_thread * stride + i % per_thread] = pb_key(r, first + i);
-    const pb_u32* own = keys + threadIdx.x * stride;
-    const int mine = max(0, min(per_thread, n - (int)threadIdx.x * per_thread));
+    const int n = min(run, r.length - first); // may be negative
+    constexpr int batch = PB_KPT < 8 ? PB_KPT : 8; // loads on the way at once
+#pragma unroll 1
+    for (int q = 0; q < PB_KPT; q += batch) {
+        float score[batch], place[batch];
+#pragma unroll
+        for (int j = 0; j < batch; ++j) { // every load before the first use
+            const int i = first + (q + j) * threads + threadIdx.x;
+            score[j] = i < r.length && i < r.ns ? r.scores[i] : 0.0f;
+            place[j] = i < r.length && i < r.np ? r.places[i] : -1.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < batch; ++j) {
+            const int i = (q + j) * threads + threadIdx.x;
+            keys[i / PB_KPT * stride + i % PB_KPT] = pb_key_of(r, first + i, score[j], place[j]);
+        }
+    }
+    pb_u32* own = keys + threadIdx.x * stride;
+    const int mine = max(0, min(PB_KPT, n - (int)threadIdx.x * PB_KPT));
 
     pb_u32 limit = 0; // the bits of the threshold so far
     int want = budget;
@@ -288,13 +360,12 @@ extern "C" __global__ void __launch_bounds__(1024) pb_evict_select(
         ties = pb_block_scan(make_int2(count, 0), warps, total).x;
         if (threadIdx.x == 0) totals[0] = total.x;
         pb_cluster_sync();
-        if (PB_CLUSTER > 1)
-            for (pb_u32 c = 0; c < rank; ++c) ties += pb_peer(totals, c);
+        ties += pb_before(totals, rank, &before).x;
     }
     pb_u64 kept = 0; // up to 64 slots a thread
     int2 count = make_int2(0, 0); // free places, late slots
     int seen = ties;
-    const int slot0 = first + threadIdx.x * per_thread;
+    const int slot0 = first + threadIdx.x * PB_KPT;
     for (int j = 0; j < mine; ++j) {
         const pb_u32 key = own[j];
         const bool keep = whole ? key >= limit : key > limit || (key == limit && seen++ < want);
@@ -304,29 +375,31 @@ extern "C" __global__ void __launch_bounds__(1024) pb_evict_select(
         count.y += !low && keep;
     }
     int2 at = pb_block_scan(count, warps, total);
-    if (PB_CLUSTER > 1) {
-        if (threadIdx.x == 0) { totals[1] = total.x; totals[2] = total.y; }
-        pb_cluster_sync();
-        for (pb_u32 c = 0; c < rank; ++c) {
-            at.x += pb_peer(totals + 1, c);
-            at.y += pb_peer(totals + 2, c);
-        }
-    }
+    if (threadIdx.x == 0) { totals[2] = total.x; totals[3] = total.y; }
+    pb_cluster_sync();
+    const int2 earlier = pb_before(totals + 2, rank, &before);
+    at.x += earlier.x;
+    at.y += earlier.y;
     for (int j = 0; j < mine; ++j) {
         const int i = slot0 + j;
         const bool keep = kept >> j & 1u;
-        if (i < budget) {
-            if (keep) pb_keep(r, out_scores, out_places, row * budget + i, i);
-            else holes[row * pairs + at.x++] = i;
-        } else if (keep) {
-            lates[row * pairs + at.y++] = i;
-        }
+        if (i < budget && !keep) holes[row * pairs + at.x++] = i;
+        if (i >= budget && keep) lates[row * pairs + at.y++] = i;
+        own[j] = keep;
     }
-    if (PB_CLUSTER > 1) {
-        if (rank == PB_CLUSTER - 1 && threadIdx.x == threads - 1) counts[row] = at.y;
-        pb_cluster_sync(); // nobody leaves while its shared memory is read
-    } else if (threadIdx.x == threads - 1) {
-        counts[row] = at.y;
+    __syncthreads();
+    for (int i = threadIdx.x; i < min(n, budget - first); i += threads)
+        if (keys[i / PB_KPT * stride + i % PB_KPT]) pb_keep(r, out_scores, out_places, row * budget + first + i, first + i);
+    if (rank == PB_CLUSTER - 1 && threadIdx.x == threads - 1) counts[row] = at.y;
+    // The row's lists are complete, and nobody leaves while its shared memory is read.
+    pb_cluster_sync();
+    if (fused) {
+        const int groups = (pairs + PB_MOVES - 1) / PB_MOVES;
+        for (int g = rank * (threads / 32) + (threadIdx.x >> 5); g < groups; g += PB_CLUSTER * (threads / 32)) {
+            const pb_pairs p = pb_list(holes, lates, counts, row * groups + g, (row + 1) * groups, groups, pairs);
+            if (p.count <= 0) break;
+            pb_move(p, r, pk, pv, tables, out_scores, out_places, row, width, budget);
+        }
     }
 }
 #endif
@@ -345,7 +418,7 @@ static __device__ __forceinline__ int pb_block_rank(bool flag, int2* warps, int&
 extern "C" __global__ void __launch_bounds__(1024) pb_evict_select_long(
     const float* scores, const float* places, const int* lengths, const int* newest, float* out_scores,
     float* out_places, int* holes, int* lates, int* counts, pb_i64 ns, pb_i64 np, int budget, int recent, int sinks,
-    int pairs, int per_thread) {
+    int pairs) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     __shared__ int hist[256], chosen[3];
     __shared__ int2 warps[32];
@@ -394,67 +467,63 @@ extern "C" __global__ void __launch_bounds__(1024) pb_evict_select_long(
     if (threadIdx.x == 0) counts[row] = nlate;
 }
 
-// Moves the late rows, keys and values, with their scores and positions. A
-// warp takes PB_MOVES pairs, all loads before the first store, so that it has
-// as many bytes on the way as a row's size allows. Sources lie at or past the
-// budget, destinations below it.
 extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
     char* pk, char* pv, const int* tables, const float* scores, const float* places, const int* lengths,
     const int* newest, float* out_scores, float* out_places, const int* holes, const int* lates, const int* counts,
     pb_i64 ns, pb_i64 np, pb_i64 rows, int width, int budget, int pairs) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int groups = (pairs + PB_MOVES - 1) / PB_MOVES, lane = threadIdx.x & 31;
-    const pb_i64 id = ((pb_i64)blockIdx.x * 256 + threadIdx.x) / 32, row = id / groups;
-    if (row >= rows) return;
-    const int j0 = (int)(id - row * groups) * PB_MOVES, count = counts[row];
-    if (j0 >= count) return;
-    const int s = (int)(row / PB_H), h = (int)(row % PB_H);
-    const int* table = tables + (pb_i64)s * width;
-    int from = 0, to = 0;
-    if (lane < PB_MOVES && j0 + lane < count) {
-        from = lates[row * pairs + j0 + lane];
-        to = holes[row * pairs + j0 + lane];
-        const pb_row r = pb_row_of(scores, places, lengths, newest, ns, np, 0, 0, row);
-        pb_keep(r, out_scores, out_places, row * budget + to, from);
-    }
-    // 16 bytes a lane: chunk c of the 2 * PB_ROW bytes of a slot, keys first.
-    uint4 v[PB_MOVES][PB_CHUNKS];
-    pb_i64 to_row[PB_MOVES];
-#pragma unroll
-    for (int m = 0; m < PB_MOVES; ++m) {
-        const int f = __shfl_sync(0xffffffffu, from, m), t = __shfl_sync(0xffffffffu, to, m);
-        const pb_i64 a = (((pb_i64)table[f / PB_PS] * PB_H + h) * PB_PS + f % PB_PS) * PB_ROW;
-        to_row[m] = (((pb_i64)table[t / PB_PS] * PB_H + h) * PB_PS + t % PB_PS) * PB_ROW;
-#pragma unroll
-        for (int c = 0; c < PB_CHUNKS; ++c) {
-            const int at = (c * 32 + lane) * 16;
-            if (j0 + m < count && at < 2 * PB_ROW)
-                v[m][c] = *reinterpret_cast<const uint4*>(at < PB_ROW ? pk + a + at : pv + a + at - PB_ROW);
-        }
-    }
-#pragma unroll
-    for (int m = 0; m < PB_MOVES; ++m)
-#pragma unroll
-        for (int c = 0; c < PB_CHUNKS; ++c) {
-            const int at = (c * 32 + lane) * 16;
-            const pb_i64 b = to_row[m];
-            if (j0 + m < count && at < 2 * PB_ROW)
-                *reinterpret_cast<uint4*>(at < PB_ROW ? pk + b + at : pv + b + at - PB_ROW) = v[m][c];
-        }
+    const int groups = (pairs + PB_MOVES - 1) / PB_MOVES;
+    const pb_i64 id = (pb_i64)blockIdx.x * 8 + (threadIdx.x >> 5), row = id / groups;
+    const pb_pairs p = pb_list(holes, lates, counts, id, rows * groups, groups, pairs);
+    if (p.count <= 0) return;
+    const pb_row r = pb_row_of(scores, places, lengths, newest, ns, np, 0, 0, row);
+    pb_move(p, r, pk, pv, tables, out_scores, out_places, row, width, budget);
 }
 #endif
 )PB";
         }
 
-        int moves_of(const kv_cache& c) { return 2 * c.dim * c.width() <= 512 ? 4 : 2; } // pairs a warp moves
+        // How the select shares out a row of `longest` slots.
+        struct select_shape {
+            int cluster = 0, threads = 0, per_thread = 0; // cluster 0: the long form
+            uint32_t smem() const { return static_cast<uint32_t>(threads * (per_thread | 1) * 4); }
+        };
+        select_shape shape_for(int64_t longest, int64_t rows, int sms) {
+            static constexpr int kShapes[][2] = {{256, 4}, {256, 8}, {512, 8}, {512, 16}, {1024, 16}, {1024, 32}, {1024, 48}};
+            select_shape r;
+            // More CTAs for each row as long as all of them fit the GPU at
+            // once, two of an SM, and each has a few thousand slots; more
+            // still where the keys need the room.
+            int64_t c = 1;
+            while (c < 8 && rows * c * 2 <= 2 * sms && longest >= 4096 * c) c *= 2;
+            for (; c <= 8; c *= 2)
+                for (const auto& [threads, per_thread] : kShapes)
+                    if (int64_t{threads} * per_thread * c >= longest) {
+                        r.cluster = static_cast<int>(c);
+                        r.threads = threads;
+                        r.per_thread = per_thread;
+                        return r;
+                    }
+            return r;
+        }
 
-        std::string defines(const kv_cache& c, bool wide, int cluster = 0) {
+        // Rows with at most so many late slots move them in the select.
+        constexpr int kFewPairs = 128;
+
+        // Pairs that a warp moves: 2 KB on the way, more where one pair is larger.
+        // (8 KB at half the occupancy took 31 us where 2 KB take 27, for 64 MB
+        // of pairs; a persistent form that reads its lists ahead took 41.)
+        int moves_of(const kv_cache& c) { return std::max<int>(1, 4 / static_cast<int>((2 * c.dim * c.width() + 511) / 512)); }
+
+        std::string defines(const kv_cache& c, bool wide, const select_shape& f = {}) {
             std::ostringstream os;
             os << "#define PB_H " << c.heads << "\n#define PB_D " << c.dim << "\n#define PB_PS " << c.page_size
                << "\n#define PB_ROW " << c.dim * c.width() << "\n#define PB_BF16 " << (c.type == cache_type::bf16 ? 1 : 0)
                << "\n#define PB_WIDE " << (wide ? 1 : 0) << "\n#define PB_MOVES " << moves_of(c)
                << "\n#define PB_CHUNKS " << (2 * c.dim * c.width() + 511) / 512 << "\n";
-            if (cluster != 0) os << "#define PB_CLUSTER " << cluster << "\n";
+            if (f.cluster != 0)
+                os << "#define PB_CLUSTER " << f.cluster << "\n#define PB_THREADS " << f.threads << "\n#define PB_KPT "
+                   << f.per_thread << "\n";
             return os.str();
         }
 
@@ -463,36 +532,15 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
         const char kSelectLong[] = "pb_evict_select_long";
         const char kMove[] = "pb_evict_move";
 
-        op_kernel& kernel_of(const char* name, const kv_cache& c, bool wide = true, int cluster = 0, uint32_t smem = 0) {
-            const op_key key{reinterpret_cast<int64_t>(name), c.heads, c.dim, c.page_size, static_cast<int64_t>(c.type), wide, cluster};
+        op_kernel& kernel_of(const char* name, const kv_cache& c, bool wide = true, const select_shape& f = {}) {
+            const op_key key{reinterpret_cast<int64_t>(name), c.heads, c.dim, c.page_size, static_cast<int64_t>(c.type),
+                             wide, f.cluster, f.threads, f.per_thread};
             return op_kernel_for(key, [&](op_kernel& k) {
                 k.name = name;
-                k.source = std::string{kernel_prelude()} + defines(c, wide, cluster) +
+                k.source = std::string{kernel_prelude()} + defines(c, wide, f) +
                            (name == kAppend ? append_source() : evict_source());
-                k.smem = smem;
+                k.smem = f.smem();
             });
-        }
-
-        // How the select shares out a row of `longest` slots.
-        struct select_shape {
-            int cluster = 0, threads = 0, per_thread = 0; // cluster 0: the long form
-        };
-        constexpr int kSelectSmem = 200 * 1024; // keys of a CTA, 4 bytes each
-        select_shape shape_for(int64_t longest, int64_t rows, int sms) {
-            select_shape r;
-            // A cluster for each row as long as all CTAs fit the GPU twice
-            // and each has a few thousand slots; larger where the keys need it.
-            int64_t c = 1;
-            while (c < 8 && rows * c * 2 <= 2 * sms && longest >= 4096 * c) c *= 2;
-            auto fits = [&](int64_t n) {
-                const int64_t run = (longest + n - 1) / n;
-                r.threads = run <= 2048 ? 256 : 1024;
-                r.per_thread = static_cast<int>((run + r.threads - 1) / r.threads);
-                return r.per_thread <= 64 && int64_t{r.threads} * (r.per_thread | 1) * 4 <= kSelectSmem;
-            };
-            while (c <= 8 && !fits(c)) c *= 2;
-            if (c <= 8) r.cluster = static_cast<int>(c);
-            return r;
         }
 
     } // namespace
@@ -664,20 +712,23 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
         int width = static_cast<int>(batch.table_width);
         int64_t nsv = ns, npv = np;
         select_shape f = shape_for(batch.longest, rows, sm_count(device));
-        void* sparams[] = {&xs.ptr, &xp.ptr, &batch.lengths_at, &batch.newest_at, &os.ptr, &op.ptr, &holes, &lates,
-                           &counts, &nsv,    &npv,              &b,               &rc,     &sk,     &pairs, &f.per_thread};
+        const bool moves = batch.longest > budget;
+        if (moves) {
+            order_write(*cuda_jit::buffer_access::state(c.k), stream);
+            order_write(*cuda_jit::buffer_access::state(c.v), stream);
+        }
+        uint64_t pk = address(c.k), pv = address(c.v);
+        int fused = moves && f.cluster != 0 && pairs <= kFewPairs;
+        void* sparams[] = {&xs.ptr, &xp.ptr, &batch.lengths_at, &batch.newest_at, &os.ptr, &op.ptr, &holes,
+                           &lates,  &counts, &nsv,              &npv,             &b,      &rc,     &sk,
+                           &pairs,  &pk,     &pv,               &batch.tables_at, &width,  &fused};
         if (f.cluster != 0) {
-            const uint32_t smem = static_cast<uint32_t>(f.threads * (f.per_thread | 1) * 4);
-            op_launch(kernel_of(kSelect, c, true, f.cluster, kSelectSmem), device, stream,
-                      {static_cast<uint32_t>(rows * f.cluster), 1, 1}, static_cast<uint32_t>(f.threads), sparams,
-                      static_cast<uint32_t>(f.cluster), smem);
+            op_launch(kernel_of(kSelect, c, true, f), device, stream, {static_cast<uint32_t>(rows * f.cluster), 1, 1},
+                      static_cast<uint32_t>(f.threads), sparams, static_cast<uint32_t>(f.cluster));
         } else {
             op_launch(kernel_of(kSelectLong, c), device, stream, {static_cast<uint32_t>(rows), 1, 1}, 1024, sparams);
         }
-        if (batch.longest > budget) {
-            order_write(*cuda_jit::buffer_access::state(c.k), stream);
-            order_write(*cuda_jit::buffer_access::state(c.v), stream);
-            uint64_t pk = address(c.k), pv = address(c.v);
+        if (moves && !fused) {
             const int64_t groups = (pairs + moves_of(c) - 1) / moves_of(c);
             const int64_t blocks = (rows * groups + 7) / 8;
             expect(blocks <= 0x7fffffff, "cache_evict: too many rows");
@@ -699,7 +750,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
             const std::string tag = type == cache_type::bf16 ? "_bf16" : "_f32", p = kernel_prelude();
             out.emplace_back("pb_cache_append" + tag, p + defines(c, type == cache_type::bf16) + append_source());
             out.emplace_back("pb_evict" + tag, p + defines(c, true) + evict_source());
-            out.emplace_back("pb_evict_select" + tag, p + defines(c, true, type == cache_type::bf16 ? 8 : 1) + evict_source());
+            out.emplace_back("pb_evict_select" + tag, p + defines(c, true, type == cache_type::bf16 ? select_shape{8, 1024, 48} : select_shape{1, 256, 4}) + evict_source());
         }
     }
 
