@@ -162,24 +162,29 @@ static __device__ __forceinline__ void pb_mma(float* c, const pb_u32* a, const p
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
-static __device__ __forceinline__ float pb_tf32(float x) {
-    pb_u32 r;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(x));
-    return __uint_as_float(r);
+// x = hi + lo: hi is x rounded to tf32 (10 mantissa bits, half up) by integer
+// arithmetic, which runs at the full rate that conversions do not have (16 x
+// 2049 slots of 64 channels: 37.6 us with cvt.rna, MEASURED_F32 us so); x - hi
+// is exact, and the tensor core reads its upper 10 bits: an error of at most
+// 2^-21 |x|, of either sign. A NaN stays one in lo.
+static __device__ __forceinline__ void pb_tf32_split(float x, float& hi, float& lo) {
+    hi = __uint_as_float((__float_as_uint(x) + 0x1000u) & 0xffffe000u);
+    lo = x - hi;
 }
-// x = t0 + t1 + e, tf32 each, |e| <= 2^-22 |x|.
 static __device__ __forceinline__ void pb_split_store(pb_u32 at, pb_u32 step, float x) {
-    const float hi = pb_tf32(x);
+    float hi, lo;
+    pb_tf32_split(x, hi, lo);
     asm volatile("st.shared.f32 [%0], %1;" :: "r"(at), "f"(hi) : "memory");
-    asm volatile("st.shared.f32 [%0], %1;" :: "r"(at + step), "f"(pb_tf32(x - hi)) : "memory");
+    asm volatile("st.shared.f32 [%0], %1;" :: "r"(at + step), "f"(lo) : "memory");
 }
 // hi and lo of four fragment values.
 static __device__ __forceinline__ void pb_split_frag(const pb_u32* a, pb_u32* hi, pb_u32* lo) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float x = __uint_as_float(a[i]), h = pb_tf32(x);
+        float h, l;
+        pb_tf32_split(__uint_as_float(a[i]), h, l);
         hi[i] = __float_as_uint(h);
-        lo[i] = __float_as_uint(pb_tf32(x - h));
+        lo[i] = __float_as_uint(l);
     }
 }
 #endif
@@ -205,6 +210,12 @@ static __device__ __forceinline__ bool pb_next(pb_at& a, const int* lengths, int
     return true;
 }
 
+// The page that this lane's part of the tile lies in (0 past its slots).
+static __device__ __forceinline__ int pb_page(const pb_at& a, const int* tables, int width, int lane) {
+    const int first = a.tile * 64 + lane * PB_BOX;
+    return lane * PB_BOX < 64 && first < a.length ? tables[(pb_i64)a.s * width + first / PB_PS] : 0;
+}
+
 extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
     const __grid_constant__ pb_tmap map_k, const __grid_constant__ pb_tmap map_v, const float* q, const int* lengths,
     const int* tables, const int4* work, float* out, float* partial, float2* partial_ml, float* logits, float* lse,
@@ -228,7 +239,9 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // The plan, lengths and tables were in place before the launch (their
+    // upload was waited for on the host), so they are read while the previous
+    // kernel still runs; everything else waits for it.
     const int4 mine = work[blockIdx.x];
     pb_at at;
     at.row = mine.x;
@@ -240,13 +253,14 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
         int slot = 0, unit = 0;
         pb_u32 parity = 1; // the first round finds every unit free
         bool bad = false;
+        int page = pb_page(at, tables, width, lane);
+        asm volatile("griddepcontrol.wait;" ::: "memory");
         for (int i = 0; i < mine.z && !bad; ++i) {
-            if (i) pb_next(at, lengths, chunks);
             const int base = at.tile * 64, boxes = (min(64, at.length - base) + PB_BOX - 1) / PB_BOX;
-            int y = 0;
-            if (lane < boxes) {
-                const int first = base + lane * PB_BOX;
-                y = (tables[(pb_i64)at.s * width + first / PB_PS] * PB_H + at.h) * PB_PS + first % PB_PS;
+            const int y = (page * PB_H + at.h) * PB_PS + (base + lane * PB_BOX) % PB_PS;
+            if (i + 1 < mine.z) { // the next tile's pages are looked up while this one's loads are issued
+                pb_next(at, lengths, chunks);
+                page = pb_page(at, tables, width, lane);
             }
 #pragma unroll 1
             for (int which = 0; which < 2 && !bad; ++which) {
@@ -278,6 +292,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
     }
 
     // ---- four computing warps
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int g = lane >> 2, t = lane & 3;
     int slot = 0;
     pb_u32 parity = 0;
@@ -313,9 +328,11 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
 
         // ---- S^T = K Q^T: this warp's 16 slots x all heads
         bad |= !pb_wait(full + 8 * slot, parity, &abort_flag, err, 3);
-        float c[PB_TERMS][PB_NT][4];
+        // The first term's sum, the large one, runs in two chains that are
+        // added in fp32: half the additions that cut bits in a row.
+        float c[PB_TERMS + 1][PB_NT][4];
 #pragma unroll
-        for (int x = 0; x < PB_TERMS; ++x)
+        for (int x = 0; x < PB_TERMS + 1; ++x)
 #pragma unroll
             for (int n = 0; n < PB_NT; ++n)
 #pragma unroll
@@ -340,7 +357,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                         pb_u32 b[4];
                         pb_ldm4(b, qrow + (x * PB_HT + n * 8) * PB_QROW + k2 * 64);
                         pb_mma(c[x][n], a[0], b);
-                        pb_mma(c[x][n], a[1], b + 2);
+                        pb_mma(c[x == 0 ? PB_TERMS : x][n], a[1], b + 2);
                     }
 #else
                 pb_u32 hi[2][4], lo[2][4];
@@ -353,7 +370,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                     pb_ldm4(b2, qrow + (PB_HT + n * 8) * PB_QROW + k2 * 64);
                     pb_mma(c[0][n], hi[0], b);
                     pb_mma(c[1][n], hi[0], b2);
-                    pb_mma(c[0][n], hi[1], b + 2);
+                    pb_mma(c[PB_TERMS][n], hi[1], b + 2);
                     pb_mma(c[1][n], lo[0], b);
                     pb_mma(c[1][n], hi[1], b2 + 2);
                     pb_mma(c[1][n], lo[1], b + 2);
@@ -374,9 +391,9 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
             for (int e = 0; e < 4; ++e) {
                 const int at_slot = 16 * warp + g + (e >> 1) * 8;
 #if PB_TERMS == 3
-                const float x = (c[2][n][e] + c[1][n][e] + c[0][n][e]) * scale2;
+                const float x = (c[2][n][e] + c[1][n][e] + (c[0][n][e] + c[3][n][e])) * scale2;
 #else
-                const float x = (c[1][n][e] + c[0][n][e]) * scale2;
+                const float x = (c[1][n][e] + (c[0][n][e] + c[2][n][e])) * scale2;
 #endif
                 s[n][e] = at_slot < valid ? x : __int_as_float(0xff800000);
 #if PB_SCORED
@@ -484,7 +501,11 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                                 const int r = first + (e >> 1), ch = mt * 16 + g + (e & 1) * 8;
                                 const pb_u32 where = vunit + (ch >> 5) * 8192 + r * 128 + ((((ch & 31) >> 2) ^ (r & 7)) << 4) + (ch & 3) * 4;
                                 asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[e]) : "r"(where) : "memory");
-                                if (r >= valid) v[e] = 0u;
+                            }
+                            if (valid < 64) { // what lies past the end may be anything
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    if (first + (e >> 1) >= valid) v[e] = 0u;
                             }
                             pb_u32 hi[4], lo[4];
                             pb_split_frag(v, hi, lo);
@@ -511,6 +532,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
         if (lane == 0) pb_mbar_arrive(empty + 8 * slot);
         if (++slot == PB_RING) { slot = 0; parity ^= 1u; }
 
+        if (i + 1 == mine.z) asm volatile("griddepcontrol.launch_dependents;");
         // ---- the row ends, or this CTA's part of it
         const bool row_ends = at.tile + 1 == at.tiles;
         if (row_ends || i + 1 == mine.z) {
@@ -561,38 +583,77 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
 }
 
 // Joins the parts of a row that several CTAs worked on, and writes zeros for a
-// row without slots. Block: one query head of one such row.
-extern "C" __global__ void __launch_bounds__(128) pb_paged_join(
+// row without slots. Block: one query head of one such row; its threads read
+// the parts' sums at once, then each group of D / 4 threads takes every
+// PB_JOIN-th part, four channels a thread. Latency: two rounds of loads.
+#define PB_JOIN (512 / (PB_D / 4))
+extern "C" __global__ void __launch_bounds__(512) pb_paged_join(
     const int4* rows, const float* partial, const float2* partial_ml, float* out, float* lse, int group, int chunks) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    __shared__ float weight[128];
+    __shared__ float weight[512], reduce[16];
+    __shared__ float4 sums[512];
     const int4 r = rows[blockIdx.x / PB_HT]; // row, first CTA, number of parts, the first part's place
     const int head = blockIdx.x % PB_HT, chunk = r.x % chunks, kvh = (r.x / chunks) % PB_H, s = r.x / chunks / PB_H;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (head >= group - chunk * PB_HT) return;
     const pb_i64 global = (pb_i64)s * PB_H * group + kvh * group + chunk * PB_HT + head;
-    float top = __int_as_float(0xff800000);
-    for (int i = 0; i < r.z; ++i) top = fmaxf(top, partial_ml[(pb_i64)(2 * (r.y + i) + (i ? 0 : r.w)) * PB_HT + head].x);
-    float sum = 0.0f, acc[(PB_D + 127) / 128] = {};
-    for (int from = 0; from < r.z; from += 128) {
-        const int n = min(128, r.z - from);
-        __syncthreads();
-        if (threadIdx.x < n) {
-            const int i = from + threadIdx.x;
-            weight[threadIdx.x] = pb_exp2(partial_ml[(pb_i64)(2 * (r.y + i) + (i ? 0 : r.w)) * PB_HT + head].x - top);
-        }
-        __syncthreads();
-        for (int j = 0; j < n; ++j) {
-            const int i = from + j;
-            const pb_i64 part = (pb_i64)(2 * (r.y + i) + (i ? 0 : r.w)) * PB_HT + head;
-            sum = fmaf(weight[j], partial_ml[part].y, sum);
+    const int lane = threadIdx.x & 31, quad = threadIdx.x % (PB_D / 4), team = threadIdx.x / (PB_D / 4);
+    float top = __int_as_float(0xff800000), sum = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int from = 0; from < r.z; from += 512) { // one round unless a row has over 512 parts
+        const int n = min(512, r.z - from), i = from + threadIdx.x;
+        float2 ml = make_float2(__int_as_float(0xff800000), 0.0f);
+        if (threadIdx.x < n) ml = partial_ml[(pb_i64)(2 * (r.y + i) + (i ? 0 : r.w)) * PB_HT + head];
+        float x = ml.x;
 #pragma unroll
-            for (int a = 0; a < (PB_D + 127) / 128; ++a)
-                if (threadIdx.x + 128 * a < PB_D) acc[a] = fmaf(weight[j], partial[part * PB_D + threadIdx.x + 128 * a], acc[a]);
+        for (int m = 16; m > 0; m /= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, m));
+        __syncthreads();
+        if (lane == 0) reduce[threadIdx.x >> 5] = x;
+        __syncthreads();
+        x = top;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) x = fmaxf(x, reduce[w]);
+        const float corr = pb_exp2(top - x);
+        top = x;
+        const float w = threadIdx.x < n ? pb_exp2(ml.x - top) : 0.0f;
+        weight[threadIdx.x] = w;
+        float y = w * ml.y;
+#pragma unroll
+        for (int m = 16; m > 0; m /= 2) y += __shfl_xor_sync(0xffffffffu, y, m);
+        __syncthreads();
+        if (lane == 0) reduce[threadIdx.x >> 5] = y;
+        __syncthreads();
+        y = 0.0f;
+#pragma unroll
+        for (int w2 = 0; w2 < 16; ++w2) y += reduce[w2];
+        sum = fmaf(sum, corr, y);
+        acc = make_float4(acc.x * corr, acc.y * corr, acc.z * corr, acc.w * corr);
+        if (team < PB_JOIN) {
+#pragma unroll 4
+            for (int j = team; j < n; j += PB_JOIN) {
+                const int at = from + j;
+                const pb_i64 part = (pb_i64)(2 * (r.y + at) + (at ? 0 : r.w)) * PB_HT + head;
+                const float4 o = *reinterpret_cast<const float4*>(partial + part * PB_D + 4 * quad);
+                acc.x = fmaf(weight[j], o.x, acc.x);
+                acc.y = fmaf(weight[j], o.y, acc.y);
+                acc.z = fmaf(weight[j], o.z, acc.z);
+                acc.w = fmaf(weight[j], o.w, acc.w);
+            }
         }
     }
-#pragma unroll
-    for (int a = 0; a < (PB_D + 127) / 128; ++a)
-        if (threadIdx.x + 128 * a < PB_D) out[global * PB_D + threadIdx.x + 128 * a] = r.z ? acc[a] / sum : 0.0f;
+    sums[threadIdx.x] = acc;
+    __syncthreads();
+    if (team == 0) {
+        for (int w = 1; w < PB_JOIN; ++w) {
+            const float4 o = sums[w * (PB_D / 4) + quad];
+            acc.x += o.x;
+            acc.y += o.y;
+            acc.z += o.z;
+            acc.w += o.w;
+        }
+        const float inv = r.z ? 1.0f / sum : 0.0f;
+        *reinterpret_cast<float4*>(out + global * PB_D + 4 * quad) =
+            r.z ? make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    }
 #if PB_SCORED
     if (threadIdx.x == 0) lse[global] = r.z ? top + log2f(sum) : 0.0f;
 #endif
@@ -763,7 +824,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_paged_scores(
         if (plan.joins > 0) {
             void* params[] = {&join, &partial, &ml, &out.ptr, &lse, &group, &chunks};
             op_launch(kernel_of(kJoin, f, 0), device, stream,
-                      {static_cast<uint32_t>(plan.joins * 8 * f.tiles8), 1, 1}, 128, params);
+                      {static_cast<uint32_t>(plan.joins * 8 * f.tiles8), 1, 1}, 512, params);
         }
         std::vector<tensor> results;
         results.push_back(finish(std::move(out)));
