@@ -23,6 +23,7 @@ namespace porch::detail {
         struct form {
             int heads = 1, dim = 0, page = 0;
             bool bf16 = false, scored = false;
+            int join_threads = 128;
             int tiles8 = 1; // groups of 8 query heads that a row holds (1 or 2)
             int width() const { return bf16 ? 2 : 4; }
             int planes() const { return (dim * width() + 127) / 128; }
@@ -45,7 +46,7 @@ namespace porch::detail {
             // than its bytes. At least three units, so that one is in flight
             // while two are read.
             std::pair<int, int> choose() const {
-                for (int n = unit() <= 8192 ? 4 : 2; n > 1; n /= 2) {
+                for (int n = unit() <= 8192 ? 4 : 3; n > 1; --n) {
                     const int r = ((228 * 1024) / n - 2048 - small()) / unit();
                     if (r >= 3) return {n, std::min(r, 6)};
                 }
@@ -586,21 +587,22 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
 // row without slots. Block: one query head of one such row; its threads read
 // the parts' sums at once, then each group of D / 4 threads takes every
 // PB_JOIN-th part, four channels a thread. Latency: two rounds of loads.
-#define PB_JOIN (512 / (PB_D / 4))
-extern "C" __global__ void __launch_bounds__(512) pb_paged_join(
+#define PB_JOIN (PB_JOIN_THREADS / (PB_D / 4))
+extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_join(
     const int4* rows, const float* partial, const float2* partial_ml, float* out, float* lse, int group, int chunks) {
-    __shared__ float weight[512], reduce[16];
-    __shared__ float4 sums[512];
-    const int4 r = rows[blockIdx.x / PB_HT]; // row, first CTA, number of parts, the first part's place
-    const int head = blockIdx.x % PB_HT, chunk = r.x % chunks, kvh = (r.x / chunks) % PB_H, s = r.x / chunks / PB_H;
+    __shared__ float weight[PB_JOIN_THREADS], reduce[16];
+    __shared__ float4 sums[PB_JOIN_THREADS];
+    const int heads = min(group, PB_HT);
+    const int4 r = rows[blockIdx.x / heads]; // row, first CTA, number of parts, the first part's place
+    const int head = blockIdx.x % heads, chunk = r.x % chunks, kvh = (r.x / chunks) % PB_H, s = r.x / chunks / PB_H;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (head >= group - chunk * PB_HT) return;
     const pb_i64 global = (pb_i64)s * PB_H * group + kvh * group + chunk * PB_HT + head;
     const int lane = threadIdx.x & 31, quad = threadIdx.x % (PB_D / 4), team = threadIdx.x / (PB_D / 4);
     float top = __int_as_float(0xff800000), sum = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int from = 0; from < r.z; from += 512) { // one round unless a row has over 512 parts
-        const int n = min(512, r.z - from), i = from + threadIdx.x;
+    for (int from = 0; from < r.z; from += PB_JOIN_THREADS) { // one round unless a row has over PB_JOIN_THREADS parts
+        const int n = min(PB_JOIN_THREADS, r.z - from), i = from + threadIdx.x;
         float2 ml = make_float2(__int_as_float(0xff800000), 0.0f);
         if (threadIdx.x < n) ml = partial_ml[(pb_i64)(2 * (r.y + i) + (i ? 0 : r.w)) * PB_HT + head];
         float x = ml.x;
@@ -611,7 +613,7 @@ extern "C" __global__ void __launch_bounds__(512) pb_paged_join(
         __syncthreads();
         x = top;
 #pragma unroll
-        for (int w = 0; w < 16; ++w) x = fmaxf(x, reduce[w]);
+        for (int w = 0; w < PB_JOIN_THREADS / 32; ++w) x = fmaxf(x, reduce[w]);
         const float corr = pb_exp2(top - x);
         top = x;
         const float w = threadIdx.x < n ? pb_exp2(ml.x - top) : 0.0f;
@@ -624,7 +626,7 @@ extern "C" __global__ void __launch_bounds__(512) pb_paged_join(
         __syncthreads();
         y = 0.0f;
 #pragma unroll
-        for (int w2 = 0; w2 < 16; ++w2) y += reduce[w2];
+        for (int w2 = 0; w2 < PB_JOIN_THREADS / 32; ++w2) y += reduce[w2];
         sum = fmaf(sum, corr, y);
         acc = make_float4(acc.x * corr, acc.y * corr, acc.z * corr, acc.w * corr);
         if (team < PB_JOIN) {
@@ -683,7 +685,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_paged_scores(
             std::ostringstream os;
             os << "#define PB_H " << f.heads << "\n#define PB_D " << f.dim << "\n#define PB_PS " << f.page
                << "\n#define PB_ESZ " << f.width() << "\n#define PB_NT " << f.tiles8 << "\n#define PB_RING " << f.ring()
-               << "\n#define PB_PER_SM " << f.per_sm() << "\n#define PB_SCORED " << (f.scored ? 1 : 0) << "\n";
+               << "\n#define PB_JOIN_THREADS " << f.join_threads << "\n#define PB_PER_SM " << f.per_sm() << "\n#define PB_SCORED " << (f.scored ? 1 : 0) << "\n";
             return os.str();
         }
 
@@ -692,7 +694,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_paged_scores(
         const char kScores[] = "pb_paged_scores";
 
         op_kernel& kernel_of(const char* name, const form& f, uint32_t smem) {
-            const op_key key{reinterpret_cast<int64_t>(name), f.heads, f.dim, f.page, f.bf16, f.scored, f.tiles8};
+            const op_key key{reinterpret_cast<int64_t>(name), f.heads, f.dim, f.page, f.bf16, f.scored, f.tiles8, f.join_threads};
             return op_kernel_for(key, [&](op_kernel& k) {
                 k.name = name;
                 k.source = std::string{kernel_prelude()} + defines(f) + device_source();
@@ -822,9 +824,14 @@ extern "C" __global__ void __launch_bounds__(256) pb_paged_scores(
                       {static_cast<uint32_t>(plan.ctas), 1, 1}, 160, params);
         }
         if (plan.joins > 0) {
+            // A small block where each row has a few parts (many rows: 128
+            // threads take 5.7 us where 512 take 11.7), a large one where one
+            // row has many (37 parts each: 12.5 us and 6.2).
+            if (plan.most_parts > 8) f.join_threads = 512;
             void* params[] = {&join, &partial, &ml, &out.ptr, &lse, &group, &chunks};
             op_launch(kernel_of(kJoin, f, 0), device, stream,
-                      {static_cast<uint32_t>(plan.joins * 8 * f.tiles8), 1, 1}, 512, params);
+                      {static_cast<uint32_t>(plan.joins * std::min(group, 8 * f.tiles8)), 1, 1},
+                      static_cast<uint32_t>(f.join_threads), params);
         }
         std::vector<tensor> results;
         results.push_back(finish(std::move(out)));
@@ -860,6 +867,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_paged_scores(
         p->limit = ctas;
         p->ctas = static_cast<int64_t>(s.work.size() / 4);
         p->joins = static_cast<int64_t>(s.join.size() / 4);
+        for (size_t i = 2; i < s.join.size(); i += 4) p->most_parts = std::max<int64_t>(p->most_parts, s.join[i]);
         s.work.insert(s.work.end(), s.join.begin(), s.join.end());
         const int device = batch.cache->device;
         auto stream = upload_stream(device);
