@@ -40,13 +40,13 @@ namespace porch::detail {
             int smem() const { return 1024 + ring() * unit() + small(); }
 
           private:
-            // CTAs of an SM and units of a CTA's ring. Two CTAs hide each
-            // other's barriers; a third and fourth only pay where a tile is
-            // so small (8 KB units) that its chain of barriers takes longer
-            // than its bytes. At least three units, so that one is in flight
-            // while two are read.
+            // CTAs of an SM and units of a CTA's ring: as many CTAs as leave
+            // room for three units each, so that one is on its way while two
+            // are read. CTAs hide each other's barriers (48 sequences up to
+            // 8191 slots, 128 bfloat16 channels: 134 us with two CTAs of six
+            // units, 124 with three of three).
             std::pair<int, int> choose() const {
-                for (int n = unit() <= 8192 ? 4 : 3; n > 1; --n) {
+                for (int n = 4; n > 1; --n) {
                     const int r = ((228 * 1024) / n - 2048 - small()) / unit();
                     if (r >= 3) return {n, std::min(r, 6)};
                 }
@@ -165,7 +165,7 @@ static __device__ __forceinline__ void pb_mma(float* c, const pb_u32* a, const p
 }
 // x = hi + lo: hi is x rounded to tf32 (10 mantissa bits, half up) by integer
 // arithmetic, which runs at the full rate that conversions do not have (16 x
-// 2049 slots of 64 channels: 37.6 us with cvt.rna, MEASURED_F32 us so); x - hi
+// 2049 slots of 64 channels: 37.6 us with cvt.rna, 34.2 so); x - hi
 // is exact, and the tensor core reads its upper 10 bits: an error of at most
 // 2^-21 |x|, of either sign. A NaN stays one in lo.
 static __device__ __forceinline__ void pb_tf32_split(float x, float& hi, float& lo) {
@@ -583,19 +583,24 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
     if (bad) abort_flag = 1;
 }
 
+// A row in several parts: {row, first CTA, number of parts, the first part's
+// place}. Part i's sums for a query head.
+static __device__ __forceinline__ pb_i64 pb_part(const int4& r, int i, int head) {
+    return (pb_i64)(2 * (r.y + i) + (i ? 0 : r.w)) * PB_HT + head;
+}
+
 // Joins the parts of a row that several CTAs worked on, and writes zeros for a
 // row without slots. Block: one query head of one such row; its threads read
 // the parts' sums at once, then each group of D / 4 threads takes every
 // PB_JOIN-th part, four channels a thread. Latency: two rounds of loads.
 #define PB_JOIN (PB_JOIN_THREADS / (PB_D / 4))
-extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_join(
-    const int4* rows, const float* partial, const float2* partial_ml, float* out, float* lse, int group, int chunks) {
+static __device__ __forceinline__ void pb_join(const int4* joins, const float* partial, const float2* partial_ml,
+                                               float* out, int group, int chunks, int block) {
     __shared__ float weight[PB_JOIN_THREADS], reduce[16];
     __shared__ float4 sums[PB_JOIN_THREADS];
     const int heads = min(group, PB_HT);
-    const int4 r = rows[blockIdx.x / heads]; // row, first CTA, number of parts, the first part's place
-    const int head = blockIdx.x % heads, chunk = r.x % chunks, kvh = (r.x / chunks) % PB_H, s = r.x / chunks / PB_H;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int4 r = joins[block / heads];
+    const int head = block % heads, chunk = r.x % chunks, kvh = (r.x / chunks) % PB_H, s = r.x / chunks / PB_H;
     if (head >= group - chunk * PB_HT) return;
     const pb_i64 global = (pb_i64)s * PB_H * group + kvh * group + chunk * PB_HT + head;
     const int lane = threadIdx.x & 31, quad = threadIdx.x % (PB_D / 4), team = threadIdx.x / (PB_D / 4);
@@ -604,7 +609,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_join(
     for (int from = 0; from < r.z; from += PB_JOIN_THREADS) { // one round unless a row has over PB_JOIN_THREADS parts
         const int n = min(PB_JOIN_THREADS, r.z - from), i = from + threadIdx.x;
         float2 ml = make_float2(__int_as_float(0xff800000), 0.0f);
-        if (threadIdx.x < n) ml = partial_ml[(pb_i64)(2 * (r.y + i) + (i ? 0 : r.w)) * PB_HT + head];
+        if (threadIdx.x < n) ml = partial_ml[pb_part(r, i, head)];
         float x = ml.x;
 #pragma unroll
         for (int m = 16; m > 0; m /= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, m));
@@ -633,7 +638,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_join(
 #pragma unroll 4
             for (int j = team; j < n; j += PB_JOIN) {
                 const int at = from + j;
-                const pb_i64 part = (pb_i64)(2 * (r.y + at) + (at ? 0 : r.w)) * PB_HT + head;
+                const pb_i64 part = pb_part(r, at, head);
                 const float4 o = *reinterpret_cast<const float4*>(partial + part * PB_D + 4 * quad);
                 acc.x = fmaf(weight[j], o.x, acc.x);
                 acc.y = fmaf(weight[j], o.y, acc.y);
@@ -656,28 +661,102 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_join(
         *reinterpret_cast<float4*>(out + global * PB_D + 4 * quad) =
             r.z ? make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
-#if PB_SCORED
-    if (threadIdx.x == 0) lse[global] = r.z ? top + log2f(sum) : 0.0f;
-#endif
 }
 
 #if PB_SCORED
-// new[s, h, i] = scores[s, h, i] + sum over the group of 2^(logit - lse).
-extern "C" __global__ void __launch_bounds__(256) pb_paged_scores(
-    const float* logits, const float* lse, const int* lengths, const float* scores, float* out, pb_i64 longest,
-    pb_i64 ns, int group) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const pb_u32 blocks = (pb_u32)((longest + 255) / 256);
-    const pb_i64 i = (pb_i64)(blockIdx.x % blocks) * 256 + threadIdx.x, row = blockIdx.x / blocks;
-    if (i >= longest) return;
-    float a = 0.0f;
-    if (i < lengths[row / PB_H]) {
-        for (int g = 0; g < group; ++g) a += pb_exp2(logits[(row * group + g) * longest + i] - lse[row * group + g]);
-        if (i < ns) a += scores[row * ns + i];
+// new[s, h, i] = scores[s, h, i] + sum over the group of 2^(logit - lse), where
+// a split row's lse comes from its parts, so that scores need not wait for the
+// join. Block: 4 * PB_JOIN_THREADS slots of one sequence and key head, the
+// log-sums of up to 64 query heads at a time in shared memory.
+static __device__ __forceinline__ void pb_load_logits(float (&x)[4][4], const float* l, int heads, pb_i64 i0, int length,
+                                                      pb_i64 longest) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const pb_i64 i = i0 + j * PB_JOIN_THREADS;
+            x[e][j] = e < heads && i < length ? l[e * longest + i] : 0.0f;
+        }
+}
+static __device__ __forceinline__ void pb_scores(const int4* joins, const int* split, const float2* partial_ml,
+                                                 const float* logits, const float* lse, const int* lengths,
+                                                 const float* scores, float* out, pb_i64 longest, pb_i64 ns, int group,
+                                                 int chunks, pb_u32 block) {
+    __shared__ float sums[64];
+    const pb_u32 blocks = (pb_u32)((longest + 4 * PB_JOIN_THREADS - 1) / (4 * PB_JOIN_THREADS));
+    const pb_i64 row = block / blocks; // sequence and key head
+    const pb_i64 i0 = (pb_i64)(block % blocks) * (4 * PB_JOIN_THREADS) + threadIdx.x;
+    const int length = lengths[row / PB_H];
+    float a[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const pb_i64 i = i0 + j * PB_JOIN_THREADS;
+        a[j] = i < length && i < ns ? scores[row * ns + i] : 0.0f;
     }
-    out[row * longest + i] = a;
+    for (int from = 0; from < group; from += 64) {
+        const int n = min(64, group - from);
+        // The first heads' logits are on their way while the log-sums are formed.
+        float x[4][4];
+        const float* l = logits + (row * group + from) * longest;
+        pb_load_logits(x, l, n, i0, length, longest);
+        __syncthreads();
+        for (int e = threadIdx.x >> 5; e < n; e += PB_JOIN_THREADS / 32) { // a warp for each head, a lane for each part
+            const int lane = threadIdx.x & 31, g = from + e, at = split[row * chunks + g / PB_HT];
+            float top = __int_as_float(0xff800000), sum = 0.0f;
+            if (at < 0) {
+                top = lse[row * group + g];
+                sum = lane ? 0.0f : 1.0f;
+            } else {
+                const int4 r = joins[at];
+                for (int i = lane; i < r.z; i += 32) {
+                    const float2 ml = partial_ml[pb_part(r, i, g % PB_HT)];
+                    const float now = fmaxf(top, ml.x);
+                    sum = fmaf(sum, pb_exp2(top - now), ml.y * pb_exp2(ml.x - now));
+                    top = now;
+                }
+            }
+            float all = top;
+#pragma unroll
+            for (int m = 16; m > 0; m /= 2) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, m));
+            sum = sum != 0.0f ? sum * pb_exp2(top - all) : 0.0f; // lanes without a part have no maximum
+#pragma unroll
+            for (int m = 16; m > 0; m /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+            if (lane == 0) sums[e] = all + log2f(sum);
+        }
+        __syncthreads();
+        for (int g = 0; g < n; g += 4) {
+            if (g) pb_load_logits(x, l + g * longest, n - g, i0, length, longest);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (g + e < n)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (i0 + j * PB_JOIN_THREADS < length) a[j] += pb_exp2(x[e][j] - sums[g + e]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const pb_i64 i = i0 + j * PB_JOIN_THREADS;
+        if (i < longest) out[row * longest + i] = a[j];
+    }
 }
 #endif
+
+// The first `join_blocks` blocks join, the others score.
+extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
+    const int4* joins, const int* split, const float* partial, const float2* partial_ml, float* out,
+    const float* logits, const float* lse, const int* lengths, const float* scores, float* new_scores, pb_i64 longest,
+    pb_i64 ns, int group, int chunks, int join_blocks) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (blockIdx.x < join_blocks) {
+        pb_join(joins, partial, partial_ml, out, group, chunks, blockIdx.x);
+        return;
+    }
+#if PB_SCORED
+    pb_scores(joins, split, partial_ml, logits, lse, lengths, scores, new_scores, longest, ns, group, chunks,
+              blockIdx.x - join_blocks);
+#endif
+}
 )PB";
         }
 
@@ -690,8 +769,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_paged_scores(
         }
 
         const char kAttention[] = "pb_paged_attention";
-        const char kJoin[] = "pb_paged_join";
-        const char kScores[] = "pb_paged_scores";
+        const char kFinish[] = "pb_paged_finish";
 
         op_kernel& kernel_of(const char* name, const form& f, uint32_t smem) {
             const op_key key{reinterpret_cast<int64_t>(name), f.heads, f.dim, f.page, f.bf16, f.scored, f.tiles8, f.join_threads};
@@ -709,6 +787,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_paged_scores(
         struct schedule {
             std::vector<int32_t> work; // per CTA: row, tile, tiles, 0
             std::vector<int32_t> join; // per row to join or clear: row, first CTA, parts, its place
+            std::vector<int32_t> split; // per row: its entry of `join`, or -1
         };
 
         schedule make_schedule(const std::vector<int64_t>& lengths, int64_t heads, int64_t chunks, int64_t ctas) {
@@ -723,7 +802,9 @@ extern "C" __global__ void __launch_bounds__(256) pb_paged_scores(
                 const int64_t tiles = (lengths[s] + 63) / 64;
                 for (int64_t j = 0; j < per; ++j) {
                     const int64_t row = static_cast<int64_t>(s) * per + j;
+                    r.split.push_back(-1);
                     auto add = [&](int64_t first, int64_t parts, int64_t place) {
+                        r.split.back() = static_cast<int32_t>(r.join.size() / 4);
                         for (int64_t v : {row, first, parts, place}) r.join.push_back(static_cast<int32_t>(v));
                     };
                     if (tiles == 0) {
@@ -789,6 +870,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_paged_scores(
         const batch_plan& plan = plan_of(batch, chunks, int64_t{f.per_sm()} * sm_count(device));
 
         op_result out = new_result(shape, device, stream);
+        uint64_t results_ptr = out.ptr;
         order_read(*cuda_jit::buffer_access::state(batch.data), stream);
         order_read(*cuda_jit::buffer_access::state(c.k), stream);
         order_read(*cuda_jit::buffer_access::state(c.v), stream);
@@ -823,29 +905,28 @@ extern "C" __global__ void __launch_bounds__(256) pb_paged_scores(
             op_launch(kernel_of(kAttention, f, static_cast<uint32_t>(f.smem())), device, stream,
                       {static_cast<uint32_t>(plan.ctas), 1, 1}, 160, params);
         }
-        if (plan.joins > 0) {
-            // A small block where each row has a few parts (many rows: 128
-            // threads take 5.7 us where 512 take 11.7), a large one where one
-            // row has many (37 parts each: 12.5 us and 6.2).
-            if (plan.most_parts > 8) f.join_threads = 512;
-            void* params[] = {&join, &partial, &ml, &out.ptr, &lse, &group, &chunks};
-            op_launch(kernel_of(kJoin, f, 0), device, stream,
-                      {static_cast<uint32_t>(plan.joins * std::min(group, 8 * f.tiles8)), 1, 1},
-                      static_cast<uint32_t>(f.join_threads), params);
-        }
         std::vector<tensor> results;
         results.push_back(finish(std::move(out)));
+        op_result os;
+        int64_t blocks = plan.joins * std::min(group, 8 * f.tiles8);
+        // A small block where each row has a few parts (many rows: 128 threads
+        // take 5.7 us where 512 take 11.7), a large one where one row has many
+        // (37 parts each: 12.5 us and 6.2).
+        if (plan.most_parts > 16) f.join_threads = 512;
+        int join_blocks = static_cast<int>(blocks);
         if (scored) {
-            op_result os = new_result({n, c.heads, longest}, device, stream);
-            if (longest != 0) {
-                const int64_t blocks = (longest + 255) / 256 * n * c.heads;
-                expect(blocks <= 0x7fffffff, "paged_attention_scored: too many slots");
-                void* params[] = {&logits, &lse, &batch.lengths_at, &xs.ptr, &os.ptr, &longest, &ns, &group};
-                op_launch(kernel_of(kScores, f, 0), device, stream, {static_cast<uint32_t>(blocks), 1, 1}, 256,
-                          params);
-            }
-            results.push_back(finish(std::move(os)));
+            os = new_result({n, c.heads, longest}, device, stream);
+            blocks += (longest + 4 * f.join_threads - 1) / (4 * f.join_threads) * n * c.heads;
         }
+        expect(blocks <= 0x7fffffff, "paged_attention: too many sequences, heads and slots");
+        if (blocks > 0) {
+            uint64_t split = join + static_cast<uint64_t>(plan.joins) * 16;
+            void* params[] = {&join,   &split,   &partial, &ml,  &results_ptr, &logits, &lse,        &batch.lengths_at,
+                              &xs.ptr, &os.ptr,  &longest, &ns,  &group,       &chunks, &join_blocks};
+            op_launch(kernel_of(kFinish, f, 0), device, stream, {static_cast<uint32_t>(blocks), 1, 1},
+                      static_cast<uint32_t>(f.join_threads), params);
+        }
+        if (scored) results.push_back(finish(std::move(os)));
         return results;
     }
 
@@ -869,6 +950,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_paged_scores(
         p->joins = static_cast<int64_t>(s.join.size() / 4);
         for (size_t i = 2; i < s.join.size(); i += 4) p->most_parts = std::max<int64_t>(p->most_parts, s.join[i]);
         s.work.insert(s.work.end(), s.join.begin(), s.join.end());
+        s.work.insert(s.work.end(), s.split.begin(), s.split.end());
         const int device = batch.cache->device;
         auto stream = upload_stream(device);
         p->data = allocate(device, s.work.size() * sizeof(int32_t), stream);
