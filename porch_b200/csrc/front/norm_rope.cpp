@@ -305,6 +305,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_norm_rope_grad(
                 if (live) pb_store_head(dst + (pb_i64)(h0 + m) * PB_D, x[m], lane);
             }
         }
+        if (which) asm volatile("griddepcontrol.launch_dependents;");
         pb_store_head(sums[group], dw, lane);
         __syncthreads();
         for (int c = threadIdx.x; c < PB_D; c += 256) {
@@ -316,23 +317,26 @@ extern "C" __global__ void __launch_bounds__(256) pb_norm_rope_grad(
     }
 }
 
-// dw[which][c] = sum over `rows` rows of partial[which][row][c], 8 threads a
-// column, each over every 8th row, added in order.
-extern "C" __global__ void __launch_bounds__(256) pb_norm_rope_weights(const float* partial, float* dqw, float* dkw, int rows) {
+// dw[which][c] = sum over `rows` rows of partial[which][row][c], 32 threads a
+// column, each over every 32nd row, added in order.
+extern "C" __global__ void __launch_bounds__(1024) pb_norm_rope_weights(const float* partial, float* dqw, float* dkw, int rows) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    __shared__ float sums[8][32];
+    __shared__ float sums[32][33];
     const int x = threadIdx.x % 32, y = threadIdx.x / 32, c = blockIdx.x * 32 + x;
     float s = 0.0f;
     if (c < 2 * PB_D) {
         const float* p = partial + (pb_i64)(c / PB_D) * rows * PB_D + c % PB_D;
-        for (int r = y; r < rows; r += 8) s += p[(pb_i64)r * PB_D];
+#pragma unroll 4
+        for (int r = y; r < rows; r += 32) s += p[(pb_i64)r * PB_D];
     }
     sums[y][x] = s;
     __syncthreads();
-    if (y == 0 && c < 2 * PB_D) {
-        for (int i = 1; i < 8; ++i) s += sums[i][x];
-        (c < PB_D ? dqw : dkw)[c % PB_D] = s;
-    }
+    // Warp y adds column y's 32 sums.
+    s = sums[x][y];
+#pragma unroll
+    for (int m = 16; m > 0; m /= 2) s += __shfl_xor_sync(0xffffffffu, s, m);
+    const int column = blockIdx.x * 32 + y;
+    if (x == 0 && column < 2 * PB_D) (column < PB_D ? dqw : dkw)[column % PB_D] = s;
 }
 #endif
 )PB";
@@ -422,6 +426,20 @@ extern "C" __global__ void __launch_bounds__(256) pb_norm_rope_weights(const flo
             while (s.lanes < 32 && s.lanes < items_of(s)) s.lanes *= 2;
         }
 
+        // Heads of a token that a group takes at once, sharing its angles and
+        // weights and having all their loads on the way together: as many as
+        // its registers hold, once there are heads enough to fill the GPU so.
+        // Forward, 16384 tokens x 40 heads of 128: 112 us with one, 98 with
+        // two, 98 with four. Gradient, 8192 tokens: 84, 89 and 70 us (1021 and
+        // 777 tokens: 7.0, 6.1, 6.7 and 9.1, 8.3, 9.3).
+        int heads_at_once(const shape_key& s, int64_t tokens, int most, int sms) {
+            const int items = (items_of(s) + s.lanes - 1) / s.lanes;
+            if (tokens * (s.q_heads + s.k_heads) < int64_t{32} * sms) return 1;
+            int n = most;
+            while (n > 1 && n * items > most) n /= 2;
+            return n;
+        }
+
         struct operands {
             op_operand q, k, qw, kw, cos, sin, pos;
         };
@@ -444,6 +462,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_norm_rope_weights(const flo
         if (c.tokens != 0) {
             shape_key& s = c.key;
             choose_lanes(s, std::min(vector_width(x.q), vector_width(x.k)));
+            s.per = heads_at_once(s, c.tokens, 2, sm_count(device));
             op_kernel& kernel = kernel_of(s, kNormRope, "PB_FORWARD");
             const int64_t units = c.tokens * ((s.q_heads + s.per - 1) / s.per + (s.k_heads + s.per - 1) / s.per);
             const int64_t blocks = (units + 256 / s.lanes - 1) / (256 / s.lanes);
@@ -474,11 +493,14 @@ extern "C" __global__ void __launch_bounds__(256) pb_norm_rope_weights(const flo
         } else {
             shape_key& s = c.key;
             choose_lanes(s, std::min({vector_width(x.q), vector_width(x.k), vector_width(gq), vector_width(gk)}));
+            s.per = heads_at_once(s, c.tokens, 4, sm_count(device));
             op_kernel& kernel = kernel_of(s, kNormRopeGrad, "PB_BACKWARD");
             op_kernel& weights = kernel_of(s, kNormRopeWeights, "PB_BACKWARD");
             const int64_t groups = 256 / s.lanes;
             const int64_t units = c.tokens * ((std::max(s.q_heads, s.k_heads) + s.per - 1) / s.per);
-            const int64_t blocks = std::min<int64_t>((units + groups - 1) / groups, int64_t{4} * sm_count(device));
+            // Two blocks of an SM: fewer partial sums to add (of three to
+            // eight, none was faster).
+            const int64_t blocks = std::min<int64_t>((units + groups - 1) / groups, int64_t{2} * sm_count(device));
             auto partial = allocate(device, static_cast<size_t>(2 * blocks * s.dim) * sizeof(float), stream);
             uint64_t pp = address(partial);
             float eps = a.eps;
@@ -490,7 +512,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_norm_rope_weights(const flo
                               &x.k.strides[0],  &x.k.strides[1],  &eps};
             op_launch(kernel, device, stream, {static_cast<uint32_t>(blocks), 1, 1}, 256, params);
             void* wparams[] = {&pp, &wq.ptr, &wk.ptr, &rows};
-            op_launch(weights, device, stream, {static_cast<uint32_t>((2 * s.dim + 31) / 32), 1, 1}, 256, wparams);
+            op_launch(weights, device, stream, {static_cast<uint32_t>((2 * s.dim + 31) / 32), 1, 1}, 1024, wparams);
         }
         return {finish(std::move(oq)), finish(std::move(ok)), finish(std::move(wq)), finish(std::move(wk))};
     }
@@ -498,7 +520,8 @@ extern "C" __global__ void __launch_bounds__(256) pb_norm_rope_weights(const flo
     void norm_rope_sources(std::vector<std::pair<std::string, std::string>>& out) {
         for (const auto& [dim, rot, inter, aligned] :
              {std::array<int, 4>{128, 128, 0, 4}, std::array<int, 4>{80, 40, 1, 1}, std::array<int, 4>{37, 18, 0, 1},
-              std::array<int, 4>{37, 18, 1, 1}}) {
+              std::array<int, 4>{37, 18, 1, 1},
+              std::array<int, 4>{1023, 1022, 0, 4}, std::array<int, 4>{512, 64, 0, 4}}) {
             shape_key s;
             s.dim = dim;
             s.half = rot / 2;
@@ -506,6 +529,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_norm_rope_weights(const flo
             s.k_heads = 2;
             s.interleaved = inter != 0;
             choose_lanes(s, aligned);
+            s.per = heads_at_once(s, 1 << 20, aligned, 148);
             const std::string tag = "_" + std::to_string(dim) + (inter ? "i" : "h");
             out.emplace_back("pb_norm_rope" + tag, source_of(s, "PB_FORWARD"));
             out.emplace_back("pb_norm_rope_grad" + tag, source_of(s, "PB_BACKWARD"));

@@ -145,6 +145,9 @@ CASES = [
     (2, 2, 1, 1023, 1022, False),
     (257, 6, 1, 6, 4, True),
     (600, 7, 2, 72, 72, False),
+    (1500, 5, 3, 64, 64, False),
+    (2500, 3, 1, 40, 24, True),
+    (1300, 3, 2, 513, 512, False),
 ]
 
 
