@@ -251,18 +251,18 @@ int pb_comm_wait(pb_comm* comm);
  * is contiguous. */
 
 /* A tensor with a copy of `count` floats at device address `pointer` (memory
- * of another library on the same GPU). Waits for what `stream` (a CUstream,
- * NULL for the legacy default stream) holds, and for the copy, so the source
- * may be reused on return. */
+ * of another library on the same GPU), which `stream` (a CUstream, NULL for
+ * the legacy default stream) has written. The copy is ordered behind what
+ * that stream holds, and what it does next behind the copy, on the device;
+ * so the source may be reused in that stream's order. */
 int pb_tensor_from_device(const int64_t* shape, size_t rank, uint64_t pointer, size_t count,
                           void* stream, int device, pb_tensor** out);
 
 /* What another library on the same GPU needs to read the values in place:
- * shape (up to `capacity` extents; *rank receives the rank), device address
- * (as pb_tensor_device_pointer) and this thread's stream (a CUstream), which
- * the values are ordered on. */
-int pb_tensor_interface(const pb_tensor* tensor, int64_t* shape, size_t capacity, size_t* rank,
-                        uint64_t* pointer, void** stream);
+ * out[0] the rank, out[1] the device address (as pb_tensor_device_pointer),
+ * out[2] this thread's stream (a CUstream), which the values are ordered on,
+ * out[3...] the shape; `capacity` numbers fit. */
+int pb_tensor_interface(const pb_tensor* tensor, int64_t* out, size_t capacity);
 
 /* RMS norm of each query and key head with a weight per channel, and the
  * rotation of its first 2 * R2 channels by the token's position:

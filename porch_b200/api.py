@@ -192,6 +192,9 @@ def _unary(op: int, a) -> Expr:
     return Expr(out.value)
 
 
+_Numbers = c_int64 * 19
+
+
 class Tensor:
     """porch::tensor (a shared handle)."""
 
@@ -282,10 +285,11 @@ class Tensor:
         if self._face is None:
             # The address of a realised tensor's values stays what it is once
             # it was handed out, so consumers that ask twice cost one call.
-            shape, rank, pointer, stream = (c_int64 * 16)(), c_size_t(), c_uint64(), c_void_p()
-            _check(lib().pb_tensor_interface(self._h, shape, 16, byref(rank), byref(pointer), byref(stream)))
-            self._face = {"shape": tuple(shape[:rank.value]), "typestr": "<f4", "data": (pointer.value, False),
-                          "version": 3, "stream": stream.value}
+            out = _Numbers()
+            _check(lib().pb_tensor_interface(self._h, out, 19))
+            rank, pointer, stream, *shape = out
+            self._face = {"shape": tuple(shape[:rank]), "typestr": "<f4", "data": (pointer, False), "version": 3,
+                          "stream": stream}
         return self._face
 
     def __getitem__(self, key) -> Expr:

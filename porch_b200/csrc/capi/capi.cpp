@@ -673,32 +673,41 @@ int pb_tensor_from_device(const int64_t* shape, size_t rank, uint64_t pointer, s
         auto mine = porch::detail::current_stream(at);
         auto r = porch::detail::new_result(std::move(s), at, mine);
         if (count != 0) {
-            porch::detail::check(pbrt_stream_synchronize(at, static_cast<pbrt_stream>(stream)));
+            // The copy waits for what the source's stream holds, and what that
+            // stream does next waits for the copy; the host waits for neither.
+            auto theirs = static_cast<pbrt_stream>(stream);
+            auto wait = [&](pbrt_stream waits, pbrt_stream works) {
+                pbrt_event e = nullptr;
+                porch::detail::check(pbrt_event_create(at, 0, &e));
+                int status = pbrt_event_record(at, e, works);
+                if (status == PBRT_OK) status = pbrt_stream_wait_event(at, waits, e);
+                (void)pbrt_event_destroy(at, e);
+                porch::detail::check(status);
+            };
+            wait(mine->stream, theirs);
             porch::detail::check(pbrt_memcpy_d2d_async(at, r.ptr, pointer, count * sizeof(float), mine->stream));
-            porch::detail::check(pbrt_stream_synchronize(at, mine->stream));
+            wait(theirs, mine->stream);
         }
         *out = wrap(porch::tensor_access::from_storage(std::move(r.shape), std::move(r.storage),
                                                        porch::device{device}));
     });
 }
 
-int pb_tensor_interface(const pb_tensor* t, int64_t* shape, size_t capacity, size_t* rank, uint64_t* pointer,
-                        void** stream) {
+int pb_tensor_interface(const pb_tensor* t, int64_t* out, size_t capacity) {
     return guarded([&] {
         require(t, "tensor");
-        require(rank, "rank");
-        require(pointer, "pointer");
-        require(stream, "stream");
+        require(out, "out");
+        const auto extents = t->value.shape();
+        if (capacity < 3 + extents.size()) throw std::invalid_argument("interface needs room for 3 numbers and the shape");
         const auto& buffer = t->value.device_data();
         const auto& st = porch::cuda_jit::buffer_access::state(buffer);
-        auto extents = t->value.shape();
-        *rank = extents.size();
-        for (size_t i = 0; i < extents.size() && i < capacity; ++i) shape[i] = extents[i];
-        *pointer = st ? st->ptr : 0;
         // Behind the producer, if that is another thread's stream.
         auto mine = porch::detail::current_stream(st ? st->device : t->value.placement().ordinal());
         if (st && st->ptr != 0) porch::detail::order_read(*st, mine);
-        *stream = mine->stream;
+        out[0] = static_cast<int64_t>(extents.size());
+        out[1] = static_cast<int64_t>(st ? st->ptr : 0);
+        out[2] = reinterpret_cast<int64_t>(mine->stream);
+        for (size_t i = 0; i < extents.size(); ++i) out[3 + i] = extents[i];
     });
 }
 

@@ -389,19 +389,17 @@ extern "C" __global__ void __launch_bounds__(1024) pb_norm_rope_weights(const fl
 
         // Every check that needs no device.
         checked check_args(const norm_rope_args& a) {
-            const auto q = shape_of(*a.q), k = shape_of(*a.k);
+            const auto q = a.q->shape(), k = a.k->shape();
             expect(q.size() == 3 && k.size() == 3, "qk_norm_rope: q and k must be [tokens, heads, head_dim]");
             expect(q[0] == k[0] && q[2] == k[2], "qk_norm_rope: q and k must have the same tokens and head_dim");
             expect(q[1] >= 1 && k[1] >= 1 && q[1] <= 65536 && k[1] <= 65536, "qk_norm_rope: q and k need 1 to 65536 heads");
             expect(q[2] >= 1 && q[2] <= 1024, "qk_norm_rope: head_dim must be 1 to 1024");
-            const std::vector<index_t> channel{q[2]};
-            expect(shape_of(*a.q_weight) == channel && shape_of(*a.k_weight) == channel,
-                   "qk_norm_rope: weights must be [head_dim]");
-            const auto c = shape_of(*a.cos);
-            expect(c.size() == 2 && shape_of(*a.sin) == c, "qk_norm_rope: cos and sin must be [positions, rot / 2]");
+            expect(has_shape(*a.q_weight, {q[2]}) && has_shape(*a.k_weight, {q[2]}), "qk_norm_rope: weights must be [head_dim]");
+            const auto c = a.cos->shape();
+            expect(c.size() == 2 && has_shape(*a.sin, {c[0], c[1]}), "qk_norm_rope: cos and sin must be [positions, rot / 2]");
             expect(c[0] >= 1 && c[1] >= 1 && 2 * c[1] <= q[2], "qk_norm_rope: rot must be 2 to head_dim, of at least one position");
             expect(c[0] <= (index_t{1} << 24), "qk_norm_rope: at most 2^24 positions (float32 counts them exactly)");
-            expect(shape_of(*a.positions) == std::vector<index_t>{q[0]}, "qk_norm_rope: positions must be [tokens]");
+            expect(has_shape(*a.positions, {q[0]}), "qk_norm_rope: positions must be [tokens]");
             expect(a.eps >= 0.0F, "qk_norm_rope: eps must not be negative");
             checked r;
             r.tokens = q[0];
@@ -479,7 +477,7 @@ extern "C" __global__ void __launch_bounds__(1024) pb_norm_rope_weights(const fl
 
     std::array<tensor, 4> qk_norm_rope_backward(const tensor& dq, const tensor& dk, const norm_rope_args& a) {
         checked c = check_args(a);
-        expect(shape_of(dq) == shape_of(*a.q) && shape_of(dk) == shape_of(*a.k),
+        expect(std::ranges::equal(dq.shape(), a.q->shape()) && std::ranges::equal(dk.shape(), a.k->shape()),
                "qk_norm_rope_backward: gradients must have the shapes of q and k");
         const int device = device_of(*a.q, "qk_norm_rope_backward");
         auto stream = current_stream(device);

@@ -2,6 +2,7 @@
 // operand access, results, in-place ordering.
 #include "operators.hpp"
 
+#include <algorithm>
 #include <sstream>
 #include <stdexcept>
 #include <unordered_map>
@@ -75,6 +76,8 @@ namespace porch::detail {
 
     std::vector<index_t> shape_of(const tensor& t) { return {t.shape().begin(), t.shape().end()}; }
 
+    bool has_shape(const tensor& t, std::initializer_list<index_t> shape) { return std::ranges::equal(t.shape(), shape); }
+
     int device_of(const tensor& t, const char* what) {
         auto s = tensor_access::storage(t);
         if (s->placeholder)
@@ -85,8 +88,10 @@ namespace porch::detail {
     op_operand operand(const tensor& t, const std::shared_ptr<stream_ref>& stream, bool strided) {
         op_operand x;
         x.storage = tensor_access::storage(t);
-        x.shape = shape_of(t);
-        x.strides = contiguous_strides(x.shape);
+        if (strided) {
+            x.shape = shape_of(t);
+            x.strides = contiguous_strides(x.shape);
+        }
         x.device = stream->device;
         if (x.storage->device != stream->device)
             throw std::invalid_argument("operands must live on one device");

@@ -47,7 +47,8 @@ namespace porch::detail {
     // ------------------------------------------------------------ operands --
     // A float32 operand read in place: device address of element 0 and its
     // strides (a strided view is not copied as long as its innermost axis is
-    // contiguous). Ordered behind its producer on `stream`.
+    // contiguous; otherwise, and unless `strided`, it is made contiguous and
+    // only its address is filled in). Ordered behind its producer on `stream`.
     struct op_operand {
         std::shared_ptr<realized_storage> storage;
         uint64_t ptr = 0;
@@ -59,6 +60,7 @@ namespace porch::detail {
     // Shape and device checks come first and need no device; operand() then
     // realises.
     std::vector<index_t> shape_of(const tensor& t);
+    bool has_shape(const tensor& t, std::initializer_list<index_t> shape);
     op_operand operand(const tensor& t, const std::shared_ptr<stream_ref>& stream, bool strided);
     // The device that `t`'s values live on; throws for placeholders.
     int device_of(const tensor& t, const char* what);
