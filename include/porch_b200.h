@@ -320,13 +320,13 @@ int pb_kv_append(pb_kv_batch* batch, const pb_tensor* k, const pb_tensor* v);
  * i reads key head i / (q_heads / kv_heads)). An empty sequence gives zeros.
  * Sums, maxima and the result are float32 for either cache type. */
 int pb_paged_attention(const pb_tensor* q, pb_kv_batch* batch, float scale, pb_tensor** out);
-/* How the attention of a batch with these lengths is shared out over `ctas`
- * CTAs, as text, without a GPU: a row is a (sequence, key head, chunk of query
- * heads), a tile 64 slots of it. "work <row> <tile> <tiles>" for each CTA (its
- * first row and tile, and how many it works through), and "join <row> <first
- * CTA> <parts> <place>" for each row in several parts (place: whether the
- * first CTA's part is its first, 0, or its last, 1) or without slots (0
- * parts). Text as pb_expr_describe's. */
+/* How the attention of a batch with these lengths is shared out over about
+ * `ctas` CTAs, as text, without a GPU: a row is a (sequence, key head, chunk of
+ * query heads), a tile 64 slots of it. "work <row> <tile> <tiles>" for each CTA
+ * (its first row and tile, and how many it works through; none: it clears a
+ * row without slots), and "join <row> <first CTA> <parts> <place>" for each row
+ * in several parts (place: whether the first CTA's part is its first, 0, or its
+ * last, 1). Text as pb_expr_describe's. */
 int pb_kv_plan_describe(const int64_t* lengths, size_t sequences, int64_t kv_heads,
                         int64_t chunks, int64_t ctas, char* text, size_t capacity,
                         size_t* needed);

@@ -93,7 +93,7 @@ def _declare(L: ctypes.CDLL) -> None:
         "pb_matmul_3xtf32_noalloc": (c_int, [c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64,
                                              c_void_p]),
         "pb_tensor_from_device": (c_int, [P(c_int64), c_size_t, c_uint64, c_size_t, c_void_p, c_int, P(T)]),
-        "pb_tensor_interface": (c_int, [T, P(c_int64), c_size_t]),
+        "pb_tensor_interface": (c_int, [T, c_void_p, c_size_t]),
         "pb_qk_norm_rope": (c_int, [T, T, T, T, T, T, T, c_float, c_int, P(T), P(T)]),
         "pb_qk_norm_rope_backward": (c_int, [T, T, T, T, T, T, T, T, T, c_float, c_int, P(T)]),
         "pb_kv_cache_create": (c_int, [c_int64, c_int64, c_int64, c_int64, c_int, c_int, P(T)]),

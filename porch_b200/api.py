@@ -287,9 +287,8 @@ class Tensor:
             # it was handed out, so consumers that ask twice cost one call.
             out = _Numbers()
             _check(lib().pb_tensor_interface(self._h, out, 19))
-            rank, pointer, stream, *shape = out
-            self._face = {"shape": tuple(shape[:rank]), "typestr": "<f4", "data": (pointer, False), "version": 3,
-                          "stream": stream}
+            self._face = {"shape": tuple(out[3:3 + out[0]]), "typestr": "<f4", "data": (out[1], False), "version": 3,
+                          "stream": out[2]}
         return self._face
 
     def __getitem__(self, key) -> Expr:

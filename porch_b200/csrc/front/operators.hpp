@@ -111,6 +111,11 @@ namespace porch::detail {
         int device = 0;
         cuda_jit::device_buffer k, v;
         int width() const { return type == cache_type::bf16 ? 2 : 4; } // bytes of a value
+        // TMA maps of both pools as [rows, dim]: boxes of 128 bytes by a page,
+        // or by 64 rows of a larger one.
+        struct alignas(64) tensor_map {
+            unsigned char bytes[128];
+        } map_k, map_v;
     };
     std::shared_ptr<kv_cache> make_cache(int64_t pages, int64_t page_size, int64_t heads, int64_t dim,
                                          cache_type type, int device);

@@ -294,6 +294,12 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
 
     // ---- four computing warps
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (mine.z == 0) { // a row without slots
+        const int heads = min(PB_HT, group - at.chunk * PB_HT);
+        const pb_i64 to = (pb_i64)at.s * PB_H * group + at.h * group + at.chunk * PB_HT;
+        for (int e = threadIdx.x; e < heads * PB_D; e += 128) out[to * PB_D + e] = 0.0f;
+        return;
+    }
     const int g = lane >> 2, t = lane & 3;
     int slot = 0;
     pb_u32 parity = 0;
@@ -589,8 +595,7 @@ static __device__ __forceinline__ pb_i64 pb_part(const int4& r, int i, int head)
     return (pb_i64)(2 * (r.y + i) + (i ? 0 : r.w)) * PB_HT + head;
 }
 
-// Joins the parts of a row that several CTAs worked on, and writes zeros for a
-// row without slots. Block: one query head of one such row; its threads read
+// Joins the parts of a row that several CTAs worked on. Block: one query head of one such row; its threads read
 // the parts' sums at once, then each group of D / 4 threads takes every
 // PB_JOIN-th part, four channels a thread. Latency: two rounds of loads.
 #define PB_JOIN (PB_JOIN_THREADS / (PB_D / 4))
@@ -657,9 +662,9 @@ static __device__ __forceinline__ void pb_join(const int4* joins, const float* p
             acc.z += o.z;
             acc.w += o.w;
         }
-        const float inv = r.z ? 1.0f / sum : 0.0f;
+        const float inv = 1.0f / sum;
         *reinterpret_cast<float4*>(out + global * PB_D + 4 * quad) =
-            r.z ? make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
     }
 }
 
@@ -783,48 +788,65 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         // Even runs of 64-slot tiles, over all rows one after the other: the
         // CTAs' shares differ by one tile at most, whatever the lengths. A run
         // begins and ends inside a row at most once each, so a CTA leaves at
-        // most two parts behind.
+        // most two parts behind. Where every row is short and they all fit,
+        // each has a CTA of its own instead: up to kWholeRow tiles in a row
+        // take less time than the second launch that joins parts. A row
+        // without slots has a CTA that writes its zeros, after the others.
         struct schedule {
             std::vector<int32_t> work; // per CTA: row, tile, tiles, 0
-            std::vector<int32_t> join; // per row to join or clear: row, first CTA, parts, its place
+            std::vector<int32_t> join; // per row in parts: row, first CTA, parts, its place
             std::vector<int32_t> split; // per row: its entry of `join`, or -1
         };
+        constexpr int64_t kWholeRow = 6;
 
         schedule make_schedule(const std::vector<int64_t>& lengths, int64_t heads, int64_t chunks, int64_t ctas) {
             schedule r;
             const int64_t per = heads * chunks;
-            int64_t total = 0;
-            for (int64_t n : lengths) total += (n + 63) / 64 * per;
-            const int64_t n = std::min(total, ctas);
+            int64_t total = 0, rows = 0, most = 0;
+            for (int64_t length : lengths) {
+                const int64_t tiles = (length + 63) / 64;
+                total += tiles * per;
+                most = std::max(most, tiles);
+                if (tiles != 0) rows += per;
+            }
+            const bool whole = most <= kWholeRow && rows <= ctas;
+            const int64_t n = whole ? rows : std::min(total, ctas);
             int64_t cta = 0, from = 0; // `from`: the row's first tile in the whole order
             auto start = [&](int64_t c) { return n == 0 ? 0 : static_cast<int64_t>(static_cast<__int128>(total) * c / n); };
+            auto put = [](std::vector<int32_t>& to, std::initializer_list<int64_t> values) {
+                for (int64_t v : values) to.push_back(static_cast<int32_t>(v));
+            };
+            std::vector<int32_t> empty;
             for (size_t s = 0; s < lengths.size(); ++s) {
                 const int64_t tiles = (lengths[s] + 63) / 64;
                 for (int64_t j = 0; j < per; ++j) {
                     const int64_t row = static_cast<int64_t>(s) * per + j;
                     r.split.push_back(-1);
-                    auto add = [&](int64_t first, int64_t parts, int64_t place) {
-                        r.split.back() = static_cast<int32_t>(r.join.size() / 4);
-                        for (int64_t v : {row, first, parts, place}) r.join.push_back(static_cast<int32_t>(v));
-                    };
                     if (tiles == 0) {
-                        add(0, 0, 0);
+                        put(empty, {row, 0, 0, 0});
+                        continue;
+                    }
+                    if (whole) {
+                        put(r.work, {row, 0, tiles, 0});
                         continue;
                     }
                     // CTAs that begin in this row.
                     while (cta < n && start(cta) < from + tiles) {
-                        for (int64_t v : {row, start(cta) - from, start(cta + 1) - start(cta), int64_t{0}})
-                            r.work.push_back(static_cast<int32_t>(v));
+                        put(r.work, {row, start(cta) - from, start(cta + 1) - start(cta), 0});
                         ++cta;
                     }
                     // Its first part belongs to the last CTA that begins at or before it.
                     int64_t first = cta - 1;
                     while (start(first) > from) --first;
                     const int64_t parts = cta - first;
-                    if (parts > 1) add(first, parts, start(first) < from ? 1 : 0);
+                    if (parts > 1) {
+                        r.split.back() = static_cast<int32_t>(r.join.size() / 4);
+                        put(r.join, {row, first, parts, start(first) < from ? 1 : 0});
+                    }
                     from += tiles;
                 }
             }
+            r.work.insert(r.work.end(), empty.begin(), empty.end());
             return r;
         }
 
@@ -888,18 +910,8 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         uint64_t work = address(plan.data), join = work + static_cast<uint64_t>(plan.ctas) * 16, err = 0;
         if (plan.ctas > 0) {
             check(pbrt_error_word(device, &err));
-            struct alignas(64) map {
-                unsigned char bytes[128];
-            } mk, mv;
-            const uint64_t dims[2] = {static_cast<uint64_t>(c.dim), static_cast<uint64_t>(c.pages * c.heads * c.page_size)};
-            const uint64_t strides[1] = {static_cast<uint64_t>(c.dim * c.width())};
-            const uint32_t box[2] = {static_cast<uint32_t>(128 / c.width()), static_cast<uint32_t>(std::min<int64_t>(64, c.page_size))};
-            const uint32_t ones[2] = {1, 1};
-            // bfloat16 or float32, 128-byte swizzle, 256-byte L2 promotion, zeros past the head size.
-            for (auto [m, p] : {std::pair{&mk, &c.k}, std::pair{&mv, &c.v}})
-                check(pbrt_tensor_map_encode_tiled(m->bytes, f.bf16 ? 9 : 7, 2, address(*p), dims, strides, box, ones, 0, 3, 3, 0));
             float scale2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
-            void* params[] = {&mk,     &mv,    &x.ptr, &batch.lengths_at, &batch.tables_at, &work,
+            void* params[] = {&c.map_k, &c.map_v, &x.ptr, &batch.lengths_at, &batch.tables_at, &work,
                               &out.ptr, &partial, &ml, &logits, &lse, &width, &group, &chunks,
                               &x.strides[0], &x.strides[1], &longest32, &scale2, &err};
             op_launch(kernel_of(kAttention, f, static_cast<uint32_t>(f.smem())), device, stream,

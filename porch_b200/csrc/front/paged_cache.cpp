@@ -568,6 +568,14 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
         auto stream = current_stream(c->device);
         c->k = allocate(c->device, bytes, stream);
         c->v = allocate(c->device, bytes, stream);
+        const uint64_t dims[2] = {static_cast<uint64_t>(dim), static_cast<uint64_t>(pages * heads * page_size)};
+        const uint64_t strides[1] = {static_cast<uint64_t>(dim * c->width())};
+        const uint32_t box[2] = {static_cast<uint32_t>(128 / c->width()), static_cast<uint32_t>(std::min<int64_t>(64, page_size))};
+        const uint32_t ones[2] = {1, 1};
+        // bfloat16 or float32, 128-byte swizzle, 256-byte L2 promotion, zeros past the head size.
+        for (auto [m, p] : {std::pair{&c->map_k, &c->k}, std::pair{&c->map_v, &c->v}})
+            check(pbrt_tensor_map_encode_tiled(m->bytes, type == cache_type::bf16 ? 9 : 7, 2, address(*p), dims, strides,
+                                               box, ones, 0, 3, 3, 0));
         return c;
     }
 

@@ -177,6 +177,8 @@ def test_every_tile_is_worked_on_once_and_every_split_row_joined(api, seed):
     heads, chunks, ctas = int(rng.integers(1, 6)), int(rng.integers(1, 4)), int(rng.integers(1, 600))
     if seed == 0:
         lengths = [0] * n
+    if seed > 30:
+        lengths = [x % 385 for x in lengths]
     tiles = np.repeat([-(-x // 64) for x in lengths], heads * chunks)
     work, join = [], {}
     for line in api.attention_plan(lengths, heads, ctas, chunks).splitlines():
@@ -187,8 +189,15 @@ def test_every_tile_is_worked_on_once_and_every_split_row_joined(api, seed):
             row, *rest = (int(x) for x in v)
             assert row not in join
             join[row] = rest
-    assert len(work) == min(ctas, tiles.sum())
-    assert not work or max(w[2] for w in work) - min(w[2] for w in work) <= 1
+    # Rows without slots have a CTA each, at the end.
+    clear = [w[0] for w in work if w[2] == 0]
+    assert clear == list(np.flatnonzero(tiles == 0)) and [w[2] for w in work[len(work) - len(clear):]] == [0] * len(clear)
+    work = work[: len(work) - len(clear)]
+    if tiles.max() <= 6 and (tiles > 0).sum() <= ctas:  # short rows: a CTA each
+        assert not join and [w[2] for w in work] == list(tiles[tiles > 0])
+    else:
+        assert len(work) == min(ctas, tiles.sum())
+        assert not work or max(w[2] for w in work) - min(w[2] for w in work) <= 1
     seen, parts = np.zeros(tiles.sum(), int), {}
     first = np.concatenate([[0], np.cumsum(tiles)])
     for c, (row, tile, count) in enumerate(work):
@@ -209,8 +218,7 @@ def test_every_tile_is_worked_on_once_and_every_split_row_joined(api, seed):
                     while tiles[row] == 0:
                         row += 1
     assert (seen == 1).all()
-    want = {r: [] for r in np.flatnonzero(tiles == 0)} | parts
-    assert want == {r: [(c + i, 0 if i else place) for i in range(k)] for r, (c, k, place) in join.items()}
+    assert parts == {r: [(c + i, 0 if i else place) for i in range(k)] for r, (c, k, place) in join.items()}
 
 
 @pytest.mark.gpu
