@@ -318,7 +318,9 @@ int pb_kv_append(pb_kv_batch* batch, const pb_tensor* k, const pb_tensor* v);
 /* softmax(scale q K^T) V for one query per sequence: q and the result
  * [sequences, q_heads, head_dim], q_heads a multiple of kv_heads (query head
  * i reads key head i / (q_heads / kv_heads)). An empty sequence gives zeros.
- * Sums, maxima and the result are float32 for either cache type. */
+ * Sums, maxima and the result are float32 for either cache type. A query, or
+ * a key or value in use, that is not finite makes results of the heads that
+ * read it not finite (infinity or NaN), and no others. */
 int pb_paged_attention(const pb_tensor* q, pb_kv_batch* batch, float scale, pb_tensor** out);
 /* How the attention of a batch with these lengths is shared out over about
  * `ctas` CTAs, as text, without a GPU: a row is a (sequence, key head, chunk of
@@ -362,6 +364,10 @@ int pb_operator_sources(char* text, size_t capacity, size_t* needed);
  * flight, frees its tensor memory and returns; the next synchronisation
  * raises PB_ERR_RUNTIME. Only for tests of that path. */
 int pb_test_gemm_stall(int enable);
+/* The same for paged attention: while enabled, its first CTA's tiles are
+ * never loaded, its bounded waits give up and the kernel records a code of
+ * 0x7d00 and more. */
+int pb_test_attention_stall(int enable);
 
 /* ---- matmul without allocation ------------------------------------------ */
 /* C = A @ B in fp32 (3xTF32 on tcgen05), on raw device pointers, allocating

@@ -853,6 +853,10 @@ int pb_kv_evict(pb_kv_batch* batch, const pb_tensor* scores, const pb_tensor* po
     });
 }
 
+int pb_test_attention_stall(int enable) {
+    return guarded([&] { porch::detail::set_test_attention_stall(enable != 0); });
+}
+
 namespace {
     void copy_text(const std::string& s, char* text, size_t capacity, size_t* needed) {
         if (needed) *needed = s.size() + 1;

@@ -155,6 +155,9 @@ namespace porch::detail {
 
     const batch_plan& plan_of(kv_batch& batch, int64_t chunks, int64_t ctas);
     int attention_ctas_per_sm(const kv_cache& c);
+    // Test hook (off by default): block 0 of an attention never gets its
+    // tiles, so its bounded waits expire.
+    void set_test_attention_stall(bool on);
     // The plan as text ("work <row> <tile> <tiles>" per CTA, "join <row>
     // <first CTA> <parts> <place>" per row), without a device.
     std::string attention_schedule(const std::vector<int64_t>& lengths, int64_t heads, int64_t chunks, int64_t ctas);

@@ -22,7 +22,7 @@ namespace porch::detail {
         // The whole layout of a kernel follows from these.
         struct form {
             int heads = 1, dim = 0, page = 0;
-            bool bf16 = false, scored = false;
+            bool bf16 = false, scored = false, stall = false;
             int join_threads = 128;
             int tiles8 = 1; // groups of 8 query heads that a row holds (1 or 2)
             int width() const { return bf16 ? 2 : 4; }
@@ -256,6 +256,9 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
         bool bad = false;
         int page = pb_page(at, tables, width, lane);
         asm volatile("griddepcontrol.wait;" ::: "memory");
+#ifdef PB_TEST_STALL
+        if (blockIdx.x == 0) return; // its tiles never arrive
+#endif
         for (int i = 0; i < mine.z && !bad; ++i) {
             const int base = at.tile * 64, boxes = (min(64, at.length - base) + PB_BOX - 1) / PB_BOX;
             const int y = (page * PB_H + at.h) * PB_PS + (base + lane * PB_BOX) % PB_PS;
@@ -770,14 +773,17 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             os << "#define PB_H " << f.heads << "\n#define PB_D " << f.dim << "\n#define PB_PS " << f.page
                << "\n#define PB_ESZ " << f.width() << "\n#define PB_NT " << f.tiles8 << "\n#define PB_RING " << f.ring()
                << "\n#define PB_JOIN_THREADS " << f.join_threads << "\n#define PB_PER_SM " << f.per_sm() << "\n#define PB_SCORED " << (f.scored ? 1 : 0) << "\n";
+            if (f.stall) os << "#define PB_TEST_STALL 1\n";
             return os.str();
         }
+
+        std::atomic<bool> g_test_stall{false};
 
         const char kAttention[] = "pb_paged_attention";
         const char kFinish[] = "pb_paged_finish";
 
         op_kernel& kernel_of(const char* name, const form& f, uint32_t smem) {
-            const op_key key{reinterpret_cast<int64_t>(name), f.heads, f.dim, f.page, f.bf16, f.scored, f.tiles8, f.join_threads};
+            const op_key key{reinterpret_cast<int64_t>(name), f.heads, f.dim, f.page, f.bf16, f.scored, f.tiles8, f.join_threads, f.stall};
             return op_kernel_for(key, [&](op_kernel& k) {
                 k.name = name;
                 k.source = std::string{kernel_prelude()} + defines(f) + device_source();
@@ -881,6 +887,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         f.page = static_cast<int>(c.page_size);
         f.bf16 = c.type == cache_type::bf16;
         f.scored = scored;
+        f.stall = g_test_stall.load(std::memory_order_relaxed);
         int heads = static_cast<int>(shape[1]), group = static_cast<int>(shape[1] / c.heads);
         // 16 query heads share a tile's loads, 8 where 16 would leave the ring
         // less than three units.
@@ -941,6 +948,8 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         if (scored) results.push_back(finish(std::move(os)));
         return results;
     }
+
+    void set_test_attention_stall(bool on) { g_test_stall.store(on); }
 
     int attention_ctas_per_sm(const kv_cache& c) {
         form f;

@@ -28,6 +28,10 @@ CASES = [
     ([9001, 3], 2, 6, 128, 128, "bf16"),
     ([20000], 1, 9, 112, 64, "bf16"),
     ([7] * 300, 1, 2, 24, 8, "bf16"),
+    ([1000, 70], 1, 12, 256, 16, "f32"),
+    ([700, 500], 2, 16, 128, 64, "bf16"),
+    ([700, 3], 1, 10, 256, 32, "bf16"),
+    ([385, 384, 0], 1, 1, 128, 8, "bf16"),
 ]
 
 
@@ -134,6 +138,74 @@ def test_queries_read_in_place_and_pages_shared_by_sequences(gpu):
     host.k, host.v = host.v, host.k
     out, tol, _, _ = host.attend(fused[:, 3:7, 1:], 0.125)
     assert (np.abs(gpu.paged_attention(q, both.on(other)).cpu().reshape(out.shape) - out) <= tol).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("first", [0, 1, 4])
+def test_new_tokens_read_in_place(gpu, dtype, first):
+    # Keys and values as heads of a fused projection, at aligned and odd channels.
+    rng = np.random.default_rng(first)
+    host = paged.Host(rng, [9, 20, 4], 2, 24, 8, dtype)
+    fused = rng.normal(0, 1, (33, 6, 28)).astype(np.float32)
+    ends = np.cumsum([0, 9, 20, 4])
+    for s in range(3):
+        host.k[s] = fused[ends[s] : ends[s + 1], 1:3, first : first + 24]
+        host.v[s] = fused[ends[s] : ends[s + 1], 4:6, first : first + 24]
+    cache = gpu.KVCache(host.pages, 8, 2, 24, dtype=dtype)
+    f = gpu.tensor([33, 6, 28], fused)
+    k, v = (gpu.materialize(f[gpu.all, h : h + 2, first : first + 24]) for h in (1, 4))
+    batch = cache.batch(host.tables, [9, 20, 4], appended=[9, 20, 4])
+    batch.append(k, v)
+    q = rng.normal(0, 1, (3, 4, 24)).astype(np.float32)
+    out, tol, _, _ = host.attend(q, 0.2)
+    got = gpu.paged_attention(gpu.tensor([3, 4, 24], q), batch, scale=0.2).cpu().reshape(q.shape)
+    assert (np.abs(got - out) <= tol).all()
+
+
+@pytest.mark.gpu
+def test_a_cache_written_by_one_thread_and_read_by_another(gpu):
+    import threading
+
+    rng = np.random.default_rng(6)
+    host = paged.Host(rng, [3000], 2, 64, 32, "f32")
+    cache = gpu.KVCache(host.pages, 32, 2, 64)
+    q = rng.normal(0, 1, (1, 4, 64)).astype(np.float32)
+    t = gpu.tensor([1, 4, 64], q)
+    batch = cache.batch(host.tables, [3000], appended=[3000])
+    read = cache.batch(host.tables, [3000], appended=[0])
+    rows = [(gpu.tensor([3000, 2, 64], host.k[0] * f), gpu.tensor([3000, 2, 64], host.v[0] * f)) for f in (1, 0.5, 2)]
+    for f, (k, v) in zip((1, 0.5, 2), rows):  # each write waits for the reads before it
+        th = threading.Thread(target=lambda: batch.append(gpu.materialize(k * 1.0), gpu.materialize(v * 1.0)))
+        th.start()
+        th.join()
+        got = gpu.paged_attention(t, read)
+        copy = paged.Host(np.random.default_rng(6), [3000], 2, 64, 32, "f32")
+        copy.k[0], copy.v[0] = copy.k[0] * np.float32(f), copy.v[0] * np.float32(f)
+        out, tol, _, _ = copy.attend(q, 0.125)
+        assert (np.abs(got.cpu().reshape(q.shape) - out) <= tol).all()
+
+
+@pytest.mark.gpu
+def test_a_wait_that_runs_out_is_reported_and_the_gpu_recovers(gpu):
+    # Block 0's loads are never issued: its bounded waits give up (about two
+    # seconds), the kernel records 0x7d00 + site and returns.
+    from porch_b200._lib import lib
+
+    rng = np.random.default_rng(6)
+    host = paged.Host(rng, [500, 40], 2, 64, 32, "bf16")
+    q = rng.normal(0, 1, (2, 4, 64)).astype(np.float32)
+    _, batch = host.build(gpu)
+    t = gpu.tensor([2, 4, 64], q)
+    assert lib().pb_test_attention_stall(1) == 0
+    try:
+        with pytest.raises(RuntimeError, match="kernel error code 32003"):  # 0x7d00 + site 3
+            gpu.paged_attention(t, batch).cpu()
+    finally:
+        assert lib().pb_test_attention_stall(0) == 0
+    out, tol, _, _ = host.attend(q, 0.125)
+    for _ in range(2):
+        assert (np.abs(gpu.paged_attention(t, batch).cpu().reshape(q.shape) - out) <= tol).all()
 
 
 @pytest.mark.gpu
