@@ -211,7 +211,7 @@ static __device__ __forceinline__ void pb_move(const pb_pairs& p, const pb_row& 
         for (int c = 0; c < PB_CHUNKS; ++c) {
             const int at = (c * 32 + lane) * 16;
             if (m < p.count && at < 2 * PB_ROW)
-                v[m][c] = *reinterpret_cast<const uint4*>(at < PB_ROW ? pk + a + at : pv + a + at - PB_ROW);
+                v[m][c] = __ldcs(reinterpret_cast<const uint4*>(at < PB_ROW ? pk + a + at : pv + a + at - PB_ROW));
         }
     }
     if (lane < p.count) pb_keep(r, out_scores, out_places, row * budget + p.to, p.from);
@@ -222,7 +222,7 @@ static __device__ __forceinline__ void pb_move(const pb_pairs& p, const pb_row& 
             const int at = (c * 32 + lane) * 16;
             const pb_i64 b = to_row[m];
             if (m < p.count && at < 2 * PB_ROW)
-                *reinterpret_cast<uint4*>(at < PB_ROW ? pk + b + at : pv + b + at - PB_ROW) = v[m][c];
+                __stcs(reinterpret_cast<uint4*>(at < PB_ROW ? pk + b + at : pv + b + at - PB_ROW), v[m][c]);
         }
 }
 
@@ -304,7 +304,7 @@ extern "C" __global__ void __launch_bounds__(PB_THREADS, PB_THREADS < 1024 ? 2 :
         return;
     }
     const int n = min(run, r.length - first); // may be negative
-    constexpr int batch = PB_KPT < 8 ? PB_KPT : 8; // loads on the way at once
+    constexpr int batch = PB_KPT < 16 ? PB_KPT : 16; // loads on the way at once
 #pragma unroll 1
     for (int q = 0; q < PB_KPT; q += batch) {
         float score[batch], place[batch];
@@ -388,8 +388,24 @@ extern "C" __global__ void __launch_bounds__(PB_THREADS, PB_THREADS < 1024 ? 2 :
         own[j] = keep;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < min(n, budget - first); i += threads)
-        if (keys[i / PB_KPT * stride + i % PB_KPT]) pb_keep(r, out_scores, out_places, row * budget + first + i, first + i);
+    // Slots that stay where they are: their scores and positions, four on the way.
+    const int stay = min(n, budget - first);
+    for (int base = threadIdx.x; base < stay; base += 4 * threads) {
+        float score[4], place[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = base + j * threads;
+            const bool keep = i < stay && keys[i / PB_KPT * stride + i % PB_KPT];
+            score[j] = keep ? pb_score(r, first + i) : 0.0f;
+            place[j] = keep ? pb_place(r, first + i) : -1.0f; // a position is not negative
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (place[j] >= 0.0f) {
+                out_scores[row * budget + first + base + j * threads] = score[j];
+                out_places[row * budget + first + base + j * threads] = place[j];
+            }
+    }
     if (rank == PB_CLUSTER - 1 && threadIdx.x == threads - 1) counts[row] = at.y;
     // The row's lists are complete, and nobody leaves while its shared memory is read.
     pb_cluster_sync();
