@@ -310,6 +310,18 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
     int segment = 0; // how many rows this CTA has begun
     float m[PB_NT][2], l[PB_NT][2], o[PB_MTW][PB_NT][4];
     bool begun_at_zero = true;
+#if PB_ESZ == 4
+    // Where this thread's four values of V^T lie in each of its channel tiles
+    // (slots 2 t and 2 t + 1 of a group of 8, channels g and g + 8).
+    pb_u32 v_at[PB_MTW][4];
+#pragma unroll
+    for (int a = 0; a < PB_MTW; ++a)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int r = 2 * t + (e >> 1), ch = (warp + 4 * a) * 16 + g + (e & 1) * 8;
+            v_at[a][e] = (ch >> 5) * 8192 + r * 128 + ((((ch & 31) >> 2) ^ r) << 4) + (ch & 3) * 4;
+        }
+#endif
     for (int i = 0; i < mine.z; ++i) {
         if (i) fresh = pb_next(at, lengths, chunks);
         const int hg = min(PB_HT, group - at.chunk * PB_HT);             // query heads of this row
@@ -317,10 +329,18 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
         if (fresh) {
             begun_at_zero = at.tile == 0;
             // The row's queries, split into terms; zero past the head size.
-            for (int e = threadIdx.x; e < PB_HT * (PB_STEPS * 32 / PB_ESZ); e += 128) {
-                const int head = e / (PB_STEPS * 32 / PB_ESZ), d = e % (PB_STEPS * 32 / PB_ESZ);
-                const float x = head < hg && d < PB_D ? __ldg(q + at.s * q_seq + (head0 + head) * q_head + d) : 0.0f;
-                pb_split_store(qs + head * PB_QROW + d * PB_ESZ, PB_HT * PB_QROW, x);
+            // Every load before the first use.
+            constexpr int per_head = PB_STEPS * 32 / PB_ESZ, each = (PB_HT * per_head + 127) / 128;
+            float x[each];
+#pragma unroll
+            for (int j = 0; j < each; ++j) {
+                const int e = threadIdx.x + 128 * j, head = e / per_head, d = e % per_head;
+                x[j] = head < hg && d < PB_D ? __ldg(q + at.s * q_seq + (head0 + head) * q_head + d) : 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < each; ++j) {
+                const int e = threadIdx.x + 128 * j, head = e / per_head, d = e % per_head;
+                if (e < PB_HT * per_head) pb_split_store(qs + head * PB_QROW + d * PB_ESZ, PB_HT * PB_QROW, x[j]);
             }
 #pragma unroll
             for (int n = 0; n < PB_NT; ++n)
@@ -507,11 +527,9 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                             // their rows' swizzles put the loads on distinct banks.
                             const int first = (2 * k2 + k) * 8 + 2 * t;
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const int r = first + (e >> 1), ch = mt * 16 + g + (e & 1) * 8;
-                                const pb_u32 where = vunit + (ch >> 5) * 8192 + r * 128 + ((((ch & 31) >> 2) ^ (r & 7)) << 4) + (ch & 3) * 4;
-                                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[e]) : "r"(where) : "memory");
-                            }
+                            for (int e = 0; e < 4; ++e)
+                                asm volatile("ld.shared.u32 %0, [%1];"
+                                             : "=r"(v[e]) : "r"(vunit + v_at[a][e] + (2 * k2 + k) * 1024) : "memory");
                             if (valid < 64) { // what lies past the end may be anything
 #pragma unroll
                                 for (int e = 0; e < 4; ++e)
