@@ -217,6 +217,21 @@ static __device__ __forceinline__ int pb_page(const pb_at& a, const int* tables,
     return lane * PB_BOX < 64 && first < a.length ? tables[(pb_i64)a.s * width + first / PB_PS] : 0;
 }
 
+// A row's queries, PB_Q_EACH values of each of 128 threads, every load before
+// the first use; zero past its heads and the head size.
+#define PB_Q_HEAD (PB_STEPS * 32 / PB_ESZ)
+#define PB_Q_EACH ((PB_HT * PB_Q_HEAD + 127) / 128)
+struct pb_queries { float x[PB_Q_EACH]; };
+static __device__ __forceinline__ void pb_load_queries(pb_queries& r, const float* q, const pb_at& a, pb_i64 q_seq,
+                                                       pb_i64 q_head, int group) {
+    const int heads = min(PB_HT, group - a.chunk * PB_HT), first = a.h * group + a.chunk * PB_HT;
+#pragma unroll
+    for (int j = 0; j < PB_Q_EACH; ++j) {
+        const int e = threadIdx.x + 128 * j, head = e / PB_Q_HEAD, d = e % PB_Q_HEAD;
+        r.x[j] = head < heads && d < PB_D ? __ldg(q + a.s * q_seq + (first + head) * q_head + d) : 0.0f;
+    }
+}
+
 extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
     const __grid_constant__ pb_tmap map_k, const __grid_constant__ pb_tmap map_v, const float* q, const int* lengths,
     const int* tables, const int4* work, float* out, float* partial, float2* partial_ml, float* logits, float* lse,
@@ -322,25 +337,29 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
             v_at[a][e] = (ch >> 5) * 8192 + r * 128 + ((((ch & 31) >> 2) ^ r) << 4) + (ch & 3) * 4;
         }
 #endif
+    // The next tile is looked up, and the next row's queries are loaded, a tile
+    // ahead, so that neither is waited for (queries only where they take few
+    // registers).
+    pb_at next = at;
+    bool next_fresh = false;
+    pb_queries ahead;
+    pb_load_queries(ahead, q, at, q_seq, q_head, group);
     for (int i = 0; i < mine.z; ++i) {
-        if (i) fresh = pb_next(at, lengths, chunks);
+        if (i) {
+            at = next;
+            fresh = next_fresh;
+        }
+        if (i + 1 < mine.z) next_fresh = pb_next(next, lengths, chunks);
         const int hg = min(PB_HT, group - at.chunk * PB_HT);             // query heads of this row
         const int head0 = at.h * group + at.chunk * PB_HT;                // the first
         if (fresh) {
             begun_at_zero = at.tile == 0;
             // The row's queries, split into terms; zero past the head size.
-            // Every load before the first use.
-            constexpr int per_head = PB_STEPS * 32 / PB_ESZ, each = (PB_HT * per_head + 127) / 128;
-            float x[each];
+            if (PB_Q_EACH > 8 && i) pb_load_queries(ahead, q, at, q_seq, q_head, group);
 #pragma unroll
-            for (int j = 0; j < each; ++j) {
-                const int e = threadIdx.x + 128 * j, head = e / per_head, d = e % per_head;
-                x[j] = head < hg && d < PB_D ? __ldg(q + at.s * q_seq + (head0 + head) * q_head + d) : 0.0f;
-            }
-#pragma unroll
-            for (int j = 0; j < each; ++j) {
-                const int e = threadIdx.x + 128 * j, head = e / per_head, d = e % per_head;
-                if (e < PB_HT * per_head) pb_split_store(qs + head * PB_QROW + d * PB_ESZ, PB_HT * PB_QROW, x[j]);
+            for (int j = 0; j < PB_Q_EACH; ++j) {
+                const int e = threadIdx.x + 128 * j, head = e / PB_Q_HEAD, d = e % PB_Q_HEAD;
+                if (e < PB_HT * PB_Q_HEAD) pb_split_store(qs + head * PB_QROW + d * PB_ESZ, PB_HT * PB_QROW, ahead.x[j]);
             }
 #pragma unroll
             for (int n = 0; n < PB_NT; ++n)
@@ -354,6 +373,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                     for (int e = 0; e < 4; ++e) o[a][n][e] = 0.0f;
             if (pb_bar_any(bad)) { bad = true; break; }
         }
+        if (PB_Q_EACH <= 8 && i + 1 < mine.z && next_fresh) pb_load_queries(ahead, q, next, q_seq, q_head, group);
         const int base = at.tile * 64, valid = min(64, at.length - base);
 
         // ---- S^T = K Q^T: this warp's 16 slots x all heads
