@@ -580,6 +580,10 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
         if (lane == 0) pb_mbar_arrive(empty + 8 * slot);
         if (++slot == PB_RING) { slot = 0; parity ^= 1u; }
 
+        // Only here: joining blocks that come in earlier, or an attention that
+        // comes in beside them, take the room of CTAs that are still to run
+        // (48 sequences up to 8191 slots: 128 us so, 168 with the launch at
+        // every kernel's start).
         if (i + 1 == mine.z) asm volatile("griddepcontrol.launch_dependents;");
         // ---- the row ends, or this CTA's part of it
         const bool row_ends = at.tile + 1 == at.tiles;
