@@ -718,13 +718,13 @@ static __device__ __forceinline__ void pb_join(const int4* joins, const float* p
 // a split row's lse comes from its parts, so that scores need not wait for the
 // join. Block: 4 * PB_JOIN_THREADS slots of one sequence and key head, the
 // log-sums of up to 64 query heads at a time in shared memory.
-static __device__ __forceinline__ void pb_load_logits(float (&x)[4][4], const float* l, int heads, pb_i64 i0, int length,
+static __device__ __forceinline__ void pb_load_logits(float (&x)[4][4], const float* l, int heads, int i0, int length,
                                                       pb_i64 longest) {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const pb_i64 i = i0 + j * PB_JOIN_THREADS;
+            const int i = i0 + j * PB_JOIN_THREADS;
             x[e][j] = e < heads && i < length ? l[e * longest + i] : 0.0f;
         }
 }
@@ -735,15 +735,17 @@ static __device__ __forceinline__ void pb_scores(const int4* joins, const int* s
     __shared__ float sums[64];
     const pb_u32 blocks = (pb_u32)((longest + 4 * PB_JOIN_THREADS - 1) / (4 * PB_JOIN_THREADS));
     const pb_i64 row = block / blocks; // sequence and key head
-    const pb_i64 i0 = (pb_i64)(block % blocks) * (4 * PB_JOIN_THREADS) + threadIdx.x;
+    const int i0 = (int)(block % blocks) * (4 * PB_JOIN_THREADS) + threadIdx.x; // lengths are below 2^30
     const int length = lengths[row / PB_H];
+    const float* before = scores + row * ns;
     float a[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const pb_i64 i = i0 + j * PB_JOIN_THREADS;
-        a[j] = i < length && i < ns ? scores[row * ns + i] : 0.0f;
+        const int i = i0 + j * PB_JOIN_THREADS;
+        a[j] = i < length && i < ns ? before[i] : 0.0f;
     }
-    for (int from = 0; from < group; from += 64) {
+    // Blocks past the length only write zeros.
+    for (int from = 0; from < group && (int)(block % blocks) * (4 * PB_JOIN_THREADS) < length; from += 64) {
         const int n = min(64, group - from);
         // The first heads' logits are on their way while the log-sums are formed.
         float x[4][4];
@@ -784,10 +786,11 @@ static __device__ __forceinline__ void pb_scores(const int4* joins, const int* s
                         if (i0 + j * PB_JOIN_THREADS < length) a[j] += pb_exp2(x[e][j] - sums[g + e]);
         }
     }
+    float* to = out + row * longest;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const pb_i64 i = i0 + j * PB_JOIN_THREADS;
-        if (i < longest) out[row * longest + i] = a[j];
+        const int i = i0 + j * PB_JOIN_THREADS;
+        if (i < longest) to[i] = a[j];
     }
 }
 #endif

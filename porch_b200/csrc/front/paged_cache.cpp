@@ -176,13 +176,10 @@ static __device__ __forceinline__ void pb_pick(const int* bins, int want, int* c
 
 // Up to PB_MOVES pairs of one row: late slot and free place, one a lane.
 struct pb_pairs { int from, to, count; };
-static __device__ __forceinline__ pb_pairs pb_list(const int* holes, const int* lates, const int* counts, pb_i64 id,
-                                                   pb_i64 last, int groups, int pairs) {
+static __device__ __forceinline__ pb_pairs pb_list(const int* holes, const int* lates, const int* counts, pb_i64 row,
+                                                   int group, int pairs) {
     pb_pairs p = {0, 0, 0};
-    if (id >= last) return p;
-    const int lane = threadIdx.x & 31;
-    const pb_i64 row = id / groups;
-    const int j = (int)(id - row * groups) * PB_MOVES;
+    const int lane = threadIdx.x & 31, j = group * PB_MOVES;
     if (lane < PB_MOVES && j + lane < pairs) { // read beside the count; what lies past it is not used
         p.from = lates[row * pairs + j + lane];
         p.to = holes[row * pairs + j + lane];
@@ -199,31 +196,35 @@ static __device__ __forceinline__ void pb_move(const pb_pairs& p, const pb_row& 
                                                float* out_scores, float* out_places, pb_i64 row, int width, int budget) {
     const int lane = threadIdx.x & 31, h = (int)(row % PB_H);
     const int* table = tables + row / PB_H * width;
+    // Lane m finds where pair m's rows lie; all lanes move them.
+    pb_i64 from = 0, to = 0;
+    if (lane < p.count) {
+        from = (((pb_i64)__ldg(table + p.from / PB_PS) * PB_H + h) * PB_PS + p.from % PB_PS) * PB_ROW;
+        to = (((pb_i64)__ldg(table + p.to / PB_PS) * PB_H + h) * PB_PS + p.to % PB_PS) * PB_ROW;
+    }
     // 16 bytes a lane: chunk c of the 2 * PB_ROW bytes of a slot, keys first.
     uint4 v[PB_MOVES][PB_CHUNKS];
-    pb_i64 to_row[PB_MOVES];
 #pragma unroll
     for (int m = 0; m < PB_MOVES; ++m) {
-        const int f = __shfl_sync(0xffffffffu, p.from, m), t = __shfl_sync(0xffffffffu, p.to, m);
-        const pb_i64 a = (((pb_i64)__ldg(table + f / PB_PS) * PB_H + h) * PB_PS + f % PB_PS) * PB_ROW;
-        to_row[m] = (((pb_i64)__ldg(table + t / PB_PS) * PB_H + h) * PB_PS + t % PB_PS) * PB_ROW;
+        const pb_i64 a = __shfl_sync(0xffffffffu, from, m);
 #pragma unroll
         for (int c = 0; c < PB_CHUNKS; ++c) {
             const int at = (c * 32 + lane) * 16;
             if (m < p.count && at < 2 * PB_ROW)
-                v[m][c] = __ldcs(reinterpret_cast<const uint4*>(at < PB_ROW ? pk + a + at : pv + a + at - PB_ROW));
+                v[m][c] = __ldcs(reinterpret_cast<const uint4*>((at < PB_ROW ? pk + at : pv + at - PB_ROW) + a));
         }
     }
     if (lane < p.count) pb_keep(r, out_scores, out_places, row * budget + p.to, p.from);
 #pragma unroll
-    for (int m = 0; m < PB_MOVES; ++m)
+    for (int m = 0; m < PB_MOVES; ++m) {
+        const pb_i64 b = __shfl_sync(0xffffffffu, to, m);
 #pragma unroll
         for (int c = 0; c < PB_CHUNKS; ++c) {
             const int at = (c * 32 + lane) * 16;
-            const pb_i64 b = to_row[m];
             if (m < p.count && at < 2 * PB_ROW)
-                __stcs(reinterpret_cast<uint4*>(at < PB_ROW ? pk + b + at : pv + b + at - PB_ROW), v[m][c]);
+                __stcs(reinterpret_cast<uint4*>((at < PB_ROW ? pk + at : pv + at - PB_ROW) + b), v[m][c]);
         }
+    }
 }
 
 #ifdef PB_CLUSTER
@@ -412,7 +413,7 @@ extern "C" __global__ void __launch_bounds__(PB_THREADS, PB_THREADS < 1024 ? 2 :
     if (fused) {
         const int groups = (pairs + PB_MOVES - 1) / PB_MOVES;
         for (int g = rank * (threads / 32) + (threadIdx.x >> 5); g < groups; g += PB_CLUSTER * (threads / 32)) {
-            const pb_pairs p = pb_list(holes, lates, counts, row * groups + g, (row + 1) * groups, groups, pairs);
+            const pb_pairs p = pb_list(holes, lates, counts, row, g, pairs);
             if (p.count <= 0) break;
             pb_move(p, r, pk, pv, tables, out_scores, out_places, row, width, budget);
         }
@@ -486,11 +487,11 @@ extern "C" __global__ void __launch_bounds__(1024) pb_evict_select_long(
 extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
     char* pk, char* pv, const int* tables, const float* scores, const float* places, const int* lengths,
     const int* newest, float* out_scores, float* out_places, const int* holes, const int* lates, const int* counts,
-    pb_i64 ns, pb_i64 np, pb_i64 rows, int width, int budget, int pairs) {
+    pb_i64 ns, pb_i64 np, int width, int budget, int pairs, pb_u32 blocks) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int groups = (pairs + PB_MOVES - 1) / PB_MOVES;
-    const pb_i64 id = (pb_i64)blockIdx.x * 8 + (threadIdx.x >> 5), row = id / groups;
-    const pb_pairs p = pb_list(holes, lates, counts, id, rows * groups, groups, pairs);
+    // Blocks of 8 warps, `blocks` of them for each row.
+    const pb_i64 row = blockIdx.x / blocks;
+    const pb_pairs p = pb_list(holes, lates, counts, row, (blockIdx.x % blocks) * 8 + (threadIdx.x >> 5), pairs);
     if (p.count <= 0) return;
     const pb_row r = pb_row_of(scores, places, lengths, newest, ns, np, 0, 0, row);
     pb_move(p, r, pk, pv, tables, out_scores, out_places, row, width, budget);
@@ -755,12 +756,12 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
             op_launch(kernel_of(kSelectLong, c), device, stream, {static_cast<uint32_t>(rows), 1, 1}, 1024, sparams);
         }
         if (moves && !fused) {
-            const int64_t groups = (pairs + moves_of(c) - 1) / moves_of(c);
-            const int64_t blocks = (rows * groups + 7) / 8;
+            uint32_t per_row = static_cast<uint32_t>((pairs + 8 * moves_of(c) - 1) / (8 * moves_of(c)));
+            const int64_t blocks = rows * per_row;
             expect(blocks <= 0x7fffffff, "cache_evict: too many rows");
             void* mparams[] = {&pk,     &pv,    &batch.tables_at, &xs.ptr, &xp.ptr, &batch.lengths_at, &batch.newest_at,
                                &os.ptr, &op.ptr, &holes,          &lates,  &counts, &nsv,              &npv,
-                               &rows,   &width, &b,               &pairs};
+                               &width, &b,      &pairs,           &per_row};
             op_launch(kernel_of(kMove, c), device, stream, {static_cast<uint32_t>(blocks), 1, 1}, 256, mparams);
         }
         return {finish(std::move(os)), finish(std::move(op))};
