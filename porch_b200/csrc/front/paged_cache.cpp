@@ -530,8 +530,8 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
         constexpr int kFewPairs = 128;
 
         // Pairs that a warp moves: 2 KB on the way, more where one pair is larger.
-        // (8 KB at half the occupancy took 31 us where 2 KB take 27, for 64 MB
-        // of pairs; a persistent form that reads its lists ahead took 41.)
+        // 64 MB of pairs take 24.8 us with 1 KB, 22.7 with 2 and 22.0 with 4,
+        // which costs the select, where it moves few pairs itself, its registers.
         int moves_of(const kv_cache& c) { return std::max<int>(1, 4 / static_cast<int>((2 * c.dim * c.width() + 511) / 512)); }
 
         std::string defines(const kv_cache& c, bool wide, const select_shape& f = {}) {
