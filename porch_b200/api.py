@@ -362,7 +362,9 @@ def tensor_from_pointer(shape: Sequence[int], pointer: int, count: int, device: 
 
 def tensor_from_device(array, device: int = 0) -> Tensor:
     """A tensor with a copy of a contiguous float32 array of another library
-    on the same GPU (anything with __cuda_array_interface__)."""
+    on the same GPU (anything with __cuda_array_interface__). The copy is
+    ordered behind the stream that the interface names, or the legacy default
+    stream; an array that another stream writes needs a synchronize first."""
     face = array.__cuda_array_interface__
     shape = face["shape"]
     if face["typestr"] != "<f4":
