@@ -836,13 +836,15 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             });
         }
 
-        // Even runs of 64-slot tiles, over all rows one after the other: the
-        // CTAs' shares differ by one tile at most, whatever the lengths. A run
-        // begins and ends inside a row at most once each, so a CTA leaves at
-        // most two parts behind. Where every row is short and they all fit,
-        // each has a CTA of its own instead: up to kWholeRow tiles in a row
-        // take less time than the second launch that joins parts. A row
-        // without slots has a CTA that writes its zeros, after the others.
+        // Even runs of 64-slot tiles, over all rows one after the other, where a
+        // row counts as one tile more than it has, for its queries, its sums
+        // and its result (32 sequences of 8 rows up to 4096 slots of 80 channels:
+        // 39.4 us with tiles alone, 36.4 so). A run begins and ends inside a row at
+        // most once each, so a CTA leaves at most two parts behind. Where every
+        // row is short and they all fit, each has a CTA of its own instead: up
+        // to kWholeRow tiles in a row take less time than the second launch
+        // that joins parts. A row without slots has a CTA that writes its
+        // zeros, after the others.
         struct schedule {
             std::vector<int32_t> work; // per CTA: row, tile, tiles, 0
             std::vector<int32_t> join; // per row in parts: row, first CTA, parts, its place
@@ -861,9 +863,30 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
                 if (tiles != 0) rows += per;
             }
             const bool whole = most <= kWholeRow && rows <= ctas;
-            const int64_t n = whole ? rows : std::min(total, ctas);
+            // The tile, in the order of all rows, that each CTA begins with.
+            std::vector<int64_t> starts;
+            if (!whole) {
+                const int64_t n = std::min(total, ctas);
+                int64_t row_cost = 0, row_tile = 0, cut = 0; // where the row begins
+                for (int64_t length : lengths) {
+                    const int64_t tiles = (length + 63) / 64;
+                    if (tiles == 0) continue;
+                    for (int64_t j = 0; j < per; ++j) {
+                        for (; cut < n; ++cut) {
+                            const int64_t at = static_cast<int64_t>(static_cast<__int128>(total + rows) * cut / n) - row_cost;
+                            if (at > tiles) break;
+                            const int64_t tile = row_tile + std::max<int64_t>(0, at - 1);
+                            if (starts.empty() || starts.back() != tile) starts.push_back(tile);
+                        }
+                        row_cost += tiles + 1;
+                        row_tile += tiles;
+                    }
+                }
+                starts.push_back(total);
+            }
+            const int64_t n = whole ? rows : static_cast<int64_t>(starts.size()) - 1;
             int64_t cta = 0, from = 0; // `from`: the row's first tile in the whole order
-            auto start = [&](int64_t c) { return n == 0 ? 0 : static_cast<int64_t>(static_cast<__int128>(total) * c / n); };
+            auto start = [&](int64_t c) { return starts[static_cast<size_t>(c)]; };
             auto put = [](std::vector<int32_t>& to, std::initializer_list<int64_t> values) {
                 for (int64_t v : values) to.push_back(static_cast<int32_t>(v));
             };
