@@ -4,6 +4,37 @@
 // scored form, which adds each slot's attention weight, summed over the query
 // heads of its key head, to running scores (what eviction ranks slots by).
 // A sequence without slots gives zeros.
+//
+// Bound: HBM, which has to deliver every key and value in use once (2 x slots
+// x kv_heads x head_dim x 2 or 4 bytes). 48 sequences up to 8191 slots, 32
+// query heads over 8 of 128 bfloat16 channels: 784 MB in 126 us = 6.20 TB/s;
+// one sequence of 262147 slots: 1074 MB in 165 us = 6.5 TB/s, what a copy
+// reaches. Few or short rows are bound by the launch and the first loads'
+// latency instead (about 6 us).
+//
+// pb_paged_attention, 160 threads: a producer warp loads tiles of 64 slots, K
+// then V, through a ring of TMA boxes (a page, or 64 rows of a larger one; 128
+// bytes wide, swizzled, zeros past the head size), and four computing warps
+// keep an online softmax over them: S^T = K Q^T for 16 slots each, a maximum
+// over the tile, weights to shared memory, O^T += V^T P^T for a quarter of the
+// channels each. The transposed products put slots and channels on the tensor
+// core's 16 rows and query heads on its 8 columns, so 1 to 8 heads cost the
+// same. One query per sequence leaves nothing for the 128-row tiles of
+// tcgen05; with mma.sync the tensor pipe is 31 % busy at full bandwidth.
+//
+// Accuracy: float32. Queries and weights are split into three bfloat16 terms
+// (24 bits) against a bfloat16 cache, whose products are then exact; a float32
+// cache is split into two tf32 terms like the queries (3 products of 4, error
+// 2^-21). The tensor core's accumulator cuts low bits at every addition, so a
+// tile's products start from zero and are added to the running sums in fp32,
+// rounded to nearest.
+//
+// Work is shared out in even runs of tiles over all rows, one wave of CTAs
+// (more waves, which would even out CTAs of different speed, took 1 to 5 %
+// longer), and rows that span CTAs are joined from their parts in order, so
+// results depend on the lengths and the number of SMs alone. Joining in the
+// CTA that finishes a row's last part instead of a second launch took 2 to 13
+// us longer: its fences and loads come at the very end.
 #include "operators.hpp"
 
 #include <algorithm>
