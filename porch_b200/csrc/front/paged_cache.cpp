@@ -514,11 +514,12 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
         select_shape shape_for(int64_t longest, int64_t rows, int sms) {
             static constexpr int kShapes[][2] = {{256, 4}, {256, 8}, {512, 8}, {512, 16}, {1024, 16}, {1024, 32}, {1024, 48}};
             select_shape r;
-            // More CTAs for each row as long as all of them fit the GPU at
-            // once, two of an SM, and each has a few thousand slots; more
-            // still where the keys need the room.
+            // More CTAs for each row as long as every CTA has an SM of its own and
+            // a few thousand slots (32 rows of 65533 slots: 22.4 us with 4 CTAs of
+            // 1024 threads each, 23.5 with 8 of 512, two of an SM, 31.9 with 2);
+            // more still where the keys need the room.
             int64_t c = 1;
-            while (c < 8 && rows * c * 2 <= 2 * sms && longest >= 4096 * c) c *= 2;
+            while (c < 8 && rows * c * 2 <= sms && longest >= 4096 * c) c *= 2;
             for (; c <= 8; c *= 2)
                 for (const auto& [threads, per_thread] : kShapes)
                     if (int64_t{threads} * per_thread * c >= longest) {
