@@ -334,7 +334,8 @@ int pb_kv_plan_describe(const int64_t* lengths, size_t sequences, int64_t kv_hea
                         size_t* needed);
 /* The same, and new scores [sequences, kv_heads, longest length]: `scores`
  * (NULL or slots past its end: 0) plus each slot's attention weight summed
- * over the query heads of its key head; 0 past a sequence's length. */
+ * over the query heads of its key head; 0 past a sequence's length. Takes 4
+ * bytes of workspace per query head and slot. */
 int pb_paged_attention_scored(const pb_tensor* q, pb_kv_batch* batch, const pb_tensor* scores,
                               float scale, pb_tensor** out, pb_tensor** new_scores);
 /* Keeps, per sequence and key head, `budget` slots: the newest `recent`

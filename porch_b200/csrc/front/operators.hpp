@@ -124,7 +124,8 @@ namespace porch::detail {
     struct batch_plan {
         int64_t chunks = 1; // query heads of a key head come in this many rows
         int64_t limit = 0;  // CTAs asked for
-        int64_t ctas = 0, joins = 0, most_parts = 0;
+        int64_t ctas = 0, working = 0; // working: those that have tiles; the others clear empty rows
+        int64_t joins = 0, most_parts = 0;
         cuda_jit::device_buffer data; // 16 bytes per CTA, then 16 per row to join
     };
     struct batch_plans {

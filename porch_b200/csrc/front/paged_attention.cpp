@@ -265,7 +265,7 @@ static __device__ __forceinline__ void pb_load_queries(pb_queries& r, const floa
 
 extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
     const __grid_constant__ pb_tmap map_k, const __grid_constant__ pb_tmap map_v, const float* q, const int* lengths,
-    const int* tables, const int4* work, float* out, float* partial, float2* partial_ml, float* logits, float* lse,
+    const int* tables, const int4* work, float* out, float* partial, float2* partial_ml, float* logits, float2* norms,
     int width, int group, int chunks, pb_i64 q_seq, pb_i64 q_head, int longest, float scale2, int* err) {
     extern __shared__ char raw[];
     __shared__ pb_u64 bars[2 * PB_RING];
@@ -655,7 +655,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                     if (warp == 0 && g == 0) {
                         if (!whole) partial_ml[part * PB_HT + head] = make_float2(m[n][e], sum);
 #if PB_SCORED
-                        else lse[global] = m[n][e] + log2f(sum);
+                        else norms[global] = make_float2(m[n][e], 1.0f / sum);
 #endif
                     }
                 }
@@ -671,9 +671,10 @@ static __device__ __forceinline__ pb_i64 pb_part(const int4& r, int i, int head)
     return (pb_i64)(2 * (r.y + i) + (i ? 0 : r.w)) * PB_HT + head;
 }
 
-// Joins the parts of a row that several CTAs worked on. Block: one query head of one such row; its threads read
-// the parts' sums at once, then each group of D / 4 threads takes every
-// PB_JOIN-th part, four channels a thread. Latency: two rounds of loads.
+// Joins the parts of a row that several CTAs worked on. Block: one query head
+// of one such row; its threads read the parts' sums at once, then each group of
+// D / 4 threads takes every PB_JOIN-th part, four channels a thread. Latency:
+// two rounds of loads.
 #define PB_JOIN (PB_JOIN_THREADS / (PB_D / 4))
 static __device__ __forceinline__ void pb_join(const int4* joins, const float* partial, const float2* partial_ml,
                                                float* out, int group, int chunks, int block) {
@@ -745,10 +746,10 @@ static __device__ __forceinline__ void pb_join(const int4* joins, const float* p
 }
 
 #if PB_SCORED
-// new[s, h, i] = scores[s, h, i] + sum over the group of 2^(logit - lse), where
-// a split row's lse comes from its parts, so that scores need not wait for the
-// join. Block: 4 * PB_JOIN_THREADS slots of one sequence and key head, the
-// log-sums of up to 64 query heads at a time in shared memory.
+// new[s, h, i] = scores[s, h, i] + sum over the group of 2^(logit - top) / sum,
+// where a split row's top and sum come from its parts, so that scores need not
+// wait for the join. Block: 4 * PB_JOIN_THREADS slots of one sequence and key
+// head, the norms of up to 64 query heads at a time in shared memory.
 static __device__ __forceinline__ void pb_load_logits(float (&x)[4][4], const float* l, int heads, int i0, int length,
                                                       pb_i64 longest) {
 #pragma unroll
@@ -760,10 +761,10 @@ static __device__ __forceinline__ void pb_load_logits(float (&x)[4][4], const fl
         }
 }
 static __device__ __forceinline__ void pb_scores(const int4* joins, const int* split, const float2* partial_ml,
-                                                 const float* logits, const float* lse, const int* lengths,
+                                                 const float* logits, const float2* norms, const int* lengths,
                                                  const float* scores, float* out, pb_i64 longest, pb_i64 ns, int group,
                                                  int chunks, pb_u32 block) {
-    __shared__ float sums[64];
+    __shared__ float2 shared_norms[64];
     const pb_u32 blocks = (pb_u32)((longest + 4 * PB_JOIN_THREADS - 1) / (4 * PB_JOIN_THREADS));
     const pb_i64 row = block / blocks; // sequence and key head
     const int i0 = (int)(block % blocks) * (4 * PB_JOIN_THREADS) + threadIdx.x; // lengths are below 2^30
@@ -778,7 +779,7 @@ static __device__ __forceinline__ void pb_scores(const int4* joins, const int* s
     // Blocks past the length only write zeros.
     for (int from = 0; from < group && (int)(block % blocks) * (4 * PB_JOIN_THREADS) < length; from += 64) {
         const int n = min(64, group - from);
-        // The first heads' logits are on their way while the log-sums are formed.
+        // The first heads' logits are on their way while the norms are formed.
         float x[4][4];
         const float* l = logits + (row * group + from) * longest;
         pb_load_logits(x, l, n, i0, length, longest);
@@ -787,8 +788,9 @@ static __device__ __forceinline__ void pb_scores(const int4* joins, const int* s
             const int lane = threadIdx.x & 31, g = from + e, at = split[row * chunks + g / PB_HT];
             float top = __int_as_float(0xff800000), sum = 0.0f;
             if (at < 0) {
-                top = lse[row * group + g];
-                sum = lane ? 0.0f : 1.0f;
+                const float2 v = norms[row * group + g];
+                top = v.x;
+                sum = lane ? 0.0f : 1.0f / v.y;
             } else {
                 const int4 r = joins[at];
                 for (int i = lane; i < r.z; i += 32) {
@@ -804,7 +806,7 @@ static __device__ __forceinline__ void pb_scores(const int4* joins, const int* s
             sum = sum != 0.0f ? sum * pb_exp2(top - all) : 0.0f; // lanes without a part have no maximum
 #pragma unroll
             for (int m = 16; m > 0; m /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-            if (lane == 0) sums[e] = all + log2f(sum);
+            if (lane == 0) shared_norms[e] = make_float2(all, 1.0f / sum);
         }
         __syncthreads();
         for (int g = 0; g < n; g += 4) {
@@ -814,7 +816,7 @@ static __device__ __forceinline__ void pb_scores(const int4* joins, const int* s
                 if (g + e < n)
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
-                        if (i0 + j * PB_JOIN_THREADS < length) a[j] += pb_exp2(x[e][j] - sums[g + e]);
+                        if (i0 + j * PB_JOIN_THREADS < length) a[j] = fmaf(pb_exp2(x[e][j] - shared_norms[g + e].x), shared_norms[g + e].y, a[j]);
         }
     }
     float* to = out + row * longest;
@@ -829,7 +831,7 @@ static __device__ __forceinline__ void pb_scores(const int4* joins, const int* s
 // The first `join_blocks` blocks join, the others score.
 extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
     const int4* joins, const int* split, const float* partial, const float2* partial_ml, float* out,
-    const float* logits, const float* lse, const int* lengths, const float* scores, float* new_scores, pb_i64 longest,
+    const float* logits, const float2* norms, const int* lengths, const float* scores, float* new_scores, pb_i64 longest,
     pb_i64 ns, int group, int chunks, int join_blocks) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (blockIdx.x < join_blocks) {
@@ -837,7 +839,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         return;
     }
 #if PB_SCORED
-    pb_scores(joins, split, partial_ml, logits, lse, lengths, scores, new_scores, longest, ns, group, chunks,
+    pb_scores(joins, split, partial_ml, logits, norms, lengths, scores, new_scores, longest, ns, group, chunks,
               blockIdx.x - join_blocks);
 #endif
 }
@@ -848,7 +850,8 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             std::ostringstream os;
             os << "#define PB_H " << f.heads << "\n#define PB_D " << f.dim << "\n#define PB_PS " << f.page
                << "\n#define PB_ESZ " << f.width() << "\n#define PB_NT " << f.tiles8 << "\n#define PB_RING " << f.ring()
-               << "\n#define PB_JOIN_THREADS " << f.join_threads << "\n#define PB_PER_SM " << f.per_sm() << "\n#define PB_SCORED " << (f.scored ? 1 : 0) << "\n";
+               << "\n#define PB_JOIN_THREADS " << f.join_threads << "\n#define PB_PER_SM " << f.per_sm()
+               << "\n#define PB_SCORED " << (f.scored ? 1 : 0) << "\n";
             if (f.stall) os << "#define PB_TEST_STALL 1\n";
             return os.str();
         }
@@ -1006,19 +1009,21 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
 
         int64_t longest = batch.longest;
         int width = static_cast<int>(batch.table_width), longest32 = static_cast<int>(longest);
-        // Workspace: the parts of split rows, and for scores the logits and
-        // each head's log-sum.
-        const size_t part_heads = static_cast<size_t>(plan.ctas) * 2 * static_cast<size_t>(8 * f.tiles8);
-        const size_t parts = part_heads * static_cast<size_t>(c.dim), sums = scored ? static_cast<size_t>(n * heads) : 0;
-        const size_t all = parts + 2 * part_heads + sums + (scored ? static_cast<size_t>(n * heads * longest) : 0);
-        auto scratch = allocate(device, std::max<size_t>(1, all) * sizeof(float), stream);
-        uint64_t ml = address(scratch), partial = ml + 2 * part_heads * 4, lse = partial + parts * 4, logits = lse + sums * 4;
+        // Workspace: sums and results of split rows' parts, and for scores the
+        // logits and each head's maximum and sum.
+        const size_t part_heads = plan.joins == 0 ? 0 : static_cast<size_t>(plan.working) * 2 * static_cast<size_t>(8 * f.tiles8);
+        const size_t parts = part_heads * static_cast<size_t>(c.dim), scored_heads = scored ? static_cast<size_t>(n * heads) : 0;
+        const size_t all = parts + 2 * part_heads + (2 + static_cast<size_t>(longest)) * scored_heads;
+        cuda_jit::device_buffer scratch;
+        if (all != 0) scratch = allocate(device, all * sizeof(float), stream);
+        uint64_t ml = address(scratch), partial = ml + 2 * part_heads * 4, norms = partial + parts * 4,
+                 logits = norms + 2 * scored_heads * 4;
         uint64_t work = address(plan.data), join = work + static_cast<uint64_t>(plan.ctas) * 16, err = 0;
         if (plan.ctas > 0) {
             check(pbrt_error_word(device, &err));
             float scale2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
             void* params[] = {&c.map_k, &c.map_v, &x.ptr, &batch.lengths_at, &batch.tables_at, &work,
-                              &out.ptr, &partial, &ml, &logits, &lse, &width, &group, &chunks,
+                              &out.ptr, &partial, &ml, &logits, &norms, &width, &group, &chunks,
                               &x.strides[0], &x.strides[1], &longest32, &scale2, &err};
             op_launch(kernel_of(kAttention, f, static_cast<uint32_t>(f.smem())), device, stream,
                       {static_cast<uint32_t>(plan.ctas), 1, 1}, 160, params);
@@ -1039,7 +1044,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         expect(blocks <= 0x7fffffff, "paged_attention: too many sequences, heads and slots");
         if (blocks > 0) {
             uint64_t split = join + static_cast<uint64_t>(plan.joins) * 16;
-            void* params[] = {&join,   &split,   &partial, &ml,  &results_ptr, &logits, &lse,        &batch.lengths_at,
+            void* params[] = {&join,   &split,   &partial, &ml,  &results_ptr, &logits, &norms,      &batch.lengths_at,
                               &xs.ptr, &os.ptr,  &longest, &ns,  &group,       &chunks, &join_blocks};
             op_launch(kernel_of(kFinish, f, 0), device, stream, {static_cast<uint32_t>(blocks), 1, 1},
                       static_cast<uint32_t>(f.join_threads), params);
@@ -1067,6 +1072,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         p->chunks = chunks;
         p->limit = ctas;
         p->ctas = static_cast<int64_t>(s.work.size() / 4);
+        for (size_t i = 2; i < s.work.size(); i += 4) p->working += s.work[i] != 0;
         p->joins = static_cast<int64_t>(s.join.size() / 4);
         for (size_t i = 2; i < s.join.size(); i += 4) p->most_parts = std::max<int64_t>(p->most_parts, s.join[i]);
         s.work.insert(s.work.end(), s.join.begin(), s.join.end());
