@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p
 from pathlib import Path
 
@@ -33,6 +34,19 @@ def lib() -> ctypes.CDLL:
         _declare(L)
         _lib = L
     return _lib
+
+
+def binding():
+    """The compiled part of the binding (porch_b200/csrc/python/binding.cpp),
+    behind the library that it calls."""
+    lib()
+    path = LIBRARY.parent / "_binding.so"
+    if not path.exists():
+        raise ImportError(f"{path} is not built; run `python -m porch_b200.build`")
+    spec = importlib.util.spec_from_file_location("porch_b200._binding", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
 
 
 def _declare(L: ctypes.CDLL) -> None:

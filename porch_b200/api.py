@@ -23,7 +23,9 @@ from typing import Iterable, Sequence
 
 import numpy as np
 
-from ._lib import lib, pb_index
+from ._lib import binding, lib, pb_index
+
+_binding = binding()
 
 PB_ADD, PB_SUBTRACT, PB_MULTIPLY, PB_DIVIDE, PB_MAXIMUM, PB_MINIMUM, PB_MATMUL = range(7)
 PB_EXP, PB_RECIPROCAL, PB_TRANSPOSE, PB_RELU, PB_LOGISTIC, PB_SUM, PB_MAX = range(7, 14)
@@ -192,26 +194,10 @@ def _unary(op: int, a) -> Expr:
     return Expr(out.value)
 
 
-_Numbers = c_int64 * 19
-
-
-class Tensor:
+class Tensor(_binding.Handle):
     """porch::tensor (a shared handle)."""
 
-    __slots__ = ("_h", "_face")
-
-    def __init__(self, handle: int):
-        self._h = c_void_p(handle)
-        self._face = None
-
-    def __del__(self):
-        h = getattr(self, "_h", None)
-        if h is not None and h.value:
-            try:
-                lib().pb_tensor_release(h)
-                self._h = c_void_p(None)
-            except Exception:
-                pass
+    __slots__ = ()
 
     # -- metadata
     def shape(self) -> list[int]:
@@ -276,20 +262,6 @@ class Tensor:
         b = c_size_t(0)
         _check(lib().pb_tensor_device_pointer(self._h, byref(p), byref(b)))
         return p.value, b.value
-
-    @property
-    def __cuda_array_interface__(self) -> dict:
-        """The values in place, for another library on the same GPU (as
-        device_data(): a raw handle, so a consumer that does not order its
-        work behind `stream` calls synchronize() first)."""
-        if self._face is None:
-            # The address of a realised tensor's values stays what it is once
-            # it was handed out, so consumers that ask twice cost one call.
-            out = _Numbers()
-            _check(lib().pb_tensor_interface(self._h, out, 19))
-            self._face = {"shape": tuple(out[3:3 + out[0]]), "typestr": "<f4", "data": (out[1], False), "version": 3,
-                          "stream": out[2]}
-        return self._face
 
     def __getitem__(self, key) -> Expr:
         if not isinstance(key, tuple):
@@ -414,6 +386,9 @@ def materialize(e) -> Tensor:
 def as_tensor(e) -> Tensor:
     """`porch::tensor t = expr;` (lazy)."""
     return _expr(e).to_tensor()
+
+
+_binding.bind(Tensor, materialize, _check)
 
 
 def add(a, b):
@@ -545,20 +520,14 @@ def qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps: float = 1e-
     per channel, and the rotation of its first 2 * R2 channels by the token's
     position; cos, sin [positions, R2], positions [T] whole numbers. Pairs are
     channels (i, i + R2), or (2i, 2i + 1) when interleaved. An extension."""
-    t = [_realised(x) for x in (q, k, q_weight, k_weight, cos, sin, positions)]
-    oq, ok = c_void_p(), c_void_p()
-    _check(lib().pb_qk_norm_rope(*[x._h for x in t], eps, interleaved, byref(oq), byref(ok)))
-    return Tensor(oq.value), Tensor(ok.value)
+    return _binding.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
 
 
 def qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, cos, sin, positions, eps: float = 1e-6,
                           interleaved: bool = False) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     """Gradients (q, k, q_weight, k_weight) of qk_norm_rope, from those of its
     results and its inputs. An extension."""
-    t = [_realised(x) for x in (dq, dk, q, k, q_weight, k_weight, cos, sin, positions)]
-    out = (c_void_p * 4)()
-    _check(lib().pb_qk_norm_rope_backward(*[x._h for x in t], eps, interleaved, out))
-    return tuple(Tensor(h) for h in out)
+    return _binding.qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
 
 
 class _Pool:
@@ -644,6 +613,7 @@ class Batch:
 
         _check(lib().pb_kv_batch_create(cache._h, at(table, ctypes.c_int32), n, width, at(self.lengths, c_int64),
                                         at(fresh, c_int64), at(last, c_int64), byref(self._h)))
+        self._address = self._h.value
 
     def __del__(self):
         h = getattr(self, "_h", None)
@@ -660,6 +630,7 @@ class Batch:
         other = Batch.__new__(Batch)
         other._h, other.cache, other.lengths = c_void_p(), cache, self.lengths
         _check(lib().pb_kv_batch_on(self._h, cache._h, byref(other._h)))
+        other._address = other._h.value
         return other
 
     def append(self, k, v) -> None:
@@ -685,24 +656,15 @@ def paged_attention(q, batch: Batch, scale: float | None = None) -> Tensor:
     """softmax(scale q K^T) V of one query per sequence, [sequences, q_heads,
     head_dim], over the batch's slots; scale defaults to head_dim ** -0.5. An
     extension."""
-    t = _realised(q)
-    out = c_void_p()
-    _check(lib().pb_paged_attention(t._h, batch._h, batch.cache.head_dim ** -0.5 if scale is None else scale,
-                                    byref(out)))
-    return Tensor(out.value)
+    return _binding.paged_attention(q, batch._address, batch.cache.head_dim ** -0.5 if scale is None else scale)
 
 
 def paged_attention_scored(q, batch: Batch, scores=None, scale: float | None = None) -> tuple[Tensor, Tensor]:
     """paged_attention, and `scores` (None: zeros) plus each slot's attention
     weight summed over the query heads of its key head, [sequences, kv_heads,
     longest]. An extension."""
-    t = _realised(q)
-    s = None if scores is None else _realised(scores)
-    out, new = c_void_p(), c_void_p()
-    _check(lib().pb_paged_attention_scored(t._h, batch._h, None if s is None else s._h,
-                                           batch.cache.head_dim ** -0.5 if scale is None else scale,
-                                           byref(out), byref(new)))
-    return Tensor(out.value), Tensor(new.value)
+    return _binding.paged_attention_scored(q, batch._address, scores,
+                                           batch.cache.head_dim ** -0.5 if scale is None else scale)
 
 
 def cache_evict(batch: Batch, scores, positions=None, *, budget: int, recent: int = 0,
@@ -712,12 +674,7 @@ def cache_evict(batch: Batch, scores, positions=None, *, budget: int, recent: in
     move in place. Returns the kept slots' scores and positions, [sequences,
     kv_heads, budget]; the next batch has lengths min(length, budget) plus its
     new tokens. An extension."""
-    s = _realised(scores)
-    p = None if positions is None else _realised(positions)
-    new_scores, new_positions = c_void_p(), c_void_p()
-    _check(lib().pb_kv_evict(batch._h, s._h, None if p is None else p._h, int(budget), int(recent), int(sinks),
-                             byref(new_scores), byref(new_positions)))
-    return Tensor(new_scores.value), Tensor(new_positions.value)
+    return _binding.kv_evict(batch._address, scores, positions, budget, recent, sinks)
 
 
 def operator_sources() -> str:

@@ -1,7 +1,8 @@
 """Build recipe for the porch_b200 native library.
 
 Compiles every C++ source under porch_b200/csrc with g++ into
-porch_b200/lib/libporch_b200.so. The library reaches CUDA only through
+porch_b200/lib/libporch_b200.so, and the compiled part of the Python binding
+beside it. The library reaches CUDA only through
 dlopen'ed libcuda / libnvrtc / libnccl, so it builds on a machine without a
 GPU; the CUDA toolkit headers (cuda.h, nvrtc.h) and nccl.h are needed for
 their type declarations only.
@@ -23,6 +24,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
@@ -31,6 +33,7 @@ CSRC = PACKAGE / "csrc"
 LIB_DIR = PACKAGE / "lib"
 OBJ_DIR = ROOT / "_build" / "obj"
 LIBRARY = LIB_DIR / "libporch_b200.so"
+BINDING = LIB_DIR / "_binding.so"  # compiled part of the Python binding
 
 CUDA_HOME = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
 # The system g++ links the C++ runtime dynamically; a toolchain wrapper that
@@ -58,7 +61,11 @@ NVCCFLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "
 
 
 def sources() -> list[Path]:
-    return sorted(p for p in CSRC.rglob("*.cpp")) + sorted(p for p in CSRC.rglob("*.cu"))
+    return (sorted(p for p in CSRC.rglob("*.cpp") if p.parent.name != "python")
+            + sorted(p for p in CSRC.rglob("*.cu")))
+
+
+BINDING_SOURCE = CSRC / "python" / "binding.cpp"
 
 
 def headers() -> list[Path]:
@@ -84,6 +91,7 @@ def build(force: bool = False) -> Path:
     srcs = sources()
     newest = max(p.stat().st_mtime for p in srcs + headers() + [Path(__file__)])
     if LIBRARY.exists() and not force and LIBRARY.stat().st_mtime >= newest:
+        _build_binding(force)
         return LIBRARY
     LIB_DIR.mkdir(parents=True, exist_ok=True)
     with concurrent.futures.ThreadPoolExecutor(max_workers=os.cpu_count() or 4) as ex:
@@ -98,7 +106,23 @@ def build(force: bool = False) -> Path:
     if res.returncode != 0:
         raise RuntimeError(f"link failed: {' '.join(cmd)}\n{res.stderr}")
     os.replace(tmp, LIBRARY)
+    _build_binding(force)
     return LIBRARY
+
+
+def _build_binding(force: bool = False) -> None:
+    """The extension module that api.py imports, for the interpreter that runs
+    this; it finds the library beside it."""
+    newest = max(p.stat().st_mtime for p in [BINDING_SOURCE, ROOT / "include" / "porch_b200.h", Path(__file__)])
+    if BINDING.exists() and not force and BINDING.stat().st_mtime >= newest:
+        return
+    tmp = BINDING.with_suffix(".so.tmp")
+    cmd = [CXX, *CXXFLAGS, "-Wno-missing-field-initializers", f"-I{sysconfig.get_paths()['include']}", "-shared",
+           str(BINDING_SOURCE), "-o", str(tmp), f"-L{LIB_DIR}", "-lporch_b200", "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"binding failed: {' '.join(cmd)}\n{res.stderr}")
+    os.replace(tmp, BINDING)
 
 
 def check_kernels(out_dir: Path | None = None) -> list[str]:

@@ -13,7 +13,7 @@
 //
 // Bytes: each score once, and twice the rows that move; after long prompts (4
 // sequences x 8 heads of 65533 slots to 4096) 8.4 MB and 128 MB: the select
-// takes 23.5 us, bound by the latency of its passes, the move 22.7 us = 5.6
+// takes 22.4 us, bound by the latency of its passes, the move 22.7 us = 5.6
 // TB/s. After a few decoding steps (1048 slots to 1024) the one launch of both
 // takes 15 us.
 #include "operators.hpp"
