@@ -673,15 +673,16 @@ static __device__ __forceinline__ pb_i64 pb_part(const int4& r, int i, int head)
 
 // Joins the parts of a row that several CTAs worked on. Block: one query head
 // of one such row; its threads read the parts' sums at once, then each group of
-// D / 4 threads takes every PB_JOIN-th part, four channels a thread. Latency:
-// two rounds of loads.
+// D / 4 threads takes every PB_JOIN-th part, four channels a thread, its first
+// two on their way beside the sums. Latency: one round of loads.
 #define PB_JOIN (PB_JOIN_THREADS / (PB_D / 4))
 static __device__ __forceinline__ void pb_join(const int4* joins, const float* partial, const float2* partial_ml,
                                                float* out, int group, int chunks, int block) {
     __shared__ float weight[PB_JOIN_THREADS], reduce[16];
     __shared__ float4 sums[PB_JOIN_THREADS];
     const int heads = min(group, PB_HT);
-    const int4 r = joins[block / heads];
+    const int4 r = joins[block / heads]; // of the plan, in place before the launch
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int head = block % heads, chunk = r.x % chunks, kvh = (r.x / chunks) % PB_H, s = r.x / chunks / PB_H;
     if (head >= group - chunk * PB_HT) return;
     const pb_i64 global = (pb_i64)s * PB_H * group + kvh * group + chunk * PB_HT + head;
@@ -692,6 +693,11 @@ static __device__ __forceinline__ void pb_join(const int4* joins, const float* p
         const int n = min(PB_JOIN_THREADS, r.z - from), i = from + threadIdx.x;
         float2 ml = make_float2(__int_as_float(0xff800000), 0.0f);
         if (threadIdx.x < n) ml = partial_ml[pb_part(r, i, head)];
+        float4 early[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            if (team < PB_JOIN && team + e * PB_JOIN < n)
+                early[e] = *reinterpret_cast<const float4*>(partial + pb_part(r, from + team + e * PB_JOIN, head) * PB_D + 4 * quad);
         float x = ml.x;
 #pragma unroll
         for (int m = 16; m > 0; m /= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, m));
@@ -717,16 +723,18 @@ static __device__ __forceinline__ void pb_join(const int4* joins, const float* p
         sum = fmaf(sum, corr, y);
         acc = make_float4(acc.x * corr, acc.y * corr, acc.z * corr, acc.w * corr);
         if (team < PB_JOIN) {
+            auto add = [&](const float4& o, float w) {
+                acc.x = fmaf(w, o.x, acc.x);
+                acc.y = fmaf(w, o.y, acc.y);
+                acc.z = fmaf(w, o.z, acc.z);
+                acc.w = fmaf(w, o.w, acc.w);
+            };
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (team + e * PB_JOIN < n) add(early[e], weight[team + e * PB_JOIN]);
 #pragma unroll 4
-            for (int j = team; j < n; j += PB_JOIN) {
-                const int at = from + j;
-                const pb_i64 part = pb_part(r, at, head);
-                const float4 o = *reinterpret_cast<const float4*>(partial + part * PB_D + 4 * quad);
-                acc.x = fmaf(weight[j], o.x, acc.x);
-                acc.y = fmaf(weight[j], o.y, acc.y);
-                acc.z = fmaf(weight[j], o.z, acc.z);
-                acc.w = fmaf(weight[j], o.w, acc.w);
-            }
+            for (int j = team + 2 * PB_JOIN; j < n; j += PB_JOIN)
+                add(*reinterpret_cast<const float4*>(partial + pb_part(r, from + j, head) * PB_D + 4 * quad), weight[j]);
         }
     }
     sums[threadIdx.x] = acc;
@@ -769,6 +777,7 @@ static __device__ __forceinline__ void pb_scores(const int4* joins, const int* s
     const pb_i64 row = block / blocks; // sequence and key head
     const int i0 = (int)(block % blocks) * (4 * PB_JOIN_THREADS) + threadIdx.x; // lengths are below 2^30
     const int length = lengths[row / PB_H];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const float* before = scores + row * ns;
     float a[4];
 #pragma unroll
@@ -833,7 +842,6 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
     const int4* joins, const int* split, const float* partial, const float2* partial_ml, float* out,
     const float* logits, const float2* norms, const int* lengths, const float* scores, float* new_scores, pb_i64 longest,
     pb_i64 ns, int group, int chunks, int join_blocks) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (blockIdx.x < join_blocks) {
         pb_join(joins, partial, partial_ml, out, group, chunks, blockIdx.x);
         return;
