@@ -591,8 +591,8 @@ class Batch:
         self._h = c_void_p()
         self.cache = cache
         table = np.asarray(tables)
-        if table.ndim != 2:
-            raise InvalidArgument("cache batch: tables must be [sequences, width]")
+        if table.ndim != 2 or (table.size and table.dtype.kind not in "iu"):
+            raise InvalidArgument("cache batch: tables must be [sequences, width] whole numbers")
         if table.size and (table.min() < -(1 << 31) or table.max() >= 1 << 31):
             raise OutOfRange("cache batch: a page is not one of the cache's")
         table = np.ascontiguousarray(table, dtype=np.int32)
@@ -601,10 +601,10 @@ class Batch:
         def whole(values):
             if values is None:
                 return None
-            a = np.ascontiguousarray(values, dtype=np.int64)
-            if a.shape != (n,):
-                raise InvalidArgument("cache batch: one length, new tokens and newest position per sequence")
-            return a
+            a = np.asarray(values)
+            if a.shape != (n,) or (n and a.dtype.kind not in "iu"):
+                raise InvalidArgument("cache batch: one whole length, new tokens and newest position per sequence")
+            return np.ascontiguousarray(a, dtype=np.int64)
 
         self.lengths, fresh, last = whole(lengths), whole(appended), whole(newest)
 

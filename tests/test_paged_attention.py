@@ -315,7 +315,10 @@ def test_refusals(gpu):
     refused(bad, "newest", cache.batch, tables, [20, 32], newest=[19, 30])
     refused(bad, "newest", cache.batch, tables, [20, 32], newest=[19, 1 << 24])
     refused(bad, "same row", cache.batch, [[0, 1], [0, 1]], [20, 20])
-    refused(bad, "one length", cache.batch, tables, [20])
+    refused(bad, "one whole length", cache.batch, tables, [20])
+    refused(bad, "one whole length", cache.batch, tables, [20.5, 32.0])
+    refused(bad, "whole numbers", cache.batch, tables + 0.5, [20, 32])
+    assert cache.batch([[]], [0]).lengths.tolist() == [0]
     refused(bad, "width", cache.batch, [0, 1], [20])
     refused(bad, "sequences", cache.batch, np.zeros((0, 2), np.int32), [])
     refused(bad, "shape, type or device", batch.on, gpu.KVCache(6, 16, 2, 64, dtype="bf16"))
