@@ -34,9 +34,10 @@ namespace porch::detail {
         const char* append_source() {
             return R"PB(
 typedef long long pb_i64;
-// Thread: 8 values of one token's key or value. Bound by HBM: 4 B read and
-// the cache's width written per value; a float32 value is rounded to nearest
-// even bfloat16, the type that the cache holds.
+// Thread: 8 values of one token's key and value. Bound by HBM: 4 B read and
+// the cache's width written per value (65536 tokens x 8 heads x 128 into
+// bfloat16: 120 us = 6.7 TB/s); a float32 value is rounded to nearest even
+// bfloat16, the type that the cache holds.
 static __device__ __forceinline__ pb_u32 pb_bf16_pair(float lo, float hi) {
     pb_u32 r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -275,6 +276,7 @@ static __device__ __forceinline__ int2 pb_before(const int* totals, pb_u32 rank,
 #endif
 }
 
+#ifndef PB_LONG
 // One cluster per sequence and key head. Each CTA holds the keys of a run of
 // slots; a thread owns PB_KPT consecutive ones, handed over through shared
 // memory (an odd stride apart, so that threads use distinct banks), and the
@@ -426,70 +428,174 @@ extern "C" __global__ void __launch_bounds__(PB_THREADS, PB_THREADS < 1024 ? 2 :
     }
 }
 #endif
+#endif
 
-#ifndef PB_CLUSTER
-// Rank of this thread's flag among the block's 1024, and their number.
-static __device__ __forceinline__ int pb_block_rank(bool flag, int2* warps, int& total) {
-    int2 sum;
-    const int2 r = pb_block_scan(make_int2(flag, 0), warps, sum);
-    total = sum.x;
-    return r.x;
-}
-
-// The same for rows too long for a cluster's shared memory: one block per
-// row, which reads the row again in every pass.
+#if defined(PB_CLUSTER) && defined(PB_LONG)
+// The same for rows whose keys do not fit a cluster's shared memory: each CTA
+// reads its run of slots again, 4096 at a time, in every pass of the select,
+// once to count what it keeps, and once to write. One row of 420000
+// slots: 1137 us with one CTA, 104 with 8 (of 390000, held: 43).
 extern "C" __global__ void __launch_bounds__(1024) pb_evict_select_long(
     const float* scores, const float* places, const int* lengths, const int* newest, float* out_scores,
     float* out_places, int* holes, int* lates, int* counts, pb_i64 ns, pb_i64 np, int budget, int recent, int sinks,
     int pairs) {
+    constexpr int round = 4096;
+    __shared__ int hist[2][256], bins[256], chosen[3], totals[4];
+    __shared__ int2 warps[32], before[2];
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    __shared__ int hist[256], chosen[3];
-    __shared__ int2 warps[32];
-    const pb_i64 row = blockIdx.x;
+    const pb_i64 row = blockIdx.x / PB_CLUSTER;
+    const int rank = (int)pb_rank();
     const pb_row r = pb_row_of(scores, places, lengths, newest, ns, np, recent, sinks, row);
+    for (pb_i64 i = (pb_i64)r.length + rank * 1024 + threadIdx.x; i < budget; i += PB_CLUSTER * 1024) {
+        out_scores[row * budget + i] = 0.0f;
+        out_places[row * budget + i] = -1.0f;
+    }
+    if (r.length <= budget) { // the same in every CTA of the cluster
+        for (int i = rank * 1024 + threadIdx.x; i < r.length; i += PB_CLUSTER * 1024)
+            pb_keep(r, out_scores, out_places, row * budget + i, i);
+        if (rank == 0 && threadIdx.x == 0) counts[row] = 0;
+        return;
+    }
+    const int run = (r.length + PB_CLUSTER * round - 1) / (PB_CLUSTER * round) * round;
+    const int first = (int)min((pb_i64)rank * run, (pb_i64)r.length), last = (int)min((pb_i64)first + run, (pb_i64)r.length);
+    // This thread's four slots of the round at `base`, every load before the first use.
+    auto load = [&](int base, pb_u32* key) {
+        float score[4], place[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = base + threadIdx.x * 4 + j;
+            score[j] = i < last && i < r.ns ? r.scores[i] : 0.0f;
+            place[j] = i < last && i < r.np ? r.places[i] : -1.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) key[j] = pb_key_of(r, base + threadIdx.x * 4 + j, score[j], place[j]);
+    };
+
     pb_u32 limit = 0;
     int want = budget;
-    if (r.length > budget) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (threadIdx.x < 256) hist[threadIdx.x] = 0;
-            __syncthreads();
-            for (int i = threadIdx.x; i < r.length; i += 1024) {
-                const pb_u32 key = pb_key(r, i);
-                if (shift == 24 || ((key ^ limit) >> (shift + 8)) == 0) atomicAdd(&hist[(key >> shift) & 255u], 1);
-            }
-            __syncthreads();
-            if (threadIdx.x < 32) pb_pick(hist, want, chosen);
-            __syncthreads();
-            limit |= (pb_u32)chosen[0] << shift;
-            want = chosen[1];
-            __syncthreads();
+    bool whole = false;
+    for (int i = threadIdx.x; i < 256; i += 1024) hist[0][i] = 0;
+    __syncthreads();
+    for (int pass = 0; pass < 4 && !whole; ++pass) {
+        const int shift = 24 - 8 * pass;
+        int* h = hist[pass & 1];
+        for (int base = first; base < last; base += round) {
+            pb_u32 key[4];
+            load(base, key);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (base + (int)threadIdx.x * 4 + j < last && (pass == 0 || ((key[j] ^ limit) >> (shift + 8)) == 0))
+                    atomicAdd(&h[(key[j] >> shift) & 255u], 1);
         }
-    }
-    int ties = 0, nholes = 0, nlate = 0, total = 0;
-    for (pb_i64 base = 0; base < max(r.length, budget); base += 1024) {
-        const int i = (int)(base + threadIdx.x); // lengths and budgets are at most 2^30
-        const bool live = i < r.length, all = r.length <= budget;
-        const pb_u32 key = live && !all ? pb_key(r, i) : 0u;
-        const bool tie = live && !all && key == limit;
-        const int place = ties + pb_block_rank(tie, warps, total);
-        ties += total;
-        const bool kept = live && (all || key > limit || (tie && place < want));
-        const bool hole = live && i < budget && !kept;
-        const int h = nholes + pb_block_rank(hole, warps, total);
-        nholes += total;
-        const int l = nlate + pb_block_rank(i >= budget && kept, warps, total);
-        nlate += total;
-        if (hole) holes[row * pairs + h] = i;
-        if (i >= budget && kept) lates[row * pairs + l] = i;
-        if (i < budget && kept) pb_keep(r, out_scores, out_places, row * budget + i, i);
-        if (i < budget && !live) {
-            out_scores[row * budget + i] = 0.0f;
-            out_places[row * budget + i] = -1.0f;
+        pb_cluster_sync();
+        for (int i = threadIdx.x; i < 256; i += 1024) {
+            int sum = 0;
+#pragma unroll
+            for (int c = 0; c < PB_CLUSTER; ++c) sum += pb_peer(h + i, c);
+            bins[i] = sum;
+            hist[(pass & 1) ^ 1][i] = 0; // every CTA has read it: it was before this barrier
         }
+        __syncthreads();
+        if (threadIdx.x < 32) pb_pick(bins, want, chosen);
+        __syncthreads();
+        limit |= (pb_u32)chosen[0] << shift;
+        want = chosen[1];
+        whole = chosen[2];
     }
-    if (threadIdx.x == 0) counts[row] = nlate;
-}
 
+    // Keys equal to the limit and keys above it, below the budget and past it.
+    int2 equal = make_int2(0, 0), above = make_int2(0, 0), total;
+    for (int base = first; base < last; base += round) {
+        pb_u32 key[4];
+        load(base, key);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = base + threadIdx.x * 4 + j;
+            if (i >= last) continue;
+            const bool over = whole ? key[j] >= limit : key[j] > limit, same = !whole && key[j] == limit;
+            equal.x += same && i < budget;
+            equal.y += same && i >= budget;
+            above.x += over && i < budget;
+            above.y += over && i >= budget;
+        }
+    }
+    (void)pb_block_scan(equal, warps, total);
+    if (threadIdx.x == 0) { totals[0] = total.x; totals[1] = total.y; }
+    (void)pb_block_scan(above, warps, total);
+    if (threadIdx.x == 0) { totals[2] = total.x; totals[3] = total.y; }
+    pb_cluster_sync();
+    if (threadIdx.x < 32) {
+        // Lane c: what CTA c keeps, given the ties of those before it.
+        const int c = threadIdx.x;
+        int t[4] = {0, 0, 0, 0};
+        if (c < PB_CLUSTER)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t[j] = pb_peer(totals + j, c);
+        int ties = t[0] + t[1];
+#pragma unroll
+        for (int m = 1; m < PB_CLUSTER; m *= 2) {
+            const int v = __shfl_up_sync(0xffffffffu, ties, m);
+            if (c >= m) ties += v;
+        }
+        ties -= t[0] + t[1];
+        const int kept = max(0, min(want - ties, t[0] + t[1])), low = min(kept, t[0]);
+        const pb_i64 from = (pb_i64)c * run;
+        const int slots = (int)max((pb_i64)0, min((pb_i64)budget, min(from + run, (pb_i64)r.length)) - from);
+        int2 sum = c < rank ? make_int2(slots - t[2] - low, t[3] + kept - low) : make_int2(0, 0);
+#pragma unroll
+        for (int m = 4; m > 0; m /= 2) {
+            sum.x += __shfl_down_sync(0xffffffffu, sum.x, m);
+            sum.y += __shfl_down_sync(0xffffffffu, sum.y, m);
+        }
+        if (c == 0) before[0] = sum;
+        if (c == rank) before[1] = make_int2(ties, 0);
+    }
+    __syncthreads();
+    int2 at = before[0]; // free places and late slots so far
+    int ties = before[1].x;
+    for (int base = first; base < last; base += round) {
+        pb_u32 key[4];
+        load(base, key);
+        const int i0 = base + threadIdx.x * 4;
+        int seen = ties;
+        if (!whole) {
+            int same = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) same += i0 + j < last && key[j] == limit;
+            seen += pb_block_scan(make_int2(same, 0), warps, total).x;
+            ties += total.x;
+        }
+        int2 count = make_int2(0, 0);
+        int kept = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (i0 + j >= last) continue;
+            const bool keep = whole ? key[j] >= limit : key[j] > limit || (key[j] == limit && seen++ < want);
+            kept |= keep << j;
+            count.x += i0 + j < budget && !keep;
+            count.y += i0 + j >= budget && keep;
+        }
+        int2 mine = pb_block_scan(count, warps, total);
+        mine.x += at.x;
+        mine.y += at.y;
+        at.x += total.x;
+        at.y += total.y;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = i0 + j;
+            if (i >= last) continue;
+            const bool keep = kept >> j & 1;
+            if (i < budget && !keep) holes[row * pairs + mine.x++] = i;
+            if (i < budget && keep) pb_keep(r, out_scores, out_places, row * budget + i, i);
+            if (i >= budget && keep) lates[row * pairs + mine.y++] = i;
+        }
+    }
+    if (rank == PB_CLUSTER - 1 && threadIdx.x == 0) counts[row] = at.y;
+    pb_cluster_sync(); // nobody leaves while its shared memory is read
+}
+#endif
+
+#ifndef PB_CLUSTER
 extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
     char* pk, char* pv, const int* tables, const float* scores, const float* places, const int* lengths,
     const int* newest, float* out_scores, float* out_places, const int* holes, const int* lates, const int* counts,
@@ -508,8 +614,9 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
 
         // How the select shares out a row of `longest` slots.
         struct select_shape {
-            int cluster = 0, threads = 0, per_thread = 0; // cluster 0: the long form
-            uint32_t smem() const { return static_cast<uint32_t>(threads * (per_thread | 1) * 4); }
+            int cluster = 0, threads = 0, per_thread = 0;
+            bool held = true; // false: the long form, which reads the row again
+            uint32_t smem() const { return held ? static_cast<uint32_t>(threads * (per_thread | 1) * 4) : 0; }
         };
         select_shape shape_for(int64_t longest, int64_t rows, int sms) {
             static constexpr int kShapes[][2] = {{256, 4}, {256, 8}, {512, 8}, {512, 16}, {1024, 16}, {1024, 32}, {1024, 48}};
@@ -528,6 +635,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
                         r.per_thread = per_thread;
                         return r;
                     }
+            r = {8, 1024, 4, false};
             return r;
         }
 
@@ -549,7 +657,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
                << "\n#define PB_CHUNKS " << (2 * c.dim * c.width() + 511) / 512 << "\n";
             if (f.cluster != 0)
                 os << "#define PB_CLUSTER " << f.cluster << "\n#define PB_THREADS " << f.threads << "\n#define PB_KPT "
-                   << f.per_thread << "\n";
+                   << f.per_thread << "\n" << (f.held ? "" : "#define PB_LONG 1\n");
             return os.str();
         }
 
@@ -560,7 +668,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
 
         op_kernel& kernel_of(const char* name, const kv_cache& c, bool wide = true, const select_shape& f = {}) {
             const op_key key{reinterpret_cast<int64_t>(name), c.heads, c.dim, c.page_size, static_cast<int64_t>(c.type),
-                             wide, f.cluster, f.threads, f.per_thread};
+                             wide, f.cluster, f.threads, f.per_thread, f.held};
             return op_kernel_for(key, [&](op_kernel& k) {
                 k.name = name;
                 k.source = std::string{kernel_prelude()} + defines(c, wide, f) +
@@ -752,16 +860,13 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
             order_write(*cuda_jit::buffer_access::state(c.v), stream);
         }
         uint64_t pk = address(c.k), pv = address(c.v);
-        int fused = moves && f.cluster != 0 && pairs <= kFewPairs;
+        int fused = moves && f.held && pairs <= kFewPairs;
         void* sparams[] = {&xs.ptr, &xp.ptr, &batch.lengths_at, &batch.newest_at, &os.ptr, &op.ptr, &holes,
                            &lates,  &counts, &nsv,              &npv,             &b,      &rc,     &sk,
                            &pairs,  &pk,     &pv,               &batch.tables_at, &width,  &fused};
-        if (f.cluster != 0) {
-            op_launch(kernel_of(kSelect, c, true, f), device, stream, {static_cast<uint32_t>(rows * f.cluster), 1, 1},
-                      static_cast<uint32_t>(f.threads), sparams, static_cast<uint32_t>(f.cluster));
-        } else {
-            op_launch(kernel_of(kSelectLong, c), device, stream, {static_cast<uint32_t>(rows), 1, 1}, 1024, sparams);
-        }
+        op_launch(kernel_of(f.held ? kSelect : kSelectLong, c, true, f), device, stream,
+                  {static_cast<uint32_t>(rows * f.cluster), 1, 1}, static_cast<uint32_t>(f.threads), sparams,
+                  static_cast<uint32_t>(f.cluster));
         if (moves && !fused) {
             uint32_t per_row = static_cast<uint32_t>((pairs + 8 * moves_of(c) - 1) / (8 * moves_of(c)));
             const int64_t blocks = rows * per_row;
@@ -785,6 +890,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
             out.emplace_back("pb_cache_append" + tag, p + defines(c, type == cache_type::bf16) + append_source());
             out.emplace_back("pb_evict" + tag, p + defines(c, true) + evict_source());
             out.emplace_back("pb_evict_select" + tag, p + defines(c, true, type == cache_type::bf16 ? select_shape{8, 1024, 48} : select_shape{1, 256, 4}) + evict_source());
+            out.emplace_back("pb_evict_select_long" + tag, p + defines(c, true, {8, 1024, 4, false}) + evict_source());
         }
     }
 

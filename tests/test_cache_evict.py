@@ -41,6 +41,7 @@ CASES = [
     ([420000, 1500], 1, 8, 256, "bf16", 3000, 500, 4),
     ([420000, 1500], 1, 8, 256, "f32", 419000, 500, 4),
     ([30, 20], 2, 8, 8, "f32", 5000, 500, 4),
+    ([393217, 4096, 4097], 1, 8, 256, "bf16", 4096, 0, 0),
 ]
 
 
