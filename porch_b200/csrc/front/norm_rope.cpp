@@ -135,9 +135,17 @@ static __device__ __forceinline__ void pb_load_angle(pb_angle& g, const float* c
         if (2 * i < PB_R) { g.c[n][0][0] = __ldg(c + i); g.s[n][0][0] = __ldg(s + i); }
 #else
 #pragma unroll
-        for (int e = 0; e < PB_VEC; e += 2) {
-            if (pb_at_a(i) < PB_R) { g.c[n][0][e] = __ldg(c + pb_at_a(i) / 2 + e / 2); g.s[n][0][e] = __ldg(s + pb_at_a(i) / 2 + e / 2); }
-            if (pb_at_b(i) < PB_R) { g.c[n][1][e] = __ldg(c + pb_at_b(i) / 2 + e / 2); g.s[n][1][e] = __ldg(s + pb_at_b(i) / 2 + e / 2); }
+        for (int v = 0; v < 2; ++v) {
+            const int at = v ? pb_at_b(i) : pb_at_a(i);
+            if (at >= PB_R) continue;
+#if PB_VEC == 4 // the table's rows are of an even number of values then
+            const float2 x = __ldg(reinterpret_cast<const float2*>(c + at / 2)), y = __ldg(reinterpret_cast<const float2*>(s + at / 2));
+            g.c[n][v][0] = x.x; g.c[n][v][2] = x.y;
+            g.s[n][v][0] = y.x; g.s[n][v][2] = y.y;
+#else
+            g.c[n][v][0] = __ldg(c + at / 2);
+            g.s[n][v][0] = __ldg(s + at / 2);
+#endif
         }
 #endif
     }
@@ -419,13 +427,25 @@ extern "C" __global__ void __launch_bounds__(1024) pb_norm_rope_weights(const fl
         // Vectors as wide as the sizes let both partners of a pair, and the
         // table's rows, start on; lanes for one item each, up to a warp.
         // `aligned`: the width at which every row of the operands starts.
-        void choose_lanes(shape_key& s, int aligned) {
+        // `few`: of 4 to 32 lanes the number that leaves the fewest idle, the
+        // larger of equals. Head sizes of 80 and 96 have 10 and 12 items: 4
+        // lanes of three take 56 and 53 us forward where 16 of one take 63 and
+        // 59 (25000 and 20833 tokens x 20 heads), but 77 and 61 where 16 take
+        // 61 and 56 with pairs side by side, and 133 and 113 where 16 take 105
+        // and 97 in the gradient, whose registers then hold one head at once.
+        void choose_lanes(shape_key& s, int aligned, bool few) {
             s.vec = 4;
             while (s.vec > 1 && (s.dim % s.vec != 0 || (s.interleaved ? (2 * s.half) % s.vec : s.half % s.vec) != 0))
                 s.vec /= 2;
             s.wide = aligned >= s.vec;
+            const int items = items_of(s);
             s.lanes = 1;
-            while (s.lanes < 32 && s.lanes < items_of(s)) s.lanes *= 2;
+            while (s.lanes < 32 && s.lanes < items) s.lanes *= 2;
+            if (!few) return;
+            for (int lanes = s.lanes / 2; lanes >= 4; lanes /= 2) {
+                const int each = (items + lanes - 1) / lanes, now = (items + s.lanes - 1) / s.lanes;
+                if (each <= 4 && each * lanes < now * s.lanes) s.lanes = lanes;
+            }
         }
 
         // Heads of a token that a group takes at once, sharing its angles and
@@ -463,7 +483,7 @@ extern "C" __global__ void __launch_bounds__(1024) pb_norm_rope_weights(const fl
         op_result oq = new_result(x.q.shape, device, stream), ok = new_result(x.k.shape, device, stream);
         if (c.tokens != 0) {
             shape_key& s = c.key;
-            choose_lanes(s, std::min(vector_width(x.q), vector_width(x.k)));
+            choose_lanes(s, std::min(vector_width(x.q), vector_width(x.k)), !a.interleaved);
             s.per = heads_at_once(s, c.tokens, 2, sm_count(device));
             op_kernel& kernel = kernel_of(s, kNormRope, "PB_FORWARD");
             const int64_t units = c.tokens * ((s.q_heads + s.per - 1) / s.per + (s.k_heads + s.per - 1) / s.per);
@@ -494,7 +514,7 @@ extern "C" __global__ void __launch_bounds__(1024) pb_norm_rope_weights(const fl
             check(pbrt_memset_d32_async(device, wk.ptr, 0, static_cast<size_t>(c.key.dim), stream->stream));
         } else {
             shape_key& s = c.key;
-            choose_lanes(s, std::min({vector_width(x.q), vector_width(x.k), vector_width(gq), vector_width(gk)}));
+            choose_lanes(s, std::min({vector_width(x.q), vector_width(x.k), vector_width(gq), vector_width(gk)}), false);
             s.per = heads_at_once(s, c.tokens, 4, sm_count(device));
             op_kernel& kernel = kernel_of(s, kNormRopeGrad, "PB_BACKWARD");
             op_kernel& weights = kernel_of(s, kNormRopeWeights, "PB_BACKWARD");
@@ -523,14 +543,14 @@ extern "C" __global__ void __launch_bounds__(1024) pb_norm_rope_weights(const fl
         for (const auto& [dim, rot, inter, aligned] :
              {std::array<int, 4>{128, 128, 0, 4}, std::array<int, 4>{80, 40, 1, 1}, std::array<int, 4>{37, 18, 0, 1},
               std::array<int, 4>{37, 18, 1, 1},
-              std::array<int, 4>{1023, 1022, 0, 4}, std::array<int, 4>{512, 64, 0, 4}}) {
+              std::array<int, 4>{1023, 1022, 0, 4}, std::array<int, 4>{96, 48, 0, 4}, std::array<int, 4>{512, 64, 0, 4}}) {
             shape_key s;
             s.dim = dim;
             s.half = rot / 2;
             s.q_heads = 5;
             s.k_heads = 2;
             s.interleaved = inter != 0;
-            choose_lanes(s, aligned);
+            choose_lanes(s, aligned, inter == 0);
             s.per = heads_at_once(s, 1 << 20, aligned, 148);
             const std::string tag = "_" + std::to_string(dim) + (inter ? "i" : "h");
             out.emplace_back("pb_norm_rope" + tag, source_of(s, "PB_FORWARD"));
