@@ -248,7 +248,10 @@ extern "C" __global__ void __launch_bounds__(256) pb_norm_rope(
 // set of registers gathers a weight's gradient; a block adds its groups in
 // order and writes one row of partial sums per weight, which
 // pb_norm_rope_weights adds in order: the result depends on the sizes alone.
-extern "C" __global__ void __launch_bounds__(256) pb_norm_rope_grad(
+// Two blocks of an SM at once, at the price of a few spilled registers (half
+// rotated heads of 96 side by side, 20833 tokens x 20: 105 us with one, 84.5 so;
+// the worst loss, half rotated heads of 256: 76.4 and 79.7).
+extern "C" __global__ void __launch_bounds__(256, PB_NI * PB_HPG <= 4 ? 2 : 1) pb_norm_rope_grad(
     const float* dyq, const float* dyk, const float* q, const float* k, const float* qw, const float* kw,
     const float* cs, const float* sn, const float* pos, float* dq, float* dk, float* partial, pb_i64 T, pb_i64 P,
     pb_i64 gqt, pb_i64 gqh, pb_i64 gkt, pb_i64 gkh, pb_i64 qt, pb_i64 qh, pb_i64 kt, pb_i64 kh, float eps) {
