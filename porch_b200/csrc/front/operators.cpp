@@ -88,6 +88,7 @@ namespace porch::detail {
     op_operand operand(const tensor& t, const std::shared_ptr<stream_ref>& stream, bool strided) {
         op_operand x;
         x.storage = tensor_access::storage(t);
+        if (x.storage->placeholder) throw std::runtime_error("operands: placeholder tensors hold no values");
         if (strided) {
             x.shape = shape_of(t);
             x.strides = contiguous_strides(x.shape);

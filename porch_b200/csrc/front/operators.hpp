@@ -61,6 +61,7 @@ namespace porch::detail {
     // realises.
     std::vector<index_t> shape_of(const tensor& t);
     bool has_shape(const tensor& t, std::initializer_list<index_t> shape);
+    // Throws for placeholders: they have no address.
     op_operand operand(const tensor& t, const std::shared_ptr<stream_ref>& stream, bool strided);
     // The device that `t`'s values live on; throws for placeholders.
     int device_of(const tensor& t, const char* what);

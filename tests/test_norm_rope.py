@@ -234,6 +234,18 @@ def test_positions_outside_the_table_and_values_that_are_not_finite(gpu, interle
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("at", range(9))
+def test_every_operand_needs_values(gpu, at):
+    given = [gpu.zeros(s) for s in ([3, 4, 8], [3, 2, 8], [3, 4, 8], [3, 2, 8], [8], [8], [16, 4], [16, 4], [3])]
+    given[at] = gpu.placeholder(given[at].shape())
+    with pytest.raises(RuntimeError, match="placeholder"):
+        gpu.qk_norm_rope_backward(*given)
+    if at >= 2:
+        with pytest.raises(RuntimeError, match="placeholder"):
+            gpu.qk_norm_rope(*given[2:])
+
+
+@pytest.mark.gpu
 def test_no_tokens(gpu):
     rng = np.random.default_rng(4)
     x = inputs(rng, 0, 2, 1, 16, 8, 20)
