@@ -698,6 +698,7 @@ int pb_tensor_interface(const pb_tensor* t, int64_t* out, size_t capacity) {
         require(t, "tensor");
         require(out, "out");
         const auto extents = t->value.shape();
+        (void)porch::detail::device_of(t->value, "interface"); // no null address for values that are not there
         if (capacity < 3 + extents.size()) throw std::invalid_argument("interface needs room for 3 numbers and the shape");
         const auto& buffer = t->value.device_data();
         const auto& st = porch::cuda_jit::buffer_access::state(buffer);

@@ -78,6 +78,13 @@ def test_interface(gpu):
 
 
 @pytest.mark.gpu
+def test_interface_of_a_placeholder(gpu):
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="placeholder"):
+            gpu.placeholder([2, 3]).__cuda_array_interface__
+
+
+@pytest.mark.gpu
 def test_batch_arguments(gpu):
     cache = gpu.KVCache(4, 8, 1, 8)
     batch = cache.batch([[0, 1]], [9])
