@@ -256,7 +256,7 @@ extern "C" __global__ void __launch_bounds__(256, PB_NI * PB_HPG <= 4 ? 2 : 1) p
     const float* cs, const float* sn, const float* pos, float* dq, float* dk, float* partial, pb_i64 T, pb_i64 P,
     pb_i64 gqt, pb_i64 gqh, pb_i64 gkt, pb_i64 gkh, pb_i64 qt, pb_i64 qh, pb_i64 kt, pb_i64 kh, float eps) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    __shared__ float sums[PB_GPB][PB_D];
+    __shared__ __align__(16) float sums[PB_GPB][PB_D]; // stored to in vectors
     const int lane = threadIdx.x % PB_L, group = threadIdx.x / PB_L;
     const int first = (threadIdx.x & ~31) / PB_L; // the warp's first group
 #pragma unroll 1

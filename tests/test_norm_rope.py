@@ -129,6 +129,14 @@ def test_refusals(api):
         api.qk_norm_rope_backward(good[0], good[1], *good)
 
 
+def test_shared_memory_written_in_vectors_is_aligned(api):
+    # pb_store_head writes a group's row of `sums` in up to 16 bytes; the
+    # language only promises a float's alignment for an array of floats.
+    text = api.operator_sources()
+    declared = [line for line in text.splitlines() if "__shared__" in line and " sums[PB_GPB]" in line]
+    assert declared and all("__align__(16)" in line for line in declared)
+
+
 CASES = [
     # tokens, q heads, k heads, head size, rotated, interleaved
     (1, 1, 1, 2, 2, False),
