@@ -460,7 +460,9 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
             }
         }
         __syncwarp();
-        if (lane == 0) pb_mbar_arrive(empty + 8 * slot);
+        // Not after a wait that gave up: the unit's load may still be on its
+        // way, and the producer would issue another one into it.
+        if (lane == 0 && !bad) pb_mbar_arrive(empty + 8 * slot);
         if (++slot == PB_RING) { slot = 0; parity ^= 1u; }
 
         // Logits in units of log2, -inf past the sequence's end. Thread: slots

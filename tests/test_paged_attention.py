@@ -208,6 +208,19 @@ def test_a_wait_that_runs_out_is_reported_and_the_gpu_recovers(gpu):
         assert (np.abs(gpu.paged_attention(t, batch).cpu().reshape(q.shape) - out) <= tol).all()
 
 
+def test_a_unit_is_handed_back_only_after_its_load_has_landed(api):
+    # Both places where a computing warp hands a unit back to the producer: the
+    # first stands before the barrier at which a wait that gave up makes all
+    # warps leave, so it has a condition; the second stands behind that barrier.
+    text = api.operator_sources()
+    text = text[text.index("extern \"C\" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention") :]
+    text = text[: text.index("---- the row ends")]
+    waits, leaves = "bad |= !pb_wait(full", "if (pb_bar_any(bad)) { bad = true; break; }"
+    first, second = [i for i in range(len(text)) if text.startswith("pb_mbar_arrive(empty", i)]
+    assert text.count(waits) == 2 and text[:first].endswith("if (lane == 0 && !bad) ")
+    assert text.rindex(waits) < text.rindex(leaves) < second
+
+
 @pytest.mark.gpu
 def test_the_same_every_time_and_from_another_thread(gpu):
     import threading
