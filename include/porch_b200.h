@@ -366,8 +366,9 @@ int pb_operator_sources(char* text, size_t capacity, size_t* needed);
  * raises PB_ERR_RUNTIME. Only for tests of that path. */
 int pb_test_gemm_stall(int enable);
 /* The same for paged attention: while enabled, its first CTA's tiles are
- * never loaded, its bounded waits give up and the kernel records a code of
- * 0x7d00 and more. */
+ * never loaded and its bounded waits give up (1), or it gives up at once,
+ * while its first tiles are on their way (2); the kernel records a code of
+ * 0x7d00 and more, and leaves when nothing is in flight any more. */
 int pb_test_attention_stall(int enable);
 
 /* ---- matmul without allocation ------------------------------------------ */

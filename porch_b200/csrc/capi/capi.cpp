@@ -855,7 +855,10 @@ int pb_kv_evict(pb_kv_batch* batch, const pb_tensor* scores, const pb_tensor* po
 }
 
 int pb_test_attention_stall(int enable) {
-    return guarded([&] { porch::detail::set_test_attention_stall(enable != 0); });
+    return guarded([&] {
+        if (enable < 0 || enable > 2) throw std::invalid_argument("attention stall: mode must be 0, 1 or 2");
+        porch::detail::set_test_attention_stall(enable);
+    });
 }
 
 namespace {

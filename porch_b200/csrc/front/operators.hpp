@@ -157,9 +157,10 @@ namespace porch::detail {
 
     const batch_plan& plan_of(kv_batch& batch, int64_t chunks, int64_t ctas);
     int attention_ctas_per_sm(const kv_cache& c);
-    // Test hook (off by default): block 0 of an attention never gets its
-    // tiles, so its bounded waits expire.
-    void set_test_attention_stall(bool on);
+    // Test hook (0: off): block 0 of an attention never gets its tiles, so its
+    // bounded waits expire (1), or gives up while its first ones are on their
+    // way (2).
+    void set_test_attention_stall(int mode);
     // The plan as text ("work <row> <tile> <tiles>" per CTA, "join <row>
     // <first CTA> <parts> <place>" per row), without a device.
     std::string attention_schedule(const std::vector<int64_t>& lengths, int64_t heads, int64_t chunks, int64_t ctas);

@@ -53,7 +53,8 @@ namespace porch::detail {
         // The whole layout of a kernel follows from these.
         struct form {
             int heads = 1, dim = 0, page = 0;
-            bool bf16 = false, scored = false, stall = false;
+            bool bf16 = false, scored = false;
+            int stall = 0; // the test hook's mode
             int join_threads = 128;
             int tiles8 = 1; // groups of 8 query heads that a row holds (1 or 2)
             int width() const { return bf16 ? 2 : 4; }
@@ -123,6 +124,13 @@ static __device__ __forceinline__ pb_u32 pb_mbar_try(pb_u32 bar, pb_u32 parity) 
                  : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
     return ok;
 }
+// Records where a wait gave up; the first one stays.
+static __device__ __forceinline__ void pb_gave_up(int* err, int site) {
+    if (atomicCAS(err, 0, 0x7d00 + site) == 0) {
+        err[1] = site;
+        err[2] = (int)blockIdx.x;
+    }
+}
 // Bounded wait: false when the budget ran out or another role gave up.
 static __device__ __forceinline__ bool pb_wait(pb_u32 bar, pb_u32 parity, volatile int* abort_flag, int* err, int site) {
     if (pb_mbar_try(bar, parity)) return true;
@@ -132,10 +140,7 @@ static __device__ __forceinline__ bool pb_wait(pb_u32 bar, pb_u32 parity, volati
         if (*abort_flag) return false;
         if (clock64() - start > PB_WAIT_CYCLES) {
             *abort_flag = 1;
-            if (atomicCAS(err, 0, 0x7d00 + site) == 0) {
-                err[1] = site;
-                err[2] = (int)blockIdx.x;
-            }
+            pb_gave_up(err, site);
             return false;
         }
     }
@@ -302,7 +307,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
         bool bad = false;
         int page = pb_page(at, tables, width, lane);
         asm volatile("griddepcontrol.wait;" ::: "memory");
-#ifdef PB_TEST_STALL
+#if PB_TEST_STALL == 1
         if (blockIdx.x == 0) return; // its tiles never arrive
 #endif
         for (int i = 0; i < mine.z && !bad; ++i) {
@@ -329,9 +334,10 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                 if (++slot == PB_RING) { slot = 0; parity ^= 1u; }
             }
         }
-        // Nothing may land after this CTA is gone: wait (bounded) for what
-        // is still in flight, which is only ever the case after an abort.
-        if (bad && lane == 0) {
+        // Nothing may land after this CTA is gone: wait (bounded) for what is
+        // still in flight. Always, since the computing warps may give up after
+        // the last load was issued; while they do not, they wait for the same.
+        if (lane == 0) {
             for (int u = unit > PB_RING ? unit - PB_RING : 0; u < unit; ++u) {
                 const long long start = clock64();
                 while (!pb_mbar_try(full + 8 * (u % PB_RING), (u / PB_RING) & 1) && clock64() - start <= PB_WAIT_CYCLES) {
@@ -408,6 +414,12 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
         const int base = at.tile * 64, valid = min(64, at.length - base);
 
         // ---- S^T = K Q^T: this warp's 16 slots x all heads
+#if PB_TEST_STALL == 2
+        if (blockIdx.x == 0) { // gives up at once, its first loads on their way
+            pb_gave_up(err, 5);
+            bad = true;
+        } else
+#endif
         bad |= !pb_wait(full + 8 * slot, parity, &abort_flag, err, 3);
         // The first term's sum, the large one, runs in two chains that are
         // added in fp32: half the additions that cut bits in a row.
@@ -862,11 +874,11 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
                << "\n#define PB_ESZ " << f.width() << "\n#define PB_NT " << f.tiles8 << "\n#define PB_RING " << f.ring()
                << "\n#define PB_JOIN_THREADS " << f.join_threads << "\n#define PB_PER_SM " << f.per_sm()
                << "\n#define PB_SCORED " << (f.scored ? 1 : 0) << "\n";
-            if (f.stall) os << "#define PB_TEST_STALL 1\n";
+            if (f.stall != 0) os << "#define PB_TEST_STALL " << f.stall << "\n";
             return os.str();
         }
 
-        std::atomic<bool> g_test_stall{false};
+        std::atomic<int> g_test_stall{0};
 
         const char kAttention[] = "pb_paged_attention";
         const char kFinish[] = "pb_paged_finish";
@@ -1064,7 +1076,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         return results;
     }
 
-    void set_test_attention_stall(bool on) { g_test_stall.store(on); }
+    void set_test_attention_stall(int mode) { g_test_stall.store(mode); }
 
     int attention_ctas_per_sm(const kv_cache& c) {
         form f;

@@ -222,6 +222,38 @@ def test_a_unit_is_handed_back_only_after_its_load_has_landed(api):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lengths", [[40, 30], [70, 5], [5000, 40]])
+def test_giving_up_while_loads_are_on_their_way(gpu, lengths):
+    # Block 0's computing warps give up at their first tile. Where its row has
+    # few tiles the producer has issued every load by then: it has to stay until
+    # they have landed, since shared memory is the next block's after it.
+    from porch_b200._lib import lib
+
+    rng = np.random.default_rng(7)
+    host = paged.Host(rng, lengths, 2, 64, 32, "bf16")
+    q = rng.normal(0, 1, (2, 4, 64)).astype(np.float32)
+    _, batch = host.build(gpu)
+    t = gpu.tensor([2, 4, 64], q)
+    assert lib().pb_test_attention_stall(2) == 0
+    try:
+        for _ in range(3):
+            with pytest.raises(RuntimeError, match="kernel error code 32005"):  # 0x7d00 + site 5
+                gpu.paged_attention(t, batch).cpu()
+    finally:
+        assert lib().pb_test_attention_stall(0) == 0
+    out, tol, _, _ = host.attend(q, 0.125)
+    for _ in range(2):
+        assert (np.abs(gpu.paged_attention(t, batch).cpu().reshape(q.shape) - out) <= tol).all()
+
+
+def test_the_producer_waits_for_its_loads_whoever_gave_up(api):
+    # Its last waits stand under no condition but the lane's.
+    text = api.operator_sources()
+    at = text.index("Nothing may land after this CTA is gone")
+    assert "if (lane == 0) {" in text[at : at + 400] and "bad" not in text[at : text.index("pb_mbar_try", at)]
+
+
+@pytest.mark.gpu
 def test_the_same_every_time_and_from_another_thread(gpu):
     import threading
 
