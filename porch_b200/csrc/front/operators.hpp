@@ -29,7 +29,7 @@ namespace porch::detail {
         std::mutex mutex;
         std::array<std::atomic<pbrt_function>, 16> function{};
 
-        pbrt_function on(int device);
+        pbrt_function on(int device); // loaded by the first call
     };
 
     // The kernel for `key` (its name's address and every constant of its
@@ -111,6 +111,11 @@ namespace porch::detail {
         cache_type type = cache_type::f32;
         int device = 0;
         cuda_jit::device_buffer k, v;
+        // Held from a call's ordering on the pools until its last kernel on
+        // them is enqueued: the order of calls from several threads is the
+        // order of their kernels. Kernels are compiled and memory is allocated
+        // before it is taken.
+        std::mutex order;
         int width() const { return type == cache_type::bf16 ? 2 : 4; } // bytes of a value
         // TMA maps of both pools as [rows, dim]: boxes of 128 bytes by a page,
         // or by 64 rows of a larger one.

@@ -1025,11 +1025,6 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
 
         op_result out = new_result(shape, device, stream);
         uint64_t results_ptr = out.ptr;
-        order_read(*cuda_jit::buffer_access::state(batch.data), stream);
-        order_read(*cuda_jit::buffer_access::state(c.k), stream);
-        order_read(*cuda_jit::buffer_access::state(c.v), stream);
-        if (plan.data.size_bytes() != 0) order_read(*cuda_jit::buffer_access::state(plan.data), stream);
-
         int64_t longest = batch.longest;
         int width = static_cast<int>(batch.table_width), longest32 = static_cast<int>(longest);
         // Workspace: sums and results of split rows' parts, and for scores the
@@ -1042,17 +1037,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         uint64_t ml = address(scratch), partial = ml + 2 * part_heads * 4, norms = partial + parts * 4,
                  logits = norms + 2 * scored_heads * 4;
         uint64_t work = address(plan.data), join = work + static_cast<uint64_t>(plan.ctas) * 16, err = 0;
-        if (plan.ctas > 0) {
-            check(pbrt_error_word(device, &err));
-            float scale2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
-            void* params[] = {&c.map_k, &c.map_v, &x.ptr, &batch.lengths_at, &batch.tables_at, &work,
-                              &out.ptr, &partial, &ml, &logits, &norms, &width, &group, &chunks,
-                              &x.strides[0], &x.strides[1], &longest32, &scale2, &err};
-            op_launch(kernel_of(kAttention, f, static_cast<uint32_t>(f.smem())), device, stream,
-                      {static_cast<uint32_t>(plan.ctas), 1, 1}, 160, params);
-        }
-        std::vector<tensor> results;
-        results.push_back(finish(std::move(out)));
+        op_kernel* attention = plan.ctas > 0 ? &kernel_of(kAttention, f, static_cast<uint32_t>(f.smem())) : nullptr;
         op_result os;
         int64_t blocks = plan.joins * std::min(group, 8 * f.tiles8);
         // A small block where each row has a few parts (many rows: 128 threads
@@ -1065,13 +1050,30 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             blocks += (longest + 4 * f.join_threads - 1) / (4 * f.join_threads) * n * c.heads;
         }
         expect(blocks <= 0x7fffffff, "paged_attention: too many sequences, heads and slots");
-        if (blocks > 0) {
+        op_kernel* finishing = blocks > 0 ? &kernel_of(kFinish, f, 0) : nullptr;
+        order_read(*cuda_jit::buffer_access::state(batch.data), stream);
+        if (plan.data.size_bytes() != 0) order_read(*cuda_jit::buffer_access::state(plan.data), stream);
+        if (attention != nullptr) {
+            (void)attention->on(device);
+            check(pbrt_error_word(device, &err));
+            float scale2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
+            void* params[] = {&c.map_k, &c.map_v, &x.ptr, &batch.lengths_at, &batch.tables_at, &work,
+                              &out.ptr, &partial, &ml, &logits, &norms, &width, &group, &chunks,
+                              &x.strides[0], &x.strides[1], &longest32, &scale2, &err};
+            std::scoped_lock lock{c.order};
+            order_read(*cuda_jit::buffer_access::state(c.k), stream);
+            order_read(*cuda_jit::buffer_access::state(c.v), stream);
+            op_launch(*attention, device, stream, {static_cast<uint32_t>(plan.ctas), 1, 1}, 160, params);
+        }
+        if (finishing != nullptr) {
             uint64_t split = join + static_cast<uint64_t>(plan.joins) * 16;
             void* params[] = {&join,   &split,   &partial, &ml,  &results_ptr, &logits, &norms,      &batch.lengths_at,
                               &xs.ptr, &os.ptr,  &longest, &ns,  &group,       &chunks, &join_blocks};
-            op_launch(kernel_of(kFinish, f, 0), device, stream, {static_cast<uint32_t>(blocks), 1, 1},
+            op_launch(*finishing, device, stream, {static_cast<uint32_t>(blocks), 1, 1},
                       static_cast<uint32_t>(f.join_threads), params);
         }
+        std::vector<tensor> results;
+        results.push_back(finish(std::move(out)));
         if (scored) results.push_back(finish(std::move(os)));
         return results;
     }

@@ -808,14 +808,16 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
         op_operand xk = operand(k, stream, true), xv = operand(v, stream, true);
         const bool wide = std::min(vector_width(xk), vector_width(xv)) == 4;
         op_kernel& kernel = kernel_of(kAppend, c, wide);
-        order_read(*cuda_jit::buffer_access::state(batch.data), stream);
-        order_write(*cuda_jit::buffer_access::state(c.k), stream);
-        order_write(*cuda_jit::buffer_access::state(c.v), stream);
+        (void)kernel.on(device);
         uint64_t pk = address(c.k), pv = address(c.v);
         const int64_t blocks = (batch.tokens * c.heads * (c.dim / 8) + 255) / 256;
         expect(blocks <= 0x7fffffff, "cache_append: too many new tokens");
         void* params[] = {&xk.ptr,        &xv.ptr,        &pk,            &pv,            &batch.rows_at,
                           &batch.tokens,  &xk.strides[0], &xk.strides[1], &xv.strides[0], &xv.strides[1]};
+        order_read(*cuda_jit::buffer_access::state(batch.data), stream);
+        std::scoped_lock lock{c.order};
+        order_write(*cuda_jit::buffer_access::state(c.k), stream);
+        order_write(*cuda_jit::buffer_access::state(c.v), stream);
         op_launch(kernel, device, stream, {static_cast<uint32_t>(blocks), 1, 1}, 256, params);
     }
 
@@ -855,26 +857,31 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
         int64_t nsv = ns, npv = np;
         select_shape f = shape_for(batch.longest, rows, sm_count(device));
         const bool moves = batch.longest > budget;
-        if (moves) {
-            order_write(*cuda_jit::buffer_access::state(c.k), stream);
-            order_write(*cuda_jit::buffer_access::state(c.v), stream);
-        }
         uint64_t pk = address(c.k), pv = address(c.v);
         int fused = moves && f.held && pairs <= kFewPairs;
+        op_kernel& select = kernel_of(f.held ? kSelect : kSelectLong, c, true, f);
+        op_kernel* move = moves && !fused ? &kernel_of(kMove, c) : nullptr;
+        uint32_t per_row = static_cast<uint32_t>((pairs + 8 * moves_of(c) - 1) / (8 * moves_of(c)));
+        const int64_t blocks = rows * per_row; // of the move
+        expect(move == nullptr || blocks <= 0x7fffffff, "cache_evict: too many rows");
+        (void)select.on(device);
+        if (move != nullptr) (void)move->on(device);
         void* sparams[] = {&xs.ptr, &xp.ptr, &batch.lengths_at, &batch.newest_at, &os.ptr, &op.ptr, &holes,
                            &lates,  &counts, &nsv,              &npv,             &b,      &rc,     &sk,
                            &pairs,  &pk,     &pv,               &batch.tables_at, &width,  &fused};
-        op_launch(kernel_of(f.held ? kSelect : kSelectLong, c, true, f), device, stream,
-                  {static_cast<uint32_t>(rows * f.cluster), 1, 1}, static_cast<uint32_t>(f.threads), sparams,
-                  static_cast<uint32_t>(f.cluster));
-        if (moves && !fused) {
-            uint32_t per_row = static_cast<uint32_t>((pairs + 8 * moves_of(c) - 1) / (8 * moves_of(c)));
-            const int64_t blocks = rows * per_row;
-            expect(blocks <= 0x7fffffff, "cache_evict: too many rows");
-            void* mparams[] = {&pk,     &pv,    &batch.tables_at, &xs.ptr, &xp.ptr, &batch.lengths_at, &batch.newest_at,
-                               &os.ptr, &op.ptr, &holes,          &lates,  &counts, &nsv,              &npv,
-                               &width, &b,      &pairs,           &per_row};
-            op_launch(kernel_of(kMove, c), device, stream, {static_cast<uint32_t>(blocks), 1, 1}, 256, mparams);
+        void* mparams[] = {&pk,     &pv,    &batch.tables_at, &xs.ptr, &xp.ptr, &batch.lengths_at, &batch.newest_at,
+                           &os.ptr, &op.ptr, &holes,          &lates,  &counts, &nsv,              &npv,
+                           &width, &b,      &pairs,           &per_row};
+        {
+            std::scoped_lock lock{c.order};
+            if (moves) {
+                order_write(*cuda_jit::buffer_access::state(c.k), stream);
+                order_write(*cuda_jit::buffer_access::state(c.v), stream);
+            }
+            op_launch(select, device, stream, {static_cast<uint32_t>(rows * f.cluster), 1, 1},
+                      static_cast<uint32_t>(f.threads), sparams, static_cast<uint32_t>(f.cluster));
+            if (move != nullptr)
+                op_launch(*move, device, stream, {static_cast<uint32_t>(blocks), 1, 1}, 256, mparams);
         }
         return {finish(std::move(os)), finish(std::move(op))};
     }

@@ -187,6 +187,49 @@ def test_a_cache_written_by_one_thread_and_read_by_another(gpu):
 
 
 @pytest.mark.gpu
+def test_a_read_beside_writes_of_another_thread_sees_one_of_them(gpu):
+    # All values of a write are one power of two, so the attention is that
+    # number, within the weighted sum's (2 n + 128) u; of two writes at once it
+    # would be something between.
+    import threading
+
+    n, heads, dim = 6000, 4, 64
+    rng = np.random.default_rng(6)
+    host = paged.Host(rng, [n], heads, dim, 32, "f32")
+    cache = gpu.KVCache(host.pages, 32, heads, dim)
+    write = cache.batch(host.tables, [n], appended=[n])
+    read = cache.batch(host.tables, [n], appended=[0])
+    k = gpu.tensor([n, heads, dim], host.k[0])
+    values = [gpu.tensor([n, heads, dim], np.full(n * heads * dim, 2.0**f, np.float32)) for f in range(12)]
+    write.append(k, values[0])
+    q = gpu.tensor([1, 2 * heads, dim], rng.normal(0, 1, (1, 2 * heads, dim)).astype(np.float32))
+    failed = []
+
+    def writer():
+        try:
+            for _ in range(20):
+                for v in values:
+                    write.append(k, v)
+            gpu.synchronize()
+        except Exception as e:  # a thread's exception would be lost
+            failed.append(e)
+
+    th = threading.Thread(target=writer)
+    th.start()
+    got = []
+    while th.is_alive() or len(got) < 50:
+        got.append(gpu.paged_attention(q, read))
+        if len(got) % 20 == 0:
+            gpu.synchronize()
+    th.join()
+    assert not failed
+    for out in got:
+        x = out.cpu()
+        seen = 2.0 ** np.round(np.log2(x[0]))
+        assert (np.abs(x - seen) <= (2 * n + 128) * 2.0**-24 * seen).all()
+
+
+@pytest.mark.gpu
 def test_a_wait_that_runs_out_is_reported_and_the_gpu_recovers(gpu):
     # Block 0's loads are never issued: its bounded waits give up (about two
     # seconds), the kernel records 0x7d00 + site and returns.
