@@ -300,6 +300,11 @@ void pb_kv_cache_release(pb_kv_cache* cache);
 /* Device addresses of the pools and the bytes of each. A raw handle: order
  * other work on it yourself (pb_synchronize). */
 int pb_kv_cache_data(const pb_kv_cache* cache, uint64_t* keys, uint64_t* values, size_t* bytes);
+/* What another library on the same GPU needs to read the pools in place: their
+ * addresses, and this thread's stream (a CUstream), on which everything that
+ * was called on the cache so far is ordered. Asked for again after each call
+ * that the reader has to see. */
+int pb_kv_cache_interface(pb_kv_cache* cache, uint64_t* keys, uint64_t* values, void** stream);
 /* The sequences of one step: `tables` [sequences, width] names the pages of
  * each, `lengths` its slots in use (new tokens included). `appended` (NULL: 1
  * each, 0 for an empty one) says how many of them are new, the last ones;

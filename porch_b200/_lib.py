@@ -114,6 +114,7 @@ def _declare(L: ctypes.CDLL) -> None:
         "pb_kv_cache_create": (c_int, [c_int64, c_int64, c_int64, c_int64, c_int, c_int, P(T)]),
         "pb_kv_cache_release": (None, [T]),
         "pb_kv_cache_data": (c_int, [T, P(c_uint64), P(c_uint64), P(c_size_t)]),
+        "pb_kv_cache_interface": (c_int, [T, P(c_uint64), P(c_uint64), P(c_void_p)]),
         "pb_kv_batch_create": (c_int, [T, P(c_int32), c_size_t, c_size_t, P(c_int64), P(c_int64), P(c_int64), P(T)]),
         "pb_kv_batch_on": (c_int, [T, T, P(T)]),
         "pb_kv_batch_release": (None, [T]),

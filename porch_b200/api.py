@@ -532,16 +532,19 @@ def qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, cos, sin, positions,
 
 class _Pool:
     """A cache pool in place, for another library on the same GPU; a bfloat16
-    pool as its 16 raw bits. Keeps the cache alive."""
+    pool as its 16 raw bits. Keeps the cache alive. Each time it is asked for
+    its interface, the `stream` in it is the calling thread's, behind all that
+    was called on the cache so far."""
 
-    def __init__(self, cache: "KVCache", pointer: int):
-        stream = c_void_p()
-        _check_rt(lib().pbrt_stream_current(cache.device, byref(stream)))
-        self.cache = cache
-        self.__cuda_array_interface__ = {
-            "shape": (cache.pages, cache.kv_heads, cache.page_size, cache.head_dim),
-            "typestr": "<u2" if cache.dtype == "bf16" else "<f4", "data": (pointer, False), "version": 3,
-            "stream": stream.value}
+    def __init__(self, cache: "KVCache", which: int):
+        self.cache, self._which = cache, which
+
+    @property
+    def __cuda_array_interface__(self) -> dict:
+        c, at, stream = self.cache, (c_uint64(), c_uint64()), c_void_p()
+        _check(lib().pb_kv_cache_interface(c._h, byref(at[0]), byref(at[1]), byref(stream)))
+        return {"shape": (c.pages, c.kv_heads, c.page_size, c.head_dim), "typestr": "<u2" if c.dtype == "bf16" else "<f4",
+                "data": (at[self._which].value, False), "version": 3, "stream": stream.value}
 
 
 class KVCache:
@@ -574,8 +577,7 @@ class KVCache:
 
     def pools(self) -> tuple[_Pool, _Pool]:
         """Keys and values in place (__cuda_array_interface__)."""
-        k, v, _ = self.device_data()
-        return _Pool(self, k), _Pool(self, v)
+        return _Pool(self, 0), _Pool(self, 1)
 
     def batch(self, tables, lengths, appended=None, newest=None) -> "Batch":
         """The sequences of one step: tables [sequences, width] of page

@@ -780,6 +780,18 @@ int pb_kv_cache_data(const pb_kv_cache* cache, uint64_t* keys, uint64_t* values,
     });
 }
 
+int pb_kv_cache_interface(pb_kv_cache* cache, uint64_t* keys, uint64_t* values, void** stream) {
+    return guarded([&] {
+        require(cache, "cache");
+        require(keys, "keys");
+        require(values, "values");
+        require(stream, "stream");
+        *stream = porch::detail::cache_ordered(*cache->value);
+        *keys = porch::detail::address(cache->value->k);
+        *values = porch::detail::address(cache->value->v);
+    });
+}
+
 int pb_kv_batch_create(pb_kv_cache* cache, const int32_t* tables, size_t sequences, size_t width,
                        const int64_t* lengths, const int64_t* appended, const int64_t* newest, pb_kv_batch** out) {
     return guarded([&] {

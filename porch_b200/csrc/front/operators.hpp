@@ -126,6 +126,9 @@ namespace porch::detail {
     std::shared_ptr<kv_cache> make_cache(int64_t pages, int64_t page_size, int64_t heads, int64_t dim,
                                          cache_type type, int device);
 
+    // The calling thread's stream, made to wait for what was called on the cache.
+    pbrt_stream cache_ordered(kv_cache& c);
+
     // How attention's CTAs share a batch's slots, uploaded.
     struct batch_plan {
         int64_t chunks = 1; // query heads of a key head come in this many rows

@@ -713,6 +713,14 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
         return c;
     }
 
+    pbrt_stream cache_ordered(kv_cache& c) {
+        auto stream = current_stream(c.device);
+        std::scoped_lock lock{c.order};
+        order_read(*cuda_jit::buffer_access::state(c.k), stream);
+        order_read(*cuda_jit::buffer_access::state(c.v), stream);
+        return stream->stream;
+    }
+
     std::shared_ptr<kv_batch> make_batch(std::shared_ptr<kv_cache> cache, const int32_t* tables, size_t sequences,
                                          size_t width, const int64_t* lengths, const int64_t* appended,
                                          const int64_t* newest) {

@@ -78,3 +78,59 @@ calls["score"]()
 """
     _, log = fake_driver.run(program, tmp_path)
     assert fake_driver.unordered(log, conflict) == []
+
+
+def test_the_pools_interface_names_a_stream_behind_every_call(api, tmp_path):
+    # A reader enqueues its work on the stream that a pool's interface names: a
+    # launch of its own stands for it in the log. Asked from the thread that
+    # called the operators, and from another one.
+    program = SETUP + """
+pools = cache.pools()
+def faces():
+    a, b = (p.__cuda_array_interface__ for p in pools)
+    assert a["stream"] == b["stream"] == q.__cuda_array_interface__["stream"]
+    k, v, _ = cache.device_data()
+    assert (a["data"], b["data"]) == ((k, False), (v, False)) and a["typestr"] == "<u2"
+    assert a["shape"] == (64, 2, 64, 64)
+    return a["stream"]
+for name in ("append", "evict"):
+    kept.append(calls[name]())
+    print(hex(faces()), flush=True)
+seen = []
+kept.append(calls["append"]())
+q = api.tensor([1, 4, 64], np.zeros(256, np.float32))
+t = threading.Thread(target=lambda: (api.zeros([1]).realize(), seen.append(pools[0].__cuda_array_interface__["stream"])))
+t.start()
+t.join()
+print(hex(seen[0]))
+"""
+    out, log = fake_driver.run(program, tmp_path)
+    here, again, other = out.split()
+    assert here == again != other
+    streams = {line[2] for line in log if line[1] == "launch" and line[3] in WRITES}
+    assert streams == {here}
+    log += [["0", "launch", stream, "reader", "1", "1", "0"] for stream in (here, other)]
+    assert fake_driver.unordered(log, lambda a, b: a in WRITES and b == "reader") == []
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_pools_read_behind_the_stream_of_their_interface(gpu, dtype):
+    # Nothing but the stream orders the copy behind a write that takes long.
+    import numpy as np
+
+    torch = pytest.importorskip("torch")
+    n = 1 << 17
+    cache = gpu.KVCache(n // 256, 256, 2, 64, dtype)
+    batch = cache.batch(np.arange(n // 256)[None], [n], appended=[n])
+    pools = cache.pools()
+    rows = [gpu.tensor([n, 2, 64], np.full(n * 128, x, np.float32)) for x in (1.0, 2.0, 4.0)]
+    for x, r in zip((1.0, 2.0, 4.0), rows):
+        for other in rows:
+            batch.append(other, other)
+        batch.append(r, r)
+        stream = torch.cuda.ExternalStream(pools[1].__cuda_array_interface__["stream"])
+        with torch.cuda.stream(stream):
+            got = torch.as_tensor(pools[1], device="cuda").clone()
+        stream.synchronize()
+        assert bool((got.view(torch.bfloat16 if dtype == "bf16" else torch.float32) == x).all())
