@@ -325,7 +325,9 @@ int pb_kv_append(pb_kv_batch* batch, const pb_tensor* k, const pb_tensor* v);
  * i reads key head i / (q_heads / kv_heads)). An empty sequence gives zeros.
  * Sums, maxima and the result are float32 for either cache type. A query, or
  * a key or value in use, that is not finite makes results of the heads that
- * read it not finite (infinity or NaN), and no others. */
+ * read it not finite (infinity or NaN), and no others. A logit below float32's
+ * range weighs 0; one above it, or a row of which every logit lies below it,
+ * gives NaN. */
 int pb_paged_attention(const pb_tensor* q, pb_kv_batch* batch, float scale, pb_tensor** out);
 /* How the attention of a batch with these lengths is shared out over about
  * `ctas` CTAs, as text, without a GPU: a row is a (sequence, key head, chunk of

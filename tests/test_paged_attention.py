@@ -77,6 +77,30 @@ def test_logits_far_apart(gpu, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("length,below", [(100, 64), (200, 130), (9001, 8000), (9001, 9000), (70000, 60001)])
+def test_logits_below_the_range_of_float32_weigh_nothing(gpu, dtype, length, below):
+    # The first `below` slots' logits are -2^134 x scale, past float32's range:
+    # whole tiles, and whole parts of a row, with a maximum of -inf. What is left
+    # is the attention of the other slots.
+    rng = np.random.default_rng(length)
+    host = paged.Host(rng, [length], 2, 64, 32, dtype)
+    host.k[0][:, :, 0] = 0
+    host.k[0][:below, :, 0] = -(2.0**84)
+    _, batch = host.build(gpu)
+    q = rng.normal(0, 1, (1, 6, 64)).astype(np.float32)
+    q[:, :, 0] = 2.0**50
+    t = gpu.tensor([1, 6, 64], q)
+    host.k[0], host.v[0], host.lengths = host.k[0][below:], host.v[0][below:], [length - below]
+    out, tol, new, new_tol = host.attend(np.where(np.arange(64) == 0, 0, q).astype(np.float32), 0.125)
+    assert (np.abs(gpu.paged_attention(t, batch, scale=0.125).cpu().reshape(q.shape) - out) <= tol).all()
+    got, weights = gpu.paged_attention_scored(t, batch, scale=0.125)
+    assert (np.abs(got.cpu().reshape(q.shape) - out) <= tol).all()
+    w = weights.cpu().reshape(1, 2, length)
+    assert not w[:, :, :below].any() and (np.abs(w[:, :, below:] - new) <= new_tol).all()
+
+
+@pytest.mark.gpu
 def test_values_that_are_not_finite_stay_in_their_row(gpu):
     rng = np.random.default_rng(2)
     host = paged.Host(rng, [100, 90, 65], 2, 64, 16, "bf16")
