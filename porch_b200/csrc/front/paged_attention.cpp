@@ -162,10 +162,10 @@ static __device__ __forceinline__ float pb_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// What weights are taken relative to, given the maximum so far: where that is
-// -inf (every logit so far lies below float32's range), 0, so that their
-// weights are 0 instead of the NaN of -inf - -inf.
-static __device__ __forceinline__ float pb_base(float top) { return top == __int_as_float(0xff800000) ? 0.0f : top; }
+// What a maximum over logits begins with: the lowest finite value, so that
+// logits of -inf (below float32's range) weigh exp2(-inf) = 0 also where a tile
+// or a part holds no other; from -inf they would be the NaN of -inf - -inf.
+#define PB_LOWEST __int_as_float(0xff7fffff)
 
 static __device__ __forceinline__ void pb_ldm4(pb_u32* r, pb_u32 addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -405,7 +405,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
 #pragma unroll
             for (int n = 0; n < PB_NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) { m[n][e] = __int_as_float(0xff800000); l[n][e] = 0.0f; }
+                for (int e = 0; e < 2; ++e) { m[n][e] = PB_LOWEST; l[n][e] = 0.0f; }
 #pragma unroll
             for (int a = 0; a < PB_MTW; ++a)
 #pragma unroll
@@ -526,14 +526,13 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const float now = fmaxf(m[n][e], top[n][e]);
-                top[n][e] = pb_base(now);
-                corr[n][e] = pb_exp2(m[n][e] - top[n][e]);
+                corr[n][e] = pb_exp2(m[n][e] - now);
                 m[n][e] = now;
                 l[n][e] *= corr[n][e];
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float p = pb_exp2(s[n][e] - top[n][e & 1]);
+                const float p = pb_exp2(s[n][e] - m[n][e & 1]);
                 l[n][e & 1] += p;
                 const int at_slot = 16 * warp + g + (e >> 1) * 8, head = 8 * n + 2 * t + (e & 1);
 #if PB_ESZ == 2
@@ -726,9 +725,9 @@ static __device__ __forceinline__ void pb_join(const int4* joins, const float* p
         x = top;
 #pragma unroll
         for (int w = 0; w < PB_JOIN_THREADS / 32; ++w) x = fmaxf(x, reduce[w]);
-        const float base = pb_base(x), corr = pb_exp2(top - base);
+        const float corr = pb_exp2(top - x);
         top = x;
-        const float w = threadIdx.x < n ? pb_exp2(ml.x - base) : 0.0f;
+        const float w = threadIdx.x < n ? pb_exp2(ml.x - top) : 0.0f;
         weight[threadIdx.x] = w;
         float y = w * ml.y;
 #pragma unroll
@@ -823,8 +822,8 @@ static __device__ __forceinline__ void pb_scores(const int4* joins, const int* s
                 const int4 r = joins[at];
                 for (int i = lane; i < r.z; i += 32) {
                     const float2 ml = partial_ml[pb_part(r, i, g % PB_HT)];
-                    const float now = fmaxf(top, ml.x), base = pb_base(now);
-                    sum = fmaf(sum, pb_exp2(top - base), ml.y * pb_exp2(ml.x - base));
+                    const float now = fmaxf(top, ml.x);
+                    sum = fmaf(sum, pb_exp2(top - now), ml.y * pb_exp2(ml.x - now));
                     top = now;
                 }
             }
