@@ -339,7 +339,12 @@ int pb_paged_attention(const pb_tensor* q, pb_kv_batch* batch, float scale, pb_t
 int pb_kv_plan_describe(const int64_t* lengths, size_t sequences, int64_t kv_heads,
                         int64_t chunks, int64_t ctas, char* text, size_t capacity,
                         size_t* needed);
-/* The same, and new scores [sequences, kv_heads, longest length]: `scores`
+/* How many CTAs of an SM the attention counts on that serves `group` query
+ * heads of each key head from a cache of this head size and type, and the bytes
+ * of shared memory that each of them takes, the system's share included. */
+int pb_kv_attention_shape(int64_t head_dim, int type, int64_t group, int64_t* ctas_per_sm,
+                          int64_t* shared_bytes);
+/* As pb_paged_attention, and new scores [sequences, kv_heads, longest length]: `scores`
  * (NULL or slots past its end: 0) plus each slot's attention weight summed
  * over the query heads of its key head; 0 past a sequence's length. Takes 4
  * bytes of workspace per query head and slot. */

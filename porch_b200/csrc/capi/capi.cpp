@@ -895,6 +895,19 @@ int pb_kv_plan_describe(const int64_t* lengths, size_t sequences, int64_t kv_hea
     });
 }
 
+int pb_kv_attention_shape(int64_t head_dim, int type, int64_t group, int64_t* ctas_per_sm, int64_t* shared_bytes) {
+    return guarded([&] {
+        require(ctas_per_sm, "ctas_per_sm");
+        require(shared_bytes, "shared_bytes");
+        if (head_dim < 8 || head_dim > 256 || head_dim % 8 != 0 || type < PB_CACHE_F32 || type > PB_CACHE_BF16 || group < 1)
+            throw std::invalid_argument("attention shape: no such head size, type or group");
+        const auto [ctas, bytes] =
+            porch::detail::attention_shape(head_dim, static_cast<porch::detail::cache_type>(type), group);
+        *ctas_per_sm = ctas;
+        *shared_bytes = bytes;
+    });
+}
+
 int pb_operator_sources(char* text, size_t capacity, size_t* needed) {
     return guarded([&] { copy_text(porch::detail::operator_sources(), text, capacity, needed); });
 }

@@ -165,6 +165,9 @@ namespace porch::detail {
 
     const batch_plan& plan_of(kv_batch& batch, int64_t chunks, int64_t ctas);
     int attention_ctas_per_sm(const kv_cache& c);
+    // How many CTAs of an SM a plan for `group` query heads of each key head
+    // counts on, and the bytes of shared memory that each takes.
+    std::pair<int, int> attention_shape(int64_t dim, cache_type type, int64_t group);
     // Test hook (0: off): block 0 of an attention never gets its tiles, so its
     // bounded waits expire (1), or gives up while its first ones are on their
     // way (2).

@@ -65,11 +65,18 @@ namespace porch::detail {
             int q_row() const { return steps() * 32 + 16; }
             int p_row() const { return 64 * width() + 16; }
             int small() const { // everything but the ring
-                return terms() * tiles8 * 8 * (q_row() + p_row()) + 2 * 4 * tiles8 * 8 * 4 + 256;
+                return terms() * tiles8 * 8 * (q_row() + p_row()) + 2 * 4 * tiles8 * 8 * 4;
             }
             int per_sm() const { return choose().first; }
             int ring() const { return choose().second; }
+            int chunks(int group) const { return (group + 8 * tiles8 - 1) / (8 * tiles8); } // rows of a key head
             int smem() const { return 1024 + ring() * unit() + small(); }
+            // What a CTA takes of an SM's 228 KB: that, the kernel's static
+            // arrays (the ring's barriers and a flag, which the kernel checks
+            // against kStatic) with the rounding of the sum, and the KB that
+            // the system keeps for each CTA.
+            static constexpr int kStatic = 256;
+            int shared() const { return smem() + kStatic + 1024; }
 
           private:
             // CTAs of an SM and units of a CTA's ring: as many CTAs as leave
@@ -79,10 +86,10 @@ namespace porch::detail {
             // units, 124 with three of three).
             std::pair<int, int> choose() const {
                 for (int n = 4; n > 1; --n) {
-                    const int r = ((228 * 1024) / n - 2048 - small()) / unit();
+                    const int r = ((228 * 1024) / n - 2048 - kStatic - small()) / unit();
                     if (r >= 3) return {n, std::min(r, 6)};
                 }
-                return {1, std::min((227 * 1024 - 1024 - small()) / unit(), 6)};
+                return {1, std::min((227 * 1024 - 1024 - kStatic - small()) / unit(), 6)};
             }
         };
 
@@ -279,6 +286,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
     extern __shared__ char raw[];
     __shared__ pb_u64 bars[2 * PB_RING];
     __shared__ int abort_flag;
+    static_assert(sizeof(bars) + sizeof(abort_flag) + 128 <= PB_STATIC, "shared memory that the launch does not count");
     const pb_u32 ring = (pb_smem(raw) + 1023u) & ~1023u;
     const pb_u32 qs = ring + PB_RING * PB_UNIT;
     const pb_u32 ps = qs + PB_TERMS * PB_HT * PB_QROW;
@@ -877,12 +885,25 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             os << "#define PB_H " << f.heads << "\n#define PB_D " << f.dim << "\n#define PB_PS " << f.page
                << "\n#define PB_ESZ " << f.width() << "\n#define PB_NT " << f.tiles8 << "\n#define PB_RING " << f.ring()
                << "\n#define PB_JOIN_THREADS " << f.join_threads << "\n#define PB_PER_SM " << f.per_sm()
-               << "\n#define PB_SCORED " << (f.scored ? 1 : 0) << "\n";
+               << "\n#define PB_STATIC " << form::kStatic << "\n#define PB_SCORED " << (f.scored ? 1 : 0) << "\n";
             if (f.stall != 0) os << "#define PB_TEST_STALL " << f.stall << "\n";
             return os.str();
         }
 
         std::atomic<int> g_test_stall{0};
+
+        // The form for `group` query heads of each key head: 16 share a tile's
+        // loads, 8 where 16 would leave the ring less than three units.
+        form form_of(const kv_cache& c, int64_t group) {
+            form f;
+            f.heads = static_cast<int>(c.heads);
+            f.dim = static_cast<int>(c.dim);
+            f.page = static_cast<int>(c.page_size);
+            f.bf16 = c.type == cache_type::bf16;
+            f.tiles8 = group > 8 ? 2 : 1;
+            if (f.ring() < 3) f.tiles8 = 1;
+            return f;
+        }
 
         const char kAttention[] = "pb_paged_attention";
         const char kFinish[] = "pb_paged_finish";
@@ -1010,19 +1031,11 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         auto stream = current_stream(device);
         op_operand x = operand(q, stream, true), xs;
         if (scores != nullptr) xs = operand(*scores, stream, false);
-        form f;
-        f.heads = static_cast<int>(c.heads);
-        f.dim = static_cast<int>(c.dim);
-        f.page = static_cast<int>(c.page_size);
-        f.bf16 = c.type == cache_type::bf16;
+        int heads = static_cast<int>(shape[1]), group = static_cast<int>(shape[1] / c.heads);
+        form f = form_of(c, group);
         f.scored = scored;
         f.stall = g_test_stall.load(std::memory_order_relaxed);
-        int heads = static_cast<int>(shape[1]), group = static_cast<int>(shape[1] / c.heads);
-        // 16 query heads share a tile's loads, 8 where 16 would leave the ring
-        // less than three units.
-        f.tiles8 = group > 8 ? 2 : 1;
-        if (f.ring() < 3) f.tiles8 = 1;
-        int chunks = (group + 8 * f.tiles8 - 1) / (8 * f.tiles8);
+        int chunks = f.chunks(group);
         const int64_t rows = n * c.heads * chunks;
         expect(rows < (int64_t{1} << 27), "paged_attention: too many sequences and heads");
         const batch_plan& plan = plan_of(batch, chunks, int64_t{f.per_sm()} * sm_count(device));
@@ -1084,12 +1097,14 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
 
     void set_test_attention_stall(int mode) { g_test_stall.store(mode); }
 
-    int attention_ctas_per_sm(const kv_cache& c) {
-        form f;
-        f.heads = static_cast<int>(c.heads);
-        f.dim = static_cast<int>(c.dim);
-        f.bf16 = c.type == cache_type::bf16;
-        return f.per_sm();
+    int attention_ctas_per_sm(const kv_cache& c) { return form_of(c, 1).per_sm(); }
+
+    std::pair<int, int> attention_shape(int64_t dim, cache_type type, int64_t group) {
+        kv_cache c;
+        c.dim = dim;
+        c.type = type;
+        const form f = form_of(c, group);
+        return {f.per_sm(), f.shared()};
     }
 
     const batch_plan& plan_of(kv_batch& batch, int64_t chunks, int64_t ctas) {

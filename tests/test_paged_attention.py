@@ -352,6 +352,24 @@ def test_refusals_that_need_no_device(api):
         api.KVCache(4, 16, 1, 64, dtype="f16")
 
 
+def test_the_ctas_that_a_plan_counts_on_fit_an_sm(api):
+    # An SM has 228 KB of shared memory for its CTAs; of one's, 1 KB is the
+    # system's and at most 227 KB the kernel's. A group of 1, and of 9, which
+    # may take the wider form.
+    from ctypes import byref, c_int64
+
+    from porch_b200._lib import lib
+
+    for dim in range(8, 257, 8):
+        for kind in (0, 1):
+            for group in (1, 9):
+                ctas, shared = c_int64(), c_int64()
+                assert lib().pb_kv_attention_shape(dim, kind, group, byref(ctas), byref(shared)) == 0
+                assert ctas.value >= 1 and ctas.value * shared.value <= 228 * 1024, (dim, kind, group)
+    for bad in ((0, 0, 1), (12, 0, 1), (264, 0, 1), (64, 2, 1), (64, 0, 0)):
+        assert lib().pb_kv_attention_shape(*bad, byref(ctas), byref(shared)) != 0
+
+
 @pytest.mark.parametrize("seed", range(40))
 def test_every_tile_is_worked_on_once_and_every_split_row_joined(api, seed):
     # Walks the CTAs as the kernel does.
