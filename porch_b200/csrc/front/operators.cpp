@@ -27,7 +27,8 @@ namespace porch::detail {
         if (f != nullptr) return f;
         std::scoped_lock lock{mutex};
         check(pbrt_get_function(device, image_key, name.c_str(), &f));
-        if (smem > 48 * 1024) check(pbrt_function_set_max_dynamic_smem(f, static_cast<int>(smem)));
+        // The default limit of 48 KB is on dynamic and static memory together.
+        if (smem != 0) check(pbrt_function_set_max_dynamic_smem(f, static_cast<int>(smem)));
         slot.store(f, std::memory_order_release);
         return f;
     }

@@ -7,6 +7,8 @@
  *   <thread> record <stream> <event> | wait <stream> <event> | sync <stream>
  *   <thread> copy <stream> | create <stream> | load
  *   <thread> compile <seconds>           (1 where the source has the text FAKE_CUDA_SLOW_COMPILE, else 0)
+ * As the driver, it refuses a launch of over 48 KB of shared memory that was not
+ * asked for; of the static kind it takes every kernel to have a quarter KB.
  * Built and loaded by fake_driver.py. No GPU is involved. */
 #define _GNU_SOURCE
 #include <cuda.h>
@@ -101,11 +103,17 @@ CUresult cuMemsetD32Async(CUdeviceptr p, unsigned int v, size_t n, CUstream s) {
 CUresult cuDeviceCanAccessPeer(int* can, CUdevice a, CUdevice b) { *can = 0; return CUDA_SUCCESS; }
 CUresult cuCtxEnablePeerAccess(CUcontext c, unsigned int flags) { return CUDA_SUCCESS; }
 CUresult cuModuleLoadData(CUmodule* m, const void* image) { *m = handle(); say("load"); return CUDA_SUCCESS; }
+struct function { char name[64]; unsigned dynamic; };
 CUresult cuModuleGetFunction(CUfunction* f, CUmodule m, const char* name) {
-    *f = (CUfunction)strdup(name);
+    struct function* x = calloc(1, sizeof *x);
+    strncpy(x->name, name, sizeof x->name - 1);
+    *f = (CUfunction)x;
     return CUDA_SUCCESS;
 }
-CUresult cuFuncSetAttribute(CUfunction f, CUfunction_attribute a, int v) { return CUDA_SUCCESS; }
+CUresult cuFuncSetAttribute(CUfunction f, CUfunction_attribute a, int v) {
+    if (a == CU_FUNC_ATTRIBUTE_MAX_DYNAMIC_SHARED_SIZE_BYTES) ((struct function*)f)->dynamic = v;
+    return CUDA_SUCCESS;
+}
 CUresult cuFuncGetAttribute(int* v, CUfunction_attribute a, CUfunction f) { *v = 0; return CUDA_SUCCESS; }
 CUresult cuOccupancyMaxActiveBlocksPerMultiprocessor(int* n, CUfunction f, int threads, size_t smem) {
     *n = 1;
@@ -113,7 +121,9 @@ CUresult cuOccupancyMaxActiveBlocksPerMultiprocessor(int* n, CUfunction f, int t
 }
 CUresult cuOccupancyMaxActiveClusters(int* n, CUfunction f, const CUlaunchConfig* c) { *n = 1; return CUDA_SUCCESS; }
 CUresult cuLaunchKernelEx(const CUlaunchConfig* c, CUfunction f, void** params, void** extra) {
-    const char *name = (const char*)f, *slow = getenv("FAKE_CUDA_SLOW");
+    const char *name = ((struct function*)f)->name, *slow = getenv("FAKE_CUDA_SLOW");
+    const unsigned dynamic = c->sharedMemBytes, asked = ((struct function*)f)->dynamic;
+    if (dynamic > asked && dynamic + 256 > 48 * 1024) return CUDA_ERROR_INVALID_VALUE;
     if (slow != NULL && strcmp(slow, name) == 0) {
         say("begin %p %s", c->hStream, name);
         usleep(400000);
