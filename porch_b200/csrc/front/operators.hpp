@@ -104,6 +104,14 @@ namespace porch::detail {
     // --------------------------------------------------------------- cache --
     enum class cache_type : int { f32 = 0, bf16 = 1 };
 
+    // How the last attention over a cache shared out its work, for which the
+    // next batch prepares its plan: with the upload that the batch waits for
+    // anyway, instead of one that the step's first attention would wait for.
+    struct plan_hint {
+        std::mutex mutex;
+        int64_t chunks = 0, ctas = 0; // 0: none yet
+    };
+
     // Pools of pages of keys and values: [pages, heads, page_size, dim], so
     // the rows of one page and head are one contiguous block.
     struct kv_cache {
@@ -116,6 +124,7 @@ namespace porch::detail {
         // order of their kernels. Kernels are compiled and memory is allocated
         // before it is taken.
         std::mutex order;
+        std::shared_ptr<plan_hint> hint = std::make_shared<plan_hint>();
         int width() const { return type == cache_type::bf16 ? 2 : 4; } // bytes of a value
         // TMA maps of both pools as [rows, dim]: boxes of 128 bytes by a page,
         // or by 64 rows of a larger one.
@@ -138,6 +147,7 @@ namespace porch::detail {
         cuda_jit::device_buffer data; // 16 bytes per CTA, then 16 per row to join
     };
     struct batch_plans {
+        std::shared_ptr<plan_hint> hint; // of the cache that the batch was made for
         std::mutex mutex;
         std::vector<std::unique_ptr<batch_plan>> made;
     };
@@ -153,8 +163,9 @@ namespace porch::detail {
         int64_t table_width = 0;
         bool shared_pages = false;       // a page serves two sequences, or one twice
         cuda_jit::device_buffer data;    // int32: lengths, newest, tables, then 8-byte rows
-        // Made once with the batch for the usual number of query heads, and
-        // by the first call that needs another.
+        // Made once with the batch for the number of query heads that its cache
+        // last saw (up to 8 for each key head until then), and by the first
+        // call that needs another.
         std::shared_ptr<batch_plans> plans = std::make_shared<batch_plans>();
         uint64_t lengths_at = 0, newest_at = 0, tables_at = 0, rows_at = 0; // device addresses
         int64_t sequences() const { return static_cast<int64_t>(lengths.size()); }
@@ -163,8 +174,10 @@ namespace porch::detail {
                                          size_t width, const int64_t* lengths, const int64_t* appended,
                                          const int64_t* newest);
 
+    // The plan for this many chunks and CTAs, which the cache's next batch gets.
     const batch_plan& plan_of(kv_batch& batch, int64_t chunks, int64_t ctas);
-    int attention_ctas_per_sm(const kv_cache& c);
+    // The plan that a new batch begins with.
+    void prepare_plan(kv_batch& batch);
     // How many CTAs of an SM a plan for `group` query heads of each key head
     // counts on, and the bytes of shared memory that each takes.
     std::pair<int, int> attention_shape(int64_t dim, cache_type type, int64_t group);

@@ -1097,8 +1097,6 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
 
     void set_test_attention_stall(int mode) { g_test_stall.store(mode); }
 
-    int attention_ctas_per_sm(const kv_cache& c) { return form_of(c, 1).per_sm(); }
-
     std::pair<int, int> attention_shape(int64_t dim, cache_type type, int64_t group) {
         kv_cache c;
         c.dim = dim;
@@ -1108,6 +1106,11 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
     }
 
     const batch_plan& plan_of(kv_batch& batch, int64_t chunks, int64_t ctas) {
+        if (batch.plans->hint != nullptr) {
+            std::scoped_lock lock{batch.plans->hint->mutex};
+            batch.plans->hint->chunks = chunks;
+            batch.plans->hint->ctas = ctas;
+        }
         std::scoped_lock lock{batch.plans->mutex};
         for (const auto& p : batch.plans->made)
             if (p->chunks == chunks && p->limit == ctas) return *p;
@@ -1128,6 +1131,20 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         check(pbrt_stream_synchronize(device, stream->stream));
         batch.plans->made.push_back(std::move(p));
         return *batch.plans->made.back();
+    }
+
+    void prepare_plan(kv_batch& batch) {
+        int64_t chunks = 0, ctas = 0;
+        {
+            std::scoped_lock lock{batch.plans->hint->mutex};
+            chunks = batch.plans->hint->chunks;
+            ctas = batch.plans->hint->ctas;
+        }
+        if (chunks == 0) {
+            chunks = 1;
+            ctas = int64_t{form_of(*batch.cache, 1).per_sm()} * sm_count(batch.cache->device);
+        }
+        (void)plan_of(batch, chunks, ctas);
     }
 
     std::string attention_schedule(const std::vector<int64_t>& lengths, int64_t heads, int64_t chunks, int64_t ctas) {

@@ -790,7 +790,8 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
         b->newest_at = at + sequences * sizeof(int32_t);
         b->tables_at = at + tables_from * sizeof(int32_t);
         b->rows_at = at + rows_from * sizeof(int32_t);
-        (void)plan_of(*b, 1, int64_t{attention_ctas_per_sm(*cache)} * sm_count(cache->device));
+        b->plans->hint = cache->hint;
+        prepare_plan(*b);
         return b;
     }
 

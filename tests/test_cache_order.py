@@ -113,6 +113,29 @@ print(hex(seen[0]))
     assert fake_driver.unordered(log, lambda a, b: a in WRITES and b == "reader") == []
 
 
+@pytest.mark.parametrize("group,dim,dtype", [(1, 64, "bf16"), (12, 128, "f32"), (17, 64, "bf16"), (40, 64, "f32")])
+def test_a_step_uploads_and_waits_only_where_its_batch_is_made(api, tmp_path, group, dim, dtype):
+    # From the second step on an attention only enqueues, whatever the number of
+    # query heads, over the batch's own cache and another layer's, and a batch
+    # makes two uploads.
+    program = f"""
+caches = [api.KVCache(8, 64, 2, {dim}, "{dtype}") for _ in range(2)]
+q = api.tensor([2, 2 * {group}, {dim}], np.ones(4 * {group} * {dim}, np.float32))
+lines = lambda: [l.split()[1] for l in open(os.environ["FAKE_CUDA_LOG"])]
+busy = lambda l: (l.count("copy"), l.count("sync"))
+for step in range(3):
+    a = len(lines())
+    batch = caches[0].batch(np.arange(8).reshape(2, 4), [100 + step, 50])
+    b = len(lines())
+    for c in caches:
+        api.paged_attention_scored(q, batch.on(c))
+    log = lines()
+    print(*busy(log[a:b]), *busy(log[b:]))
+"""
+    out, _ = fake_driver.run(program, tmp_path)
+    assert out.splitlines()[1:] == ["2 2 0 0"] * 2
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_pools_read_behind_the_stream_of_their_interface(gpu, dtype):
