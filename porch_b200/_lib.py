@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes
 import importlib.util
+import sysconfig
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p
 from pathlib import Path
 
@@ -16,6 +17,7 @@ class pb_index(ctypes.Structure):
 
 
 _lib = None
+_binding = None
 
 
 def lib() -> ctypes.CDLL:
@@ -32,21 +34,31 @@ def lib() -> ctypes.CDLL:
         ctypes.CDLL("libstdc++.so.6", mode=ctypes.RTLD_GLOBAL)
         L = ctypes.CDLL(str(LIBRARY), mode=ctypes.RTLD_GLOBAL)
         _declare(L)
+        binding().connect(str(LIBRARY))
         _lib = L
     return _lib
 
 
+def binding_path() -> Path:
+    """The compiled part of the binding, named after the interpreter that it is
+    built for."""
+    return LIBRARY.parent / f"_binding{sysconfig.get_config_var('EXT_SUFFIX')}"
+
+
 def binding():
-    """The compiled part of the binding (porch_b200/csrc/python/binding.cpp),
-    behind the library that it calls."""
-    lib()
-    path = LIBRARY.parent / "_binding.so"
-    if not path.exists():
-        raise ImportError(f"{path} is not built; run `python -m porch_b200.build`")
-    spec = importlib.util.spec_from_file_location("porch_b200._binding", path)
-    module = importlib.util.module_from_spec(spec)
-    spec.loader.exec_module(module)
-    return module
+    """The compiled part of the binding (porch_b200/csrc/python/binding.cpp), or,
+    for an interpreter that it was not built for, the same in ctypes. Loads no
+    native library: lib() does, and connects it."""
+    global _binding
+    if _binding is None:
+        path = binding_path()
+        if path.exists():
+            spec = importlib.util.spec_from_file_location("porch_b200._binding", path)
+            _binding = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(_binding)
+        else:
+            from . import ctypes_binding as _binding
+    return _binding
 
 
 def _declare(L: ctypes.CDLL) -> None:

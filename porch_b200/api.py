@@ -388,7 +388,7 @@ def as_tensor(e) -> Tensor:
     return _expr(e).to_tensor()
 
 
-_binding.bind(Tensor, materialize, _check)
+_binding.bind(Tensor, materialize, _check, lib)
 
 
 def add(a, b):

@@ -33,7 +33,8 @@ CSRC = PACKAGE / "csrc"
 LIB_DIR = PACKAGE / "lib"
 OBJ_DIR = ROOT / "_build" / "obj"
 LIBRARY = LIB_DIR / "libporch_b200.so"
-BINDING = LIB_DIR / "_binding.so"  # compiled part of the Python binding
+# The compiled part of the Python binding, for the interpreter that runs this.
+BINDING = LIB_DIR / f"_binding{sysconfig.get_config_var('EXT_SUFFIX')}"
 
 CUDA_HOME = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
 # The system g++ links the C++ runtime dynamically; a toolchain wrapper that
@@ -111,14 +112,18 @@ def build(force: bool = False) -> Path:
 
 
 def _build_binding(force: bool = False) -> None:
-    """The extension module that api.py imports, for the interpreter that runs
-    this; it finds the library beside it."""
+    """The extension module that api.py imports. An interpreter without headers
+    goes without it (porch_b200/ctypes_binding.py)."""
+    include = Path(sysconfig.get_paths()["include"])
+    if not (include / "Python.h").exists():
+        print(f"porch_b200: no Python headers in {include}; the binding stays with ctypes", file=sys.stderr)
+        return
     newest = max(p.stat().st_mtime for p in [BINDING_SOURCE, ROOT / "include" / "porch_b200.h", Path(__file__)])
     if BINDING.exists() and not force and BINDING.stat().st_mtime >= newest:
         return
     tmp = BINDING.with_suffix(".so.tmp")
-    cmd = [CXX, *CXXFLAGS, "-Wno-missing-field-initializers", f"-I{sysconfig.get_paths()['include']}", "-shared",
-           str(BINDING_SOURCE), "-o", str(tmp), f"-L{LIB_DIR}", "-lporch_b200", "-Wl,-rpath,$ORIGIN"]
+    cmd = [CXX, *CXXFLAGS, "-Wno-missing-field-initializers", f"-I{include}", "-shared", str(BINDING_SOURCE),
+           "-o", str(tmp), "-ldl"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"binding failed: {' '.join(cmd)}\n{res.stderr}")

@@ -2,15 +2,37 @@
 // and the decode-step operators, whose kernels take a few microseconds. A
 // ctypes call of such an operator cost 2 to 5 us more than the operator, and
 // handing a result to another library 2 us more; everything else stays with
-// ctypes (porch_b200/api.py).
+// ctypes (porch_b200/api.py). Interpreters that this module was not built for use
+// porch_b200/ctypes_binding.py in its place.
+//
+// The native library is not linked: importing the module does not load it, and
+// porch_b200/_lib.py hands it over (connect) once the first use has.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
 #include "porch_b200.h"
 
 #include <array>
+#include <dlfcn.h>
 
 namespace {
+
+    // The library's functions that are called here.
+#define PB_CALLS(X)                                                                                          \
+    X(pb_tensor_release)                                                                                     \
+    X(pb_tensor_interface)                                                                                   \
+    X(pb_qk_norm_rope)                                                                                       \
+    X(pb_qk_norm_rope_backward)                                                                              \
+    X(pb_paged_attention)                                                                                    \
+    X(pb_paged_attention_scored)                                                                             \
+    X(pb_kv_evict)
+#define PB_POINTER(name) decltype(&::name) name = nullptr;
+    struct {
+        PB_CALLS(PB_POINTER)
+    } native;
+#undef PB_POINTER
+    bool g_connected = false;
+    PyObject* g_load = nullptr; // loads the library and connects it
 
     PyObject* g_tensor_type = nullptr; // api.Tensor, the type of results
     PyObject* g_realise = nullptr;     // realises an expression
@@ -22,9 +44,23 @@ namespace {
         PyObject* face; // __cuda_array_interface__, once asked for
     };
 
+    void release(pb_tensor* t) { // a tensor exists only once the library does
+        if (t != nullptr && g_connected) native.pb_tensor_release(t);
+    }
+
+    // Whether the library is there; loads it, or sets the exception.
+    bool ready() {
+        if (g_connected) return true;
+        PyObject* r = g_load == nullptr ? nullptr : PyObject_CallNoArgs(g_load);
+        Py_XDECREF(r);
+        if (g_connected) return true;
+        if (!PyErr_Occurred()) PyErr_SetString(PyExc_ImportError, "the native library is not connected");
+        return false;
+    }
+
     void handle_dealloc(PyObject* self) {
         auto* h = reinterpret_cast<handle_object*>(self);
-        if (h->tensor != nullptr) pb_tensor_release(h->tensor);
+        release(h->tensor);
         Py_XDECREF(h->face);
         Py_TYPE(self)->tp_free(self);
     }
@@ -35,7 +71,7 @@ namespace {
         void* p = value == Py_None ? nullptr : PyLong_AsVoidPtr(value);
         if (p == nullptr && PyErr_Occurred()) return -1;
         auto* h = reinterpret_cast<handle_object*>(self);
-        if (h->tensor != nullptr) pb_tensor_release(h->tensor);
+        release(h->tensor);
         Py_CLEAR(h->face);
         h->tensor = static_cast<pb_tensor*>(p);
         return 0;
@@ -65,7 +101,7 @@ namespace {
         auto* h = reinterpret_cast<handle_object*>(self);
         if (h->face == nullptr) {
             int64_t v[19];
-            if (!checked(pb_tensor_interface(h->tensor, v, 19))) return nullptr;
+            if (!ready() || !checked(native.pb_tensor_interface(h->tensor, v, 19))) return nullptr;
             PyObject* shape = PyTuple_New(static_cast<Py_ssize_t>(v[0]));
             if (shape == nullptr) return nullptr;
             for (int64_t i = 0; i < v[0]; ++i) PyTuple_SET_ITEM(shape, i, PyLong_FromLongLong(v[3 + i]));
@@ -91,7 +127,7 @@ namespace {
         auto* type = reinterpret_cast<PyTypeObject*>(g_tensor_type);
         PyObject* self = type->tp_alloc(type, 0);
         if (self == nullptr) {
-            pb_tensor_release(t);
+            release(t);
             return nullptr;
         }
         reinterpret_cast<handle_object*>(self)->tensor = t;
@@ -104,7 +140,7 @@ namespace {
         bool good = out != nullptr;
         for (size_t i = 0; i < N; ++i) {
             if (!good) {
-                pb_tensor_release(t[i]);
+                release(t[i]);
                 continue;
             }
             PyObject* x = wrap(t[i]);
@@ -160,6 +196,7 @@ namespace {
 
     template <typename F>
     bool call(F&& f) {
+        if (!ready()) return false;
         int status = 0;
         Py_BEGIN_ALLOW_THREADS // a first call compiles its kernel
         status = f();
@@ -176,7 +213,7 @@ namespace {
         if (interleaved < 0) return nullptr;
         const auto& v = t.value;
         if (!call([&] {
-                return pb_qk_norm_rope(v[0], v[1], v[2], v[3], v[4], v[5], v[6], eps, interleaved, &out[0], &out[1]);
+                return native.pb_qk_norm_rope(v[0], v[1], v[2], v[3], v[4], v[5], v[6], eps, interleaved, &out[0], &out[1]);
             }))
             return nullptr;
         return wrap_all(out);
@@ -191,7 +228,7 @@ namespace {
         if (interleaved < 0) return nullptr;
         const auto& v = t.value;
         if (!call([&] {
-                return pb_qk_norm_rope_backward(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8], eps, interleaved,
+                return native.pb_qk_norm_rope_backward(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], v[8], eps, interleaved,
                                                 out.data());
             }))
             return nullptr;
@@ -205,7 +242,7 @@ namespace {
         float scale = 0;
         pb_tensor* out = nullptr;
         if (!expect(n, 3) || !t.take(args, 1) || !integer(args[1], batch) || !number(args[2], scale)) return nullptr;
-        if (!call([&] { return pb_paged_attention(t.value[0], reinterpret_cast<pb_kv_batch*>(batch), scale, &out); }))
+        if (!call([&] { return native.pb_paged_attention(t.value[0], reinterpret_cast<pb_kv_batch*>(batch), scale, &out); }))
             return nullptr;
         return wrap(out);
     }
@@ -220,7 +257,7 @@ namespace {
             (args[2] != Py_None && !scores.take(args + 2, 1)) || !number(args[3], scale))
             return nullptr;
         if (!call([&] {
-                return pb_paged_attention_scored(t.value[0], reinterpret_cast<pb_kv_batch*>(batch), scores.value[0],
+                return native.pb_paged_attention_scored(t.value[0], reinterpret_cast<pb_kv_batch*>(batch), scores.value[0],
                                                  scale, &out[0], &out[1]);
             }))
             return nullptr;
@@ -237,16 +274,38 @@ namespace {
             !integer(args[4], recent) || !integer(args[5], sinks))
             return nullptr;
         if (!call([&] {
-                return pb_kv_evict(reinterpret_cast<pb_kv_batch*>(batch), scores.value[0], places.value[0], budget,
+                return native.pb_kv_evict(reinterpret_cast<pb_kv_batch*>(batch), scores.value[0], places.value[0], budget,
                                    recent, sinks, &out[0], &out[1]);
             }))
             return nullptr;
         return wrap_all(out);
     }
 
-    // (tensor type, realise, check)
+    // (path of the library, loaded)
+    PyObject* connect(PyObject*, PyObject* const* args, Py_ssize_t n) {
+        if (!expect(n, 1)) return nullptr;
+        const char* path = PyUnicode_AsUTF8(args[0]);
+        if (path == nullptr) return nullptr;
+        void* library = dlopen(path, RTLD_NOW | RTLD_LOCAL);
+        if (library == nullptr) {
+            PyErr_SetString(PyExc_ImportError, dlerror());
+            return nullptr;
+        }
+#define PB_FIND(name)                                                                                        \
+    native.name = reinterpret_cast<decltype(native.name)>(dlsym(library, #name));                            \
+    if (native.name == nullptr) {                                                                            \
+        PyErr_SetString(PyExc_ImportError, "the native library lacks " #name);                               \
+        return nullptr;                                                                                      \
+    }
+        PB_CALLS(PB_FIND)
+#undef PB_FIND
+        g_connected = true;
+        Py_RETURN_NONE;
+    }
+
+    // (tensor type, realise, check, load)
     PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
-        if (!expect(n, 3)) return nullptr;
+        if (!expect(n, 4)) return nullptr;
         if (!PyType_Check(args[0]) || !PyType_IsSubtype(reinterpret_cast<PyTypeObject*>(args[0]), &handle_type)) {
             PyErr_SetString(PyExc_TypeError, "the tensor type must derive from Handle");
             return nullptr;
@@ -254,6 +313,7 @@ namespace {
         Py_XSETREF(g_tensor_type, Py_NewRef(args[0]));
         Py_XSETREF(g_realise, Py_NewRef(args[1]));
         Py_XSETREF(g_check, Py_NewRef(args[2]));
+        Py_XSETREF(g_load, Py_NewRef(args[3]));
         Py_RETURN_NONE;
     }
 
@@ -267,6 +327,7 @@ namespace {
         method("paged_attention_scored", paged_attention_scored),
         method("kv_evict", kv_evict),
         method("bind", bind),
+        method("connect", connect),
         {nullptr, nullptr, 0, nullptr},
     };
 

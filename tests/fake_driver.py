@@ -9,11 +9,12 @@ HERE = Path(__file__).resolve().parent
 CUDA = Path(os.environ.get("CUDA_HOME", "/usr/local/cuda"))
 
 
-def run(program, folder, slow=None, slow_compile=None):
+def run(program, folder, slow=None, slow_compile=None, before=""):
     """Runs `program` (Python text, with `api` and `np` in hand) in a process
     whose CUDA driver and NVRTC are the stand-in; its output, and the log's
     lines, split. `slow`: a kernel each of whose launches takes 0.4 s on the
-    host; `slow_compile`: text of sources that take a second to compile."""
+    host; `slow_compile`: text of sources that take a second to compile;
+    `before` runs before the import of the api."""
     library, log = folder / "libcuda.so.1", folder / "log"
     if not library.exists():
         (folder / "libnvrtc.so.12").symlink_to(library)
@@ -23,7 +24,7 @@ def run(program, folder, slow=None, slow_compile=None):
                FAKE_CUDA_LOG=str(log), PYTHONPATH=str(HERE.parent), **{k: v for k, v in
                (("FAKE_CUDA_SLOW", slow), ("FAKE_CUDA_SLOW_COMPILE", slow_compile)) if v})
     env.pop("PORCH_B200_CACHE_DIR", None)
-    head = "import threading, time, os\nimport numpy as np\nfrom porch_b200 import api\n"
+    head = before + "import threading, time, os\nimport numpy as np\nfrom porch_b200 import api\n"
     done = subprocess.run([sys.executable, "-c", head + program], env=env, capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, done.stderr
     return done.stdout, [line.split() for line in log.read_text().splitlines()]

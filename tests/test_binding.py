@@ -1,9 +1,120 @@
 """The compiled part of the Python binding: argument kinds, errors, lifetimes."""
 
 import gc
+import subprocess
+import sys
+from pathlib import Path
 
 import numpy as np
 import pytest
+
+import fake_driver
+
+ROOT = Path(__file__).resolve().parent.parent
+# Before the import of porch_b200.api, as on an interpreter without the compiled module.
+NOT_COMPILED = """
+from pathlib import Path
+from porch_b200 import _lib
+_lib.binding_path = lambda: Path("/nowhere/_binding.so")
+"""
+
+
+def python(program):
+    done = subprocess.run([sys.executable, "-c", program], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr
+    return done.stdout
+
+
+@pytest.mark.parametrize("before", ["", NOT_COMPILED])
+def test_an_import_loads_no_native_library(api, before):
+    python(before + """
+loaded = lambda: "libporch_b200.so" in open("/proc/self/maps").read()
+from porch_b200 import api
+assert not loaded()
+assert api.placeholder([2, 3]).shape() == [2, 3]
+assert loaded()
+""")
+
+
+@pytest.mark.parametrize("before", ["", NOT_COMPILED])
+def test_a_library_that_is_not_built_fails_at_its_first_use(api, before):
+    python(before + """
+from pathlib import Path
+from porch_b200 import _lib
+path = _lib.binding_path() # the compiled part stays where it is
+_lib.binding_path = lambda: path
+_lib.LIBRARY = Path("/nowhere/libporch_b200.so")
+from porch_b200 import api
+for use in (lambda: api.placeholder([2]), lambda: api.Tensor(None).__cuda_array_interface__,
+            lambda: api.qk_norm_rope(*[api.Tensor(None)] * 7)):
+    try:
+        use()
+        raise SystemExit("no error")
+    except ImportError as e:
+        assert "is not built" in str(e), e
+""")
+
+
+OPERATORS = """
+x = lambda *shape: api.tensor(list(shape), np.arange(np.prod(shape), dtype=np.float32))
+cache = api.KVCache(8, 8, 2, 16)
+batch = cache.batch(np.arange(8).reshape(2, 4), [20, 30])
+q, k = api.qk_norm_rope(x(2, 4, 16), x(2, 2, 16) + 1.0, x(16), x(16), x(9, 8), x(9, 8), x(2), interleaved=True)
+grads = api.qk_norm_rope_backward(q, k, q, k, x(16), x(16), x(9, 8), x(9, 8), x(2), eps=0.5)
+batch.append(k, k)
+out = api.paged_attention(q, batch)
+out, scores = api.paged_attention_scored(q, batch, None, 0.25)
+out, scores = api.paged_attention_scored(q, batch, scores + 0.0)
+kept, places = api.cache_evict(batch, scores, budget=np.int64(12), recent=3)
+kept, places = api.cache_evict(batch, scores, places, budget=12, sinks=1)
+for t in (q, k, *grads, out, scores, kept, places):
+    assert type(t) is api.Tensor and isinstance(t._h, int)
+    face = t.__cuda_array_interface__
+    assert face is t.__cuda_array_interface__ and face["stream"] == q.__cuda_array_interface__["stream"]
+    print(t.shape(), face["shape"], face["typestr"], face["version"], face["data"] == (t.device_data()[0], False))
+p = api.placeholder
+good = [p([3, 4, 8]), p([3, 2, 8]), p([8]), p([8]), p([16, 4]), p([16, 4]), p([3])]
+for call in (lambda: api.qk_norm_rope(*good, eps="small"), lambda: api.qk_norm_rope("q", *good[1:]),
+             lambda: api.qk_norm_rope(None, *good[1:]), lambda: api.qk_norm_rope(api.Tensor(None), *good[1:]),
+             lambda: api.qk_norm_rope(1.0, *good[1:]), lambda: api.Tensor("text"), lambda: api.Tensor(None).shape(),
+             lambda: api.Tensor(None).__cuda_array_interface__, lambda: p([2]).__cuda_array_interface__,
+             lambda: api.paged_attention(q, batch, scale="1"), lambda: api.paged_attention(p([2, 4, 16]), batch),
+             lambda: api.cache_evict(batch, scores, budget="4"), lambda: api.cache_evict(batch, scores, budget=0),
+             lambda: api.paged_attention(q, cache)):
+    try:
+        call()
+        raise SystemExit("no error")
+    except Exception as e:
+        print(type(e).__name__, e if isinstance(e, (api.InvalidArgument, RuntimeError)) else "")
+"""
+
+
+def test_without_the_compiled_module_everything_is_the_same(api, tmp_path):
+    # Over the driver's stand-in: shapes, interfaces, errors, and what is launched.
+    seen = []
+    for name, before in (("compiled", ""), ("ctypes", NOT_COMPILED)):
+        folder = tmp_path / name
+        folder.mkdir()
+        out, log = fake_driver.run(OPERATORS, folder, before=before)
+        launches = [line[3:] for line in log if line[1] == "launch"]
+        assert {n[0] for n in launches} >= {"pb_norm_rope", "pb_norm_rope_grad", "pb_cache_append", "pb_paged_attention",
+                                            "pb_paged_finish", "pb_evict_select"}
+        seen.append((out, launches))
+    assert seen[0] == seen[1]
+
+
+@pytest.mark.gpu
+def test_without_the_compiled_module_results_are_the_same(gpu):
+    program = """
+import numpy as np
+from porch_b200 import api, _lib
+""" + OPERATORS[: OPERATORS.index("for t in")] + """
+for t in (q, k, *grads, out, scores, kept, places):
+    print(t.cpu().tobytes().hex())
+print(type(_lib.binding().paged_attention).__name__)
+"""
+    (*a, compiled), (*b, plain) = python(program).split(), python(NOT_COMPILED + program).split()
+    assert a == b and compiled == "builtin_function_or_method" and plain == "function"
 
 
 def test_handles(api):
