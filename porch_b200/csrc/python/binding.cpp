@@ -44,8 +44,11 @@ namespace {
         PyObject* face; // __cuda_array_interface__, once asked for
     };
 
-    void release(pb_tensor* t) { // a tensor exists only once the library does
-        if (t != nullptr && g_connected) native.pb_tensor_release(t);
+    void release(pb_tensor* t) {
+        if (t == nullptr || !g_connected) return; // a tensor exists only once the library does
+        Py_BEGIN_ALLOW_THREADS // it may have to wait for other streams' readers
+        native.pb_tensor_release(t);
+        Py_END_ALLOW_THREADS
     }
 
     // Whether the library is there; loads it, or sets the exception.
@@ -95,19 +98,36 @@ namespace {
         return false;
     }
 
+    // A call of the library that returns a status, without the interpreter's lock.
+    template <typename F>
+    bool call(F&& f) {
+        if (!ready()) return false;
+        int status = 0;
+        Py_BEGIN_ALLOW_THREADS // a first call compiles its kernel
+        status = f();
+        Py_END_ALLOW_THREADS
+        return checked(status);
+    }
+
     // The address of a realised tensor's values stays what it is once it was
     // handed out, so consumers that ask twice cost one call.
     PyObject* handle_interface(PyObject* self, void*) {
         auto* h = reinterpret_cast<handle_object*>(self);
         if (h->face == nullptr) {
             int64_t v[19];
-            if (!ready() || !checked(native.pb_tensor_interface(h->tensor, v, 19))) return nullptr;
+            pb_tensor* t = h->tensor;
+            // A lazy tensor is realised, which may compile its kernel.
+            if (!call([&] { return native.pb_tensor_interface(t, v, 19); })) return nullptr;
             PyObject* shape = PyTuple_New(static_cast<Py_ssize_t>(v[0]));
             if (shape == nullptr) return nullptr;
             for (int64_t i = 0; i < v[0]; ++i) PyTuple_SET_ITEM(shape, i, PyLong_FromLongLong(v[3 + i]));
-            h->face = Py_BuildValue("{s:N,s:s,s:(KO),s:i,s:K}", "shape", shape, "typestr", "<f4", "data",
-                                    static_cast<unsigned long long>(v[1]), Py_False, "version", 3, "stream",
-                                    static_cast<unsigned long long>(v[2]));
+            PyObject* face = Py_BuildValue("{s:N,s:s,s:(KO),s:i,s:K}", "shape", shape, "typestr", "<f4", "data",
+                                           static_cast<unsigned long long>(v[1]), Py_False, "version", 3, "stream",
+                                           static_cast<unsigned long long>(v[2]));
+            if (h->face == nullptr)
+                h->face = face;
+            else
+                Py_XDECREF(face); // another thread was first
         }
         return Py_XNewRef(h->face);
     }
@@ -192,16 +212,6 @@ namespace {
         const double v = PyFloat_AsDouble(x);
         out = static_cast<float>(v);
         return !(v == -1.0 && PyErr_Occurred());
-    }
-
-    template <typename F>
-    bool call(F&& f) {
-        if (!ready()) return false;
-        int status = 0;
-        Py_BEGIN_ALLOW_THREADS // a first call compiles its kernel
-        status = f();
-        Py_END_ALLOW_THREADS
-        return checked(status);
     }
 
     PyObject* qk_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {

@@ -61,7 +61,12 @@ CUresult cuStreamSynchronize(CUstream s) { say("sync %p", s); return CUDA_SUCCES
 CUresult cuStreamWaitEvent(CUstream s, CUevent e, unsigned int flags) { say("wait %p %p", s, e); return CUDA_SUCCESS; }
 CUresult cuEventCreate(CUevent* e, unsigned int flags) { *e = handle(); return CUDA_SUCCESS; }
 CUresult cuEventDestroy_v2(CUevent e) { return CUDA_SUCCESS; }
-CUresult cuEventRecord(CUevent e, CUstream s) { say("record %p %p", s, e); return CUDA_SUCCESS; }
+CUresult cuEventRecord(CUevent e, CUstream s) {
+    const char* slow = getenv("FAKE_CUDA_SLOW");
+    if (slow != NULL && strcmp(slow, "cuEventRecord") == 0) usleep(400000);
+    say("record %p %p", s, e);
+    return CUDA_SUCCESS;
+}
 CUresult cuEventSynchronize(CUevent e) { return CUDA_SUCCESS; }
 CUresult cuEventQuery(CUevent e) { return CUDA_SUCCESS; }
 CUresult cuEventElapsedTime(float* ms, CUevent a, CUevent b) { *ms = 0; return CUDA_SUCCESS; }

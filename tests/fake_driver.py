@@ -13,7 +13,7 @@ def run(program, folder, slow=None, slow_compile=None, before=""):
     """Runs `program` (Python text, with `api` and `np` in hand) in a process
     whose CUDA driver and NVRTC are the stand-in; its output, and the log's
     lines, split. `slow`: a kernel each of whose launches takes 0.4 s on the
-    host; `slow_compile`: text of sources that take a second to compile;
+    host (or cuEventRecord); `slow_compile`: text of sources that take a second to compile;
     `before` runs before the import of the api."""
     library, log = folder / "libcuda.so.1", folder / "log"
     if not library.exists():

@@ -103,6 +103,42 @@ def test_without_the_compiled_module_everything_is_the_same(api, tmp_path):
     assert seen[0] == seen[1]
 
 
+@pytest.mark.parametrize("before", ["", NOT_COMPILED])
+@pytest.mark.parametrize("slow,what", [
+    (dict(slow_compile="pb_elem"), "lazy.__cuda_array_interface__"),  # compiles a kernel: a second
+    (dict(slow="cuEventRecord"), "tensors.clear()"),  # a tensor that another stream reads: 0.4 s
+])
+def test_other_threads_run_meanwhile(api, tmp_path, before, slow, what):
+    fake_driver.run("""
+tensors = [api.tensor([1000], np.ones(1000, np.float32))]
+lazy = api.as_tensor(tensors[0] * 2.0)
+q = [api.tensor([1, 1, 8], np.ones(8, np.float32))] * 2
+def read():
+    w = api.tensor([8], np.ones(8, np.float32))
+    c = api.tensor([4, 4], np.ones(16, np.float32))
+    tensors.append(api.qk_norm_rope(*q, w, w, c, c, api.tensor([1], np.ones(1, np.float32)))[0])
+t = threading.Thread(target=read)
+t.start()
+t.join()
+tensors.append(q.pop())
+q.clear()
+if """ + repr("lazy" not in what) + """:
+    del lazy
+def work():
+    began = time.perf_counter()
+    """ + what + """
+    took.append(time.perf_counter() - began)
+took, gap, last = [], 0.0, time.perf_counter()
+t = threading.Thread(target=work)
+t.start()
+while t.is_alive():
+    time.sleep(0.002)
+    now = time.perf_counter()
+    gap, last = max(gap, now - last), now
+assert took[0] > 0.35 and gap < 0.25, (took, gap)
+""", tmp_path, before=before, **slow)
+
+
 @pytest.mark.gpu
 def test_without_the_compiled_module_results_are_the_same(gpu):
     program = """
