@@ -44,17 +44,32 @@ namespace porch::detail {
     } // namespace
 
     op_kernel& op_kernel_for(const op_key& key, const std::function<void(op_kernel&)>& make) {
+        // The table's lock is held for the lookup alone: a kernel compiles under
+        // its own entry's, so that it holds up nobody but those who need it.
+        struct entry {
+            std::mutex mutex;
+            std::unique_ptr<op_kernel> made;
+            std::atomic<op_kernel*> ready{nullptr};
+        };
         static std::mutex mutex;
-        static auto* table = new std::unordered_map<op_key, std::unique_ptr<op_kernel>, key_hash>(); // lives until exit
-        std::scoped_lock lock{mutex};
-        auto& entry = (*table)[key];
-        if (entry == nullptr) {
+        static auto* table = new std::unordered_map<op_key, std::unique_ptr<entry>, key_hash>(); // lives until exit
+        entry* e = nullptr;
+        {
+            std::scoped_lock lock{mutex};
+            auto& slot = (*table)[key];
+            if (slot == nullptr) slot = std::make_unique<entry>();
+            e = slot.get();
+        }
+        if (op_kernel* k = e->ready.load(std::memory_order_acquire)) return *k;
+        std::scoped_lock lock{e->mutex};
+        if (e->made == nullptr) {
             auto k = std::make_unique<op_kernel>();
             make(*k);
             k->image_key = compile(k->source);
-            entry = std::move(k);
+            e->made = std::move(k); // one that failed is tried again
+            e->ready.store(e->made.get(), std::memory_order_release);
         }
-        return *entry;
+        return *e->made;
     }
 
     void op_launch(op_kernel& k, int device, const std::shared_ptr<stream_ref>& stream,

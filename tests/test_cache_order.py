@@ -113,6 +113,31 @@ print(hex(seen[0]))
     assert fake_driver.unordered(log, lambda a, b: a in WRITES and b == "reader") == []
 
 
+def test_a_kernel_that_compiles_holds_up_only_those_who_need_it(api, tmp_path):
+    # Head size 24 takes a second to compile. Two threads want it, and get it
+    # with one compilation of each kernel; this one runs a kernel that is there.
+    program = SETUP + """
+calls["append"]()
+other = api.KVCache(8, 8, 1, 24)
+wide = other.batch([[0, 1]], [16], appended=[16])
+x = api.tensor([16, 1, 24], np.ones(384, np.float32))
+threads = [threading.Thread(target=lambda: wide.append(x, x)) for _ in range(2)]
+for t in threads:
+    t.start()
+while not any(l.split()[1:] == ["compile", "1"] for l in open(os.environ["FAKE_CUDA_LOG"])):
+    time.sleep(0.005)
+began = time.perf_counter()
+calls["append"]()
+took = time.perf_counter() - began
+assert any(t.is_alive() for t in threads)
+for t in threads:
+    t.join()
+assert took < 0.3, took
+"""
+    _, log = fake_driver.run(program, tmp_path, slow_compile="#define PB_D 24")
+    assert sum(line[1:] == ["compile", "1"] for line in log) == 1
+
+
 @pytest.mark.parametrize("group,dim,dtype", [(1, 64, "bf16"), (12, 128, "f32"), (17, 64, "bf16"), (40, 64, "f32")])
 def test_a_step_uploads_and_waits_only_where_its_batch_is_made(api, tmp_path, group, dim, dtype):
     # From the second step on an attention only enqueues, whatever the number of
