@@ -76,6 +76,8 @@ class Decoder:
     def step(self, tokens: np.ndarray) -> np.ndarray:
         """Takes one token of each sequence; the next ones' probabilities."""
         m, n = self.model, self.n
+        if self.seen >= len(m.cos):  # the operator would turn by NaN
+            raise ValueError(f"the model has angles for {len(m.cos)} positions")
         self.length += 1
         batch = self.caches[0].batch(self.tables, [self.length] * n, newest=[self.seen] * n)
         at = api.full([n], float(self.seen), self.device)
@@ -109,7 +111,7 @@ def main(argv: list[str] | None = None) -> None:
     parser.add_argument("--budget", type=int, default=64)
     parser.add_argument("--dtype", choices=("f32", "bf16"), default="bf16")
     a = parser.parse_args(argv)
-    model = Model()
+    model = Model(positions=max(4096, a.steps))
     decoder = Decoder(model, a.sequences, a.budget, a.dtype)
     tokens = np.arange(a.sequences) % model.vocabulary
     said, times = [tokens], []

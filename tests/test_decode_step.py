@@ -3,6 +3,7 @@
 import numpy as np
 import pytest
 
+import fake_driver
 import paged
 
 
@@ -55,6 +56,23 @@ class Plain:
         logits = x @ m.head.astype(np.float64)
         p = np.exp(logits - logits.max(1, keepdims=True))
         return p / p.sum(1, keepdims=True)
+
+
+def test_positions_end_with_the_models_table(api, tmp_path):
+    # Over the driver's stand-in: a step past the table is an error, not NaN
+    # probabilities, and the command's model has a table for all its steps.
+    out, _ = fake_driver.run("""
+from porch_b200 import decode_step
+d = decode_step.Decoder(decode_step.Model(vocabulary=16, width=16, heads=2, kv_heads=1, head_dim=8, positions=5), 2, 8)
+try:
+    for step in range(9):
+        d.step(np.arange(2))
+except ValueError as e:
+    print(step, e)
+decode_step.Decoder = lambda model, *a: exit(len(model.cos) != 5000)
+decode_step.main(["--steps", "5000"])
+""", tmp_path)
+    assert out.split("\n")[0] == "5 the model has angles for 5 positions"
 
 
 @pytest.mark.gpu
