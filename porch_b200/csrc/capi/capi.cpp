@@ -888,9 +888,13 @@ int pb_kv_plan_describe(const int64_t* lengths, size_t sequences, int64_t kv_hea
                         char* text, size_t capacity, size_t* needed) {
     return guarded([&] {
         if (sequences != 0) require(lengths, "lengths");
+        // What a batch and its attention allow, so that nothing here overflows.
+        constexpr int64_t most_length = int64_t{1} << 30, most_ctas = int64_t{1} << 20, most_rows = int64_t{1} << 27;
+        if (sequences > 65535 || kv_heads < 1 || kv_heads > 1024 || chunks < 1 || chunks > 65536 || ctas < 1 || ctas > most_ctas ||
+            static_cast<int64_t>(sequences) * kv_heads * chunks >= most_rows ||
+            std::any_of(lengths, lengths + sequences, [](int64_t v) { return v < 0 || v >= most_length; }))
+            throw std::invalid_argument("plan: at most 65535 sequences of 0 to 2^30 slots, 1 to 1024 heads, 2^27 rows, 2^20 CTAs");
         std::vector<int64_t> n(lengths, lengths + sequences);
-        if (kv_heads < 1 || chunks < 1 || ctas < 1 || std::any_of(n.begin(), n.end(), [](int64_t v) { return v < 0; }))
-            throw std::invalid_argument("plan: lengths must not be negative, heads, chunks and CTAs positive");
         copy_text(porch::detail::attention_schedule(n, kv_heads, chunks, ctas), text, capacity, needed);
     });
 }

@@ -425,6 +425,15 @@ def test_every_tile_is_worked_on_once_and_every_split_row_joined(api, seed):
     assert parts == {r: [(c + i, 0 if i else place) for i in range(k)] for r, (c, k, place) in join.items()}
 
 
+@pytest.mark.parametrize("lengths,heads,ctas,chunks", [
+    ([2**63 - 1], 1, 8, 1), ([1 << 30], 1, 8, 1), ([-1], 1, 8, 1), ([64], 0, 8, 1), ([64], 1025, 8, 1), ([64], 1, 0, 1),
+    ([64], 1, 1 << 40, 1), ([64], 1, 8, 0), ([64], 1, 8, 1 << 50), ([1] * 200, 1024, 8, 1024), ([1] * 65536, 1, 8, 1),
+])
+def test_plans_of_sizes_that_no_batch_has_are_refused(api, lengths, heads, ctas, chunks):
+    with pytest.raises(api.InvalidArgument, match="plan"):
+        api.attention_plan(lengths, heads, ctas, chunks)
+
+
 @pytest.mark.gpu
 def test_refusals(gpu):
     cache = gpu.KVCache(6, 16, 2, 64)
