@@ -1017,7 +1017,9 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
                "paged_attention: q must be [sequences, q_heads, head_dim] of the batch");
         expect(shape[1] >= c.heads && shape[1] % c.heads == 0 && shape[1] <= 65536,
                "paged_attention: q_heads must be a multiple of the cache's kv_heads");
-        expect(std::isfinite(scale), "paged_attention: scale must be finite");
+        // The kernels' logits are in units of log2.
+        float scale2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
+        expect(std::isfinite(scale2), "paged_attention: scale must be finite, and below 2.3e38");
         int64_t ns = 0;
         if (scores != nullptr) {
             const auto s = shape_of(*scores);
@@ -1073,7 +1075,6 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         if (attention != nullptr) {
             (void)attention->on(device);
             check(pbrt_error_word(device, &err));
-            float scale2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
             void* params[] = {&c.map_k, &c.map_v, &x.ptr, &batch.lengths_at, &batch.tables_at, &work,
                               &out.ptr, &partial, &ml, &logits, &norms, &width, &group, &chunks,
                               &x.strides[0], &x.strides[1], &longest32, &scale2, &err};

@@ -113,6 +113,21 @@ print(hex(seen[0]))
     assert fake_driver.unordered(log, lambda a, b: a in WRITES and b == "reader") == []
 
 
+def test_a_scale_that_overflows_in_units_of_log2_is_refused(api, tmp_path):
+    out, log = fake_driver.run(SETUP + """
+for scale in (float("nan"), float("inf"), 2.5e38, -3.4e38):
+    for call in (api.paged_attention, api.paged_attention_scored):
+        try:
+            call(q, batch, scale=scale)
+        except api.InvalidArgument as e:
+            assert "scale" in str(e)
+            print("refused")
+api.paged_attention(q, batch, scale=-2.3e38)
+""", tmp_path)
+    assert out.split() == ["refused"] * 8
+    assert [line[3] for line in log if line[1] == "launch"] == ["pb_paged_attention", "pb_paged_finish"]
+
+
 def test_a_kernel_that_compiles_holds_up_only_those_who_need_it(api, tmp_path):
     # Head size 24 takes a second to compile. Two threads want it, and get it
     # with one compilation of each kernel; this one runs a kernel that is there.
