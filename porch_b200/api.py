@@ -341,6 +341,8 @@ def tensor_from_device(array, device: int = 0) -> Tensor:
     shape = face["shape"]
     if face["typestr"] != "<f4":
         raise InvalidArgument("tensor_from_device needs a float32 array")
+    if face.get("mask") is not None:
+        raise InvalidArgument("tensor_from_device takes no masked array")
     strides, step = face.get("strides"), 4
     if strides is not None:
         for extent, stride in zip(reversed(shape), reversed(strides)):

@@ -103,6 +103,16 @@ def test_without_the_compiled_module_everything_is_the_same(api, tmp_path):
     assert seen[0] == seen[1]
 
 
+def test_an_array_of_another_library_is_refused_where_a_copy_would_not_be_it(api):
+    class Face:
+        def __init__(self, **more):
+            self.__cuda_array_interface__ = dict(shape=(2, 3), typestr="<f4", data=(0, False), version=3, **more)
+
+    for more, match in ((dict(mask=Face()), "mask"), (dict(strides=(4, 8)), "contiguous")):
+        with pytest.raises(api.InvalidArgument, match=match):
+            api.tensor_from_device(Face(**more))
+
+
 @pytest.mark.parametrize("before", ["", NOT_COMPILED])
 @pytest.mark.parametrize("slow,what", [
     (dict(slow_compile="pb_elem"), "lazy.__cuda_array_interface__"),  # compiles a kernel: a second
