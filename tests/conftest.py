@@ -16,6 +16,20 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs a CUDA device (runs on the B200 box)")
 
 
+def pytest_collection_modifyitems(items):
+    """Where the checkers built from the reference's sources are missing, the
+    tests that fail for want of them come last: a run that stops at its first
+    failure still reaches every other test."""
+    if (ROOT / "oracle" / "_ref" / "ref_runner").exists():
+        return
+    need = {"test_nonfinite_matmul_operands_match_the_reference", "test_reference_test_suite_against_this_library"}
+
+    def needs(item):
+        return item.path.name == "test_ref_fullsize.py" or getattr(item, "originalname", None) in need
+
+    items.sort(key=needs)
+
+
 @pytest.fixture(scope="session")
 def api():
     from porch_b200.build import build as build_library
