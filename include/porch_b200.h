@@ -246,9 +246,12 @@ int pb_comm_wait(pb_comm* comm);
 /* ---- operators of a transformer's decode step --------------------------- */
 /* No counterpart in the reference, whose operators end at matmul and
  * softmax. Each takes tensors of one device (a lazy one is realised first),
- * enqueues its kernels on this thread's stream and returns realised tensors;
- * nothing waits. Strided views are read in place where their innermost axis
- * is contiguous. */
+ * enqueues its kernels on this thread's stream and returns realised tensors
+ * without waiting for them. The host waits where a batch is made (its upload),
+ * for a kernel that has to be compiled first (once for its sizes), and where an
+ * attention has another number of query heads than the last one of its cache
+ * (the upload of its plan, which the next batch then has). Strided views are
+ * read in place where their innermost axis is contiguous. */
 
 /* A tensor with a copy of `count` floats at device address `pointer` (memory
  * of another library on the same GPU), which `stream` (a CUstream, NULL for
@@ -290,7 +293,7 @@ int pb_qk_norm_rope_backward(const pb_tensor* dq_out, const pb_tensor* dk_out,
  * bfloat16; head_dim a multiple of 8 up to 256. The values start undefined;
  * nothing reads a slot past a sequence's length. Calls that write a cache
  * (append, evict) and calls that read it are ordered on the device in the
- * order in which they are made. */
+ * order in which they are made, from whatever threads. */
 typedef struct pb_kv_cache_s pb_kv_cache;
 typedef struct pb_kv_batch_s pb_kv_batch;
 enum pb_cache_type { PB_CACHE_F32 = 0, PB_CACHE_BF16 = 1 };
@@ -323,8 +326,12 @@ int pb_kv_append(pb_kv_batch* batch, const pb_tensor* k, const pb_tensor* v);
 /* softmax(scale q K^T) V for one query per sequence: q and the result
  * [sequences, q_heads, head_dim], q_heads a multiple of kv_heads (query head
  * i reads key head i / (q_heads / kv_heads)). An empty sequence gives zeros.
- * Sums, maxima and the result are float32 for either cache type. A query, or
- * a key or value in use, that is not finite makes results of the heads that
+ * Sums, maxima and the result are float32 for either cache type. Against a
+ * bfloat16 cache, queries and weights keep all 24 bits; against a float32 one,
+ * queries, keys, weights and values are each two tf32 terms, off by up to 2^-21,
+ * so that a product is off by up to 2^-19.6 of itself. A query, or a key or
+ * value in use, that is not finite (or within 0.2 % of float32's largest value,
+ * where rounding to its first term makes it infinite) makes results of the heads that
  * read it not finite (infinity or NaN), and no others. A logit below float32's
  * range weighs 0; one above it, or a row of which every logit lies below it,
  * gives NaN. */
@@ -344,10 +351,11 @@ int pb_kv_plan_describe(const int64_t* lengths, size_t sequences, int64_t kv_hea
  * of shared memory that each of them takes, the system's share included. */
 int pb_kv_attention_shape(int64_t head_dim, int type, int64_t group, int64_t* ctas_per_sm,
                           int64_t* shared_bytes);
-/* As pb_paged_attention, and new scores [sequences, kv_heads, longest length]: `scores`
- * (NULL or slots past its end: 0) plus each slot's attention weight summed
- * over the query heads of its key head; 0 past a sequence's length. Takes 4
- * bytes of workspace per query head and slot. */
+/* As pb_paged_attention, and new scores [sequences, kv_heads, longest length]:
+ * `scores` (NULL or slots past its end: 0) plus each slot's attention weight
+ * summed over the query heads of its key head; 0 past a sequence's length. Takes
+ * 4 bytes of workspace per query head, for every sequence and as many slots as
+ * the longest one has. */
 int pb_paged_attention_scored(const pb_tensor* q, pb_kv_batch* batch, const pb_tensor* scores,
                               float scale, pb_tensor** out, pb_tensor** new_scores);
 /* Keeps, per sequence and key head, `budget` slots: the newest `recent`

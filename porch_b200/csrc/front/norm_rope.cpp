@@ -432,10 +432,11 @@ extern "C" __global__ void __launch_bounds__(1024) pb_norm_rope_weights(const fl
         // `aligned`: the width at which every row of the operands starts.
         // `few`: of 4 to 32 lanes the number that leaves the fewest idle, the
         // larger of equals. Head sizes of 80 and 96 have 10 and 12 items: 4
-        // lanes of three take 56 and 53 us forward where 16 of one take 63 and
-        // 59 (25000 and 20833 tokens x 20 heads), but 77 and 61 where 16 take
-        // 61 and 56 with pairs side by side, and 133 and 113 where 16 take 105
-        // and 97 in the gradient, whose registers then hold one head at once.
+        // lanes of three take 60 and 54 us forward where 16 of one take 67 and
+        // 61 (25000 and 20833 tokens x 20 heads, rotated whole), but 77 and 61
+        // where 16 take 61 and 56 with pairs side by side, and 133 and 113 where
+        // 16 take 105 and 97 in the gradient, whose registers then hold one head
+        // at once.
         void choose_lanes(shape_key& s, int aligned, bool few) {
             s.vec = 4;
             while (s.vec > 1 && (s.dim % s.vec != 0 || (s.interleaved ? (2 * s.half) % s.vec : s.half % s.vec) != 0))

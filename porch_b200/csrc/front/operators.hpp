@@ -37,8 +37,11 @@ namespace porch::detail {
     using op_key = std::array<int64_t, 12>;
     op_kernel& op_kernel_for(const op_key& key, const std::function<void(op_kernel&)>& make);
 
-    // Launches `k` on `stream`; every kernel here begins with
-    // griddepcontrol.wait, so the launch overlaps the previous kernel's tail.
+    // Launches `k` on `stream` so that it overlaps the previous kernel's tail:
+    // every kernel here executes griddepcontrol.wait before it reads or writes
+    // what other kernels do. What comes before the wait (attention's and its
+    // join's plan, lengths and tables) is only ever written by an upload that
+    // the host has waited for, never by a kernel.
     void op_launch(op_kernel& k, int device, const std::shared_ptr<stream_ref>& stream,
                    std::array<uint32_t, 3> grid, uint32_t threads, void** params, uint32_t cluster = 1);
 

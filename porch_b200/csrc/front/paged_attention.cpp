@@ -10,7 +10,7 @@
 // query heads over 8 of 128 bfloat16 channels: 784 MB in 126 us = 6.20 TB/s;
 // one sequence of 262147 slots: 1074 MB in 165 us = 6.5 TB/s, what a copy
 // reaches. Few or short rows are bound by the launch and the first loads'
-// latency instead (about 6 us).
+// latency instead (about 6 us, 3 of the stream where calls follow each other).
 //
 // pb_paged_attention, 160 threads: a producer warp loads tiles of 64 slots, K
 // then V, through a ring of TMA boxes (a page, or 64 rows of a larger one; 128
@@ -24,10 +24,11 @@
 //
 // Accuracy: float32. Queries and weights are split into three bfloat16 terms
 // (24 bits) against a bfloat16 cache, whose products are then exact; a float32
-// cache is split into two tf32 terms like the queries (3 products of 4, error
-// 2^-21). The tensor core's accumulator cuts low bits at every addition, so a
-// tile's products start from zero and are added to the running sums in fp32,
-// rounded to nearest.
+// cache is split into two tf32 terms like the queries (each off by up to 2^-21,
+// and of four products the smallest is left out: 2^-19.6 of a product at most).
+// The tensor core's accumulator cuts low bits at every addition, so a tile's
+// products start from zero and are added to the running sums in fp32, rounded to
+// nearest.
 //
 // Work is shared out in even runs of tiles over all rows, one wave of CTAs
 // (more waves, which would even out CTAs of different speed, took 1 to 5 %

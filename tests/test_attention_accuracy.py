@@ -10,8 +10,8 @@ more operations round (0.6 u each): 1.9 u of the logit, of size 0.9 on average,
 so 1.7 u of a weight. exp2's error is at most 4 u, 2.3 u on average. Weights of
 five slots average those to about 0.55 of 2.9 u: 1.6 u. The weighted sum is cut
 and rounded, the sum of the weights, its reciprocal and the product round: 2 u.
-In all 2.6 u; the bound is 4 u. Two tf32 terms leave up to 8 u of a product
-against a float32 cache, cut toward zero: the bound is 6 u.
+In all 2.6 u; the bound is 4 u. Two tf32 terms leave up to 8 u of each
+operand against a float32 cache, cut toward zero: the bound is 6 u.
 
 That the bounds see a term that is missing is checked on the same arithmetic in
 numpy: 12 u and more against a bfloat16 cache, a thousand against a float32 one.
