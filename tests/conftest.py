@@ -17,9 +17,9 @@ def pytest_configure(config):
 
 
 def pytest_collection_modifyitems(items):
-    """Where the checkers built from the reference's sources are missing, the
-    tests that fail for want of them come last: a run that stops at its first
-    failure still reaches every other test."""
+    """Where the programs built from the reference's sources are missing, the
+    tests that compare with them, and fail, come last: a run that stops at its
+    first failure still reaches every other test."""
     if (ROOT / "oracle" / "_ref" / "ref_runner").exists():
         return
     need = {"test_nonfinite_matmul_operands_match_the_reference", "test_reference_test_suite_against_this_library"}
