@@ -287,6 +287,25 @@ int pb_qk_norm_rope_backward(const pb_tensor* dq_out, const pb_tensor* dk_out,
                              const pb_tensor* positions, float eps, int interleaved,
                              pb_tensor* out[4]);
 
+/* What each row of `logits` [T, V] (V up to 2^24) says of its tokens:
+ *   out[0] [T]      log softmax(x)_t of `tokens` [T], whole numbers below V; 0
+ *                   for -1 (a padded row), NaN for any other value;
+ *   out[1] [T]      the entropy -sum p log p, masked logits (-inf) adding nothing;
+ *   out[2] [T, 2]   the largest logit m and sum exp(x - m), which the gradient takes;
+ *   out[3] [T, top] the `top` (0 to 32, at most V) likeliest tokens' log
+ *                   probabilities in falling order, equal ones by the lower
+ *                   token, NaN last, and
+ *   out[4] [T, top] their numbers (NULL both where `top` is 0).
+ * A row with a NaN or +inf, or with nothing but -inf, gives NaN (but out[2]'s m,
+ * out[4], and 0 where it is padded). */
+int pb_token_logprobs(const pb_tensor* logits, const pb_tensor* tokens, int64_t top, pb_tensor* out[5]);
+/* The gradient of the logits from those of out[0] and out[1]; `norm` and
+ * `entropy` as the forward gave them. d_entropy and entropy may both be NULL.
+ * A padded row (without a gradient of its entropy) gives zeros. */
+int pb_token_logprobs_backward(const pb_tensor* d_logprobs, const pb_tensor* logits, const pb_tensor* tokens,
+                               const pb_tensor* norm, const pb_tensor* d_entropy, const pb_tensor* entropy,
+                               pb_tensor** d_logits);
+
 /* ---- a paged key/value cache --------------------------------------------- */
 /* Pools of `pages` pages of `page_size` (a power of two, 8 to 256) slots for
  * keys and for values, [pages, kv_heads, page_size, head_dim], in float32 or

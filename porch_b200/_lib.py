@@ -123,6 +123,8 @@ def _declare(L: ctypes.CDLL) -> None:
         "pb_tensor_interface": (c_int, [T, c_void_p, c_size_t]),
         "pb_qk_norm_rope": (c_int, [T, T, T, T, T, T, T, c_float, c_int, P(T), P(T)]),
         "pb_qk_norm_rope_backward": (c_int, [T, T, T, T, T, T, T, T, T, c_float, c_int, P(T)]),
+        "pb_token_logprobs": (c_int, [T, T, c_int64, P(T)]),
+        "pb_token_logprobs_backward": (c_int, [T, T, T, T, T, T, P(T)]),
         "pb_kv_cache_create": (c_int, [c_int64, c_int64, c_int64, c_int64, c_int, c_int, P(T)]),
         "pb_kv_cache_release": (None, [T]),
         "pb_kv_cache_data": (c_int, [T, P(c_uint64), P(c_uint64), P(c_size_t)]),

@@ -532,6 +532,22 @@ def qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, cos, sin, positions,
     return _binding.qk_norm_rope_backward(dq, dk, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
 
 
+def token_logprobs(logits, tokens, top: int = 0) -> tuple[Tensor, ...]:
+    """Of each row of logits [T, V]: the log probability of its token (tokens
+    [T], whole numbers; 0 for -1, a padded row), the entropy, and its largest
+    logit beside the sum of exponentials relative to it, [T, 2]. With `top`
+    (up to 32) also the likeliest tokens' log probabilities in falling order
+    and their numbers, [T, top]. An extension."""
+    return _binding.token_logprobs(logits, tokens, top)
+
+
+def token_logprobs_backward(d_logprobs, logits, tokens, norm, d_entropy=None, entropy=None) -> Tensor:
+    """Gradient of the logits from those of token_logprobs' log probabilities
+    and entropies (d_entropy, with the entropies themselves); norm is its
+    third result. An extension."""
+    return _binding.token_logprobs_backward(d_logprobs, logits, tokens, norm, d_entropy, entropy)
+
+
 class _Pool:
     """A cache pool in place, for another library on the same GPU; a bfloat16
     pool as its 16 raw bits. Keeps the cache alive. Each time it is asked for

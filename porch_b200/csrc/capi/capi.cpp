@@ -759,6 +759,33 @@ int pb_qk_norm_rope_backward(const pb_tensor* dq_out, const pb_tensor* dk_out, c
     });
 }
 
+int pb_token_logprobs(const pb_tensor* logits, const pb_tensor* tokens, int64_t top, pb_tensor* out[5]) {
+    return guarded([&] {
+        require(out, "out");
+        out[0] = out[1] = out[2] = out[3] = out[4] = nullptr;
+        require(logits, "logits");
+        require(tokens, "tokens");
+        auto r = porch::detail::token_logprobs(logits->value, tokens->value, top);
+        for (size_t i = 0; i < r.size(); ++i) out[i] = wrap(std::move(r[i]));
+    });
+}
+
+int pb_token_logprobs_backward(const pb_tensor* d_logprobs, const pb_tensor* logits, const pb_tensor* tokens,
+                               const pb_tensor* norm, const pb_tensor* d_entropy, const pb_tensor* entropy,
+                               pb_tensor** d_logits) {
+    return guarded([&] {
+        require(d_logits, "d_logits");
+        *d_logits = nullptr;
+        require(d_logprobs, "d_logprobs");
+        require(logits, "logits");
+        require(tokens, "tokens");
+        require(norm, "norm");
+        *d_logits = wrap(porch::detail::token_logprobs_backward(
+            d_logprobs->value, logits->value, tokens->value, norm->value, d_entropy != nullptr ? &d_entropy->value : nullptr,
+            entropy != nullptr ? &entropy->value : nullptr));
+    });
+}
+
 int pb_kv_cache_create(int64_t pages, int64_t page_size, int64_t kv_heads, int64_t head_dim, int type, int device,
                        pb_kv_cache** out) {
     return guarded([&] {

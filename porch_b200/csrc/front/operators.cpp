@@ -184,6 +184,7 @@ namespace porch::detail {
     std::string operator_sources() {
         std::vector<std::pair<std::string, std::string>> all;
         norm_rope_sources(all);
+        token_logprobs_sources(all);
         paged_cache_sources(all);
         paged_attention_sources(all);
         std::ostringstream os;

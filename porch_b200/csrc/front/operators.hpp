@@ -104,6 +104,14 @@ namespace porch::detail {
     std::array<tensor, 2> qk_norm_rope(const norm_rope_args& a);
     std::array<tensor, 4> qk_norm_rope_backward(const tensor& dq, const tensor& dk, const norm_rope_args& a);
 
+    // ------------------------------------------------------ log probabilities --
+    // {log probabilities, entropies, norms}, and where `top` is not 0 the
+    // alternatives' log probabilities and tokens.
+    std::vector<tensor> token_logprobs(const tensor& logits, const tensor& tokens, int64_t top);
+    // The logits' gradient; d_entropy and entropy both or neither.
+    tensor token_logprobs_backward(const tensor& d_said, const tensor& logits, const tensor& tokens, const tensor& norm,
+                                   const tensor* d_entropy, const tensor* entropy);
+
     // --------------------------------------------------------------- cache --
     enum class cache_type : int { f32 = 0, bf16 = 1 };
 
@@ -208,6 +216,7 @@ namespace porch::detail {
     std::string operator_sources();
     using kernel_list = std::vector<std::pair<std::string, std::string>>;
     void norm_rope_sources(kernel_list& out);
+    void token_logprobs_sources(kernel_list& out);
     void paged_cache_sources(kernel_list& out);
     void paged_attention_sources(kernel_list& out);
 

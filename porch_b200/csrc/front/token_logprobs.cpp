@@ -1,0 +1,501 @@
+// What a row of logits x says of its tokens, in one pass over it, and the
+// gradient. With m = max x, s = sum exp(x - m) and w = sum exp(x - m) (x - m):
+//   log p(t) = x_t - m - log s,   H = log s - w / s,
+// beside the `top` largest logits (equal ones: the lower token). From the
+// gradients g of log p(t) and h of H:
+//   dx_i = g ([i = t] - p_i) - h p_i (log p_i + H).
+//
+// Bound: HBM, 4 bytes a logit forward and 8 in the gradient. A thread holds 16
+// logits at a time and a running (m, s, w), which is rescaled where their
+// maximum is a new one; sums are fp32, of a few hundred terms a thread, then
+// joined pairwise. One launch: a row that few others keep company is shared
+// out over a cluster, whose first CTA joins the parts from the others' shared
+// memory.
+#include "operators.hpp"
+
+#include <algorithm>
+#include <sstream>
+#include <stdexcept>
+
+namespace porch::detail {
+
+    namespace {
+
+        void expect(bool ok, const char* message) {
+            if (!ok) throw std::invalid_argument(message);
+        }
+
+        const char* device_source() {
+            return R"PB(
+typedef long long pb_i64;
+#define PB_WARPS (PB_THREADS / 32)
+#define PB_LOWEST __int_as_float(0xff7fffff)
+#define PB_NAN __int_as_float(0x7fffffff)
+#define PB_LOG2E 1.4426950408889634f
+
+static __device__ __forceinline__ float pb_exp2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// Finite where x is -inf, so that a weight of 0 times it is 0.
+static __device__ __forceinline__ float pb_finite(float x) { return fmaxf(x, -1e30f); }
+
+// Four values of the row from element 4 j - shift on (`shift` of them lie
+// before the row, so that the others start on 16 bytes); `none` outside it.
+static __device__ __forceinline__ float4 pb_four(const float* row, pb_i64 at, pb_i64 n, float none) {
+    if (at >= 0 && at + 4 <= n) return __ldcs(reinterpret_cast<const float4*>(row + at));
+    float v[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = at + e >= 0 && at + e < n ? __ldg(row + at + e) : none;
+    return make_float4(v[0], v[1], v[2], v[3]);
+}
+
+// What the tokens' numbers say: the token, -1 for a padded row, -2 for anything else.
+static __device__ __forceinline__ pb_i64 pb_token(float t, pb_i64 V) {
+    if (t == -1.0f) return -1;
+    return t >= 0.0f && t < (float)V && t == truncf(t) ? (pb_i64)t : -2;
+}
+
+#ifdef PB_FORWARD
+struct pb_sums { float m, s, w; };
+static __device__ __forceinline__ void pb_rescale(pb_sums& a, float m) {
+    const float d = pb_finite(a.m - m), c = pb_exp2(d * PB_LOG2E);
+    a.w = fmaf(a.s, d, a.w) * c;
+    a.s *= c;
+    a.m = m;
+}
+static __device__ __forceinline__ pb_sums pb_join(pb_sums a, pb_sums b) {
+    const float m = fmaxf(a.m, b.m);
+    pb_rescale(a, m);
+    pb_rescale(b, m);
+    a.s += b.s;
+    a.w += b.w;
+    return a;
+}
+
+static __device__ __forceinline__ pb_u32 pb_rank() {
+    pb_u32 r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+static __device__ __forceinline__ void pb_cluster_sync() {
+#if PB_CLUSTER > 1
+    asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+#endif
+}
+// A word of CTA `rank` of the cluster.
+static __device__ __forceinline__ pb_u32 pb_peer(const void* p, pb_u32 rank) {
+    pb_u32 v, a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((pb_u32)__cvta_generic_to_shared(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+
+#if PB_TOP
+// A logit and its token as one number that orders as alternatives do: larger
+// logits first (NaN last), of equal ones the lower token. 0 is no entry.
+static __device__ __forceinline__ pb_u64 pb_key(float x, pb_u32 token) {
+    const pb_u32 u = __float_as_uint(x + 0.0f); // -0 becomes 0
+    const pb_u32 k = x == x ? (u & 0x80000000u ? ~u : u | 0x80000000u) : 1u;
+    return (pb_u64)k << 32 | (0xffffffffu - token);
+}
+static __device__ __forceinline__ float pb_logit(pb_u64 key) {
+    const pb_u32 k = (pb_u32)(key >> 32);
+    return k <= 1u ? PB_NAN : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+// A warp's list: the largest keys so far in falling order, one a lane.
+static __device__ __forceinline__ void pb_insert(pb_u64& list, pb_u64 key, int lane) {
+    const int at = __popc(__ballot_sync(0xffffffffu, list > key)); // falling: a run of lanes from 0
+    const pb_u64 above = __shfl_up_sync(0xffffffffu, list, 1);
+    if (lane >= at) list = lane == at ? key : above;
+}
+// The 32 largest of two such lists: the larger of entry i and the other's entry
+// 31 - i, which rise and then fall, sorted by halving distances.
+static __device__ __forceinline__ pb_u64 pb_merge(pb_u64 a, pb_u64 b, int lane) {
+    const pb_u64 r = __shfl_xor_sync(0xffffffffu, b, 31);
+    a = a > r ? a : r;
+#pragma unroll
+    for (int m = 16; m > 0; m /= 2) {
+        const pb_u64 o = __shfl_xor_sync(0xffffffffu, a, m);
+        a = ((lane & m) == 0) == (a > o) ? a : o;
+    }
+    return a;
+}
+// Sorts one key a lane, falling.
+static __device__ __forceinline__ pb_u32 pb_sorted(pb_u32 a, int lane) {
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+        for (int m = size / 2; m > 0; m /= 2) {
+            const pb_u32 o = __shfl_xor_sync(0xffffffffu, a, m);
+            const bool keep_larger = ((lane & m) == 0) == ((lane & size) == 0);
+            a = keep_larger ? max(a, o) : min(a, o);
+        }
+    return a;
+}
+#endif
+
+// Cluster: one row, each CTA a run of `run` vectors of it.
+extern "C" __global__ void __launch_bounds__(PB_THREADS, 1024 / PB_THREADS) pb_token_logprobs(
+    const float* logits, const float* tokens, float* said, float* entropy, float* norm, float* top_said, float* top_tokens,
+    pb_i64 V, pb_i64 stride, int run, int top) {
+    __shared__ float sums[PB_WARPS][3];
+#if PB_TOP
+    __shared__ pb_u64 lists[PB_WARPS][32];
+    __shared__ pb_u32 floor_key; // no logit below it is one of the row's `top` largest
+    if (threadIdx.x == 0) floor_key = 0;
+    __syncthreads();
+#endif
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const pb_u32 row = blockIdx.x / PB_CLUSTER, rank = PB_CLUSTER > 1 ? pb_rank() : 0;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const float* x = logits + (pb_i64)row * stride;
+    const pb_i64 shift = (pb_i64)(reinterpret_cast<pb_u64>(x) >> 2 & 3);
+    const pb_i64 vectors = (V + shift + 3) >> 2, first = (pb_i64)rank * run, last = min(vectors, first + run);
+    pb_sums a = {PB_LOWEST, 0.0f, 0.0f};
+#if PB_TOP
+    pb_u64 list = 0, least = 0; // least: the list's entry `top` - 1
+#endif
+#pragma unroll 1
+    for (pb_i64 base = first; base < last; base += 4 * PB_THREADS) {
+        float v[16];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const pb_i64 j = base + q * PB_THREADS + threadIdx.x;
+            const float4 f = j < last ? pb_four(x, 4 * j - shift, V, __int_as_float(0xff800000))
+                                      : make_float4(__int_as_float(0xff800000), __int_as_float(0xff800000),
+                                                    __int_as_float(0xff800000), __int_as_float(0xff800000));
+            v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
+        }
+        float most = v[0];
+#pragma unroll
+        for (int e = 1; e < 16; ++e) most = fmaxf(most, v[e]);
+        if (most > a.m) pb_rescale(a, most);
+        float s[2] = {0.0f, 0.0f}, w[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float d = v[e] - a.m, p = pb_exp2(d * PB_LOG2E);
+            s[e & 1] += p;
+            w[e & 1] = fmaf(p, pb_finite(d), w[e & 1]);
+        }
+        a.s += s[0] + s[1];
+        a.w += w[0] + w[1];
+#if PB_TOP
+        // A lane's largest of 16 stands for one logit at least, so the `top`-th
+        // largest of 32 lanes' is a floor for all; the warps of a CTA share the
+        // highest that any of them found.
+        if (base == first) {
+            const pb_u32 mine = (pb_u32)(pb_key(most, 0) >> 32);
+            const pb_u32 bound = __shfl_sync(0xffffffffu, pb_sorted(mine, lane), top - 1);
+            if (lane == 0) atomicMax(&floor_key, bound);
+            __syncwarp();
+        }
+        pb_u32 bound = max(*reinterpret_cast<volatile pb_u32*>(&floor_key), (pb_u32)(least >> 32));
+        // As a float: what is below it (never NaN) is passed over.
+        const float low = bound <= 1u ? __int_as_float(0xff800000) : __uint_as_float(bound & 0x80000000u ? bound & 0x7fffffffu : ~bound);
+        if (__any_sync(0xffffffffu, !(most < low))) {
+            bool grew = false;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const pb_i64 at = 4 * (base + (e >> 2) * PB_THREADS + threadIdx.x) - shift + (e & 3);
+                const bool in = base + (e >> 2) * PB_THREADS + threadIdx.x < last && at >= 0 && at < V;
+                pb_u64 key = in && !(v[e] < low) ? pb_key(v[e], (pb_u32)at) : 0;
+                pb_u32 wanting = __ballot_sync(0xffffffffu, key > least);
+                while (wanting != 0) {
+                    const int from = __ffs(wanting) - 1;
+                    pb_insert(list, __shfl_sync(0xffffffffu, key, from), lane);
+                    least = __shfl_sync(0xffffffffu, list, top - 1);
+                    wanting = (wanting & (wanting - 1)) & __ballot_sync(0xffffffffu, key > least);
+                    grew = true;
+                }
+            }
+            if (grew && lane == 0) atomicMax(&floor_key, (pb_u32)(least >> 32));
+            __syncwarp();
+        }
+#endif
+    }
+    asm volatile("griddepcontrol.launch_dependents;");
+#pragma unroll
+    for (int m = 16; m > 0; m /= 2) {
+        const pb_sums o = {__shfl_xor_sync(0xffffffffu, a.m, m), __shfl_xor_sync(0xffffffffu, a.s, m),
+                           __shfl_xor_sync(0xffffffffu, a.w, m)};
+        a = pb_join(a, o);
+    }
+    if (lane == 0) { sums[warp][0] = a.m; sums[warp][1] = a.s; sums[warp][2] = a.w; }
+#if PB_TOP
+    lists[warp][lane] = list;
+    // The lists in pairs, pairs of pairs, ...
+#pragma unroll
+    for (int m = 1; m < PB_WARPS; m *= 2) {
+        __syncthreads();
+        if (warp % (2 * m) == 0) {
+            list = pb_merge(list, lists[warp + m][lane], lane);
+            lists[warp][lane] = list;
+        }
+    }
+#endif
+    __syncthreads();
+    if (warp == 0) {
+        a = lane < PB_WARPS ? pb_sums{sums[lane][0], sums[lane][1], sums[lane][2]} : pb_sums{PB_LOWEST, 0.0f, 0.0f};
+#pragma unroll
+        for (int m = PB_WARPS / 2; m > 0; m /= 2) {
+            const pb_sums o = {__shfl_xor_sync(0xffffffffu, a.m, m), __shfl_xor_sync(0xffffffffu, a.s, m),
+                               __shfl_xor_sync(0xffffffffu, a.w, m)};
+            a = pb_join(a, o);
+        }
+        __syncwarp();
+        if (lane == 0) { sums[0][0] = a.m; sums[0][1] = a.s; sums[0][2] = a.w; }
+    }
+    pb_cluster_sync();
+    if (rank == 0 && warp == 0) {
+#if PB_CLUSTER > 1
+        if (lane < PB_CLUSTER) a = {__uint_as_float(pb_peer(&sums[0][0], lane)), __uint_as_float(pb_peer(&sums[0][1], lane)),
+                                    __uint_as_float(pb_peer(&sums[0][2], lane))};
+        else a = {PB_LOWEST, 0.0f, 0.0f};
+#pragma unroll
+        for (int m = PB_CLUSTER / 2; m > 0; m /= 2) {
+            const pb_sums o = {__shfl_xor_sync(0xffffffffu, a.m, m), __shfl_xor_sync(0xffffffffu, a.s, m),
+                               __shfl_xor_sync(0xffffffffu, a.w, m)};
+            a = pb_join(a, o);
+        }
+#endif
+        a = {__shfl_sync(0xffffffffu, a.m, 0), __shfl_sync(0xffffffffu, a.s, 0), __shfl_sync(0xffffffffu, a.w, 0)};
+        const bool good = a.s > 0.0f; // not: nothing but -inf, or a NaN or +inf
+        const float total = good ? a.s : PB_NAN, log_total = logf(total);
+        if (lane == 0) {
+            const pb_i64 t = pb_token(__ldg(tokens + row), V);
+            said[row] = t >= 0 ? (__ldg(x + t) - a.m) - log_total : (t == -1 ? 0.0f : PB_NAN);
+            entropy[row] = log_total - a.w / total;
+            norm[2 * (pb_i64)row] = a.m;
+            norm[2 * (pb_i64)row + 1] = total;
+        }
+#if PB_TOP
+#if PB_CLUSTER > 1
+        pb_u64 other[PB_CLUSTER - 1];
+#pragma unroll
+        for (int c = 1; c < PB_CLUSTER; ++c)
+            other[c - 1] = (pb_u64)pb_peer(reinterpret_cast<const pb_u32*>(&lists[0][lane]) + 1, c) << 32 |
+                           pb_peer(&lists[0][lane], c);
+#pragma unroll
+        for (int c = 1; c < PB_CLUSTER; ++c) list = pb_merge(list, other[c - 1], lane);
+#endif
+        if (lane < top) {
+            top_said[(pb_i64)row * top + lane] = (pb_logit(list) - a.m) - log_total;
+            top_tokens[(pb_i64)row * top + lane] = (float)(0xffffffffu - (pb_u32)list);
+        }
+#endif
+    }
+    pb_cluster_sync(); // nobody leaves while its shared memory is read
+}
+#endif
+
+#ifdef PB_BACKWARD
+// Block: `PB_ROUNDS` times 1024 gradients of one row. exp(d) = 2^(t + r) with
+// t the rounded product d log2 e and r what the rounding left, so that p is
+// within a few units of its last place also far below the maximum.
+#define PB_ROUNDS 4
+extern "C" __global__ void __launch_bounds__(256) pb_token_logprobs_grad(
+    const float* d_said, const float* d_entropy, const float* logits, const float* tokens, const float* norm,
+    const float* entropy, float* out, pb_i64 V, pb_i64 stride, pb_u32 blocks) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const pb_u32 row = blockIdx.x / blocks;
+    const float* x = logits + (pb_i64)row * stride;
+    float* to = out + (pb_i64)row * V;
+    const pb_i64 shift = (pb_i64)(reinterpret_cast<pb_u64>(to) >> 2 & 3);
+    const bool same = (pb_i64)(reinterpret_cast<pb_u64>(x) >> 2 & 3) == shift; // the stores are aligned, the loads where they can be
+    const pb_i64 t = pb_token(__ldg(tokens + row), V);
+    float g = __ldg(d_said + row), m = __ldg(norm + 2 * (pb_i64)row), s = __ldg(norm + 2 * (pb_i64)row + 1);
+#if PB_ENTROPY
+    const float h = __ldg(d_entropy + row), ent = __ldg(entropy + row);
+#endif
+    g = t >= 0 ? g : (t == -1 ? 0.0f : PB_NAN);
+    const float inv = 1.0f / s;
+#if PB_ENTROPY
+    const float rest = ent - logf(s);
+    const bool nothing = t == -1 && h == 0.0f; // a padded row, whatever it holds
+#else
+    const bool nothing = t == -1;
+#endif
+    const pb_i64 first = (pb_i64)(blockIdx.x % blocks) * (PB_ROUNDS * 256) + threadIdx.x;
+    float4 v[PB_ROUNDS];
+#pragma unroll
+    for (int q = 0; q < PB_ROUNDS; ++q) {
+        const pb_i64 at = 4 * (first + q * 256) - shift;
+        if (at >= V) { v[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f); continue; }
+        if (same) v[q] = pb_four(x, at, V, 0.0f);
+        else {
+            float e[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) e[i] = at + i >= 0 && at + i < V ? __ldg(x + at + i) : 0.0f;
+            v[q] = make_float4(e[0], e[1], e[2], e[3]);
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < PB_ROUNDS; ++q) {
+        const pb_i64 at = 4 * (first + q * 256) - shift;
+        if (at >= V) break;
+        float d[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float rel = pb_get(v[q], e) - m, low = pb_finite(rel);
+            const float b = low * PB_LOG2E, r = fmaf(low, PB_LOG2E, -b) + low * 1.9259629911266175e-8f;
+            const float z = pb_exp2(b);
+            const float p = (rel == rel ? fmaf(z * r, 0.69314718055994531f, z) : rel) * inv;
+#if PB_ENTROPY
+            const float c = p == 0.0f ? 0.0f : -fmaf(h, low + rest, g);
+#else
+            const float c = -g;
+#endif
+            d[e] = nothing ? 0.0f : fmaf(p, c, at + e == t ? g : 0.0f);
+        }
+        if (at >= 0 && at + 4 <= V) __stcs(reinterpret_cast<float4*>(to + at), make_float4(d[0], d[1], d[2], d[3]));
+        else
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (at + e >= 0 && at + e < V) to[at + e] = d[e];
+    }
+}
+#endif
+)PB";
+        }
+
+        // How rows are shared out.
+        struct shape {
+            int cluster = 1, threads = 256;
+            bool top = false;
+        };
+
+        // CTAs of a row: more as long as they all run at once and each thread
+        // has its 16 logits; and threads of a CTA, more where an SM has one.
+        shape shape_for(int64_t rows, int64_t vocab, bool top, int sms) {
+            shape r;
+            r.top = top;
+            while (r.cluster < 8 && rows * r.cluster * 2 <= int64_t{4} * sms && vocab >= int64_t{r.cluster} * 2 * 4096) r.cluster *= 2;
+            while (r.threads < 1024 && rows * r.cluster * r.threads * 2 <= int64_t{1024} * sms &&
+                   vocab >= int64_t{r.cluster} * r.threads * 32)
+                r.threads *= 2;
+            return r;
+        }
+
+        std::string forward_source(const shape& f) {
+            std::ostringstream os;
+            os << kernel_prelude() << "#define PB_FORWARD 1\n#define PB_CLUSTER " << f.cluster << "\n#define PB_THREADS "
+               << f.threads << "\n#define PB_TOP " << (f.top ? 1 : 0) << "\n" << device_source();
+            return os.str();
+        }
+
+        std::string backward_source(bool entropy) {
+            std::ostringstream os;
+            os << kernel_prelude() << "#define PB_BACKWARD 1\n#define PB_THREADS 256\n#define PB_ENTROPY " << (entropy ? 1 : 0)
+               << "\n" << device_source();
+            return os.str();
+        }
+
+        const char kForward[] = "pb_token_logprobs";
+        const char kBackward[] = "pb_token_logprobs_grad";
+
+        op_kernel& forward_kernel(const shape& f) {
+            const op_key key{reinterpret_cast<int64_t>(kForward), f.cluster, f.threads, f.top};
+            return op_kernel_for(key, [&](op_kernel& k) {
+                k.name = kForward;
+                k.source = forward_source(f);
+            });
+        }
+
+        op_kernel& backward_kernel(bool entropy) {
+            const op_key key{reinterpret_cast<int64_t>(kBackward), entropy};
+            return op_kernel_for(key, [&](op_kernel& k) {
+                k.name = kBackward;
+                k.source = backward_source(entropy);
+            });
+        }
+
+        // [rows, vocabulary] of logits, and a token of each row.
+        void check_logits(const tensor& logits, const tensor& tokens) {
+            const auto s = logits.shape();
+            expect(s.size() == 2, "token_logprobs: logits must be [rows, vocabulary]");
+            expect(s[1] >= 1 && s[1] <= (index_t{1} << 24), "token_logprobs: a vocabulary of 1 to 2^24 tokens (float32 counts them exactly)");
+            expect(has_shape(tokens, {s[0]}), "token_logprobs: tokens must be [rows]");
+        }
+
+    } // namespace
+
+    std::vector<tensor> token_logprobs(const tensor& logits, const tensor& tokens, int64_t top) {
+        check_logits(logits, tokens);
+        const auto s = shape_of(logits);
+        expect(top >= 0 && top <= 32 && top <= s[1], "token_logprobs: top must be 0 to 32, and at most the vocabulary");
+        const int device = device_of(logits, "token_logprobs");
+        expect(device_of(tokens, "token_logprobs") == device, "token_logprobs: operands must live on one device");
+        auto stream = current_stream(device);
+        op_operand x = operand(logits, stream, true), t = operand(tokens, stream, false);
+        int64_t rows = s[0], vocab = s[1];
+        op_result said = new_result({rows}, device, stream), entropy = new_result({rows}, device, stream);
+        op_result norm = new_result({rows, 2}, device, stream);
+        op_result top_said, top_tokens;
+        if (top != 0) {
+            top_said = new_result({rows, top}, device, stream);
+            top_tokens = new_result({rows, top}, device, stream);
+        }
+        if (rows != 0) {
+            const shape f = shape_for(rows, vocab, top != 0, sm_count(device));
+            op_kernel& kernel = forward_kernel(f);
+            expect(rows <= 0x7fffffff / f.cluster, "token_logprobs: too many rows");
+            // Vectors of a CTA: with up to three values before the row's first.
+            int run = static_cast<int>(((vocab + 6) / 4 + f.cluster - 1) / f.cluster), most = static_cast<int>(top);
+            int64_t stride = rows > 1 ? x.strides[0] : vocab;
+            void* params[] = {&x.ptr,        &t.ptr,          &said.ptr, &entropy.ptr, &norm.ptr, &top_said.ptr,
+                              &top_tokens.ptr, &vocab,        &stride,   &run,         &most};
+            op_launch(kernel, device, stream, {static_cast<uint32_t>(rows * f.cluster), 1, 1},
+                      static_cast<uint32_t>(f.threads), params, static_cast<uint32_t>(f.cluster));
+        }
+        std::vector<tensor> out;
+        out.push_back(finish(std::move(said)));
+        out.push_back(finish(std::move(entropy)));
+        out.push_back(finish(std::move(norm)));
+        if (top != 0) {
+            out.push_back(finish(std::move(top_said)));
+            out.push_back(finish(std::move(top_tokens)));
+        }
+        return out;
+    }
+
+    tensor token_logprobs_backward(const tensor& d_said, const tensor& logits, const tensor& tokens, const tensor& norm,
+                                   const tensor* d_entropy, const tensor* entropy) {
+        check_logits(logits, tokens);
+        const auto s = shape_of(logits);
+        expect(has_shape(d_said, {s[0]}), "token_logprobs_backward: d_logprobs must be [rows]");
+        expect(has_shape(norm, {s[0], 2}), "token_logprobs_backward: norm must be [rows, 2], as token_logprobs gave it");
+        expect((d_entropy != nullptr) == (entropy != nullptr), "token_logprobs_backward: d_entropy needs entropy, and entropy d_entropy");
+        expect(d_entropy == nullptr || (has_shape(*d_entropy, {s[0]}) && has_shape(*entropy, {s[0]})),
+               "token_logprobs_backward: d_entropy and entropy must be [rows]");
+        const int device = device_of(logits, "token_logprobs_backward");
+        auto stream = current_stream(device);
+        op_operand x = operand(logits, stream, true), t = operand(tokens, stream, false), g = operand(d_said, stream, false),
+                   n = operand(norm, stream, false), h, e;
+        if (d_entropy != nullptr) {
+            h = operand(*d_entropy, stream, false);
+            e = operand(*entropy, stream, false);
+        }
+        op_result out = new_result(s, device, stream);
+        int64_t rows = s[0], vocab = s[1];
+        if (rows != 0) {
+            op_kernel& kernel = backward_kernel(d_entropy != nullptr);
+            uint32_t per_row = static_cast<uint32_t>(((vocab + 6) / 4 + 1023) / 1024);
+            expect(rows <= 0x7fffffff / static_cast<int64_t>(per_row), "token_logprobs_backward: too many rows");
+            int64_t stride = rows > 1 ? x.strides[0] : vocab;
+            void* params[] = {&g.ptr, &h.ptr, &x.ptr, &t.ptr, &n.ptr, &e.ptr, &out.ptr, &vocab, &stride, &per_row};
+            op_launch(kernel, device, stream, {static_cast<uint32_t>(rows * per_row), 1, 1}, 256, params);
+        }
+        return finish(std::move(out));
+    }
+
+    void token_logprobs_sources(kernel_list& out) {
+        for (const shape& f : {shape{1, 256, false}, shape{1, 256, true}, shape{8, 1024, true}, shape{4, 512, false}})
+            out.emplace_back("pb_token_logprobs_" + std::to_string(f.cluster) + "x" + std::to_string(f.threads) + (f.top ? "_top" : ""),
+                             forward_source(f));
+        out.emplace_back("pb_token_logprobs_grad", backward_source(false));
+        out.emplace_back("pb_token_logprobs_grad_entropy", backward_source(true));
+    }
+
+} // namespace porch::detail

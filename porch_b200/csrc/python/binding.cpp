@@ -23,6 +23,8 @@ namespace {
     X(pb_tensor_interface)                                                                                   \
     X(pb_qk_norm_rope)                                                                                       \
     X(pb_qk_norm_rope_backward)                                                                              \
+    X(pb_token_logprobs)                                                                                     \
+    X(pb_token_logprobs_backward)                                                                            \
     X(pb_paged_attention)                                                                                    \
     X(pb_paged_attention_scored)                                                                             \
     X(pb_kv_evict)
@@ -245,6 +247,32 @@ namespace {
         return wrap_all(out);
     }
 
+    // (logits, tokens, top)
+    PyObject* token_logprobs(PyObject*, PyObject* const* args, Py_ssize_t n) {
+        tensors t;
+        int64_t top = 0;
+        std::array<pb_tensor*, 5> out{};
+        if (!expect(n, 3) || !t.take(args, 2) || !integer(args[2], top)) return nullptr;
+        if (!call([&] { return native.pb_token_logprobs(t.value[0], t.value[1], top, out.data()); })) return nullptr;
+        if (top != 0) return wrap_all(out);
+        return wrap_all(std::array<pb_tensor*, 3>{out[0], out[1], out[2]});
+    }
+
+    // (gradient, logits, tokens, norm, gradient of the entropy or None, entropy or None)
+    PyObject* token_logprobs_backward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+        tensors t, more[2];
+        pb_tensor* out = nullptr;
+        if (!expect(n, 6) || !t.take(args, 4)) return nullptr;
+        for (int i = 0; i < 2; ++i)
+            if (args[4 + i] != Py_None && !more[i].take(args + 4 + i, 1)) return nullptr;
+        const auto& v = t.value;
+        if (!call([&] {
+                return native.pb_token_logprobs_backward(v[0], v[1], v[2], v[3], more[0].value[0], more[1].value[0], &out);
+            }))
+            return nullptr;
+        return wrap(out);
+    }
+
     // (q, batch, scale)
     PyObject* paged_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
         tensors t;
@@ -333,6 +361,8 @@ namespace {
     PyMethodDef methods[] = {
         method("qk_norm_rope", qk_norm_rope),
         method("qk_norm_rope_backward", qk_norm_rope_backward),
+        method("token_logprobs", token_logprobs),
+        method("token_logprobs_backward", token_logprobs_backward),
         method("paged_attention", paged_attention),
         method("paged_attention_scored", paged_attention_scored),
         method("kv_evict", kv_evict),

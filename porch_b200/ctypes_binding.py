@@ -77,6 +77,19 @@ def qk_norm_rope_backward(*args):
     return tuple(_tensor_type(x) for x in out)
 
 
+def token_logprobs(logits, tokens, top):
+    t, top = _tensors([logits, tokens]), operator.index(top)
+    out = (c_void_p * 5)()
+    _check(_load().pb_token_logprobs(*[x._h for x in t], top, out))
+    return tuple(_tensor_type(x) for x in out if x)
+
+
+def token_logprobs_backward(*args):
+    t = _tensors(args[:4])
+    more = [None if x is None else _tensors([x])[0] for x in args[4:6]]
+    return _call("pb_token_logprobs_backward", 1, *[x._h for x in t], *[x and x._h for x in more])[0]
+
+
 def paged_attention(q, batch, scale):
     (q,), scale = _tensors([q]), c_float(scale)
     return _call("pb_paged_attention", 1, q._h, batch, scale)[0]
