@@ -308,14 +308,18 @@ int pb_token_logprobs_backward(const pb_tensor* d_logprobs, const pb_tensor* log
 
 /* ---- a paged key/value cache --------------------------------------------- */
 /* Pools of `pages` pages of `page_size` (a power of two, 8 to 256) slots for
- * keys and for values, [pages, kv_heads, page_size, head_dim], in float32 or
- * bfloat16; head_dim a multiple of 8 up to 256. The values start undefined;
+ * keys and for values, [pages, kv_heads, page_size, head_dim], in float32,
+ * bfloat16 or int8; head_dim a multiple of 8 up to 256 (of 16 in int8). An int8
+ * cache keeps a float32 scale for each row (the key or value of one token and
+ * head), the row's largest size / 127, and the row / scale rounded to nearest,
+ * ties to even; what it holds is code x scale. A row with a value that is not
+ * finite is held as NaN, one whose values are all below 2^-96 as zeros. The values start undefined;
  * nothing reads a slot past a sequence's length. Calls that write a cache
  * (append, evict) and calls that read it are ordered on the device in the
  * order in which they are made, from whatever threads. */
 typedef struct pb_kv_cache_s pb_kv_cache;
 typedef struct pb_kv_batch_s pb_kv_batch;
-enum pb_cache_type { PB_CACHE_F32 = 0, PB_CACHE_BF16 = 1 };
+enum pb_cache_type { PB_CACHE_F32 = 0, PB_CACHE_BF16 = 1, PB_CACHE_INT8 = 3 };
 int pb_kv_cache_create(int64_t pages, int64_t page_size, int64_t kv_heads, int64_t head_dim,
                        int type, int device, pb_kv_cache** out);
 void pb_kv_cache_release(pb_kv_cache* cache);
@@ -327,6 +331,9 @@ int pb_kv_cache_data(const pb_kv_cache* cache, uint64_t* keys, uint64_t* values,
  * was called on the cache so far is ordered. Asked for again after each call
  * that the reader has to see. */
 int pb_kv_cache_interface(pb_kv_cache* cache, uint64_t* keys, uint64_t* values, void** stream);
+/* Device addresses of an int8 cache's scales, [pages, kv_heads, page_size]; to
+ * be ordered as the pools. */
+int pb_kv_cache_scales(const pb_kv_cache* cache, uint64_t* keys, uint64_t* values);
 /* The sequences of one step: `tables` [sequences, width] names the pages of
  * each, `lengths` its slots in use (new tokens included). `appended` (NULL: 1
  * each, 0 for an empty one) says how many of them are new, the last ones;
@@ -340,8 +347,11 @@ int pb_kv_batch_create(pb_kv_cache* cache, const int32_t* tables, size_t sequenc
 int pb_kv_batch_on(const pb_kv_batch* batch, pb_kv_cache* cache, pb_kv_batch** out);
 void pb_kv_batch_release(pb_kv_batch* batch);
 /* Writes k and v, [new tokens of all sequences, kv_heads, head_dim], into
- * the new slots (rounded to nearest in a bfloat16 cache). */
+ * the new slots (rounded to nearest in a bfloat16 or int8 cache). */
 int pb_kv_append(pb_kv_batch* batch, const pb_tensor* k, const pb_tensor* v);
+/* Keys and values of every slot in use, sequence after sequence, as float32:
+ * [slots of all sequences, kv_heads, head_dim] each. */
+int pb_kv_read(pb_kv_batch* batch, pb_tensor** k, pb_tensor** v);
 /* softmax(scale q K^T) V for one query per sequence: q and the result
  * [sequences, q_heads, head_dim], q_heads a multiple of kv_heads (query head
  * i reads key head i / (q_heads / kv_heads)). An empty sequence gives zeros.

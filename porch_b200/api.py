@@ -550,31 +550,37 @@ def token_logprobs_backward(d_logprobs, logits, tokens, norm, d_entropy=None, en
 
 class _Pool:
     """A cache pool in place, for another library on the same GPU; a bfloat16
-    pool as its 16 raw bits. Keeps the cache alive. Each time it is asked for
+    pool as its 16 raw bits, an int8 pool's scales as a pool of their own. Keeps the cache alive. Each time it is asked for
     its interface, the `stream` in it is the calling thread's, behind all that
     was called on the cache so far."""
 
-    def __init__(self, cache: "KVCache", which: int):
-        self.cache, self._which = cache, which
+    def __init__(self, cache: "KVCache", which: int, scales: bool = False):
+        self.cache, self._which, self._scales = cache, which, scales
 
     @property
     def __cuda_array_interface__(self) -> dict:
         c, at, stream = self.cache, (c_uint64(), c_uint64()), c_void_p()
         _check(lib().pb_kv_cache_interface(c._h, byref(at[0]), byref(at[1]), byref(stream)))
-        return {"shape": (c.pages, c.kv_heads, c.page_size, c.head_dim), "typestr": "<u2" if c.dtype == "bf16" else "<f4",
+        shape, kind = (c.pages, c.kv_heads, c.page_size), "<f4"
+        if self._scales:
+            _check(lib().pb_kv_cache_scales(c._h, byref(at[0]), byref(at[1])))
+        else:
+            shape, kind = (*shape, c.head_dim), {"f32": "<f4", "bf16": "<u2", "int8": "|i1"}[c.dtype]
+        return {"shape": shape, "typestr": kind,
                 "data": (at[self._which].value, False), "version": 3, "stream": stream.value}
 
 
 class KVCache:
     """Pools of pages of keys and values, [pages, kv_heads, page_size,
-    head_dim], in "f32" or "bf16". An extension."""
+    head_dim], in "f32", "bf16" or "int8" (codes and a scale for each row, its
+    largest size / 127). An extension."""
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: str = "f32", device: int = 0):
         self._h = c_void_p()
-        if dtype not in ("f32", "bf16"):
-            raise InvalidArgument('cache: dtype must be "f32" or "bf16"')
+        if dtype not in ("f32", "bf16", "int8"):
+            raise InvalidArgument('cache: dtype must be "f32", "bf16" or "int8"')
         _check(lib().pb_kv_cache_create(int(pages), int(page_size), int(kv_heads), int(head_dim),
-                                        int(dtype == "bf16"), int(device), byref(self._h)))
+                                        {"f32": 0, "bf16": 1, "int8": 3}[dtype], int(device), byref(self._h)))
         self.pages, self.page_size, self.kv_heads, self.head_dim = int(pages), int(page_size), int(kv_heads), int(head_dim)
         self.dtype, self.device = dtype, int(device)
 
@@ -596,6 +602,13 @@ class KVCache:
     def pools(self) -> tuple[_Pool, _Pool]:
         """Keys and values in place (__cuda_array_interface__)."""
         return _Pool(self, 0), _Pool(self, 1)
+
+    def scales(self) -> tuple[_Pool, _Pool]:
+        """An int8 cache's scales of keys and values in place, [pages,
+        kv_heads, page_size]."""
+        if self.dtype != "int8":
+            raise InvalidArgument("cache: only an int8 cache has scales")
+        return _Pool(self, 0, True), _Pool(self, 1, True)
 
     def batch(self, tables, lengths, appended=None, newest=None) -> "Batch":
         """The sequences of one step: tables [sequences, width] of page
@@ -658,6 +671,11 @@ class Batch:
         head_dim] in the order of the sequences."""
         k, v = _realised(k), _realised(v)
         _check(lib().pb_kv_append(self._h, k._h, v._h))
+
+    def read(self) -> tuple[Tensor, Tensor]:
+        """Keys and values of every slot in use as float32, [slots of all
+        sequences, kv_heads, head_dim], sequence after sequence."""
+        return _binding.kv_read(self._address)
 
 
 def attention_plan(lengths, kv_heads: int, ctas: int, chunks: int = 1) -> str:

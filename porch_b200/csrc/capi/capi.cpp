@@ -803,7 +803,7 @@ int pb_kv_cache_data(const pb_kv_cache* cache, uint64_t* keys, uint64_t* values,
         require(cache, "cache");
         if (keys) *keys = porch::detail::address(cache->value->k);
         if (values) *values = porch::detail::address(cache->value->v);
-        if (bytes) *bytes = cache->value->k.size_bytes();
+        if (bytes) *bytes = static_cast<size_t>(cache->value->values_bytes());
     });
 }
 
@@ -816,6 +816,18 @@ int pb_kv_cache_interface(pb_kv_cache* cache, uint64_t* keys, uint64_t* values, 
         *stream = porch::detail::cache_ordered(*cache->value);
         *keys = porch::detail::address(cache->value->k);
         *values = porch::detail::address(cache->value->v);
+    });
+}
+
+int pb_kv_cache_scales(const pb_kv_cache* cache, uint64_t* keys, uint64_t* values) {
+    return guarded([&] {
+        require(cache, "cache");
+        require(keys, "keys");
+        require(values, "values");
+        const auto& c = *cache->value;
+        if (c.type != porch::detail::cache_type::i8) throw std::invalid_argument("cache: only an int8 cache has scales");
+        *keys = porch::detail::address(c.k) + static_cast<uint64_t>(c.values_bytes());
+        *values = porch::detail::address(c.v) + static_cast<uint64_t>(c.values_bytes());
     });
 }
 
@@ -850,6 +862,18 @@ int pb_kv_append(pb_kv_batch* batch, const pb_tensor* k, const pb_tensor* v) {
         require(k, "k");
         require(v, "v");
         porch::detail::cache_append(*batch->value, k->value, v->value);
+    });
+}
+
+int pb_kv_read(pb_kv_batch* batch, pb_tensor** k, pb_tensor** v) {
+    return guarded([&] {
+        require(k, "k");
+        require(v, "v");
+        *k = *v = nullptr;
+        require(batch, "batch");
+        auto r = porch::detail::cache_read(*batch->value);
+        *k = wrap(std::move(r[0]));
+        *v = wrap(std::move(r[1]));
     });
 }
 
@@ -930,7 +954,7 @@ int pb_kv_attention_shape(int64_t head_dim, int type, int64_t group, int64_t* ct
     return guarded([&] {
         require(ctas_per_sm, "ctas_per_sm");
         require(shared_bytes, "shared_bytes");
-        if (head_dim < 8 || head_dim > 256 || head_dim % 8 != 0 || type < PB_CACHE_F32 || type > PB_CACHE_BF16 || group < 1)
+        if (head_dim < 8 || head_dim > 256 || head_dim % 8 != 0 || (type != PB_CACHE_F32 && type != PB_CACHE_BF16 && type != PB_CACHE_INT8) || (type == PB_CACHE_INT8 && head_dim % 16 != 0) || group < 1)
             throw std::invalid_argument("attention shape: no such head size, type or group");
         const auto [ctas, bytes] =
             porch::detail::attention_shape(head_dim, static_cast<porch::detail::cache_type>(type), group);

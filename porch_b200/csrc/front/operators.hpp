@@ -113,7 +113,7 @@ namespace porch::detail {
                                    const tensor* d_entropy, const tensor* entropy);
 
     // --------------------------------------------------------------- cache --
-    enum class cache_type : int { f32 = 0, bf16 = 1 };
+    enum class cache_type : int { f32 = 0, bf16 = 1, i8 = 3 };
 
     // How the last attention over a cache shared out its work, for which the
     // next batch prepares its plan: with the upload that the batch waits for
@@ -124,7 +124,8 @@ namespace porch::detail {
     };
 
     // Pools of pages of keys and values: [pages, heads, page_size, dim], so
-    // the rows of one page and head are one contiguous block.
+    // the rows of one page and head are one contiguous block. An 8-bit pool has
+    // its rows' scales, [pages, heads, page_size], behind the codes.
     struct kv_cache {
         int64_t pages = 0, page_size = 0, heads = 0, dim = 0;
         cache_type type = cache_type::f32;
@@ -136,7 +137,8 @@ namespace porch::detail {
         // before it is taken.
         std::mutex order;
         std::shared_ptr<plan_hint> hint = std::make_shared<plan_hint>();
-        int width() const { return type == cache_type::bf16 ? 2 : 4; } // bytes of a value
+        int width() const { return type == cache_type::f32 ? 4 : (type == cache_type::bf16 ? 2 : 1); } // bytes of a value
+        int64_t values_bytes() const { return pages * heads * page_size * dim * width(); } // of one pool, without scales
         // TMA maps of both pools as [rows, dim]: boxes of 128 bytes by a page,
         // or by 64 rows of a larger one.
         struct alignas(64) tensor_map {
@@ -170,15 +172,16 @@ namespace porch::detail {
         std::shared_ptr<kv_cache> cache;
         std::vector<int64_t> lengths;
         std::vector<int64_t> newest;   // position of each sequence's newest slot
-        int64_t longest = 0, tokens = 0; // tokens: new ones, over all sequences
+        int64_t longest = 0, tokens = 0, slots = 0; // tokens: new ones, slots: all, over all sequences
         int64_t table_width = 0;
         bool shared_pages = false;       // a page serves two sequences, or one twice
-        cuda_jit::device_buffer data;    // int32: lengths, newest, tables, then 8-byte rows
+        cuda_jit::device_buffer data;    // int32: lengths, newest, tables, then 8-byte rows and starts
         // Made once with the batch for the number of query heads that its cache
         // last saw (up to 8 for each key head until then), and by the first
         // call that needs another.
         std::shared_ptr<batch_plans> plans = std::make_shared<batch_plans>();
-        uint64_t lengths_at = 0, newest_at = 0, tables_at = 0, rows_at = 0; // device addresses
+        // Device addresses. starts: the slots of all sequences before each, and of all.
+        uint64_t lengths_at = 0, newest_at = 0, tables_at = 0, rows_at = 0, starts_at = 0;
         int64_t sequences() const { return static_cast<int64_t>(lengths.size()); }
     };
     std::shared_ptr<kv_batch> make_batch(std::shared_ptr<kv_cache> cache, const int32_t* tables, size_t sequences,
@@ -205,6 +208,8 @@ namespace porch::detail {
 
     // Writes the step's new keys and values, [tokens, heads, dim], into their rows.
     void cache_append(kv_batch& batch, const tensor& k, const tensor& v);
+    // {keys, values} of every slot in use, [slots of all sequences, heads, dim].
+    std::array<tensor, 2> cache_read(kv_batch& batch);
     // {attention, new scores} (the second only when `scored`).
     std::vector<tensor> paged_attention(const tensor& q, kv_batch& batch, float scale, bool scored,
                                         const tensor* scores);

@@ -54,24 +54,27 @@ namespace porch::detail {
         // The whole layout of a kernel follows from these.
         struct form {
             int heads = 1, dim = 0, page = 0;
-            bool bf16 = false, scored = false;
+            cache_type type = cache_type::f32;
+            bool scored = false;
             int stall = 0; // the test hook's mode
             int join_threads = 128;
             int tiles8 = 1; // groups of 8 query heads that a row holds (1 or 2)
-            int width() const { return bf16 ? 2 : 4; }
+            int width() const { return type == cache_type::f32 ? 4 : (type == cache_type::bf16 ? 2 : 1); }
             int planes() const { return (dim * width() + 127) / 128; }
             int unit() const { return planes() * 8192; }                       // 64 slots of K or of V
             int steps() const { return ((dim * width() + 31) / 32 + 1) & ~1; } // 32-byte k-steps, an even number
-            int terms() const { return bf16 ? 3 : 2; }
+            int scales() const { return type == cache_type::i8 ? 256 : 0; } // bytes of a unit's
+            int terms() const { return type == cache_type::f32 ? 2 : 3; }
             int q_row() const { return steps() * 32 + 16; }
             int p_row() const { return 64 * width() + 16; }
             int small() const { // everything but the ring
-                return terms() * tiles8 * 8 * (q_row() + p_row()) + 2 * 4 * tiles8 * 8 * 4;
+                return terms() * tiles8 * 8 * (q_row() + p_row()) + 2 * 4 * tiles8 * 8 * 4 +
+                       (type == cache_type::i8 ? 5 * tiles8 * 8 * 4 : 0);
             }
             int per_sm() const { return choose().first; }
             int ring() const { return choose().second; }
             int chunks(int group) const { return (group + 8 * tiles8 - 1) / (8 * tiles8); } // rows of a key head
-            int smem() const { return 1024 + ring() * unit() + small(); }
+            int smem() const { return 1024 + ring() * (unit() + scales()) + small(); }
             // What a CTA takes of an SM's 228 KB: that, the kernel's static
             // arrays (the ring's barriers and a flag, which the kernel checks
             // against kStatic) with the rounding of the sum, and the KB that
@@ -87,10 +90,10 @@ namespace porch::detail {
             // units, 124 with three of three).
             std::pair<int, int> choose() const {
                 for (int n = 4; n > 1; --n) {
-                    const int r = ((228 * 1024) / n - 2048 - kStatic - small()) / unit();
+                    const int r = ((228 * 1024) / n - 2048 - kStatic - small()) / (unit() + scales());
                     if (r >= 3) return {n, std::min(r, 6)};
                 }
-                return {1, std::min((227 * 1024 - 1024 - kStatic - small()) / unit(), 6)};
+                return {1, std::min((227 * 1024 - 1024 - kStatic - small()) / (unit() + scales()), 6)};
             }
         };
 
@@ -108,10 +111,15 @@ typedef long long pb_i64;
 #define PB_PROW (64 * PB_ESZ + 16)
 #define PB_MT ((PB_D + 15) / 16)         // 16-channel tiles of the result
 #define PB_MTW ((PB_MT + 3) / 4)         // of one warp
-#if PB_ESZ == 2
-#define PB_TERMS 3
-#else
+#if PB_ESZ == 4
 #define PB_TERMS 2
+#else
+#define PB_TERMS 3
+#endif
+#if PB_ESZ == 1 // sums of products of integers are exact
+typedef int pb_acc;
+#else
+typedef float pb_acc;
 #endif
 
 struct __align__(64) pb_tmap { unsigned long long opaque[16]; };
@@ -153,6 +161,18 @@ static __device__ __forceinline__ bool pb_wait(pb_u32 bar, pb_u32 parity, volati
         }
     }
 }
+#if PB_ESZ == 1
+// PB_BOX scales, 32 bytes or more.
+static __device__ __forceinline__ void pb_bulk_load(pb_u32 dst, const float* src, pb_u32 bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 :: "r"(dst), "l"((unsigned long long)src), "r"(PB_BOX * 4), "r"(bar) : "memory");
+}
+static __device__ __forceinline__ float pb_shared(pb_u32 at) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+#endif
 static __device__ __forceinline__ void pb_tma_load(pb_u32 dst, const pb_tmap* map, pb_u32 bar, int x, int y) {
     asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
                  :: "r"(dst), "l"((unsigned long long)map), "r"(bar), "r"(x), "r"(y) : "memory");
@@ -183,7 +203,33 @@ static __device__ __forceinline__ void pb_ldm4t(pb_u32* r, pb_u32 addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-#if PB_ESZ == 2
+#if PB_ESZ == 1
+static __device__ __forceinline__ void pb_mma(int* c, const pb_u32* a, const pb_u32* b) {
+    asm volatile("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+// Digits of a whole number of up to PB_DIGITS = 127 (65536 + 256 + 1), base 256
+// and from -127 or -128 to 127, lowest first, in its bytes: adding 128 at each
+// place and flipping each byte's top bit makes the carries.
+#define PB_DIGITS 8355711
+#define PB_WEIGHTS 8347552.0f // of those less 2^-10
+static __device__ __forceinline__ pb_u32 pb_digits(int x) { return ((pb_u32)x + 0x00808080u) ^ 0x00808080u; }
+// What they say of a sum of products: exact in integers but for the last step.
+static __device__ __forceinline__ float pb_of_digits(int lowest, int middle, int highest) {
+    return fmaf((float)highest, 65536.0f, (float)(middle * 256 + lowest));
+}
+static __device__ __forceinline__ float pb_max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+static __device__ __forceinline__ float pb_log2(float x) {
+    float r;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+#elif PB_ESZ == 2
 static __device__ __forceinline__ void pb_mma(float* c, const pb_u32* a, const pb_u32* b) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -269,30 +315,90 @@ static __device__ __forceinline__ int pb_page(const pb_at& a, const int* tables,
 // the first use; zero past its heads and the head size.
 #define PB_Q_HEAD (PB_STEPS * 32 / PB_ESZ)
 #define PB_Q_EACH ((PB_HT * PB_Q_HEAD + 127) / 128)
+#if PB_ESZ == 1
+#define PB_Q_RUNS ((PB_Q_HEAD + 127) / 128)
+#define PB_Q_EACH8 (PB_HT / 4 * PB_Q_RUNS * 4)
+struct pb_queries { float x[PB_Q_EACH8]; };
+#else
+#define PB_Q_EACH8 PB_Q_EACH
 struct pb_queries { float x[PB_Q_EACH]; };
+#endif
 static __device__ __forceinline__ void pb_load_queries(pb_queries& r, const float* q, const pb_at& a, pb_i64 q_seq,
                                                        pb_i64 q_head, int group) {
     const int heads = min(PB_HT, group - a.chunk * PB_HT), first = a.h * group + a.chunk * PB_HT;
+#if PB_ESZ == 1 // a warp has every fourth head, a lane runs of four channels
+#pragma unroll
+    for (int j = 0; j < PB_Q_EACH8; ++j) {
+        const int head = (threadIdx.x >> 5) + 4 * (j / (4 * PB_Q_RUNS));
+        const int d = (j / 4 % PB_Q_RUNS) * 128 + (threadIdx.x & 31) * 4 + j % 4;
+        r.x[j] = head < heads && d < PB_D ? __ldg(q + a.s * q_seq + (first + head) * q_head + d) : 0.0f;
+    }
+#else
 #pragma unroll
     for (int j = 0; j < PB_Q_EACH; ++j) {
         const int e = threadIdx.x + 128 * j, head = e / PB_Q_HEAD, d = e % PB_Q_HEAD;
         r.x[j] = head < heads && d < PB_D ? __ldg(q + a.s * q_seq + (first + head) * q_head + d) : 0.0f;
     }
+#endif
 }
+#if PB_ESZ == 1
+// A head's queries as three digits each, in units of a power of two 2^-22 to
+// 2^-23 of the head's largest size: 24 bits of that, and a rounding to nearest.
+// A head that nowhere reaches 2^-100 counts as zeros; one that is not finite has
+// a unit of NaN. Channels past the head size are zeros.
+static __device__ __forceinline__ void pb_split_queries(const pb_queries& r, pb_u32 qs, float* units) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < PB_HT / 4; ++i) {
+        const int head = warp + 4 * i;
+        pb_u32 most = 0;
+#pragma unroll
+        for (int j = 0; j < 4 * PB_Q_RUNS; ++j) most = max(most, __float_as_uint(r.x[4 * PB_Q_RUNS * i + j]) & 0x7fffffffu);
+#pragma unroll
+        for (int m = 16; m > 0; m /= 2) most = max(most, __shfl_xor_sync(0xffffffffu, most, m));
+        const bool finite = most < 0x7f800000u, zero = most < 0x0d800000u; // 2^-100
+        pb_u32 power = 127 + 22 + 127 - (most >> 23); // biased
+        if (finite && !zero && __uint_as_float(most) * __uint_as_float(power << 23) > (float)PB_DIGITS) --power;
+        const float to = finite && !zero ? __uint_as_float(power << 23) : 0.0f;
+        if (lane == 0) units[head] = finite ? (zero ? 0.0f : __uint_as_float((254 - power) << 23)) : __int_as_float(0x7fffffff);
+#pragma unroll
+        for (int run = 0; run < PB_Q_RUNS; ++run) {
+            pb_u32 d[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) d[e] = pb_digits(__float2int_rn(r.x[4 * (PB_Q_RUNS * i + run) + e] * to));
+            const pb_u32 low = __byte_perm(d[0], d[1], 0x5140), high = __byte_perm(d[2], d[3], 0x5140); // bytes 0 and 1 of both
+            const pb_u32 tops = __byte_perm(__byte_perm(d[0], d[1], 0x0062), __byte_perm(d[2], d[3], 0x0062), 0x5410);
+            const int at = run * 128 + lane * 4;
+            if (at < PB_Q_HEAD) {
+                const pb_u32 row = qs + head * PB_QROW + at;
+                asm volatile("st.shared.u32 [%0], %1;" :: "r"(row), "r"(__byte_perm(low, high, 0x5410)) : "memory");
+                asm volatile("st.shared.u32 [%0], %1;" :: "r"(row + PB_HT * PB_QROW), "r"(__byte_perm(low, high, 0x7632)) : "memory");
+                asm volatile("st.shared.u32 [%0], %1;" :: "r"(row + 2 * PB_HT * PB_QROW), "r"(tops) : "memory");
+            }
+        }
+    }
+}
+#endif
 
 extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
     const __grid_constant__ pb_tmap map_k, const __grid_constant__ pb_tmap map_v, const float* q, const int* lengths,
     const int* tables, const int4* work, float* out, float* partial, float2* partial_ml, float* logits, float2* norms,
-    int width, int group, int chunks, pb_i64 q_seq, pb_i64 q_head, int longest, float scale2, int* err) {
+    int width, int group, int chunks, pb_i64 q_seq, pb_i64 q_head, int longest, float scale2, int* err,
+    const float* scales_k, const float* scales_v) {
     extern __shared__ char raw[];
     __shared__ pb_u64 bars[2 * PB_RING];
     __shared__ int abort_flag;
     static_assert(sizeof(bars) + sizeof(abort_flag) + 128 <= PB_STATIC, "shared memory that the launch does not count");
     const pb_u32 ring = (pb_smem(raw) + 1023u) & ~1023u;
-    const pb_u32 qs = ring + PB_RING * PB_UNIT;
+    const pb_u32 unit_scales = ring + PB_RING * PB_UNIT; // 256 bytes of each unit, in 8 bits
+    const pb_u32 qs = unit_scales + (PB_ESZ == 1 ? PB_RING * 256 : 0);
     const pb_u32 ps = qs + PB_TERMS * PB_HT * PB_QROW;
     float* wmax = reinterpret_cast<float*>(raw + (ps + PB_TERMS * PB_HT * PB_PROW - pb_smem(raw)));
     float* wsum = wmax + 4 * PB_HT;
+#if PB_ESZ == 1
+    float* wscaled = wsum + 4 * PB_HT; // the warps' maxima of weight x value scale, in log2
+    float* units = wscaled + 4 * PB_HT; // of the row's queries
+#endif
     const pb_u32 full = pb_smem(bars), empty = full + 8 * PB_RING;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
@@ -335,13 +441,16 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                 bad = !pb_wait(empty + 8 * slot, parity, &abort_flag, err, 1 + which);
                 bad = __any_sync(0xffffffffu, bad);
                 if (bad) break;
-                if (lane == 0) pb_mbar_expect_tx(full + 8 * slot, boxes * PB_BOX * 128 * PB_PLANES);
+                if (lane == 0) pb_mbar_expect_tx(full + 8 * slot, boxes * PB_BOX * (128 * PB_PLANES + (PB_ESZ == 1 ? 4 : 0)));
                 __syncwarp();
                 if (lane < boxes) {
                     const pb_u32 dst = ring + slot * PB_UNIT + lane * PB_BOX * 128;
 #pragma unroll
                     for (int c = 0; c < PB_PLANES; ++c)
                         pb_tma_load(dst + c * 8192, which ? &map_v : &map_k, full + 8 * slot, c * PB_CE, y);
+#if PB_ESZ == 1
+                    pb_bulk_load(unit_scales + slot * 256 + lane * PB_BOX * 4, (which ? scales_v : scales_k) + y, full + 8 * slot);
+#endif
                 }
                 ++unit;
                 if (++slot == PB_RING) { slot = 0; parity ^= 1u; }
@@ -405,12 +514,16 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
         if (fresh) {
             begun_at_zero = at.tile == 0;
             // The row's queries, split into terms; zero past the head size.
-            if (PB_Q_EACH > 8 && i) pb_load_queries(ahead, q, at, q_seq, q_head, group);
+            if (PB_Q_EACH8 > 8 && i) pb_load_queries(ahead, q, at, q_seq, q_head, group);
+#if PB_ESZ == 1
+            pb_split_queries(ahead, qs, units);
+#else
 #pragma unroll
             for (int j = 0; j < PB_Q_EACH; ++j) {
                 const int e = threadIdx.x + 128 * j, head = e / PB_Q_HEAD, d = e % PB_Q_HEAD;
                 if (e < PB_HT * PB_Q_HEAD) pb_split_store(qs + head * PB_QROW + d * PB_ESZ, PB_HT * PB_QROW, ahead.x[j]);
             }
+#endif
 #pragma unroll
             for (int n = 0; n < PB_NT; ++n)
 #pragma unroll
@@ -423,7 +536,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                     for (int e = 0; e < 4; ++e) o[a][n][e] = 0.0f;
             if (pb_bar_any(bad)) { bad = true; break; }
         }
-        if (PB_Q_EACH <= 8 && i + 1 < mine.z && next_fresh) pb_load_queries(ahead, q, next, q_seq, q_head, group);
+        if (PB_Q_EACH8 <= 8 && i + 1 < mine.z && next_fresh) pb_load_queries(ahead, q, next, q_seq, q_head, group);
         const int base = at.tile * 64, valid = min(64, at.length - base);
 
         // ---- S^T = K Q^T: this warp's 16 slots x all heads
@@ -436,13 +549,13 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
         bad |= !pb_wait(full + 8 * slot, parity, &abort_flag, err, 3);
         // The first term's sum, the large one, runs in two chains that are
         // added in fp32: half the additions that cut bits in a row.
-        float c[PB_TERMS + 1][PB_NT][4];
+        pb_acc c[PB_TERMS + 1][PB_NT][4];
 #pragma unroll
         for (int x = 0; x < PB_TERMS + 1; ++x)
 #pragma unroll
             for (int n = 0; n < PB_NT; ++n)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) c[x][n][e] = 0.0f;
+                for (int e = 0; e < 4; ++e) c[x][n][e] = 0;
         {
             const int r = 16 * warp + (lane & 15);
             const pb_u32 krow = ring + slot * PB_UNIT + r * 128;
@@ -455,7 +568,17 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                     const int chunk = (2 * k2 + k) * 2; // 16-byte chunk of the row; its plane and place
                     pb_ldm4(a[k], krow + (chunk >> 3) * 8192 + ((((chunk & 7) + (lane >> 4)) ^ (r & 7)) << 4));
                 }
-#if PB_ESZ == 2
+#if PB_ESZ == 1
+#pragma unroll
+                for (int x = 0; x < PB_TERMS; ++x)
+#pragma unroll
+                    for (int n = 0; n < PB_NT; ++n) {
+                        pb_u32 b[4];
+                        pb_ldm4(b, qrow + (x * PB_HT + n * 8) * PB_QROW + k2 * 64);
+                        pb_mma(c[x][n], a[0], b);
+                        pb_mma(c[x][n], a[1], b + 2);
+                    }
+#elif PB_ESZ == 2
 #pragma unroll
                 for (int x = 0; x < PB_TERMS; ++x)
 #pragma unroll
@@ -484,11 +607,20 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
 #endif
             }
         }
+#if PB_ESZ == 1
+        // The scales of this thread's two slots, 0 past the sequence's end.
+        float key_scale[2], value_scale[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+            key_scale[j] = 16 * warp + g + 8 * j < valid ? pb_shared(unit_scales + slot * 256 + (16 * warp + g + 8 * j) * 4) : 0.0f;
+#endif
         __syncwarp();
         // Not after a wait that gave up: the unit's load may still be on its
         // way, and the producer would issue another one into it.
         if (lane == 0 && !bad) pb_mbar_arrive(empty + 8 * slot);
         if (++slot == PB_RING) { slot = 0; parity ^= 1u; }
+
+        auto wait_for_values = [&] { bad |= !pb_wait(full + 8 * slot, parity, &abort_flag, err, 4); };
 
         // Logits in units of log2, -inf past the sequence's end. Thread: slots
         // 16 warp + g and + 8, heads 8 n + 2 t and + 1.
@@ -498,7 +630,9 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int at_slot = 16 * warp + g + (e >> 1) * 8;
-#if PB_TERMS == 3
+#if PB_ESZ == 1
+                const float x = pb_of_digits(c[0][n][e], c[1][n][e], c[2][n][e]) * (units[8 * n + 2 * t + (e & 1)] * scale2) * key_scale[e >> 1];
+#elif PB_TERMS == 3
                 const float x = (c[2][n][e] + c[1][n][e] + (c[0][n][e] + c[3][n][e])) * scale2;
 #else
                 const float x = (c[1][n][e] + (c[0][n][e] + c[2][n][e])) * scale2;
@@ -520,10 +654,47 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
             }
             if (g == 0) *reinterpret_cast<float2*>(wmax + warp * PB_HT + 8 * n + 2 * t) = make_float2(top[n][0], top[n][1]);
         }
+#if PB_ESZ == 1
+        wait_for_values(); // earlier than in other types: their scales go into the weights
+        float scaled[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            value_scale[j] = 16 * warp + g + 8 * j < valid ? pb_shared(unit_scales + slot * 256 + (16 * warp + g + 8 * j) * 4) : 0.0f;
+            scaled[j] = pb_log2(value_scale[j]);
+        }
+#pragma unroll
+        for (int n = 0; n < PB_NT; ++n) {
+            float2 most;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float x = pb_max_nan(s[n][e] + scaled[0], s[n][e + 2] + scaled[1]);
+                x = pb_max_nan(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                x = pb_max_nan(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                x = pb_max_nan(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                if (e) most.y = x; else most.x = x;
+            }
+            if (g == 0) *reinterpret_cast<float2*>(wscaled + warp * PB_HT + 8 * n + 2 * t) = most;
+        }
+#endif
         if (pb_bar_any(bad)) { bad = true; break; }
 
         // ---- weights relative to the running maximum, split into terms
         float corr[PB_NT][2];
+#if PB_ESZ == 1
+        // weight x value scale, in units of which a tile's largest is up to
+        // PB_DIGITS (but for 2^-10 of it, what its logarithms may be off by) and
+        // at least half that; the unit is 2^power of the weights' over that.
+        float power[PB_NT][2];
+#pragma unroll
+        for (int n = 0; n < PB_NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float x = PB_LOWEST;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) x = pb_max_nan(x, wscaled[w * PB_HT + 8 * n + 2 * t + e]);
+                power[n][e] = x;
+            }
+#endif
 #pragma unroll
         for (int n = 0; n < PB_NT; ++n) {
 #pragma unroll
@@ -538,21 +709,37 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                 corr[n][e] = pb_exp2(m[n][e] - now);
                 m[n][e] = now;
                 l[n][e] *= corr[n][e];
+#if PB_ESZ == 1
+                // What lies 2^-100 below the running maximum's weight weighs nothing.
+                power[n][e] = pb_max_nan(ceilf(power[n][e] - now), -100.0f);
+#endif
             }
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const float p = pb_exp2(s[n][e] - m[n][e & 1]);
                 l[n][e & 1] += p;
                 const int at_slot = 16 * warp + g + (e >> 1) * 8, head = 8 * n + 2 * t + (e & 1);
+#if PB_ESZ == 1
+                // As V's fragments count slots: 2 t, 2 t + 1, 2 t + 8, 2 t + 9 side by side.
+                const int place = (at_slot & ~15) + ((at_slot & 7) >> 1) * 4 + ((at_slot >> 3) & 1) * 2 + (at_slot & 1);
+                const pb_u32 digits = pb_digits(__float2int_rn(p * value_scale[e >> 1] * (pb_exp2(-power[n][e & 1]) * PB_WEIGHTS)));
+                const pb_u32 to = ps + head * PB_PROW + place;
+                asm volatile("st.shared.u8 [%0], %1;" :: "r"(to), "r"(digits) : "memory");
+                asm volatile("st.shared.u8 [%0], %1;" :: "r"(to + PB_HT * PB_PROW), "r"(digits >> 8) : "memory");
+                asm volatile("st.shared.u8 [%0], %1;" :: "r"(to + 2 * PB_HT * PB_PROW), "r"(digits >> 16) : "memory");
+#else
 #if PB_ESZ == 2
                 const int place = at_slot;
 #else
                 const int place = (at_slot & ~7) + ((at_slot & 7) >> 1) + (at_slot & 1) * 4; // as V's fragments count slots
 #endif
                 pb_split_store(ps + head * PB_PROW + place * PB_ESZ, PB_HT * PB_PROW, p);
+#endif
             }
         }
-        bad |= !pb_wait(full + 8 * slot, parity, &abort_flag, err, 4);
+#if PB_ESZ != 1
+        wait_for_values();
+#endif
         if (pb_bar_any(bad)) { bad = true; break; }
 
         // ---- O^T += V^T P^T: this warp's channels x all heads. The tile's sum
@@ -561,15 +748,17 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
         {
             const pb_u32 vunit = ring + slot * PB_UNIT;
             const pb_u32 prow = ps + (lane & 7) * PB_PROW + (lane >> 3) * 16;
-            float d[PB_MTW][PB_NT][2][4];
+            pb_acc d[PB_MTW][PB_NT][PB_ESZ == 1 ? 3 : 2][4];
 #pragma unroll
             for (int a = 0; a < PB_MTW; ++a)
 #pragma unroll
                 for (int n = 0; n < PB_NT; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) d[a][n][0][e] = d[a][n][1][e] = 0.0f;
+                    for (int x = 0; x < (PB_ESZ == 1 ? 3 : 2); ++x)
 #pragma unroll
-            for (int k2 = 0; k2 < 2 * PB_ESZ / 2; ++k2) { // two k-steps at a time
+                        for (int e = 0; e < 4; ++e) d[a][n][x][e] = 0;
+#pragma unroll
+            for (int k2 = 0; k2 < PB_ESZ; ++k2) { // two k-steps at a time
                 pb_u32 b[PB_TERMS][PB_NT][4];
 #pragma unroll
                 for (int x = 0; x < PB_TERMS; ++x)
@@ -582,7 +771,23 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
                             pb_u32 v[4];
-#if PB_ESZ == 2
+#if PB_ESZ == 1
+                            // Transposed as pairs of bytes: a register has channels 2 g and
+                            // 2 g + 1 of two slots; rows g and g + 8 of the product are
+                            // those two, and its columns the slots as they come. What
+                            // lies past the end is finite, and its weight 0.
+                            const int r = (2 * k2 + k) * 32 + lane;
+                            pb_u32 pair[4];
+                            pb_ldm4t(pair, vunit + (mt >> 3) * 8192 + r * 128 + (((mt & 7) ^ (r & 7)) << 4));
+                            v[0] = __byte_perm(pair[0], pair[1], 0x6420);
+                            v[1] = __byte_perm(pair[0], pair[1], 0x7531);
+                            v[2] = __byte_perm(pair[2], pair[3], 0x6420);
+                            v[3] = __byte_perm(pair[2], pair[3], 0x7531);
+#pragma unroll
+                            for (int n = 0; n < PB_NT; ++n)
+#pragma unroll
+                                for (int x = 0; x < 3; ++x) pb_mma(d[a][n][x], v, b[x][n] + 2 * k);
+#elif PB_ESZ == 2
                             const int first = (2 * k2 + k) * 16;
                             const int r = first + (lane >> 4) * 8 + (lane & 7);
                             const int chunk = mt * 2 + ((lane >> 3) & 1);
@@ -632,7 +837,12 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                 for (int n = 0; n < PB_NT; ++n)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
+#if PB_ESZ == 1
+                        o[a][n][e] = fmaf(pb_of_digits(d[a][n][0][e], d[a][n][1][e], d[a][n][2][e]),
+                                          pb_exp2(power[n][e & 1]) * (1.0f / PB_WEIGHTS), o[a][n][e] * corr[n][e & 1]);
+#else
                         o[a][n][e] = fmaf(o[a][n][e], corr[n][e & 1], d[a][n][1][e] + d[a][n][0][e]);
+#endif
         }
         __syncwarp();
         if (lane == 0) pb_mbar_arrive(empty + 8 * slot);
@@ -675,9 +885,14 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                     const float inv = whole ? 1.0f / sum : 1.0f;
 #pragma unroll
                     for (int a = 0; a < PB_MTW; ++a) {
+#if PB_ESZ == 1 // head sizes are whole tiles of channels
+                        const int ch = (warp + 4 * a) * 16 + 2 * g;
+                        if (ch < PB_D) *reinterpret_cast<float2*>(to + ch) = make_float2(o[a][n][e] * inv, o[a][n][e + 2] * inv);
+#else
                         const int ch = (warp + 4 * a) * 16 + g;
                         if (ch < PB_D) to[ch] = o[a][n][e] * inv;
                         if (ch + 8 < PB_D) to[ch + 8] = o[a][n][e + 2] * inv;
+#endif
                     }
                     if (warp == 0 && g == 0) {
                         if (!whole) partial_ml[part * PB_HT + head] = make_float2(m[n][e], sum);
@@ -900,7 +1115,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             f.heads = static_cast<int>(c.heads);
             f.dim = static_cast<int>(c.dim);
             f.page = static_cast<int>(c.page_size);
-            f.bf16 = c.type == cache_type::bf16;
+            f.type = c.type;
             f.tiles8 = group > 8 ? 2 : 1;
             if (f.ring() < 3) f.tiles8 = 1;
             return f;
@@ -910,7 +1125,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         const char kFinish[] = "pb_paged_finish";
 
         op_kernel& kernel_of(const char* name, const form& f, uint32_t smem) {
-            const op_key key{reinterpret_cast<int64_t>(name), f.heads, f.dim, f.page, f.bf16, f.scored, f.tiles8, f.join_threads, f.stall};
+            const op_key key{reinterpret_cast<int64_t>(name), f.heads, f.dim, f.page, static_cast<int64_t>(f.type), f.scored, f.tiles8, f.join_threads, f.stall};
             return op_kernel_for(key, [&](op_kernel& k) {
                 k.name = name;
                 k.source = std::string{kernel_prelude()} + defines(f) + device_source();
@@ -1076,9 +1291,10 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         if (attention != nullptr) {
             (void)attention->on(device);
             check(pbrt_error_word(device, &err));
+            uint64_t scales_k = address(c.k) + static_cast<uint64_t>(c.values_bytes()), scales_v = address(c.v) + static_cast<uint64_t>(c.values_bytes());
             void* params[] = {&c.map_k, &c.map_v, &x.ptr, &batch.lengths_at, &batch.tables_at, &work,
                               &out.ptr, &partial, &ml, &logits, &norms, &width, &group, &chunks,
-                              &x.strides[0], &x.strides[1], &longest32, &scale2, &err};
+                              &x.strides[0], &x.strides[1], &longest32, &scale2, &err, &scales_k, &scales_v};
             std::scoped_lock lock{c.order};
             order_read(*cuda_jit::buffer_access::state(c.k), stream);
             order_read(*cuda_jit::buffer_access::state(c.v), stream);
@@ -1163,15 +1379,16 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         for (const auto& [dim, width, tiles8, page] :
              {std::array<int, 4>{128, 2, 1, 64}, std::array<int, 4>{64, 2, 1, 16}, std::array<int, 4>{64, 4, 1, 16},
               std::array<int, 4>{128, 4, 1, 8}, std::array<int, 4>{256, 4, 1, 256}, std::array<int, 4>{256, 2, 2, 32},
-              std::array<int, 4>{72, 2, 2, 32}, std::array<int, 4>{8, 4, 2, 32}}) {
+              std::array<int, 4>{72, 2, 2, 32}, std::array<int, 4>{8, 4, 2, 32}, std::array<int, 4>{128, 1, 1, 64},
+              std::array<int, 4>{80, 1, 2, 8}, std::array<int, 4>{256, 1, 2, 256}, std::array<int, 4>{16, 1, 1, 16}}) {
             form f;
             f.heads = 8;
             f.dim = dim;
-            f.bf16 = width == 2;
+            f.type = width == 1 ? cache_type::i8 : (width == 2 ? cache_type::bf16 : cache_type::f32);
             f.tiles8 = tiles8;
             f.page = page;
             f.scored = true;
-            out.emplace_back("pb_paged_attention_" + std::to_string(dim) + (f.bf16 ? "_bf16_" : "_f32_") + std::to_string(8 * tiles8),
+            out.emplace_back("pb_paged_attention_" + std::to_string(dim) + (width == 1 ? "_i8_" : (width == 2 ? "_bf16_" : "_f32_")) + std::to_string(8 * tiles8),
                              std::string{kernel_prelude()} + defines(f) + device_source());
         }
     }

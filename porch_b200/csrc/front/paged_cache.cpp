@@ -43,6 +43,77 @@ static __device__ __forceinline__ pb_u32 pb_bf16_pair(float lo, float hi) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
+#if PB_I8
+// Eight bits: a row is kept as codes -127 to 127 and a scale, its largest size /
+// 127. A code is x / scale rounded to nearest, ties to even, by real arithmetic:
+// 127 x / top in float32 is off by less than 2^-15 of a code, so within 2^-14 of
+// halfway between two of them 127 |x| and (n + 1/2) top are compared in 64 bits,
+// where both are exact. A row with a value that is not finite is kept as NaN
+// (by its scale), one that nowhere reaches 2^-96 as zeros. Eight lanes: one row,
+// four channels at a time. Bound by HBM: 4 B read and 1 B written per value.
+#define PB_ITEMS ((PB_D + 31) / 32)
+static __device__ __forceinline__ int pb_code(float x, float inv, float top) {
+    const float t = fabsf(x) * inv, low = floorf(t), part = t - low;
+    float n = part > 0.5f ? low + 1.0f : low;
+    if (fabsf(part - 0.5f) < 6.103515625e-05f) {
+        const double a = 127.0 * (double)fabsf(x), b = ((double)low + 0.5) * (double)top;
+        n = a > b || (a == b && ((int)low & 1)) ? low + 1.0f : low;
+    }
+    return x < 0.0f ? -(int)n : (int)n;
+}
+extern "C" __global__ void __launch_bounds__(256) pb_cache_append(
+    const float* k, const float* v, char* pk, char* pv, const pb_i64* rows, pb_i64 tokens,
+    pb_i64 kt, pb_i64 kh, pb_i64 vt, pb_i64 vh, pb_i64 scales) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int lane = threadIdx.x & 7;
+    const pb_i64 want = (pb_i64)blockIdx.x * 32 + (threadIdx.x >> 3), n = tokens * PB_H * 2;
+    const pb_i64 id = min(want, n - 1);
+    const int which = (int)(id & 1), h = (int)(id / 2 % PB_H);
+    const pb_i64 t = id / 2 / PB_H;
+    const float* src = which ? v + t * vt + h * vh : k + t * kt + h * kh;
+    float x[PB_ITEMS][4];
+#pragma unroll
+    for (int i = 0; i < PB_ITEMS; ++i) {
+        const int c = (i * 8 + lane) * 4;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[i][e] = 0.0f;
+        if (c >= PB_D) continue;
+#if PB_WIDE
+        const float4 a = pb_ld4(src + c);
+        x[i][0] = a.x; x[i][1] = a.y; x[i][2] = a.z; x[i][3] = a.w;
+#else
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[i][e] = __ldg(src + c + e);
+#endif
+    }
+    const pb_i64 to = (rows[t] / PB_PS * PB_H + h) * PB_PS + rows[t] % PB_PS;
+    // As integers, sizes order as they do as numbers, infinity and NaN above all.
+    pb_u32 most = 0;
+#pragma unroll
+    for (int i = 0; i < PB_ITEMS; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = max(most, __float_as_uint(x[i][e]) & 0x7fffffffu);
+#pragma unroll
+    for (int m = 4; m > 0; m /= 2) most = max(most, __shfl_xor_sync(0xffffffffu, most, m));
+    const float top = __uint_as_float(most);
+    const bool finite = most < 0x7f800000u, kept = finite && top >= 1.262177448e-29f; // 2^-96
+    const float inv = kept ? 127.0f / top : 0.0f;
+    if (want >= n) return;
+    char* pool = which ? pv : pk;
+#pragma unroll
+    for (int i = 0; i < PB_ITEMS; ++i) {
+        const int c = (i * 8 + lane) * 4;
+        if (c >= PB_D) continue;
+        pb_u32 codes = 0;
+        if (kept)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) codes |= ((pb_u32)pb_code(x[i][e], inv, top) & 255u) << (8 * e);
+        *reinterpret_cast<pb_u32*>(pool + to * PB_D + c) = codes;
+    }
+    if (lane == 0)
+        *reinterpret_cast<float*>(pool + scales + to * 4) = kept ? top / 127.0f : (finite ? 0.0f : __int_as_float(0x7fffffff));
+}
+#else
 extern "C" __global__ void __launch_bounds__(256) pb_cache_append(
     const float* k, const float* v, char* pk, char* pv, const pb_i64* rows, pb_i64 tokens,
     pb_i64 kt, pb_i64 kh, pb_i64 vt, pb_i64 vh) {
@@ -74,6 +145,68 @@ extern "C" __global__ void __launch_bounds__(256) pb_cache_append(
         *reinterpret_cast<float4*>(dst + to * 4) = make_float4(x[0], x[1], x[2], x[3]);
         *reinterpret_cast<float4*>(dst + to * 4 + 16) = make_float4(x[4], x[5], x[6], x[7]);
 #endif
+    }
+}
+#endif
+)PB";
+        }
+
+        const char* read_source() {
+            return R"PB(
+typedef long long pb_i64;
+// Block: PB_TOKENS slots, keys and values of every head, as float32 (which holds
+// a bfloat16 value, and 8 bits times their scale rounded once). Its first threads
+// find the sequence and row of one slot each; the rest is copying, four values a
+// thread and PB_EACH of those on the way at once. Bound by HBM.
+#define PB_QUADS (PB_TOKENS * PB_H * (PB_D / 4))
+extern "C" __global__ void __launch_bounds__(256) pb_cache_read(
+    const char* pk, const char* pv, const int* tables, const pb_i64* starts, float* ok, float* ov, int sequences, int width,
+    pb_i64 scales) {
+    __shared__ pb_i64 rows[PB_TOKENS]; // of head 0
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const pb_i64 first = (pb_i64)blockIdx.x * PB_TOKENS;
+    const int n = (int)min((pb_i64)PB_TOKENS, starts[sequences] - first);
+    if (threadIdx.x < n) {
+        const pb_i64 t = first + threadIdx.x;
+        int low = 0, high = sequences - 1; // the last sequence that starts at or before it, and is not empty
+        while (low < high) {
+            const int middle = (low + high + 1) / 2;
+            if (starts[middle] <= t) low = middle; else high = middle - 1;
+        }
+        const int slot = (int)(t - starts[low]);
+        rows[threadIdx.x] = (pb_i64)tables[(pb_i64)low * width + slot / PB_PS] * PB_H * PB_PS + slot % PB_PS;
+    }
+    __syncthreads();
+    const int quads = n * PB_H * (PB_D / 4);
+    for (int base = threadIdx.x; base < 2 * quads; base += 256 * PB_EACH) {
+        float4 x[PB_EACH];
+#pragma unroll
+        for (int j = 0; j < PB_EACH; ++j) {
+            const int id = base + j * 256;
+            if (id >= 2 * quads) break;
+            const int q = id < quads ? id : id - quads, c = q % (PB_D / 4), h = q / (PB_D / 4) % PB_H;
+            const char* pool = id < quads ? pk : pv;
+            const pb_i64 row = rows[q / (PB_D / 4 * PB_H)] + h * PB_PS;
+#if PB_I8
+            const pb_u32 w = __ldcs(reinterpret_cast<const pb_u32*>(pool + row * PB_D + 4 * c));
+            const float s = __ldg(reinterpret_cast<const float*>(pool + scales) + row);
+            x[j] = make_float4((float)(signed char)(w & 255u) * s, (float)(signed char)(w >> 8 & 255u) * s,
+                               (float)(signed char)(w >> 16 & 255u) * s, (float)(signed char)(w >> 24) * s);
+#elif PB_BF16
+            const uint2 w = __ldcs(reinterpret_cast<const uint2*>(pool + (row * PB_D + 4 * c) * 2));
+            x[j] = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u),
+                               __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+#else
+            x[j] = __ldcs(reinterpret_cast<const float4*>(pool + (row * PB_D + 4 * c) * 4));
+#endif
+        }
+#pragma unroll
+        for (int j = 0; j < PB_EACH; ++j) {
+            const int id = base + j * 256;
+            if (id >= 2 * quads) break;
+            const int q = id < quads ? id : id - quads;
+            __stcs(reinterpret_cast<float4*>((id < quads ? ok : ov) + first * PB_H * PB_D) + q, x[j]);
+        }
     }
 }
 )PB";
@@ -200,7 +333,8 @@ static __device__ __forceinline__ pb_pairs pb_list(const int* holes, const int* 
 // warp, all loads before the first store, so that it has as many bytes on the
 // way as PB_MOVES rows. Sources lie at or past the budget, destinations below.
 static __device__ __forceinline__ void pb_move(const pb_pairs& p, const pb_row& r, char* pk, char* pv, const int* tables,
-                                               float* out_scores, float* out_places, pb_i64 row, int width, int budget) {
+                                               float* out_scores, float* out_places, pb_i64 row, int width, int budget,
+                                               pb_i64 scales) {
     const int lane = threadIdx.x & 31, h = (int)(row % PB_H);
     const int* table = tables + row / PB_H * width;
     // Lane m finds where pair m's rows lie; all lanes move them.
@@ -221,6 +355,14 @@ static __device__ __forceinline__ void pb_move(const pb_pairs& p, const pb_row& 
                 v[m][c] = __ldcs(reinterpret_cast<const uint4*>((at < PB_ROW ? pk + at : pv + at - PB_ROW) + a));
         }
     }
+#if PB_I8
+    if (lane < p.count) { // the rows' scales go with them
+        const float* sk = reinterpret_cast<const float*>(pk + scales), *sv = reinterpret_cast<const float*>(pv + scales);
+        const float a = sk[from / PB_ROW], b = sv[from / PB_ROW];
+        reinterpret_cast<float*>(pk + scales)[to / PB_ROW] = a;
+        reinterpret_cast<float*>(pv + scales)[to / PB_ROW] = b;
+    }
+#endif
     if (lane < p.count) pb_keep(r, out_scores, out_places, row * budget + p.to, p.from);
 #pragma unroll
     for (int m = 0; m < PB_MOVES; ++m) {
@@ -291,7 +433,7 @@ static __device__ __forceinline__ int2 pb_before(const int* totals, pb_u32 rank,
 extern "C" __global__ void __launch_bounds__(PB_THREADS, PB_THREADS < 1024 ? 2 : 1) pb_evict_select(
     const float* scores, const float* places, const int* lengths, const int* newest, float* out_scores,
     float* out_places, int* holes, int* lates, int* counts, pb_i64 ns, pb_i64 np, int budget, int recent, int sinks,
-    int pairs, char* pk, char* pv, const int* tables, int width, int fused) {
+    int pairs, char* pk, char* pv, const int* tables, int width, int fused, pb_i64 scales) {
     constexpr int threads = PB_THREADS, run = PB_THREADS * PB_KPT, stride = PB_KPT | 1;
     extern __shared__ pb_u32 keys[];
     __shared__ int hist[2][256], bins[256], chosen[3], totals[4];
@@ -423,7 +565,7 @@ extern "C" __global__ void __launch_bounds__(PB_THREADS, PB_THREADS < 1024 ? 2 :
         for (int g = rank * (threads / 32) + (threadIdx.x >> 5); g < groups; g += PB_CLUSTER * (threads / 32)) {
             const pb_pairs p = pb_list(holes, lates, counts, row, g, pairs);
             if (p.count <= 0) break;
-            pb_move(p, r, pk, pv, tables, out_scores, out_places, row, width, budget);
+            pb_move(p, r, pk, pv, tables, out_scores, out_places, row, width, budget, scales);
         }
     }
 }
@@ -599,14 +741,14 @@ extern "C" __global__ void __launch_bounds__(1024) pb_evict_select_long(
 extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
     char* pk, char* pv, const int* tables, const float* scores, const float* places, const int* lengths,
     const int* newest, float* out_scores, float* out_places, const int* holes, const int* lates, const int* counts,
-    pb_i64 ns, pb_i64 np, int width, int budget, int pairs, pb_u32 blocks) {
+    pb_i64 ns, pb_i64 np, int width, int budget, int pairs, pb_u32 blocks, pb_i64 scales) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     // Blocks of 8 warps, `blocks` of them for each row.
     const pb_i64 row = blockIdx.x / blocks;
     const pb_pairs p = pb_list(holes, lates, counts, row, (blockIdx.x % blocks) * 8 + (threadIdx.x >> 5), pairs);
     if (p.count <= 0) return;
     const pb_row r = pb_row_of(scores, places, lengths, newest, ns, np, 0, 0, row);
-    pb_move(p, r, pk, pv, tables, out_scores, out_places, row, width, budget);
+    pb_move(p, r, pk, pv, tables, out_scores, out_places, row, width, budget, scales);
 }
 #endif
 )PB";
@@ -653,7 +795,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
             std::ostringstream os;
             os << "#define PB_H " << c.heads << "\n#define PB_D " << c.dim << "\n#define PB_PS " << c.page_size
                << "\n#define PB_ROW " << c.dim * c.width() << "\n#define PB_BF16 " << (c.type == cache_type::bf16 ? 1 : 0)
-               << "\n#define PB_WIDE " << (wide ? 1 : 0) << "\n#define PB_MOVES " << moves_of(c)
+               << "\n#define PB_I8 " << (c.type == cache_type::i8 ? 1 : 0) << "\n#define PB_WIDE " << (wide ? 1 : 0) << "\n#define PB_MOVES " << moves_of(c)
                << "\n#define PB_CHUNKS " << (2 * c.dim * c.width() + 511) / 512 << "\n";
             if (f.cluster != 0)
                 os << "#define PB_CLUSTER " << f.cluster << "\n#define PB_THREADS " << f.threads << "\n#define PB_KPT "
@@ -661,7 +803,16 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
             return os.str();
         }
 
+        // Slots of a block that reads back: about 64 values of keys and of values a thread.
+        int read_tokens(const kv_cache& c) {
+            return static_cast<int>(std::clamp<int64_t>(16384 / (c.heads * c.dim), 1, 256));
+        }
+        std::string read_defines(const kv_cache& c) {
+            return "#define PB_TOKENS " + std::to_string(read_tokens(c)) + "\n#define PB_EACH 8\n";
+        }
+
         const char kAppend[] = "pb_cache_append";
+        const char kRead[] = "pb_cache_read";
         const char kSelect[] = "pb_evict_select";
         const char kSelectLong[] = "pb_evict_select_long";
         const char kMove[] = "pb_evict_move";
@@ -671,8 +822,8 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
                              wide, f.cluster, f.threads, f.per_thread, f.held};
             return op_kernel_for(key, [&](op_kernel& k) {
                 k.name = name;
-                k.source = std::string{kernel_prelude()} + defines(c, wide, f) +
-                           (name == kAppend ? append_source() : evict_source());
+                k.source = std::string{kernel_prelude()} + defines(c, wide, f);
+                k.source += name == kAppend ? append_source() : (name == kRead ? read_defines(c) + read_source() : evict_source());
                 k.smem = f.smem();
             });
         }
@@ -681,12 +832,14 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
 
     std::shared_ptr<kv_cache> make_cache(int64_t pages, int64_t page_size, int64_t heads, int64_t dim,
                                          cache_type type, int device) {
-        expect(type == cache_type::f32 || type == cache_type::bf16, "cache: type must be float32 or bfloat16");
+        expect(type == cache_type::f32 || type == cache_type::bf16 || type == cache_type::i8,
+               "cache: type must be float32, bfloat16 or int8");
         expect(pages >= 1 && pages <= (int64_t{1} << 30), "cache: pages must be 1 to 2^30");
         expect(page_size >= 8 && page_size <= 256 && (page_size & (page_size - 1)) == 0,
                "cache: page_size must be a power of two from 8 to 256");
         expect(heads >= 1 && heads <= 1024, "cache: kv_heads must be 1 to 1024");
         expect(dim >= 8 && dim <= 256 && dim % 8 == 0, "cache: head_dim must be a multiple of 8 up to 256");
+        expect(type != cache_type::i8 || dim % 16 == 0, "cache: head_dim must be a multiple of 16 in int8"); // rows start on 16 bytes
         // Rows are counted in 31 bits by the tile loads.
         expect(pages * heads * page_size < (int64_t{1} << 31), "cache: pages x kv_heads x page_size must be below 2^31");
         int ndev = 0;
@@ -698,7 +851,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
         c->dim = dim;
         c->type = type;
         c->device = checked_ordinal(device, ndev);
-        const size_t bytes = static_cast<size_t>(pages * heads * page_size * dim) * static_cast<size_t>(c->width());
+        const size_t bytes = static_cast<size_t>(c->values_bytes() + (type == cache_type::i8 ? pages * heads * page_size * 4 : 0));
         auto stream = current_stream(c->device);
         c->k = allocate(c->device, bytes, stream);
         c->v = allocate(c->device, bytes, stream);
@@ -706,10 +859,10 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
         const uint64_t strides[1] = {static_cast<uint64_t>(dim * c->width())};
         const uint32_t box[2] = {static_cast<uint32_t>(128 / c->width()), static_cast<uint32_t>(std::min<int64_t>(64, page_size))};
         const uint32_t ones[2] = {1, 1};
-        // bfloat16 or float32, 128-byte swizzle, 256-byte L2 promotion, zeros past the head size.
+        // Bytes, bfloat16 or float32, 128-byte swizzle, 256-byte L2 promotion, zeros past the head size.
+        const int element = type == cache_type::i8 ? 0 : (type == cache_type::bf16 ? 9 : 7);
         for (auto [m, p] : {std::pair{&c->map_k, &c->k}, std::pair{&c->map_v, &c->v}})
-            check(pbrt_tensor_map_encode_tiled(m->bytes, type == cache_type::bf16 ? 9 : 7, 2, address(*p), dims, strides,
-                                               box, ones, 0, 3, 3, 0));
+            check(pbrt_tensor_map_encode_tiled(m->bytes, element, 2, address(*p), dims, strides, box, ones, 0, 3, 3, 0));
         return c;
     }
 
@@ -730,7 +883,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
         b->cache = cache;
         b->lengths.assign(lengths, lengths + sequences);
         std::vector<char> used(static_cast<size_t>(cache->pages), 0);
-        std::vector<int64_t> rows;
+        std::vector<int64_t> rows, starts{0};
         for (size_t s = 0; s < sequences; ++s) {
             const int64_t n = lengths[s];
             const std::string at = "cache batch: sequence " + std::to_string(s) + ": ";
@@ -755,6 +908,8 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
             expect(newest == nullptr || n == 0 || last >= n - 1, at + "newest position must be at least its length - 1");
             b->newest.push_back(last);
             b->longest = std::max(b->longest, n);
+            b->slots += n;
+            starts.push_back(b->slots);
             b->table_width = std::max(b->table_width, pages);
         }
         if (b->shared_pages) {
@@ -764,9 +919,9 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
         b->tokens = static_cast<int64_t>(rows.size());
         b->table_width = std::max<int64_t>(1, b->table_width);
 
-        // One upload: lengths, newest, tables, rows (8-byte aligned).
+        // One upload: lengths, newest, tables, rows and starts (8-byte aligned).
         std::vector<int32_t> host;
-        host.reserve(sequences * (2 + static_cast<size_t>(b->table_width)) + 2 * rows.size() + 1);
+        host.reserve(sequences * (2 + static_cast<size_t>(b->table_width)) + 2 * (rows.size() + starts.size()) + 1);
         for (int64_t n : b->lengths) host.push_back(static_cast<int32_t>(n));
         for (int64_t n : b->newest) host.push_back(static_cast<int32_t>(n));
         const size_t tables_from = host.size();
@@ -775,10 +930,11 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
                 host.push_back(j * page < lengths[s] ? tables[s * width + static_cast<size_t>(j)] : 0);
         if (host.size() % 2 != 0) host.push_back(0);
         const size_t rows_from = host.size();
-        for (int64_t r : rows) {
-            host.push_back(static_cast<int32_t>(static_cast<uint64_t>(r) & 0xffffffffu));
-            host.push_back(static_cast<int32_t>(static_cast<uint64_t>(r) >> 32));
-        }
+        for (const auto* list : {&rows, &starts})
+            for (int64_t r : *list) {
+                host.push_back(static_cast<int32_t>(static_cast<uint64_t>(r) & 0xffffffffu));
+                host.push_back(static_cast<int32_t>(static_cast<uint64_t>(r) >> 32));
+            }
         // On the upload stream, so that waiting for the copy does not wait
         // for the step that is still running.
         auto stream = upload_stream(cache->device);
@@ -790,6 +946,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
         b->newest_at = at + sequences * sizeof(int32_t);
         b->tables_at = at + tables_from * sizeof(int32_t);
         b->rows_at = at + rows_from * sizeof(int32_t);
+        b->starts_at = b->rows_at + rows.size() * sizeof(int64_t);
         b->plans->hint = cache->hint;
         prepare_plan(*b);
         return b;
@@ -819,15 +976,40 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
         op_kernel& kernel = kernel_of(kAppend, c, wide);
         (void)kernel.on(device);
         uint64_t pk = address(c.k), pv = address(c.v);
-        const int64_t blocks = (batch.tokens * c.heads * (c.dim / 8) + 255) / 256;
+        const int64_t threads = batch.tokens * c.heads * (c.type == cache_type::i8 ? 16 : c.dim / 8);
+        const int64_t blocks = (threads + 255) / 256;
         expect(blocks <= 0x7fffffff, "cache_append: too many new tokens");
+        int64_t scales = c.values_bytes();
         void* params[] = {&xk.ptr,        &xv.ptr,        &pk,            &pv,            &batch.rows_at,
-                          &batch.tokens,  &xk.strides[0], &xk.strides[1], &xv.strides[0], &xv.strides[1]};
+                          &batch.tokens,  &xk.strides[0], &xk.strides[1], &xv.strides[0], &xv.strides[1], &scales};
         order_read(*cuda_jit::buffer_access::state(batch.data), stream);
         std::scoped_lock lock{c.order};
         order_write(*cuda_jit::buffer_access::state(c.k), stream);
         order_write(*cuda_jit::buffer_access::state(c.v), stream);
         op_launch(kernel, device, stream, {static_cast<uint32_t>(blocks), 1, 1}, 256, params);
+    }
+
+    std::array<tensor, 2> cache_read(kv_batch& batch) {
+        kv_cache& c = *batch.cache;
+        auto stream = current_stream(c.device);
+        const std::vector<index_t> shape{batch.slots, c.heads, c.dim};
+        op_result k = new_result(shape, c.device, stream), v = new_result(shape, c.device, stream);
+        if (batch.slots != 0) {
+            op_kernel& kernel = kernel_of(kRead, c);
+            (void)kernel.on(c.device);
+            const int64_t per = read_tokens(c), blocks = (batch.slots + per - 1) / per;
+            expect(blocks <= 0x7fffffff, "cache_read: too many slots");
+            uint64_t pk = address(c.k), pv = address(c.v);
+            int sequences = static_cast<int>(batch.sequences()), width = static_cast<int>(batch.table_width);
+            int64_t scales = c.values_bytes();
+            void* params[] = {&pk, &pv, &batch.tables_at, &batch.starts_at, &k.ptr, &v.ptr, &sequences, &width, &scales};
+            order_read(*cuda_jit::buffer_access::state(batch.data), stream);
+            std::scoped_lock lock{c.order};
+            order_read(*cuda_jit::buffer_access::state(c.k), stream);
+            order_read(*cuda_jit::buffer_access::state(c.v), stream);
+            op_launch(kernel, c.device, stream, {static_cast<uint32_t>(blocks), 1, 1}, 256, params);
+        }
+        return {finish(std::move(k)), finish(std::move(v))};
     }
 
     std::array<tensor, 2> cache_evict(kv_batch& batch, const tensor& scores, const tensor* positions,
@@ -863,7 +1045,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
         order_read(*cuda_jit::buffer_access::state(batch.data), stream);
         int b = static_cast<int>(budget), rc = static_cast<int>(recent), sk = static_cast<int>(sinks);
         int width = static_cast<int>(batch.table_width);
-        int64_t nsv = ns, npv = np;
+        int64_t nsv = ns, npv = np, scales = c.values_bytes();
         select_shape f = shape_for(batch.longest, rows, sm_count(device));
         const bool moves = batch.longest > budget;
         uint64_t pk = address(c.k), pv = address(c.v);
@@ -877,10 +1059,10 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
         if (move != nullptr) (void)move->on(device);
         void* sparams[] = {&xs.ptr, &xp.ptr, &batch.lengths_at, &batch.newest_at, &os.ptr, &op.ptr, &holes,
                            &lates,  &counts, &nsv,              &npv,             &b,      &rc,     &sk,
-                           &pairs,  &pk,     &pv,               &batch.tables_at, &width,  &fused};
+                           &pairs,  &pk,     &pv,               &batch.tables_at, &width,  &fused, &scales};
         void* mparams[] = {&pk,     &pv,    &batch.tables_at, &xs.ptr, &xp.ptr, &batch.lengths_at, &batch.newest_at,
                            &os.ptr, &op.ptr, &holes,          &lates,  &counts, &nsv,              &npv,
-                           &width, &b,      &pairs,           &per_row};
+                           &width, &b,      &pairs,           &per_row, &scales};
         {
             std::scoped_lock lock{c.order};
             if (moves) {
@@ -900,9 +1082,10 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
         c.heads = 5;
         c.dim = 80;
         c.page_size = 8;
-        for (const auto type : {cache_type::f32, cache_type::bf16}) {
+        for (const auto type : {cache_type::f32, cache_type::bf16, cache_type::i8}) {
             c.type = type;
-            const std::string tag = type == cache_type::bf16 ? "_bf16" : "_f32", p = kernel_prelude();
+            const std::string tag = type == cache_type::i8 ? "_i8" : (type == cache_type::bf16 ? "_bf16" : "_f32"), p = kernel_prelude();
+            out.emplace_back("pb_cache_read" + tag, p + defines(c, true) + read_defines(c) + read_source());
             out.emplace_back("pb_cache_append" + tag, p + defines(c, type == cache_type::bf16) + append_source());
             out.emplace_back("pb_evict" + tag, p + defines(c, true) + evict_source());
             out.emplace_back("pb_evict_select" + tag, p + defines(c, true, type == cache_type::bf16 ? select_shape{8, 1024, 48} : select_shape{1, 256, 4}) + evict_source());

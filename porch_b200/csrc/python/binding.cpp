@@ -27,6 +27,7 @@ namespace {
     X(pb_token_logprobs_backward)                                                                            \
     X(pb_paged_attention)                                                                                    \
     X(pb_paged_attention_scored)                                                                             \
+    X(pb_kv_read)                                                                                            \
     X(pb_kv_evict)
 #define PB_POINTER(name) decltype(&::name) name = nullptr;
     struct {
@@ -302,6 +303,15 @@ namespace {
         return wrap_all(out);
     }
 
+    // (batch)
+    PyObject* kv_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+        int64_t batch = 0;
+        std::array<pb_tensor*, 2> out{};
+        if (!expect(n, 1) || !integer(args[0], batch)) return nullptr;
+        if (!call([&] { return native.pb_kv_read(reinterpret_cast<pb_kv_batch*>(batch), &out[0], &out[1]); })) return nullptr;
+        return wrap_all(out);
+    }
+
     // (batch, scores, positions or None, budget, recent, sinks)
     PyObject* kv_evict(PyObject*, PyObject* const* args, Py_ssize_t n) {
         tensors scores, places;
@@ -365,6 +375,7 @@ namespace {
         method("token_logprobs_backward", token_logprobs_backward),
         method("paged_attention", paged_attention),
         method("paged_attention_scored", paged_attention_scored),
+        method("kv_read", kv_read),
         method("kv_evict", kv_evict),
         method("bind", bind),
         method("connect", connect),

@@ -100,6 +100,10 @@ def paged_attention_scored(q, batch, scores, scale):
     return _call("pb_paged_attention_scored", 2, q._h, batch, scores[0]._h if scores else None, scale)
 
 
+def kv_read(batch):
+    return _call("pb_kv_read", 2, batch)
+
+
 def kv_evict(batch, scores, positions, budget, recent, sinks):
     scores, *positions = _tensors([scores] if positions is None else [scores, positions])
     sizes = [operator.index(x) for x in (budget, recent, sinks)]
