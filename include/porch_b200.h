@@ -344,6 +344,15 @@ int pb_kv_cache_scales(const pb_kv_cache* cache, uint64_t* keys, uint64_t* value
 int pb_kv_batch_create(pb_kv_cache* cache, const int32_t* tables, size_t sequences, size_t width,
                        const int64_t* lengths, const int64_t* appended, const int64_t* newest,
                        pb_kv_batch** out);
+/* The same for sequences that share prefixes: the first prefix[s] slots (whole
+ * pages, 0 for none, none of them new) of sequences next to each other that
+ * begin on the same page and have the same prefix[s] are one prefix, which
+ * pb_paged_attention then works through once for all of them. Their tables name
+ * the same pages for it. Without `appended` a sequence that ends with its prefix
+ * has no new token. NULL: as pb_kv_batch_create. */
+int pb_kv_batch_create_shared(pb_kv_cache* cache, const int32_t* tables, size_t sequences, size_t width,
+                              const int64_t* lengths, const int64_t* appended, const int64_t* newest,
+                              const int64_t* prefix, pb_kv_batch** out);
 int pb_kv_batch_on(const pb_kv_batch* batch, pb_kv_cache* cache, pb_kv_batch** out);
 void pb_kv_batch_release(pb_kv_batch* batch);
 /* Writes k and v, [new tokens of all sequences, kv_heads, head_dim], into

@@ -132,6 +132,8 @@ def _declare(L: ctypes.CDLL) -> None:
         "pb_kv_cache_scales": (c_int, [T, P(c_uint64), P(c_uint64)]),
         "pb_kv_read": (c_int, [T, P(T), P(T)]),
         "pb_kv_batch_create": (c_int, [T, P(c_int32), c_size_t, c_size_t, P(c_int64), P(c_int64), P(c_int64), P(T)]),
+        "pb_kv_batch_create_shared": (c_int, [T, P(c_int32), c_size_t, c_size_t, P(c_int64), P(c_int64), P(c_int64),
+                                              P(c_int64), P(T)]),
         "pb_kv_batch_on": (c_int, [T, T, P(T)]),
         "pb_kv_batch_release": (None, [T]),
         "pb_kv_append": (c_int, [T, T, T]),

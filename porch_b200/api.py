@@ -610,17 +610,20 @@ class KVCache:
             raise InvalidArgument("cache: only an int8 cache has scales")
         return _Pool(self, 0, True), _Pool(self, 1, True)
 
-    def batch(self, tables, lengths, appended=None, newest=None) -> "Batch":
+    def batch(self, tables, lengths, appended=None, newest=None, prefix=None) -> "Batch":
         """The sequences of one step: tables [sequences, width] of page
         numbers, lengths in slots (new tokens included), how many of them are
-        new (default 1), and the newest slot's position (default length - 1)."""
-        return Batch(self, tables, lengths, appended, newest)
+        new (default 1), and the newest slot's position (default length - 1).
+        prefix (default none): how many of each one's first slots, in whole
+        pages, it shares with the sequences beside it that begin on the same
+        page; paged_attention works through them once."""
+        return Batch(self, tables, lengths, appended, newest, prefix)
 
 
 class Batch:
     """Page tables and lengths of one step's sequences (KVCache.batch)."""
 
-    def __init__(self, cache: KVCache, tables, lengths, appended=None, newest=None):
+    def __init__(self, cache: KVCache, tables, lengths, appended=None, newest=None, prefix=None):
         self._h = c_void_p()
         self.cache = cache
         table = np.asarray(tables)
@@ -636,16 +639,16 @@ class Batch:
                 return None
             a = np.asarray(values)
             if a.shape != (n,) or (n and a.dtype.kind not in "iu"):
-                raise InvalidArgument("cache batch: one whole length, new tokens and newest position per sequence")
+                raise InvalidArgument("cache batch: one whole length, new tokens, newest position and prefix per sequence")
             return np.ascontiguousarray(a, dtype=np.int64)
 
-        self.lengths, fresh, last = whole(lengths), whole(appended), whole(newest)
+        self.lengths, fresh, last, shared = whole(lengths), whole(appended), whole(newest), whole(prefix)
 
         def at(a, kind):
             return None if a is None else a.ctypes.data_as(ctypes.POINTER(kind))
 
-        _check(lib().pb_kv_batch_create(cache._h, at(table, ctypes.c_int32), n, width, at(self.lengths, c_int64),
-                                        at(fresh, c_int64), at(last, c_int64), byref(self._h)))
+        _check(lib().pb_kv_batch_create_shared(cache._h, at(table, ctypes.c_int32), n, width, at(self.lengths, c_int64),
+                                               at(fresh, c_int64), at(last, c_int64), at(shared, c_int64), byref(self._h)))
         self._address = self._h.value
 
     def __del__(self):

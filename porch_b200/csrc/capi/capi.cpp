@@ -833,6 +833,12 @@ int pb_kv_cache_scales(const pb_kv_cache* cache, uint64_t* keys, uint64_t* value
 
 int pb_kv_batch_create(pb_kv_cache* cache, const int32_t* tables, size_t sequences, size_t width,
                        const int64_t* lengths, const int64_t* appended, const int64_t* newest, pb_kv_batch** out) {
+    return pb_kv_batch_create_shared(cache, tables, sequences, width, lengths, appended, newest, nullptr, out);
+}
+
+int pb_kv_batch_create_shared(pb_kv_cache* cache, const int32_t* tables, size_t sequences, size_t width,
+                              const int64_t* lengths, const int64_t* appended, const int64_t* newest,
+                              const int64_t* prefix, pb_kv_batch** out) {
     return guarded([&] {
         require(out, "out");
         *out = nullptr;
@@ -840,7 +846,7 @@ int pb_kv_batch_create(pb_kv_cache* cache, const int32_t* tables, size_t sequenc
         require(lengths, "lengths");
         if (width != 0) require(tables, "tables");
         *out = new pb_kv_batch_s{
-            porch::detail::make_batch(cache->value, tables, sequences, width, lengths, appended, newest)};
+            porch::detail::make_batch(cache->value, tables, sequences, width, lengths, appended, newest, prefix)};
     });
 }
 

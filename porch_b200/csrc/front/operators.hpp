@@ -121,6 +121,7 @@ namespace porch::detail {
     struct plan_hint {
         std::mutex mutex;
         int64_t chunks = 0, ctas = 0; // 0: none yet
+        int64_t group = 0;            // query heads of a key head, of the last shared prefix
     };
 
     // Pools of pages of keys and values: [pages, heads, page_size, dim], so
@@ -159,10 +160,21 @@ namespace porch::detail {
         int64_t joins = 0, most_parts = 0;
         cuda_jit::device_buffer data; // 16 bytes per CTA, then 16 per row to join
     };
+    // The same for sequences that share a prefix. Rows are runs of slots of one
+    // key head with the queries that read them: the prefixes' first, then what
+    // follows them in each sequence.
+    struct shared_plan {
+        int64_t group = 0;                       // query heads of a key head
+        int tiles8 = 1;                          // of 8 queries that a row holds
+        int64_t ctas = 0, parts = 0, most_parts = 0;
+        cuda_jit::device_buffer data;
+        uint64_t rows_at = 0, work_at = 0, parts_at = 0, outs_at = 0; // device addresses
+    };
     struct batch_plans {
         std::shared_ptr<plan_hint> hint; // of the cache that the batch was made for
         std::mutex mutex;
         std::vector<std::unique_ptr<batch_plan>> made;
+        std::vector<std::unique_ptr<shared_plan>> shared;
     };
 
     // The sequences of one step: page tables, slots in use and the rows that
@@ -175,6 +187,11 @@ namespace porch::detail {
         int64_t longest = 0, tokens = 0, slots = 0; // tokens: new ones, slots: all, over all sequences
         int64_t table_width = 0;
         bool shared_pages = false;       // a page serves two sequences, or one twice
+        // Sequences next to each other whose first `slots` slots are the same pages.
+        struct group {
+            int64_t first = 0, members = 0, slots = 0;
+        };
+        std::vector<group> groups;
         cuda_jit::device_buffer data;    // int32: lengths, newest, tables, then 8-byte rows and starts
         // Made once with the batch for the number of query heads that its cache
         // last saw (up to 8 for each key head until then), and by the first
@@ -186,7 +203,7 @@ namespace porch::detail {
     };
     std::shared_ptr<kv_batch> make_batch(std::shared_ptr<kv_cache> cache, const int32_t* tables, size_t sequences,
                                          size_t width, const int64_t* lengths, const int64_t* appended,
-                                         const int64_t* newest);
+                                         const int64_t* newest, const int64_t* prefix = nullptr);
 
     // The plan for this many chunks and CTAs, which the cache's next batch gets.
     const batch_plan& plan_of(kv_batch& batch, int64_t chunks, int64_t ctas);

@@ -55,7 +55,7 @@ namespace porch::detail {
         struct form {
             int heads = 1, dim = 0, page = 0;
             cache_type type = cache_type::f32;
-            bool scored = false;
+            bool scored = false, shared = false;
             int stall = 0; // the test hook's mode
             int join_threads = 128;
             int tiles8 = 1; // groups of 8 query heads that a row holds (1 or 2)
@@ -80,7 +80,7 @@ namespace porch::detail {
             // against kStatic) with the rounding of the sum, and the KB that
             // the system keeps for each CTA.
             static constexpr int kStatic = 256;
-            int shared() const { return smem() + kStatic + 1024; }
+            int shared_bytes() const { return smem() + kStatic + 1024; }
 
           private:
             // CTAs of an SM and units of a CTA's ring: as many CTAs as leave
@@ -286,7 +286,35 @@ static __device__ __forceinline__ void pb_split_frag(const pb_u32* a, pb_u32* hi
 
 // Where a row's tiles come from. Rows are (sequence, key head, chunk of query
 // heads), tiles 64 slots of a row; a CTA works through a run of tiles.
+#if PB_SHARED
+// Sequences that share a prefix: a row is a run of slots of one key head, the
+// prefix or what follows it, and the queries that read it, of sequence after
+// sequence from `first` on, from the f0-th of their heads.
+struct pb_at { int row, tile; int s, h, begin, length, tiles, first, f0, count; };
+static __device__ __forceinline__ void pb_enter(pb_at& a, const int* rows, int) {
+    const int4 x = reinterpret_cast<const int4*>(rows)[2 * a.row], y = reinterpret_cast<const int4*>(rows)[2 * a.row + 1];
+    a.s = x.x;
+    a.h = x.y;
+    a.begin = x.z;
+    a.length = x.w;
+    a.first = y.x;
+    a.f0 = y.y;
+    a.count = y.z;
+    a.tiles = (a.length - a.begin + 63) >> 6;
+}
+static __device__ __forceinline__ int pb_base(const pb_at& a) { return a.begin + a.tile * 64; }
+static __device__ __forceinline__ int pb_heads(const pb_at& a, int) { return a.count; }
+static __device__ __forceinline__ pb_i64 pb_query(const pb_at& a, int head, int group, pb_i64 q_seq, pb_i64 q_head) {
+    const int f = a.f0 + head;
+    return (a.first + f / group) * q_seq + (a.h * group + f % group) * q_head;
+}
+#else
 struct pb_at { int row, tile; int s, h, chunk, length, tiles; };
+static __device__ __forceinline__ int pb_base(const pb_at& a) { return a.tile * 64; }
+static __device__ __forceinline__ int pb_heads(const pb_at& a, int group) { return min(PB_HT, group - a.chunk * PB_HT); }
+static __device__ __forceinline__ pb_i64 pb_query(const pb_at& a, int head, int group, pb_i64 q_seq, pb_i64 q_head) {
+    return a.s * q_seq + (a.h * group + a.chunk * PB_HT + head) * q_head;
+}
 static __device__ __forceinline__ void pb_enter(pb_at& a, const int* lengths, int chunks) {
     a.chunk = a.row % chunks;
     a.h = (a.row / chunks) % PB_H;
@@ -294,6 +322,7 @@ static __device__ __forceinline__ void pb_enter(pb_at& a, const int* lengths, in
     a.length = lengths[a.s];
     a.tiles = (a.length + 63) >> 6;
 }
+#endif
 // The next tile; skips sequences without slots. True when it is another row's.
 static __device__ __forceinline__ bool pb_next(pb_at& a, const int* lengths, int chunks) {
     if (++a.tile < a.tiles) return false;
@@ -307,7 +336,7 @@ static __device__ __forceinline__ bool pb_next(pb_at& a, const int* lengths, int
 
 // The page that this lane's part of the tile lies in (0 past its slots).
 static __device__ __forceinline__ int pb_page(const pb_at& a, const int* tables, int width, int lane) {
-    const int first = a.tile * 64 + lane * PB_BOX;
+    const int first = pb_base(a) + lane * PB_BOX;
     return lane * PB_BOX < 64 && first < a.length ? tables[(pb_i64)a.s * width + first / PB_PS] : 0;
 }
 
@@ -325,19 +354,19 @@ struct pb_queries { float x[PB_Q_EACH]; };
 #endif
 static __device__ __forceinline__ void pb_load_queries(pb_queries& r, const float* q, const pb_at& a, pb_i64 q_seq,
                                                        pb_i64 q_head, int group) {
-    const int heads = min(PB_HT, group - a.chunk * PB_HT), first = a.h * group + a.chunk * PB_HT;
+    const int heads = pb_heads(a, group);
 #if PB_ESZ == 1 // a warp has every fourth head, a lane runs of four channels
 #pragma unroll
     for (int j = 0; j < PB_Q_EACH8; ++j) {
         const int head = (threadIdx.x >> 5) + 4 * (j / (4 * PB_Q_RUNS));
         const int d = (j / 4 % PB_Q_RUNS) * 128 + (threadIdx.x & 31) * 4 + j % 4;
-        r.x[j] = head < heads && d < PB_D ? __ldg(q + a.s * q_seq + (first + head) * q_head + d) : 0.0f;
+        r.x[j] = head < heads && d < PB_D ? __ldg(q + pb_query(a, head, group, q_seq, q_head) + d) : 0.0f;
     }
 #else
 #pragma unroll
     for (int j = 0; j < PB_Q_EACH; ++j) {
         const int e = threadIdx.x + 128 * j, head = e / PB_Q_HEAD, d = e % PB_Q_HEAD;
-        r.x[j] = head < heads && d < PB_D ? __ldg(q + a.s * q_seq + (first + head) * q_head + d) : 0.0f;
+        r.x[j] = head < heads && d < PB_D ? __ldg(q + pb_query(a, head, group, q_seq, q_head) + d) : 0.0f;
     }
 #endif
 }
@@ -430,7 +459,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
         if (blockIdx.x == 0) return; // its tiles never arrive
 #endif
         for (int i = 0; i < mine.z && !bad; ++i) {
-            const int base = at.tile * 64, boxes = (min(64, at.length - base) + PB_BOX - 1) / PB_BOX;
+            const int base = pb_base(at), boxes = (min(64, at.length - base) + PB_BOX - 1) / PB_BOX;
             const int y = (page * PB_H + at.h) * PB_PS + (base + lane * PB_BOX) % PB_PS;
             if (i + 1 < mine.z) { // the next tile's pages are looked up while this one's loads are issued
                 pb_next(at, lengths, chunks);
@@ -472,9 +501,8 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
     // ---- four computing warps
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (mine.z == 0) { // a row without slots
-        const int heads = min(PB_HT, group - at.chunk * PB_HT);
-        const pb_i64 to = (pb_i64)at.s * PB_H * group + at.h * group + at.chunk * PB_HT;
-        for (int e = threadIdx.x; e < heads * PB_D; e += 128) out[to * PB_D + e] = 0.0f;
+        for (int e = threadIdx.x; e < pb_heads(at, group) * PB_D; e += 128)
+            out[pb_query(at, e / PB_D, group, PB_H * group, 1) * PB_D + e % PB_D] = 0.0f;
         return;
     }
     const int g = lane >> 2, t = lane & 3;
@@ -509,8 +537,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
             fresh = next_fresh;
         }
         if (i + 1 < mine.z) next_fresh = pb_next(next, lengths, chunks);
-        const int hg = min(PB_HT, group - at.chunk * PB_HT);             // query heads of this row
-        const int head0 = at.h * group + at.chunk * PB_HT;                // the first
+        const int hg = pb_heads(at, group); // query heads of this row
         if (fresh) {
             begun_at_zero = at.tile == 0;
             // The row's queries, split into terms; zero past the head size.
@@ -537,7 +564,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
             if (pb_bar_any(bad)) { bad = true; break; }
         }
         if (PB_Q_EACH8 <= 8 && i + 1 < mine.z && next_fresh) pb_load_queries(ahead, q, next, q_seq, q_head, group);
-        const int base = at.tile * 64, valid = min(64, at.length - base);
+        const int base = pb_base(at), valid = min(64, at.length - base);
 
         // ---- S^T = K Q^T: this warp's 16 slots x all heads
 #if PB_TEST_STALL == 2
@@ -641,7 +668,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
 #if PB_SCORED
                 const int head = 8 * n + 2 * t + (e & 1);
                 if (at_slot < valid && head < hg)
-                    logits[((pb_i64)at.s * PB_H * group + head0 + head) * longest + base + at_slot] = x;
+                    logits[pb_query(at, head, group, PB_H * group, 1) * longest + base + at_slot] = x;
 #endif
             }
 #pragma unroll
@@ -869,8 +896,12 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                 if (g == 0) *reinterpret_cast<float2*>(wsum + warp * PB_HT + 8 * n + 2 * t) = make_float2(l[n][0], l[n][1]);
             }
             if (pb_bar_any(bad)) { bad = true; break; }
-            const bool whole = begun_at_zero && row_ends;
+            const bool whole = !PB_SHARED && begun_at_zero && row_ends;
+#if PB_SHARED
+            const pb_i64 part = (pb_i64)mine.w + segment;
+#else
             const pb_i64 part = (pb_i64)blockIdx.x * 2 + (segment ? 1 : 0);
+#endif
 #pragma unroll
             for (int n = 0; n < PB_NT; ++n)
 #pragma unroll
@@ -880,7 +911,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
 #pragma unroll
                     for (int w = 0; w < 4; ++w) sum += wsum[w * PB_HT + head];
                     if (head >= hg) continue;
-                    const pb_i64 global = (pb_i64)at.s * PB_H * group + head0 + head;
+                    const pb_i64 global = pb_query(at, head, group, PB_H * group, 1);
                     float* to = whole ? out + global * PB_D : partial + (part * PB_HT + head) * PB_D;
                     const float inv = whole ? 1.0f / sum : 1.0f;
 #pragma unroll
@@ -907,6 +938,97 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
     if (bad) abort_flag = 1;
 }
 
+#if PB_SHARED
+// Joins the parts of a query head that reads a shared prefix and what follows
+// it. Parts of a row lie one behind the other: {first, how many} of each in
+// `rows`; a sequence's key head is {its first row, the prefix's first row (-1
+// where there is none), its first query's place among those that read the
+// prefix}. Block: one query head, as pb_join's; `h1`, `h2`: queries of a row of
+// the prefix and of a sequence.
+#define PB_JOIN (PB_JOIN_THREADS / (PB_D / 4))
+extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_shared_finish(
+    const int4* outs, const int2* rows, const float* partial1, const float2* ml1, const float* partial2, const float2* ml2,
+    float* out, int group, int h1, int h2) {
+    __shared__ float weight[PB_JOIN_THREADS], reduce[16];
+    __shared__ float4 sums[PB_JOIN_THREADS];
+    const int head = blockIdx.x % group;
+    const int4 o = outs[blockIdx.x / group]; // of the plan, in place before the launch
+    int2 r1 = make_int2(0, 0), r2 = make_int2(0, 0);
+    const int f = o.z + head;
+    if (o.y >= 0) r1 = rows[o.y + f / h1];
+    if (o.x >= 0) r2 = rows[o.x + head / h2];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int parts = r1.y + r2.y;
+    if (parts == 0) return; // already there
+    const float* p1 = partial1 + ((pb_i64)r1.x * h1 + f % h1) * PB_D;
+    const float* p2 = partial2 + ((pb_i64)r2.x * h2 + head % h2) * PB_D;
+    auto row = [&](int i) { return i < r1.y ? p1 + (pb_i64)i * h1 * PB_D : p2 + (pb_i64)(i - r1.y) * h2 * PB_D; };
+    const int lane = threadIdx.x & 31, quad = threadIdx.x % (PB_D / 4), team = threadIdx.x / (PB_D / 4);
+    float top = PB_LOWEST, sum = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int from = 0; from < parts; from += PB_JOIN_THREADS) {
+        const int n = min(PB_JOIN_THREADS, parts - from), i = from + threadIdx.x;
+        float2 ml = make_float2(PB_LOWEST, 0.0f);
+        if (threadIdx.x < n) ml = i < r1.y ? ml1[((pb_i64)r1.x + i) * h1 + f % h1] : ml2[((pb_i64)r2.x + i - r1.y) * h2 + head % h2];
+        float4 early[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            if (team < PB_JOIN && team + e * PB_JOIN < n) early[e] = *(reinterpret_cast<const float4*>(row(from + team + e * PB_JOIN)) + quad);
+        float x = ml.x;
+#pragma unroll
+        for (int m = 16; m > 0; m /= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, m));
+        __syncthreads();
+        if (lane == 0) reduce[threadIdx.x >> 5] = x;
+        __syncthreads();
+        x = top;
+#pragma unroll
+        for (int w = 0; w < PB_JOIN_THREADS / 32; ++w) x = fmaxf(x, reduce[w]);
+        const float corr = pb_exp2(top - x);
+        top = x;
+        const float w = threadIdx.x < n ? pb_exp2(ml.x - top) : 0.0f;
+        weight[threadIdx.x] = w;
+        float y = threadIdx.x < n ? w * ml.y : 0.0f;
+#pragma unroll
+        for (int m = 16; m > 0; m /= 2) y += __shfl_xor_sync(0xffffffffu, y, m);
+        __syncthreads();
+        if (lane == 0) reduce[threadIdx.x >> 5] = y;
+        __syncthreads();
+        y = 0.0f;
+#pragma unroll
+        for (int v = 0; v < PB_JOIN_THREADS / 32; ++v) y += reduce[v];
+        sum = fmaf(sum, corr, y);
+        acc = make_float4(acc.x * corr, acc.y * corr, acc.z * corr, acc.w * corr);
+        if (team < PB_JOIN) {
+            auto add = [&](const float4& v, float w) {
+                acc.x = fmaf(w, v.x, acc.x);
+                acc.y = fmaf(w, v.y, acc.y);
+                acc.z = fmaf(w, v.z, acc.z);
+                acc.w = fmaf(w, v.w, acc.w);
+            };
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                if (team + e * PB_JOIN < n) add(early[e], weight[team + e * PB_JOIN]);
+#pragma unroll 4
+            for (int j = team + 2 * PB_JOIN; j < n; j += PB_JOIN)
+                add(*(reinterpret_cast<const float4*>(row(from + j)) + quad), weight[j]);
+        }
+    }
+    sums[threadIdx.x] = acc;
+    __syncthreads();
+    if (team == 0) {
+        for (int w = 1; w < PB_JOIN; ++w) {
+            const float4 v = sums[w * (PB_D / 4) + quad];
+            acc.x += v.x;
+            acc.y += v.y;
+            acc.z += v.z;
+            acc.w += v.w;
+        }
+        const float inv = 1.0f / sum;
+        *reinterpret_cast<float4*>(out + (pb_i64)blockIdx.x * PB_D + 4 * quad) =
+            make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
+    }
+}
+#else
 // A row in several parts: {row, first CTA, number of parts, the first part's
 // place}. Part i's sums for a query head.
 static __device__ __forceinline__ pb_i64 pb_part(const int4& r, int i, int head) {
@@ -1093,6 +1215,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
               blockIdx.x - join_blocks);
 #endif
 }
+#endif
 )PB";
         }
 
@@ -1101,7 +1224,8 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             os << "#define PB_H " << f.heads << "\n#define PB_D " << f.dim << "\n#define PB_PS " << f.page
                << "\n#define PB_ESZ " << f.width() << "\n#define PB_NT " << f.tiles8 << "\n#define PB_RING " << f.ring()
                << "\n#define PB_JOIN_THREADS " << f.join_threads << "\n#define PB_PER_SM " << f.per_sm()
-               << "\n#define PB_STATIC " << form::kStatic << "\n#define PB_SCORED " << (f.scored ? 1 : 0) << "\n";
+               << "\n#define PB_STATIC " << form::kStatic << "\n#define PB_SCORED " << (f.scored ? 1 : 0) << "\n#define PB_SHARED " << (f.shared ? 1 : 0)
+               << "\n";
             if (f.stall != 0) os << "#define PB_TEST_STALL " << f.stall << "\n";
             return os.str();
         }
@@ -1123,9 +1247,10 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
 
         const char kAttention[] = "pb_paged_attention";
         const char kFinish[] = "pb_paged_finish";
+        const char kSharedFinish[] = "pb_shared_finish";
 
         op_kernel& kernel_of(const char* name, const form& f, uint32_t smem) {
-            const op_key key{reinterpret_cast<int64_t>(name), f.heads, f.dim, f.page, static_cast<int64_t>(f.type), f.scored, f.tiles8, f.join_threads, f.stall};
+            const op_key key{reinterpret_cast<int64_t>(name), f.heads, f.dim, f.page, static_cast<int64_t>(f.type), f.scored, f.tiles8, f.join_threads, f.stall, f.shared};
             return op_kernel_for(key, [&](op_kernel& k) {
                 k.name = name;
                 k.source = std::string{kernel_prelude()} + defines(f) + device_source();
@@ -1222,6 +1347,189 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             return r;
         }
 
+        // Rows of `tiles` tiles each (none is empty) in even runs over at most
+        // `ctas` CTAs, a row counting as a tile more than it has. Parts, a CTA's
+        // run of one row each, are numbered in the CTAs' order, so that a row's
+        // lie one behind the other.
+        struct runs {
+            std::vector<int32_t> work; // per CTA: row, tile, tiles, its first part
+            std::vector<int32_t> rows; // per row: its first part, how many
+            int64_t parts = 0;
+        };
+        runs share_out(const std::vector<int64_t>& tiles, int64_t ctas) {
+            runs r;
+            int64_t cost = 0;
+            for (int64_t t : tiles) cost += t + 1;
+            const int64_t n = std::min(ctas, cost - static_cast<int64_t>(tiles.size()));
+            r.rows.resize(2 * tiles.size(), 0);
+            int64_t at = 0, cut = 1; // cost so far; the next CTA's number
+            bool open = false;       // a CTA has begun
+            auto begin = [&](size_t row, int64_t tile) {
+                for (int64_t v : {static_cast<int64_t>(row), tile, int64_t{0}, r.parts}) r.work.push_back(static_cast<int32_t>(v));
+                open = true;
+            };
+            for (size_t row = 0; row < tiles.size(); ++row) {
+                r.rows[2 * row] = static_cast<int32_t>(r.parts);
+                int64_t tile = 0;
+                while (tile < tiles[row]) {
+                    if (!open) begin(row, tile);
+                    // Tiles up to where the next CTA begins; one at least, so that none is empty.
+                    const int64_t until = cut < n ? static_cast<int64_t>(static_cast<__int128>(cost) * cut / n) - at - 1 : tiles[row];
+                    const int64_t take = std::min(tiles[row], std::max(until, tile + 1)) - tile;
+                    r.work[r.work.size() - 2] += static_cast<int32_t>(take);
+                    tile += take;
+                    ++r.parts;
+                    ++r.rows[2 * row + 1];
+                    if (cut < n && at + 1 + tile >= static_cast<int64_t>(static_cast<__int128>(cost) * cut / n)) {
+                        ++cut;
+                        open = false;
+                    }
+                }
+                at += tiles[row] + 1;
+            }
+            return r;
+        }
+
+    } // namespace
+
+    namespace {
+
+        // The form of a shared prefix's rows: 16 queries share a tile's loads
+        // where there are as many.
+        form shared_form(const kv_batch& batch, int64_t group) {
+            form f = form_of(*batch.cache, 1);
+            f.shared = true;
+            int64_t most = group;
+            for (const auto& g : batch.groups) most = std::max(most, g.members * group);
+            f.tiles8 = most > 8 ? 2 : 1;
+            if (f.ring() < 3) f.tiles8 = 1;
+            return f;
+        }
+
+        // The plan for `group` query heads of each key head, which the cache's next
+        // such batch gets.
+        const shared_plan& shared_plan_of(kv_batch& batch, int64_t group) {
+            if (batch.plans->hint != nullptr) {
+                std::scoped_lock lock{batch.plans->hint->mutex};
+                batch.plans->hint->group = group;
+            }
+            std::scoped_lock lock{batch.plans->mutex};
+            for (const auto& p : batch.plans->shared)
+                if (p->group == group) return *p;
+            const kv_cache& c = *batch.cache;
+            const form f = shared_form(batch, group);
+            auto p = std::make_unique<shared_plan>();
+            p->group = group;
+            p->tiles8 = f.tiles8;
+            const int64_t per = 8 * f.tiles8, heads = c.heads, n = batch.sequences();
+            std::vector<int32_t> rows;
+            std::vector<int64_t> tiles;
+            std::vector<int32_t> outs(static_cast<size_t>(4 * n * heads), -1);
+            auto put = [&](int64_t seq, int64_t h, int64_t begin, int64_t end, int64_t first, int64_t queries) {
+                const auto row = static_cast<int32_t>(rows.size() / 8);
+                for (int64_t f0 = 0; f0 < queries; f0 += per)
+                    for (int64_t v : {seq, h, begin, end, first, f0, std::min(per, queries - f0), int64_t{0}})
+                        rows.push_back(static_cast<int32_t>(v));
+                if (end > begin) tiles.insert(tiles.end(), static_cast<size_t>((queries + per - 1) / per), (end - begin + 63) / 64);
+                return row;
+            };
+            std::vector<int64_t> begin(static_cast<size_t>(n), 0);
+            for (const auto& g : batch.groups)
+                for (int64_t h = 0; h < heads; ++h) {
+                    const int32_t row = put(g.first, h, 0, g.slots, g.first, g.members * group);
+                    for (int64_t s = g.first; s < g.first + g.members; ++s) {
+                        begin[static_cast<size_t>(s)] = g.slots;
+                        outs[static_cast<size_t>(4 * (s * heads + h) + 1)] = row;
+                        outs[static_cast<size_t>(4 * (s * heads + h) + 2)] = static_cast<int32_t>((s - g.first) * group);
+                    }
+                }
+            for (int64_t s = 0; s < n; ++s) {
+                const int64_t from = begin[static_cast<size_t>(s)], to = batch.lengths[static_cast<size_t>(s)];
+                if (to > from)
+                    for (int64_t h = 0; h < heads; ++h)
+                        outs[static_cast<size_t>(4 * (s * heads + h))] = put(s, h, from, to, s, group);
+            }
+            expect(rows.size() / 8 < (size_t{1} << 27), "paged_attention: too many sequences and heads");
+            runs r = share_out(tiles, int64_t{f.per_sm()} * sm_count(c.device));
+            p->parts = r.parts;
+            // Rows without slots, whose CTAs write zeros, come last.
+            for (int64_t s = 0; s < n; ++s)
+                if (batch.lengths[static_cast<size_t>(s)] == 0)
+                    for (int64_t h = 0; h < heads; ++h) {
+                        const int32_t row = put(s, h, 0, 0, s, group);
+                        for (int64_t i = 0; i < (group + per - 1) / per; ++i)
+                            for (int32_t v : {static_cast<int32_t>(row + i), 0, 0, 0}) r.work.push_back(v);
+                    }
+            p->ctas = static_cast<int64_t>(r.work.size() / 4);
+            for (int64_t s = 0; s < n; ++s) { // the most parts of a query: of the first head's, others have as many
+                int64_t parts = 0;
+                for (int64_t i : {0, 1}) {
+                    const int32_t row = outs[static_cast<size_t>(4 * s * heads + i)];
+                    if (row >= 0) parts += r.rows[static_cast<size_t>(2 * row + 1)];
+                }
+                p->most_parts = std::max(p->most_parts, parts);
+            }
+            // Rows and outs are read 16 bytes at a time: rows, work, outs, parts.
+            std::vector<int32_t> host = std::move(rows);
+            const size_t work = host.size();
+            host.insert(host.end(), r.work.begin(), r.work.end());
+            const size_t out = host.size();
+            host.insert(host.end(), outs.begin(), outs.end());
+            const size_t part = host.size();
+            host.insert(host.end(), r.rows.begin(), r.rows.end());
+            auto stream = upload_stream(c.device);
+            p->data = allocate(c.device, host.size() * sizeof(int32_t), stream);
+            p->rows_at = address(p->data);
+            p->work_at = p->rows_at + work * 4;
+            p->outs_at = p->rows_at + out * 4;
+            p->parts_at = p->rows_at + part * 4;
+            check(pbrt_memcpy_h2d_async(c.device, p->rows_at, host.data(), host.size() * sizeof(int32_t), stream->stream));
+            check(pbrt_stream_synchronize(c.device, stream->stream));
+            batch.plans->shared.push_back(std::move(p));
+            return *batch.plans->shared.back();
+        }
+
+        // Attention of sequences that share prefixes; the operands are checked.
+        tensor shared_attention(const op_operand& x, kv_batch& batch, float scale2, const std::shared_ptr<stream_ref>& stream) {
+            kv_cache& c = *batch.cache;
+            const int device = c.device;
+            int group = static_cast<int>(x.shape[1] / c.heads);
+            form f = shared_form(batch, group);
+            f.stall = g_test_stall.load(std::memory_order_relaxed);
+            const shared_plan& plan = shared_plan_of(batch, group);
+            op_result out = new_result(x.shape, device, stream);
+            // Workspace: the parts' maxima and sums, and their results.
+            int per = 8 * f.tiles8;
+            const size_t part_heads = static_cast<size_t>(plan.parts) * static_cast<size_t>(per);
+            cuda_jit::device_buffer scratch = allocate(device, part_heads * static_cast<size_t>(c.dim + 2) * sizeof(float), stream);
+            uint64_t partial = address(scratch), ml = partial + part_heads * static_cast<size_t>(c.dim) * 4;
+            op_kernel& attention = kernel_of(kAttention, f, static_cast<uint32_t>(f.smem()));
+            if (plan.most_parts > 16) f.join_threads = 512;
+            op_kernel& finishing = kernel_of(kSharedFinish, f, 0);
+            (void)attention.on(device);
+            (void)finishing.on(device);
+            order_read(*cuda_jit::buffer_access::state(batch.data), stream);
+            order_read(*cuda_jit::buffer_access::state(plan.data), stream);
+            uint64_t err = 0, none = 0, queries = x.ptr;
+            check(pbrt_error_word(device, &err));
+            uint64_t rows = plan.rows_at, work = plan.work_at, parts = plan.parts_at, outs = plan.outs_at;
+            uint64_t scales_k = address(c.k) + static_cast<uint64_t>(c.values_bytes()), scales_v = address(c.v) + static_cast<uint64_t>(c.values_bytes());
+            int width = static_cast<int>(batch.table_width), chunks = 0, longest = 0;
+            int64_t q_seq = x.strides[0], q_head = x.strides[1];
+            {
+                void* params[] = {&c.map_k, &c.map_v, &queries, &rows, &batch.tables_at, &work, &out.ptr, &partial, &ml,
+                                  &none, &none, &width, &group, &chunks, &q_seq, &q_head, &longest, &scale2, &err, &scales_k, &scales_v};
+                std::scoped_lock lock{c.order};
+                order_read(*cuda_jit::buffer_access::state(c.k), stream);
+                order_read(*cuda_jit::buffer_access::state(c.v), stream);
+                op_launch(attention, device, stream, {static_cast<uint32_t>(plan.ctas), 1, 1}, 160, params);
+            }
+            void* params[] = {&outs, &parts, &partial, &ml, &partial, &ml, &out.ptr, &group, &per, &per};
+            op_launch(finishing, device, stream, {static_cast<uint32_t>(x.shape[0] * x.shape[1]), 1, 1},
+                      static_cast<uint32_t>(f.join_threads), params);
+            return finish(std::move(out));
+        }
+
     } // namespace
 
     std::vector<tensor> paged_attention(const tensor& q, kv_batch& batch, float scale, bool scored,
@@ -1249,6 +1557,11 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         auto stream = current_stream(device);
         op_operand x = operand(q, stream, true), xs;
         if (scores != nullptr) xs = operand(*scores, stream, false);
+        if (!scored && !batch.groups.empty()) {
+            std::vector<tensor> results;
+            results.push_back(shared_attention(x, batch, scale2, stream));
+            return results;
+        }
         int heads = static_cast<int>(shape[1]), group = static_cast<int>(shape[1] / c.heads);
         form f = form_of(c, group);
         f.scored = scored;
@@ -1320,7 +1633,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         c.dim = dim;
         c.type = type;
         const form f = form_of(c, group);
-        return {f.per_sm(), f.shared()};
+        return {f.per_sm(), f.shared_bytes()};
     }
 
     const batch_plan& plan_of(kv_batch& batch, int64_t chunks, int64_t ctas) {
@@ -1352,11 +1665,16 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
     }
 
     void prepare_plan(kv_batch& batch) {
-        int64_t chunks = 0, ctas = 0;
+        int64_t chunks = 0, ctas = 0, group = 0;
         {
             std::scoped_lock lock{batch.plans->hint->mutex};
             chunks = batch.plans->hint->chunks;
             ctas = batch.plans->hint->ctas;
+            group = batch.plans->hint->group;
+        }
+        if (!batch.groups.empty()) {
+            (void)shared_plan_of(batch, group != 0 ? group : 1);
+            return;
         }
         if (chunks == 0) {
             chunks = 1;
@@ -1387,8 +1705,9 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             f.type = width == 1 ? cache_type::i8 : (width == 2 ? cache_type::bf16 : cache_type::f32);
             f.tiles8 = tiles8;
             f.page = page;
-            f.scored = true;
-            out.emplace_back("pb_paged_attention_" + std::to_string(dim) + (width == 1 ? "_i8_" : (width == 2 ? "_bf16_" : "_f32_")) + std::to_string(8 * tiles8),
+            f.shared = page == 32;
+            f.scored = !f.shared;
+            out.emplace_back("pb_paged_attention_" + std::to_string(dim) + (width == 1 ? "_i8_" : (width == 2 ? "_bf16_" : "_f32_")) + std::to_string(8 * tiles8) + (f.shared ? "_shared" : ""),
                              std::string{kernel_prelude()} + defines(f) + device_source());
         }
     }

@@ -876,7 +876,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
 
     std::shared_ptr<kv_batch> make_batch(std::shared_ptr<kv_cache> cache, const int32_t* tables, size_t sequences,
                                          size_t width, const int64_t* lengths, const int64_t* appended,
-                                         const int64_t* newest) {
+                                         const int64_t* newest, const int64_t* prefix) {
         const int64_t page = cache->page_size;
         expect(sequences >= 1 && sequences <= 65535, "cache batch: 1 to 65535 sequences");
         auto b = std::make_shared<kv_batch>();
@@ -899,10 +899,24 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
                     b->shared_pages = true;
                 }
             }
-            const int64_t fresh = appended != nullptr ? appended[s] : std::min<int64_t>(1, n);
+            const int64_t shared = prefix != nullptr ? prefix[s] : 0;
+            const int64_t fresh = appended != nullptr ? appended[s] : std::clamp<int64_t>(n - shared, 0, 1);
             expect(fresh >= 0 && fresh <= n, at + "new tokens must be 0 to its length");
             for (int64_t i = n - fresh; i < n; ++i)
                 rows.push_back(int64_t{tables[s * width + static_cast<size_t>(i / page)]} * page + i % page);
+            if (prefix != nullptr) {
+                expect(shared >= 0 && shared % page == 0, at + "a prefix must be whole pages");
+                expect(shared <= n - fresh, at + "a prefix must end before its length and its new tokens");
+                // One group with the sequence before where both begin on the same page.
+                const bool joins = s != 0 && shared != 0 && prefix[s - 1] == shared && tables[s * width] == tables[(s - 1) * width];
+                if (joins) {
+                    expect(std::equal(tables + s * width, tables + s * width + shared / page, tables + (s - 1) * width),
+                           at + "its prefix begins as the sequence's before, but has other pages");
+                    ++b->groups.back().members;
+                } else if (shared != 0) {
+                    b->groups.push_back({static_cast<int64_t>(s), 1, shared});
+                }
+            }
             const int64_t last = newest != nullptr ? newest[s] : std::max<int64_t>(0, n - 1);
             expect(last >= 0 && last < (int64_t{1} << 24), at + "newest position must be 0 to 2^24 (float32 counts them exactly)");
             expect(newest == nullptr || n == 0 || last >= n - 1, at + "newest position must be at least its length - 1");
@@ -912,6 +926,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
             starts.push_back(b->slots);
             b->table_width = std::max(b->table_width, pages);
         }
+        std::erase_if(b->groups, [](const kv_batch::group& g) { return g.members == 1; }); // shared with nobody
         if (b->shared_pages) {
             std::unordered_set<int64_t> distinct(rows.begin(), rows.end());
             expect(distinct.size() == rows.size(), "cache batch: two new tokens go to the same row");
