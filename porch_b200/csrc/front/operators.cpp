@@ -187,6 +187,7 @@ namespace porch::detail {
         token_logprobs_sources(all);
         paged_cache_sources(all);
         paged_attention_sources(all);
+        prefix_attention_sources(all);
         std::ostringstream os;
         for (const auto& [name, source] : all) (void)compile(source); // NVRTC takes it, too
         for (const auto& [name, source] : all) os << "kernel " << name << " : operator\n" << source << "\n";

@@ -164,11 +164,18 @@ namespace porch::detail {
     // key head with the queries that read them: the prefixes' first, then what
     // follows them in each sequence.
     struct shared_plan {
-        int64_t group = 0;                       // query heads of a key head
-        int tiles8 = 1;                          // of 8 queries that a row holds
-        int64_t ctas = 0, parts = 0, most_parts = 0;
+        int64_t group = 0; // query heads of a key head
+        // One launch's rows. The prefixes have one of their own where the tensor
+        // cores' large tiles take them (else the second has them, too).
+        struct stage {
+            int per = 8; // queries that a row holds
+            int64_t ctas = 0, parts = 0;
+            uint64_t rows_at = 0, work_at = 0; // device addresses
+        };
+        stage prefix, rest;
+        int64_t most_parts = 0;
         cuda_jit::device_buffer data;
-        uint64_t rows_at = 0, work_at = 0, parts_at = 0, outs_at = 0; // device addresses
+        uint64_t parts_at = 0, outs_at = 0;
     };
     struct batch_plans {
         std::shared_ptr<plan_hint> hint; // of the cache that the batch was made for
@@ -241,5 +248,11 @@ namespace porch::detail {
     void token_logprobs_sources(kernel_list& out);
     void paged_cache_sources(kernel_list& out);
     void paged_attention_sources(kernel_list& out);
+    void prefix_attention_sources(kernel_list& out);
+
+    // Whether there is a kernel of 128 queries a row for prefixes in this cache
+    // (bfloat16, head_dim up to 128), and that kernel: 512 threads, a CTA an SM.
+    bool prefix_attention_takes(const kv_cache& c);
+    op_kernel& prefix_attention_kernel(const kv_cache& c, int stall);
 
 } // namespace porch::detail

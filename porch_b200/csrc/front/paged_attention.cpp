@@ -1348,7 +1348,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         }
 
         // Rows of `tiles` tiles each (none is empty) in even runs over at most
-        // `ctas` CTAs, a row counting as a tile more than it has. Parts, a CTA's
+        // `ctas` CTAs, a row counting as `extra` tiles more than it has. Parts, a CTA's
         // run of one row each, are numbered in the CTAs' order, so that a row's
         // lie one behind the other.
         struct runs {
@@ -1356,11 +1356,12 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             std::vector<int32_t> rows; // per row: its first part, how many
             int64_t parts = 0;
         };
-        runs share_out(const std::vector<int64_t>& tiles, int64_t ctas) {
+        constexpr int64_t kRowCost = 3; // of 128 queries: they are split, and results stored
+        runs share_out(const std::vector<int64_t>& tiles, int64_t ctas, int64_t extra) {
             runs r;
             int64_t cost = 0;
-            for (int64_t t : tiles) cost += t + 1;
-            const int64_t n = std::min(ctas, cost - static_cast<int64_t>(tiles.size()));
+            for (int64_t t : tiles) cost += t + extra;
+            const int64_t n = std::min(ctas, cost - extra * static_cast<int64_t>(tiles.size()));
             r.rows.resize(2 * tiles.size(), 0);
             int64_t at = 0, cut = 1; // cost so far; the next CTA's number
             bool open = false;       // a CTA has begun
@@ -1374,18 +1375,18 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
                 while (tile < tiles[row]) {
                     if (!open) begin(row, tile);
                     // Tiles up to where the next CTA begins; one at least, so that none is empty.
-                    const int64_t until = cut < n ? static_cast<int64_t>(static_cast<__int128>(cost) * cut / n) - at - 1 : tiles[row];
+                    const int64_t until = cut < n ? static_cast<int64_t>(static_cast<__int128>(cost) * cut / n) - at - extra : tiles[row];
                     const int64_t take = std::min(tiles[row], std::max(until, tile + 1)) - tile;
                     r.work[r.work.size() - 2] += static_cast<int32_t>(take);
                     tile += take;
                     ++r.parts;
                     ++r.rows[2 * row + 1];
-                    if (cut < n && at + 1 + tile >= static_cast<int64_t>(static_cast<__int128>(cost) * cut / n)) {
+                    if (cut < n && at + extra + tile >= static_cast<int64_t>(static_cast<__int128>(cost) * cut / n)) {
                         ++cut;
                         open = false;
                     }
                 }
-                at += tiles[row] + 1;
+                at += tiles[row] + extra;
             }
             return r;
         }
@@ -1394,11 +1395,20 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
 
     namespace {
 
-        // The form of a shared prefix's rows: 16 queries share a tile's loads
-        // where there are as many.
+        // Whether prefixes are worked through 128 queries at a time: where more
+        // than 16, which the other form has, read one.
+        bool prefix_stage(const kv_batch& batch, int64_t group) {
+            int64_t most = 0;
+            for (const auto& g : batch.groups) most = std::max(most, g.members * group);
+            return prefix_attention_takes(*batch.cache) && most > 16;
+        }
+
+        // The form of what follows the prefixes, and of prefixes without a stage of
+        // their own: 16 queries share a tile's loads where there are as many.
         form shared_form(const kv_batch& batch, int64_t group) {
-            form f = form_of(*batch.cache, 1);
+            form f = form_of(*batch.cache, group);
             f.shared = true;
+            if (prefix_stage(batch, group)) return f;
             int64_t most = group;
             for (const auto& g : batch.groups) most = std::max(most, g.members * group);
             f.tiles8 = most > 8 ? 2 : 1;
@@ -1418,14 +1428,16 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
                 if (p->group == group) return *p;
             const kv_cache& c = *batch.cache;
             const form f = shared_form(batch, group);
+            const bool own_stage = prefix_stage(batch, group);
             auto p = std::make_unique<shared_plan>();
             p->group = group;
-            p->tiles8 = f.tiles8;
-            const int64_t per = 8 * f.tiles8, heads = c.heads, n = batch.sequences();
+            p->rest.per = 8 * f.tiles8;
+            p->prefix.per = own_stage ? 128 : p->rest.per;
+            const int64_t heads = c.heads, n = batch.sequences();
             std::vector<int32_t> rows;
             std::vector<int64_t> tiles;
             std::vector<int32_t> outs(static_cast<size_t>(4 * n * heads), -1);
-            auto put = [&](int64_t seq, int64_t h, int64_t begin, int64_t end, int64_t first, int64_t queries) {
+            auto put = [&](int64_t per, int64_t seq, int64_t h, int64_t begin, int64_t end, int64_t first, int64_t queries) {
                 const auto row = static_cast<int32_t>(rows.size() / 8);
                 for (int64_t f0 = 0; f0 < queries; f0 += per)
                     for (int64_t v : {seq, h, begin, end, first, f0, std::min(per, queries - f0), int64_t{0}})
@@ -1436,54 +1448,69 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             std::vector<int64_t> begin(static_cast<size_t>(n), 0);
             for (const auto& g : batch.groups)
                 for (int64_t h = 0; h < heads; ++h) {
-                    const int32_t row = put(g.first, h, 0, g.slots, g.first, g.members * group);
+                    const int32_t row = put(p->prefix.per, g.first, h, 0, g.slots, g.first, g.members * group);
                     for (int64_t s = g.first; s < g.first + g.members; ++s) {
                         begin[static_cast<size_t>(s)] = g.slots;
                         outs[static_cast<size_t>(4 * (s * heads + h) + 1)] = row;
                         outs[static_cast<size_t>(4 * (s * heads + h) + 2)] = static_cast<int32_t>((s - g.first) * group);
                     }
                 }
+            runs first;
+            const auto prefix_rows = static_cast<int32_t>(tiles.size());
+            if (own_stage) {
+                first = share_out(tiles, sm_count(c.device), kRowCost);
+                tiles.clear();
+            }
             for (int64_t s = 0; s < n; ++s) {
                 const int64_t from = begin[static_cast<size_t>(s)], to = batch.lengths[static_cast<size_t>(s)];
                 if (to > from)
                     for (int64_t h = 0; h < heads; ++h)
-                        outs[static_cast<size_t>(4 * (s * heads + h))] = put(s, h, from, to, s, group);
+                        outs[static_cast<size_t>(4 * (s * heads + h))] = put(p->rest.per, s, h, from, to, s, group);
             }
             expect(rows.size() / 8 < (size_t{1} << 27), "paged_attention: too many sequences and heads");
-            runs r = share_out(tiles, int64_t{f.per_sm()} * sm_count(c.device));
-            p->parts = r.parts;
+            runs r = share_out(tiles, int64_t{f.per_sm()} * sm_count(c.device), 1);
+            p->prefix.parts = first.parts;
+            p->prefix.ctas = static_cast<int64_t>(first.work.size() / 4);
+            p->rest.parts = r.parts;
+            // Each launch counts its rows from its first.
+            std::vector<int32_t> parts = first.rows;
+            parts.insert(parts.end(), r.rows.begin(), r.rows.end());
+            const int32_t rest_row = own_stage ? prefix_rows : 0;
             // Rows without slots, whose CTAs write zeros, come last.
             for (int64_t s = 0; s < n; ++s)
                 if (batch.lengths[static_cast<size_t>(s)] == 0)
                     for (int64_t h = 0; h < heads; ++h) {
-                        const int32_t row = put(s, h, 0, 0, s, group);
-                        for (int64_t i = 0; i < (group + per - 1) / per; ++i)
-                            for (int32_t v : {static_cast<int32_t>(row + i), 0, 0, 0}) r.work.push_back(v);
+                        const int32_t row = put(p->rest.per, s, h, 0, 0, s, group);
+                        for (int64_t i = 0; i < (group + p->rest.per - 1) / p->rest.per; ++i)
+                            for (int32_t v : {static_cast<int32_t>(row - rest_row + i), 0, 0, 0}) r.work.push_back(v);
                     }
-            p->ctas = static_cast<int64_t>(r.work.size() / 4);
-            for (int64_t s = 0; s < n; ++s) { // the most parts of a query: of the first head's, others have as many
-                int64_t parts = 0;
+            p->rest.ctas = static_cast<int64_t>(r.work.size() / 4);
+            for (int64_t s = 0; s < n; ++s) { // the most parts of a query: of the first head's, others have about as many
+                int64_t count = 0;
                 for (int64_t i : {0, 1}) {
                     const int32_t row = outs[static_cast<size_t>(4 * s * heads + i)];
-                    if (row >= 0) parts += r.rows[static_cast<size_t>(2 * row + 1)];
+                    if (row >= 0) count += parts[static_cast<size_t>(2 * row + 1)];
                 }
-                p->most_parts = std::max(p->most_parts, parts);
+                p->most_parts = std::max(p->most_parts, count);
             }
-            // Rows and outs are read 16 bytes at a time: rows, work, outs, parts.
+            // Rows, work and outs are read 16 bytes at a time, parts 8.
             std::vector<int32_t> host = std::move(rows);
-            const size_t work = host.size();
-            host.insert(host.end(), r.work.begin(), r.work.end());
-            const size_t out = host.size();
-            host.insert(host.end(), outs.begin(), outs.end());
-            const size_t part = host.size();
-            host.insert(host.end(), r.rows.begin(), r.rows.end());
+            auto add = [&](const std::vector<int32_t>& v) {
+                const size_t at = host.size();
+                host.insert(host.end(), v.begin(), v.end());
+                return at * 4;
+            };
+            const size_t prefix_work = add(first.work), rest_work = add(r.work), out = add(outs), part = add(parts);
             auto stream = upload_stream(c.device);
             p->data = allocate(c.device, host.size() * sizeof(int32_t), stream);
-            p->rows_at = address(p->data);
-            p->work_at = p->rows_at + work * 4;
-            p->outs_at = p->rows_at + out * 4;
-            p->parts_at = p->rows_at + part * 4;
-            check(pbrt_memcpy_h2d_async(c.device, p->rows_at, host.data(), host.size() * sizeof(int32_t), stream->stream));
+            const uint64_t at = address(p->data);
+            p->prefix.rows_at = at;
+            p->rest.rows_at = at + static_cast<uint64_t>(rest_row) * 32;
+            p->prefix.work_at = at + prefix_work;
+            p->rest.work_at = at + rest_work;
+            p->outs_at = at + out;
+            p->parts_at = at + part;
+            check(pbrt_memcpy_h2d_async(c.device, at, host.data(), host.size() * sizeof(int32_t), stream->stream));
             check(pbrt_stream_synchronize(c.device, stream->stream));
             batch.plans->shared.push_back(std::move(p));
             return *batch.plans->shared.back();
@@ -1498,33 +1525,49 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             f.stall = g_test_stall.load(std::memory_order_relaxed);
             const shared_plan& plan = shared_plan_of(batch, group);
             op_result out = new_result(x.shape, device, stream);
-            // Workspace: the parts' maxima and sums, and their results.
-            int per = 8 * f.tiles8;
-            const size_t part_heads = static_cast<size_t>(plan.parts) * static_cast<size_t>(per);
-            cuda_jit::device_buffer scratch = allocate(device, part_heads * static_cast<size_t>(c.dim + 2) * sizeof(float), stream);
-            uint64_t partial = address(scratch), ml = partial + part_heads * static_cast<size_t>(c.dim) * 4;
-            op_kernel& attention = kernel_of(kAttention, f, static_cast<uint32_t>(f.smem()));
+            // Workspace: the parts' results, and their maxima and sums; the prefixes' first.
+            const size_t heads1 = static_cast<size_t>(plan.prefix.parts * plan.prefix.per), heads2 = static_cast<size_t>(plan.rest.parts * plan.rest.per);
+            const size_t dim = static_cast<size_t>(c.dim);
+            cuda_jit::device_buffer scratch = allocate(device, (heads1 + heads2) * (dim + 2) * sizeof(float), stream);
+            uint64_t partial1 = address(scratch), partial2 = partial1 + heads1 * dim * 4, ml1 = partial2 + heads2 * dim * 4, ml2 = ml1 + heads1 * 8;
+            op_kernel* prefix = plan.prefix.ctas > 0 ? &prefix_attention_kernel(c, f.stall) : nullptr;
+            op_kernel* rest = plan.rest.ctas > 0 ? &kernel_of(kAttention, f, static_cast<uint32_t>(f.smem())) : nullptr;
             if (plan.most_parts > 16) f.join_threads = 512;
             op_kernel& finishing = kernel_of(kSharedFinish, f, 0);
-            (void)attention.on(device);
+            if (prefix != nullptr) (void)prefix->on(device);
+            if (rest != nullptr) (void)rest->on(device);
             (void)finishing.on(device);
             order_read(*cuda_jit::buffer_access::state(batch.data), stream);
             order_read(*cuda_jit::buffer_access::state(plan.data), stream);
             uint64_t err = 0, none = 0, queries = x.ptr;
             check(pbrt_error_word(device, &err));
-            uint64_t rows = plan.rows_at, work = plan.work_at, parts = plan.parts_at, outs = plan.outs_at;
+            uint64_t rows1 = plan.prefix.rows_at, work1 = plan.prefix.work_at, rows2 = plan.rest.rows_at, work2 = plan.rest.work_at;
+            uint64_t parts = plan.parts_at, outs = plan.outs_at;
             uint64_t scales_k = address(c.k) + static_cast<uint64_t>(c.values_bytes()), scales_v = address(c.v) + static_cast<uint64_t>(c.values_bytes());
-            int width = static_cast<int>(batch.table_width), chunks = 0, longest = 0;
+            int width = static_cast<int>(batch.table_width), chunks = 0, longest = 0, pool_rows = static_cast<int>(c.pages * c.heads * c.page_size);
             int64_t q_seq = x.strides[0], q_head = x.strides[1];
             {
-                void* params[] = {&c.map_k, &c.map_v, &queries, &rows, &batch.tables_at, &work, &out.ptr, &partial, &ml,
-                                  &none, &none, &width, &group, &chunks, &q_seq, &q_head, &longest, &scale2, &err, &scales_k, &scales_v};
                 std::scoped_lock lock{c.order};
                 order_read(*cuda_jit::buffer_access::state(c.k), stream);
                 order_read(*cuda_jit::buffer_access::state(c.v), stream);
-                op_launch(attention, device, stream, {static_cast<uint32_t>(plan.ctas), 1, 1}, 160, params);
+                if (prefix != nullptr) {
+                    void* params[] = {&c.map_k, &c.map_v, &queries, &rows1,  &batch.tables_at, &work1,     &partial1, &ml1,
+                                      &width,   &group,   &q_seq,   &q_head, &pool_rows,       &scale2,    &err};
+                    op_launch(*prefix, device, stream, {static_cast<uint32_t>(plan.prefix.ctas), 1, 1}, 512, params);
+                }
+                if (rest != nullptr) {
+                    void* params[] = {&c.map_k, &c.map_v, &queries, &rows2, &batch.tables_at, &work2, &out.ptr, &partial2, &ml2, &none, &none,
+                                      &width,   &group,   &chunks,  &q_seq, &q_head, &longest, &scale2, &err, &scales_k, &scales_v};
+                    op_launch(*rest, device, stream, {static_cast<uint32_t>(plan.rest.ctas), 1, 1}, 160, params);
+                }
             }
-            void* params[] = {&outs, &parts, &partial, &ml, &partial, &ml, &out.ptr, &group, &per, &per};
+            // Without a stage of their own the prefixes' parts are among the others.
+            if (prefix == nullptr) {
+                partial1 = partial2;
+                ml1 = ml2;
+            }
+            int per1 = plan.prefix.per, per2 = plan.rest.per;
+            void* params[] = {&outs, &parts, &partial1, &ml1, &partial2, &ml2, &out.ptr, &group, &per1, &per2};
             op_launch(finishing, device, stream, {static_cast<uint32_t>(x.shape[0] * x.shape[1]), 1, 1},
                       static_cast<uint32_t>(f.join_threads), params);
             return finish(std::move(out));

@@ -213,6 +213,29 @@ def test_from_several_threads(gpu):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("mode", [1, 2])
+def test_waits_that_run_out_are_reported_and_the_gpu_recovers(gpu, mode):
+    # Mode 1: the first CTA multiplies nothing, so its other roles' waits run out;
+    # 2: its softmax gives up at once, while loads and products are on their way.
+    from porch_b200._lib import lib
+
+    rng = np.random.default_rng(6)
+    host = Shared(rng, [(30, 1024)], [1100] * 30, 2, 128, 64, "bf16")
+    _, batch = host.build(gpu)
+    q = rng.normal(0, 1, (30, 4, 128)).astype(np.float32)
+    t = gpu.tensor([30, 4, 128], q)
+    want = gpu.paged_attention(t, batch).cpu()
+    assert lib().pb_test_attention_stall(mode) == 0
+    try:
+        with pytest.raises(RuntimeError, match="kernel error code"):
+            gpu.paged_attention(t, batch).cpu()
+    finally:
+        assert lib().pb_test_attention_stall(0) == 0
+    for _ in range(2):
+        assert np.array_equal(gpu.paged_attention(t, batch).cpu(), want)
+
+
+@pytest.mark.gpu
 def test_refusals(gpu):
     cache = gpu.KVCache(20, 16, 2, 64, dtype="bf16")
     tables = np.array([[0, 1, 2, 5], [0, 1, 3, 6], [0, 4, 7, 8]])
