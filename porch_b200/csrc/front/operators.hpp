@@ -251,8 +251,9 @@ namespace porch::detail {
     void prefix_attention_sources(kernel_list& out);
 
     // Whether there is a kernel of 128 queries a row for prefixes in this cache
-    // (bfloat16, head_dim up to 128), and that kernel: 512 threads, a CTA an SM.
+    // (bfloat16, head_dim up to 128), and that kernel: 384 threads, a CTA an SM;
+    // `wide`: every query's row starts on 16 bytes.
     bool prefix_attention_takes(const kv_cache& c);
-    op_kernel& prefix_attention_kernel(const kv_cache& c, int stall);
+    op_kernel& prefix_attention_kernel(const kv_cache& c, bool wide, int stall);
 
 } // namespace porch::detail

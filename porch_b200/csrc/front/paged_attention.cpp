@@ -944,11 +944,12 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
 // `rows`; a sequence's key head is {its first row, the prefix's first row (-1
 // where there is none), its first query's place among those that read the
 // prefix}. Block: one query head, as pb_join's; `h1`, `h2`: queries of a row of
-// the prefix and of a sequence.
+// the prefix and of a sequence. A prefix's own stage leaves two sums for each of
+// its queries, and results four channels of all queries side by side (`own`).
 #define PB_JOIN (PB_JOIN_THREADS / (PB_D / 4))
 extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_shared_finish(
     const int4* outs, const int2* rows, const float* partial1, const float2* ml1, const float* partial2, const float2* ml2,
-    float* out, int group, int h1, int h2) {
+    float* out, int group, int h1, int h2, int own) {
     __shared__ float weight[PB_JOIN_THREADS], reduce[16];
     __shared__ float4 sums[PB_JOIN_THREADS];
     const int head = blockIdx.x % group;
@@ -960,20 +961,32 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_shared_finish(
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int parts = r1.y + r2.y;
     if (parts == 0) return; // already there
-    const float* p1 = partial1 + ((pb_i64)r1.x * h1 + f % h1) * PB_D;
+    const float* p1 = partial1 + (pb_i64)r1.x * h1 * PB_D + (own ? f % h1 * 4 : f % h1 * PB_D);
     const float* p2 = partial2 + ((pb_i64)r2.x * h2 + head % h2) * PB_D;
-    auto row = [&](int i) { return i < r1.y ? p1 + (pb_i64)i * h1 * PB_D : p2 + (pb_i64)(i - r1.y) * h2 * PB_D; };
     const int lane = threadIdx.x & 31, quad = threadIdx.x % (PB_D / 4), team = threadIdx.x / (PB_D / 4);
+    const int step1 = own ? 4 * h1 : 4; // from quad to quad
+    auto result = [&](int i) {
+        return *reinterpret_cast<const float4*>(i < r1.y ? p1 + (pb_i64)i * h1 * PB_D + quad * step1
+                                                         : p2 + (pb_i64)(i - r1.y) * h2 * PB_D + quad * 4);
+    };
     float top = PB_LOWEST, sum = 0.0f;
     float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     for (int from = 0; from < parts; from += PB_JOIN_THREADS) {
         const int n = min(PB_JOIN_THREADS, parts - from), i = from + threadIdx.x;
         float2 ml = make_float2(PB_LOWEST, 0.0f);
-        if (threadIdx.x < n) ml = i < r1.y ? ml1[((pb_i64)r1.x + i) * h1 + f % h1] : ml2[((pb_i64)r2.x + i - r1.y) * h2 + head % h2];
+        if (threadIdx.x < n) {
+            if (i < r1.y) {
+                const float2* at = ml1 + (pb_i64)(r1.x + i) * (1 + own) * h1 + f % h1;
+                ml = at[0];
+                if (own) ml.y += at[h1].y;
+            } else {
+                ml = ml2[((pb_i64)r2.x + i - r1.y) * h2 + head % h2];
+            }
+        }
         float4 early[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-            if (team < PB_JOIN && team + e * PB_JOIN < n) early[e] = *(reinterpret_cast<const float4*>(row(from + team + e * PB_JOIN)) + quad);
+            if (team < PB_JOIN && team + e * PB_JOIN < n) early[e] = result(from + team + e * PB_JOIN);
         float x = ml.x;
 #pragma unroll
         for (int m = 16; m > 0; m /= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, m));
@@ -1010,7 +1023,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_shared_finish(
                 if (team + e * PB_JOIN < n) add(early[e], weight[team + e * PB_JOIN]);
 #pragma unroll 4
             for (int j = team + 2 * PB_JOIN; j < n; j += PB_JOIN)
-                add(*(reinterpret_cast<const float4*>(row(from + j)) + quad), weight[j]);
+                add(result(from + j), weight[j]);
         }
     }
     sums[threadIdx.x] = acc;
@@ -1442,7 +1455,8 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
                 for (int64_t f0 = 0; f0 < queries; f0 += per)
                     for (int64_t v : {seq, h, begin, end, first, f0, std::min(per, queries - f0), int64_t{0}})
                         rows.push_back(static_cast<int32_t>(v));
-                if (end > begin) tiles.insert(tiles.end(), static_cast<size_t>((queries + per - 1) / per), (end - begin + 63) / 64);
+                const int64_t tile = per == 128 ? 128 : 64; // slots
+                if (end > begin) tiles.insert(tiles.end(), static_cast<size_t>((queries + per - 1) / per), (end - begin + tile - 1) / tile);
                 return row;
             };
             std::vector<int64_t> begin(static_cast<size_t>(n), 0);
@@ -1528,9 +1542,9 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             // Workspace: the parts' results, and their maxima and sums; the prefixes' first.
             const size_t heads1 = static_cast<size_t>(plan.prefix.parts * plan.prefix.per), heads2 = static_cast<size_t>(plan.rest.parts * plan.rest.per);
             const size_t dim = static_cast<size_t>(c.dim);
-            cuda_jit::device_buffer scratch = allocate(device, (heads1 + heads2) * (dim + 2) * sizeof(float), stream);
-            uint64_t partial1 = address(scratch), partial2 = partial1 + heads1 * dim * 4, ml1 = partial2 + heads2 * dim * 4, ml2 = ml1 + heads1 * 8;
-            op_kernel* prefix = plan.prefix.ctas > 0 ? &prefix_attention_kernel(c, f.stall) : nullptr;
+            cuda_jit::device_buffer scratch = allocate(device, (heads1 * (dim + 4) + heads2 * (dim + 2)) * sizeof(float), stream);
+            uint64_t partial1 = address(scratch), partial2 = partial1 + heads1 * dim * 4, ml1 = partial2 + heads2 * dim * 4, ml2 = ml1 + heads1 * 16;
+            op_kernel* prefix = plan.prefix.ctas > 0 ? &prefix_attention_kernel(c, vector_width(x) == 4, f.stall) : nullptr;
             op_kernel* rest = plan.rest.ctas > 0 ? &kernel_of(kAttention, f, static_cast<uint32_t>(f.smem())) : nullptr;
             if (plan.most_parts > 16) f.join_threads = 512;
             op_kernel& finishing = kernel_of(kSharedFinish, f, 0);
@@ -1553,7 +1567,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
                 if (prefix != nullptr) {
                     void* params[] = {&c.map_k, &c.map_v, &queries, &rows1,  &batch.tables_at, &work1,     &partial1, &ml1,
                                       &width,   &group,   &q_seq,   &q_head, &pool_rows,       &scale2,    &err};
-                    op_launch(*prefix, device, stream, {static_cast<uint32_t>(plan.prefix.ctas), 1, 1}, 512, params);
+                    op_launch(*prefix, device, stream, {static_cast<uint32_t>(plan.prefix.ctas), 1, 1}, 384, params);
                 }
                 if (rest != nullptr) {
                     void* params[] = {&c.map_k, &c.map_v, &queries, &rows2, &batch.tables_at, &work2, &out.ptr, &partial2, &ml2, &none, &none,
@@ -1566,8 +1580,8 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
                 partial1 = partial2;
                 ml1 = ml2;
             }
-            int per1 = plan.prefix.per, per2 = plan.rest.per;
-            void* params[] = {&outs, &parts, &partial1, &ml1, &partial2, &ml2, &out.ptr, &group, &per1, &per2};
+            int per1 = plan.prefix.per, per2 = plan.rest.per, own = prefix != nullptr ? 1 : 0;
+            void* params[] = {&outs, &parts, &partial1, &ml1, &partial2, &ml2, &out.ptr, &group, &per1, &per2, &own};
             op_launch(finishing, device, stream, {static_cast<uint32_t>(x.shape[0] * x.shape[1]), 1, 1},
                       static_cast<uint32_t>(f.join_threads), params);
             return finish(std::move(out));
