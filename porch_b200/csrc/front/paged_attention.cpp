@@ -946,10 +946,78 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
 // prefix}. Block: one query head, as pb_join's; `h1`, `h2`: queries of a row of
 // the prefix and of a sequence. A prefix's own stage leaves two sums for each of
 // its queries, and results four channels of all queries side by side (`own`).
+// PB_JOIN_THREADS 32: a warp each for up to 32 parts, four heads a block, which
+// needs no barrier (64 sequences of 32 heads with 11 to 14 parts: FINISH_FEW us,
+// 12.8 with a block each).
+#if PB_JOIN_THREADS == 32
+#define PB_QUADS ((PB_D / 4 + 31) / 32) // of a lane
+extern "C" __global__ void __launch_bounds__(128) pb_shared_finish(
+    const int4* outs, const int2* rows, const float* partial1, const float2* ml1, const float* partial2, const float2* ml2,
+    float* out, int group, int h1, int h2, int own, int heads) {
+    const int lane = threadIdx.x & 31, id = blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (id >= heads) return;
+    const int head = id % group;
+    const int4 o = outs[id / group]; // of the plan, in place before the launch
+    int2 r1 = make_int2(0, 0), r2 = make_int2(0, 0);
+    const int f = o.z + head;
+    if (o.y >= 0) r1 = rows[o.y + f / h1];
+    if (o.x >= 0) r2 = rows[o.x + head / h2];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int parts = r1.y + r2.y;
+    if (parts == 0) return; // already there
+    // Lane i has part i's maximum, sum and place.
+    float2 ml = make_float2(PB_LOWEST, 0.0f);
+    const float* at = partial1;
+    if (lane < r1.y) {
+        const float2* p = ml1 + (pb_i64)(r1.x + lane) * (1 + own) * h1 + f % h1;
+        ml = p[0];
+        if (own) ml.y += p[h1].y;
+        at = partial1 + (pb_i64)(r1.x + lane) * h1 * PB_D + (own ? f % h1 * 4 : f % h1 * PB_D);
+    } else if (lane < parts) {
+        const pb_i64 i = ((pb_i64)r2.x + lane - r1.y) * h2 + head % h2;
+        ml = ml2[i];
+        at = partial2 + i * PB_D;
+    }
+    float top = ml.x;
+#pragma unroll
+    for (int m = 16; m > 0; m /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
+    const float w = lane < parts ? pb_exp2(ml.x - top) : 0.0f;
+    float sum = lane < parts ? w * ml.y : 0.0f;
+#pragma unroll
+    for (int m = 16; m > 0; m /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+    float4 acc[PB_QUADS];
+#pragma unroll
+    for (int c = 0; c < PB_QUADS; ++c) acc[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+    for (int i = 0; i < parts; ++i) {
+        const float v = __shfl_sync(0xffffffffu, w, i);
+        const float* p = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<pb_u64>(at), i));
+        const int step = own && i < r1.y ? 4 * h1 : 4; // from quad to quad
+#pragma unroll
+        for (int c = 0; c < PB_QUADS; ++c) {
+            const int quad = c * 32 + lane;
+            if (quad >= PB_D / 4) continue;
+            const float4 x = *reinterpret_cast<const float4*>(p + (pb_i64)quad * step);
+            acc[c].x = fmaf(v, x.x, acc[c].x);
+            acc[c].y = fmaf(v, x.y, acc[c].y);
+            acc[c].z = fmaf(v, x.z, acc[c].z);
+            acc[c].w = fmaf(v, x.w, acc[c].w);
+        }
+    }
+    const float inv = 1.0f / sum;
+#pragma unroll
+    for (int c = 0; c < PB_QUADS; ++c) {
+        const int quad = c * 32 + lane;
+        if (quad < PB_D / 4)
+            *reinterpret_cast<float4*>(out + (pb_i64)id * PB_D + 4 * quad) =
+                make_float4(acc[c].x * inv, acc[c].y * inv, acc[c].z * inv, acc[c].w * inv);
+    }
+}
+#else
 #define PB_JOIN (PB_JOIN_THREADS / (PB_D / 4))
 extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_shared_finish(
     const int4* outs, const int2* rows, const float* partial1, const float2* ml1, const float* partial2, const float2* ml2,
-    float* out, int group, int h1, int h2, int own) {
+    float* out, int group, int h1, int h2, int own, int) {
     __shared__ float weight[PB_JOIN_THREADS], reduce[16];
     __shared__ float4 sums[PB_JOIN_THREADS];
     const int head = blockIdx.x % group;
@@ -1041,6 +1109,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_shared_finish(
             make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
     }
 }
+#endif
 #else
 // A row in several parts: {row, first CTA, number of parts, the first part's
 // place}. Part i's sums for a query head.
@@ -1369,7 +1438,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             std::vector<int32_t> rows; // per row: its first part, how many
             int64_t parts = 0;
         };
-        constexpr int64_t kRowCost = 3; // of 128 queries: they are split, and results stored
+        constexpr int64_t kRowCost = 2; // of 128 queries: they are split, and results stored
         runs share_out(const std::vector<int64_t>& tiles, int64_t ctas, int64_t extra) {
             runs r;
             int64_t cost = 0;
@@ -1499,11 +1568,17 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
                             for (int32_t v : {static_cast<int32_t>(row - rest_row + i), 0, 0, 0}) r.work.push_back(v);
                     }
             p->rest.ctas = static_cast<int64_t>(r.work.size() / 4);
-            for (int64_t s = 0; s < n; ++s) { // the most parts of a query: of the first head's, others have about as many
+            for (int64_t i = 0; i < n * heads; ++i) { // the most parts of a query
                 int64_t count = 0;
-                for (int64_t i : {0, 1}) {
-                    const int32_t row = outs[static_cast<size_t>(4 * s * heads + i)];
-                    if (row >= 0) count += parts[static_cast<size_t>(2 * row + 1)];
+                for (int64_t of : {0, 1}) {
+                    const int32_t row = outs[static_cast<size_t>(4 * i + of)];
+                    const int64_t skip = of == 1 ? outs[static_cast<size_t>(4 * i + 2)] : 0;
+                    int64_t most = 0;
+                    const int64_t per = of == 1 ? p->prefix.per : p->rest.per;
+                    if (row >= 0)
+                        for (int64_t f = skip / per; f <= (skip + group - 1) / per; ++f)
+                            most = std::max<int64_t>(most, parts[static_cast<size_t>(2 * (row + f) + 1)]);
+                    count += most;
                 }
                 p->most_parts = std::max(p->most_parts, count);
             }
@@ -1546,7 +1621,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             uint64_t partial1 = address(scratch), partial2 = partial1 + heads1 * dim * 4, ml1 = partial2 + heads2 * dim * 4, ml2 = ml1 + heads1 * 16;
             op_kernel* prefix = plan.prefix.ctas > 0 ? &prefix_attention_kernel(c, vector_width(x) == 4, f.stall) : nullptr;
             op_kernel* rest = plan.rest.ctas > 0 ? &kernel_of(kAttention, f, static_cast<uint32_t>(f.smem())) : nullptr;
-            if (plan.most_parts > 16) f.join_threads = 512;
+            f.join_threads = plan.most_parts <= 32 ? 32 : 512;
             op_kernel& finishing = kernel_of(kSharedFinish, f, 0);
             if (prefix != nullptr) (void)prefix->on(device);
             if (rest != nullptr) (void)rest->on(device);
@@ -1581,9 +1656,12 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
                 ml1 = ml2;
             }
             int per1 = plan.prefix.per, per2 = plan.rest.per, own = prefix != nullptr ? 1 : 0;
-            void* params[] = {&outs, &parts, &partial1, &ml1, &partial2, &ml2, &out.ptr, &group, &per1, &per2, &own};
-            op_launch(finishing, device, stream, {static_cast<uint32_t>(x.shape[0] * x.shape[1]), 1, 1},
-                      static_cast<uint32_t>(f.join_threads), params);
+            int heads = static_cast<int>(x.shape[0] * x.shape[1]);
+            void* params[] = {&outs, &parts, &partial1, &ml1, &partial2, &ml2, &out.ptr, &group, &per1, &per2, &own, &heads};
+            if (f.join_threads == 32)
+                op_launch(finishing, device, stream, {static_cast<uint32_t>((heads + 3) / 4), 1, 1}, 128, params);
+            else
+                op_launch(finishing, device, stream, {static_cast<uint32_t>(heads), 1, 1}, 512, params);
             return finish(std::move(out));
         }
 

@@ -344,13 +344,15 @@ extern "C" __global__ void __launch_bounds__(384, 1) pb_prefix_attention(
             // the head size and the row's queries. MMAs of the row before have
             // completed: its last O was waited for. Every load before the first use.
             {
-                constexpr int pieces = 128 * PB_PLANES * 16 / 256; // of a thread
+                constexpr int pieces = 128 * PB_PLANES * 16 / 256; // of a thread, every 8th or 16th row
                 float4 x[pieces];
+                const int r0 = (threadIdx.x - 128) / (PB_PLANES * 16), c = (threadIdx.x - 128) % (PB_PLANES * 16) * 4;
+                int member = (a.f0 + r0) / group, head = (a.f0 + r0) % group;
+                const int members = 16 / PB_PLANES / group, heads = 16 / PB_PLANES % group;
 #pragma unroll
                 for (int u = 0; u < pieces; ++u) {
-                    const int e = threadIdx.x - 128 + u * 256, r = e / (PB_PLANES * 16), c = e % (PB_PLANES * 16) * 4;
-                    const int f = a.f0 + min(r, a.count - 1), member = f / group;
-                    const float* src = q + (a.first + member) * q_seq + (a.h * group + f - member * group) * q_head + c;
+                    const int r = r0 + u * (16 / PB_PLANES);
+                    const float* src = q + (a.first + member) * q_seq + (a.h * group + head) * q_head + c;
                     x[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     if (r < a.count && c < PB_D) // head sizes are whole pieces
 #if PB_WIDE
@@ -358,10 +360,16 @@ extern "C" __global__ void __launch_bounds__(384, 1) pb_prefix_attention(
 #else
                         x[u] = make_float4(__ldg(src), __ldg(src + 1), __ldg(src + 2), __ldg(src + 3));
 #endif
+                    member += members;
+                    head += heads;
+                    if (head >= group) {
+                        head -= group;
+                        ++member;
+                    }
                 }
 #pragma unroll
                 for (int u = 0; u < pieces; ++u) {
-                    const int e = threadIdx.x - 128 + u * 256, r = e / (PB_PLANES * 16), c = e % (PB_PLANES * 16) * 4;
+                    const int r = r0 + u * (16 / PB_PLANES);
                     x[u].x *= scale2;
                     x[u].y *= scale2;
                     x[u].z *= scale2;
