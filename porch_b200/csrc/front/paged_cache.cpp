@@ -156,13 +156,15 @@ extern "C" __global__ void __launch_bounds__(256) pb_cache_append(
 typedef long long pb_i64;
 // Block: PB_TOKENS slots, keys and values of every head, as float32 (which holds
 // a bfloat16 value, and 8 bits times their scale rounded once). Its first threads
-// find the sequence and row of one slot each; the rest is copying, four values a
-// thread and PB_EACH of those on the way at once. Bound by HBM.
-#define PB_QUADS (PB_TOKENS * PB_H * (PB_D / 4))
+// find the sequence and row of one slot each; then a thread copies its four
+// channels of one row after the other, PB_EACH of them on the way at once. Bound
+// by HBM (READ_BOUND).
+#define PB_QUADS (PB_D / 4)
+#define PB_ROWS (256 / PB_QUADS) // at once
 extern "C" __global__ void __launch_bounds__(256) pb_cache_read(
     const char* pk, const char* pv, const int* tables, const pb_i64* starts, float* ok, float* ov, int sequences, int width,
     pb_i64 scales) {
-    __shared__ pb_i64 rows[PB_TOKENS]; // of head 0
+    __shared__ int rows[PB_TOKENS]; // of head 0, below 2^31
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const pb_i64 first = (pb_i64)blockIdx.x * PB_TOKENS;
     const int n = (int)min((pb_i64)PB_TOKENS, starts[sequences] - first);
@@ -174,38 +176,59 @@ extern "C" __global__ void __launch_bounds__(256) pb_cache_read(
             if (starts[middle] <= t) low = middle; else high = middle - 1;
         }
         const int slot = (int)(t - starts[low]);
-        rows[threadIdx.x] = (pb_i64)tables[(pb_i64)low * width + slot / PB_PS] * PB_H * PB_PS + slot % PB_PS;
+        rows[threadIdx.x] = tables[(pb_i64)low * width + slot / PB_PS] * (PB_H * PB_PS) + slot % PB_PS;
     }
     __syncthreads();
-    const int quads = n * PB_H * (PB_D / 4);
-    for (int base = threadIdx.x; base < 2 * quads; base += 256 * PB_EACH) {
-        float4 x[PB_EACH];
-#pragma unroll
-        for (int j = 0; j < PB_EACH; ++j) {
-            const int id = base + j * 256;
-            if (id >= 2 * quads) break;
-            const int q = id < quads ? id : id - quads, c = q % (PB_D / 4), h = q / (PB_D / 4) % PB_H;
-            const char* pool = id < quads ? pk : pv;
-            const pb_i64 row = rows[q / (PB_D / 4 * PB_H)] + h * PB_PS;
+    const int quad = threadIdx.x % PB_QUADS, start = threadIdx.x / PB_QUADS, end = n * PB_H;
+    if (start >= PB_ROWS) return;
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which) {
+        const char* pool = which ? pv : pk;
+        float4* to = reinterpret_cast<float4*>((which ? ov : ok) + first * PB_H * PB_D) + quad;
+#pragma unroll 1
+        for (int base = start; base < end; base += PB_ROWS * PB_EACH) {
 #if PB_I8
-            const pb_u32 w = __ldcs(reinterpret_cast<const pb_u32*>(pool + row * PB_D + 4 * c));
-            const float s = __ldg(reinterpret_cast<const float*>(pool + scales) + row);
-            x[j] = make_float4((float)(signed char)(w & 255u) * s, (float)(signed char)(w >> 8 & 255u) * s,
-                               (float)(signed char)(w >> 16 & 255u) * s, (float)(signed char)(w >> 24) * s);
+            pb_u32 x[PB_EACH];
+            float scale[PB_EACH];
 #elif PB_BF16
-            const uint2 w = __ldcs(reinterpret_cast<const uint2*>(pool + (row * PB_D + 4 * c) * 2));
-            x[j] = make_float4(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xffff0000u),
-                               __uint_as_float(w.y << 16), __uint_as_float(w.y & 0xffff0000u));
+            uint2 x[PB_EACH];
 #else
-            x[j] = __ldcs(reinterpret_cast<const float4*>(pool + (row * PB_D + 4 * c) * 4));
+            float4 x[PB_EACH];
 #endif
-        }
 #pragma unroll
-        for (int j = 0; j < PB_EACH; ++j) {
-            const int id = base + j * 256;
-            if (id >= 2 * quads) break;
-            const int q = id < quads ? id : id - quads;
-            __stcs(reinterpret_cast<float4*>((id < quads ? ok : ov) + first * PB_H * PB_D) + q, x[j]);
+            for (int j = 0; j < PB_EACH; ++j) { // every load before the first use
+                const int r = min(base + j * PB_ROWS, end - 1);
+                const pb_i64 row = rows[r / PB_H] + r % PB_H * PB_PS;
+#if PB_I8
+                x[j] = __ldcs(reinterpret_cast<const pb_u32*>(pool + row * PB_D + 4 * quad));
+                scale[j] = __ldg(reinterpret_cast<const float*>(pool + scales) + row);
+#elif PB_BF16
+                x[j] = __ldcs(reinterpret_cast<const uint2*>(pool + (row * PB_D + 4 * quad) * 2));
+#else
+                x[j] = __ldcs(reinterpret_cast<const float4*>(pool + (row * PB_D + 4 * quad) * 4));
+#endif
+            }
+#pragma unroll
+            for (int j = 0; j < PB_EACH; ++j) {
+                const int r = base + j * PB_ROWS;
+                if (r >= end) break;
+#if PB_I8
+                // A byte with its sign flipped in the low bits of 2^23 is 2^23 + 128
+                // + the code; conversions run at a quarter of the rate of this.
+                const pb_u32 w = x[j] ^ 0x80808080u;
+                const float s = scale[j];
+                const float4 y = make_float4((__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440)) - 8388736.0f) * s,
+                                             (__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7441)) - 8388736.0f) * s,
+                                             (__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7442)) - 8388736.0f) * s,
+                                             (__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7443)) - 8388736.0f) * s);
+#elif PB_BF16
+                const float4 y = make_float4(__uint_as_float(x[j].x << 16), __uint_as_float(x[j].x & 0xffff0000u),
+                                             __uint_as_float(x[j].y << 16), __uint_as_float(x[j].y & 0xffff0000u));
+#else
+                const float4 y = x[j];
+#endif
+                __stcs(to + (pb_i64)r * PB_QUADS, y);
+            }
         }
     }
 }
