@@ -95,14 +95,19 @@ static __device__ __forceinline__ pb_u32 pb_peer(const void* p, pb_u32 rank) {
 #if PB_TOP
 // A logit and its token as one number that orders as alternatives do: larger
 // logits first (NaN last), of equal ones the lower token. 0 is no entry.
-static __device__ __forceinline__ pb_u64 pb_key(float x, pb_u32 token) {
+static __device__ __forceinline__ pb_u32 pb_order(float x) {
     const pb_u32 u = __float_as_uint(x + 0.0f); // -0 becomes 0
-    const pb_u32 k = x == x ? (u & 0x80000000u ? ~u : u | 0x80000000u) : 1u;
-    return (pb_u64)k << 32 | (0xffffffffu - token);
+    return x == x ? (u & 0x80000000u ? ~u : u | 0x80000000u) : 1u;
+}
+// -inf for NaN and for no entry.
+static __device__ __forceinline__ float pb_unorder(pb_u32 k) {
+    return k <= 1u ? __int_as_float(0xff800000) : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+}
+static __device__ __forceinline__ pb_u64 pb_key(float x, pb_u32 token) {
+    return (pb_u64)pb_order(x) << 32 | (0xffffffffu - token);
 }
 static __device__ __forceinline__ float pb_logit(pb_u64 key) {
-    const pb_u32 k = (pb_u32)(key >> 32);
-    return k <= 1u ? PB_NAN : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
+    return (pb_u32)(key >> 32) <= 1u ? PB_NAN : pb_unorder((pb_u32)(key >> 32));
 }
 // A warp's list: the largest keys so far in falling order, one a lane.
 static __device__ __forceinline__ void pb_insert(pb_u64& list, pb_u64 key, int lane) {
@@ -112,29 +117,42 @@ static __device__ __forceinline__ void pb_insert(pb_u64& list, pb_u64 key, int l
 }
 // The 32 largest of two such lists: the larger of entry i and the other's entry
 // 31 - i, which rise and then fall, sorted by halving distances.
-static __device__ __forceinline__ pb_u64 pb_merge(pb_u64 a, pb_u64 b, int lane) {
-    const pb_u64 r = __shfl_xor_sync(0xffffffffu, b, 31);
+template <typename T>
+static __device__ __forceinline__ T pb_merge(T a, T b, int lane) {
+    const T r = __shfl_xor_sync(0xffffffffu, b, 31);
     a = a > r ? a : r;
 #pragma unroll
     for (int m = 16; m > 0; m /= 2) {
-        const pb_u64 o = __shfl_xor_sync(0xffffffffu, a, m);
+        const T o = __shfl_xor_sync(0xffffffffu, a, m);
         a = ((lane & m) == 0) == (a > o) ? a : o;
     }
     return a;
 }
 // Sorts one key a lane, falling.
-static __device__ __forceinline__ pb_u32 pb_sorted(pb_u32 a, int lane) {
+template <typename T>
+static __device__ __forceinline__ T pb_sorted(T a, int lane) {
 #pragma unroll
     for (int size = 2; size <= 32; size *= 2)
 #pragma unroll
         for (int m = size / 2; m > 0; m /= 2) {
-            const pb_u32 o = __shfl_xor_sync(0xffffffffu, a, m);
+            const T o = __shfl_xor_sync(0xffffffffu, a, m);
             const bool keep_larger = ((lane & m) == 0) == ((lane & size) == 0);
-            a = keep_larger ? max(a, o) : min(a, o);
+            a = keep_larger == (a > o) ? a : o;
         }
     return a;
 }
 #endif
+
+// A thread's 16 logits of the round at vector `base`; -inf outside the run and the row.
+static __device__ __forceinline__ void pb_load(float* v, const float* x, pb_i64 base, pb_i64 last, pb_i64 shift, pb_i64 V, bool on) {
+    const float none = __int_as_float(0xff800000);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        const pb_i64 j = base + q * PB_THREADS + threadIdx.x;
+        const float4 f = on && j < last ? pb_four(x, 4 * j - shift, V, none) : make_float4(none, none, none, none);
+        v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
+    }
+}
 
 // Cluster: one row, each CTA a run of `run` vectors of it.
 extern "C" __global__ void __launch_bounds__(PB_THREADS, 1024 / PB_THREADS) pb_token_logprobs(
@@ -143,9 +161,8 @@ extern "C" __global__ void __launch_bounds__(PB_THREADS, 1024 / PB_THREADS) pb_t
     __shared__ float sums[PB_WARPS][3];
 #if PB_TOP
     __shared__ pb_u64 lists[PB_WARPS][32];
-    __shared__ pb_u32 floor_key; // no logit below it is one of the row's `top` largest
-    if (threadIdx.x == 0) floor_key = 0;
-    __syncthreads();
+    __shared__ pb_u32 groups[PB_THREADS];
+    __shared__ int listed;
 #endif
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const pb_u32 row = blockIdx.x / PB_CLUSTER, rank = PB_CLUSTER > 1 ? pb_rank() : 0;
@@ -155,19 +172,14 @@ extern "C" __global__ void __launch_bounds__(PB_THREADS, 1024 / PB_THREADS) pb_t
     const pb_i64 vectors = (V + shift + 3) >> 2, first = (pb_i64)rank * run, last = min(vectors, first + run);
     pb_sums a = {PB_LOWEST, 0.0f, 0.0f};
 #if PB_TOP
-    pb_u64 list = 0, least = 0; // least: the list's entry `top` - 1
+    // This lane's largest of a round, that round, and the largest of the others.
+    float m1 = __int_as_float(0xff800000), m2 = m1;
+    pb_i64 b1 = first;
 #endif
 #pragma unroll 1
     for (pb_i64 base = first; base < last; base += 4 * PB_THREADS) {
         float v[16];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const pb_i64 j = base + q * PB_THREADS + threadIdx.x;
-            const float4 f = j < last ? pb_four(x, 4 * j - shift, V, __int_as_float(0xff800000))
-                                      : make_float4(__int_as_float(0xff800000), __int_as_float(0xff800000),
-                                                    __int_as_float(0xff800000), __int_as_float(0xff800000));
-            v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
-        }
+        pb_load(v, x, base, last, shift, V, true);
         float most = v[0];
 #pragma unroll
         for (int e = 1; e < 16; ++e) most = fmaxf(most, v[e]);
@@ -182,39 +194,73 @@ extern "C" __global__ void __launch_bounds__(PB_THREADS, 1024 / PB_THREADS) pb_t
         a.s += s[0] + s[1];
         a.w += w[0] + w[1];
 #if PB_TOP
-        // A lane's largest of 16 stands for one logit at least, so the `top`-th
-        // largest of 32 lanes' is a floor for all; the warps of a CTA share the
-        // highest that any of them found.
-        if (base == first) {
-            const pb_u32 mine = (pb_u32)(pb_key(most, 0) >> 32);
-            const pb_u32 bound = __shfl_sync(0xffffffffu, pb_sorted(mine, lane), top - 1);
-            if (lane == 0) atomicMax(&floor_key, bound);
-            __syncwarp();
-        }
-        pb_u32 bound = max(*reinterpret_cast<volatile pb_u32*>(&floor_key), (pb_u32)(least >> 32));
-        // As a float: what is below it (never NaN) is passed over.
-        const float low = bound <= 1u ? __int_as_float(0xff800000) : __uint_as_float(bound & 0x80000000u ? bound & 0x7fffffffu : ~bound);
-        if (__any_sync(0xffffffffu, !(most < low))) {
-            bool grew = false;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const pb_i64 at = 4 * (base + (e >> 2) * PB_THREADS + threadIdx.x) - shift + (e & 3);
-                const bool in = base + (e >> 2) * PB_THREADS + threadIdx.x < last && at >= 0 && at < V;
-                pb_u64 key = in && !(v[e] < low) ? pb_key(v[e], (pb_u32)at) : 0;
-                pb_u32 wanting = __ballot_sync(0xffffffffu, key > least);
-                while (wanting != 0) {
-                    const int from = __ffs(wanting) - 1;
-                    pb_insert(list, __shfl_sync(0xffffffffu, key, from), lane);
-                    least = __shfl_sync(0xffffffffu, list, top - 1);
-                    wanting = (wanting & (wanting - 1)) & __ballot_sync(0xffffffffu, key > least);
-                    grew = true;
-                }
-            }
-            if (grew && lane == 0) atomicMax(&floor_key, (pb_u32)(least >> 32));
-            __syncwarp();
-        }
+        if (most > m1) { m2 = m1; m1 = most; b1 = base; }
+        else m2 = fmaxf(m2, most);
 #endif
     }
+#if PB_TOP
+    // The alternatives. The largest of a group of logits stands for one of them, so
+    // the `top`-th largest of 64 groups' is a floor for all; with the CTA's logits
+    // in 64 groups some 24 lie at or above it for 20 alternatives and 44 for 32,
+    // whatever their number. The lanes that have some look at them once more (where the largest of
+    // a lane's other rounds is below the floor, at one round alone) and list them;
+    // NaN is none. The list is then sorted, 32 a warp. Only where it is too long,
+    // as of a row of equal logits, they are inserted one by one.
+    pb_u64 list = 0;
+    int lists_used = 0;
+    if (last > first) { // the same for the whole CTA
+        groups[threadIdx.x] = pb_order(m1);
+        if (threadIdx.x == 0) listed = 0;
+        __syncthreads();
+        pb_u32 mine[2] = {0, 0};
+#pragma unroll
+        for (int w = 0; w < PB_WARPS; ++w) mine[w & 1] = max(mine[w & 1], groups[w * 32 + lane]);
+        const pb_u32 largest = pb_merge(pb_sorted(mine[0], lane), pb_sorted(mine[1], lane), lane);
+        const float low = pb_unorder(__shfl_sync(0xffffffffu, largest, top - 1));
+        if (m1 >= low)
+            for (pb_i64 base = m2 >= low ? first : b1; base < last; base += 4 * PB_THREADS) {
+                float v[16];
+                pb_load(v, x, base, last, shift, V, true);
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (v[e] >= low) {
+                        const pb_i64 j = base + (e >> 2) * PB_THREADS + threadIdx.x, at = 4 * j - shift + (e & 3);
+                        if (j < last && at >= 0 && at < V) {
+                            const int place = atomicAdd(&listed, 1);
+                            if (place < PB_THREADS) lists[place / 32][place % 32] = pb_key(v[e], (pb_u32)at);
+                        }
+                    }
+                if (m2 < low) break;
+            }
+        __syncthreads();
+        const int count = listed;
+        if (count <= PB_THREADS) {
+            lists_used = (count + 31) / 32;
+            if (warp < lists_used) list = pb_sorted(32 * warp + lane < count ? lists[warp][lane] : 0, lane);
+        } else {
+            lists_used = PB_WARPS;
+            pb_u64 least = 0; // the list's entry `top` - 1
+#pragma unroll 1
+            for (pb_i64 base = first; base < last; base += 4 * PB_THREADS) {
+                float v[16];
+                pb_load(v, x, base, last, shift, V, m1 >= low);
+#pragma unroll 1
+                for (int e = 0; e < 16; ++e) {
+                    float y = v[0];
+#pragma unroll
+                    for (int i = 1; i < 16; ++i) y = i == e ? v[i] : y;
+                    const pb_i64 j = base + (e >> 2) * PB_THREADS + threadIdx.x, at = 4 * j - shift + (e & 3);
+                    const pb_u64 key = y >= low && j < last && at >= 0 && at < V ? pb_key(y, (pb_u32)at) : 0;
+                    for (pb_u32 wanting = __ballot_sync(0xffffffffu, key > least); wanting != 0;) {
+                        pb_insert(list, __shfl_sync(0xffffffffu, key, __ffs(wanting) - 1), lane);
+                        least = __shfl_sync(0xffffffffu, list, top - 1);
+                        wanting = (wanting & (wanting - 1)) & __ballot_sync(0xffffffffu, key > least);
+                    }
+                }
+            }
+        }
+    }
+#endif
     asm volatile("griddepcontrol.launch_dependents;");
 #pragma unroll
     for (int m = 16; m > 0; m /= 2) {
@@ -224,12 +270,12 @@ extern "C" __global__ void __launch_bounds__(PB_THREADS, 1024 / PB_THREADS) pb_t
     }
     if (lane == 0) { sums[warp][0] = a.m; sums[warp][1] = a.s; sums[warp][2] = a.w; }
 #if PB_TOP
+    __syncthreads();
     lists[warp][lane] = list;
     // The lists in pairs, pairs of pairs, ...
-#pragma unroll
-    for (int m = 1; m < PB_WARPS; m *= 2) {
+    for (int m = 1; m < lists_used; m *= 2) {
         __syncthreads();
-        if (warp % (2 * m) == 0) {
+        if (warp % (2 * m) == 0 && warp + m < lists_used) {
             list = pb_merge(list, lists[warp + m][lane], lane);
             lists[warp][lane] = list;
         }
@@ -272,14 +318,24 @@ extern "C" __global__ void __launch_bounds__(PB_THREADS, 1024 / PB_THREADS) pb_t
         }
 #if PB_TOP
 #if PB_CLUSTER > 1
-        pb_u64 other[PB_CLUSTER - 1];
+        pb_u64 of[PB_CLUSTER];
+        of[0] = list;
 #pragma unroll
         for (int c = 1; c < PB_CLUSTER; ++c)
-            other[c - 1] = (pb_u64)pb_peer(reinterpret_cast<const pb_u32*>(&lists[0][lane]) + 1, c) << 32 |
-                           pb_peer(&lists[0][lane], c);
+            of[c] = (pb_u64)pb_peer(reinterpret_cast<const pb_u32*>(&lists[0][lane]) + 1, c) << 32 | pb_peer(&lists[0][lane], c);
 #pragma unroll
-        for (int c = 1; c < PB_CLUSTER; ++c) list = pb_merge(list, other[c - 1], lane);
+        for (int m = 1; m < PB_CLUSTER; m *= 2)
+#pragma unroll
+            for (int c = 0; c < PB_CLUSTER; c += 2 * m) of[c] = pb_merge(of[c], of[c + m], lane);
+        list = of[0];
 #endif
+        // Fewer numbers than alternatives: NaN comes last, in order.
+        if (__shfl_sync(0xffffffffu, list, top - 1) == 0)
+            for (pb_i64 i = 0; i < V; i += 32) {
+                const float y = i + lane < V ? __ldg(x + i + lane) : 0.0f;
+                for (pb_u32 nans = __ballot_sync(0xffffffffu, y != y); nans != 0; nans &= nans - 1)
+                    pb_insert(list, pb_key(PB_NAN, (pb_u32)(i + __ffs(nans) - 1)), lane);
+            }
         if (lane < top) {
             top_said[(pb_i64)row * top + lane] = (pb_logit(list) - a.m) - log_total;
             top_tokens[(pb_i64)row * top + lane] = (float)(0xffffffffu - (pb_u32)list);
