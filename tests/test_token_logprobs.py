@@ -296,3 +296,32 @@ def test_every_operand_needs_values(gpu, at):
     if at in (1, 2):
         with pytest.raises(RuntimeError, match="placeholder"):
             gpu.token_logprobs(*given[1:3])
+
+
+@pytest.mark.gpu
+def test_gradient_of_many_rows(gpu):
+    # As many as take several rounds a block; every row against the formula.
+    rng = np.random.default_rng(21)
+    rows, vocab = 700, 65539
+    x, tokens = make(rng, rows, vocab)
+    x[:, 60000:] = -np.inf
+    tokens = np.minimum(tokens, 59999)
+    tokens[::7] = -1
+    g, h = (rng.normal(0, 1, rows).astype(np.float32) for _ in range(2))
+    logits, t = gpu.tensor([rows, vocab], x), gpu.tensor([rows], tokens)
+    _, entropy, norm = gpu.token_logprobs(logits, t)
+    got = gpu.token_logprobs_backward(gpu.tensor([rows], g), logits, t, norm, gpu.tensor([rows], h), entropy)
+    got = got.cpu().reshape(rows, vocab)
+    for i in range(0, rows, 13):
+        y, at = x[i : i + 1].astype(np.float64), tokens[i : i + 1]
+        _, ent, m, s, p, logp = define(y, at)
+        off = sum_error(y, m, p)
+        inner = np.where(p > 0, logp + ent, 0)
+        hot = (np.arange(vocab) == at[0]) & (at[0] >= 0)
+        want = (g[i] if at[0] >= 0 else 0.0) * (hot - p) - h[i] * p * inner
+        gap = np.where(p > 0, m - y, 0)
+        p_off = p * (U * gap + 2.0**-22 + 12 * U + off)
+        inner_off = off + (3 * off + 8 * U) * (p * gap).sum() + 6 * U * (gap + ent + 2 * np.log(s) + 1)
+        tol = np.abs(g[i]) * (p_off + 4 * U * (p + hot)) + np.abs(h[i]) * (p_off * np.abs(inner) + p * inner_off + 4 * U * p * np.abs(inner))
+        tol = tol + 2.0**-126 * (1 + np.abs(g[i]) + np.abs(h[i]) * (1 + np.abs(inner)))
+        assert (np.abs(got[i] - want[0]) <= tol[0]).all()
