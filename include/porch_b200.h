@@ -347,8 +347,8 @@ int pb_kv_batch_create(pb_kv_cache* cache, const int32_t* tables, size_t sequenc
 /* The same for sequences that share prefixes: the first prefix[s] slots (whole
  * pages, 0 for none, none of them new) of sequences next to each other that
  * begin on the same page and have the same prefix[s] are one prefix, which
- * pb_paged_attention then works through once for all of them. Their tables name
- * the same pages for it. Without `appended` a sequence that ends with its prefix
+ * pb_paged_attention then works through once for all of them (where that spares
+ * enough reading to pay). Their tables name the same pages for it. Without `appended` a sequence that ends with its prefix
  * has no new token. NULL: as pb_kv_batch_create. */
 int pb_kv_batch_create_shared(pb_kv_cache* cache, const int32_t* tables, size_t sequences, size_t width,
                               const int64_t* lengths, const int64_t* appended, const int64_t* newest,
@@ -428,6 +428,9 @@ int pb_test_gemm_stall(int enable);
  * while its first tiles are on their way (2); the kernel records a code of
  * 0x7d00 and more, and leaves when nothing is in flight any more. */
 int pb_test_attention_stall(int enable);
+/* While enabled, shared prefixes are worked through once whatever their size;
+ * otherwise where that spares enough reading. Only for tests. */
+int pb_test_share_prefix(int enable);
 
 /* ---- matmul without allocation ------------------------------------------ */
 /* C = A @ B in fp32 (3xTF32 on tcgen05), on raw device pointers, allocating

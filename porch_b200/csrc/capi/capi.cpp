@@ -930,6 +930,10 @@ int pb_test_attention_stall(int enable) {
     });
 }
 
+int pb_test_share_prefix(int enable) {
+    return guarded([&] { porch::detail::set_test_share_prefix(enable != 0); });
+}
+
 namespace {
     void copy_text(const std::string& s, char* text, size_t capacity, size_t* needed) {
         if (needed) *needed = s.size() + 1;

@@ -223,6 +223,8 @@ namespace porch::detail {
     // bounded waits expire (1), or gives up while its first ones are on their
     // way (2).
     void set_test_attention_stall(int mode);
+    // Test hook: prefixes are worked through once whatever their size.
+    void set_test_share_prefix(bool on);
     // The plan as text ("work <row> <tile> <tiles>" per CTA, "join <row>
     // <first CTA> <parts> <place>" per row), without a device.
     std::string attention_schedule(const std::vector<int64_t>& lengths, int64_t heads, int64_t chunks, int64_t ctas);

@@ -1313,6 +1313,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         }
 
         std::atomic<int> g_test_stall{0};
+        std::atomic<bool> g_test_share{false};
 
         // The form for `group` query heads of each key head: 16 share a tile's
         // loads, 8 where 16 would leave the ring less than three units.
@@ -1483,6 +1484,20 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             int64_t most = 0;
             for (const auto& g : batch.groups) most = std::max(most, g.members * group);
             return prefix_attention_takes(*batch.cache) && most > 16;
+        }
+
+        // Whether working through the prefixes once pays: it takes up to two launches
+        // more, so where it spares reading less than some 96 MB (most of which the L2
+        // cache would deliver) every sequence reads its prefix itself. 32 query heads
+        // over 8 of 128 bfloat16 channels, shared and by themselves: 16 sequences
+        // behind 1024 slots (63 MB) 17.3 and 15.8 us, 8 behind 4096 (117 MB) 22.2 and
+        // 23.4, 64 behind 512 (132 MB) 21.3 and 26.1, behind 2048 30.9 and 75.0.
+        bool worth_sharing(const kv_batch& batch, int64_t group) {
+            const kv_cache& c = *batch.cache;
+            const int64_t per = prefix_stage(batch, group) ? 128 : 16; // queries that read a prefix together
+            int64_t slots = 0;
+            for (const auto& g : batch.groups) slots += (g.members - (g.members * group + per - 1) / per) * g.slots;
+            return !batch.groups.empty() && (g_test_share.load(std::memory_order_relaxed) || slots * c.heads * 2 * c.dim * c.width() >= 96000000);
         }
 
         // The form of what follows the prefixes, and of prefixes without a stage of
@@ -1692,7 +1707,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         auto stream = current_stream(device);
         op_operand x = operand(q, stream, true), xs;
         if (scores != nullptr) xs = operand(*scores, stream, false);
-        if (!scored && !batch.groups.empty()) {
+        if (!scored && worth_sharing(batch, shape[1] / c.heads)) {
             std::vector<tensor> results;
             results.push_back(shared_attention(x, batch, scale2, stream));
             return results;
@@ -1762,6 +1777,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
     }
 
     void set_test_attention_stall(int mode) { g_test_stall.store(mode); }
+    void set_test_share_prefix(bool on) { g_test_share.store(on); }
 
     std::pair<int, int> attention_shape(int64_t dim, cache_type type, int64_t group) {
         kv_cache c;
@@ -1807,8 +1823,8 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             ctas = batch.plans->hint->ctas;
             group = batch.plans->hint->group;
         }
-        if (!batch.groups.empty()) {
-            (void)shared_plan_of(batch, group != 0 ? group : 1);
+        if (group != 0 && worth_sharing(batch, group)) {
+            (void)shared_plan_of(batch, group);
             return;
         }
         if (chunks == 0) {

@@ -8,6 +8,19 @@ import pytest
 import int8_cache
 
 
+@pytest.fixture(autouse=True)
+def shared(request):
+    """Prefixes are shared at these sizes, too, which the library would not do."""
+    if request.node.get_closest_marker("gpu") is None:
+        yield
+        return
+    from porch_b200._lib import lib
+
+    assert lib().pb_test_share_prefix(1) == 0
+    yield
+    assert lib().pb_test_share_prefix(0) == 0
+
+
 class Shared(int8_cache.Host):
     """Groups of (members, shared slots); lengths are whole ones."""
 
@@ -172,6 +185,31 @@ def test_scores_and_appending_and_another_layer(gpu, dtype):
     assert (np.abs(gpu.paged_attention(t, batch.on(other)).cpu().reshape(q.shape) - out) <= tol).all()
     for _ in range(3):
         assert np.array_equal(gpu.paged_attention(t, batch).cpu().reshape(q.shape), first)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "int8"])
+def test_by_size(gpu, dtype):
+    # Without the hook: a small prefix is each sequence's own, to the bit; a large
+    # one is shared, and its attention the definition's.
+    from porch_b200._lib import lib
+
+    assert lib().pb_test_share_prefix(0) == 0
+    rng = np.random.default_rng(8)
+    for members, shared, heads, same in ((20, 512, 2, True), (120, 2048, 4, False)):
+        lengths = [shared + 1 + i % 3 for i in range(members)]
+        host = Shared(rng, [(members, shared)], lengths, heads, 128, 64, dtype)
+        cache, batch = host.build(gpu)
+        q = rng.normal(0, 1, (members, heads, 128)).astype(np.float32)
+        t = gpu.tensor(list(q.shape), q)
+        got = gpu.paged_attention(t, batch).cpu()
+        plain = gpu.paged_attention(t, cache.batch(host.tables, lengths, appended=[0] * members)).cpu()
+        assert np.array_equal(got, plain) == same
+        out, tol, _, _ = host.attend(q, 128**-0.5)
+        assert (np.abs(got.reshape(q.shape) - out) <= tol).all()
+        # Again, by a batch whose plan was made with it.
+        again = cache.batch(host.tables, lengths, appended=[0] * members, prefix=host.prefix)
+        assert np.array_equal(gpu.paged_attention(t, again).cpu(), got)
 
 
 @pytest.mark.gpu
