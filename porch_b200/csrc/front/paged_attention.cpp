@@ -55,7 +55,7 @@ namespace porch::detail {
         struct form {
             int heads = 1, dim = 0, page = 0;
             cache_type type = cache_type::f32;
-            bool scored = false, shared = false;
+            bool scored = false, shared = false, late = false;
             int stall = 0; // the test hook's mode
             int join_threads = 128;
             int tiles8 = 1; // groups of 8 query heads that a row holds (1 or 2)
@@ -409,6 +409,10 @@ static __device__ __forceinline__ void pb_split_queries(const pb_queries& r, pb_
 }
 #endif
 
+// PB_LATE_WAIT: what follows a prefix's own launch, which lets it begin once all
+// before that launch is complete, and neither reads nor writes what the other
+// writes. It takes SMs as they come free, and ends after the other has, so that
+// who waits for this kernel has both.
 extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
     const __grid_constant__ pb_tmap map_k, const __grid_constant__ pb_tmap map_v, const float* q, const int* lengths,
     const int* tables, const int4* work, float* out, float* partial, float2* partial_ml, float* logits, float2* norms,
@@ -454,7 +458,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
         pb_u32 parity = 1; // the first round finds every unit free
         bool bad = false;
         int page = pb_page(at, tables, width, lane);
-        asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (!PB_LATE_WAIT) asm volatile("griddepcontrol.wait;" ::: "memory");
 #if PB_TEST_STALL == 1
         if (blockIdx.x == 0) return; // its tiles never arrive
 #endif
@@ -495,11 +499,12 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                 }
             }
         }
+        if (PB_LATE_WAIT) asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
 
     // ---- four computing warps
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!PB_LATE_WAIT) asm volatile("griddepcontrol.wait;" ::: "memory");
     if (mine.z == 0) { // a row without slots
         for (int e = threadIdx.x; e < pb_heads(at, group) * PB_D; e += 128)
             out[pb_query(at, e / PB_D, group, PB_H * group, 1) * PB_D + e % PB_D] = 0.0f;
@@ -1307,7 +1312,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
                << "\n#define PB_ESZ " << f.width() << "\n#define PB_NT " << f.tiles8 << "\n#define PB_RING " << f.ring()
                << "\n#define PB_JOIN_THREADS " << f.join_threads << "\n#define PB_PER_SM " << f.per_sm()
                << "\n#define PB_STATIC " << form::kStatic << "\n#define PB_SCORED " << (f.scored ? 1 : 0) << "\n#define PB_SHARED " << (f.shared ? 1 : 0)
-               << "\n";
+               << "\n#define PB_LATE_WAIT " << (f.late ? 1 : 0) << "\n";
             if (f.stall != 0) os << "#define PB_TEST_STALL " << f.stall << "\n";
             return os.str();
         }
@@ -1333,7 +1338,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         const char kSharedFinish[] = "pb_shared_finish";
 
         op_kernel& kernel_of(const char* name, const form& f, uint32_t smem) {
-            const op_key key{reinterpret_cast<int64_t>(name), f.heads, f.dim, f.page, static_cast<int64_t>(f.type), f.scored, f.tiles8, f.join_threads, f.stall, f.shared};
+            const op_key key{reinterpret_cast<int64_t>(name), f.heads, f.dim, f.page, static_cast<int64_t>(f.type), f.scored, f.tiles8, f.join_threads, f.stall, f.shared + 2 * f.late};
             return op_kernel_for(key, [&](op_kernel& k) {
                 k.name = name;
                 k.source = std::string{kernel_prelude()} + defines(f) + device_source();
@@ -1505,7 +1510,8 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         form shared_form(const kv_batch& batch, int64_t group) {
             form f = form_of(*batch.cache, group);
             f.shared = true;
-            if (prefix_stage(batch, group)) return f;
+            f.late = prefix_stage(batch, group);
+            if (f.late) return f;
             int64_t most = group;
             for (const auto& g : batch.groups) most = std::max(most, g.members * group);
             f.tiles8 = most > 8 ? 2 : 1;
@@ -1857,6 +1863,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             f.tiles8 = tiles8;
             f.page = page;
             f.shared = page == 32;
+            f.late = f.shared && width == 2;
             f.scored = !f.shared;
             out.emplace_back("pb_paged_attention_" + std::to_string(dim) + (width == 1 ? "_i8_" : (width == 2 ? "_bf16_" : "_f32_")) + std::to_string(8 * tiles8) + (f.shared ? "_shared" : ""),
                              std::string{kernel_prelude()} + defines(f) + device_source());

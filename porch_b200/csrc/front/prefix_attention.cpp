@@ -215,6 +215,9 @@ extern "C" __global__ void __launch_bounds__(384, 1) pb_prefix_attention(
     if (warp == 0) {
         // ---- producer
         asm volatile("griddepcontrol.wait;" ::: "memory");
+        // Every CTA has its SM by the time that all are here; the next launch takes
+        // those that come free first.
+        asm volatile("griddepcontrol.launch_dependents;");
         int unit = 0, row = mine.x, tile = mine.y, left = mine.z;
         bool good = true;
         auto load = [&](const pb_tmap* map, int y) {
@@ -465,7 +468,6 @@ extern "C" __global__ void __launch_bounds__(384, 1) pb_prefix_attention(
                 pb_mbar_arrive(p_ready);
             }
             if (good) drain(t - 1, corr);
-            if (left == n) asm volatile("griddepcontrol.launch_dependents;");
             if (good && query < a.count) {
                 partial_ml[((pb_i64)part * 2 + half) * 128 + query] = make_float2(m, l);
                 // Four channels of every query side by side: a warp's stores are whole
