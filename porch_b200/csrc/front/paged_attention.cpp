@@ -51,6 +51,11 @@ namespace porch::detail {
             if (!ok) throw std::invalid_argument(message);
         }
 
+        // Slots of a tile: 128 of an 8-bit cache, whose 64 take hardly more time than
+        // what a tile takes by itself (TILE128), as long as that leaves room for
+        // several CTAs.
+        int tile_of(cache_type type, int64_t dim) { return type == cache_type::i8 && dim <= 128 ? 128 : 64; }
+
         // The whole layout of a kernel follows from these.
         struct form {
             int heads = 1, dim = 0, page = 0;
@@ -61,12 +66,13 @@ namespace porch::detail {
             int tiles8 = 1; // groups of 8 query heads that a row holds (1 or 2)
             int width() const { return type == cache_type::f32 ? 4 : (type == cache_type::bf16 ? 2 : 1); }
             int planes() const { return (dim * width() + 127) / 128; }
-            int unit() const { return planes() * 8192; }                       // 64 slots of K or of V
+            int tile() const { return tile_of(type, dim); }                    // slots
+            int unit() const { return planes() * tile() * 128; }               // a tile of K or of V
             int steps() const { return ((dim * width() + 31) / 32 + 1) & ~1; } // 32-byte k-steps, an even number
-            int scales() const { return type == cache_type::i8 ? 256 : 0; } // bytes of a unit's
+            int scales() const { return type == cache_type::i8 ? tile() * 4 : 0; } // bytes of a unit's
             int terms() const { return type == cache_type::f32 ? 2 : 3; }
             int q_row() const { return steps() * 32 + 16; }
-            int p_row() const { return 64 * width() + 16; }
+            int p_row() const { return tile() * width() + 16; }
             int small() const { // everything but the ring
                 return terms() * tiles8 * 8 * (q_row() + p_row()) + 2 * 4 * tiles8 * 8 * 4 +
                        (type == cache_type::i8 ? 5 * tiles8 * 8 * 4 : 0);
@@ -103,12 +109,14 @@ typedef long long pb_i64;
 #define PB_WAIT_CYCLES 4000000000ll
 #define PB_HT (8 * PB_NT)                // query heads of a row, padded
 #define PB_PLANES ((PB_D * PB_ESZ + 127) / 128)
-#define PB_UNIT (PB_PLANES * 8192)       // 64 slots, one 128-byte plane after the other
+#define PB_PLANE (PB_TS * 128)
+#define PB_UNIT (PB_PLANES * PB_PLANE)   // a tile's slots, one 128-byte plane after the other
+#define PB_MB (PB_TS / 64)               // 16 slots of each warp
 #define PB_CE (128 / PB_ESZ)             // values of a plane's row
 #define PB_BOX (PB_PS < 64 ? PB_PS : 64) // slots of one tile load
 #define PB_STEPS ((((PB_D * PB_ESZ + 31) / 32) + 1) & ~1)
 #define PB_QROW (PB_STEPS * 32 + 16)
-#define PB_PROW (64 * PB_ESZ + 16)
+#define PB_PROW (PB_TS * PB_ESZ + 16)
 #define PB_MT ((PB_D + 15) / 16)         // 16-channel tiles of the result
 #define PB_MTW ((PB_MT + 3) / 4)         // of one warp
 #if PB_ESZ == 4
@@ -285,7 +293,7 @@ static __device__ __forceinline__ void pb_split_frag(const pb_u32* a, pb_u32* hi
 #endif
 
 // Where a row's tiles come from. Rows are (sequence, key head, chunk of query
-// heads), tiles 64 slots of a row; a CTA works through a run of tiles.
+// heads), tiles PB_TS slots of a row; a CTA works through a run of tiles.
 #if PB_SHARED
 // Sequences that share a prefix: a row is a run of slots of one key head, the
 // prefix or what follows it, and the queries that read it, of sequence after
@@ -300,9 +308,9 @@ static __device__ __forceinline__ void pb_enter(pb_at& a, const int* rows, int) 
     a.first = y.x;
     a.f0 = y.y;
     a.count = y.z;
-    a.tiles = (a.length - a.begin + 63) >> 6;
+    a.tiles = (a.length - a.begin + PB_TS - 1) / PB_TS;
 }
-static __device__ __forceinline__ int pb_base(const pb_at& a) { return a.begin + a.tile * 64; }
+static __device__ __forceinline__ int pb_base(const pb_at& a) { return a.begin + a.tile * PB_TS; }
 static __device__ __forceinline__ int pb_heads(const pb_at& a, int) { return a.count; }
 static __device__ __forceinline__ pb_i64 pb_query(const pb_at& a, int head, int group, pb_i64 q_seq, pb_i64 q_head) {
     const int f = a.f0 + head;
@@ -310,7 +318,7 @@ static __device__ __forceinline__ pb_i64 pb_query(const pb_at& a, int head, int 
 }
 #else
 struct pb_at { int row, tile; int s, h, chunk, length, tiles; };
-static __device__ __forceinline__ int pb_base(const pb_at& a) { return a.tile * 64; }
+static __device__ __forceinline__ int pb_base(const pb_at& a) { return a.tile * PB_TS; }
 static __device__ __forceinline__ int pb_heads(const pb_at& a, int group) { return min(PB_HT, group - a.chunk * PB_HT); }
 static __device__ __forceinline__ pb_i64 pb_query(const pb_at& a, int head, int group, pb_i64 q_seq, pb_i64 q_head) {
     return a.s * q_seq + (a.h * group + a.chunk * PB_HT + head) * q_head;
@@ -320,7 +328,7 @@ static __device__ __forceinline__ void pb_enter(pb_at& a, const int* lengths, in
     a.h = (a.row / chunks) % PB_H;
     a.s = a.row / chunks / PB_H;
     a.length = lengths[a.s];
-    a.tiles = (a.length + 63) >> 6;
+    a.tiles = (a.length + PB_TS - 1) / PB_TS;
 }
 #endif
 // The next tile; skips sequences without slots. True when it is another row's.
@@ -337,7 +345,7 @@ static __device__ __forceinline__ bool pb_next(pb_at& a, const int* lengths, int
 // The page that this lane's part of the tile lies in (0 past its slots).
 static __device__ __forceinline__ int pb_page(const pb_at& a, const int* tables, int width, int lane) {
     const int first = pb_base(a) + lane * PB_BOX;
-    return lane * PB_BOX < 64 && first < a.length ? tables[(pb_i64)a.s * width + first / PB_PS] : 0;
+    return lane * PB_BOX < PB_TS && first < a.length ? tables[(pb_i64)a.s * width + first / PB_PS] : 0;
 }
 
 // A row's queries, PB_Q_EACH values of each of 128 threads, every load before
@@ -423,8 +431,8 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
     __shared__ int abort_flag;
     static_assert(sizeof(bars) + sizeof(abort_flag) + 128 <= PB_STATIC, "shared memory that the launch does not count");
     const pb_u32 ring = (pb_smem(raw) + 1023u) & ~1023u;
-    const pb_u32 unit_scales = ring + PB_RING * PB_UNIT; // 256 bytes of each unit, in 8 bits
-    const pb_u32 qs = unit_scales + (PB_ESZ == 1 ? PB_RING * 256 : 0);
+    const pb_u32 unit_scales = ring + PB_RING * PB_UNIT; // of each unit, in 8 bits
+    const pb_u32 qs = unit_scales + (PB_ESZ == 1 ? PB_RING * PB_TS * 4 : 0);
     const pb_u32 ps = qs + PB_TERMS * PB_HT * PB_QROW;
     float* wmax = reinterpret_cast<float*>(raw + (ps + PB_TERMS * PB_HT * PB_PROW - pb_smem(raw)));
     float* wsum = wmax + 4 * PB_HT;
@@ -463,7 +471,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
         if (blockIdx.x == 0) return; // its tiles never arrive
 #endif
         for (int i = 0; i < mine.z && !bad; ++i) {
-            const int base = pb_base(at), boxes = (min(64, at.length - base) + PB_BOX - 1) / PB_BOX;
+            const int base = pb_base(at), boxes = (min(PB_TS, at.length - base) + PB_BOX - 1) / PB_BOX;
             const int y = (page * PB_H + at.h) * PB_PS + (base + lane * PB_BOX) % PB_PS;
             if (i + 1 < mine.z) { // the next tile's pages are looked up while this one's loads are issued
                 pb_next(at, lengths, chunks);
@@ -480,9 +488,9 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                     const pb_u32 dst = ring + slot * PB_UNIT + lane * PB_BOX * 128;
 #pragma unroll
                     for (int c = 0; c < PB_PLANES; ++c)
-                        pb_tma_load(dst + c * 8192, which ? &map_v : &map_k, full + 8 * slot, c * PB_CE, y);
+                        pb_tma_load(dst + c * PB_PLANE, which ? &map_v : &map_k, full + 8 * slot, c * PB_CE, y);
 #if PB_ESZ == 1
-                    pb_bulk_load(unit_scales + slot * 256 + lane * PB_BOX * 4, (which ? scales_v : scales_k) + y, full + 8 * slot);
+                    pb_bulk_load(unit_scales + slot * (PB_TS * 4) + lane * PB_BOX * 4, (which ? scales_v : scales_k) + y, full + 8 * slot);
 #endif
                 }
                 ++unit;
@@ -517,7 +525,9 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
     int segment = 0; // how many rows this CTA has begun
     float m[PB_NT][2], l[PB_NT][2], o[PB_MTW][PB_NT][4];
     bool begun_at_zero = true;
-#if PB_ESZ == 4
+#if PB_ESZ == 1
+    float query_unit[PB_NT][2];
+#elif PB_ESZ == 4
     // Where this thread's four values of V^T lie in each of its channel tiles
     // (slots 2 t and 2 t + 1 of a group of 8, channels g and g + 8).
     pb_u32 v_at[PB_MTW][4];
@@ -526,7 +536,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int r = 2 * t + (e >> 1), ch = (warp + 4 * a) * 16 + g + (e & 1) * 8;
-            v_at[a][e] = (ch >> 5) * 8192 + r * 128 + ((((ch & 31) >> 2) ^ r) << 4) + (ch & 3) * 4;
+            v_at[a][e] = (ch >> 5) * PB_PLANE + r * 128 + ((((ch & 31) >> 2) ^ r) << 4) + (ch & 3) * 4;
         }
 #endif
     // The next tile is looked up, and the next row's queries are loaded, a tile
@@ -567,9 +577,15 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[a][n][e] = 0.0f;
             if (pb_bar_any(bad)) { bad = true; break; }
+#if PB_ESZ == 1
+#pragma unroll
+            for (int n = 0; n < PB_NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) query_unit[n][e] = units[8 * n + 2 * t + e] * scale2;
+#endif
         }
         if (PB_Q_EACH8 <= 8 && i + 1 < mine.z && next_fresh) pb_load_queries(ahead, q, next, q_seq, q_head, group);
-        const int base = pb_base(at), valid = min(64, at.length - base);
+        const int base = pb_base(at), valid = min(PB_TS, at.length - base);
 
         // ---- S^T = K Q^T: this warp's 16 slots x all heads
 #if PB_TEST_STALL == 2
@@ -581,25 +597,30 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
         bad |= !pb_wait(full + 8 * slot, parity, &abort_flag, err, 3);
         // The first term's sum, the large one, runs in two chains that are
         // added in fp32: half the additions that cut bits in a row.
-        pb_acc c[PB_TERMS + 1][PB_NT][4];
+        pb_acc c[PB_MB][PB_TERMS + 1][PB_NT][4];
 #pragma unroll
-        for (int x = 0; x < PB_TERMS + 1; ++x)
+        for (int b = 0; b < PB_MB; ++b)
 #pragma unroll
-            for (int n = 0; n < PB_NT; ++n)
+            for (int x = 0; x < PB_TERMS + 1; ++x)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) c[x][n][e] = 0;
+                for (int n = 0; n < PB_NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) c[b][x][n][e] = 0;
         {
             const int r = 16 * warp + (lane & 15);
             const pb_u32 krow = ring + slot * PB_UNIT + r * 128;
             const pb_u32 qrow = qs + (lane & 7) * PB_QROW + (lane >> 3) * 16;
 #pragma unroll
             for (int k2 = 0; k2 < PB_STEPS / 2; ++k2) {
-                pb_u32 a[2][4];
+                pb_u32 slots[PB_MB][2][4]; // of 64 b + 16 warp and following
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const int chunk = (2 * k2 + k) * 2; // 16-byte chunk of the row; its plane and place
-                    pb_ldm4(a[k], krow + (chunk >> 3) * 8192 + ((((chunk & 7) + (lane >> 4)) ^ (r & 7)) << 4));
-                }
+                for (int b = 0; b < PB_MB; ++b)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const int chunk = (2 * k2 + k) * 2; // 16-byte chunk of the row; its plane and place
+                        pb_ldm4(slots[b][k], krow + b * 8192 + (chunk >> 3) * PB_PLANE + ((((chunk & 7) + (lane >> 4)) ^ (r & 7)) << 4));
+                    }
+                pb_u32 (&a)[2][4] = slots[0];
 #if PB_ESZ == 1
 #pragma unroll
                 for (int x = 0; x < PB_TERMS; ++x)
@@ -607,8 +628,11 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                     for (int n = 0; n < PB_NT; ++n) {
                         pb_u32 b[4];
                         pb_ldm4(b, qrow + (x * PB_HT + n * 8) * PB_QROW + k2 * 64);
-                        pb_mma(c[x][n], a[0], b);
-                        pb_mma(c[x][n], a[1], b + 2);
+#pragma unroll
+                        for (int i = 0; i < PB_MB; ++i) {
+                            pb_mma(c[i][x][n], slots[i][0], b);
+                            pb_mma(c[i][x][n], slots[i][1], b + 2);
+                        }
                     }
 #elif PB_ESZ == 2
 #pragma unroll
@@ -617,8 +641,8 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                     for (int n = 0; n < PB_NT; ++n) {
                         pb_u32 b[4];
                         pb_ldm4(b, qrow + (x * PB_HT + n * 8) * PB_QROW + k2 * 64);
-                        pb_mma(c[x][n], a[0], b);
-                        pb_mma(c[x == 0 ? PB_TERMS : x][n], a[1], b + 2);
+                        pb_mma(c[0][x][n], a[0], b);
+                        pb_mma(c[0][x == 0 ? PB_TERMS : x][n], a[1], b + 2);
                     }
 #else
                 pb_u32 hi[2][4], lo[2][4];
@@ -629,22 +653,24 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                     pb_u32 b[4], b2[4];
                     pb_ldm4(b, qrow + (n * 8) * PB_QROW + k2 * 64);
                     pb_ldm4(b2, qrow + (PB_HT + n * 8) * PB_QROW + k2 * 64);
-                    pb_mma(c[0][n], hi[0], b);
-                    pb_mma(c[1][n], hi[0], b2);
-                    pb_mma(c[PB_TERMS][n], hi[1], b + 2);
-                    pb_mma(c[1][n], lo[0], b);
-                    pb_mma(c[1][n], hi[1], b2 + 2);
-                    pb_mma(c[1][n], lo[1], b + 2);
+                    pb_mma(c[0][0][n], hi[0], b);
+                    pb_mma(c[0][1][n], hi[0], b2);
+                    pb_mma(c[0][PB_TERMS][n], hi[1], b + 2);
+                    pb_mma(c[0][1][n], lo[0], b);
+                    pb_mma(c[0][1][n], hi[1], b2 + 2);
+                    pb_mma(c[0][1][n], lo[1], b + 2);
                 }
 #endif
             }
         }
 #if PB_ESZ == 1
-        // The scales of this thread's two slots, 0 past the sequence's end.
-        float key_scale[2], value_scale[2];
+        // The scales of this thread's slots, 0 past the sequence's end.
+        float key_scale[PB_MB][2], value_scale[PB_MB][2];
+        auto scale_of = [&](int i) { return i < valid ? pb_shared(unit_scales + slot * (PB_TS * 4) + i * 4) : 0.0f; };
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-            key_scale[j] = 16 * warp + g + 8 * j < valid ? pb_shared(unit_scales + slot * 256 + (16 * warp + g + 8 * j) * 4) : 0.0f;
+        for (int b = 0; b < PB_MB; ++b)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) key_scale[b][j] = scale_of(64 * b + 16 * warp + g + 8 * j);
 #endif
         __syncwarp();
         // Not after a wait that gave up: the unit's load may still be on its
@@ -655,30 +681,34 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
         auto wait_for_values = [&] { bad |= !pb_wait(full + 8 * slot, parity, &abort_flag, err, 4); };
 
         // Logits in units of log2, -inf past the sequence's end. Thread: slots
-        // 16 warp + g and + 8, heads 8 n + 2 t and + 1.
-        float s[PB_NT][4], top[PB_NT][2];
+        // 16 warp + g and + 8 (of each 64), heads 8 n + 2 t and + 1.
+        float s[PB_MB][PB_NT][4], top[PB_NT][2];
 #pragma unroll
         for (int n = 0; n < PB_NT; ++n) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int at_slot = 16 * warp + g + (e >> 1) * 8;
+            for (int b = 0; b < PB_MB; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int at_slot = 64 * b + 16 * warp + g + (e >> 1) * 8;
 #if PB_ESZ == 1
-                const float x = pb_of_digits(c[0][n][e], c[1][n][e], c[2][n][e]) * (units[8 * n + 2 * t + (e & 1)] * scale2) * key_scale[e >> 1];
+                    const float x = pb_of_digits(c[b][0][n][e], c[b][1][n][e], c[b][2][n][e]) * query_unit[n][e & 1] * key_scale[b][e >> 1];
 #elif PB_TERMS == 3
-                const float x = (c[2][n][e] + c[1][n][e] + (c[0][n][e] + c[3][n][e])) * scale2;
+                    const float x = (c[b][2][n][e] + c[b][1][n][e] + (c[b][0][n][e] + c[b][3][n][e])) * scale2;
 #else
-                const float x = (c[1][n][e] + (c[0][n][e] + c[2][n][e])) * scale2;
+                    const float x = (c[b][1][n][e] + (c[b][0][n][e] + c[b][2][n][e])) * scale2;
 #endif
-                s[n][e] = at_slot < valid ? x : __int_as_float(0xff800000);
+                    s[b][n][e] = at_slot < valid ? x : __int_as_float(0xff800000);
 #if PB_SCORED
-                const int head = 8 * n + 2 * t + (e & 1);
-                if (at_slot < valid && head < hg)
-                    logits[pb_query(at, head, group, PB_H * group, 1) * longest + base + at_slot] = x;
+                    const int head = 8 * n + 2 * t + (e & 1);
+                    if (at_slot < valid && head < hg)
+                        logits[pb_query(at, head, group, PB_H * group, 1) * longest + base + at_slot] = x;
 #endif
-            }
+                }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                float x = fmaxf(s[n][e], s[n][e + 2]);
+                float x = fmaxf(s[0][n][e], s[0][n][e + 2]);
+#pragma unroll
+                for (int b = 1; b < PB_MB; ++b) x = fmaxf(x, fmaxf(s[b][n][e], s[b][n][e + 2]));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -688,18 +718,22 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
         }
 #if PB_ESZ == 1
         wait_for_values(); // earlier than in other types: their scales go into the weights
-        float scaled[2];
+        float scaled[PB_MB][2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            value_scale[j] = 16 * warp + g + 8 * j < valid ? pb_shared(unit_scales + slot * 256 + (16 * warp + g + 8 * j) * 4) : 0.0f;
-            scaled[j] = pb_log2(value_scale[j]);
-        }
+        for (int b = 0; b < PB_MB; ++b)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                value_scale[b][j] = scale_of(64 * b + 16 * warp + g + 8 * j);
+                scaled[b][j] = pb_log2(value_scale[b][j]);
+            }
 #pragma unroll
         for (int n = 0; n < PB_NT; ++n) {
             float2 most;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                float x = pb_max_nan(s[n][e] + scaled[0], s[n][e + 2] + scaled[1]);
+                float x = PB_LOWEST;
+#pragma unroll
+                for (int b = 0; b < PB_MB; ++b) x = pb_max_nan(x, pb_max_nan(s[b][n][e] + scaled[b][0], s[b][n][e + 2] + scaled[b][1]));
                 x = pb_max_nan(x, __shfl_xor_sync(0xffffffffu, x, 4));
                 x = pb_max_nan(x, __shfl_xor_sync(0xffffffffu, x, 8));
                 x = pb_max_nan(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -747,27 +781,29 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
 #endif
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float p = pb_exp2(s[n][e] - m[n][e & 1]);
-                l[n][e & 1] += p;
-                const int at_slot = 16 * warp + g + (e >> 1) * 8, head = 8 * n + 2 * t + (e & 1);
+            for (int b = 0; b < PB_MB; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float p = pb_exp2(s[b][n][e] - m[n][e & 1]);
+                    l[n][e & 1] += p;
+                    const int at_slot = 64 * b + 16 * warp + g + (e >> 1) * 8, head = 8 * n + 2 * t + (e & 1);
 #if PB_ESZ == 1
-                // As V's fragments count slots: 2 t, 2 t + 1, 2 t + 8, 2 t + 9 side by side.
-                const int place = (at_slot & ~15) + ((at_slot & 7) >> 1) * 4 + ((at_slot >> 3) & 1) * 2 + (at_slot & 1);
-                const pb_u32 digits = pb_digits(__float2int_rn(p * value_scale[e >> 1] * (pb_exp2(-power[n][e & 1]) * PB_WEIGHTS)));
-                const pb_u32 to = ps + head * PB_PROW + place;
-                asm volatile("st.shared.u8 [%0], %1;" :: "r"(to), "r"(digits) : "memory");
-                asm volatile("st.shared.u8 [%0], %1;" :: "r"(to + PB_HT * PB_PROW), "r"(digits >> 8) : "memory");
-                asm volatile("st.shared.u8 [%0], %1;" :: "r"(to + 2 * PB_HT * PB_PROW), "r"(digits >> 16) : "memory");
+                    // As V's fragments count slots: 2 t, 2 t + 1, 2 t + 8, 2 t + 9 side by side.
+                    const int place = (at_slot & ~15) + ((at_slot & 7) >> 1) * 4 + ((at_slot >> 3) & 1) * 2 + (at_slot & 1);
+                    const pb_u32 digits = pb_digits(__float2int_rn(p * value_scale[b][e >> 1] * (pb_exp2(-power[n][e & 1]) * PB_WEIGHTS)));
+                    const pb_u32 to = ps + head * PB_PROW + place;
+                    asm volatile("st.shared.u8 [%0], %1;" :: "r"(to), "r"(digits) : "memory");
+                    asm volatile("st.shared.u8 [%0], %1;" :: "r"(to + PB_HT * PB_PROW), "r"(digits >> 8) : "memory");
+                    asm volatile("st.shared.u8 [%0], %1;" :: "r"(to + 2 * PB_HT * PB_PROW), "r"(digits >> 16) : "memory");
 #else
 #if PB_ESZ == 2
-                const int place = at_slot;
+                    const int place = at_slot;
 #else
-                const int place = (at_slot & ~7) + ((at_slot & 7) >> 1) + (at_slot & 1) * 4; // as V's fragments count slots
+                    const int place = (at_slot & ~7) + ((at_slot & 7) >> 1) + (at_slot & 1) * 4; // as V's fragments count slots
 #endif
-                pb_split_store(ps + head * PB_PROW + place * PB_ESZ, PB_HT * PB_PROW, p);
+                    pb_split_store(ps + head * PB_PROW + place * PB_ESZ, PB_HT * PB_PROW, p);
 #endif
-            }
+                }
         }
 #if PB_ESZ != 1
         wait_for_values();
@@ -790,7 +826,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
 #pragma unroll
                         for (int e = 0; e < 4; ++e) d[a][n][x][e] = 0;
 #pragma unroll
-            for (int k2 = 0; k2 < PB_ESZ; ++k2) { // two k-steps at a time
+            for (int k2 = 0; k2 < PB_ESZ * PB_MB; ++k2) { // two k-steps at a time
                 pb_u32 b[PB_TERMS][PB_NT][4];
 #pragma unroll
                 for (int x = 0; x < PB_TERMS; ++x)
@@ -810,7 +846,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                             // lies past the end is finite, and its weight 0.
                             const int r = (2 * k2 + k) * 32 + lane;
                             pb_u32 pair[4];
-                            pb_ldm4t(pair, vunit + (mt >> 3) * 8192 + r * 128 + (((mt & 7) ^ (r & 7)) << 4));
+                            pb_ldm4t(pair, vunit + (mt >> 3) * PB_PLANE + r * 128 + (((mt & 7) ^ (r & 7)) << 4));
                             v[0] = __byte_perm(pair[0], pair[1], 0x6420);
                             v[1] = __byte_perm(pair[0], pair[1], 0x7531);
                             v[2] = __byte_perm(pair[2], pair[3], 0x6420);
@@ -823,7 +859,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                             const int first = (2 * k2 + k) * 16;
                             const int r = first + (lane >> 4) * 8 + (lane & 7);
                             const int chunk = mt * 2 + ((lane >> 3) & 1);
-                            pb_ldm4t(v, vunit + (chunk >> 3) * 8192 + r * 128 + (((chunk & 7) ^ (r & 7)) << 4));
+                            pb_ldm4t(v, vunit + (chunk >> 3) * PB_PLANE + r * 128 + (((chunk & 7) ^ (r & 7)) << 4));
                             if (valid < 64) { // what lies past the end may be anything
 #pragma unroll
                                 for (int e = 0; e < 4; ++e) {
@@ -1310,6 +1346,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             std::ostringstream os;
             os << "#define PB_H " << f.heads << "\n#define PB_D " << f.dim << "\n#define PB_PS " << f.page
                << "\n#define PB_ESZ " << f.width() << "\n#define PB_NT " << f.tiles8 << "\n#define PB_RING " << f.ring()
+               << "\n#define PB_TS " << f.tile()
                << "\n#define PB_JOIN_THREADS " << f.join_threads << "\n#define PB_PER_SM " << f.per_sm()
                << "\n#define PB_STATIC " << form::kStatic << "\n#define PB_SCORED " << (f.scored ? 1 : 0) << "\n#define PB_SHARED " << (f.shared ? 1 : 0)
                << "\n#define PB_LATE_WAIT " << (f.late ? 1 : 0) << "\n";
@@ -1346,7 +1383,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             });
         }
 
-        // Even runs of 64-slot tiles, over all rows one after the other, where a
+        // Even runs of tiles (of 64 slots, but for 8 bits), over all rows one after the other, where a
         // row counts as one tile more than it has, for its queries, its sums
         // and its result (32 sequences of 8 rows up to 4096 slots of 80 channels:
         // 39.4 us with tiles alone, 36.4 so). A run begins and ends inside a row at
@@ -1363,24 +1400,24 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         };
         constexpr int64_t kWholeRow = 8;
 
-        schedule make_schedule(const std::vector<int64_t>& lengths, int64_t heads, int64_t chunks, int64_t ctas) {
+        schedule make_schedule(const std::vector<int64_t>& lengths, int64_t heads, int64_t chunks, int64_t ctas, int64_t tile = 64) {
             schedule r;
             const int64_t per = heads * chunks;
             int64_t total = 0, rows = 0, most = 0;
             for (int64_t length : lengths) {
-                const int64_t tiles = (length + 63) / 64;
+                const int64_t tiles = (length + tile - 1) / tile;
                 total += tiles * per;
                 most = std::max(most, tiles);
                 if (tiles != 0) rows += per;
             }
-            const bool whole = most <= kWholeRow && rows <= ctas;
+            const bool whole = most * tile <= kWholeRow * 64 && rows <= ctas;
             // The tile, in the order of all rows, that each CTA begins with.
             std::vector<int64_t> starts;
             if (!whole) {
                 const int64_t n = std::min(total, ctas);
                 int64_t row_cost = 0, row_tile = 0, cut = 0; // where the row begins
                 for (int64_t length : lengths) {
-                    const int64_t tiles = (length + 63) / 64;
+                    const int64_t tiles = (length + tile - 1) / tile;
                     if (tiles == 0) continue;
                     for (int64_t j = 0; j < per; ++j) {
                         for (; cut < n; ++cut) {
@@ -1403,7 +1440,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             };
             std::vector<int32_t> empty;
             for (size_t s = 0; s < lengths.size(); ++s) {
-                const int64_t tiles = (lengths[s] + 63) / 64;
+                const int64_t tiles = (lengths[s] + tile - 1) / tile;
                 for (int64_t j = 0; j < per; ++j) {
                     const int64_t row = static_cast<int64_t>(s) * per + j;
                     r.split.push_back(-1);
@@ -1545,7 +1582,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
                 for (int64_t f0 = 0; f0 < queries; f0 += per)
                     for (int64_t v : {seq, h, begin, end, first, f0, std::min(per, queries - f0), int64_t{0}})
                         rows.push_back(static_cast<int32_t>(v));
-                const int64_t tile = per == 128 ? 128 : 64; // slots
+                const int64_t tile = per == 128 ? 128 : f.tile(); // slots
                 if (end > begin) tiles.insert(tiles.end(), static_cast<size_t>((queries + per - 1) / per), (end - begin + tile - 1) / tile);
                 return row;
             };
@@ -1802,7 +1839,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         std::scoped_lock lock{batch.plans->mutex};
         for (const auto& p : batch.plans->made)
             if (p->chunks == chunks && p->limit == ctas) return *p;
-        schedule s = make_schedule(batch.lengths, batch.cache->heads, chunks, ctas);
+        schedule s = make_schedule(batch.lengths, batch.cache->heads, chunks, ctas, tile_of(batch.cache->type, batch.cache->dim));
         auto p = std::make_unique<batch_plan>();
         p->chunks = chunks;
         p->limit = ctas;
