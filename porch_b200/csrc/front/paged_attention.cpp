@@ -1537,9 +1537,11 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         bool worth_sharing(const kv_batch& batch, int64_t group) {
             const kv_cache& c = *batch.cache;
             const int64_t per = prefix_stage(batch, group) ? 128 : 16; // queries that read a prefix together
-            int64_t slots = 0;
-            for (const auto& g : batch.groups) slots += (g.members - (g.members * group + per - 1) / per) * g.slots;
-            return !batch.groups.empty() && (g_test_share.load(std::memory_order_relaxed) || slots * c.heads * 2 * c.dim * c.width() >= 96000000);
+            double slots = 0; // that are not read again
+            for (const auto& g : batch.groups)
+                slots += static_cast<double>(g.members - (g.members * group + per - 1) / per) * static_cast<double>(g.slots);
+            return !batch.groups.empty() && (g_test_share.load(std::memory_order_relaxed) ||
+                                             slots * static_cast<double>(c.heads * 2 * c.dim * c.width()) >= 96e6);
         }
 
         // The form of what follows the prefixes, and of prefixes without a stage of
@@ -1750,6 +1752,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         auto stream = current_stream(device);
         op_operand x = operand(q, stream, true), xs;
         if (scores != nullptr) xs = operand(*scores, stream, false);
+        expect(n * c.heads * ((shape[1] / c.heads + 7) / 8) < (int64_t{1} << 27), "paged_attention: too many sequences and heads");
         if (!scored && worth_sharing(batch, shape[1] / c.heads)) {
             std::vector<tensor> results;
             results.push_back(shared_attention(x, batch, scale2, stream));
