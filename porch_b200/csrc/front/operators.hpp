@@ -173,9 +173,9 @@ namespace porch::detail {
             uint64_t rows_at = 0, work_at = 0; // device addresses
         };
         stage prefix, rest;
-        int64_t most_parts = 0;
+        int64_t most_parts = 0, units = 0; // units: of the join
         cuda_jit::device_buffer data;
-        uint64_t parts_at = 0, outs_at = 0;
+        uint64_t parts_at = 0, outs_at = 0, units_at = 0;
     };
     struct batch_plans {
         std::shared_ptr<plan_hint> hint; // of the cache that the batch was made for

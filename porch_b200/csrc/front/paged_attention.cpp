@@ -984,81 +984,99 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
 // it. Parts of a row lie one behind the other: {first, how many} of each in
 // `rows`; a sequence's key head is {its first row, the prefix's first row (-1
 // where there is none), its first query's place among those that read the
-// prefix}. Block: one query head, as pb_join's; `h1`, `h2`: queries of a row of
-// the prefix and of a sequence. A prefix's own stage leaves two sums for each of
-// its queries, and results four channels of all queries side by side (`own`).
-// PB_JOIN_THREADS 32: a warp each for up to 32 parts, four heads a block, which
-// needs no barrier (64 sequences of 32 heads with 11 to 14 parts: FINISH_FEW us,
-// 12.8 with a block each).
+// prefix}. `h1`, `h2`: queries of a row of the prefix and of a sequence. A prefix's
+// own stage leaves two sums for each of its queries, and results four queries of
+// four channels each side by side (`own`).
+//
+// PB_JOIN_THREADS 32, up to 32 parts: a warp has 32 channels of four queries, the
+// `units` {prefix's row or -1, first query, first sequence, key head + 2^20 x how
+// many}, and every part's on the way at once, so that it reads whole lines and
+// needs no barrier (64 sequences of 32 heads with 11 to 14 parts: 7 us of the
+// stream, 9.8 with a warp for each query's channels, 28 with a block each).
 #if PB_JOIN_THREADS == 32
-#define PB_QUADS ((PB_D / 4 + 31) / 32) // of a lane
+#define PB_CHUNKS ((PB_D + 31) / 32)
 extern "C" __global__ void __launch_bounds__(128) pb_shared_finish(
     const int4* outs, const int2* rows, const float* partial1, const float2* ml1, const float* partial2, const float2* ml2,
-    float* out, int group, int h1, int h2, int own, int heads) {
+    float* out, int group, int h1, int h2, int own, const int4* units, int count) {
     const int lane = threadIdx.x & 31, id = blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (id >= heads) return;
-    const int head = id % group;
-    const int4 o = outs[id / group]; // of the plan, in place before the launch
+    if (id >= count * PB_CHUNKS) return;
+    const int4 u = units[id / PB_CHUNKS]; // of the plan, in place before the launch
+    const int j = lane & 3, quad = id % PB_CHUNKS * 8 + (lane >> 2), kvh = u.w & 0xfffff;
+    const int f = u.y + min(j, (u.w >> 20) - 1), head = f % group, seq = u.z + f / group;
+    const int4 o = outs[seq * PB_H + kvh];
     int2 r1 = make_int2(0, 0), r2 = make_int2(0, 0);
-    const int f = o.z + head;
-    if (o.y >= 0) r1 = rows[o.y + f / h1];
+    if (u.x >= 0) r1 = rows[u.x];
     if (o.x >= 0) r2 = rows[o.x + head / h2];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int parts = r1.y + r2.y;
-    if (parts == 0) return; // already there
-    // Lane i has part i's maximum, sum and place.
-    float2 ml = make_float2(PB_LOWEST, 0.0f);
-    const float* at = partial1;
-    if (lane < r1.y) {
-        const float2* p = ml1 + (pb_i64)(r1.x + lane) * (1 + own) * h1 + f % h1;
-        ml = p[0];
-        if (own) ml.y += p[h1].y;
-        at = partial1 + (pb_i64)(r1.x + lane) * h1 * PB_D + (own ? f % h1 * 4 : f % h1 * PB_D);
-    } else if (lane < parts) {
-        const pb_i64 i = ((pb_i64)r2.x + lane - r1.y) * h2 + head % h2;
-        ml = ml2[i];
-        at = partial2 + i * PB_D;
+    const int most = __reduce_max_sync(0xffffffffu, parts);
+    if (most == 0) return; // already there
+    // Lane (i % 8, j) has the maxima and sums of query j's parts i, i + 8, ...
+    float top = PB_LOWEST, w[4], sum = 0.0f;
+    float2 ml[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const int i = 8 * k + (lane >> 2);
+        ml[k] = make_float2(PB_LOWEST, 0.0f);
+        if (i < r1.y) {
+            const float2* p = ml1 + (pb_i64)(r1.x + i) * (1 + own) * h1 + f % h1;
+            ml[k] = p[0];
+            if (own) ml[k].y += p[h1].y;
+        } else if (i < parts) {
+            ml[k] = ml2[((pb_i64)r2.x + i - r1.y) * h2 + head % h2];
+        }
+        top = fmaxf(top, ml[k].x);
     }
-    float top = ml.x;
+    // Every part's results on the way; nothing of them is used before the weights are there.
+    const float4 none = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    const bool in = quad < PB_D / 4;
+    const float4* p1 = reinterpret_cast<const float4*>(partial1) + (pb_i64)r1.x * h1 * (PB_D / 4) +
+                       (own ? (f % h1 / 4 * (PB_D / 4) + quad) * 4 + f % 4 : f % h1 * (PB_D / 4) + quad);
+    const float4* p2 = reinterpret_cast<const float4*>(partial2) + ((pb_i64)r2.x * h2 + head % h2) * (PB_D / 4) + quad;
+    auto result = [&](int i) {
+        return !in || i >= parts ? none : (i < r1.y ? p1[(pb_i64)i * h1 * (PB_D / 4)] : p2[(pb_i64)(i - r1.y) * h2 * (PB_D / 4)]);
+    };
+    float4 x[8];
 #pragma unroll
-    for (int m = 16; m > 0; m /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
-    const float w = lane < parts ? pb_exp2(ml.x - top) : 0.0f;
-    float sum = lane < parts ? w * ml.y : 0.0f;
+    for (int i = 0; i < 8; ++i) x[i] = result(i);
 #pragma unroll
-    for (int m = 16; m > 0; m /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, m);
-    float4 acc[PB_QUADS];
+    for (int m = 4; m < 32; m *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, m));
 #pragma unroll
-    for (int c = 0; c < PB_QUADS; ++c) acc[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-    for (int i = 0; i < parts; ++i) {
-        const float v = __shfl_sync(0xffffffffu, w, i);
-        const float* p = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<pb_u64>(at), i));
-        const int step = own && i < r1.y ? 4 * h1 : 4; // from quad to quad
+    for (int k = 0; k < 4; ++k) {
+        w[k] = 8 * k + (lane >> 2) < parts ? pb_exp2(ml[k].x - top) : 0.0f;
+        sum = fmaf(w[k], ml[k].y, sum);
+    }
 #pragma unroll
-        for (int c = 0; c < PB_QUADS; ++c) {
-            const int quad = c * 32 + lane;
-            if (quad >= PB_D / 4) continue;
-            const float4 x = *reinterpret_cast<const float4*>(p + (pb_i64)quad * step);
-            acc[c].x = fmaf(v, x.x, acc[c].x);
-            acc[c].y = fmaf(v, x.y, acc[c].y);
-            acc[c].z = fmaf(v, x.z, acc[c].z);
-            acc[c].w = fmaf(v, x.w, acc[c].w);
+    for (int m = 4; m < 32; m *= 2) sum += __shfl_xor_sync(0xffffffffu, sum, m);
+    float4 acc = none;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        if (8 * k >= most) break;
+        float4 y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            y[i] = x[i];
+            if (k < 3 && 8 * (k + 1) < most) x[i] = result(8 * (k + 1) + i);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float v = __shfl_sync(0xffffffffu, w[k], i * 4 + j);
+            acc.x = fmaf(v, y[i].x, acc.x);
+            acc.y = fmaf(v, y[i].y, acc.y);
+            acc.z = fmaf(v, y[i].z, acc.z);
+            acc.w = fmaf(v, y[i].w, acc.w);
         }
     }
     const float inv = 1.0f / sum;
-#pragma unroll
-    for (int c = 0; c < PB_QUADS; ++c) {
-        const int quad = c * 32 + lane;
-        if (quad < PB_D / 4)
-            *reinterpret_cast<float4*>(out + (pb_i64)id * PB_D + 4 * quad) =
-                make_float4(acc[c].x * inv, acc[c].y * inv, acc[c].z * inv, acc[c].w * inv);
-    }
+    if (in && parts != 0 && j < (u.w >> 20))
+        *reinterpret_cast<float4*>(out + (((pb_i64)seq * PB_H + kvh) * group + head) * PB_D + 4 * quad) =
+            make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
 }
 #else
 #define PB_JOIN (PB_JOIN_THREADS / (PB_D / 4))
 extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_shared_finish(
     const int4* outs, const int2* rows, const float* partial1, const float2* ml1, const float* partial2, const float2* ml2,
-    float* out, int group, int h1, int h2, int own, int) {
+    float* out, int group, int h1, int h2, int own, const int4*, int) {
     __shared__ float weight[PB_JOIN_THREADS], reduce[16];
     __shared__ float4 sums[PB_JOIN_THREADS];
     const int head = blockIdx.x % group;
@@ -1070,10 +1088,10 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_shared_finish(
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int parts = r1.y + r2.y;
     if (parts == 0) return; // already there
-    const float* p1 = partial1 + (pb_i64)r1.x * h1 * PB_D + (own ? f % h1 * 4 : f % h1 * PB_D);
+    const float* p1 = partial1 + (pb_i64)r1.x * h1 * PB_D + (own ? (f % h1 / 4 * PB_D + f % 4) * 4 : f % h1 * PB_D);
     const float* p2 = partial2 + ((pb_i64)r2.x * h2 + head % h2) * PB_D;
     const int lane = threadIdx.x & 31, quad = threadIdx.x % (PB_D / 4), team = threadIdx.x / (PB_D / 4);
-    const int step1 = own ? 4 * h1 : 4; // from quad to quad
+    const int step1 = own ? 16 : 4; // from quad to quad
     auto result = [&](int i) {
         return *reinterpret_cast<const float4*>(i < r1.y ? p1 + (pb_i64)i * h1 * PB_D + quad * step1
                                                          : p2 + (pb_i64)(i - r1.y) * h2 * PB_D + quad * 4);
@@ -1649,7 +1667,24 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
                 host.insert(host.end(), v.begin(), v.end());
                 return at * 4;
             };
-            const size_t prefix_work = add(first.work), rest_work = add(r.work), out = add(outs), part = add(parts);
+            // Units of the join: four queries of a prefix, or of a sequence without one.
+            std::vector<int32_t> units;
+            auto put_units = [&](int64_t seq, int64_t queries, bool shared) {
+                for (int64_t h = 0; h < heads; ++h)
+                    for (int64_t f0 = 0; f0 < queries; f0 += 4) {
+                        const int32_t row = shared ? outs[static_cast<size_t>(4 * (seq * heads + h) + 1)] : -1;
+                        for (int64_t v : {shared ? row + f0 / p->prefix.per : int64_t{-1}, f0, seq, h + (std::min<int64_t>(4, queries - f0) << 20)})
+                            units.push_back(static_cast<int32_t>(v));
+                    }
+            };
+            for (int64_t s = 0, g = 0; s < n;) {
+                const bool shared = g < static_cast<int64_t>(batch.groups.size()) && batch.groups[static_cast<size_t>(g)].first == s;
+                const int64_t members = shared ? batch.groups[static_cast<size_t>(g++)].members : 1;
+                put_units(s, members * group, shared);
+                s += members;
+            }
+            p->units = static_cast<int64_t>(units.size() / 4);
+            const size_t prefix_work = add(first.work), rest_work = add(r.work), out = add(outs), unit = add(units), part = add(parts);
             auto stream = upload_stream(c.device);
             p->data = allocate(c.device, host.size() * sizeof(int32_t), stream);
             const uint64_t at = address(p->data);
@@ -1658,6 +1693,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             p->prefix.work_at = at + prefix_work;
             p->rest.work_at = at + rest_work;
             p->outs_at = at + out;
+            p->units_at = at + unit;
             p->parts_at = at + part;
             check(pbrt_memcpy_h2d_async(c.device, at, host.data(), host.size() * sizeof(int32_t), stream->stream));
             check(pbrt_stream_synchronize(c.device, stream->stream));
@@ -1716,12 +1752,11 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
                 ml1 = ml2;
             }
             int per1 = plan.prefix.per, per2 = plan.rest.per, own = prefix != nullptr ? 1 : 0;
-            int heads = static_cast<int>(x.shape[0] * x.shape[1]);
-            void* params[] = {&outs, &parts, &partial1, &ml1, &partial2, &ml2, &out.ptr, &group, &per1, &per2, &own, &heads};
-            if (f.join_threads == 32)
-                op_launch(finishing, device, stream, {static_cast<uint32_t>((heads + 3) / 4), 1, 1}, 128, params);
-            else
-                op_launch(finishing, device, stream, {static_cast<uint32_t>(heads), 1, 1}, 512, params);
+            uint64_t units = plan.units_at;
+            int count = static_cast<int>(plan.units);
+            void* params[] = {&outs, &parts, &partial1, &ml1, &partial2, &ml2, &out.ptr, &group, &per1, &per2, &own, &units, &count};
+            const int64_t blocks = f.join_threads == 32 ? (plan.units * ((c.dim + 31) / 32) + 3) / 4 : x.shape[0] * x.shape[1];
+            op_launch(finishing, device, stream, {static_cast<uint32_t>(blocks), 1, 1}, f.join_threads == 32 ? 128 : 512, params);
             return finish(std::move(out));
         }
 
@@ -1904,6 +1939,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             f.page = page;
             f.shared = page == 32;
             f.late = f.shared && width == 2;
+            f.join_threads = f.late ? 32 : 128;
             f.scored = !f.shared;
             out.emplace_back("pb_paged_attention_" + std::to_string(dim) + (width == 1 ? "_i8_" : (width == 2 ? "_bf16_" : "_f32_")) + std::to_string(8 * tiles8) + (f.shared ? "_shared" : ""),
                              std::string{kernel_prelude()} + defines(f) + device_source());

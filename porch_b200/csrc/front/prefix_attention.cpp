@@ -470,12 +470,14 @@ extern "C" __global__ void __launch_bounds__(384, 1) pb_prefix_attention(
             if (good) drain(t - 1, corr);
             if (good && query < a.count) {
                 partial_ml[((pb_i64)part * 2 + half) * 128 + query] = make_float2(m, l);
-                // Four channels of every query side by side: a warp's stores are whole
-                // lines (query after query they took 4500 cycles of a row's end).
-                float4* to = reinterpret_cast<float4*>(partial) + ((pb_i64)part * (PB_D / 4) + first / 4) * 128 + query;
+                // Four channels of four queries side by side, as the join reads them: a
+                // warp's stores fill whole sectors (query after query they took 4500
+                // cycles of a row's end).
+                float4* to = reinterpret_cast<float4*>(partial) +
+                             (((pb_i64)part * 32 + (query >> 2)) * (PB_D / 4) + first / 4) * 4 + (query & 3);
 #pragma unroll
                 for (int j = 0; j < PB_NH; j += 4)
-                    if (first + j < PB_D) to[j / 4 * 128] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                    if (first + j < PB_D) to[j] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
             }
             left -= n;
             tile = 0;
