@@ -382,3 +382,29 @@ def test_refusals(gpu):
         gpu.KVCache(4, 16, 2, 64, dtype="bf16").scales()
     with pytest.raises(RuntimeError, match="placeholder"):
         batch.append(gpu.placeholder([1, 2, 64]), gpu.zeros([1, 2, 64]))
+
+
+@pytest.mark.gpu
+def test_pools_past_two_to_the_32_bytes(gpu):
+    # 2^24 + 2^20 rows of 256 codes: the last pages lie past 2^32 bytes, and the
+    # scales behind them.
+    pages, page, dim = ((1 << 24) + (1 << 20)) // 64, 64, 256
+    cache = gpu.KVCache(pages, page, 1, dim, dtype="int8")
+    rng = np.random.default_rng(2)
+    host = int8_cache.Host(rng, [150], 1, dim, page)
+    host.tables = np.array([[pages - 1, 3, pages - 2]], dtype=np.int32)
+    batch = cache.batch(host.tables, [150], appended=[150])
+    batch.append(gpu.tensor([150, 1, dim], host.k[0]), gpu.tensor([150, 1, dim], host.v[0]))
+    for got, x in zip(batch.read(), (host.k[0], host.v[0])):
+        codes, scale = int8_cache.quantise(x)
+        assert np.array_equal(got.cpu().reshape(x.shape), codes.astype(np.float32) * scale[..., None])
+    q = rng.normal(0, 0.2, (1, 3, dim)).astype(np.float32)
+    out, tol, _, _ = host.attend(q, 1.0)
+    got = gpu.paged_attention(gpu.tensor([1, 3, dim], q), batch, scale=1.0).cpu().reshape(q.shape)
+    assert (np.abs(got - out) <= tol).all()
+    scores = rng.uniform(0, 1, (1, 1, 150)).astype(np.float32)
+    gpu.cache_evict(batch, gpu.tensor([1, 1, 150], scores), budget=70, recent=9)
+    source, _, _ = paged.evict([150], [149], scores, None, 70, 9, 0)
+    k, _ = cache.batch(host.tables, [70], appended=[0]).read()
+    codes, scale = int8_cache.quantise(host.k[0][source[0, 0]])
+    assert np.array_equal(k.cpu().reshape(70, 1, dim), codes.astype(np.float32) * scale[..., None])

@@ -291,3 +291,36 @@ def test_refusals(gpu):
         gpu.cache_evict(batch, gpu.zeros([3, 2, 60]), budget=20)
     with pytest.raises(gpu.InvalidArgument, match="q must be"):
         gpu.paged_attention(gpu.zeros([2, 4, 64]), batch)
+
+
+@pytest.mark.gpu
+def test_a_prefix_past_two_to_the_32_bytes(gpu):
+    pages, page, dim = ((1 << 24) + (1 << 20)) // 64, 64, 128
+    cache = gpu.KVCache(pages, page, 1, dim, dtype="bf16")
+    rng = np.random.default_rng(2)
+    host = Shared(rng, [(30, 128)], [150] * 30, 1, dim, page, "bf16")
+    host.tables = pages - 1 - np.maximum(host.tables, 0)
+    for s in range(30):
+        one = cache.batch(host.tables[s : s + 1], [150], appended=[150])
+        one.append(gpu.tensor([150, 1, dim], host.k[s]), gpu.tensor([150, 1, dim], host.v[s]))
+    q = rng.normal(0, 1, (30, 2, dim)).astype(np.float32)
+    out, tol, _, _ = host.attend(q, dim**-0.5)
+    batch = cache.batch(host.tables, [150] * 30, prefix=host.prefix)
+    got = gpu.paged_attention(gpu.tensor(list(q.shape), q), batch).cpu().reshape(q.shape)
+    assert (np.abs(got - out) <= tol).all()
+
+
+@pytest.mark.gpu
+def test_many_parts_and_many_rows(gpu):
+    # One long prefix of one key head in more parts than a warp joins, beside
+    # groups and sequences of all kinds in one batch.
+    rng = np.random.default_rng(12)
+    groups = [(17, 12800), (1, 0), (2, 64), (1, 64), (40, 128), (3, 0), (5, 64)]
+    lengths = [12800 + i for i in range(17)] + [0, 64, 65, 100] + [130] * 40 + [3, 0, 700] + [64, 65, 66, 67, 200]
+    lengths = lengths[: sum(m for m, _ in groups)]
+    host = Shared(rng, groups, lengths, 1, 64, 64, "bf16")
+    _, batch = host.build(gpu)
+    q = rng.normal(0, 2, (len(lengths), 2, 64)).astype(np.float32)
+    out, tol, _, _ = host.attend(q, 0.125)
+    got = gpu.paged_attention(gpu.tensor(list(q.shape), q), batch).cpu().reshape(q.shape)
+    assert (np.abs(got - out) <= tol).all()

@@ -325,3 +325,23 @@ def test_gradient_of_many_rows(gpu):
         tol = np.abs(g[i]) * (p_off + 4 * U * (p + hot)) + np.abs(h[i]) * (p_off * np.abs(inner) + p * inner_off + 4 * U * p * np.abs(inner))
         tol = tol + 2.0**-126 * (1 + np.abs(g[i]) + np.abs(h[i]) * (1 + np.abs(inner)))
         assert (np.abs(got[i] - want[0]) <= tol[0]).all()
+
+
+@pytest.mark.gpu
+def test_more_than_two_to_the_31_logits(gpu):
+    rows, vocab = 16400, 131072
+    logits = gpu.zeros([rows, vocab])
+    tokens = np.arange(rows, dtype=np.float32)
+    t = gpu.tensor([rows], tokens)
+    said, entropy, norm, _, best = gpu.token_logprobs(logits, t, top=2)
+    flat = np.log(np.float64(vocab))
+    # Sums of equal terms in a tree with a thread's 32 rounds at its ends: 64 roundings.
+    assert np.abs(said.cpu() + flat).max() <= 64 * U + 4 * U * flat and np.abs(entropy.cpu() - flat).max() <= 64 * U + 4 * U * flat
+    assert (best.cpu().reshape(rows, 2) == [0, 1]).all()
+    d = gpu.token_logprobs_backward(gpu.tensor([rows], np.ones(rows, np.float32)), logits, t, norm)
+    for row in (0, 16383, 16384, rows - 1):
+        x = gpu.materialize(d[row : row + 1, gpu.all]).cpu().reshape(vocab)
+        want = -np.full(vocab, 1.0 / vocab)
+        want[row] += 1
+        assert np.abs(x - want).max() <= 2.0**-20
+        assert np.abs(np.delete(x, row) * vocab + 1).max() <= 2.0**-17
