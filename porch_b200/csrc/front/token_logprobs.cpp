@@ -10,7 +10,9 @@
 // maximum is a new one; sums are fp32, of a few hundred terms a thread, then
 // joined pairwise. One launch: a row that few others keep company is shared
 // out over a cluster, whose first CTA joins the parts from the others' shared
-// memory.
+// memory. 4093 x 50257: 131 us = 6.3 TB/s; its gradient at 4096 x 65536: 322 us =
+// 6.7 TB/s. Few rows are bound by latencies: 64 x 131072 with the 20 largest 18 us of
+// the stream (10 without), one row of 32000 with 5 of them 7 us.
 #include "operators.hpp"
 
 #include <algorithm>
@@ -43,7 +45,7 @@ static __device__ __forceinline__ float pb_finite(float x) { return fmaxf(x, -1e
 
 // Four values of the row from element 4 j - shift on (`shift` of them lie
 // before the row, so that the others start on 16 bytes); `none` outside it.
-static __device__ __forceinline__ float4 pb_four(const float* row, pb_i64 at, pb_i64 n, float none) {
+static __device__ __forceinline__ float4 pb_four(const float* row, int at, int n, float none) {
     if (at >= 0 && at + 4 <= n) return __ldcs(reinterpret_cast<const float4*>(row + at));
     float v[4];
 #pragma unroll
@@ -52,9 +54,9 @@ static __device__ __forceinline__ float4 pb_four(const float* row, pb_i64 at, pb
 }
 
 // What the tokens' numbers say: the token, -1 for a padded row, -2 for anything else.
-static __device__ __forceinline__ pb_i64 pb_token(float t, pb_i64 V) {
+static __device__ __forceinline__ int pb_token(float t, int V) {
     if (t == -1.0f) return -1;
-    return t >= 0.0f && t < (float)V && t == truncf(t) ? (pb_i64)t : -2;
+    return t >= 0.0f && t < (float)V && t == truncf(t) ? (int)t : -2;
 }
 
 #ifdef PB_FORWARD
@@ -144,11 +146,11 @@ static __device__ __forceinline__ T pb_sorted(T a, int lane) {
 #endif
 
 // A thread's 16 logits of the round at vector `base`; -inf outside the run and the row.
-static __device__ __forceinline__ void pb_load(float* v, const float* x, pb_i64 base, pb_i64 last, pb_i64 shift, pb_i64 V, bool on) {
+static __device__ __forceinline__ void pb_load(float* v, const float* x, int base, int last, int shift, int V, bool on) {
     const float none = __int_as_float(0xff800000);
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-        const pb_i64 j = base + q * PB_THREADS + threadIdx.x;
+        const int j = base + q * PB_THREADS + threadIdx.x;
         const float4 f = on && j < last ? pb_four(x, 4 * j - shift, V, none) : make_float4(none, none, none, none);
         v[4 * q] = f.x; v[4 * q + 1] = f.y; v[4 * q + 2] = f.z; v[4 * q + 3] = f.w;
     }
@@ -157,7 +159,7 @@ static __device__ __forceinline__ void pb_load(float* v, const float* x, pb_i64 
 // Cluster: one row, each CTA a run of `run` vectors of it.
 extern "C" __global__ void __launch_bounds__(PB_THREADS, 1024 / PB_THREADS) pb_token_logprobs(
     const float* logits, const float* tokens, float* said, float* entropy, float* norm, float* top_said, float* top_tokens,
-    pb_i64 V, pb_i64 stride, int run, int top) {
+    int V, pb_i64 stride, int run, int top) { // a vocabulary is below 2^25, and so is every place in it
     __shared__ float sums[PB_WARPS][3];
 #if PB_TOP
     __shared__ pb_u64 lists[PB_WARPS][32];
@@ -168,16 +170,16 @@ extern "C" __global__ void __launch_bounds__(PB_THREADS, 1024 / PB_THREADS) pb_t
     const pb_u32 row = blockIdx.x / PB_CLUSTER, rank = PB_CLUSTER > 1 ? pb_rank() : 0;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float* x = logits + (pb_i64)row * stride;
-    const pb_i64 shift = (pb_i64)(reinterpret_cast<pb_u64>(x) >> 2 & 3);
-    const pb_i64 vectors = (V + shift + 3) >> 2, first = (pb_i64)rank * run, last = min(vectors, first + run);
+    const int shift = (int)(reinterpret_cast<pb_u64>(x) >> 2 & 3);
+    const int vectors = (V + shift + 3) >> 2, first = (int)rank * run, last = min(vectors, first + run);
     pb_sums a = {PB_LOWEST, 0.0f, 0.0f};
 #if PB_TOP
     // This lane's largest of a round, that round, and the largest of the others.
     float m1 = __int_as_float(0xff800000), m2 = m1;
-    pb_i64 b1 = first;
+    int b1 = first;
 #endif
 #pragma unroll 1
-    for (pb_i64 base = first; base < last; base += 4 * PB_THREADS) {
+    for (int base = first; base < last; base += 4 * PB_THREADS) {
         float v[16];
         pb_load(v, x, base, last, shift, V, true);
         float most = v[0];
@@ -218,13 +220,13 @@ extern "C" __global__ void __launch_bounds__(PB_THREADS, 1024 / PB_THREADS) pb_t
         const pb_u32 largest = pb_merge(pb_sorted(mine[0], lane), pb_sorted(mine[1], lane), lane);
         const float low = pb_unorder(__shfl_sync(0xffffffffu, largest, top - 1));
         if (m1 >= low)
-            for (pb_i64 base = m2 >= low ? first : b1; base < last; base += 4 * PB_THREADS) {
+            for (int base = m2 >= low ? first : b1; base < last; base += 4 * PB_THREADS) {
                 float v[16];
                 pb_load(v, x, base, last, shift, V, true);
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
                     if (v[e] >= low) {
-                        const pb_i64 j = base + (e >> 2) * PB_THREADS + threadIdx.x, at = 4 * j - shift + (e & 3);
+                        const int j = base + (e >> 2) * PB_THREADS + threadIdx.x, at = 4 * j - shift + (e & 3);
                         if (j < last && at >= 0 && at < V) {
                             const int place = atomicAdd(&listed, 1);
                             if (place < PB_THREADS) lists[place / 32][place % 32] = pb_key(v[e], (pb_u32)at);
@@ -241,7 +243,7 @@ extern "C" __global__ void __launch_bounds__(PB_THREADS, 1024 / PB_THREADS) pb_t
             lists_used = PB_WARPS;
             pb_u64 least = 0; // the list's entry `top` - 1
 #pragma unroll 1
-            for (pb_i64 base = first; base < last; base += 4 * PB_THREADS) {
+            for (int base = first; base < last; base += 4 * PB_THREADS) {
                 float v[16];
                 pb_load(v, x, base, last, shift, V, m1 >= low);
 #pragma unroll 1
@@ -249,7 +251,7 @@ extern "C" __global__ void __launch_bounds__(PB_THREADS, 1024 / PB_THREADS) pb_t
                     float y = v[0];
 #pragma unroll
                     for (int i = 1; i < 16; ++i) y = i == e ? v[i] : y;
-                    const pb_i64 j = base + (e >> 2) * PB_THREADS + threadIdx.x, at = 4 * j - shift + (e & 3);
+                    const int j = base + (e >> 2) * PB_THREADS + threadIdx.x, at = 4 * j - shift + (e & 3);
                     const pb_u64 key = y >= low && j < last && at >= 0 && at < V ? pb_key(y, (pb_u32)at) : 0;
                     for (pb_u32 wanting = __ballot_sync(0xffffffffu, key > least); wanting != 0;) {
                         pb_insert(list, __shfl_sync(0xffffffffu, key, __ffs(wanting) - 1), lane);
@@ -310,7 +312,7 @@ extern "C" __global__ void __launch_bounds__(PB_THREADS, 1024 / PB_THREADS) pb_t
         const bool good = a.s > 0.0f; // not: nothing but -inf, or a NaN or +inf
         const float total = good ? a.s : PB_NAN, log_total = logf(total);
         if (lane == 0) {
-            const pb_i64 t = pb_token(__ldg(tokens + row), V);
+            const int t = pb_token(__ldg(tokens + row), V);
             said[row] = t >= 0 ? (__ldg(x + t) - a.m) - log_total : (t == -1 ? 0.0f : PB_NAN);
             entropy[row] = log_total - a.w / total;
             norm[2 * (pb_i64)row] = a.m;
@@ -331,7 +333,7 @@ extern "C" __global__ void __launch_bounds__(PB_THREADS, 1024 / PB_THREADS) pb_t
 #endif
         // Fewer numbers than alternatives: NaN comes last, in order.
         if (__shfl_sync(0xffffffffu, list, top - 1) == 0)
-            for (pb_i64 i = 0; i < V; i += 32) {
+            for (int i = 0; i < V; i += 32) {
                 const float y = i + lane < V ? __ldg(x + i + lane) : 0.0f;
                 for (pb_u32 nans = __ballot_sync(0xffffffffu, y != y); nans != 0; nans &= nans - 1)
                     pb_insert(list, pb_key(PB_NAN, (pb_u32)(i + __ffs(nans) - 1)), lane);
@@ -349,73 +351,83 @@ extern "C" __global__ void __launch_bounds__(PB_THREADS, 1024 / PB_THREADS) pb_t
 #ifdef PB_BACKWARD
 // Block: PB_LOOPS times 4096 gradients of one row, 16 a thread at once. Where there
 // are many, four times: what the row has one of is loaded once for them (4096 x
-// 65536: 349 us, 372 with one; 37 x 50257: 14.8, 11.6 with one). Five blocks of an
-// SM at once (390 us with the four that the registers would leave). exp(d) = 2^(t + r) with
-// t the rounded product d log2 e and r what the rounding left, so that p is
-// within a few units of its last place also far below the maximum.
+// 65536: 322 us, 327 with one; 37 x 50257, cold: 14.8, 12.6 with one). Five blocks of an SM at
+// once (324 us with four, and with six).
+//
+// e^d = 2^b e^(d - b log 2) for any b, here d log2 e rounded; what the rounding
+// left is so small that e to it is 1 plus it (two terms of log 2 take the
+// difference), so p is within a few units of its last place also far below the
+// maximum. Below e^-200, which float32 has no number for, every d counts as -200.
+// The row's scale, sign and constants are folded into two numbers outside the loop,
+// since the instructions show: 322 us, 349 with them taken at each logit.
 #define PB_ROUNDS 4
 extern "C" __global__ void __launch_bounds__(256, 5) pb_token_logprobs_grad(
     const float* d_said, const float* d_entropy, const float* logits, const float* tokens, const float* norm,
-    const float* entropy, float* out, pb_i64 V, pb_i64 stride, pb_u32 blocks) {
+    const float* entropy, float* out, int V, pb_i64 stride, pb_u32 blocks) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const pb_u32 row = blockIdx.x / blocks;
     const float* x = logits + (pb_i64)row * stride;
     float* to = out + (pb_i64)row * V;
-    const pb_i64 shift = (pb_i64)(reinterpret_cast<pb_u64>(to) >> 2 & 3);
-    const bool same = (pb_i64)(reinterpret_cast<pb_u64>(x) >> 2 & 3) == shift; // the stores are aligned, the loads where they can be
-    const pb_i64 t = pb_token(__ldg(tokens + row), V);
-    float g = __ldg(d_said + row), m = __ldg(norm + 2 * (pb_i64)row), s = __ldg(norm + 2 * (pb_i64)row + 1);
+    const int shift = (int)(reinterpret_cast<pb_u64>(to) >> 2 & 3);
+    const bool same = (int)(reinterpret_cast<pb_u64>(x) >> 2 & 3) == shift; // the stores are aligned, the loads where they can be
+    const int t = pb_token(__ldg(tokens + row), V);
+    const float m = __ldg(norm + 2 * (pb_i64)row), s = __ldg(norm + 2 * (pb_i64)row + 1);
+    const float g = t >= 0 ? __ldg(d_said + row) : (t == -1 ? 0.0f : PB_NAN);
 #if PB_ENTROPY
-    const float h = __ldg(d_entropy + row), ent = __ldg(entropy + row);
-#endif
-    g = t >= 0 ? g : (t == -1 ? 0.0f : PB_NAN);
-    const float inv = 1.0f / s;
-#if PB_ENTROPY
-    const float rest = ent - logf(s);
+    // -p (g + h (d - log s + H)) = -p (c + h d)
+    const float h = __ldg(d_entropy + row), c = fmaf(h, __ldg(entropy + row) - logf(s), g), scale = -1.0f / s;
     const bool nothing = t == -1 && h == 0.0f; // a padded row, whatever it holds
 #else
+    const float scale = -g / s;
     const bool nothing = t == -1;
 #endif
-    pb_i64 first = (pb_i64)(blockIdx.x % blocks) * (PB_LOOPS * PB_ROUNDS * 256) + threadIdx.x;
+    int first = (int)(blockIdx.x % blocks) * (PB_LOOPS * PB_ROUNDS * 256) + threadIdx.x;
 #pragma unroll 1
     for (int loop = 0; loop < PB_LOOPS; ++loop, first += PB_ROUNDS * 256) {
         float4 v[PB_ROUNDS];
 #pragma unroll
         for (int q = 0; q < PB_ROUNDS; ++q) {
-            const pb_i64 at = 4 * (first + q * 256) - shift;
-            if (at >= V) { v[q] = make_float4(0.0f, 0.0f, 0.0f, 0.0f); continue; }
-            if (same) v[q] = pb_four(x, at, V, 0.0f);
-            else {
+            const int at = 4 * (first + q * 256) - shift;
+            if (at >= V || nothing) {
+                v[q] = make_float4(m, m, m, m);
+            } else if (same) {
+                v[q] = pb_four(x, at, V, 0.0f);
+            } else {
                 float e[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) e[i] = at + i >= 0 && at + i < V ? __ldg(x + at + i) : 0.0f;
                 v[q] = make_float4(e[0], e[1], e[2], e[3]);
             }
-    }
+        }
 #pragma unroll
         for (int q = 0; q < PB_ROUNDS; ++q) {
-            const pb_i64 at = 4 * (first + q * 256) - shift;
+            const int at = 4 * (first + q * 256) - shift;
             if (at >= V) break;
             float d[4];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const float rel = pb_get(v[q], e) - m, low = pb_finite(rel);
-                const float b = low * PB_LOG2E, r = fmaf(low, PB_LOG2E, -b) + low * 1.9259629911266175e-8f;
-                const float z = pb_exp2(b);
-                const float p = (rel == rel ? fmaf(z * r, 0.69314718055994531f, z) : rel) * inv;
+                const float rel = fmaxf(pb_get(v[q], e) - m, -200.0f), b = rel * PB_LOG2E;
+                const float left = fmaf(b, 1.90465432e-09f, fmaf(b, -0.693147182f, rel));
+                const float z = pb_exp2(b) * scale;
+                const float p = fmaf(z, left, z);
 #if PB_ENTROPY
-                const float c = p == 0.0f ? 0.0f : -fmaf(h, low + rest, g);
+                d[e] = p * fmaf(h, rel, c);
 #else
-                const float c = -g;
+                d[e] = p;
 #endif
-                d[e] = nothing ? 0.0f : fmaf(p, c, at + e == t ? g : 0.0f);
+                if (nothing) d[e] = 0.0f;
             }
-            if (at >= 0 && at + 4 <= V) __stcs(reinterpret_cast<float4*>(to + at), make_float4(d[0], d[1], d[2], d[3]));
-            else
+            if ((pb_u32)(t - at) < 4u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) d[e] += at + e == t ? g : 0.0f;
+            if (at >= 0 && at + 4 <= V) {
+                __stcs(reinterpret_cast<float4*>(to + at), make_float4(d[0], d[1], d[2], d[3]));
+            } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (at + e >= 0 && at + e < V) to[at + e] = d[e];
-    }
+            }
+        }
     }
 }
 #endif
@@ -491,7 +503,8 @@ extern "C" __global__ void __launch_bounds__(256, 5) pb_token_logprobs_grad(
         expect(device_of(tokens, "token_logprobs") == device, "token_logprobs: operands must live on one device");
         auto stream = current_stream(device);
         op_operand x = operand(logits, stream, true), t = operand(tokens, stream, false);
-        int64_t rows = s[0], vocab = s[1];
+        const int64_t rows = s[0], vocab = s[1];
+        int V = static_cast<int>(vocab);
         op_result said = new_result({rows}, device, stream), entropy = new_result({rows}, device, stream);
         op_result norm = new_result({rows, 2}, device, stream);
         op_result top_said, top_tokens;
@@ -507,7 +520,7 @@ extern "C" __global__ void __launch_bounds__(256, 5) pb_token_logprobs_grad(
             int run = static_cast<int>(((vocab + 6) / 4 + f.cluster - 1) / f.cluster), most = static_cast<int>(top);
             int64_t stride = rows > 1 ? x.strides[0] : vocab;
             void* params[] = {&x.ptr,        &t.ptr,          &said.ptr, &entropy.ptr, &norm.ptr, &top_said.ptr,
-                              &top_tokens.ptr, &vocab,        &stride,   &run,         &most};
+                              &top_tokens.ptr, &V,            &stride,   &run,         &most};
             op_launch(kernel, device, stream, {static_cast<uint32_t>(rows * f.cluster), 1, 1},
                       static_cast<uint32_t>(f.threads), params, static_cast<uint32_t>(f.cluster));
         }
@@ -540,7 +553,8 @@ extern "C" __global__ void __launch_bounds__(256, 5) pb_token_logprobs_grad(
             e = operand(*entropy, stream, false);
         }
         op_result out = new_result(s, device, stream);
-        int64_t rows = s[0], vocab = s[1];
+        const int64_t rows = s[0], vocab = s[1];
+        int V = static_cast<int>(vocab);
         if (rows != 0) {
             const int64_t vectors = (vocab + 6) / 4; // with up to three values before the row's first
             const int loops = rows * (vectors / 4096) >= int64_t{16} * sm_count(device) ? 4 : 1;
@@ -548,7 +562,7 @@ extern "C" __global__ void __launch_bounds__(256, 5) pb_token_logprobs_grad(
             uint32_t per_row = static_cast<uint32_t>((vectors + 1024 * loops - 1) / (1024 * loops));
             expect(rows <= 0x7fffffff / static_cast<int64_t>(per_row), "token_logprobs_backward: too many rows");
             int64_t stride = rows > 1 ? x.strides[0] : vocab;
-            void* params[] = {&g.ptr, &h.ptr, &x.ptr, &t.ptr, &n.ptr, &e.ptr, &out.ptr, &vocab, &stride, &per_row};
+            void* params[] = {&g.ptr, &h.ptr, &x.ptr, &t.ptr, &n.ptr, &e.ptr, &out.ptr, &V, &stride, &per_row};
             op_launch(kernel, device, stream, {static_cast<uint32_t>(rows * per_row), 1, 1}, 256, params);
         }
         return finish(std::move(out));
