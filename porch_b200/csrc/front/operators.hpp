@@ -1,6 +1,6 @@
 // Eager operators of a transformer's decode step (norms and rotation of
-// query and key heads, a paged key/value cache, its attention and its
-// eviction). They have no counterpart in the reference, whose graphs end at
+// query and key heads, a paged key/value cache, its attention, its eviction and
+// its reading, log probabilities of tokens and their gradient). They have no counterpart in the reference, whose graphs end at
 // matmul and softmax; each takes realised tensors (a lazy one is realised
 // first), enqueues its kernels on the calling thread's stream and returns
 // realised tensors, as allgather_rows does.

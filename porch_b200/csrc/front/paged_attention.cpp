@@ -6,10 +6,11 @@
 // A sequence without slots gives zeros.
 //
 // Bound: HBM, which has to deliver every key and value in use once (2 x slots
-// x kv_heads x head_dim x 2 or 4 bytes). 48 sequences up to 8191 slots, 32
+// x kv_heads x head_dim x 1, 2 or 4 bytes, and 4 for a scale of 8 bits). 48 sequences up to 8191 slots, 32
 // query heads over 8 of 128 bfloat16 channels: 784 MB in 126 us = 6.20 TB/s;
 // one sequence of 262147 slots: 1074 MB in 165 us = 6.5 TB/s, what a copy
-// reaches. Few or short rows are bound by the launch and the first loads'
+// reaches. The same in 8 bits: 404 MB in 71 us and 554 MB in 91, 5.7 and 6.1 TB/s
+// with both launches. Few or short rows are bound by the launch and the first loads'
 // latency instead (about 6 us, 3 of the stream where calls follow each other).
 //
 // pb_paged_attention, 160 threads: a producer warp loads tiles of 64 slots, K
@@ -19,7 +20,7 @@
 // over the tile, weights to shared memory, O^T += V^T P^T for a quarter of the
 // channels each. The transposed products put slots and channels on the tensor
 // core's 16 rows and query heads on its 8 columns, so 1 to 8 heads cost the
-// same. One query per sequence leaves nothing for the 128-row tiles of
+// same. One query per sequence and head leaves nothing for the 128-row tiles of
 // tcgen05; with mma.sync the tensor pipe is 31 % busy at full bandwidth.
 //
 // Accuracy: float32. Queries and weights are split into three bfloat16 terms
@@ -28,7 +29,14 @@
 // and of four products the smallest is left out: 2^-19.6 of a product at most).
 // The tensor core's accumulator cuts low bits at every addition, so a tile's
 // products start from zero and are added to the running sums in fp32, rounded to
-// nearest.
+// nearest. An 8-bit cache is multiplied as it is: queries and weights are three
+// digits to base 256 of a whole number, whose sums of products are exact, and a
+// slot's scales go into its score and its weight.
+//
+// Sequences that share a prefix (a prompt, say) read it once: their queries, up to
+// 16 for one key head here, or up to 128 where the large tiles of tcgen05 pay, are
+// one row over the prefix, and each has another over what follows; a last launch
+// joins them. The rule, with what both sides take, is beside worth_sharing.
 //
 // Work is shared out in even runs of tiles over all rows, one wave of CTAs
 // (more waves, which would even out CTAs of different speed, took 1 to 5 %
@@ -52,8 +60,8 @@ namespace porch::detail {
         }
 
         // Slots of a tile: 128 of an 8-bit cache, whose 64 take hardly more time than
-        // what a tile takes by itself (TILE128), as long as that leaves room for
-        // several CTAs.
+        // what a tile takes by itself (48 sequences up to 8191 slots: 78 us with 64, 72
+        // so; one of 262147: 103 and 93), as long as that leaves room for several CTAs.
         int tile_of(cache_type type, int64_t dim) { return type == cache_type::i8 && dim <= 128 ? 128 : 64; }
 
         // The whole layout of a kernel follows from these.
