@@ -313,8 +313,8 @@ int pb_token_logprobs_backward(const pb_tensor* d_logprobs, const pb_tensor* log
  * cache keeps a float32 scale for each row (the key or value of one token and
  * head), the row's largest size / 127, and the row / scale rounded to nearest,
  * ties to even; what it holds is code x scale. A row with a value that is not
- * finite is held as NaN, one whose values are all below 2^-96 as zeros. The values start undefined;
- * nothing reads a slot past a sequence's length. Calls that write a cache
+ * finite is held as NaN, one whose values are all below 2^-96 as zeros. The
+ * values start undefined; nothing reads a slot past a sequence's length. Calls that write a cache
  * (append, evict) and calls that read it are ordered on the device in the
  * order in which they are made, from whatever threads. */
 typedef struct pb_kv_cache_s pb_kv_cache;
@@ -348,8 +348,9 @@ int pb_kv_batch_create(pb_kv_cache* cache, const int32_t* tables, size_t sequenc
  * pages, 0 for none, none of them new) of sequences next to each other that
  * begin on the same page and have the same prefix[s] are one prefix, which
  * pb_paged_attention then works through once for all of them (where that spares
- * enough reading to pay). Their tables name the same pages for it. Without `appended` a sequence that ends with its prefix
- * has no new token. NULL: as pb_kv_batch_create. */
+ * enough reading to pay). Their tables name the same pages for it. Without
+ * `appended` a sequence that ends with its prefix has no new token. NULL: as
+ * pb_kv_batch_create. */
 int pb_kv_batch_create_shared(pb_kv_cache* cache, const int32_t* tables, size_t sequences, size_t width,
                               const int64_t* lengths, const int64_t* appended, const int64_t* newest,
                               const int64_t* prefix, pb_kv_batch** out);

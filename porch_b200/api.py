@@ -550,9 +550,9 @@ def token_logprobs_backward(d_logprobs, logits, tokens, norm, d_entropy=None, en
 
 class _Pool:
     """A cache pool in place, for another library on the same GPU; a bfloat16
-    pool as its 16 raw bits, an int8 pool's scales as a pool of their own. Keeps the cache alive. Each time it is asked for
-    its interface, the `stream` in it is the calling thread's, behind all that
-    was called on the cache so far."""
+    pool as its 16 raw bits, an int8 pool's scales as a pool of their own. Keeps
+    the cache alive. Each time it is asked for its interface, the `stream` in it
+    is the calling thread's, behind all that was called on the cache so far."""
 
     def __init__(self, cache: "KVCache", which: int, scales: bool = False):
         self.cache, self._which, self._scales = cache, which, scales

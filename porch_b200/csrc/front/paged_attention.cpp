@@ -6,12 +6,13 @@
 // A sequence without slots gives zeros.
 //
 // Bound: HBM, which has to deliver every key and value in use once (2 x slots
-// x kv_heads x head_dim x 1, 2 or 4 bytes, and 4 for a scale of 8 bits). 48 sequences up to 8191 slots, 32
-// query heads over 8 of 128 bfloat16 channels: 784 MB in 126 us = 6.20 TB/s;
-// one sequence of 262147 slots: 1074 MB in 165 us = 6.5 TB/s, what a copy
-// reaches. The same in 8 bits: 404 MB in 71 us and 554 MB in 91, 5.7 and 6.1 TB/s
-// with both launches. Few or short rows are bound by the launch and the first loads'
-// latency instead (about 6 us, 3 of the stream where calls follow each other).
+// x kv_heads x head_dim x 1, 2 or 4 bytes, and 4 for the scale of an 8-bit row).
+// 48 sequences up to 8191 slots, 32 query heads over 8 of 128 bfloat16 channels:
+// 784 MB in 126 us = 6.20 TB/s; one sequence of 262147 slots: 1074 MB in 165 us =
+// 6.5 TB/s, what a copy reaches. The same in 8 bits: 404 MB in 71 us and 554 MB in
+// 91, 5.7 and 6.1 TB/s with both launches. Few or short rows are bound by the
+// launch and the first loads' latency instead (about 6 us, 3 of the stream where
+// calls follow each other).
 //
 // pb_paged_attention, 160 threads: a producer warp loads tiles of 64 slots, K
 // then V, through a ring of TMA boxes (a page, or 64 rows of a larger one; 128
@@ -1555,11 +1556,15 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         }
 
         // Whether working through the prefixes once pays: it takes up to two launches
-        // more, so where it spares reading less than some 96 MB (most of which the L2
+        // more, so where it spares reading less than some 66 MB (most of which the L2
         // cache would deliver) every sequence reads its prefix itself. 32 query heads
-        // over 8 of 128 bfloat16 channels, shared and by themselves: 16 sequences
-        // behind 1024 slots (63 MB) 17.3 and 15.8 us, 8 behind 4096 (117 MB) 22.2 and
-        // 23.4, 64 behind 512 (132 MB) 21.3 and 26.1, behind 2048 30.9 and 75.0.
+        // over 8 of 128 bfloat16 channels, shared and by themselves: 8 sequences behind
+        // 2048 slots (59 MB) 16.6 and 14.3 us, 64 behind 256 (65 MB) 19.1 and 17.1, 2
+        // behind 16384 (67 MB) 17.8 and 24.1, 4 behind 6144 (75 MB) 18.4 and 19.6, 8
+        // behind 4096 (117 MB) 17.6 and 23.3, 64 behind 2048 27.5 and 75.0. In float32
+        // 2 behind 8192 (67 MB) 16.6 and 22.1, 64 behind 384 (151 MB) 35.8 and 32.5, 16
+        // behind 2048 (201 MB) 27.1 and 35.5; in 8 bits 2 behind 32768 (67 MB) 18.1 and
+        // 25.2, 64 behind 1024 (101 MB) 29.4 and 28.0, behind 2048 39.1 and 45.0.
         bool worth_sharing(const kv_batch& batch, int64_t group) {
             const kv_cache& c = *batch.cache;
             const int64_t per = prefix_stage(batch, group) ? 128 : 16; // queries that read a prefix together
@@ -1567,7 +1572,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             for (const auto& g : batch.groups)
                 slots += static_cast<double>(g.members - (g.members * group + per - 1) / per) * static_cast<double>(g.slots);
             return !batch.groups.empty() && (g_test_share.load(std::memory_order_relaxed) ||
-                                             slots * static_cast<double>(c.heads * 2 * c.dim * c.width()) >= 96e6);
+                                             slots * static_cast<double>(c.heads * 2 * c.dim * c.width()) >= 66e6);
         }
 
         // The form of what follows the prefixes, and of prefixes without a stage of

@@ -351,8 +351,8 @@ extern "C" __global__ void __launch_bounds__(PB_THREADS, 1024 / PB_THREADS) pb_t
 #ifdef PB_BACKWARD
 // Block: PB_LOOPS times 4096 gradients of one row, 16 a thread at once. Where there
 // are many, four times: what the row has one of is loaded once for them (4096 x
-// 65536: 322 us, 327 with one; 37 x 50257, cold: 14.8, 12.6 with one). Five blocks of an SM at
-// once (324 us with four, and with six).
+// 65536: 322 us, 327 with one; 37 x 50257, cold: 14.8, 12.6 with one). Five blocks
+// of an SM at once (324 us with four, and with six).
 //
 // e^d = 2^b e^(d - b log 2) for any b, here d log2 e rounded; what the rounding
 // left is so small that e to it is 1 plus it (two terms of log 2 take the
