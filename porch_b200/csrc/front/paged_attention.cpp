@@ -428,8 +428,8 @@ static __device__ __forceinline__ void pb_split_queries(const pb_queries& r, pb_
 
 // PB_LATE_WAIT: what follows a prefix's own launch, which lets it begin once all
 // before that launch is complete, and neither reads nor writes what the other
-// writes. It takes SMs as they come free, and ends after the other has, so that
-// who waits for this kernel has both.
+// writes. It takes SMs that the other leaves and those that come free, and ends
+// after the other has, so that who waits for this kernel has both.
 extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
     const __grid_constant__ pb_tmap map_k, const __grid_constant__ pb_tmap map_v, const float* q, const int* lengths,
     const int* tables, const int4* work, float* out, float* partial, float2* partial_ml, float* logits, float2* norms,
@@ -516,7 +516,8 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                 }
             }
         }
-        if (PB_LATE_WAIT) asm volatile("griddepcontrol.wait;" ::: "memory");
+        // One CTA is enough, and the last keeps nobody from its SM.
+        if (PB_LATE_WAIT && blockIdx.x + 1 == gridDim.x) asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
 
@@ -1556,12 +1557,12 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         }
 
         // Whether working through the prefixes once pays: it takes up to two launches
-        // more, so where it spares reading less than some 66 MB (most of which the L2
+        // more, so where it spares reading less than some 62 MB (most of which the L2
         // cache would deliver) every sequence reads its prefix itself. 32 query heads
         // over 8 of 128 bfloat16 channels, shared and by themselves: 8 sequences behind
-        // 2048 slots (59 MB) 16.6 and 14.3 us, 64 behind 256 (65 MB) 19.1 and 17.1, 2
-        // behind 16384 (67 MB) 17.8 and 24.1, 4 behind 6144 (75 MB) 18.4 and 19.6, 8
-        // behind 4096 (117 MB) 17.6 and 23.3, 64 behind 2048 27.5 and 75.0. In float32
+        // 2048 slots (59 MB) 14.7 and 14.2 us, 16 behind 1024 (63 MB) 12.4 and 15.6, 64
+        // behind 256 (65 MB) 16.2 and 17.1, 2 behind 16384 (67 MB) 17.8 and 24.1, 8
+        // behind 4096 (117 MB) 17.5 and 23.2, 64 behind 2048 22.2 and 75.2. In float32
         // 2 behind 8192 (67 MB) 16.6 and 22.1, 64 behind 384 (151 MB) 35.8 and 32.5, 16
         // behind 2048 (201 MB) 27.1 and 35.5; in 8 bits 2 behind 32768 (67 MB) 18.1 and
         // 25.2, 64 behind 1024 (101 MB) 29.4 and 28.0, behind 2048 39.1 and 45.0.
@@ -1572,7 +1573,48 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             for (const auto& g : batch.groups)
                 slots += static_cast<double>(g.members - (g.members * group + per - 1) / per) * static_cast<double>(g.slots);
             return !batch.groups.empty() && (g_test_share.load(std::memory_order_relaxed) ||
-                                             slots * static_cast<double>(c.heads * 2 * c.dim * c.width()) >= 66e6);
+                                             slots * static_cast<double>(c.heads * 2 * c.dim * c.width()) >= 62e6);
+        }
+
+        // How many CTAs (SMs) work through prefixes in their own launch, while what
+        // follows them has the other SMs, `per` CTAs each, and then all. 32 query heads
+        // over 8 of 128 channels, 64 sequences of 400 slots behind 16384: 72 us where
+        // the prefix has every SM, 69 without 4, 63 without a third, 76 without half.
+        // Of 256 behind 4096: 37, 35, 36, 31. Of 64 behind 16384: 51, 50, 58, 71. So
+        // it goes without 4, or, if there are more tiles than one for each CTA, without
+        // what looks better by this estimate, in us: a tile of 128 channels takes 2.3 of
+        // a prefix and 0.78 of the rest, by an SM's CTAs together, a quarter more where
+        // all SMs share HBM; CTAs come and go in waves. Of 19 batches it took the best
+        // of the three for 13, and one within 7 % for the others.
+        int64_t prefix_ctas(int64_t tiles, int64_t rows, int64_t rest, int64_t per, int64_t dim, int64_t sms) {
+            const int64_t most = std::max<int64_t>(1, sms - 4), runs = per * sms;
+            if (rest <= runs) return rest == 0 ? sms : most;
+            const double width = static_cast<double>(dim) / 128;
+            const double wave = 1 + static_cast<double>(rest) / static_cast<double>(runs) * 0.78 * static_cast<double>(per) * width;
+            auto takes = [&](int64_t ctas) {
+                ctas = std::min(ctas, tiles);
+                const double prefix = 4 + static_cast<double>(tiles + kRowCost * rows) / static_cast<double>(ctas) * 2.3 * width;
+                double t = 0;
+                int64_t left = runs;
+                for (int i = 1, j = 1; left > 0;) { // the next CTAs to end: of the other SMs, or after a prefix
+                    const double apart = i * wave, after = prefix + j * 1.25 * wave;
+                    const bool first = apart <= after;
+                    left -= per * (first ? sms - ctas : ctas);
+                    t = first ? apart : after;
+                    ++(first ? i : j);
+                }
+                return std::max(t, prefix);
+            };
+            int64_t best = most;
+            double least = 0.97 * takes(most);
+            for (int64_t part : {3, 2}) {
+                const int64_t ctas = std::max<int64_t>(1, sms - (sms + part - 1) / part);
+                const double t = takes(ctas);
+                if (t >= least) continue;
+                best = ctas;
+                least = t;
+            }
+            return best;
         }
 
         // The form of what follows the prefixes, and of prefixes without a stage of
@@ -1632,7 +1674,12 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             runs first;
             const auto prefix_rows = static_cast<int32_t>(tiles.size());
             if (own_stage) {
-                first = share_out(tiles, sm_count(c.device), kRowCost);
+                int64_t rest = 0, all = 0; // tiles
+                for (int64_t s = 0; s < n; ++s)
+                    rest += (batch.lengths[static_cast<size_t>(s)] - begin[static_cast<size_t>(s)] + f.tile() - 1) / f.tile();
+                rest *= heads * ((group + p->rest.per - 1) / p->rest.per);
+                for (int64_t t : tiles) all += t;
+                first = share_out(tiles, prefix_ctas(all, prefix_rows, rest, f.per_sm(), c.dim, sm_count(c.device)), kRowCost);
                 tiles.clear();
             }
             for (int64_t s = 0; s < n; ++s) {
