@@ -477,7 +477,10 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
         int page = pb_page(at, tables, width, lane);
         if (!PB_LATE_WAIT) asm volatile("griddepcontrol.wait;" ::: "memory");
 #if PB_TEST_STALL == 1
-        if (blockIdx.x == 0) return; // its tiles never arrive
+        if (blockIdx.x == 0) { // its tiles never arrive
+            if (PB_LATE_WAIT) asm volatile("griddepcontrol.wait;" ::: "memory");
+            return;
+        }
 #endif
         for (int i = 0; i < mine.z && !bad; ++i) {
             const int base = pb_base(at), boxes = (min(PB_TS, at.length - base) + PB_BOX - 1) / PB_BOX;
