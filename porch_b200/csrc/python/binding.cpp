@@ -112,6 +112,29 @@ namespace {
         return checked(status);
     }
 
+    // {"shape": shape, "typestr": "<f4", "data": (address, False), "version": 3,
+    // "stream": stream}; takes `shape`. What is the same in each is made once.
+    PyObject* interface_of(PyObject* shape, uint64_t address, uint64_t stream) {
+        static PyObject* const words[] = {PyUnicode_InternFromString("shape"), PyUnicode_InternFromString("typestr"),
+                                          PyUnicode_InternFromString("data"), PyUnicode_InternFromString("version"),
+                                          PyUnicode_InternFromString("stream"), PyUnicode_InternFromString("<f4")};
+        static PyObject* const version = PyLong_FromLong(3);
+        PyObject* data = PyTuple_New(2);
+        PyObject* at = PyLong_FromUnsignedLongLong(address);
+        PyObject* on = PyLong_FromUnsignedLongLong(stream);
+        PyObject* face = PyDict_New();
+        bool good = data != nullptr && at != nullptr && on != nullptr && face != nullptr;
+        if (good) {
+            PyTuple_SET_ITEM(data, 0, Py_NewRef(at));
+            PyTuple_SET_ITEM(data, 1, Py_NewRef(Py_False));
+            PyObject* const values[] = {shape, words[5], data, version, on};
+            for (int i = 0; i < 5; ++i) good = good && PyDict_SetItem(face, words[i], values[i]) == 0;
+        }
+        if (!good) Py_CLEAR(face);
+        for (PyObject* x : {shape, data, at, on}) Py_XDECREF(x);
+        return face;
+    }
+
     // The address of a realised tensor's values stays what it is once it was
     // handed out, so consumers that ask twice cost one call.
     PyObject* handle_interface(PyObject* self, void*) {
@@ -124,9 +147,8 @@ namespace {
             PyObject* shape = PyTuple_New(static_cast<Py_ssize_t>(v[0]));
             if (shape == nullptr) return nullptr;
             for (int64_t i = 0; i < v[0]; ++i) PyTuple_SET_ITEM(shape, i, PyLong_FromLongLong(v[3 + i]));
-            PyObject* face = Py_BuildValue("{s:N,s:s,s:(KO),s:i,s:K}", "shape", shape, "typestr", "<f4", "data",
-                                           static_cast<unsigned long long>(v[1]), Py_False, "version", 3, "stream",
-                                           static_cast<unsigned long long>(v[2]));
+            PyObject* face = interface_of(shape, static_cast<uint64_t>(v[1]), static_cast<uint64_t>(v[2]));
+            if (face == nullptr) return nullptr;
             if (h->face == nullptr)
                 h->face = face;
             else
