@@ -1201,6 +1201,10 @@ static __device__ __forceinline__ void pb_join(const int4* joins, const float* p
     const int heads = min(group, PB_HT);
     const int4 r = joins[block / heads]; // of the plan, in place before the launch
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    // The next launch may begin beside this one (48 sequences to 8191 slots, in 8 and in
+    // 16 bits: 72.4 and 125 us a call, 72.9 and 127 where it waits for its end). After
+    // pb_shared_finish that took 0.8 us longer: its next launch needs whole SMs.
+    asm volatile("griddepcontrol.launch_dependents;");
     const int head = block % heads, chunk = r.x % chunks, kvh = (r.x / chunks) % PB_H, s = r.x / chunks / PB_H;
     if (head >= group - chunk * PB_HT) return;
     const pb_i64 global = (pb_i64)s * PB_H * group + kvh * group + chunk * PB_HT + head;
@@ -1296,6 +1300,7 @@ static __device__ __forceinline__ void pb_scores(const int4* joins, const int* s
     const int i0 = (int)(block % blocks) * (4 * PB_JOIN_THREADS) + threadIdx.x; // lengths are below 2^30
     const int length = lengths[row / PB_H];
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;");
     const float* before = scores + row * ns;
     float a[4];
 #pragma unroll
