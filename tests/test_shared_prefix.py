@@ -324,3 +324,21 @@ def test_many_parts_and_many_rows(gpu):
     out, tol, _, _ = host.attend(q, 0.125)
     got = gpu.paged_attention(gpu.tensor(list(q.shape), q), batch).cpu().reshape(q.shape)
     assert (np.abs(got - out) <= tol).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("members,shared,own,heads,group,dim", [
+    (64, 4096, 250, 8, 4, 128), (64, 4096, 400, 8, 2, 64), (60, 1024, 700, 8, 1, 80), (63, 6144, 70, 8, 8, 16)])
+def test_what_follows_runs_beside_the_prefix(gpu, members, shared, own, heads, group, dim):
+    # More tiles behind the prefix than CTAs at once: the launches share the SMs.
+    rng = np.random.default_rng(members + own)
+    lengths = [shared + own + s % 5 for s in range(members)]
+    lengths[7] = shared
+    host = Shared(rng, [(members, shared)], lengths, heads, dim, 64, "bf16")
+    _, batch = host.build(gpu)
+    q = rng.normal(0, 1, (members, heads * group, dim)).astype(np.float32)
+    t = gpu.tensor(list(q.shape), q)
+    got = [gpu.paged_attention(t, batch).cpu() for _ in range(3)]
+    out, tol, _, _ = host.attend(q, dim**-0.5)
+    assert (np.abs(got[0].reshape(q.shape) - out) <= tol).all()
+    assert all(np.array_equal(got[0], x) for x in got[1:])
