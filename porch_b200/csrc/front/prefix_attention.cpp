@@ -26,8 +26,8 @@
 //
 // Bound: tensor cores and the shared memory that feeds them. With three terms S and
 // P V are 6 products of 128 x 128 x head_dim a tile where the formula has 2. 64
-// sequences behind 16384 slots, 32 heads of 128 over 8: 43 to 46 us with the tensor
-// pipe 68 % busy; a tile takes 4300 cycles, some 2100 of them S, whose operands both
+// sequences behind 16384 slots, 32 heads of 128 over 8: 43 to 46 us on every SM with
+// the tensor pipe 68 % busy (it leaves some to what follows: prefix_ctas()); a tile takes 4300 cycles, some 2100 of them S, whose operands both
 // come from shared memory, and 1750 P V, whose weights come from tensor memory. Every mbarrier wait
 // is bounded, and nobody leaves while loads or MMAs are in flight.
 #include "operators.hpp"
