@@ -446,7 +446,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
     float* wmax = reinterpret_cast<float*>(raw + (ps + PB_TERMS * PB_HT * PB_PROW - pb_smem(raw)));
     float* wsum = wmax + 4 * PB_HT;
 #if PB_ESZ == 1
-    float* wscaled = wsum + 4 * PB_HT; // the warps' maxima of weight x value scale, in log2
+    float* wscaled = wsum + 4 * PB_HT; // the warps' maxima of weight x value scale, in log2 and relative to wmax
     float* units = wscaled + 4 * PB_HT; // of the row's queries
 #endif
     const pb_u32 full = pb_smem(bars), empty = full + 8 * PB_RING;
@@ -745,8 +745,10 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 float x = PB_LOWEST;
+                const float from = fmaxf(top[n][e], PB_LOWEST);
 #pragma unroll
-                for (int b = 0; b < PB_MB; ++b) x = pb_max_nan(x, pb_max_nan(s[b][n][e] + scaled[b][0], s[b][n][e + 2] + scaled[b][1]));
+                for (int b = 0; b < PB_MB; ++b)
+                    x = pb_max_nan(x, pb_max_nan((s[b][n][e] - from) + scaled[b][0], (s[b][n][e + 2] - from) + scaled[b][1]));
                 x = pb_max_nan(x, __shfl_xor_sync(0xffffffffu, x, 4));
                 x = pb_max_nan(x, __shfl_xor_sync(0xffffffffu, x, 8));
                 x = pb_max_nan(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -763,24 +765,24 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
         // weight x value scale, in units of which a tile's largest is up to
         // PB_DIGITS (but for 2^-10 of it, what its logarithms may be off by) and
         // at least half that; the unit is 2^power of the weights' over that.
+        // Logits are taken relative to a warp's maximum before the scale's logarithm
+        // is added, and the warp's to the running one after that: such a difference
+        // is exact where the two lie within a factor of two, and otherwise matters
+        // only up to some 2^9 (beyond, weight x scale is below 2^-100), so whatever
+        // size logits have, five sums are off by 2^-16 each at most, lg2 by 2^-15 and
+        // the weight's own exponent by 2^-16: 2^-13.7 of the weight. (Adding the
+        // logarithm to the logit itself rounded it at the logit's size, and from 2^15
+        // on a weight could pass PB_DIGITS and come out negative.)
         float power[PB_NT][2];
-#pragma unroll
-        for (int n = 0; n < PB_NT; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                float x = PB_LOWEST;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) x = pb_max_nan(x, wscaled[w * PB_HT + 8 * n + 2 * t + e]);
-                power[n][e] = x;
-            }
 #endif
 #pragma unroll
         for (int n = 0; n < PB_NT; ++n) {
+            float2 x[4];
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                const float2 x = *reinterpret_cast<const float2*>(wmax + w * PB_HT + 8 * n + 2 * t);
-                top[n][0] = fmaxf(top[n][0], x.x);
-                top[n][1] = fmaxf(top[n][1], x.y);
+                x[w] = *reinterpret_cast<const float2*>(wmax + w * PB_HT + 8 * n + 2 * t);
+                top[n][0] = fmaxf(top[n][0], x[w].x);
+                top[n][1] = fmaxf(top[n][1], x[w].y);
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -789,8 +791,12 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                 m[n][e] = now;
                 l[n][e] *= corr[n][e];
 #if PB_ESZ == 1
+                float most = PB_LOWEST;
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+                    most = pb_max_nan(most, wscaled[w * PB_HT + 8 * n + 2 * t + e] + (fmaxf(e ? x[w].y : x[w].x, PB_LOWEST) - now));
                 // What lies 2^-100 below the running maximum's weight weighs nothing.
-                power[n][e] = pb_max_nan(ceilf(power[n][e] - now), -100.0f);
+                power[n][e] = pb_max_nan(ceilf(most), -100.0f);
 #endif
             }
 #pragma unroll
