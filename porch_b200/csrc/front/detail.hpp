@@ -44,6 +44,10 @@ namespace porch::detail {
     // The calling thread's host-to-device upload stream on `device`
     // (pb_tensor_create_async); readers order behind it with events.
     std::shared_ptr<stream_ref> upload_stream(int device);
+    // Another stream of the calling thread on `device`, for a launch that runs beside
+    // one on its current stream: whoever uses it orders it behind that stream before,
+    // and that stream behind it after.
+    std::shared_ptr<stream_ref> side_stream(int device);
 
     // ------------------------------------------------------- dry run --
     // True while a plan is being inspected without a device (placeholder

@@ -44,6 +44,7 @@ namespace porch::detail {
         };
         thread_local thread_stream_table tl_streams;
         thread_local thread_stream_table tl_upload_streams;
+        thread_local thread_stream_table tl_side_streams;
 
         std::shared_ptr<stream_ref> stream_in(thread_stream_table& t, int device) {
             auto& table = t.streams;
@@ -62,6 +63,7 @@ namespace porch::detail {
     } // namespace
 
     std::shared_ptr<stream_ref> upload_stream(int device) { return stream_in(tl_upload_streams, device); }
+    std::shared_ptr<stream_ref> side_stream(int device) { return stream_in(tl_side_streams, device); }
 
     std::shared_ptr<stream_ref> current_stream(int device) {
         auto& table = tl_streams.streams;

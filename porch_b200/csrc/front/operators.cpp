@@ -161,6 +161,15 @@ namespace porch::detail {
         return tensor_access::from_storage(std::move(r.shape), std::move(r.storage), placement);
     }
 
+    void order_behind(const std::shared_ptr<stream_ref>& first, const std::shared_ptr<stream_ref>& stream) {
+        pbrt_event e = nullptr;
+        check(pbrt_event_create(first->device, 0, &e));
+        int s = pbrt_event_record(first->device, e, first->stream);
+        if (s == PBRT_OK) s = pbrt_stream_wait_event(stream->device, stream->stream, e);
+        (void)pbrt_event_destroy(first->device, e);
+        check(s);
+    }
+
     void order_write(cuda_jit::device_buffer_state& buffer, const std::shared_ptr<stream_ref>& stream) {
         std::vector<std::shared_ptr<stream_ref>> others;
         {
@@ -171,14 +180,7 @@ namespace porch::detail {
             buffer.readers.clear();
             buffer.producer = stream;
         }
-        for (const auto& o : others) {
-            pbrt_event e = nullptr;
-            check(pbrt_event_create(o->device, 0, &e));
-            int s = pbrt_event_record(o->device, e, o->stream);
-            if (s == PBRT_OK) s = pbrt_stream_wait_event(stream->device, stream->stream, e);
-            (void)pbrt_event_destroy(o->device, e);
-            check(s);
-        }
+        for (const auto& o : others) order_behind(o, stream);
     }
 
     std::string operator_sources() {

@@ -85,6 +85,9 @@ namespace porch::detail {
         return st == nullptr ? 0 : st->ptr;
     }
 
+    // Makes `stream` wait for what is enqueued on `first` so far.
+    void order_behind(const std::shared_ptr<stream_ref>& first, const std::shared_ptr<stream_ref>& stream);
+
     // Makes `stream` wait for everything that reads or wrote the buffer on
     // other streams and then owns it: called before a kernel writes in place.
     void order_write(cuda_jit::device_buffer_state& buffer, const std::shared_ptr<stream_ref>& stream);

@@ -69,7 +69,7 @@ namespace porch::detail {
         struct form {
             int heads = 1, dim = 0, page = 0;
             cache_type type = cache_type::f32;
-            bool scored = false, shared = false, late = false;
+            bool scored = false, shared = false;
             int stall = 0; // the test hook's mode
             int join_threads = 128;
             int tiles8 = 1; // groups of 8 query heads that a row holds (1 or 2)
@@ -426,10 +426,6 @@ static __device__ __forceinline__ void pb_split_queries(const pb_queries& r, pb_
 }
 #endif
 
-// PB_LATE_WAIT: what follows a prefix's own launch, which lets it begin once all
-// before that launch is complete, and neither reads nor writes what the other
-// writes. It takes SMs that the other leaves and those that come free, and ends
-// after the other has, so that who waits for this kernel has both.
 extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
     const __grid_constant__ pb_tmap map_k, const __grid_constant__ pb_tmap map_v, const float* q, const int* lengths,
     const int* tables, const int4* work, float* out, float* partial, float2* partial_ml, float* logits, float2* norms,
@@ -475,12 +471,9 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
         pb_u32 parity = 1; // the first round finds every unit free
         bool bad = false;
         int page = pb_page(at, tables, width, lane);
-        if (!PB_LATE_WAIT) asm volatile("griddepcontrol.wait;" ::: "memory");
+        asm volatile("griddepcontrol.wait;" ::: "memory");
 #if PB_TEST_STALL == 1
-        if (blockIdx.x == 0) { // its tiles never arrive
-            if (PB_LATE_WAIT) asm volatile("griddepcontrol.wait;" ::: "memory");
-            return;
-        }
+        if (blockIdx.x == 0) return; // its tiles never arrive
 #endif
         for (int i = 0; i < mine.z && !bad; ++i) {
             const int base = pb_base(at), boxes = (min(PB_TS, at.length - base) + PB_BOX - 1) / PB_BOX;
@@ -519,13 +512,11 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                 }
             }
         }
-        // One CTA is enough, and the last keeps nobody from its SM.
-        if (PB_LATE_WAIT && blockIdx.x + 1 == gridDim.x) asm volatile("griddepcontrol.wait;" ::: "memory");
         return;
     }
 
     // ---- four computing warps
-    if (!PB_LATE_WAIT) asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     if (mine.z == 0) { // a row without slots
         for (int e = threadIdx.x; e < pb_heads(at, group) * PB_D; e += 128)
             out[pb_query(at, e / PB_D, group, PB_H * group, 1) * PB_D + e % PB_D] = 0.0f;
@@ -1391,7 +1382,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
                << "\n#define PB_TS " << f.tile()
                << "\n#define PB_JOIN_THREADS " << f.join_threads << "\n#define PB_PER_SM " << f.per_sm()
                << "\n#define PB_STATIC " << form::kStatic << "\n#define PB_SCORED " << (f.scored ? 1 : 0) << "\n#define PB_SHARED " << (f.shared ? 1 : 0)
-               << "\n#define PB_LATE_WAIT " << (f.late ? 1 : 0) << "\n";
+               << "\n";
             if (f.stall != 0) os << "#define PB_TEST_STALL " << f.stall << "\n";
             return os.str();
         }
@@ -1417,7 +1408,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         const char kSharedFinish[] = "pb_shared_finish";
 
         op_kernel& kernel_of(const char* name, const form& f, uint32_t smem) {
-            const op_key key{reinterpret_cast<int64_t>(name), f.heads, f.dim, f.page, static_cast<int64_t>(f.type), f.scored, f.tiles8, f.join_threads, f.stall, f.shared + 2 * f.late};
+            const op_key key{reinterpret_cast<int64_t>(name), f.heads, f.dim, f.page, static_cast<int64_t>(f.type), f.scored, f.tiles8, f.join_threads, f.stall, f.shared};
             return op_kernel_for(key, [&](op_kernel& k) {
                 k.name = name;
                 k.source = std::string{kernel_prelude()} + defines(f) + device_source();
@@ -1592,14 +1583,14 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
 
         // How many CTAs (SMs) work through prefixes in their own launch, while what
         // follows them has the other SMs, `per` CTAs each, and then all. 32 query heads
-        // over 8 of 128 channels, 64 sequences of 400 slots behind 16384: 72 us where
-        // the prefix has every SM, 69 without 4, 63 without a third, 76 without half.
-        // Of 256 behind 4096: 37, 35, 36, 31. Of 64 behind 16384: 51, 50, 58, 71. So
-        // it goes without 4, or, if there are more tiles than one for each CTA, without
-        // what looks better by this estimate, in us: a tile of 128 channels takes 2.3 of
-        // a prefix and 0.78 of the rest, by an SM's CTAs together, a quarter more where
-        // all SMs share HBM; CTAs come and go in waves. Of 19 batches it took the best
-        // of the three for 13, and one within 7 % for the others.
+        // over 8 of 128 channels, inputs rotated past the L2 cache: 64 sequences of 400
+        // slots behind 16384 take 69.5 us where the prefix has all SMs but 4, 67.0
+        // without a third, 79.6 without half; of 777 82, 85 and 81; of 256 behind 4096
+        // 40.4, 41.5 and 37.7; of 400 behind 2048 42 each. So it goes without 4, or, if
+        // there are more tiles than one for each CTA, without what looks better by this
+        // estimate, in us: a tile of 128 channels takes 2.3 of a prefix and 0.78 of the
+        // rest, by an SM's CTAs together, a quarter more where all SMs share HBM; CTAs
+        // come and go in waves. It took the best of the three for these four.
         int64_t prefix_ctas(int64_t tiles, int64_t rows, int64_t rest, int64_t per, int64_t dim, int64_t sms) {
             const int64_t most = std::max<int64_t>(1, sms - 4), runs = per * sms;
             if (rest <= runs) return rest == 0 ? sms : most;
@@ -1636,8 +1627,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         form shared_form(const kv_batch& batch, int64_t group) {
             form f = form_of(*batch.cache, group);
             f.shared = true;
-            f.late = prefix_stage(batch, group);
-            if (f.late) return f;
+            if (prefix_stage(batch, group)) return f;
             int64_t most = group;
             for (const auto& g : batch.groups) most = std::max(most, g.members * group);
             f.tiles8 = most > 8 ? 2 : 1;
@@ -1809,6 +1799,15 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
                 std::scoped_lock lock{c.order};
                 order_read(*cuda_jit::buffer_access::state(c.k), stream);
                 order_read(*cuda_jit::buffer_access::state(c.v), stream);
+                // What follows a prefix runs beside it on a stream of its own, behind
+                // all that came before both; each kernel waits for that in the way of
+                // its stream. (On one stream the second waits for the first: 64 sequences
+                // of 400 slots behind 16384, 32 heads over 8 of 128, inputs rotated past
+                // the L2 cache: 69.7 us so, 66.9 apart; of 256 behind 4096 40.7 and 37.5,
+                // of 1 behind 2048 31.3 and 27.5; 2 of 1 behind 16384 20.0 and 20.4.)
+                const bool apart = prefix != nullptr && rest != nullptr;
+                const auto side = apart ? side_stream(device) : stream;
+                if (apart) order_behind(stream, side);
                 if (prefix != nullptr) {
                     void* params[] = {&c.map_k, &c.map_v, &queries, &rows1,  &batch.tables_at, &work1,     &partial1, &ml1,
                                       &width,   &group,   &q_seq,   &q_head, &pool_rows,       &scale2,    &err};
@@ -1817,7 +1816,15 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
                 if (rest != nullptr) {
                     void* params[] = {&c.map_k, &c.map_v, &queries, &rows2, &batch.tables_at, &work2, &out.ptr, &partial2, &ml2, &none, &none,
                                       &width,   &group,   &chunks,  &q_seq, &q_head, &longest, &scale2, &err, &scales_k, &scales_v};
-                    op_launch(*rest, device, stream, {static_cast<uint32_t>(plan.rest.ctas), 1, 1}, 160, params);
+                    op_launch(*rest, device, side, {static_cast<uint32_t>(plan.rest.ctas), 1, 1}, 160, params);
+                }
+                if (apart) {
+                    try {
+                        order_behind(side, stream);
+                    } catch (...) { // the workspace goes back to `stream`, which does not know of the launch
+                        (void)pbrt_stream_synchronize(device, side->stream);
+                        throw;
+                    }
                 }
             }
             // Without a stage of their own the prefixes' parts are among the others.
@@ -2012,8 +2019,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             f.tiles8 = tiles8;
             f.page = page;
             f.shared = page == 32;
-            f.late = f.shared && width == 2;
-            f.join_threads = f.late ? 32 : 128;
+            f.join_threads = f.shared && width == 2 ? 32 : 128;
             f.scored = !f.shared;
             out.emplace_back("pb_paged_attention_" + std::to_string(dim) + (width == 1 ? "_i8_" : (width == 2 ? "_bf16_" : "_f32_")) + std::to_string(8 * tiles8) + (f.shared ? "_shared" : ""),
                              std::string{kernel_prelude()} + defines(f) + device_source());

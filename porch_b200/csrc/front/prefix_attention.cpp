@@ -218,8 +218,8 @@ extern "C" __global__ void __launch_bounds__(384, 1) pb_prefix_attention(
     if (warp == 0) {
         // ---- producer
         asm volatile("griddepcontrol.wait;" ::: "memory");
-        // Every CTA has its SM by the time that all are here; the next launch takes
-        // those that come free first.
+        // Every CTA has its SM by the time that all are here; the join, which is next on
+        // this stream, may come in as SMs come free and waits there.
         asm volatile("griddepcontrol.launch_dependents;");
         int unit = 0, row = mine.x, tile = mine.y, left = mine.z;
         bool good = true;
