@@ -1561,24 +1561,55 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
             return prefix_attention_takes(*batch.cache) && most > 16;
         }
 
-        // Whether working through the prefixes once pays: it takes up to two launches
-        // more, so where it spares reading less than some 62 MB (most of which the L2
-        // cache would deliver) every sequence reads its prefix itself. 32 query heads
-        // over 8 of 128 bfloat16 channels, shared and by themselves: 8 sequences behind
-        // 2048 slots (59 MB) 14.7 and 14.2 us, 16 behind 1024 (63 MB) 12.4 and 15.6, 64
-        // behind 256 (65 MB) 16.2 and 17.1, 2 behind 16384 (67 MB) 17.8 and 24.1, 8
-        // behind 4096 (117 MB) 17.5 and 23.2, 64 behind 2048 22.2 and 75.2. In float32
-        // 2 behind 8192 (67 MB) 16.6 and 22.1, 64 behind 384 (151 MB) 35.8 and 32.5, 16
-        // behind 2048 (201 MB) 27.1 and 35.5; in 8 bits 2 behind 32768 (67 MB) 18.1 and
-        // 25.2, 64 behind 1024 (101 MB) 29.4 and 28.0, behind 2048 39.1 and 45.0.
+        // The form of what follows the prefixes, and of prefixes without a stage of
+        // their own: 16 queries share a tile's loads where there are as many.
+        form shared_form(const kv_batch& batch, int64_t group) {
+            form f = form_of(*batch.cache, group);
+            f.shared = true;
+            if (prefix_stage(batch, group)) return f;
+            int64_t most = group;
+            for (const auto& g : batch.groups) most = std::max(most, g.members * group);
+            f.tiles8 = most > 8 ? 2 : 1;
+            if (f.ring() < 3) f.tiles8 = 1;
+            return f;
+        }
+
+        // Whether working through the prefixes once pays, by an estimate of both sides in
+        // us. Either way a row of up to 8 queries (16 where there are more) takes
+        // `pass8` (`pass16`) for each MB of keys and values that it works through, most
+        // of which the L2 cache delivers; sharing makes fewer rows of the prefixes, 128
+        // queries each where they have a launch of their own, and takes `start` for the
+        // launches and parts that it adds, and `joined` for each million channels that
+        // are joined. Fitted to 398 batches of 2 to 64 sequences, inputs rotated past the
+        // L2 cache; for 18 of them it takes what took over 5 % (at most 31 %) longer. 32
+        // query heads over 8 of 128 channels, shared and by themselves: in bfloat16 2
+        // sequences behind 16384 slots 20.0 and 24.1 us, 8 behind 2048 19.7 and 14.4,
+        // behind 8192 26.9 and 39.8, 64 behind 256 20.7 and 17.7, behind 512 21.3 and
+        // 26.9; in float32 64 behind 256 37.6 and 26.8, behind 1024 54.8 and 68.5; in 8
+        // bits 64 behind 1024 30.1 and 28.8, behind 2048 40.5 and 46.5.
         bool worth_sharing(const kv_batch& batch, int64_t group) {
+            if (batch.groups.empty()) return false;
+            if (g_test_share.load(std::memory_order_relaxed)) return true;
+            struct rates {
+                double start, joined, pass8, pass16;
+            };
+            constexpr rates kF32{2.5, 34, 0.078, 0.135}, kBf16{4.0, 17, 0.094, 0.19}, kI8{3.9, 17, 0.070, 0.122},
+                kStage{5.0, 7.4, 0.085, 0.156};
+            constexpr double kPass128 = 0.325;
             const kv_cache& c = *batch.cache;
-            const int64_t per = prefix_stage(batch, group) ? 128 : 16; // queries that read a prefix together
-            double slots = 0; // that are not read again
+            const bool stage = prefix_stage(batch, group);
+            const rates& r = stage ? kStage : (c.type == cache_type::f32 ? kF32 : (c.type == cache_type::bf16 ? kBf16 : kI8));
+            const form apart = form_of(c, group), together = shared_form(batch, group);
+            const int64_t per = stage ? 128 : 8 * together.tiles8; // queries that read a prefix together
+            const double alone = apart.tiles8 == 2 ? r.pass16 : r.pass8;
+            const double shared = stage ? kPass128 : (together.tiles8 == 2 ? r.pass16 : r.pass8);
+            double spared = 0; // us for each MB of a slot
             for (const auto& g : batch.groups)
-                slots += static_cast<double>(g.members - (g.members * group + per - 1) / per) * static_cast<double>(g.slots);
-            return !batch.groups.empty() && (g_test_share.load(std::memory_order_relaxed) ||
-                                             slots * static_cast<double>(c.heads * 2 * c.dim * c.width()) >= 62e6);
+                spared += static_cast<double>(g.slots) * (static_cast<double>(g.members * apart.chunks(static_cast<int>(group))) * alone -
+                                                          static_cast<double>((g.members * group + per - 1) / per) * shared);
+            const double slot = static_cast<double>(c.heads * 2 * c.dim * c.width()) * 1e-6;
+            const double channels = static_cast<double>(batch.sequences() * c.heads * group * c.dim) * 1e-6;
+            return spared * slot > r.start + r.joined * channels;
         }
 
         // How many CTAs (SMs) work through prefixes in their own launch, while what
@@ -1620,19 +1651,6 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
                 least = t;
             }
             return best;
-        }
-
-        // The form of what follows the prefixes, and of prefixes without a stage of
-        // their own: 16 queries share a tile's loads where there are as many.
-        form shared_form(const kv_batch& batch, int64_t group) {
-            form f = form_of(*batch.cache, group);
-            f.shared = true;
-            if (prefix_stage(batch, group)) return f;
-            int64_t most = group;
-            for (const auto& g : batch.groups) most = std::max(most, g.members * group);
-            f.tiles8 = most > 8 ? 2 : 1;
-            if (f.ring() < 3) f.tiles8 = 1;
-            return f;
         }
 
         // The plan for `group` query heads of each key head, which the cache's next
