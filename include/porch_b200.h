@@ -377,7 +377,7 @@ int pb_kv_read(pb_kv_batch* batch, pb_tensor** k, pb_tensor** v);
 int pb_paged_attention(const pb_tensor* q, pb_kv_batch* batch, float scale, pb_tensor** out);
 /* How the attention of a batch with these lengths is shared out over about
  * `ctas` CTAs, as text, without a GPU: a row is a (sequence, key head, chunk of
- * query heads), a tile 64 slots of it. "work <row> <tile> <tiles>" for each CTA
+ * query heads), a tile 64 slots of it, as in a float32 or bfloat16 cache. "work <row> <tile> <tiles>" for each CTA
  * (its first row and tile, and how many it works through; none: it clears a
  * row without slots), and "join <row> <first CTA> <parts> <place>" for each row
  * in several parts (place: whether the first CTA's part is its first, 0, or its
@@ -385,6 +385,11 @@ int pb_paged_attention(const pb_tensor* q, pb_kv_batch* batch, float scale, pb_t
 int pb_kv_plan_describe(const int64_t* lengths, size_t sequences, int64_t kv_heads,
                         int64_t chunks, int64_t ctas, char* text, size_t capacity,
                         size_t* needed);
+/* The same for a cache of this head size and type: tiles of an int8 cache have 128
+ * slots up to head_dim 128. */
+int pb_kv_plan_describe_for(int64_t head_dim, int type, const int64_t* lengths, size_t sequences,
+                            int64_t kv_heads, int64_t chunks, int64_t ctas, char* text,
+                            size_t capacity, size_t* needed);
 /* How many CTAs of an SM the attention counts on that serves `group` query
  * heads of each key head from a cache of this head size and type, and the bytes
  * of shared memory that each of them takes, the system's share included. */

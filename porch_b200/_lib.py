@@ -142,6 +142,8 @@ def _declare(L: ctypes.CDLL) -> None:
         "pb_paged_attention_scored": (c_int, [T, T, T, c_float, P(T), P(T)]),
         "pb_kv_plan_describe": (c_int, [P(c_int64), c_size_t, c_int64, c_int64, c_int64, c_char_p, c_size_t,
                                         P(c_size_t)]),
+        "pb_kv_plan_describe_for": (c_int, [c_int64, c_int, P(c_int64), c_size_t, c_int64, c_int64, c_int64, c_char_p,
+                                            c_size_t, P(c_size_t)]),
         "pb_kv_attention_shape": (c_int, [c_int64, c_int, c_int64, P(c_int64), P(c_int64)]),
         "pb_kv_evict": (c_int, [T, T, T, c_int64, c_int64, c_int64, P(T), P(T)]),
         "pb_operator_sources": (c_int, [c_char_p, c_size_t, P(c_size_t)]),

@@ -548,6 +548,12 @@ def token_logprobs_backward(d_logprobs, logits, tokens, norm, d_entropy=None, en
     return _binding.token_logprobs_backward(d_logprobs, logits, tokens, norm, d_entropy, entropy)
 
 
+def _cache_type(dtype: str) -> int:
+    if dtype not in ("f32", "bf16", "int8"):
+        raise InvalidArgument('cache: dtype must be "f32", "bf16" or "int8"')
+    return {"f32": 0, "bf16": 1, "int8": 3}[dtype]
+
+
 class _Pool:
     """A cache pool in place, for another library on the same GPU; a bfloat16
     pool as its 16 raw bits, an int8 pool's scales as a pool of their own. Keeps
@@ -577,10 +583,8 @@ class KVCache:
 
     def __init__(self, pages: int, page_size: int, kv_heads: int, head_dim: int, dtype: str = "f32", device: int = 0):
         self._h = c_void_p()
-        if dtype not in ("f32", "bf16", "int8"):
-            raise InvalidArgument('cache: dtype must be "f32", "bf16" or "int8"')
-        _check(lib().pb_kv_cache_create(int(pages), int(page_size), int(kv_heads), int(head_dim),
-                                        {"f32": 0, "bf16": 1, "int8": 3}[dtype], int(device), byref(self._h)))
+        _check(lib().pb_kv_cache_create(int(pages), int(page_size), int(kv_heads), int(head_dim), _cache_type(dtype),
+                                        int(device), byref(self._h)))
         self.pages, self.page_size, self.kv_heads, self.head_dim = int(pages), int(page_size), int(kv_heads), int(head_dim)
         self.dtype, self.device = dtype, int(device)
 
@@ -681,15 +685,17 @@ class Batch:
         return _binding.kv_read(self._address)
 
 
-def attention_plan(lengths, kv_heads: int, ctas: int, chunks: int = 1) -> str:
-    """How the attention of a batch with these lengths is shared out over
-    `ctas` CTAs (pb_kv_plan_describe); needs no GPU."""
+def attention_plan(lengths, kv_heads: int, ctas: int, chunks: int = 1, dtype: str = "f32", head_dim: int = 128) -> str:
+    """How the attention of a batch with these lengths, over a cache of this
+    type and head size, is shared out over `ctas` CTAs
+    (pb_kv_plan_describe_for); needs no GPU."""
     a = np.ascontiguousarray(lengths, dtype=np.int64)
-    args = (a.ctypes.data_as(ctypes.POINTER(c_int64)), a.size, int(kv_heads), int(chunks), int(ctas))
+    args = (int(head_dim), _cache_type(dtype), a.ctypes.data_as(ctypes.POINTER(c_int64)), a.size, int(kv_heads),
+            int(chunks), int(ctas))
     need = c_size_t(0)
-    _check(lib().pb_kv_plan_describe(*args, None, 0, byref(need)))
+    _check(lib().pb_kv_plan_describe_for(*args, None, 0, byref(need)))
     buf = ctypes.create_string_buffer(need.value)
-    _check(lib().pb_kv_plan_describe(*args, buf, need.value, byref(need)))
+    _check(lib().pb_kv_plan_describe_for(*args, buf, need.value, byref(need)))
     return buf.value.decode()
 
 

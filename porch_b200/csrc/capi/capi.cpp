@@ -943,11 +943,22 @@ namespace {
             text[n] = '\0';
         }
     }
+    // Head sizes and types that a cache can have.
+    bool attends(int64_t head_dim, int type) {
+        const bool known = type == PB_CACHE_F32 || type == PB_CACHE_BF16 || type == PB_CACHE_INT8;
+        return known && head_dim >= 8 && head_dim <= 256 && head_dim % (type == PB_CACHE_INT8 ? 16 : 8) == 0;
+    }
 } // namespace
 
 int pb_kv_plan_describe(const int64_t* lengths, size_t sequences, int64_t kv_heads, int64_t chunks, int64_t ctas,
                         char* text, size_t capacity, size_t* needed) {
+    return pb_kv_plan_describe_for(128, PB_CACHE_F32, lengths, sequences, kv_heads, chunks, ctas, text, capacity, needed);
+}
+
+int pb_kv_plan_describe_for(int64_t head_dim, int type, const int64_t* lengths, size_t sequences, int64_t kv_heads,
+                            int64_t chunks, int64_t ctas, char* text, size_t capacity, size_t* needed) {
     return guarded([&] {
+        if (!attends(head_dim, type)) throw std::invalid_argument("plan: no such head size or type");
         if (sequences != 0) require(lengths, "lengths");
         // What a batch and its attention allow, so that nothing here overflows.
         constexpr int64_t most_length = int64_t{1} << 30, most_ctas = int64_t{1} << 20, most_rows = int64_t{1} << 27;
@@ -956,7 +967,8 @@ int pb_kv_plan_describe(const int64_t* lengths, size_t sequences, int64_t kv_hea
             std::any_of(lengths, lengths + sequences, [](int64_t v) { return v < 0 || v >= most_length; }))
             throw std::invalid_argument("plan: at most 65535 sequences of 0 to 2^30 slots, 1 to 1024 heads, 2^27 rows, 2^20 CTAs");
         std::vector<int64_t> n(lengths, lengths + sequences);
-        copy_text(porch::detail::attention_schedule(n, kv_heads, chunks, ctas), text, capacity, needed);
+        const auto kind = static_cast<porch::detail::cache_type>(type);
+        copy_text(porch::detail::attention_schedule(n, kv_heads, chunks, ctas, head_dim, kind), text, capacity, needed);
     });
 }
 
@@ -964,8 +976,7 @@ int pb_kv_attention_shape(int64_t head_dim, int type, int64_t group, int64_t* ct
     return guarded([&] {
         require(ctas_per_sm, "ctas_per_sm");
         require(shared_bytes, "shared_bytes");
-        if (head_dim < 8 || head_dim > 256 || head_dim % 8 != 0 || (type != PB_CACHE_F32 && type != PB_CACHE_BF16 && type != PB_CACHE_INT8) || (type == PB_CACHE_INT8 && head_dim % 16 != 0) || group < 1)
-            throw std::invalid_argument("attention shape: no such head size, type or group");
+        if (!attends(head_dim, type) || group < 1) throw std::invalid_argument("attention shape: no such head size, type or group");
         const auto [ctas, bytes] =
             porch::detail::attention_shape(head_dim, static_cast<porch::detail::cache_type>(type), group);
         *ctas_per_sm = ctas;

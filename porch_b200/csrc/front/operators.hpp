@@ -230,7 +230,8 @@ namespace porch::detail {
     void set_test_share_prefix(bool on);
     // The plan as text ("work <row> <tile> <tiles>" per CTA, "join <row>
     // <first CTA> <parts> <place>" per row), without a device.
-    std::string attention_schedule(const std::vector<int64_t>& lengths, int64_t heads, int64_t chunks, int64_t ctas);
+    std::string attention_schedule(const std::vector<int64_t>& lengths, int64_t heads, int64_t chunks, int64_t ctas,
+                                   int64_t dim, cache_type type);
 
     // The same sequences over another cache of the same shape; shares the upload.
     std::shared_ptr<kv_batch> batch_on(const kv_batch& batch, std::shared_ptr<kv_cache> cache);

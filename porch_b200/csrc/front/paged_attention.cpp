@@ -14,10 +14,11 @@
 // launch and the first loads' latency instead (about 6 us, 3 of the stream where
 // calls follow each other).
 //
-// pb_paged_attention, 160 threads: a producer warp loads tiles of 64 slots, K
-// then V, through a ring of TMA boxes (a page, or 64 rows of a larger one; 128
-// bytes wide, swizzled, zeros past the head size), and four computing warps
-// keep an online softmax over them: S^T = K Q^T for 16 slots each, a maximum
+// pb_paged_attention, 160 threads: a producer warp loads tiles of 64 slots (128 of
+// an 8-bit cache of up to 128 channels), K then V, through a ring of TMA boxes (a
+// page, or 64 rows of a larger one; 128 bytes wide, swizzled, zeros past the head
+// size), and four computing warps keep an online softmax over them: S^T = K Q^T for
+// 16 slots of each 64 a warp, a maximum
 // over the tile, weights to shared memory, O^T += V^T P^T for a quarter of the
 // channels each. The transposed products put slots and channels on the tensor
 // core's 16 rows and query heads on its 8 columns, so 1 to 8 heads cost the
@@ -1433,7 +1434,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         };
         constexpr int64_t kWholeRow = 8;
 
-        schedule make_schedule(const std::vector<int64_t>& lengths, int64_t heads, int64_t chunks, int64_t ctas, int64_t tile = 64) {
+        schedule make_schedule(const std::vector<int64_t>& lengths, int64_t heads, int64_t chunks, int64_t ctas, int64_t tile) {
             schedule r;
             const int64_t per = heads * chunks;
             int64_t total = 0, rows = 0, most = 0;
@@ -2014,8 +2015,9 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         (void)plan_of(batch, chunks, ctas);
     }
 
-    std::string attention_schedule(const std::vector<int64_t>& lengths, int64_t heads, int64_t chunks, int64_t ctas) {
-        const schedule s = make_schedule(lengths, heads, chunks, ctas);
+    std::string attention_schedule(const std::vector<int64_t>& lengths, int64_t heads, int64_t chunks, int64_t ctas,
+                                   int64_t dim, cache_type type) {
+        const schedule s = make_schedule(lengths, heads, chunks, ctas, tile_of(type, dim));
         std::ostringstream os;
         for (size_t i = 0; i < s.work.size(); i += 4)
             os << "work " << s.work[i] << " " << s.work[i + 1] << " " << s.work[i + 2] << "\n";
