@@ -434,8 +434,8 @@ int pb_test_gemm_stall(int enable);
  * while its first tiles are on their way (2); the kernel records a code of
  * 0x7d00 and more, and leaves when nothing is in flight any more. */
 int pb_test_attention_stall(int enable);
-/* While enabled, shared prefixes are worked through once whatever their size;
- * otherwise where that spares enough reading. Only for tests. */
+/* Shared prefixes of batches that are made while it is enabled are worked through
+ * once whatever their size; otherwise where that spares enough. Only for tests. */
 int pb_test_share_prefix(int enable);
 
 /* ---- matmul without allocation ------------------------------------------ */

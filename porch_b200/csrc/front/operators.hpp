@@ -202,6 +202,7 @@ namespace porch::detail {
             int64_t first = 0, members = 0, slots = 0;
         };
         std::vector<group> groups;
+        bool always_share = false;       // whatever they spare: made while the test hook was on
         cuda_jit::device_buffer data;    // int32: lengths, newest, tables, then 8-byte rows and starts
         // Made once with the batch for the number of query heads that its cache
         // last saw (up to 8 for each key head until then), and by the first
@@ -226,8 +227,10 @@ namespace porch::detail {
     // bounded waits expire (1), or gives up while its first ones are on their
     // way (2).
     void set_test_attention_stall(int mode);
-    // Test hook: prefixes are worked through once whatever their size.
+    // Test hook: of batches made while it is on, prefixes are worked through once
+    // whatever their size.
     void set_test_share_prefix(bool on);
+    bool test_share_prefix();
     // The plan as text ("work <row> <tile> <tiles>" per CTA, "join <row>
     // <first CTA> <parts> <place>" per row), without a device.
     std::string attention_schedule(const std::vector<int64_t>& lengths, int64_t heads, int64_t chunks, int64_t ctas,

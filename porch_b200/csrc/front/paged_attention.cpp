@@ -1590,7 +1590,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         // bits 64 behind 1024 30.1 and 28.8, behind 2048 40.5 and 46.5.
         bool worth_sharing(const kv_batch& batch, int64_t group) {
             if (batch.groups.empty()) return false;
-            if (g_test_share.load(std::memory_order_relaxed)) return true;
+            if (batch.always_share) return true;
             struct rates {
                 double start, joined, pass8, pass16;
             };
@@ -1959,6 +1959,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
 
     void set_test_attention_stall(int mode) { g_test_stall.store(mode); }
     void set_test_share_prefix(bool on) { g_test_share.store(on); }
+    bool test_share_prefix() { return g_test_share.load(std::memory_order_relaxed); }
 
     std::pair<int, int> attention_shape(int64_t dim, cache_type type, int64_t group) {
         kv_cache c;

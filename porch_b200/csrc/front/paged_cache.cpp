@@ -966,6 +966,7 @@ extern "C" __global__ void __launch_bounds__(256) pb_evict_move(
             starts.push_back(b->slots);
             b->table_width = std::max(b->table_width, pages);
         }
+        b->always_share = test_share_prefix();
         std::erase_if(b->groups, [](const kv_batch::group& g) { return g.members == 1; }); // shared with nobody
         if (b->shared_pages) {
             std::unordered_set<int64_t> distinct(rows.begin(), rows.end());
