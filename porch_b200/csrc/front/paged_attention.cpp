@@ -717,7 +717,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                 x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                top[n][e] = x;
+                top[n][e] = PB_ESZ == 1 ? fmaxf(x, PB_LOWEST) : x; // 8 bits: logits are taken relative to it
             }
             if (g == 0) *reinterpret_cast<float2*>(wmax + warp * PB_HT + 8 * n + 2 * t) = make_float2(top[n][0], top[n][1]);
         }
@@ -737,10 +737,9 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 float x = PB_LOWEST;
-                const float from = fmaxf(top[n][e], PB_LOWEST);
 #pragma unroll
                 for (int b = 0; b < PB_MB; ++b)
-                    x = pb_max_nan(x, pb_max_nan((s[b][n][e] - from) + scaled[b][0], (s[b][n][e + 2] - from) + scaled[b][1]));
+                    x = pb_max_nan(x, pb_max_nan((s[b][n][e] - top[n][e]) + scaled[b][0], (s[b][n][e + 2] - top[n][e]) + scaled[b][1]));
                 x = pb_max_nan(x, __shfl_xor_sync(0xffffffffu, x, 4));
                 x = pb_max_nan(x, __shfl_xor_sync(0xffffffffu, x, 8));
                 x = pb_max_nan(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -786,7 +785,7 @@ extern "C" __global__ void __launch_bounds__(160, PB_PER_SM) pb_paged_attention(
                 float most = PB_LOWEST;
 #pragma unroll
                 for (int w = 0; w < 4; ++w)
-                    most = pb_max_nan(most, wscaled[w * PB_HT + 8 * n + 2 * t + e] + (fmaxf(e ? x[w].y : x[w].x, PB_LOWEST) - now));
+                    most = pb_max_nan(most, wscaled[w * PB_HT + 8 * n + 2 * t + e] + ((e ? x[w].y : x[w].x) - now));
                 // What lies 2^-100 below the running maximum's weight weighs nothing.
                 power[n][e] = pb_max_nan(ceilf(most), -100.0f);
 #endif
