@@ -1581,7 +1581,7 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
         // queries each where they have a launch of their own, and takes `start` for the
         // launches and parts that it adds, and `joined` for each million channels that
         // are joined. Fitted to 398 batches of 2 to 64 sequences, inputs rotated past the
-        // L2 cache; for 18 of them it takes what took over 5 % (at most 31 %) longer. 32
+        // L2 cache; for 16 of them it takes what took over 5 % (at most 29 %) longer. 32
         // query heads over 8 of 128 channels, shared and by themselves: in bfloat16 2
         // sequences behind 16384 slots 20.0 and 24.1 us, 8 behind 2048 19.7 and 14.4,
         // behind 8192 26.9 and 39.8, 64 behind 256 20.7 and 17.7, behind 512 21.3 and
@@ -1594,11 +1594,13 @@ extern "C" __global__ void __launch_bounds__(PB_JOIN_THREADS) pb_paged_finish(
                 double start, joined, pass8, pass16;
             };
             constexpr rates kF32{2.5, 34, 0.078, 0.135}, kBf16{4.0, 17, 0.094, 0.19}, kI8{3.9, 17, 0.070, 0.122},
+                kI8Wide{7.0, 24, 0.069, 0.19}, // tiles of 64 slots
                 kStage{5.0, 7.4, 0.085, 0.156};
             constexpr double kPass128 = 0.325;
             const kv_cache& c = *batch.cache;
             const bool stage = prefix_stage(batch, group);
-            const rates& r = stage ? kStage : (c.type == cache_type::f32 ? kF32 : (c.type == cache_type::bf16 ? kBf16 : kI8));
+            const rates& r = stage ? kStage
+                                   : (c.type == cache_type::f32 ? kF32 : (c.type == cache_type::bf16 ? kBf16 : (tile_of(c.type, c.dim) == 128 ? kI8 : kI8Wide)));
             const form apart = form_of(c, group), together = shared_form(batch, group);
             const int64_t per = stage ? 128 : 8 * together.tiles8; // queries that read a prefix together
             const double alone = apart.tiles8 == 2 ? r.pass16 : r.pass8;

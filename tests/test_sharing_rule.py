@@ -37,6 +37,7 @@ def same_as_alone(gpu, dtype, members, shared, heads, group, dim):
     ("int8", 64, 1024, 8, 4, 128),
     ("bf16", 64, 256, 8, 4, 256),
     ("bf16", 8, 2048, 8, 4, 128),
+    ("int8", 16, 4096, 8, 4, 256),
     # Eight queries a row at this head size, so that nothing is spared.
     ("f32", 2, 8192, 4, 8, 256),
     ("f32", 4, 4096, 4, 8, 256),
