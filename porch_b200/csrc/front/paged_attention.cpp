@@ -8,9 +8,10 @@
 // Bound: HBM, which has to deliver every key and value in use once (2 x slots
 // x kv_heads x head_dim x 1, 2 or 4 bytes, and 4 for the scale of an 8-bit row).
 // 48 sequences up to 8191 slots, 32 query heads over 8 of 128 bfloat16 channels:
-// 784 MB in 126 us = 6.20 TB/s; one sequence of 262147 slots: 1074 MB in 165 us =
-// 6.5 TB/s, what a copy reaches. The same in 8 bits: 404 MB in 71 us and 554 MB in
-// 91, 5.7 and 6.1 TB/s with both launches. Few or short rows are bound by the
+// 784 MB in 127 us = 6.2 TB/s; one sequence of 262147 slots: 1074 MB in 171 us =
+// 6.3 TB/s. The same in 8 bits: 404 MB in 76 us and 554 MB in 100, 5.3 and 5.5 TB/s
+// with both launches (a call, inputs rotated past the L2 cache). Scored, the 48 take
+// 152 us in bfloat16 and 94 in 8 bits. Few or short rows are bound by the
 // launch and the first loads' latency instead (about 6 us, 3 of the stream where
 // calls follow each other).
 //
@@ -33,7 +34,11 @@
 // products start from zero and are added to the running sums in fp32, rounded to
 // nearest. An 8-bit cache is multiplied as it is: queries and weights are three
 // digits to base 256 of a whole number, whose sums of products are exact, and a
-// slot's scales go into its score and its weight.
+// slot's scales go into its score and its weight. Whole numbers have one unit for a
+// head's query, 2^-22 of its largest channel, and one for a tile's weights, 2^-22 of
+// its largest weight x value scale: what lies far below those has fewer bits than a
+// float32 of its own would, and the result is within the other caches' 4e-7 of the
+// largest that goes into it.
 //
 // Sequences that share a prefix (a prompt, say) read it once: their queries, up to
 // 16 for one key head here, or up to 128 where the large tiles of tcgen05 pay, are

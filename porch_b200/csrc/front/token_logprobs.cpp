@@ -14,9 +14,10 @@
 // by 2^-22 more (ex2) and 2^-23 |x - m|. log p and H are so good to about 1e-7
 // absolutely, not relative to a log p near 0. One launch: a row that few others keep company is shared
 // out over a cluster, whose first CTA joins the parts from the others' shared
-// memory. 4093 x 50257: 131 us = 6.3 TB/s; its gradient at 4096 x 65536: 322 us =
-// 6.7 TB/s. Few rows are bound by latencies: 64 x 131072 with the 20 largest 18 us of
-// the stream (10 without), one row of 32000 with 5 of them 7 us.
+// memory. 4093 x 50257: 138 us = 6.0 TB/s; its gradient at 4096 x 65536: 339 us =
+// 6.3 TB/s (a call, inputs rotated past the L2 cache). Few rows are bound by latencies:
+// 64 x 131072 with the 20 largest 17 to 21 us of the stream (10.6 without), one row of
+// 32000 with 5 of them 7 us.
 #include "operators.hpp"
 
 #include <algorithm>
@@ -225,7 +226,9 @@ extern "C" __global__ void __launch_bounds__(PB_THREADS, 1024 / PB_THREADS) pb_t
     // whatever their number. The lanes that have some look at them once more (where the largest of
     // a lane's other rounds is below the floor, at one round alone) and list them;
     // NaN is none. The list is then sorted, 32 a warp. Only where it is too long,
-    // as of a row of equal logits, they are inserted one by one.
+    // as of a row of equal logits, or where fewer than `top` of a CTA's groups hold one
+    // that is not masked, they are inserted one by one (64 x 131072, 20 alternatives:
+    // 64 us with all but 50 masked, 16.5 with all but 2000).
     pb_u64 list = 0;
     int lists_used = 0;
     if (last > first) { // the same for the whole CTA
